@@ -397,6 +397,77 @@ int lmoe_combine(const void* y, const int32_t* row_idx, const uint16_t* w,
                  int T, int k, int H, const void* add, void* out,
                  hipStream_t stream);
 
+/* lmoe_combine of f32 rows: y is [T*k, H] f32, everything else the same.
+ * y, add and out 16-byte aligned (else LMOE_ERR_SHAPE). */
+int lmoe_combine_f32(const void* y, const int32_t* row_idx, const uint16_t* w,
+                     int T, int k, int H, const void* add, void* out,
+                     hipStream_t stream);
+
+/* ---- 8-bit rows, the norm in front of a MoE layer, 4-bit experts ----
+ *
+ * OCP microscaling formats: 32 neighbouring columns share a scale 2^e, stored
+ * as the byte e + 127 (255: the group is NaN).  Made here, e is the smallest
+ * integer >= -127 that keeps the group's largest magnitude within the element
+ * format, so nothing saturates; a group with a NaN or an infinity is NaN.
+ *   MX8 rows: q [R, K] e4m3 (largest 448), scale [R, K/32] u8.
+ *   MX4 weights of [N, K]: e2m1 (largest 6) codes and scales in one run of
+ *   lmoe_mx4_bytes(N, K) bytes: N/16 blocks of 16 rows; a block is its columns
+ *   by 512: 256 bytes of scales (byte 4 l + c: row l % 16, columns
+ *   128 c + 32 (l / 16).., l < 64), then for each 128 columns 1024 bytes of
+ *   codes (bytes 16 l..: row l % 16, columns 32 (l / 16).., the even column in
+ *   the low half).  Columns past K are zeros with scale 1.
+ *   w13 [P, 2I, H] holds its rows in blocks gate 0..15, up 0..15, gate 16..31,
+ *   up 16..31, ...; w2 [P, H, I] in order.
+ * No counterpart in the reference, whose offloaded experts are bf16. */
+
+/* r = x + residual; y = r / sqrt(mean(r^2) + eps) * weight, in f32.
+ *   x [T, H] bf16; residual [T, H] bf16 or f32 (residual_f32), or null: none;
+ *   weight [H] bf16 or f32 (weight_f32).
+ *   residual_out [T, H] (residual's type; given exactly when residual is) = r,
+ *   out [T, H] bf16 = y (or null), q / scale = y as MX8 rows (or null); each is
+ *   rounded once, from f32.  residual_out and out may be residual or x itself.
+ * H % 8 == 0 (H % 32 == 0 with q), H <= 32768, operands 16-byte aligned (scale
+ * any); else LMOE_ERR_SHAPE.  No counterpart in the reference (vLLM's own norm
+ * precedes the layer). */
+int lmoe_add_rms_norm(const void* x, int T, int H, const void* residual,
+                      int residual_f32, const void* weight, int weight_f32,
+                      float eps, void* residual_out, void* out, void* q,
+                      void* scale, hipStream_t stream);
+
+/* bf16 rows x [T, H] as MX8 rows.  H % 32 == 0, H <= 32768, x and q 16-byte
+ * aligned; else LMOE_ERR_SHAPE. */
+int lmoe_rows_to_mx8(const void* x, int T, int H, void* q, void* scale,
+                     hipStream_t stream);
+
+/* Bytes of MX4 weights of [N, K]; -1 unless N % 16 == 0 and K % 32 == 0. */
+long long lmoe_mx4_bytes(int N, int K);
+
+/* lmoe_gateup_silu and lmoe_down over slot banks of MX4 weights (the same
+ * permutation arguments).  Rows are bf16 (x_scale and act_scale null) or MX8
+ * rows (both given): then act is rounded to MX8 along I, and both products
+ * multiply 8-bit by 4-bit values; f32 accumulation either way, gate, up and
+ * their product in f32, act rounded once.  y is bf16 or f32 (y_f32) by pair,
+ * rows of unplaced pairs untouched.
+ * path = LMOE_PATH_GEMV (few rows per slot: a workgroup's waves split K),
+ * LMOE_PATH_MFMA (row tiles of block_m, the height given to lmoe_permute) or
+ * LMOE_PATH_AUTO; the two add the same products in different orders, each the
+ * same way whatever the batch, the slots and block_m are.
+ * H % 32 == 0, I % 32 == 0, x / act, banks and y 16-byte aligned; else
+ * LMOE_ERR_SHAPE. */
+int lmoe_mx4_gateup_silu(const void* x, const void* x_scale, int T, int H,
+                         int I, int k, const void* w13_slots, int n_slots,
+                         const int32_t* offsets, const int32_t* sorted_pairs,
+                         const int32_t* active, const int32_t* tile_off,
+                         const int32_t* meta, int n_pairs, int block_m,
+                         int path, void* act, void* act_scale,
+                         hipStream_t stream);
+int lmoe_mx4_down(const void* act, const void* act_scale, int H, int I,
+                  const void* w2_slots, int n_slots, const int32_t* offsets,
+                  const int32_t* sorted_pairs, const int32_t* active,
+                  const int32_t* tile_off, const int32_t* meta, int n_pairs,
+                  int block_m, int path, void* y, int y_f32,
+                  hipStream_t stream);
+
 /* The second half of lmoe_fused_moe_decode on its own: down GEMV from act
  * (sorted order) fused with the weighted combine into out (same argument
  * meaning).  Replaces npu_grouped_matmul GMM2 + npu_moe_token_unpermute of

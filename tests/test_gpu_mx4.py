@@ -1,0 +1,356 @@
+"""Expert products over 4-bit slot banks against the experts in 64 bits.
+
+Tolerances, per element and by stage.  A product of K terms in f32 is off by at
+most K 2^-24 sum |x| |w| (dg, du for gate and up).  act = silu(gate) up then
+moves by 1.1 |up| dg + |silu(gate)| du (|silu'| <= 1.1); its own exp, reciprocal
+and products by 2^-20; the store by half a step, 2^-8 in bf16, 2^-4 (or 2^-10 of
+the scale) in 8 bits.  y is checked against the act that the kernel stored, so
+only its own sum and store (2^-8 in bf16) count.
+
+8-bit rows: the matrix instruction adds each 8 neighbouring columns in fixed
+point.  With 2^m the largest product of the operands' powers of two among them,
+every product loses what lies below 2^(m - 13) (towards zero); blocks of 8 are
+then added in f32.  (One product of 2^8 beside one of 2^(8 - d): whole for d <=
+13, gone from 14 on, at columns 1 to 7; whole at any d <= 23 from column 8 on.)
+So a block of 8 is off by at most 8 * 2^-13 * max |x| max |w|, as 2^m <= max |x|
+max |w|, and that is added to K 2^-24 sum |x| |w|."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx
+from tests._util import to_dev_i32
+
+ROWS = ("bf16", "mx8")
+SHAPES = [
+    # H, I, rows of each slot
+    (32, 32, [1, 0, 2]),                        # one group of K either way
+    (64, 96, [3, 17, 1]),
+    (160, 64, [15, 16, 0, 31]),                 # K tails of one and two groups
+    (544, 288, [1, 32, 33, 2]),                 # a quad and one group; two chunks and one group
+    (1024, 480, [5, 65, 100, 1]),               # several passes of 32 rows
+    (2048, 768, [1, 9, 40]),
+    (7168, 64, [2, 33]),
+    (96, 1056, [7, 129, 257]),
+]
+
+
+def _native():
+    from vllm_moe_offload_amd import native
+
+    return native
+
+
+def _paths():
+    native = _native()
+    return [native.LMOE_PATH_GEMV]
+
+
+def _f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+class Layer:
+    """Random 4-bit experts and rows, on the device and as 64-bit values."""
+
+    def __init__(self, H, I, P, T, rows, seed):
+        from vllm_moe_offload_amd import mxfp4, native
+
+        rng = np.random.default_rng(seed)
+        self.H, self.I, self.P, self.rows = H, I, P, rows
+        w13 = torch.from_numpy(rng.standard_normal((P, 2 * I, H)).astype(np.float32) * 0.05)
+        w2 = torch.from_numpy(rng.standard_normal((P, H, I)).astype(np.float32) * 0.05)
+        c13, s13 = mxfp4.quantize(w13)
+        c2, s2 = mxfp4.quantize(w2)
+        self.w13 = mxfp4.pack_w13(c13, s13).cuda()
+        self.w2 = mxfp4.pack_w2(c2, s2).cuda()
+        self.v13 = [mx.values_mx4(c13[p].numpy(), s13[p].numpy()) for p in range(P)]
+        self.v2 = [mx.values_mx4(c2[p].numpy(), s2[p].numpy()) for p in range(P)]
+        x = torch.from_numpy(rng.standard_normal((T, H)).astype(np.float32)).to(torch.bfloat16).cuda()
+        self.x = x if rows == "bf16" else native.rows_to_mx8(x)
+        self.xv = _f64(self.x if rows == "bf16" else self.x.float())
+
+    def act_buffer(self, n):
+        native = _native()
+        if self.rows == "mx8":
+            a = native.Mx8Rows.allocate(n, self.I, "cuda")
+            a.q.view(torch.uint8).fill_(0x31)
+            a.scale.fill_(99)
+            return a
+        return torch.full((n, self.I), 7.0, dtype=torch.bfloat16, device="cuda")
+
+
+def sum_error(x, w, mx8):
+    """How far f32 sums over the columns of rows x and weight rows w may be off."""
+    e = np.abs(x) @ np.abs(w).T * (x.shape[1] * 2.0**-24)
+    if mx8:
+        eight = lambda v: np.abs(v).reshape(v.shape[0], -1, 8).max(axis=2)
+        e = e + 8 * 2.0**-13 * (eight(x) @ eight(w).T)
+    return e
+
+
+def check_act(got, gate, up, dg, du, mx8_scale=None):
+    sg = gate / (1.0 + np.exp(-gate))
+    act = sg * up
+    tol = 1.1 * np.abs(up) * dg + np.abs(sg) * du + dg * du + 2.0**-20 * np.abs(act)
+    if mx8_scale is None:
+        tol = tol + 2.0**-8 * np.abs(act)
+    else:
+        tol = tol * (1 + 2.0**-4) + np.maximum(2.0**-4 * np.abs(act), 2.0**-10 * np.repeat(mx8_scale, 32, axis=1))
+    assert np.all(np.abs(got - act) <= tol), float(np.max(np.abs(got - act) / np.maximum(tol, 1e-300)))
+
+
+def check_layer(layer, perm, k, act, y, ids_slot):
+    """Every placed pair's act and y; ids_slot[p]: the slot of pair p or -1."""
+    offs = perm.offsets.cpu().numpy()
+    pairs = perm.sorted_pairs.cpu().numpy()
+    mx8 = layer.rows == "mx8"
+    a = _f64(act.float() if mx8 else act)
+    sc = np.ldexp(1.0, act.scale.cpu().numpy().astype(np.int64) - 127) if mx8 else None
+    yv = _f64(y)
+    ystep = 2.0**-8 if y.dtype == torch.bfloat16 else 2.0**-24
+    for s in range(layer.P):
+        pos = np.arange(offs[s], offs[s + 1])
+        if not len(pos):
+            continue
+        assert np.all(ids_slot[pairs[pos]] == s)
+        x, w = layer.xv[pairs[pos] // k], layer.v13[s]
+        g, ab = x @ w.T, sum_error(x, w, mx8)
+        I = layer.I
+        check_act(a[pos], g[:, :I], g[:, I:], ab[:, :I], ab[:, I:], sc[pos] if mx8 else None)
+        want = a[pos] @ layer.v2[s].T
+        tol = sum_error(a[pos], layer.v2[s], mx8) * (1 + ystep) + ystep * np.abs(want)
+        got = yv[pairs[pos]]
+        assert np.all(np.abs(got - want) <= tol + 1e-30), float(np.max(np.abs(got - want) / (tol + 1e-30)))
+
+
+def _ids(counts, extra, rng):
+    ids = np.concatenate([np.repeat(np.arange(len(counts)), counts), np.full(extra, -1)]).astype(np.int32)
+    return rng.permutation(ids).reshape(-1, 1)
+
+
+def run_layer(layer, ids, k, path, *, block_m=None, log2phy=None, y_dtype=torch.bfloat16):
+    native = _native()
+    n = ids.size
+    perm = native.Permutation.allocate(n, layer.P, "cuda")
+    bm = native.mx4_block_m(n, layer.P) if block_m is None else block_m
+    native.permute(to_dev_i32(ids), perm, log2phy=log2phy, skip_unmapped=True, block_m=bm)
+    act = layer.act_buffer(n)
+    y = torch.full((n, layer.H), -7.0, dtype=y_dtype, device="cuda")
+    native.grouped_mlp(layer.x, k, layer.w13, layer.w2, perm, act, y, path=path)
+    return perm, act, y
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("H,I,counts", SHAPES)
+def test_products_are_the_experts(H, I, counts, rows):
+    native = _native()
+    rng = np.random.default_rng(H * 7 + I)
+    P, T = len(counts), sum(counts) + 3
+    ids = _ids(counts, 3, rng)
+    l2p = rng.permutation(P).astype(np.int32)
+    layer = Layer(H, I, P, T, rows, H + I)
+    slot_of = np.where(ids[:, 0] >= 0, l2p[np.maximum(ids[:, 0], 0)], -1)
+    for path in _paths():
+        for y_dtype in (torch.bfloat16, torch.float32):
+            print(f"case mx4 H={H} I={I} {rows} path={path} {y_dtype}", flush=True)
+            perm, act, y = run_layer(layer, ids, 1, path, log2phy=to_dev_i32(l2p), y_dtype=y_dtype)
+            torch.cuda.synchronize()
+            check_layer(layer, perm, 1, act, y, slot_of)
+            placed = int(perm.meta[native.META_PAIRS])
+            assert placed == sum(counts)
+            # what no pair owns is left as it was
+            assert torch.all(y[torch.from_numpy(ids[:, 0] < 0).cuda()] == -7.0)
+            if rows == "mx8":
+                assert torch.all(act.q.view(torch.uint8)[placed:] == 0x31) and torch.all(act.scale[placed:] == 99)
+            else:
+                assert torch.all(act[placed:] == 7.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+def test_several_experts_per_token_and_the_same_twice(rows):
+    """top_k 3; a token may name one expert twice: both pairs get their row."""
+    rng = np.random.default_rng(5)
+    T, k, P = 21, 3, 5
+    ids = rng.integers(0, P, (T, k)).astype(np.int32)
+    ids[4] = [2, 2, 2]
+    layer = Layer(96, 64, P, T, rows, 17)
+    for path in _paths():
+        perm, act, y = run_layer(layer, ids, k, path)
+        torch.cuda.synchronize()
+        check_layer(layer, perm, k, act, y, ids.flatten())
+        assert torch.equal(y[12], y[13]) and torch.equal(y[12], y[14])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+def test_a_bad_row_stays_its_own(rows):
+    """A token that is not a number spoils its own pairs and nothing else, also
+    where K ends inside a fragment."""
+    from vllm_moe_offload_amd import native
+
+    rng = np.random.default_rng(8)
+    ids = _ids([6, 20], 0, rng)
+    layer = Layer(160, 96, 2, 26, rows, 3)
+    for path in _paths():
+        _, _, clean = run_layer(layer, ids, 1, path)
+        for value in (float("nan"), float("inf")):
+            bad = layer.x.clone() if rows == "bf16" else layer.x.float().to(torch.bfloat16)
+            bad[5, 159] = value
+            keep, layer.x = layer.x, bad if rows == "bf16" else native.rows_to_mx8(bad)
+            _, _, y = run_layer(layer, ids, 1, path)
+            layer.x = keep
+            assert not y[5].isfinite().any()
+            other = torch.arange(26, device="cuda") != 5
+            assert torch.equal(y[other], clean[other])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+def test_extreme_scales(rows):
+    """Weights near both ends of the scales' range: exact powers of two pass through."""
+    from vllm_moe_offload_amd import mxfp4
+
+    layer = Layer(64, 32, 1, 2, rows, 1)
+    w13 = torch.zeros(1, 64, 64)
+    w13[0, :32] = torch.eye(32, 64) * 6.0
+    w13[0, 32:] = torch.eye(32, 64) * 2.0**100
+    w2 = torch.zeros(1, 64, 32)
+    w2[0, :32] = torch.eye(32) * 2.0**-100
+    layer.w13, layer.w2 = mxfp4.pack_w13(*mxfp4.quantize(w13)).cuda(), mxfp4.pack_w2(*mxfp4.quantize(w2)).cuda()
+    c, s = mxfp4.quantize(w13[0]); layer.v13 = [mx.values_mx4(c.numpy(), s.numpy())]
+    c, s = mxfp4.quantize(w2[0]); layer.v2 = [mx.values_mx4(c.numpy(), s.numpy())]
+    ids = np.zeros((2, 1), dtype=np.int32)
+    for path in _paths():
+        perm, act, y = run_layer(layer, ids, 1, path)
+        check_layer(layer, perm, 1, act, y, ids.flatten())
+        assert y[:, :32].abs().max() > 0.5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("T,k,E", [(1, 4, 8), (1, 8, 8), (3, 2, 8), (40, 4, 16), (300, 4, 8)])
+def test_fused_experts_over_a_4_bit_bank(T, k, E, rows):
+    """Permutation, products and combine through the layer's own call: out
+    against the sum of the pairs' rows, each taken from the products' call."""
+    from vllm_moe_offload_amd import fused_moe, native
+
+    H, I = 256, 160
+    rng = np.random.default_rng(T + k)
+    ids = np.stack([rng.choice(E, k, replace=False) for _ in range(T)]).astype(np.int32)
+    layer = Layer(H, I, E, T, rows, T)
+    g = torch.Generator(device="cuda").manual_seed(T)
+    w = torch.empty((T, k), device="cuda").uniform_(0.05, 1, generator=g).to(torch.bfloat16)
+    add = torch.empty((T, H), device="cuda").normal_(generator=g).to(torch.bfloat16)
+    l2p = to_dev_i32(rng.permutation(E))
+    out = fused_moe.fused_experts(layer.x, w, to_dev_i32(ids), layer.w13, layer.w2, l2p, add=add).clone()
+    ws = fused_moe.get_workspace(T, k, E, H, I, "cuda", rows=fused_moe.rows_kind(layer.x, layer.w13))
+    assert ws.y.dtype == (torch.float32 if T * k <= native.FUSED_DECODE_MAX_PAIRS else torch.bfloat16)
+    assert isinstance(ws.act, native.Mx8Rows) == (rows == "mx8")
+    path = native.mx4_path(T * k, E)
+    _, act, y = run_layer(layer, ids, k, path, log2phy=l2p, y_dtype=torch.float32)
+    yv = _f64(y).reshape(T, k, H)
+    want = (_f64(w)[:, :, None] * yv).sum(1) + _f64(add)
+    mag = (np.abs(_f64(w))[:, :, None] * np.abs(yv)).sum(1) + np.abs(_f64(add))
+    tol = 2.0**-8 * np.abs(want) + (k + 2) * 2.0**-24 * mag
+    # the rows themselves: bf16 past FUSED_DECODE_MAX_PAIRS pairs; a fused form
+    # may add the same products of act in another order
+    rowtol = 2.0**-8 if ws.y.dtype == torch.bfloat16 else 0.0
+    av = _f64(act.float() if rows == "mx8" else act)
+    worst = max(sum_error(av, v, rows == "mx8").max() for v in layer.v2)
+    tol = tol + rowtol * mag + 2 * k * worst
+    assert np.all(np.abs(_f64(out) - want) <= tol)
+    again = fused_moe.fused_experts(layer.x, w, to_dev_i32(ids), layer.w13, layer.w2, l2p, add=add)
+    assert torch.equal(again, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+def test_masked_pairs_and_a_token_without_any(rows):
+    """Pairs whose expert has no slot add nothing; a token without a pair is its
+    addend; the status words count what was dropped."""
+    from vllm_moe_offload_amd import fused_moe, native
+
+    T, k, E, H, I = 5, 2, 6, 64, 32
+    layer = Layer(H, I, 4, T, rows, 2)
+    ids = np.array([[0, 1], [4, 5], [2, 4], [3, 0], [5, 1]], dtype=np.int32)
+    l2p = to_dev_i32(np.array([0, 1, 2, 3, -1, -1]))
+    w = torch.full((T, k), 0.5, dtype=torch.bfloat16, device="cuda")
+    add = torch.randn((T, H), device="cuda").to(torch.bfloat16)
+    native.device_flags(clear=True)
+    out = fused_moe.fused_experts(layer.x, w, to_dev_i32(ids), layer.w13, layer.w2, l2p, add=add).clone()
+    assert native.device_flags(clear=True)[native.FLAG_UNPLACED] == 4
+    assert torch.equal(out[1], add[1])
+    full = fused_moe.fused_experts(layer.x, w, to_dev_i32(ids), layer.w13, layer.w2,
+                                   to_dev_i32(np.array([0, 1, 2, 3, 0, 0])), add=add).clone()
+    native.device_flags(clear=True)
+    assert torch.equal(out[0], full[0]) and torch.equal(out[3], full[3]) and not torch.equal(out[2], full[2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+def test_a_captured_step_replays(rows):
+    from vllm_moe_offload_amd import fused_moe, native
+
+    T, k, E, H, I = 6, 2, 8, 256, 96
+    rng = np.random.default_rng(1)
+    layer = Layer(H, I, E, T, rows, 4)
+    w = torch.full((T, k), 0.5, dtype=torch.bfloat16, device="cuda")
+    d_ids = to_dev_i32(rng.integers(0, E, (T, k)))
+    ws = fused_moe.get_workspace(T, k, E, H, I, "cuda", tag="graph", rows=fused_moe.rows_kind(layer.x, layer.w13))
+    out = torch.empty((T, H), dtype=torch.bfloat16, device="cuda")
+    call = lambda o, s: fused_moe.fused_experts(layer.x, w, d_ids, layer.w13, layer.w2, None, out=o, workspace=s)
+    call(out, ws)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out, ws)
+    for _ in range(3):
+        d_ids.copy_(to_dev_i32(rng.integers(0, E, (T, k))))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = call(torch.empty_like(out), None)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    native.device_flags(clear=True)
+
+
+@pytest.mark.gpu
+def test_empty_batches_and_refusals():
+    from vllm_moe_offload_amd import fused_moe, native
+
+    layer = Layer(64, 32, 2, 4, "bf16", 0)
+    ids = torch.zeros((4, 1), dtype=torch.int32, device="cuda")
+    w = torch.ones((4, 1), dtype=torch.bfloat16, device="cuda")
+    for x in (layer.x[:0], native.rows_to_mx8(layer.x)[:0]):
+        assert fused_moe.fused_experts(x, w[:0], ids[:0], layer.w13, layer.w2, None).shape == (0, 64)
+    perm = native.Permutation.allocate(4, 2, "cuda")
+    native.permute(ids, perm)
+    act, y = layer.act_buffer(4), torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
+    x8, a8 = native.rows_to_mx8(layer.x), native.Mx8Rows.allocate(4, 32, "cuda")
+    wrong = [
+        lambda: native.gateup_silu(layer.x, 1, layer.w13, perm, a8),            # rows of two kinds
+        lambda: native.gateup_silu(x8, 1, layer.w13, perm, act),
+        lambda: native.gateup_silu(layer.x.float(), 1, layer.w13, perm, act),
+        lambda: native.gateup_silu(layer.x, 1, layer.w13[:, :, :-1].contiguous(), perm, act),
+        lambda: native.gateup_silu(layer.x, 1, layer.w13[:1], perm, act),       # fewer slots
+        lambda: native.gateup_silu(layer.x, 2, layer.w13, perm, act),
+        lambda: native.gateup_silu(torch.zeros((4, 160), dtype=torch.bfloat16, device="cuda"), 1, layer.w13, perm, act),
+        # a row of 32 columns takes as many bytes as one of 64: the down bank tells them apart
+        lambda: native.grouped_mlp(layer.x[:, :32].contiguous(), 1, layer.w13, layer.w2, perm, act, y),
+        lambda: fused_moe.fused_experts(layer.x[:, :32].contiguous(), w, ids, layer.w13, layer.w2, None),
+        lambda: native.down(act, layer.w2, perm, y.half()),
+        lambda: native.down(act, layer.w2, perm, y[:2]),
+        lambda: native.down(act[:2], layer.w2, perm, y),
+        lambda: native.gateup_silu(x8, 1, torch.zeros((2, 64, 64), dtype=torch.bfloat16, device="cuda"), perm, act),
+        lambda: native.fused_moe_decode(layer.x, w, layer.w13, layer.w2, perm, act, y),
+        lambda: native.down_combine(act, w, layer.w2, perm, y),
+    ]
+    for i, call in enumerate(wrong):
+        with pytest.raises((ValueError, TypeError)):
+            call()
+            pytest.fail(f"call {i} was taken")
+    with pytest.raises(RuntimeError, match="unsupported option"):
+        native.gateup_silu(layer.x, 1, layer.w13, perm, act, path=native.LMOE_PATH_STREAM)

@@ -1,0 +1,156 @@
+"""Microscaling formats on the host: the quantizer against the definition in
+64 bits, the bank's byte order, what is refused."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx
+
+
+def _m():
+    from vllm_moe_offload_amd import mxfp4
+
+    return mxfp4
+
+
+def _special_rows(K, rng):
+    """Rows whose groups sit on the format's borders."""
+    w = rng.standard_normal((32, K)).astype(np.float32) * 0.02
+    w[0] = 0.0
+    w[1, :8] = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0]         # ties of scale 1
+    w[1, 8:16] = -w[1, :8]
+    w[2] = np.float32(1e-40)                                         # subnormal f32
+    w[3] = np.nextafter(np.float32(6.0), np.float32(7.0))            # just past a scale's reach
+    w[4] = 6.0 * 2.0 ** rng.integers(-20, 20)
+    w[5] = np.float32(2.0**120) * rng.standard_normal(K)
+    w[6] = np.float32(2.0**-125) * rng.standard_normal(K)
+    w[7, ::2] = -0.0
+    return w
+
+
+@pytest.mark.parametrize("K", [32, 96, 160, 512, 1056])
+def test_quantize_is_the_definition(K):
+    w = _special_rows(K, np.random.default_rng(K))
+    codes, scales = _m().quantize(torch.from_numpy(w))
+    want_c, want_s = mx.quantize_mx4(w)
+    assert np.array_equal(scales.numpy(), want_s)
+    assert np.array_equal(codes.numpy(), want_c)
+    got = _m().dequantize(codes, scales).numpy()
+    assert np.array_equal(got.astype(np.float64), mx.values_mx4(want_c, want_s))
+
+
+def test_quantize_bf16_and_not_a_number():
+    w = torch.randn(32, 64).to(torch.bfloat16)
+    c, s = _m().quantize(w)
+    c32, s32 = _m().quantize(w.float())
+    assert torch.equal(c, c32) and torch.equal(s, s32)
+    w[3, 5], w[4, 40] = float("nan"), float("inf")
+    c, s = _m().quantize(w)
+    assert s[3, 0] == 255 and s[4, 1] == 255 and s[3, 1] != 255 and s[4, 0] != 255
+    v = _m().dequantize(c, s)
+    assert v[3, :32].isnan().all() and v[4, 32:].isnan().all() and not v[3, 32:].isnan().any()
+
+
+@pytest.mark.parametrize("K", [32, 128, 160, 480, 512, 768, 1056])
+def test_bank_bytes_are_where_the_kernels_read_them(K):
+    m = _m()
+    N = 64
+    rng = np.random.default_rng(K)
+    codes = torch.from_numpy(rng.integers(0, 256, (2, N, K // 2), dtype=np.uint8))
+    scales = torch.from_numpy(rng.integers(0, 255, (2, N, K // 32), dtype=np.uint8))
+    bank = m.pack_w2(codes, scales)
+    assert bank.shape == (2, N, m.row_bytes(K)) and bank.is_contiguous()
+    flat = bank.reshape(2, -1)
+    block = 16 * m.row_bytes(K)
+    c, s = codes.numpy(), scales.numpy()
+    for e, n, k in [(0, 0, 0), (1, 63, K - 1), (1, 17, K // 2), (0, 33, K - 32), (1, 40, 31)]:
+        quad, chunk, group = k // 512, k // 128, k % 128 // 32
+        lane = n % 16 + 16 * group
+        base = (n // 16) * block + quad * 4352
+        byte = int(flat[e, base + 256 + (chunk % 4) * 1024 + lane * 16 + k % 32 // 2])
+        assert byte == c[e, n, k // 2]
+        assert int(flat[e, base + lane * 4 + chunk % 4]) == s[e, n, k // 32]
+    c2, s2 = m.unpack_w2(bank, K)
+    assert torch.equal(c2, codes) and torch.equal(s2, scales)
+    # gate and up rows in alternating blocks of 16
+    b13 = m.pack_w13(codes, scales)
+    order = torch.cat([torch.arange(h + 16 * b, h + 16 * b + 16) for b in range(2) for h in (0, 32)])
+    assert torch.equal(b13, m.pack_w2(codes[:, order], scales[:, order]))
+    c3, s3 = m.unpack_w13(b13, K)
+    assert torch.equal(c3, codes) and torch.equal(s3, scales)
+
+
+def test_library_and_host_agree_on_bytes():
+    from vllm_moe_offload_amd import native
+
+    lib = native.load_library()
+    for N, K in ((16, 32), (64, 160), (1536, 2048), (4096, 7168), (2048, 768)):
+        assert lib.lmoe_mx4_bytes(N, K) == N * _m().row_bytes(K)
+    for N, K in ((15, 32), (16, 48), (0, 32), (16, 0), (-16, 32)):
+        assert lib.lmoe_mx4_bytes(N, K) == -1
+
+
+def test_pack_experts_is_quantize_then_pack():
+    m = _m()
+    w13, w2 = torch.randn(3, 128, 96).to(torch.bfloat16), torch.randn(3, 96, 64).to(torch.bfloat16)
+    b13, b2 = m.pack_experts(w13, w2)
+    assert torch.equal(b13, m.pack_w13(*m.quantize(w13))) and torch.equal(b2, m.pack_w2(*m.quantize(w2)))
+
+
+def test_refusals():
+    m = _m()
+    with pytest.raises(ValueError):
+        m.row_bytes(48)
+    with pytest.raises(ValueError):
+        m.quantize(torch.zeros(16, 40))
+    with pytest.raises(ValueError):
+        m.quantize(torch.zeros(16, 64, dtype=torch.int8))
+    c, s = torch.zeros(32, 32, dtype=torch.uint8), torch.zeros(32, 2, dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        m.pack_w2(c[:20], s[:20])           # no whole blocks of 16 rows
+    with pytest.raises(ValueError):
+        m.pack_w13(c, s)                    # gate and up of 16 rows each
+    with pytest.raises(ValueError):
+        m.pack_w2(c, s[:, :1])
+    with pytest.raises(ValueError):
+        m.pack_w2(c.int(), s)
+    with pytest.raises(ValueError):
+        m.unpack_w2(m.pack_w2(c, s), 128 + 32)
+    with pytest.raises(ValueError):
+        m.pack_experts(c, c)
+
+
+P16, N = 4096, None  # a placeholder address, never read: these calls fail on the host
+
+
+def test_c_entries_check_their_arguments():
+    from vllm_moe_offload_amd import native
+
+    lib = native.load_library()
+    norm = lambda x=P16, T=1, H=64, r=P16, w=P16, eps=1e-6, ro=P16, out=P16, q=P16, s=P16: \
+        lib.lmoe_add_rms_norm(x, T, H, r, 0, w, 0, eps, ro, out, q, s, N)
+    assert norm(T=0, x=N, r=N, w=N, ro=N, out=N, q=N, s=N) == 0
+    assert norm(T=-1) == 1000 and norm(H=0) == 1000 and norm(eps=-1.0) == 1000 and norm(eps=float("nan")) == 1000
+    assert norm(x=N) == 1000 and norm(w=N) == 1000 and norm(out=N, q=N, s=N) == 1000
+    assert norm(r=N) == 1000 and norm(ro=N) == 1000 and norm(q=N) == 1000 and norm(s=N) == 1000
+    assert norm(H=36) == 1001 and norm(H=40) == 1001 and norm(H=32800) == 1001
+    for k in ("x", "r", "w", "ro", "out", "q"):
+        assert norm(**{k: P16 + 8}) == 1001, k
+    rows = lambda x=P16, T=1, H=64, q=P16, s=P16: lib.lmoe_rows_to_mx8(x, T, H, q, s, N)
+    assert rows(T=0, x=N, q=N, s=N) == 0 and rows(T=-1) == 1000 and rows(x=N) == 1000 and rows(q=N) == 1000
+    assert rows(s=N) == 1000 and rows(H=40) == 1001 and rows(x=P16 + 2) == 1001 and rows(H=65536) == 1001
+    gu = lambda x=P16, xs=P16, T=2, H=64, I=32, k=2, w=P16, P=4, n=4, path=0, act=P16, as_=P16, bm=128: \
+        lib.lmoe_mx4_gateup_silu(x, xs, T, H, I, k, w, P, P16, P16, P16, P16, P16, n, bm, path, act, as_, N)
+    assert gu(T=0, n=0, x=N, act=N) == 0
+    assert gu(T=-1) == 1000 and gu(k=0) == 1000 and gu(n=5) == 1000 and gu(P=0) == 1000 and gu(x=N) == 1000
+    assert gu(xs=N) == 1000 and gu(as_=N) == 1000 and gu(act=N) == 1000 and gu(w=N) == 1000
+    assert gu(H=48) == 1001 and gu(I=48) == 1001 and gu(x=P16 + 8) == 1001 and gu(w=P16 + 4) == 1001
+    assert gu(path=9) == 1003 and gu(path=3) == 1003
+    dn = lambda act=P16, as_=P16, H=64, I=32, w=P16, P=4, n=4, path=0, y=P16, bm=128: \
+        lib.lmoe_mx4_down(act, as_, H, I, w, P, P16, P16, P16, P16, P16, n, bm, path, y, 0, N)
+    assert dn(n=0, act=N, y=N) == 0 and dn(n=-1) == 1000 and dn(act=N) == 1000 and dn(y=N) == 1000
+    assert dn(H=48) == 1001 and dn(I=16) == 1001 and dn(y=P16 + 8) == 1001 and dn(path=9) == 1003
+    comb = lambda y=P16, w=P16, T=1, k=2, H=64, out=P16, add=N: \
+        lib.lmoe_combine_f32(y, N, w, T, k, H, add, out, N)
+    assert comb(T=0, y=N, out=N) == 0 and comb(y=N) == 1000 and comb(H=60) == 1001 and comb(out=P16 + 2) == 1001

@@ -1,0 +1,127 @@
+// Entry points of the expert products over 4-bit weights.
+#include <hip/hip_runtime.h>
+
+#include "mx4_few.h"
+
+LMOE_FLAGS_UNIT(mx4)
+
+namespace lmoe {
+
+// ---------------------------------------------------------------------------
+// weighted combine of f32 rows by pair: out[t] = add[t] + sum_j w[t][j] y[t k + j],
+// added in j order, one rounding.  A few tokens' rows come from L2; four columns
+// per thread and one wave per workgroup spread them over the CUs.
+// ---------------------------------------------------------------------------
+constexpr int kCombineStep = 8;
+
+__global__ __launch_bounds__(64) void combine_f32_kernel(
+    const float* __restrict__ y, const int32_t* __restrict__ row_idx, const uint16_t* __restrict__ w,
+    int topk, int H, const uint16_t* __restrict__ add, uint16_t* __restrict__ out) {
+  const int t = blockIdx.x;
+  const int h = (blockIdx.y * 64 + threadIdx.x) * 4;
+  if (h >= H) return;
+  f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int j0 = 0; j0 < topk; j0 += kCombineStep) {
+    f32x4_t v[kCombineStep];
+    float wj[kCombineStep];
+    bool use[kCombineStep];
+#pragma unroll
+    for (int jj = 0; jj < kCombineStep; ++jj) {  // every load issued, masked rows dropped below
+      const int j = j0 + jj;
+      const bool in = j < topk;
+      const int p = t * topk + (in ? j : 0);
+      use[jj] = in && (row_idx == nullptr || row_idx[p] >= 0);
+      if (in && !use[jj] && blockIdx.y == 0 && threadIdx.x == 0) add_device_flag(LMOE_FLAG_UNPLACED, 1);
+      wj[jj] = bf16_to_f32(w[p]);
+      v[jj] = *reinterpret_cast<const f32x4_t*>(y + static_cast<size_t>(p) * H + h);
+    }
+#pragma unroll
+    for (int jj = 0; jj < kCombineStep; ++jj)
+      if (use[jj]) acc += wj[jj] * v[jj];
+  }
+  if (add != nullptr) {
+    const uint2 a = *reinterpret_cast<const uint2*>(add + static_cast<size_t>(t) * H + h);
+    acc += f32x4_t{bf16lo(a.x), bf16hi(a.x), bf16lo(a.y), bf16hi(a.y)};
+  }
+  *reinterpret_cast<uint2*>(out + static_cast<size_t>(t) * H + h) =
+      make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
+}
+
+static bool known_path(int path) {
+  return path == LMOE_PATH_AUTO || path == LMOE_PATH_GEMV || path == LMOE_PATH_MFMA;
+}
+constexpr int kMaxSlots = 65535;  // a grid dimension
+
+static bool bad16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+template <bool GU>
+static void launch_few(const Mx4Args& g, hipStream_t stream) {
+  const dim3 grid(g.N / 32, g.n_pairs < g.P ? g.n_pairs : g.P);
+  if (g.a_scale != nullptr) mx4_few_kernel<GU, true><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
+  else mx4_few_kernel<GU, false><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
+}
+
+}  // namespace lmoe
+
+using namespace lmoe;
+
+extern "C" long long lmoe_mx4_bytes(int N, int K) {
+  if (N <= 0 || K <= 0 || N % 16 != 0 || K % kMxGroup != 0) return -1;
+  return static_cast<long long>(N / 16) * mx4_block_bytes(K);
+}
+
+extern "C" int lmoe_mx4_gateup_silu(const void* x, const void* x_scale, int T, int H, int I, int k,
+                                    const void* w13_slots, int n_slots, const int32_t* offsets,
+                                    const int32_t* sorted_pairs, const int32_t* active,
+                                    const int32_t* tile_off, const int32_t* meta, int n_pairs,
+                                    int block_m, int path, void* act, void* act_scale,
+                                    hipStream_t stream) {
+  if (T < 0 || H <= 0 || I <= 0 || k <= 0 || n_slots <= 0 || n_pairs < 0) return LMOE_ERR_ARG;
+  if (n_pairs != static_cast<long long>(T) * k) return LMOE_ERR_ARG;
+  if (H % kMxGroup != 0 || I % kMxGroup != 0 || n_slots > kMaxSlots) return LMOE_ERR_SHAPE;
+  if (!known_path(path)) return LMOE_ERR_UNSUPPORTED;
+  if (n_pairs == 0) return LMOE_OK;
+  if (x == nullptr || w13_slots == nullptr || offsets == nullptr || sorted_pairs == nullptr ||
+      active == nullptr || tile_off == nullptr || meta == nullptr || act == nullptr)
+    return LMOE_ERR_ARG;
+  if ((x_scale == nullptr) != (act_scale == nullptr)) return LMOE_ERR_ARG;
+  if (bad16(x) || bad16(w13_slots) || bad16(act)) return LMOE_ERR_SHAPE;
+  const Mx4Args g{x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(w13_slots),
+                  lmoe_mx4_bytes(2 * I, H), H, I, k, n_slots, n_pairs, offsets, sorted_pairs, active,
+                  tile_off, meta, act, static_cast<uint8_t*>(act_scale), false};
+  launch_few<true>(g, stream);
+  LMOE_RETURN_LAUNCH();
+}
+
+extern "C" int lmoe_mx4_down(const void* act, const void* act_scale, int H, int I,
+                             const void* w2_slots, int n_slots, const int32_t* offsets,
+                             const int32_t* sorted_pairs, const int32_t* active,
+                             const int32_t* tile_off, const int32_t* meta, int n_pairs, int block_m,
+                             int path, void* y, int y_f32, hipStream_t stream) {
+  if (H <= 0 || I <= 0 || n_slots <= 0 || n_pairs < 0) return LMOE_ERR_ARG;
+  if (H % kMxGroup != 0 || I % kMxGroup != 0 || n_slots > kMaxSlots) return LMOE_ERR_SHAPE;
+  if (!known_path(path)) return LMOE_ERR_UNSUPPORTED;
+  if (n_pairs == 0) return LMOE_OK;
+  if (act == nullptr || w2_slots == nullptr || offsets == nullptr || sorted_pairs == nullptr ||
+      active == nullptr || tile_off == nullptr || meta == nullptr || y == nullptr)
+    return LMOE_ERR_ARG;
+  if (bad16(act) || bad16(w2_slots) || bad16(y)) return LMOE_ERR_SHAPE;
+  const Mx4Args g{act, static_cast<const uint8_t*>(act_scale), static_cast<const uint8_t*>(w2_slots),
+                  lmoe_mx4_bytes(H, I), I, H, 1, n_slots, n_pairs, offsets, sorted_pairs, active,
+                  tile_off, meta, y, nullptr, y_f32 != 0};
+  launch_few<false>(g, stream);
+  LMOE_RETURN_LAUNCH();
+}
+
+extern "C" int lmoe_combine_f32(const void* y, const int32_t* row_idx, const uint16_t* w, int T, int k,
+                                int H, const void* add, void* out, hipStream_t stream) {
+  if (T < 0 || k <= 0 || H <= 0) return LMOE_ERR_ARG;
+  if (H % 8 != 0) return LMOE_ERR_SHAPE;
+  if (T == 0) return LMOE_OK;
+  if (y == nullptr || w == nullptr || out == nullptr) return LMOE_ERR_ARG;
+  if (bad16(y) || bad16(add) || bad16(out)) return LMOE_ERR_SHAPE;
+  combine_f32_kernel<<<dim3(T, (H + 255) / 256), 64, 0, stream>>>(
+      static_cast<const float*>(y), row_idx, w, k, H, static_cast<const uint16_t*>(add),
+      static_cast<uint16_t*>(out));
+  LMOE_RETURN_LAUNCH();
+}

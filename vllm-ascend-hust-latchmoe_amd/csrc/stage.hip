@@ -134,6 +134,7 @@ extern "C" int lmoe_abi_version(void) { return LMOE_ABI_VERSION; }
 
 namespace lmoe {
 void* flags_address_mlp();
+void* flags_address_mx4();
 void* flags_address_router_softmax();
 void* flags_address_router_sigmoid();
 }  // namespace lmoe
@@ -141,7 +142,8 @@ void* flags_address_router_sigmoid();
 extern "C" int lmoe_device_flags(int32_t* flags, int clear, hipStream_t stream) {
   if (flags == nullptr) return LMOE_ERR_ARG;
   // the units whose kernels add to their status words
-  static void* (*const units[])() = {lmoe::flags_address_mlp, lmoe::flags_address_router_softmax,
+  static void* (*const units[])() = {lmoe::flags_address_mlp, lmoe::flags_address_mx4,
+                                     lmoe::flags_address_router_softmax,
                                      lmoe::flags_address_router_sigmoid};
   constexpr int kUnits = sizeof(units) / sizeof(units[0]);
   static const int32_t zeros[LMOE_FLAG_COUNT] = {0};

@@ -36,7 +36,7 @@ from time import perf_counter
 
 import torch
 
-from vllm_moe_offload_amd import native
+from vllm_moe_offload_amd import mxfp4, native
 from vllm_moe_offload_amd.moe_offload import phase_split
 from vllm_moe_offload_amd.moe_offload.runtime import MoeOffloadRuntime, _is_current_graph_capturing
 from vllm_moe_offload_amd.moe_offload.slot_mapping import PreparedSlotWeights
@@ -48,8 +48,8 @@ from vllm_moe_offload_amd.moe_offload.slot_mapping import PreparedSlotWeights
 @dataclass
 class MoEWorkspace:
     perm: native.Permutation
-    act: torch.Tensor   # [N, I] bf16, sorted order
-    y: torch.Tensor     # [N, H] bf16, flat pair order
+    act: torch.Tensor   # [N, I] bf16 (or Mx8Rows), sorted order
+    y: torch.Tensor     # [N, H] bf16 (or f32), flat pair order
     out: torch.Tensor   # [T, H] bf16
     perm_overflow: native.Permutation | None = None  # the decode overflow pass's permutation
 
@@ -63,15 +63,30 @@ class MoEWorkspace:
 _WORKSPACES: dict[tuple, MoEWorkspace] = {}
 
 
-def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = "") -> MoEWorkspace:
-    key = (int(T), int(k), int(P), int(H), int(I), str(device), tag)
+def rows_kind(hidden, w13_slots) -> str:
+    """What a layer's workspace holds: "" for bf16 experts; for 4-bit experts
+    the kind of the rows, "bf16" or "mx8" (hidden is native.Mx8Rows)."""
+    if not mxfp4.is_mx4(w13_slots):
+        return ""
+    return "mx8" if isinstance(hidden, native.Mx8Rows) else "bf16"
+
+
+def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = "", rows: str = "") -> MoEWorkspace:
+    """The workspace of a layer shape.  rows: rows_kind of its experts.  4-bit
+    experts' rows of a few tokens stay f32 until the combine (their bytes are
+    few beside the weights')."""
+    if rows not in ("", "bf16", "mx8"):
+        raise ValueError(f"unknown rows {rows!r}")
+    key = (int(T), int(k), int(P), int(H), int(I), str(device), tag, rows)
     ws = _WORKSPACES.get(key)
     if ws is None:
         N = T * k
+        y_dtype = torch.float32 if rows and N <= native.FUSED_DECODE_MAX_PAIRS else torch.bfloat16
         ws = MoEWorkspace(
             perm=native.Permutation.allocate(N, P, device),
-            act=torch.empty((max(N, 1), I), dtype=torch.bfloat16, device=device),
-            y=torch.empty((max(N, 1), H), dtype=torch.bfloat16, device=device),
+            act=native.Mx8Rows.allocate(max(N, 1), I, device) if rows == "mx8" else
+            torch.empty((max(N, 1), I), dtype=torch.bfloat16, device=device),
+            y=torch.empty((max(N, 1), H), dtype=y_dtype, device=device),
             out=torch.empty((max(T, 1), H), dtype=torch.bfloat16, device=device),
         )
         _WORKSPACES[key] = ws
@@ -166,6 +181,8 @@ def _layer_path(hidden, k: int, n_experts: int, *w13) -> int:
     several passes, all of them): one path for every pass, so a split layer
     gives the unsplit layer's bits."""
     T, H = hidden.shape
+    if mxfp4.is_mx4(w13[0]):
+        return native.mx4_path(T * k, n_experts)
     return native.layer_path(T, k, H, int(w13[0].shape[1]) // 2, n_experts, aligned=native.aligned16(hidden, *w13))
 
 
@@ -181,10 +198,14 @@ def _overflow_perm(hidden, k: int, overflow: PreparedSlotWeights, ws: MoEWorkspa
     return ws.overflow_perm(hidden.shape[0] * k, int(overflow.physical_expert_count), hidden.device)
 
 
-def _pass_block_m(n_experts: int, H: int, I: int, device, n_pairs: int, path: int, pass_pairs: int | None = None) -> int:
+def _pass_block_m(n_experts: int, H: int, I: int, device, n_pairs: int, path: int, pass_pairs: int | None = None,
+                  *, mx4: bool = False) -> int:
     """The row-tile height to build the permutation of a pass over n_experts
     slots with: the path's own (the GEMVs read no tile table, path STREAM has
-    one height), else the MFMA kernel's for pass_pairs of n_pairs pairs."""
+    one height), else the MFMA kernel's for pass_pairs of n_pairs pairs.  mx4:
+    the experts are in 4 bits."""
+    if mx4:
+        return native.mx4_block_m(n_pairs if pass_pairs is None else pass_pairs, n_experts)
     if path == native.LMOE_PATH_GEMV:
         return native.MFMA_BLOCK_M
     if path == native.LMOE_PATH_STREAM:
@@ -196,7 +217,7 @@ def _block_m(hidden, k: int, w13_slots, path: int) -> int:
     """_pass_block_m of a pass over a whole bank."""
     T, H = hidden.shape
     P, I = int(w13_slots.shape[0]), int(w13_slots.shape[1]) // 2
-    return _pass_block_m(P, H, I, hidden.device, T * k, path)
+    return _pass_block_m(P, H, I, hidden.device, T * k, path, mx4=mxfp4.is_mx4(w13_slots))
 
 
 def _overflow_permute(hidden, topk_ids, k: int, overflow: PreparedSlotWeights, ws: MoEWorkspace, *,
@@ -227,6 +248,8 @@ def _merged_passes(hidden, k: int, w13_slots, overflow: PreparedSlotWeights, pat
     shapes, ~33 of 48 layers with an overflow pass) ran the GEMVs, shared
     launches took the layer from 186.0 to 180.2 us, and both tables' builds in
     one permutation launch on top of them to 176.0 us (same box)."""
+    if mxfp4.is_mx4(w13_slots):
+        return False
     if path == native.LMOE_PATH_GEMV:
         return hidden.shape[1] <= native.TWO_PASS_MAX_COLS and \
             int(w13_slots.shape[1]) // 2 <= native.TWO_PASS_MAX_COLS
@@ -256,12 +279,13 @@ def _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2p
     k = int(topk_ids.shape[1])
     P = int(w13_slots.shape[0])
     I = int(w13_slots.shape[1]) // 2
-    ws = workspace or get_workspace(T, k, P, H, I, hidden.device)
+    mx4 = mxfp4.is_mx4(w13_slots)
+    ws = workspace or get_workspace(T, k, P, H, I, hidden.device, rows=rows_kind(hidden, w13_slots))
     dst = out if out is not None else ws.out[:T]
     if path == native.LMOE_PATH_AUTO:
         path = _bank_layer_path(hidden, k, w13_slots, log2phy, overflow)
     # the decode body; past its pair count path GEMV runs the two GEMVs apart
-    decode = path == native.LMOE_PATH_GEMV and T * k <= native.FUSED_DECODE_MAX_PAIRS
+    decode = path == native.LMOE_PATH_GEMV and T * k <= native.FUSED_DECODE_MAX_PAIRS and not mx4
     bm = _block_m(hidden, k, w13_slots, path)
     merged = overflow is not None and log2phy is not None and not events and \
         _merged_passes(hidden, k, w13_slots, overflow, path)
@@ -361,7 +385,7 @@ def decode_layer(
     bm = _block_m(hidden, kw, w13_slots, path)
     merged = overflow is not None and log2phy is not None and _merged_passes(hidden, kw, w13_slots, overflow, path)
     perm_b = None
-    fused_body = overflow is None and path == native.LMOE_PATH_GEMV
+    fused_body = overflow is None and path == native.LMOE_PATH_GEMV and not mxfp4.is_mx4(w13_slots)
     if T == 1 and fused_body:
         # the one-token body reads the pairs in pair order: no sort at the
         # end of the router's chain (the same bits as the sorted form)
@@ -669,7 +693,7 @@ def run_wave_prefill(
     t_sched = perf_counter()
     profiling = bool(runtime.profile_path)
     wave_profiles: dict[int, dict] = {}
-    ws = get_workspace(T, k, P, H, I, hidden.device, tag="waves")
+    ws = get_workspace(T, k, P, H, I, hidden.device, tag="waves", rows=rows_kind(hidden, bank.w13_slots))
     report = WaveRunReport(plan.waves, sched.compute_order)
     staged: dict[int, tuple] = {}
     total_logical = runtime.total_logical_expert_count_for_layer(layer_id=layer_id, fallback=num_logical_experts)
@@ -722,7 +746,8 @@ def run_wave_prefill(
             try:
                 native.permute(topk_ids, ws.perm, log2phy=prepared.log2phy, skip_unmapped=True, keep_rows=not first,
                                table_len=total_logical if first else routed,
-                               block_m=_pass_block_m(len(plan.waves[w]), H, I, hidden.device, T * k, mlp_path, pairs))
+                               block_m=_pass_block_m(len(plan.waves[w]), H, I, hidden.device, T * k, mlp_path, pairs,
+                                                     mx4=mxfp4.is_mx4(prepared.w1)))
                 first = False
                 native.grouped_mlp(hidden, k, prepared.w1, prepared.w2, ws.perm, ws.act[: T * k], ws.y[: T * k],
                                    path=mlp_path, pass_pairs=pairs)
@@ -871,7 +896,8 @@ def run_device_waves(
               for b in range(min(n_buf, n_waves))]
     tables = [runtime._get_prefill_stage_log2phy_buffer(template_bank=bank, buffer_index=b, num_logical_experts=total,
                                                         device=dev) for b in range(len(stages))]
-    ws = get_workspace(T, k, int(stages[0].physical_expert_count), H, I, dev, tag="device_waves")
+    ws = get_workspace(T, k, int(stages[0].physical_expert_count), H, I, dev, tag="device_waves",
+                       rows=rows_kind(hidden, bank.w13_slots))
     capturing = _is_current_graph_capturing()
     compute = torch.cuda.current_stream(dev)
     tx = runtime.transfer_engine._transfer_stream(dev)
@@ -899,7 +925,7 @@ def run_device_waves(
     released: list = [None] * len(stages)
     mlp_path = _layer_path(hidden, k, total, bank.w13_slots) if path == native.LMOE_PATH_AUTO else path
     pairs = -(-(T * k) // n_waves)  # of a wave, on average
-    bm = _pass_block_m(P, H, I, dev, T * k, mlp_path, pairs)
+    bm = _pass_block_m(P, H, I, dev, T * k, mlp_path, pairs, mx4=mxfp4.is_mx4(bank.w13_slots))
     for w in range(n_waves):
         b = w % len(stages)
         stage, table = stages[b], tables[b]
@@ -952,7 +978,8 @@ def run_full_layer(
     )
     T, H = hidden.shape
     k = int(topk_ids.shape[1])
-    ws = get_workspace(T, k, prepared.physical_expert_count, H, int(prepared.w1.shape[1]) // 2, hidden.device, tag="full")
+    ws = get_workspace(T, k, prepared.physical_expert_count, H, int(prepared.w1.shape[1]) // 2, hidden.device, tag="full",
+                       rows=rows_kind(hidden, prepared.w1))
     dst = fused_experts(hidden, topk_weights, topk_ids, prepared.w1, prepared.w2, prepared.log2phy,
                         add=add, out=out, path=path, workspace=ws)
     if not _is_current_graph_capturing():

@@ -18,6 +18,8 @@ from pathlib import Path
 
 import torch
 
+from vllm_moe_offload_amd import mxfp4
+
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "liblatchmoe_hip.so"
 
 LMOE_SCORING_SOFTMAX = 0
@@ -62,6 +64,12 @@ EXPORTED_SYMBOLS = (
     "lmoe_decode_mlp_two_passes",
     "lmoe_stream_mlp_two_passes",
     "lmoe_combine",
+    "lmoe_combine_f32",
+    "lmoe_add_rms_norm",
+    "lmoe_rows_to_mx8",
+    "lmoe_mx4_bytes",
+    "lmoe_mx4_gateup_silu",
+    "lmoe_mx4_down",
     "lmoe_fused_moe_decode",
     "lmoe_fused_moe_decode_noalloc",
     "lmoe_down_combine",
@@ -138,6 +146,18 @@ _SIGNATURES = {
          _vp, _vp, _vp],
     ),
     "lmoe_combine": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
+    "lmoe_combine_f32": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
+    "lmoe_add_rms_norm": (_i, [_vp, _i, _i, _vp, _i, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp]),
+    "lmoe_rows_to_mx8": (_i, [_vp, _i, _i, _vp, _vp, _vp]),
+    "lmoe_mx4_bytes": (ctypes.c_longlong, [_i, _i]),
+    "lmoe_mx4_gateup_silu": (
+        _i,
+        [_vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp],
+    ),
+    "lmoe_mx4_down": (
+        _i,
+        [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _vp],
+    ),
     "lmoe_fused_moe_decode": (
         _i,
         [_vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
@@ -268,6 +288,136 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple | None = 
         raise ValueError(f"{name} must be contiguous")
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+# ---------------------------------------------------------------------------
+# 8-bit rows and the norm in front of a MoE layer
+# ---------------------------------------------------------------------------
+@dataclass(frozen=True)
+class Mx8Rows:
+    """Rows in 8 bits: e4m3 values, one power-of-two scale per 32 columns
+    (value[r, c] = q[r, c] * 2^(scale[r, c // 32] - 127); 255: NaN)."""
+
+    q: torch.Tensor      # [R, K] float8_e4m3fn
+    scale: torch.Tensor  # [R, K / 32] uint8
+
+    @classmethod
+    def allocate(cls, rows: int, columns: int, device) -> "Mx8Rows":
+        if int(columns) <= 0 or int(columns) % mxfp4.GROUP:
+            raise ValueError(f"8-bit rows are multiples of {mxfp4.GROUP} columns, got {columns}")
+        return cls(torch.empty((int(rows), int(columns)), dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty((int(rows), int(columns) // mxfp4.GROUP), dtype=torch.uint8, device=device))
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.q.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.q.device
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.q.dtype
+
+    def __getitem__(self, rows: slice) -> "Mx8Rows":
+        if not isinstance(rows, slice):
+            raise TypeError("8-bit rows are sliced by rows")
+        return Mx8Rows(self.q[rows], self.scale[rows])
+
+    def float(self) -> torch.Tensor:
+        """The f32 values that the rows stand for (checks and exports)."""
+        s = torch.ldexp(torch.ones_like(self.scale, dtype=torch.float32), self.scale.int() - 127)
+        s = torch.where(self.scale == 255, torch.full_like(s, float("nan")), s)
+        return (self.q.float().unflatten(-1, (-1, mxfp4.GROUP)) * s.unsqueeze(-1)).flatten(-2)
+
+
+def _need_mx8(rows, name: str, shape: tuple | None = None) -> None:
+    if not isinstance(rows, Mx8Rows):
+        raise TypeError(f"{name} must be Mx8Rows")
+    _need(rows.q, f"{name}.q", torch.float8_e4m3fn, shape)
+    if rows.q.dim() != 2 or rows.q.shape[1] % mxfp4.GROUP:
+        raise ValueError(f"{name} must be [R, K], K a multiple of {mxfp4.GROUP}, got {tuple(rows.q.shape)}")
+    _need(rows.scale, f"{name}.scale", torch.uint8, (rows.q.shape[0], rows.q.shape[1] // mxfp4.GROUP))
+
+
+def _same_device(*tensors) -> None:
+    """Every operand on the current device: a launch goes to its stream."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise ValueError(f"operand on {t.device}, the current device is cuda:{here}")
+
+
+def add_rms_norm(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    *,
+    residual: torch.Tensor | None = None,
+    residual_out: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    mx8: Mx8Rows | None = None,
+    eps: float = 1e-6,
+    stream=None,
+):
+    """r = x + residual; y = r / sqrt(mean(r^2) + eps) * weight.
+
+    y goes to out (bf16: the router gate, bf16 experts), to mx8 (4-bit experts'
+    8-bit rows) or to both; with neither given a bf16 out is made.  r goes to
+    residual_out, in place of residual if that is not given.  x [T, H] bf16,
+    residual bf16 or f32, weight [H] bf16 or f32; r is kept in f32 between the
+    sum and the outputs.  out or residual_out may be x or residual.  H a
+    multiple of 8 (of 32 with mx8) up to 32768.  Returns (out, mx8,
+    residual_out), None for what was not asked for."""
+    lib = load_library()
+    _need(x, "x", torch.bfloat16)
+    if x.dim() != 2:
+        raise ValueError(f"x must be [T, H], got {tuple(x.shape)}")
+    T, H = x.shape
+    if weight.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("weight must be bf16 or f32")
+    _need(weight, "weight", weight.dtype, (H,))
+    if residual is not None:
+        if residual.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("residual must be bf16 or f32")
+        _need(residual, "residual", residual.dtype, (T, H))
+        residual_out = residual if residual_out is None else residual_out
+        _need(residual_out, "residual_out", residual.dtype, (T, H))
+    elif residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    if out is None and mx8 is None:
+        out = torch.empty_like(x)
+    if out is not None:
+        _need(out, "out", torch.bfloat16, (T, H))
+    if mx8 is not None:
+        _need_mx8(mx8, "mx8", (T, H))
+    _same_device(x, weight, residual, residual_out, out, *((mx8.q, mx8.scale) if mx8 is not None else ()))
+    _check(
+        lib.lmoe_add_rms_norm(
+            _ptr(x), T, H, _ptr(residual), int(residual is not None and residual.dtype == torch.float32),
+            _ptr(weight), int(weight.dtype == torch.float32), float(eps), _ptr(residual_out), _ptr(out),
+            _ptr(mx8.q) if mx8 is not None else None, _ptr(mx8.scale) if mx8 is not None else None, _stream(stream),
+        ),
+        "lmoe_add_rms_norm",
+    )
+    return out, mx8, residual_out
+
+
+def rows_to_mx8(x: torch.Tensor, mx8: Mx8Rows | None = None, *, stream=None) -> Mx8Rows:
+    """bf16 rows x [T, H] in 8 bits (rows that were normed elsewhere)."""
+    lib = load_library()
+    _need(x, "x", torch.bfloat16)
+    if x.dim() != 2:
+        raise ValueError(f"x must be [T, H], got {tuple(x.shape)}")
+    if mx8 is None:
+        mx8 = Mx8Rows.allocate(x.shape[0], x.shape[1], x.device)
+    _need_mx8(mx8, "mx8", tuple(x.shape))
+    _same_device(x, mx8.q, mx8.scale)
+    _check(lib.lmoe_rows_to_mx8(_ptr(x), x.shape[0], x.shape[1], _ptr(mx8.q), _ptr(mx8.scale), _stream(stream)),
+           "lmoe_rows_to_mx8")
+    return mx8
 
 
 # ---------------------------------------------------------------------------
@@ -726,6 +876,20 @@ def prefill_block_m(n_experts: int, hidden: int, intermediate: int, device="cuda
     return PART_BLOCK_M
 
 
+MX4_BLOCK_M = 128  # row tiles of the 4-bit experts' prefill kernel
+
+
+def mx4_path(n_pairs: int, n_experts: int) -> int:
+    """The path of a layer of 4-bit experts, for every pass of it."""
+    return LMOE_PATH_GEMV
+
+
+def mx4_block_m(n_pairs: int, n_experts: int) -> int:
+    """Row-tile height of 4-bit experts' products (the permutation's block_m)
+    for n_pairs pairs over n_experts slots."""
+    return MX4_BLOCK_M
+
+
 @dataclass
 class Permutation:
     """Device outputs of lmoe_permute for one (n_pairs, n_slots) shape.
@@ -910,7 +1074,14 @@ def grouped_mlp(
 ) -> torch.Tensor:
     """y[pair] = W2_s . (silu(W13_s[:I] x) * W13_s[I:] x) for the placed pairs.
     pass_pairs: how many of the pairs the pass is expected to place, where it
-    is one wave of its layer (chooses the kernel's form, not its bits)."""
+    is one wave of its layer (chooses the kernel's form, not its bits).
+    4-bit banks (mxfp4.pack_experts; uint8): x and act are both bf16 or both
+    Mx8Rows, y is bf16 or f32."""
+    if mxfp4.is_mx4(w13_slots) or mxfp4.is_mx4(w2_slots):
+        if x.shape[1] != w2_slots.shape[1]:
+            raise ValueError(f"rows of {x.shape[1]} columns, w2_slots of {w2_slots.shape[1]} rows")
+        gateup_silu(x, top_k, w13_slots, perm, act, path=path, stream=stream)
+        return down(act, w2_slots, perm, y, path=path, stream=stream)
     lib = load_library()
     _need(x, "x", torch.bfloat16)
     T, H = x.shape
@@ -936,6 +1107,8 @@ def grouped_mlp(
 def gateup_silu(x: torch.Tensor, top_k: int, w13_slots: torch.Tensor, perm: Permutation, act: torch.Tensor,
                 *, path: int = LMOE_PATH_AUTO, stream=None) -> torch.Tensor:
     """act[pos] = silu(W13_s[:I] x) * (W13_s[I:] x) for the placed pairs (GMM1 + SwiGLU)."""
+    if mxfp4.is_mx4(w13_slots):
+        return _mx4_gateup_silu(x, top_k, w13_slots, perm, act, path=path, stream=stream)
     lib = load_library()
     _need(x, "x", torch.bfloat16)
     _need(w13_slots, "w13_slots", torch.bfloat16)
@@ -959,6 +1132,8 @@ def gateup_silu(x: torch.Tensor, top_k: int, w13_slots: torch.Tensor, perm: Perm
 def down(act: torch.Tensor, w2_slots: torch.Tensor, perm: Permutation, y: torch.Tensor,
          *, path: int = LMOE_PATH_AUTO, stream=None) -> torch.Tensor:
     """y[pair] = W2_s act[pos] for the placed pairs (GMM2)."""
+    if mxfp4.is_mx4(w2_slots):
+        return _mx4_down(act, w2_slots, perm, y, path=path, stream=stream)
     lib = load_library()
     _need(w2_slots, "w2_slots", torch.bfloat16)
     P, H, I = w2_slots.shape
@@ -972,6 +1147,70 @@ def down(act: torch.Tensor, w2_slots: torch.Tensor, perm: Permutation, y: torch.
             _ptr(perm.tile_off), _ptr(perm.meta), perm.n_pairs, perm.block_m, int(path), _ptr(y), _stream(stream),
         ),
         "lmoe_down",
+    )
+    return y
+
+
+def _need_mx4(bank: torch.Tensor, name: str, perm: Permutation, K: int) -> int:
+    """Check a 4-bit bank of K columns; returns its rows per expert."""
+    _need(bank, name, torch.uint8)
+    if bank.dim() != 3 or bank.shape[0] != perm.n_slots:
+        raise ValueError(f"{name} has shape {tuple(bank.shape)}, the permutation {perm.n_slots} slots")
+    if int(bank.shape[2]) != mxfp4.row_bytes(K):
+        raise ValueError(f"{name} rows of {int(bank.shape[2])} bytes do not hold {K} columns in 4 bits")
+    return int(bank.shape[1])
+
+
+def _need_rows(rows, name: str, shape: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """bf16 rows or Mx8Rows: (values, scales or None)."""
+    if isinstance(rows, Mx8Rows):
+        _need_mx8(rows, name, shape)
+        return rows.q, rows.scale
+    _need(rows, name, torch.bfloat16, shape)
+    return rows, None
+
+
+def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, act, *, path: int, stream):
+    lib = load_library()
+    xq, xs = _need_rows(x, "x")
+    T, H = xq.shape
+    two_i = _need_mx4(w13_slots, "w13_slots", perm, H)
+    if two_i % 2:
+        raise ValueError(f"w13_slots has {two_i} rows per expert")
+    if perm.n_pairs != T * int(top_k):
+        raise ValueError("permutation does not match T * top_k pairs")
+    aq, as_ = _need_rows(act, "act", (perm.n_pairs, two_i // 2))
+    if (xs is None) != (as_ is None):
+        raise ValueError("x and act must both be bf16 or both be Mx8Rows")
+    _same_device(xq, w13_slots, perm.offsets, aq)
+    _check(
+        lib.lmoe_mx4_gateup_silu(
+            _ptr(xq), _ptr(xs), T, H, two_i // 2, int(top_k), _ptr(w13_slots), perm.n_slots, _ptr(perm.offsets),
+            _ptr(perm.sorted_pairs), _ptr(perm.active), _ptr(perm.tile_off), _ptr(perm.meta), perm.n_pairs,
+            perm.block_m, int(path), _ptr(aq), _ptr(as_), _stream(stream),
+        ),
+        "lmoe_mx4_gateup_silu",
+    )
+    return act
+
+
+def _mx4_down(act, w2_slots: torch.Tensor, perm: Permutation, y: torch.Tensor, *, path: int, stream):
+    lib = load_library()
+    aq, as_ = _need_rows(act, "act")
+    if aq.dim() != 2 or aq.shape[0] != perm.n_pairs:
+        raise ValueError(f"act has shape {tuple(aq.shape)}, the permutation {perm.n_pairs} pairs")
+    H = _need_mx4(w2_slots, "w2_slots", perm, int(aq.shape[1]))
+    if y.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("y must be bf16 or f32")
+    _need(y, "y", y.dtype, (perm.n_pairs, H))
+    _same_device(aq, w2_slots, perm.offsets, y)
+    _check(
+        lib.lmoe_mx4_down(
+            _ptr(aq), _ptr(as_), H, int(aq.shape[1]), _ptr(w2_slots), perm.n_slots, _ptr(perm.offsets),
+            _ptr(perm.sorted_pairs), _ptr(perm.active), _ptr(perm.tile_off), _ptr(perm.meta), perm.n_pairs,
+            perm.block_m, int(path), _ptr(y), int(y.dtype == torch.float32), _stream(stream),
+        ),
+        "lmoe_mx4_down",
     )
     return y
 
@@ -1078,11 +1317,14 @@ def combine(
     add: torch.Tensor | None = None,
     stream=None,
 ) -> torch.Tensor:
-    """out[t] = add[t] + sum_j w[t,j] * y[t*k+j] (pairs with row_mask < 0 skipped)."""
+    """out[t] = add[t] + sum_j w[t,j] * y[t*k+j] (pairs with row_mask < 0
+    skipped); y bf16, or f32 (4-bit experts' rows of a few tokens)."""
     lib = load_library()
     _need(topk_weights, "topk_weights", torch.bfloat16)
     T, k = topk_weights.shape
-    _need(y, "y", torch.bfloat16)
+    if y.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"y must be bf16 or f32, got {y.dtype}")
+    _need(y, "y", y.dtype)
     H = y.shape[1]
     if y.shape[0] < T * k:
         raise ValueError("y has fewer rows than pairs")
@@ -1091,10 +1333,11 @@ def combine(
         _need(row_mask, "row_mask", torch.int32)
     if add is not None:
         _need(add, "add", torch.bfloat16, (T, H))
+    fn = "lmoe_combine_f32" if y.dtype == torch.float32 else "lmoe_combine"
     _check(
-        lib.lmoe_combine(_ptr(y), _ptr(row_mask), _ptr(topk_weights), T, k, H, _ptr(add),
+        getattr(lib, fn)(_ptr(y), _ptr(row_mask), _ptr(topk_weights), T, k, H, _ptr(add),
                          _ptr(out), _stream(stream)),
-        "lmoe_combine",
+        fn,
     )
     return out
 
