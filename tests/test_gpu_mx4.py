@@ -43,8 +43,9 @@ def _native():
 
 
 def _paths():
+    """(path, row-tile height): the split-K kernel, then row tiles."""
     native = _native()
-    return [native.LMOE_PATH_GEMV]
+    return [(native.LMOE_PATH_GEMV, 32)] + [(native.LMOE_PATH_MFMA, bm) for bm in native.MX4_BLOCK_M]
 
 
 def _f64(t):
@@ -153,10 +154,10 @@ def test_products_are_the_experts(H, I, counts, rows):
     l2p = rng.permutation(P).astype(np.int32)
     layer = Layer(H, I, P, T, rows, H + I)
     slot_of = np.where(ids[:, 0] >= 0, l2p[np.maximum(ids[:, 0], 0)], -1)
-    for path in _paths():
+    for path, bm in _paths():
         for y_dtype in (torch.bfloat16, torch.float32):
-            print(f"case mx4 H={H} I={I} {rows} path={path} {y_dtype}", flush=True)
-            perm, act, y = run_layer(layer, ids, 1, path, log2phy=to_dev_i32(l2p), y_dtype=y_dtype)
+            print(f"case mx4 H={H} I={I} {rows} path={path} block_m={bm} {y_dtype}", flush=True)
+            perm, act, y = run_layer(layer, ids, 1, path, block_m=bm, log2phy=to_dev_i32(l2p), y_dtype=y_dtype)
             torch.cuda.synchronize()
             check_layer(layer, perm, 1, act, y, slot_of)
             placed = int(perm.meta[native.META_PAIRS])
@@ -171,6 +172,27 @@ def test_products_are_the_experts(H, I, counts, rows):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("H,I,counts", [(160, 96, [1, 31, 32, 33, 63, 64, 65]), (1024, 416, [127, 128, 129, 5, 300])])
+def test_tile_heights_give_the_same_bits(H, I, counts, rows):
+    native = _native()
+    layer = Layer(H, I, len(counts), sum(counts), rows, 9)
+    ids = _ids(counts, 0, np.random.default_rng(9))
+    bits = lambda a, y: (y.view(torch.int16), a.q.view(torch.uint8) if rows == "mx8" else a.view(torch.int16))
+    _, *want = run_layer(layer, ids, 1, native.LMOE_PATH_MFMA, block_m=32)
+    for bm in native.MX4_BLOCK_M[1:]:
+        _, *got = run_layer(layer, ids, 1, native.LMOE_PATH_MFMA, block_m=bm)
+        for a, b in zip(bits(*got), bits(*want)):
+            assert torch.equal(a, b)
+    # a row alone, in whichever kernel form its tile then takes
+    for t in (0, sum(counts) - 1):
+        one = Layer.__new__(Layer)
+        one.__dict__.update(layer.__dict__, x=layer.x[t:t + 1])
+        _, _, y1 = run_layer(one, ids[t:t + 1], 1, native.LMOE_PATH_MFMA, block_m=64)
+        assert torch.equal(y1[0].view(torch.int16), want[1][t].view(torch.int16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
 def test_several_experts_per_token_and_the_same_twice(rows):
     """top_k 3; a token may name one expert twice: both pairs get their row."""
     rng = np.random.default_rng(5)
@@ -178,8 +200,8 @@ def test_several_experts_per_token_and_the_same_twice(rows):
     ids = rng.integers(0, P, (T, k)).astype(np.int32)
     ids[4] = [2, 2, 2]
     layer = Layer(96, 64, P, T, rows, 17)
-    for path in _paths():
-        perm, act, y = run_layer(layer, ids, k, path)
+    for path, bm in _paths():
+        perm, act, y = run_layer(layer, ids, k, path, block_m=bm)
         torch.cuda.synchronize()
         check_layer(layer, perm, k, act, y, ids.flatten())
         assert torch.equal(y[12], y[13]) and torch.equal(y[12], y[14])
@@ -195,13 +217,13 @@ def test_a_bad_row_stays_its_own(rows):
     rng = np.random.default_rng(8)
     ids = _ids([6, 20], 0, rng)
     layer = Layer(160, 96, 2, 26, rows, 3)
-    for path in _paths():
-        _, _, clean = run_layer(layer, ids, 1, path)
+    for path, bm in _paths():
+        _, _, clean = run_layer(layer, ids, 1, path, block_m=bm)
         for value in (float("nan"), float("inf")):
             bad = layer.x.clone() if rows == "bf16" else layer.x.float().to(torch.bfloat16)
             bad[5, 159] = value
             keep, layer.x = layer.x, bad if rows == "bf16" else native.rows_to_mx8(bad)
-            _, _, y = run_layer(layer, ids, 1, path)
+            _, _, y = run_layer(layer, ids, 1, path, block_m=bm)
             layer.x = keep
             assert not y[5].isfinite().any()
             other = torch.arange(26, device="cuda") != 5
@@ -224,8 +246,8 @@ def test_extreme_scales(rows):
     c, s = mxfp4.quantize(w13[0]); layer.v13 = [mx.values_mx4(c.numpy(), s.numpy())]
     c, s = mxfp4.quantize(w2[0]); layer.v2 = [mx.values_mx4(c.numpy(), s.numpy())]
     ids = np.zeros((2, 1), dtype=np.int32)
-    for path in _paths():
-        perm, act, y = run_layer(layer, ids, 1, path)
+    for path, bm in _paths():
+        perm, act, y = run_layer(layer, ids, 1, path, block_m=bm)
         check_layer(layer, perm, 1, act, y, ids.flatten())
         assert y[:, :32].abs().max() > 0.5
 

@@ -1,7 +1,10 @@
 // Entry points of the expert products over 4-bit weights.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "mx4_few.h"
+#include "mx4_tile.h"
 
 LMOE_FLAGS_UNIT(mx4)
 
@@ -61,6 +64,56 @@ static void launch_few(const Mx4Args& g, hipStream_t stream) {
   else mx4_few_kernel<GU, false><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
 }
 
+// Row tiles of BM rows, at most n_pairs / BM + one short one per slot.
+template <bool GU, bool A8, int BM>
+static int launch_tiles(const Mx4Args& g, hipStream_t stream) {
+  const int lds = Mx4Tile<A8, BM>::lds_bytes(mx4_chunks(g.K));
+  if (lds > 160 * 1024) return LMOE_ERR_SHAPE;
+  constexpr int cols = GU ? kTileCols / 2 : kTileCols;
+  const long long tiles = g.n_pairs / BM + (g.n_pairs < g.P ? g.n_pairs : g.P);
+  const long long grid = 8 * ((tiles * ((g.N + cols - 1) / cols) + 7) / 8);
+  if (grid > 0x7fffffffLL) return LMOE_ERR_SHAPE;
+  static bool raised[64] = {};  // per device: dynamic LDS past 64 KiB allowed
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return static_cast<int>(e);
+  if (dev < 0 || dev >= 64 || !raised[dev]) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx4_tile_kernel<GU, A8, BM>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e != hipSuccess) return static_cast<int>(e);
+    if (dev >= 0 && dev < 64) raised[dev] = true;
+  }
+  mx4_tile_kernel<GU, A8, BM><<<static_cast<unsigned>(grid), kTileWaves * 64, lds, stream>>>(g);
+  return LMOE_OK;
+}
+
+static bool known_block_m(int bm) { return bm == 32 || bm == 64 || bm == 128; }
+
+template <bool GU, bool A8>
+static int launch_tiles(const Mx4Args& g, int block_m, hipStream_t stream) {
+  if (block_m == 32) return launch_tiles<GU, A8, 32>(g, stream);
+  if (block_m == 64) return launch_tiles<GU, A8, 64>(g, stream);
+  return launch_tiles<GU, A8, 128>(g, stream);
+}
+
+// path AUTO: row tiles past this many pairs per slot, on average
+constexpr int kFewPairsPerSlot = 16;
+
+template <bool GU>
+static int launch(const Mx4Args& g, int path, int block_m, hipStream_t stream) {
+  if (path == LMOE_PATH_GEMV ||
+      (path == LMOE_PATH_AUTO &&
+       (!known_block_m(block_m) || g.n_pairs <= static_cast<long long>(kFewPairsPerSlot) * g.P))) {
+    launch_few<GU>(g, stream);
+  } else {
+    if (!known_block_m(block_m)) return LMOE_ERR_SHAPE;
+    const int st = g.a_scale != nullptr ? launch_tiles<GU, true>(g, block_m, stream)
+                                        : launch_tiles<GU, false>(g, block_m, stream);
+    if (st != LMOE_OK) return st;
+  }
+  LMOE_RETURN_LAUNCH();
+}
+
 }  // namespace lmoe
 
 using namespace lmoe;
@@ -89,8 +142,7 @@ extern "C" int lmoe_mx4_gateup_silu(const void* x, const void* x_scale, int T, i
   const Mx4Args g{x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(w13_slots),
                   lmoe_mx4_bytes(2 * I, H), H, I, k, n_slots, n_pairs, offsets, sorted_pairs, active,
                   tile_off, meta, act, static_cast<uint8_t*>(act_scale), false};
-  launch_few<true>(g, stream);
-  LMOE_RETURN_LAUNCH();
+  return launch<true>(g, path, block_m, stream);
 }
 
 extern "C" int lmoe_mx4_down(const void* act, const void* act_scale, int H, int I,
@@ -109,8 +161,7 @@ extern "C" int lmoe_mx4_down(const void* act, const void* act_scale, int H, int 
   const Mx4Args g{act, static_cast<const uint8_t*>(act_scale), static_cast<const uint8_t*>(w2_slots),
                   lmoe_mx4_bytes(H, I), I, H, 1, n_slots, n_pairs, offsets, sorted_pairs, active,
                   tile_off, meta, y, nullptr, y_f32 != 0};
-  launch_few<false>(g, stream);
-  LMOE_RETURN_LAUNCH();
+  return launch<false>(g, path, block_m, stream);
 }
 
 extern "C" int lmoe_combine_f32(const void* y, const int32_t* row_idx, const uint16_t* w, int T, int k,

@@ -1,0 +1,272 @@
+// Expert products over 4-bit weights in row tiles (prefill).
+//
+// A workgroup of four waves computes BM rows of one slot by 256 weight rows:
+// gate-up 128 act columns (gate and up), down 256 y columns.  Each wave takes all
+// BM rows and 64 weight rows (four 16-row blocks; gate-up: gate, up, gate, up of
+// 32 act columns).  Per chunk of 128 columns the rows go to LDS without passing
+// through registers (two buffers, the next chunk in flight under this one's
+// products), where all four waves read them; weights go from memory straight to
+// registers, one chunk ahead, since the bank's order is the fragments' order and
+// no two waves share any.
+//
+// LDS holds 16-byte piece p of row r at position p ^ sw(r), so that the sixteen
+// rows a fragment read touches spread over all banks: MX8 rows are 8 pieces a
+// chunk, sw = r % 8 ^ r / 8 % 2; bf16 rows 16 pieces, sw = r % 16.  The e4m3
+// scales of the whole tile are put into LDS once, by chunk and row.
+//
+// Every output adds its chunks in order, whatever BM is: the same bits.
+#pragma once
+
+#include "mx4_few.h"
+
+namespace lmoe {
+
+constexpr int kTileWaves = 4;
+constexpr int kTileCols = 256;  // weight rows of a workgroup
+
+__device__ __attribute__((aligned(16))) const uint32_t g_zero16[4] = {0, 0, 0, 0};
+
+template <bool A8, int BM_>
+struct Mx4Tile {
+  static constexpr int BM = BM_;
+  static constexpr int NF = BM / 16;                 // 16-row fragments
+  static constexpr int PIECES = A8 ? 8 : 16;         // 16-byte pieces of a row's chunk
+  static constexpr int ROWB = PIECES * 16;
+  static constexpr int STAGE = BM * ROWB;
+  static constexpr int RPL = 64 / PIECES;            // rows one load instruction fills
+  static constexpr int QA = STAGE / 1024 / kTileWaves;  // load instructions per wave and chunk
+  static_assert(QA * kTileWaves * 1024 == STAGE, "whole load instructions");
+  static constexpr int OFF_PAIR = 2 * STAGE;         // BM pair ids
+  static constexpr int OFF_SCALE = OFF_PAIR + BM * 4;
+  static int lds_bytes(int chunks) { return OFF_SCALE + (A8 ? BM * 4 * chunks : 0); }
+  static __device__ __forceinline__ int sw(int r) { return A8 ? ((r & 7) ^ ((r >> 3) & 1)) : (r & 15); }
+};
+
+__device__ __forceinline__ void load_lds16b(const void* src, char* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+// every load of this wave has landed and its LDS accesses are done; then the others'
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// The slot whose row tiles hold tile (tile_off ascending, P + 1 entries).
+__device__ __forceinline__ int slot_of_tile(const int32_t* tile_off, int P, int tile) {
+  int lo = 0, hi = P;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tile_off[mid] <= tile) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+template <bool GU, bool A8, int BM>
+__global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g) {
+  using C = Mx4Tile<A8, BM>;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  int* s_pair = reinterpret_cast<int*>(smem + C::OFF_PAIR);
+  uint32_t* s_scale = reinterpret_cast<uint32_t*>(smem + C::OFF_SCALE);
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // work item: XCD-contiguous chunks of (row tile, column tile)
+  constexpr int OUT_COLS = GU ? kTileCols / 2 : kTileCols;
+  const int NT = (g.N + OUT_COLS - 1) / OUT_COLS;
+  const int total = g.meta[LMOE_META_TILES] * NT;
+  const int share = (total + 7) >> 3;
+  const int jj = blockIdx.x >> 3;
+  const int item = (blockIdx.x & 7) * share + jj;
+  if (jj >= share || item >= total) return;
+  const int tile = item / NT;
+  const int n0 = (item - tile * NT) * OUT_COLS;
+  const int slot = slot_of_tile(g.tile_off, g.P, tile);
+  const int p0 = g.offsets[slot] + (tile - g.tile_off[slot]) * BM;
+  const int rows = min(BM, g.offsets[slot + 1] - p0);
+
+  const int K = g.K;
+  const int chunks = mx4_chunks(K);
+  const int tail = K & (kMxChunk - 1);  // columns of a short last chunk, 0: none
+  const size_t row_bytes = static_cast<size_t>(K) * (A8 ? 1 : 2);
+
+  // this lane's source of each load instruction: row, and piece within a chunk
+  auto a_row = [&](int q) { return (wave * C::QA + q) * C::RPL + lane / C::PIECES; };
+  auto a_piece = [&](int q) { return (lane % C::PIECES) ^ C::sw(a_row(q)); };
+  const char* a_src[C::QA];
+#pragma unroll
+  for (int q = 0; q < C::QA; ++q) {
+    const int r = a_row(q);
+    const int pos = p0 + (r < rows ? r : 0);
+    const size_t src = GU ? g.sorted_pairs[pos] / g.topk : pos;
+    a_src[q] = static_cast<const char*>(g.a) + src * row_bytes + a_piece(q) * 16;
+  }
+  auto issue = [&](int c, int buf) {
+    char* st = smem + buf * C::STAGE + wave * C::QA * 1024;
+    const bool cut = tail != 0 && c == chunks - 1;
+    if (!cut) {
+#pragma unroll
+      for (int q = 0; q < C::QA; ++q) load_lds16b(a_src[q] + static_cast<size_t>(c) * C::ROWB, st + q * 1024);
+    } else {
+#pragma unroll
+      for (int q = 0; q < C::QA; ++q) {
+        const char* p = a_src[q] + static_cast<size_t>(c) * C::ROWB;
+        if (a_piece(q) * (A8 ? 16 : 8) >= tail) p = reinterpret_cast<const char*>(g_zero16);
+        load_lds16b(p, st + q * 1024);
+      }
+    }
+  };
+
+  // this wave's four weight blocks; blocks past the matrix repeat the last one
+  const int wblocks = (GU ? 2 * g.N : g.N) / 16;
+  const int b0 = (GU ? 2 * n0 : n0) / 16 + 4 * wave;
+  const int bb = mx4_block_bytes(K);
+  const bool wave_live = b0 < wblocks;
+  const uint8_t* wsrc[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    wsrc[j] = g.w + slot * g.w_slot_bytes + static_cast<size_t>(min(b0 + j, wblocks - 1)) * bb;
+  const uint32_t code_at = 256 + lane * 16, scale_at = lane * 4;
+  auto load_w = [&](int c, i32x4_t (&w)[4], int (&sc)[4]) {
+    const int quad = (c >> 2) * kMxQuadBytes;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint8_t* p = wsrc[j] + quad;
+      w[j] = *reinterpret_cast<const i32x4_t*>(p + (c & 3) * 1024 + code_at);
+      sc[j] = *reinterpret_cast<const int*>(p + scale_at);
+    }
+  };
+
+  i32x4_t w[2][4];
+  int wsc[2][4];
+  issue(0, 0);
+  load_w(0, w[0], wsc[0]);
+  for (int r = tid; r < BM; r += kTileWaves * 64) s_pair[r] = g.sorted_pairs[p0 + (r < rows ? r : 0)];
+  if constexpr (A8) {
+    const int groups = K / kMxGroup;
+    for (int i = tid; i < BM * chunks; i += kTileWaves * 64) {
+      const int c = i / BM, r = i - c * BM;
+      const int pos = p0 + (r < rows ? r : 0);
+      const size_t src = GU ? g.sorted_pairs[pos] / g.topk : pos;
+      const uint8_t* sp = g.a_scale + src * groups + 4 * c;
+      uint32_t v;
+      if (tail == 0) {
+        v = *reinterpret_cast<const uint32_t*>(sp);
+      } else {
+        v = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v |= static_cast<uint32_t>(4 * c + e < groups ? sp[e] : kScaleOne) << (8 * e);
+      }
+      s_scale[i] = v;
+    }
+  }
+
+  f32x4_t acc[C::NF][4];
+#pragma unroll
+  for (int i = 0; i < C::NF; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const int fr = lane & 15;
+  const int fsw = C::sw(fr);  // fragments start at multiples of 16 rows
+  const int live = (rows + 15) >> 4;
+
+  // NL: 16-row fragments computed, a compile-time count so that the products are
+  // straight-line code; rows past the tile's last are dropped at the store
+  auto main_loop = [&](auto nl_tag) {
+    constexpr int NL = decltype(nl_tag)::value;
+    auto products = [&](int c, const i32x4_t (&wv)[4], const int (&sc)[4]) {
+      const char* st = smem + (c & 1) * C::STAGE + fr * C::ROWB;
+      const int shift = 8 * (c & 3);
+      // the next row fragment is on its way from LDS while this one is multiplied
+      if constexpr (A8) {
+        int s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = sc[j] >> shift;
+        RowFrag<true> x[2];
+        auto read = [&](int i) {
+          const char* p = st + i * 16 * C::ROWB;
+          const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(p + ((lg ^ fsw) * 16));
+          const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(p + (((4 + lg) ^ fsw) * 16));
+          x[i & 1].v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          x[i & 1].scale = reinterpret_cast<const uint8_t*>(s_scale + c * BM + i * 16 + fr)[lg];
+        };
+        read(0);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          if (i + 1 < NL) read(i + 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = mx4_step<true>(wv[j], s[j], x[i & 1], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        float s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = mx_scale_f32((sc[j] >> shift) & 255);
+        bf16x8v_t x[2];
+        auto read = [&](int n) {  // n: quarter of the chunk * NL + fragment
+          const int k = n / NL, i = n % NL;
+          x[n & 1] = *reinterpret_cast<const bf16x8v_t*>(st + i * 16 * C::ROWB + (((4 * lg + k) ^ fsw) * 16));
+        };
+        read(0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // quarters as mx4_step takes them
+          bf16x8v_t wb[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) wb[j] = weights_bf16(wv[j][k], s[j]);
+#pragma unroll
+          for (int i = 0; i < NL; ++i) {
+            const int n = k * NL + i;
+            if (n + 1 < 4 * NL) read(n + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j], x[n & 1], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+    };
+    auto step = [&](int c, i32x4_t (&now)[4], int (&now_sc)[4], i32x4_t (&next)[4], int (&next_sc)[4]) {
+      tile_barrier();  // chunk c is in LDS; every wave is done with the other buffer
+      if (c + 1 < chunks) {
+        issue(c + 1, (c + 1) & 1);
+        load_w(c + 1, next, next_sc);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (NL > 0) products(c, now, now_sc);
+    };
+    for (int c = 0; c < chunks; c += 2) {
+      step(c, w[0], wsc[0], w[1], wsc[1]);
+      if (c + 1 < chunks) step(c + 1, w[1], wsc[1], w[0], wsc[0]);
+    }
+  };
+  if (!wave_live) main_loop(std::integral_constant<int, 0>{});
+  else if (C::NF > 4 && live > 6) main_loop(std::integral_constant<int, C::NF>{});
+  else if (C::NF > 4 && live > 4) main_loop(std::integral_constant<int, C::NF < 6 ? C::NF : 6>{});
+  else if (C::NF > 2 && live > 2) main_loop(std::integral_constant<int, C::NF < 4 ? C::NF : 4>{});
+  else if (C::NF > 1 && live > 1) main_loop(std::integral_constant<int, C::NF < 2 ? C::NF : 2>{});
+  else main_loop(std::integral_constant<int, 1>{});
+  if (!wave_live) return;
+
+#pragma unroll
+  for (int i = 0; i < C::NF; ++i) {
+    const int r = 16 * i + fr;
+    if (i >= live) break;
+    if constexpr (GU) {
+      const f32x4_t gate[2] = {acc[i][0], acc[i][2]}, up[2] = {acc[i][1], acc[i][3]};
+      store_act<A8>(g, p0 + r, n0 + 32 * wave, lane, r < rows, gate, up);
+    } else if (r < rows) {
+      const int pair = s_pair[r];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (b0 + j < wblocks) store_y(g, pair, n0 + 64 * wave + 16 * j + 4 * lg, acc[i][j]);
+    }
+  }
+}
+
+}  // namespace lmoe

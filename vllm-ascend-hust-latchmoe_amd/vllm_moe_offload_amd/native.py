@@ -876,18 +876,23 @@ def prefill_block_m(n_experts: int, hidden: int, intermediate: int, device="cuda
     return PART_BLOCK_M
 
 
-MX4_BLOCK_M = 128  # row tiles of the 4-bit experts' prefill kernel
+MX4_BLOCK_M = (32, 64, 128)  # row-tile heights of the 4-bit experts' prefill kernel
+MX4_FEW_PAIRS_PER_EXPERT = 16
 
 
 def mx4_path(n_pairs: int, n_experts: int) -> int:
-    """The path of a layer of 4-bit experts, for every pass of it."""
-    return LMOE_PATH_GEMV
+    """The path of a layer of 4-bit experts, for every pass of it: the split-K
+    kernel for few pairs per expert, row tiles past that."""
+    return LMOE_PATH_GEMV if n_pairs <= MX4_FEW_PAIRS_PER_EXPERT * n_experts else LMOE_PATH_MFMA
 
 
 def mx4_block_m(n_pairs: int, n_experts: int) -> int:
     """Row-tile height of 4-bit experts' products (the permutation's block_m)
     for n_pairs pairs over n_experts slots."""
-    return MX4_BLOCK_M
+    for bm in MX4_BLOCK_M:
+        if n_pairs <= bm * n_experts:
+            return bm
+    return MX4_BLOCK_M[-1]
 
 
 @dataclass
