@@ -101,16 +101,16 @@ __device__ __forceinline__ bf16x8v_t weights_bf16(int word, float s) {
   return bf16x8v_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// acc += W x^T of one chunk: 16 weight rows, 16 rows.  scale: the weights' scale
-// byte in the low 8 bits.
-template <bool A8>
+// acc += W x^T of one chunk: 16 weight rows, 16 rows.  Byte B of scale: the
+// weights' scale.
+template <bool A8, int B = 0>
 __device__ __forceinline__ f32x4_t mx4_step(i32x4_t w, int scale, const RowFrag<A8>& x, f32x4_t acc) {
   if constexpr (A8) {
     const i32x8_t wide = __builtin_shufflevector(w, w, 0, 1, 2, 3, 0, 1, 2, 3);
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide, x.v, acc, 4 /* e2m1 */, 0 /* e4m3 */, 0,
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide, x.v, acc, 4 /* e2m1 */, 0 /* e4m3 */, B,
                                                             scale, 0, x.scale);
   } else {
-    const float s = mx_scale_f32(scale & 255);
+    const float s = mx_scale_f32((scale >> (8 * B)) & 255);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(weights_bf16(w[j], s), __builtin_bit_cast(bf16x8v_t, x.v[j]),

@@ -9,9 +9,11 @@
 // registers, one chunk ahead, since the bank's order is the fragments' order and
 // no two waves share any.
 //
-// LDS holds 16-byte piece p of row r at position p ^ sw(r), so that the sixteen
-// rows a fragment read touches spread over all banks: MX8 rows are 8 pieces a
-// chunk, sw = r % 8 ^ r / 8 % 2; bf16 rows 16 pieces, sw = r % 16.  The e4m3
+// LDS holds 16-byte piece p of row r at position p ^ sw(r).  A 16-byte read goes
+// by sixteen lanes at a time, 0-3, 12-15, 20-27 first and 4-11, 16-19, 28-31 next
+// (and so from 32 on); lane l reads row l % 16 and a piece that steps with l / 16.
+// sw = r / 2 for MX8 rows (8 pieces a chunk, two rows over all banks) and r + 4 for
+// bf16 rows (16 pieces) puts each sixteen on sixteen different positions.  The e4m3
 // scales of the whole tile are put into LDS once, by chunk and row.
 //
 // Every output adds its chunks in order, whatever BM is: the same bits.
@@ -39,7 +41,7 @@ struct Mx4Tile {
   static constexpr int OFF_PAIR = 2 * STAGE;         // BM pair ids
   static constexpr int OFF_SCALE = OFF_PAIR + BM * 4;
   static int lds_bytes(int chunks) { return OFF_SCALE + (A8 ? BM * 4 * chunks : 0); }
-  static __device__ __forceinline__ int sw(int r) { return A8 ? ((r & 7) ^ ((r >> 3) & 1)) : (r & 15); }
+  static __device__ __forceinline__ int sw(int r) { return A8 ? (r >> 1) & 7 : (r + 4) & 15; }
 };
 
 __device__ __forceinline__ void load_lds16b(const void* src, char* lds) {
@@ -76,16 +78,17 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   // work item: XCD-contiguous chunks of (row tile, column tile)
   constexpr int OUT_COLS = GU ? kTileCols / 2 : kTileCols;
   const int NT = (g.N + OUT_COLS - 1) / OUT_COLS;
-  const int total = g.meta[LMOE_META_TILES] * NT;
+  const int total = __builtin_amdgcn_readfirstlane(g.meta[LMOE_META_TILES]) * NT;
   const int share = (total + 7) >> 3;
   const int jj = blockIdx.x >> 3;
   const int item = (blockIdx.x & 7) * share + jj;
   if (jj >= share || item >= total) return;
   const int tile = item / NT;
   const int n0 = (item - tile * NT) * OUT_COLS;
-  const int slot = slot_of_tile(g.tile_off, g.P, tile);
-  const int p0 = g.offsets[slot] + (tile - g.tile_off[slot]) * BM;
-  const int rows = min(BM, g.offsets[slot + 1] - p0);
+  // uniform, and kept in scalar registers
+  const int slot = __builtin_amdgcn_readfirstlane(slot_of_tile(g.tile_off, g.P, tile));
+  const int p0 = __builtin_amdgcn_readfirstlane(g.offsets[slot] + (tile - g.tile_off[slot]) * BM);
+  const int rows = __builtin_amdgcn_readfirstlane(min(BM, g.offsets[slot + 1] - p0));
 
   const int K = g.K;
   const int chunks = mx4_chunks(K);
@@ -129,7 +132,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   for (int j = 0; j < 4; ++j)
     wsrc[j] = g.w + slot * g.w_slot_bytes + static_cast<size_t>(min(b0 + j, wblocks - 1)) * bb;
   const uint32_t code_at = 256 + lane * 16, scale_at = lane * 4;
-  auto load_w = [&](int c, i32x4_t (&w)[4], int (&sc)[4]) {
+  auto load_w = [&](int c, i32x4_t (&w)[4], int (&sc)[4]) {  // sc: byte c % 4 is the chunk's
     const int quad = (c >> 2) * kMxQuadBytes;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -139,10 +142,10 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
     }
   };
 
-  i32x4_t w[2][4];
-  int wsc[2][4];
+  i32x4_t w_next[4];
+  int sc_next[4];
   issue(0, 0);
-  load_w(0, w[0], wsc[0]);
+  load_w(0, w_next, sc_next);
   for (int r = tid; r < BM; r += kTileWaves * 64) s_pair[r] = g.sorted_pairs[p0 + (r < rows ? r : 0)];
   if constexpr (A8) {
     const int groups = K / kMxGroup;
@@ -178,21 +181,29 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   // straight-line code; rows past the tile's last are dropped at the store
   auto main_loop = [&](auto nl_tag) {
     constexpr int NL = decltype(nl_tag)::value;
-    auto products = [&](int c, const i32x4_t (&wv)[4], const int (&sc)[4]) {
-      const char* st = smem + (c & 1) * C::STAGE + fr * C::ROWB;
-      const int shift = 8 * (c & 3);
-      // the next row fragment is on its way from LDS while this one is multiplied
-      if constexpr (A8) {
-        int s[4];
+    for (int c = 0; c < chunks; ++c) {
+      tile_barrier();  // chunk c is in LDS; every wave is done with the other buffer
+      i32x4_t w[4];
+      int sc[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = sc[j] >> shift;
+      for (int j = 0; j < 4; ++j) {
+        w[j] = w_next[j];
+        sc[j] = sc_next[j] >> (8 * (c & 3));
+      }
+      if (c + 1 < chunks) issue(c + 1, (c + 1) & 1);
+      load_w(c + 1 < chunks ? c + 1 : c, w_next, sc_next);
+      __builtin_amdgcn_sched_barrier(0);
+      const char* st = smem + (c & 1) * C::STAGE + fr * C::ROWB;
+      // the next row fragment is on its way from LDS while this one is multiplied
+      if constexpr (A8 && NL > 0) {
         RowFrag<true> x[2];
+        const uint8_t* xs = reinterpret_cast<const uint8_t*>(s_scale + c * BM + fr) + lg;
         auto read = [&](int i) {
           const char* p = st + i * 16 * C::ROWB;
           const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(p + ((lg ^ fsw) * 16));
           const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(p + (((4 + lg) ^ fsw) * 16));
           x[i & 1].v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          x[i & 1].scale = reinterpret_cast<const uint8_t*>(s_scale + c * BM + i * 16 + fr)[lg];
+          x[i & 1].scale = xs[i * 64];
         };
         read(0);
 #pragma unroll
@@ -200,13 +211,13 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
           if (i + 1 < NL) read(i + 1);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = mx4_step<true>(wv[j], s[j], x[i & 1], acc[i][j]);
+          for (int j = 0; j < 4; ++j) acc[i][j] = mx4_step<true>(w[j], sc[j], x[i & 1], acc[i][j]);
           __builtin_amdgcn_sched_barrier(0);
         }
-      } else {
+      } else if constexpr (NL > 0) {
         float s[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = mx_scale_f32((sc[j] >> shift) & 255);
+        for (int j = 0; j < 4; ++j) s[j] = mx_scale_f32(sc[j] & 255);
         bf16x8v_t x[2];
         auto read = [&](int n) {  // n: quarter of the chunk * NL + fragment
           const int k = n / NL, i = n % NL;
@@ -217,7 +228,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
         for (int k = 0; k < 4; ++k) {  // quarters as mx4_step takes them
           bf16x8v_t wb[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) wb[j] = weights_bf16(wv[j][k], s[j]);
+          for (int j = 0; j < 4; ++j) wb[j] = weights_bf16(w[j][k], s[j]);
 #pragma unroll
           for (int i = 0; i < NL; ++i) {
             const int n = k * NL + i;
@@ -230,19 +241,6 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
           }
         }
       }
-    };
-    auto step = [&](int c, i32x4_t (&now)[4], int (&now_sc)[4], i32x4_t (&next)[4], int (&next_sc)[4]) {
-      tile_barrier();  // chunk c is in LDS; every wave is done with the other buffer
-      if (c + 1 < chunks) {
-        issue(c + 1, (c + 1) & 1);
-        load_w(c + 1, next, next_sc);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (NL > 0) products(c, now, now_sc);
-    };
-    for (int c = 0; c < chunks; c += 2) {
-      step(c, w[0], wsc[0], w[1], wsc[1]);
-      if (c + 1 < chunks) step(c + 1, w[1], wsc[1], w[0], wsc[0]);
     }
   };
   if (!wave_live) main_loop(std::integral_constant<int, 0>{});
