@@ -3,6 +3,7 @@
 
 #include <type_traits>
 
+#include "gemm_lds.h"
 #include "mx4_few.h"
 #include "mx4_tile.h"
 

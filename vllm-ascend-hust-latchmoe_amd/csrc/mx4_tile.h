@@ -40,7 +40,8 @@ struct Mx4Tile {
   static_assert(QA * kTileWaves * 1024 == STAGE, "whole load instructions");
   static constexpr int OFF_PAIR = 2 * STAGE;         // BM pair ids
   static constexpr int OFF_SCALE = OFF_PAIR + BM * 4;
-  static int lds_bytes(int chunks) { return OFF_SCALE + (A8 ? BM * 4 * chunks : 0); }
+  // scales go to LDS 64 dwords at a time: two chunks of 32 rows
+  static int lds_bytes(int chunks) { return OFF_SCALE + (A8 ? BM * 4 * ((chunks + 1) & ~1) : 0); }
   static __device__ __forceinline__ int sw(int r) { return A8 ? (r >> 1) & 7 : (r + 4) & 15; }
 };
 
@@ -53,15 +54,33 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// The slot whose row tiles hold tile (tile_off ascending, P + 1 entries).
-__device__ __forceinline__ int slot_of_tile(const int32_t* tile_off, int P, int tile) {
-  int lo = 0, hi = P;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (tile_off[mid] <= tile) lo = mid;
-    else hi = mid;
+// The slot whose row tiles hold a tile, its first tile and its rows: the last of the
+// slots from first whose tile_off is not past the tile (ascending; P + 1 entries).  A
+// wave looks 64 of them up at once, one per lane.
+struct SlotWindow {
+  int t0, o0, o1;
+};
+__device__ __forceinline__ SlotWindow load_window(const int32_t* tile_off, const int32_t* offsets, int P, int first,
+                                                  int lane) {
+  const int at = min(first + lane, P - 1);
+  return {tile_off[at], offsets[at], offsets[at + 1]};
+}
+struct TileSlot {
+  int slot, tile0, p0, p1;
+};
+// The lookup in a window that was loaded from first on; further windows as needed.
+__device__ __forceinline__ TileSlot slot_of_tile(const int32_t* tile_off, const int32_t* offsets, int P, int tile,
+                                                 int first, SlotWindow v, int lane) {
+  for (;;) {
+    const int k = __popcll(__ballot(v.t0 <= tile)) - 1;  // lane 0's always is
+    const int last = min(63, P - 1 - first);             // lanes past it repeat its entry
+    if (k < 63 || last < 63 || first + 64 >= P || tile_off[first + 64] > tile) {
+      const int l = min(k, last);
+      return {first + l, read_lane_i32(v.t0, l), read_lane_i32(v.o0, l), read_lane_i32(v.o1, l)};
+    }
+    first += 64;
+    v = load_window(tile_off, offsets, P, first, lane);
   }
-  return lo;
 }
 
 template <bool GU, bool A8, int BM>
@@ -78,17 +97,18 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   // work item: XCD-contiguous chunks of (row tile, column tile)
   constexpr int OUT_COLS = GU ? kTileCols / 2 : kTileCols;
   const int NT = (g.N + OUT_COLS - 1) / OUT_COLS;
-  const int total = __builtin_amdgcn_readfirstlane(g.meta[LMOE_META_TILES]) * NT;
+  const int total = g.meta[LMOE_META_TILES] * NT;
   const int share = (total + 7) >> 3;
   const int jj = blockIdx.x >> 3;
   const int item = (blockIdx.x & 7) * share + jj;
   if (jj >= share || item >= total) return;
   const int tile = item / NT;
   const int n0 = (item - tile * NT) * OUT_COLS;
-  // uniform, and kept in scalar registers
-  const int slot = __builtin_amdgcn_readfirstlane(slot_of_tile(g.tile_off, g.P, tile));
-  const int p0 = __builtin_amdgcn_readfirstlane(g.offsets[slot] + (tile - g.tile_off[slot]) * BM);
-  const int rows = __builtin_amdgcn_readfirstlane(min(BM, g.offsets[slot + 1] - p0));
+  const TileSlot ts = slot_of_tile(g.tile_off, g.offsets, g.P, tile, 0,
+                                   load_window(g.tile_off, g.offsets, g.P, 0, lane), lane);
+  const int slot = ts.slot;
+  const int p0 = ts.p0 + (tile - ts.tile0) * BM;
+  const int rows = min(BM, ts.p1 - p0);
 
   const int K = g.K;
   const int chunks = mx4_chunks(K);
@@ -149,21 +169,25 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   for (int r = tid; r < BM; r += kTileWaves * 64) s_pair[r] = g.sorted_pairs[p0 + (r < rows ? r : 0)];
   if constexpr (A8) {
     const int groups = K / kMxGroup;
-    for (int i = tid; i < BM * chunks; i += kTileWaves * 64) {
-      const int c = i / BM, r = i - c * BM;
-      const int pos = p0 + (r < rows ? r : 0);
-      const size_t src = GU ? g.sorted_pairs[pos] / g.topk : pos;
-      const uint8_t* sp = g.a_scale + src * groups + 4 * c;
-      uint32_t v;
-      if (tail == 0) {
-        v = *reinterpret_cast<const uint32_t*>(sp);
-      } else {
-        v = 0;
+    const int r = tid & (BM - 1);  // a row's scales, some chunks of it
+    const int pos = p0 + (r < rows ? r : 0);
+    const uint8_t* sp = g.a_scale + static_cast<size_t>(GU ? g.sorted_pairs[pos] / g.topk : pos) * groups;
+    constexpr int STEP = kTileWaves * 64 / BM;
+    if (tail == 0) {  // straight to LDS, 64 of them at a time
+      for (int c = wave * 64 / BM; c < chunks; c += STEP) {
+        const int mine = min(c + lane / BM, chunks - 1);  // two chunks where BM is 32
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(sp + 4 * mine),
+            (__attribute__((address_space(3))) void*)(s_scale + c * BM + (wave * 64 & (BM - 1))), 4, 0, 0);
+      }
+    } else {
+      for (int c = tid / BM; c < chunks; c += STEP) {
+        uint32_t v = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          v |= static_cast<uint32_t>(4 * c + e < groups ? sp[e] : kScaleOne) << (8 * e);
+          v |= static_cast<uint32_t>(4 * c + e < groups ? sp[e + 4 * c] : kScaleOne) << (8 * e);
+        s_scale[c * BM + r] = v;
       }
-      s_scale[i] = v;
     }
   }
 
@@ -258,11 +282,10 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
     if constexpr (GU) {
       const f32x4_t gate[2] = {acc[i][0], acc[i][2]}, up[2] = {acc[i][1], acc[i][3]};
       store_act<A8>(g, p0 + r, n0 + 32 * wave, lane, r < rows, gate, up);
-    } else if (r < rows) {
+    } else {
       const int pair = s_pair[r];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (b0 + j < wblocks) store_y(g, pair, n0 + 64 * wave + 16 * j + 4 * lg, acc[i][j]);
+      store_y(g, pair, n0 + 64 * wave, lane, r < rows, acc[i][0], acc[i][1]);
+      if (b0 + 2 < wblocks) store_y(g, pair, n0 + 64 * wave + 32, lane, r < rows, acc[i][2], acc[i][3]);
     }
   }
 }
