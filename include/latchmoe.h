@@ -468,6 +468,49 @@ int lmoe_mx4_down(const void* act, const void* act_scale, int H, int I,
                   int block_m, int path, void* y, int y_f32,
                   hipStream_t stream);
 
+/* Buffers of lmoe_mx4_fused_moe for T*k pairs over n_slots slots: lmoe_permute's
+ * outputs and workspace, act (with act_scale: MX8 rows) and y as lmoe_mx4_down
+ * writes it. */
+typedef struct lmoe_mx4_workspace {
+  int32_t* counts;
+  int32_t* offsets;
+  int32_t* sorted_pairs;
+  int32_t* row_idx;
+  int32_t* active;
+  int32_t* tile_off;
+  int32_t* meta;
+  void* permute_workspace;
+  size_t permute_workspace_bytes;
+  void* act;
+  void* act_scale;
+  void* y;
+  int32_t y_f32;
+} lmoe_mx4_workspace;
+
+/* A layer of 4-bit experts in one call: lmoe_permute (skip_unmapped 0),
+ * lmoe_mx4_gateup_silu, lmoe_mx4_down and the combine (add may be null), with the
+ * same arguments and results; every argument is checked before the first of
+ * them is queued.  Calls that may run at once need workspaces of their own. */
+int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int H, int I,
+                       int k, const void* w13_slots, const void* w2_slots,
+                       int n_slots, const uint16_t* w, const int32_t* ids,
+                       const int32_t* log2phy, int n_log2phy, int path,
+                       int block_m, const lmoe_mx4_workspace* ws,
+                       const void* add, void* out, hipStream_t stream);
+
+/* One token (x [H], ids and w [k]) through 4-bit experts without a permutation,
+ * in two launches: act[j] of pair j as lmoe_mx4_gateup_silu makes it (path GEMV,
+ * the same bits; rows of pairs without a slot untouched), then out = add +
+ * sum_j w[j] W2 act[j], summed in f32.  A pair whose id maps to no slot adds
+ * nothing and is counted in LMOE_FLAG_UNPLACED.  One slot may serve several
+ * pairs.  Shapes and alignment as lmoe_mx4_gateup_silu and lmoe_combine_f32. */
+int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, int I, int k,
+                        const void* w13_slots, const void* w2_slots,
+                        int n_slots, const uint16_t* w, const int32_t* ids,
+                        const int32_t* log2phy, int n_log2phy, const void* add,
+                        void* act, void* act_scale, void* out,
+                        hipStream_t stream);
+
 /* The second half of lmoe_fused_moe_decode on its own: down GEMV from act
  * (sorted order) fused with the weighted combine into out (same argument
  * meaning).  Replaces npu_grouped_matmul GMM2 + npu_moe_token_unpermute of

@@ -291,6 +291,110 @@ def test_fused_experts_over_a_4_bit_bank(T, k, E, rows):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("H,I,k,E", [(32, 32, 1, 2), (160, 96, 3, 5), (1024, 416, 5, 8), (2048, 768, 8, 16),
+                                     (544, 1056, 9, 12), (64, 64, 20, 4)])
+def test_one_token_straight_from_its_ids(H, I, k, E, rows):
+    """act has the split-K kernel's bits, out the pairs' weighted sum; a pair
+    without a slot adds nothing and is counted; a slot may serve several pairs."""
+    from vllm_moe_offload_amd import fused_moe, native
+
+    rng = np.random.default_rng(H + k)
+    ids = rng.integers(0, E, (1, k)).astype(np.int32)  # k > E, or by chance: the same twice
+    if k > 2:
+        ids[0, 1] = E + 3                              # outside the table
+    l2p = rng.permutation(E).astype(np.int32)
+    if k > 3:
+        l2p[ids[0, 3]] = -1
+    layer = Layer(H, I, E, 1, rows, H)
+    d_ids, d_l2p = to_dev_i32(ids), to_dev_i32(l2p)
+    w = torch.empty((1, k), device="cuda").uniform_(0.05, 1).to(torch.bfloat16)
+    add = torch.randn((1, H), device="cuda").to(torch.bfloat16)
+    bufs = native.Mx4Buffers(native.Permutation.allocate(k, E, "cuda"), layer.act_buffer(k),
+                             torch.empty((k, H), dtype=torch.float32, device="cuda"))
+    native.device_flags(clear=True)
+    out = native.mx4_decode_one(layer.x, w, d_ids, layer.w13, layer.w2, d_l2p, bufs,
+                                torch.empty((1, H), dtype=torch.bfloat16, device="cuda"), add=add)
+    slots = np.array([l2p[e] if e < E else -1 for e in ids[0]])
+    assert native.device_flags(clear=True)[native.FLAG_UNPLACED] == int((slots < 0).sum())
+    perm, act, y = run_layer(layer, ids, k, native.LMOE_PATH_GEMV, log2phy=d_l2p, y_dtype=torch.float32)
+    bits = lambda a: a.q.view(torch.uint8) if rows == "mx8" else a.view(torch.int16)
+    pos = perm.row_idx.cpu().numpy()
+    for j in range(k):
+        if slots[j] >= 0:
+            assert torch.equal(bits(bufs.act)[j], bits(act)[pos[j]]), j
+        else:
+            assert pos[j] == -1 and torch.equal(bits(bufs.act)[j], bits(layer.act_buffer(1))[0])
+    placed = torch.from_numpy(slots >= 0).cuda()
+    yw = _f64(y[placed]) * _f64(w)[0][slots >= 0][:, None]
+    want, mag = yw.sum(0) + _f64(add)[0], np.abs(yw).sum(0) + np.abs(_f64(add))[0]
+    av = _f64(act.float() if rows == "mx8" else act)[: int((slots >= 0).sum())]
+    worst = max((sum_error(av, v, rows == "mx8").max() for v in layer.v2), default=0.0) if len(av) else 0.0
+    tol = 2.0**-8 * np.abs(want) + (k + 10) * 2.0**-24 * mag + 2 * k * worst
+    assert np.all(np.abs(_f64(out)[0] - want) <= tol)
+    # the layer's calls take this form, with the same bits
+    if (slots >= 0).all():
+        again = fused_moe.fused_experts(layer.x, w, d_ids, layer.w13, layer.w2, d_l2p, add=add)
+        assert torch.equal(again, out)
+        inp = fused_moe.MoEFusedExpertsInput(
+            hidden_states=layer.x, topk_weights=w, topk_ids=d_ids, weights=fused_moe.MoEWeights(layer.w13, layer.w2),
+            routing=fused_moe.MoERoutingParams(log2phy=d_l2p), shared_output=add)
+        res = fused_moe.run_fused_experts_contract(inp)
+        assert torch.equal(res.routed_out, out)
+        assert np.array_equal(res.expert_tokens.cpu().numpy(), np.bincount(slots, minlength=E))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("T", [1, 2, 33])
+def test_decode_layer_over_a_4_bit_bank(T, rows):
+    """Router, permutation and experts of a decode step: the norm's two outputs
+    in, the same bits as the separate calls, captured as well as eager."""
+    from vllm_moe_offload_amd import fused_moe, native
+
+    E, H, I, k = 16, 256, 96, 4
+    layer = Layer(H, I, E, T, rows, 6)
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.empty((T, H), device="cuda").normal_(generator=g).to(torch.bfloat16)
+    res = torch.empty((T, H), device="cuda").normal_(generator=g).to(torch.bfloat16)
+    nw = torch.empty(H, device="cuda").uniform_(0.5, 1.5, generator=g).to(torch.bfloat16)
+    gate = torch.empty((E, H), device="cuda").normal_(0, 0.2, generator=g).to(torch.bfloat16)
+    hidden, ro = torch.empty_like(x), torch.empty_like(res)
+    mx8 = native.Mx8Rows.allocate(T, H, "cuda") if rows == "mx8" else None
+    spec = fused_moe.RouterSpec(top_k=k)
+    ws = fused_moe.get_workspace(T, k, E, H, I, "cuda", tag="dl", rows=rows)
+    logits = torch.empty((T, E), dtype=torch.bfloat16, device="cuda")
+    w, ids = torch.empty((T, k), dtype=torch.bfloat16, device="cuda"), torch.empty((T, k), dtype=torch.int32, device="cuda")
+    l2p = to_dev_i32(np.random.default_rng(1).permutation(E))
+    out = torch.empty_like(x)
+
+    def step():
+        native.add_rms_norm(x, nw, residual=res, residual_out=ro, out=hidden, mx8=mx8)
+        fused_moe.decode_layer(hidden, gate, spec, layer.w13, layer.w2, l2p, workspace=ws, out=out, logits_out=logits,
+                               w_out=w, ids_out=ids, expert_rows=mx8)
+
+    step()
+    torch.cuda.synchronize()
+    want = fused_moe.fused_experts(hidden if mx8 is None else mx8, w, ids, layer.w13, layer.w2, l2p).clone()
+    assert torch.equal(out, want)
+    rw, rids, _ = fused_moe.route(hidden, gate, spec)
+    assert torch.equal(rw, w) and torch.equal(rids, ids)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for seed in range(3):
+        x.normal_(generator=torch.Generator(device="cuda").manual_seed(seed + 50))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        step()
+        torch.cuda.synchronize()
+        assert torch.equal(got, out)
+        want = fused_moe.fused_experts(hidden if mx8 is None else mx8, w, ids, layer.w13, layer.w2, l2p)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
 def test_masked_pairs_and_a_token_without_any(rows):
     """Pairs whose expert has no slot add nothing; a token without a pair is its
     addend; the status words count what was dropped."""
@@ -370,9 +474,40 @@ def test_empty_batches_and_refusals():
         lambda: native.fused_moe_decode(layer.x, w, layer.w13, layer.w2, perm, act, y),
         lambda: native.down_combine(act, w, layer.w2, perm, y),
     ]
+    bf = [torch.zeros(s, dtype=torch.bfloat16, device="cuda") for s in ((2, 64, 64), (2, 64, 32))]
+    bufs = native.Mx4Buffers(perm, act, y)
+    one = native.Mx4Buffers(native.Permutation.allocate(1, 2, "cuda"), act[:1], y[:1])
+    out = torch.empty((4, 64), dtype=torch.bfloat16, device="cuda")
+    layer_call = lambda x=layer.x, w=w, ids=ids, b=bufs, w13=layer.w13, w2=layer.w2, l2p=None, o=out, **kw: \
+        native.mx4_fused_moe(x, w, ids, w13, w2, l2p, b, o, block_m=32, **kw)
+    wrong += [
+        lambda: fused_moe.fused_experts(x8, w, ids, *bf, None),                 # 8-bit rows, bf16 experts
+        lambda: fused_moe.fused_experts(layer.x, w, ids, layer.w13, layer.w2, None,
+                                        workspace=fused_moe.get_workspace(4, 1, 2, 64, 32, "cuda")),
+        lambda: fused_moe.get_workspace(4, 1, 2, 64, 32, "cuda", rows="int8"),
+        lambda: layer_call(x=x8),
+        lambda: layer_call(w=w.float()),
+        lambda: layer_call(ids=ids.long()),
+        lambda: layer_call(ids=ids[:2]),
+        lambda: layer_call(w13=layer.w13[:1]),
+        lambda: layer_call(o=out[:2]),
+        lambda: layer_call(l2p=torch.zeros(2, device="cuda")),
+        lambda: layer_call(add=out.float()),
+        lambda: native.mx4_decode_one(layer.x, w, ids, layer.w13, layer.w2, None, bufs, out),
+        lambda: native.Mx4Buffers(perm, act[:2], y),
+        lambda: native.Mx4Buffers(perm, act, y.half()),
+        lambda: fused_moe.decode_layer(layer.x, bf[0][0, :16, :].contiguous(), fused_moe.RouterSpec(top_k=1), layer.w13,
+                                       layer.w2, None, workspace=fused_moe.get_workspace(4, 1, 2, 64, 32, "cuda", rows="mx8"),
+                                       expert_rows=native.Mx8Rows.allocate(3, 64, "cuda")),
+    ]
+    layer_call()
+    native.mx4_decode_one(layer.x[:1], w[:1], ids[:1], layer.w13, layer.w2, None, one, out[:1])
     for i, call in enumerate(wrong):
         with pytest.raises((ValueError, TypeError)):
             call()
             pytest.fail(f"call {i} was taken")
+    with pytest.raises(RuntimeError, match="unsupported shape"):
+        native.mx4_fused_moe(layer.x, w, ids, layer.w13, layer.w2, None, bufs, out, block_m=256,
+                             path=native.LMOE_PATH_MFMA)
     with pytest.raises(RuntimeError, match="unsupported option"):
         native.gateup_silu(layer.x, 1, layer.w13, perm, act, path=native.LMOE_PATH_STREAM)

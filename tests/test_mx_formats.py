@@ -151,6 +151,31 @@ def test_c_entries_check_their_arguments():
         lib.lmoe_mx4_down(act, as_, H, I, w, P, P16, P16, P16, P16, P16, n, bm, path, y, 0, N)
     assert dn(n=0, act=N, y=N) == 0 and dn(n=-1) == 1000 and dn(act=N) == 1000 and dn(y=N) == 1000
     assert dn(H=48) == 1001 and dn(I=16) == 1001 and dn(y=P16 + 8) == 1001 and dn(path=9) == 1003
+    from vllm_moe_offload_amd.native import _Mx4Workspace
+    import ctypes
+
+    def ws(**kw):
+        v = {n: P16 for n, _ in _Mx4Workspace._fields_}
+        return _Mx4Workspace(**{**v, "y_f32": 1, **kw})
+
+    def fused(x=P16, xs=P16, T=2, H=64, I=32, k=2, w13=P16, w2=P16, P=4, w=P16, ids=P16, path=0, bm=32, wsp=None,
+              add=N, out=P16):
+        s = ws() if wsp is None else wsp
+        return lib.lmoe_mx4_fused_moe(x, xs, T, H, I, k, w13, w2, P, w, ids, N, 0, path, bm, ctypes.addressof(s), add,
+                                      out, N)
+
+    assert lib.lmoe_mx4_fused_moe(P16, P16, 2, 64, 32, 2, P16, P16, 4, P16, P16, N, 0, 0, 32, N, N, P16, N) == 1000
+    assert fused(T=-1) == 1000 and fused(k=0) == 1000 and fused(P=0) == 1000 and fused(x=N) == 1000 and fused(ids=N) == 1000
+    assert fused(w=N) == 1000 and fused(out=N) == 1000 and fused(xs=N) == 1000 and fused(w13=N) == 1000 and fused(w2=N) == 1000
+    assert fused(wsp=ws(act=None)) == 1000 and fused(wsp=ws(y=None)) == 1000 and fused(wsp=ws(act_scale=None)) == 1000
+    assert fused(H=48) == 1001 and fused(I=40) == 1001 and fused(P=70000) == 1001 and fused(T=1 << 30, k=4) == 1001
+    assert fused(x=P16 + 8) == 1001 and fused(add=P16 + 8) == 1001 and fused(out=P16 + 8) == 1001
+    assert fused(path=2, bm=256) == 1001 and fused(path=2, bm=128, H=32 * 4096) == 1001 and fused(path=3) == 1003
+    one = lambda x=P16, xs=P16, H=64, I=32, k=2, w13=P16, w2=P16, P=4, w=P16, ids=P16, n=0, add=N, act=P16, as_=P16, out=P16: \
+        lib.lmoe_mx4_decode_one(x, xs, H, I, k, w13, w2, P, w, ids, N, n, add, act, as_, out, N)
+    assert one(x=N) == 1000 and one(xs=N) == 1000 and one(as_=N) == 1000 and one(w=N) == 1000 and one(ids=N) == 1000
+    assert one(act=N) == 1000 and one(out=N) == 1000 and one(k=0) == 1000 and one(n=-1) == 1000 and one(w2=N) == 1000
+    assert one(H=40) == 1001 and one(I=40) == 1001 and one(k=70000) == 1001 and one(add=P16 + 2) == 1001
     comb = lambda y=P16, w=P16, T=1, k=2, H=64, out=P16, add=N: \
         lib.lmoe_combine_f32(y, N, w, T, k, H, add, out, N)
     assert comb(T=0, y=N, out=N) == 0 and comb(y=N) == 1000 and comb(H=60) == 1001 and comb(out=P16 + 2) == 1001

@@ -60,7 +60,8 @@ static bool bad16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) 
 
 template <bool GU>
 static void launch_few(const Mx4Args& g, hipStream_t stream) {
-  const dim3 grid(g.N / 32, g.n_pairs < g.P ? g.n_pairs : g.P);
+  constexpr int cols = kFewMxBlocks * (GU ? 8 : 16);
+  const dim3 grid((g.N + cols - 1) / cols, g.n_pairs < g.P ? g.n_pairs : g.P);
   if (g.a_scale != nullptr) mx4_few_kernel<GU, true><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
   else mx4_few_kernel<GU, false><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
 }
@@ -69,7 +70,6 @@ static void launch_few(const Mx4Args& g, hipStream_t stream) {
 template <bool GU, bool A8, int BM>
 static int launch_tiles(const Mx4Args& g, hipStream_t stream) {
   const int lds = Mx4Tile<A8, BM>::lds_bytes(mx4_chunks(g.K));
-  if (lds > 160 * 1024) return LMOE_ERR_SHAPE;
   constexpr int cols = GU ? kTileCols / 2 : kTileCols;
   const long long tiles = g.n_pairs / BM + (g.n_pairs < g.P ? g.n_pairs : g.P);
   const long long grid = 8 * ((tiles * ((g.N + cols - 1) / cols) + 7) / 8);
@@ -90,6 +90,15 @@ static int launch_tiles(const Mx4Args& g, hipStream_t stream) {
 
 static bool known_block_m(int bm) { return bm == 32 || bm == 64 || bm == 128; }
 
+// Whether rows of K columns fit the LDS of tiles of block_m rows (MX8 rows: their scales).
+static bool tiles_fit(int block_m, bool a8, int K) {
+  const int chunks = mx4_chunks(K);
+  const int lds = block_m == 32   ? (a8 ? Mx4Tile<true, 32>::lds_bytes(chunks) : Mx4Tile<false, 32>::lds_bytes(chunks))
+                  : block_m == 64 ? (a8 ? Mx4Tile<true, 64>::lds_bytes(chunks) : Mx4Tile<false, 64>::lds_bytes(chunks))
+                                  : (a8 ? Mx4Tile<true, 128>::lds_bytes(chunks) : Mx4Tile<false, 128>::lds_bytes(chunks));
+  return lds <= 160 * 1024;
+}
+
 template <bool GU, bool A8>
 static int launch_tiles(const Mx4Args& g, int block_m, hipStream_t stream) {
   if (block_m == 32) return launch_tiles<GU, A8, 32>(g, stream);
@@ -100,14 +109,18 @@ static int launch_tiles(const Mx4Args& g, int block_m, hipStream_t stream) {
 // path AUTO: row tiles past this many pairs per slot, on average
 constexpr int kFewPairsPerSlot = 16;
 
+static bool takes_tiles(int path, int block_m, bool a8, int H, int I, int n_pairs, int P) {
+  if (path != LMOE_PATH_AUTO) return path == LMOE_PATH_MFMA;
+  return known_block_m(block_m) && n_pairs > static_cast<long long>(kFewPairsPerSlot) * P &&
+         tiles_fit(block_m, a8, H) && tiles_fit(block_m, a8, I);
+}
+
 template <bool GU>
 static int launch(const Mx4Args& g, int path, int block_m, hipStream_t stream) {
-  if (path == LMOE_PATH_GEMV ||
-      (path == LMOE_PATH_AUTO &&
-       (!known_block_m(block_m) || g.n_pairs <= static_cast<long long>(kFewPairsPerSlot) * g.P))) {
+  if (!takes_tiles(path, block_m, g.a_scale != nullptr, g.K, g.N, g.n_pairs, g.P)) {
     launch_few<GU>(g, stream);
   } else {
-    if (!known_block_m(block_m)) return LMOE_ERR_SHAPE;
+    if (!known_block_m(block_m) || !tiles_fit(block_m, g.a_scale != nullptr, g.K)) return LMOE_ERR_SHAPE;
     const int st = g.a_scale != nullptr ? launch_tiles<GU, true>(g, block_m, stream)
                                         : launch_tiles<GU, false>(g, block_m, stream);
     if (st != LMOE_OK) return st;
@@ -175,5 +188,72 @@ extern "C" int lmoe_combine_f32(const void* y, const int32_t* row_idx, const uin
   combine_f32_kernel<<<dim3(T, (H + 255) / 256), 64, 0, stream>>>(
       static_cast<const float*>(y), row_idx, w, k, H, static_cast<const uint16_t*>(add),
       static_cast<uint16_t*>(out));
+  LMOE_RETURN_LAUNCH();
+}
+
+// The layer of few or many tokens: what the four calls do, in one.
+extern "C" int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int H, int I, int k,
+                                  const void* w13_slots, const void* w2_slots, int n_slots,
+                                  const uint16_t* w, const int32_t* ids, const int32_t* log2phy,
+                                  int n_log2phy, int path, int block_m, const lmoe_mx4_workspace* ws,
+                                  const void* add, void* out, hipStream_t stream) {
+  if (ws == nullptr || T < 0 || k <= 0) return LMOE_ERR_ARG;
+  const long long n = static_cast<long long>(T) * k;
+  if (n > 0x7fffffffLL) return LMOE_ERR_SHAPE;
+  if (T > 0 && (ids == nullptr || w == nullptr || out == nullptr)) return LMOE_ERR_ARG;
+  // every check of the products before the permutation is queued
+  if (H <= 0 || I <= 0 || n_slots <= 0) return LMOE_ERR_ARG;
+  if (H % kMxGroup != 0 || I % kMxGroup != 0 || n_slots > kMaxSlots) return LMOE_ERR_SHAPE;
+  if (!known_path(path)) return LMOE_ERR_UNSUPPORTED;
+  if (T > 0) {
+    if (x == nullptr || w13_slots == nullptr || w2_slots == nullptr || ws->act == nullptr || ws->y == nullptr ||
+        (x_scale == nullptr) != (ws->act_scale == nullptr))
+      return LMOE_ERR_ARG;
+    if (bad16(x) || bad16(w13_slots) || bad16(w2_slots) || bad16(ws->act) || bad16(ws->y) || bad16(add) || bad16(out))
+      return LMOE_ERR_SHAPE;
+    if (path == LMOE_PATH_MFMA && (!known_block_m(block_m) || !tiles_fit(block_m, x_scale != nullptr, H) ||
+                                   !tiles_fit(block_m, x_scale != nullptr, I)))
+      return LMOE_ERR_SHAPE;
+  }
+  int st = lmoe_permute(ids, static_cast<int>(n), log2phy, n_log2phy, n_slots, 0, block_m, ws->counts, ws->offsets,
+                        ws->sorted_pairs, ws->row_idx, ws->active, ws->tile_off, ws->meta, ws->permute_workspace,
+                        ws->permute_workspace_bytes, stream);
+  if (st != LMOE_OK || T == 0) return st;
+  st = lmoe_mx4_gateup_silu(x, x_scale, T, H, I, k, w13_slots, n_slots, ws->offsets, ws->sorted_pairs, ws->active,
+                            ws->tile_off, ws->meta, static_cast<int>(n), block_m, path, ws->act, ws->act_scale, stream);
+  if (st != LMOE_OK) return st;
+  st = lmoe_mx4_down(ws->act, ws->act_scale, H, I, w2_slots, n_slots, ws->offsets, ws->sorted_pairs, ws->active,
+                     ws->tile_off, ws->meta, static_cast<int>(n), block_m, path, ws->y, ws->y_f32, stream);
+  if (st != LMOE_OK) return st;
+  return ws->y_f32 ? lmoe_combine_f32(ws->y, ws->row_idx, w, T, k, H, add, out, stream)
+                   : lmoe_combine(ws->y, ws->row_idx, w, T, k, H, add, out, stream);
+}
+
+extern "C" int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, int I, int k, const void* w13_slots,
+                                   const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids,
+                                   const int32_t* log2phy, int n_log2phy, const void* add, void* act,
+                                   void* act_scale, void* out, hipStream_t stream) {
+  if (H <= 0 || I <= 0 || k <= 0 || n_slots <= 0 || n_log2phy < 0) return LMOE_ERR_ARG;
+  if (H % kMxGroup != 0 || I % kMxGroup != 0 || k > kMaxSlots) return LMOE_ERR_SHAPE;
+  if (x == nullptr || w13_slots == nullptr || w2_slots == nullptr || w == nullptr || ids == nullptr ||
+      act == nullptr || out == nullptr || (x_scale == nullptr) != (act_scale == nullptr))
+    return LMOE_ERR_ARG;
+  if (bad16(x) || bad16(w13_slots) || bad16(w2_slots) || bad16(act) || bad16(add) || bad16(out)) return LMOE_ERR_SHAPE;
+  const OneToken o{ids, log2phy, n_log2phy};
+  const Mx4Args gu{x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(w13_slots),
+                   lmoe_mx4_bytes(2 * I, H), H, I, k, n_slots, k, nullptr, nullptr, nullptr, nullptr, nullptr, act,
+                   static_cast<uint8_t*>(act_scale), false};
+  const Mx4Args dn{act, static_cast<const uint8_t*>(act_scale), static_cast<const uint8_t*>(w2_slots),
+                   lmoe_mx4_bytes(H, I), I, H, 1, n_slots, k, nullptr, nullptr, nullptr, nullptr, nullptr, out, nullptr,
+                   false};
+  const dim3 grid(I / 32, k);
+  const uint16_t* a = static_cast<const uint16_t*>(add);
+  if (x_scale != nullptr) {
+    mx4_one_gateup_kernel<true><<<grid, kOneMxWaves * 64, 0, stream>>>(gu, o);
+    mx4_one_down_kernel<true><<<H / 16, kOneMxWaves * 64, 0, stream>>>(dn, o, w, a);
+  } else {
+    mx4_one_gateup_kernel<false><<<grid, kOneMxWaves * 64, 0, stream>>>(gu, o);
+    mx4_one_down_kernel<false><<<H / 16, kOneMxWaves * 64, 0, stream>>>(dn, o, w, a);
+  }
   LMOE_RETURN_LAUNCH();
 }

@@ -4,12 +4,11 @@
 // Weights are MX4 blocks (mx.h), rows bf16 or MX8.  What bounds it is the
 // weights' bytes: each slot's are read once for up to 32 rows.
 //
-// A workgroup computes 32 output columns (gate-up: 32 gate and 32 up weight
-// rows, four 16-row blocks; down: two) for one slot.  Its eight waves split the
-// row's K between them, so that the reads of a short row are all in flight at
-// once: a wave keeps its chunks' weights (one contiguous KiB per 16 rows and
-// 128 columns) and row fragments in registers, and the waves' partial sums are
-// added in LDS, in wave order.
+// A workgroup computes 64 weight rows, four 16-row blocks, for one slot: 32 act
+// columns (gate and up) or 64 y columns.  Its waves split the row's K between them,
+// so that the reads of a short row are all in flight at once: a wave keeps its chunks'
+// weights (one contiguous KiB per 16 rows and 128 columns) and row fragments in
+// registers, and the waves' partial sums are added in LDS, in wave order.
 //
 // The matrix instruction's first operand is the weights, so a lane's four
 // results are four neighbouring output columns of one row (lane l: row l % 16,
@@ -195,27 +194,67 @@ __device__ __forceinline__ void store_y(const Mx4Args& g, int pair, int n, int l
   }
 }
 
-constexpr int kFewMxWaves = 8;
-constexpr int kFewMxRows = 32;  // rows of one pass over a slot's weights
+// Waves of a workgroup.  Past one token there are workgroups enough, and four waves
+// with twice the work each are ahead of eight (us, gate-up / down, four against
+// eight): 16 tokens over 128 experts of 2048 x 768 16.6 / 10.6 against 16.1 / 11.0,
+// 7 of 7168 x 2048 94.0 / 49.3 against 94.5 / 53.8, 61 over 60 of 2048 x 1408
+// 31.6 / 18.4 against 33.2 / 21.1.  One token has few, and short ones.
+constexpr int kFewMxWaves = 4;
+constexpr int kOneMxWaves = 8;
+constexpr int kFewMxBlocks = 4;  // 16-row weight blocks of a workgroup
+constexpr int kFewMxRows = 32;   // rows of one pass over a slot's weights
 
-// NF 16-row fragments of rows [p0, p0 + rows) of one slot.
-template <bool GU, bool A8, int NF>
-__device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, int cb, int p0, int rows,
+// Chunks [c0, c1) of RB weight blocks by NF row fragments, U chunks' loads at a time.
+// (blocks: how many of the RB there are; the last stands in for the others)
+template <bool A8, int RB, int NF, int U>
+__device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int blocks, int K, int c0, int c1, int lane,
+                                           const char* const (&row)[NF], const uint8_t* const (&row_scale)[NF],
+                                           f32x4_t (&acc)[RB][NF]) {
+  for (int c = c0; c < c1; c += U) {
+    i32x4_t w[U][RB];
+    int sc[U][RB];
+    RowFrag<A8> x[U][NF];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u > 0 && c + u >= c1) break;
+      const uint8_t* quad = wblk + ((c + u) >> 2) * kMxQuadBytes;
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        const uint8_t* p = quad + min(b, blocks - 1) * bb;
+        w[u][b] = __builtin_nontemporal_load(
+            reinterpret_cast<const i32x4_t*>(p + 256 + ((c + u) & 3) * 1024 + lane * 16));
+        sc[u][b] = p[lane * 4 + ((c + u) & 3)];
+      }
+#pragma unroll
+      for (int f = 0; f < NF; ++f) x[u][f] = load_row_frag<A8>(row[f], row_scale[f], c + u, K, lane >> 4);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u > 0 && c + u >= c1) break;
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) acc[b][f] = mx4_step<A8>(w[u][b], sc[u][b], x[u][f], acc[b][f]);
+    }
+  }
+}
+
+// NF 16-row fragments of rows [p0, p0 + rows) of one slot.  ONE: the one token's
+// row p0, whose pairs keep their order.
+template <bool GU, bool A8, int NF, int NW, bool ONE>
+__device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, int blocks, int cb, int p0, int rows,
                                          f32x4_t* s_part) {
-  constexpr int RB = GU ? 4 : 2;
-  constexpr int NW = kFewMxWaves;
+  constexpr int RB = kFewMxBlocks;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lg = lane >> 4;
   const int chunks = mx4_chunks(g.K);
-  const int bb = mx4_block_bytes(g.K);
   const char* row[NF];
   const uint8_t* row_scale[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
     const int r = 16 * f + (lane & 15);
     const int pos = p0 + (r < rows ? r : 0);
-    const size_t src = GU ? g.sorted_pairs[pos] / g.topk : pos;
+    const size_t src = ONE ? 0 : GU ? g.sorted_pairs[pos] / g.topk : pos;
     row[f] = static_cast<const char*>(g.a) + src * g.K * (A8 ? 1 : 2);
     row_scale[f] = A8 ? g.a_scale + src * (g.K / kMxGroup) : nullptr;
   }
@@ -224,66 +263,126 @@ __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, 
   for (int b = 0; b < RB; ++b)
 #pragma unroll
     for (int f = 0; f < NF; ++f) acc[b][f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  const int c1 = (wave + 1) * chunks / NW;
-#pragma unroll 2
-  for (int c = wave * chunks / NW; c < c1; ++c) {
-    i32x4_t w[RB];
-    int sc[RB];
-    const uint8_t* quad = wblk + (c >> 2) * kMxQuadBytes;
+  few_chunks<A8, RB, NF, ONE ? 2 : 1>(wblk, mx4_block_bytes(g.K), blocks, g.K, wave * chunks / NW, (wave + 1) * chunks / NW,
+                            lane, row, row_scale, acc);
+  // partial sums of a fragment, [wave][block][lane], added in wave order
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const uint8_t* p = quad + b * bb;
-      w[b] = __builtin_nontemporal_load(
-          reinterpret_cast<const i32x4_t*>(p + 256 + (c & 3) * 1024 + lane * 16));
-      sc[b] = p[lane * 4 + (c & 3)];
-    }
-    RowFrag<A8> x[NF];
+  for (int f = 0; f < NF; ++f) {
+    if (f > 0) __syncthreads();  // the last fragment's sums have been read
 #pragma unroll
-    for (int f = 0; f < NF; ++f) x[f] = load_row_frag<A8>(row[f], row_scale[f], c, g.K, lg);
+    for (int b = 0; b < RB; ++b) s_part[(wave * RB + b) * 64 + lane] = acc[b][f];
+    __syncthreads();
+    // gate-up: one wave, which has the 32 columns of a scale; down: a wave for 32 columns
+    if (wave >= (GU ? 1 : RB / 2)) continue;
+    constexpr int TB = GU ? RB : 2;
+    const int b0 = GU ? 0 : 2 * wave;
+    f32x4_t t[TB];
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
+    for (int b = 0; b < TB; ++b) {
+      t[b] = s_part[(b0 + b) * 64 + lane];
 #pragma unroll
-      for (int f = 0; f < NF; ++f) acc[b][f] = mx4_step<A8>(w[b], sc[b], x[f], acc[b][f]);
-  }
-  // partial sums, [wave][block][fragment][lane], added in wave order
-#pragma unroll
-  for (int b = 0; b < RB; ++b)
-#pragma unroll
-    for (int f = 0; f < NF; ++f) s_part[((wave * RB + b) * NF + f) * 64 + lane] = acc[b][f];
-  __syncthreads();
-  if (wave < NF) {
-    const int f = wave;
-    f32x4_t t[RB];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      t[b] = s_part[(b * NF + f) * 64 + lane];
-      for (int v = 1; v < NW; ++v) t[b] += s_part[((v * RB + b) * NF + f) * 64 + lane];
+      for (int v = 1; v < NW; ++v) t[b] += s_part[(v * RB + b0 + b) * 64 + lane];
     }
     const int r = 16 * f + (lane & 15);
     const bool live = r < rows;
     if constexpr (GU) {
       const f32x4_t gate[2] = {t[0], t[2]}, up[2] = {t[1], t[3]};
       store_act<A8>(g, p0 + r, cb * 32, lane, live, gate, up);
-    } else {
-      store_y(g, live ? g.sorted_pairs[p0 + r] : 0, cb * 32, lane, live, t[0], t[1]);
+    } else if (b0 < blocks) {
+      store_y(g, live ? g.sorted_pairs[p0 + r] : 0, cb * 64 + 32 * wave, lane, live, t[0], t[1]);
     }
   }
 }
 
+// (column block, active slot) of a grid of [ceil(N / 32 or 64), slots]
 template <bool GU, bool A8>
 __global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g) {
-  constexpr int RB = GU ? 4 : 2;
-  __shared__ f32x4_t s_part[kFewMxWaves * RB * (kFewMxRows / 16) * 64];
+  __shared__ f32x4_t s_part[kFewMxWaves * kFewMxBlocks * 64];
   const int slot = g.active[blockIdx.y];
   if (slot < 0) return;
   const int p0 = g.offsets[slot], p1 = g.offsets[slot + 1];
   const int cb = blockIdx.x;
-  const uint8_t* wblk = g.w + slot * g.w_slot_bytes + static_cast<size_t>(cb) * RB * mx4_block_bytes(g.K);
+  const int blocks = min(kFewMxBlocks, (GU ? 2 * g.N : g.N) / 16 - cb * kFewMxBlocks);
+  const uint8_t* wblk = g.w + slot * g.w_slot_bytes + static_cast<size_t>(cb) * kFewMxBlocks * mx4_block_bytes(g.K);
   for (int p = p0; p < p1; p += kFewMxRows) {
     const int rows = min(kFewMxRows, p1 - p);
     if (p > p0) __syncthreads();  // the last pass's sums have been read
-    if (rows > 16) few_rows<GU, A8, 2>(g, wblk, cb, p, rows, s_part);
-    else few_rows<GU, A8, 1>(g, wblk, cb, p, rows, s_part);
+    if (rows > 16) few_rows<GU, A8, 2, kFewMxWaves, false>(g, wblk, blocks, cb, p, rows, s_part);
+    else few_rows<GU, A8, 1, kFewMxWaves, false>(g, wblk, blocks, cb, p, rows, s_part);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// One token: no permutation.  Pair j's expert is looked up where it is needed, its
+// act row is row j, and the down product ends in the weighted combine: two launches.
+// ---------------------------------------------------------------------------
+struct OneToken {
+  const int32_t* ids;
+  const int32_t* log2phy;  // or null
+  int n_log2phy;
+};
+__device__ __forceinline__ int slot_of_pair(const OneToken& o, int P, int j) {  // -1: none
+  int s = o.ids[j];
+  if (o.log2phy != nullptr) s = s >= 0 && s < o.n_log2phy ? o.log2phy[s] : -1;
+  return s >= 0 && s < P ? s : -1;
+}
+
+template <bool A8>
+__global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_gateup_kernel(Mx4Args g, OneToken o) {
+  __shared__ f32x4_t s_part[kOneMxWaves * kFewMxBlocks * 64];
+  const int j = blockIdx.y;
+  const int slot = __builtin_amdgcn_readfirstlane(slot_of_pair(o, g.P, j));
+  if (slot < 0) return;
+  const int cb = blockIdx.x;
+  const uint8_t* wblk = g.w + slot * g.w_slot_bytes + static_cast<size_t>(cb) * 4 * mx4_block_bytes(g.K);
+  few_rows<true, A8, 1, kOneMxWaves, true>(g, wblk, kFewMxBlocks, cb, j, 1, s_part);
+}
+
+// 16 columns of out = add + sum_j w_j W2_j act_j.  The waves take (pair, part of K)
+// units in turn, each adding its units' weighted sums; the waves' sums are added in
+// order.  A unit is the whole K of a pair where there are eight pairs or more.
+template <bool A8>
+__global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_down_kernel(Mx4Args g, OneToken o,
+                                                                       const uint16_t* __restrict__ wts,
+                                                                       const uint16_t* __restrict__ add) {
+  constexpr int NW = kOneMxWaves;
+  __shared__ f32x4_t s_part[NW * 4];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int k = g.n_pairs;
+  const int chunks = mx4_chunks(g.K);
+  const int bb = mx4_block_bytes(g.K);
+  const int parts = min((NW + k - 1) / k, chunks);
+  f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int u = wave; u < k * parts; u += NW) {
+    const int j = u / parts, part = u - j * parts;
+    const int slot = __builtin_amdgcn_readfirstlane(slot_of_pair(o, g.P, j));
+    if (slot < 0) {  // counted once
+      if (blockIdx.x == 0 && part == 0 && lane == 0) add_device_flag(LMOE_FLAG_UNPLACED, 1);
+      continue;
+    }
+    const float wj = bf16_to_f32(wts[j]);
+    const char* row[1] = {static_cast<const char*>(g.a) + static_cast<size_t>(j) * g.K * (A8 ? 1 : 2)};
+    const uint8_t* row_scale[1] = {A8 ? g.a_scale + static_cast<size_t>(j) * (g.K / kMxGroup) : nullptr};
+    f32x4_t acc[1][1] = {{f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}}};
+    const uint8_t* wblk = g.w + slot * g.w_slot_bytes + static_cast<size_t>(blockIdx.x) * bb;
+    few_chunks<A8, 1, 1, 4>(wblk, bb, 1, g.K, part * chunks / parts, (part + 1) * chunks / parts, lane, row, row_scale,
+                            acc);
+    sum += wj * acc[0][0];
+  }
+  // the sixteen rows of the fragment are the same row: lanes 0, 16, 32 and 48 have it
+  if ((lane & 15) == 0) s_part[wave * 4 + (lane >> 4)] = sum;
+  __syncthreads();
+  if (threadIdx.x < 4) {
+    const int h = blockIdx.x * 16 + threadIdx.x * 4;
+    f32x4_t t = s_part[threadIdx.x];
+    for (int v = 1; v < NW; ++v) t += s_part[v * 4 + threadIdx.x];
+    if (add != nullptr) {
+      const uint2 a = *reinterpret_cast<const uint2*>(add + h);
+      t += f32x4_t{bf16lo(a.x), bf16hi(a.x), bf16lo(a.y), bf16hi(a.y)};
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(g.out) + h) =
+        make_uint2(pack_bf16x2(t[0], t[1]), pack_bf16x2(t[2], t[3]));
   }
 }
 

@@ -52,6 +52,7 @@ class MoEWorkspace:
     y: torch.Tensor     # [N, H] bf16 (or f32), flat pair order
     out: torch.Tensor   # [T, H] bf16
     perm_overflow: native.Permutation | None = None  # the decode overflow pass's permutation
+    mx4: native.Mx4Buffers | None = None  # the buffers as the calls over 4-bit banks take them
 
     def overflow_perm(self, n_pairs: int, n_slots: int, device) -> native.Permutation:
         p = self.perm_overflow
@@ -66,9 +67,12 @@ _WORKSPACES: dict[tuple, MoEWorkspace] = {}
 def rows_kind(hidden, w13_slots) -> str:
     """What a layer's workspace holds: "" for bf16 experts; for 4-bit experts
     the kind of the rows, "bf16" or "mx8" (hidden is native.Mx8Rows)."""
+    mx8 = isinstance(hidden, native.Mx8Rows)
     if not mxfp4.is_mx4(w13_slots):
+        if mx8:
+            raise ValueError("8-bit rows go through 4-bit experts only (bf16 slot bank)")
         return ""
-    return "mx8" if isinstance(hidden, native.Mx8Rows) else "bf16"
+    return "mx8" if mx8 else "bf16"
 
 
 def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = "", rows: str = "") -> MoEWorkspace:
@@ -89,6 +93,8 @@ def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = 
             y=torch.empty((max(N, 1), H), dtype=y_dtype, device=device),
             out=torch.empty((max(T, 1), H), dtype=torch.bfloat16, device=device),
         )
+        if rows:
+            ws.mx4 = native.Mx4Buffers(ws.perm, ws.act, ws.y)
         _WORKSPACES[key] = ws
     return ws
 
@@ -170,9 +176,34 @@ def fused_experts(
     combine); otherwise the grouped GEMM (path, or native.layer_path's when
     it is AUTO) and the combine.  topk_ids come from the caller, so a token
     may name one expert twice: the decode body takes its general form,
-    which holds no one-pair-per-slot assumption."""
+    which holds no one-pair-per-slot assumption.
+
+    Over 4-bit banks (uint8, mxfp4.pack_experts) hidden is bf16 or
+    native.Mx8Rows; one token goes straight from its ids, without a permutation
+    in the workspace."""
+    if w13_slots.dtype is torch.uint8:
+        return _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, add, out, path, workspace)
     return _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, add=add, out=out,
                              path=path, workspace=workspace)[0]
+
+
+def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, add, out, path, ws):
+    """fused_experts over 4-bit banks."""
+    T, H = hidden.shape
+    k = topk_ids.shape[1]
+    P = w13_slots.shape[0]
+    if ws is None:
+        ws = get_workspace(T, k, P, H, w13_slots.shape[1] // 2, hidden.device, rows=rows_kind(hidden, w13_slots))
+    if ws.mx4 is None:
+        raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
+    dst = ws.out[:T] if out is None else out
+    if path == native.LMOE_PATH_AUTO:
+        path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel())
+        if T == 1 and path == native.LMOE_PATH_GEMV:
+            return native.mx4_decode_one(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst,
+                                         add=add)
+    return native.mx4_fused_moe(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
+                                path=path, block_m=native.mx4_block_m(T * k, P))
 
 
 def _layer_path(hidden, k: int, n_experts: int, *w13) -> int:
@@ -279,8 +310,9 @@ def _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2p
     k = int(topk_ids.shape[1])
     P = int(w13_slots.shape[0])
     I = int(w13_slots.shape[1]) // 2
-    mx4 = mxfp4.is_mx4(w13_slots)
-    ws = workspace or get_workspace(T, k, P, H, I, hidden.device, rows=rows_kind(hidden, w13_slots))
+    rows = rows_kind(hidden, w13_slots)
+    mx4 = rows != ""
+    ws = workspace or get_workspace(T, k, P, H, I, hidden.device, rows=rows)
     dst = out if out is not None else ws.out[:T]
     if path == native.LMOE_PATH_AUTO:
         path = _bank_layer_path(hidden, k, w13_slots, log2phy, overflow)
@@ -289,6 +321,14 @@ def _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2p
     bm = _block_m(hidden, k, w13_slots, path)
     merged = overflow is not None and log2phy is not None and not events and \
         _merged_passes(hidden, k, w13_slots, overflow, path)
+    if mx4 and overflow is None and not events:
+        if T == 1 and path == native.LMOE_PATH_GEMV:  # the permutation for its counts alone
+            native.permute(topk_ids, ws.perm, log2phy=log2phy, block_m=bm)
+            native.mx4_decode_one(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add)
+        else:
+            native.mx4_fused_moe(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
+                                 path=path, block_m=bm)
+        return dst, ws
     if events:
         events[0].record()
     perm_b = None
@@ -351,6 +391,7 @@ def decode_layer(
     w_out: torch.Tensor | None = None,
     ids_out: torch.Tensor | None = None,
     overflow: PreparedSlotWeights | None = None,
+    expert_rows: native.Mx8Rows | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """route() followed by fused_experts(), for a slot table that is final
     before the router runs (the decode replay after staging): gate, expert
@@ -362,8 +403,14 @@ def decode_layer(
     (out, topk_weights, topk_ids), equal bit for bit to the separate calls.
     overflow: the layer's second pass (stage buffer + overflow table) for a
     working set past the bank; both passes and the combine are fixed-shape
-    launches, so a graph captured with them replays any split."""
+    launches, so a graph captured with them replays any split.
+    expert_rows: the same hidden states in 8 bits (native.add_rms_norm gives
+    both), for the experts of a 4-bit bank; the gate reads hidden."""
     T = hidden.shape[0]
+    rows = hidden if expert_rows is None else expert_rows
+    if expert_rows is not None and tuple(expert_rows.shape) != tuple(hidden.shape):
+        raise ValueError(f"expert_rows {tuple(expert_rows.shape)} are not hidden's {tuple(hidden.shape)}")
+    mx4 = rows_kind(rows, w13_slots) != ""
     k = int(spec.top_k)
     kw = k + int(spec.n_shared)  # pairs per token, shared suffix included
     P = int(w13_slots.shape[0])
@@ -385,8 +432,11 @@ def decode_layer(
     bm = _block_m(hidden, kw, w13_slots, path)
     merged = overflow is not None and log2phy is not None and _merged_passes(hidden, kw, w13_slots, overflow, path)
     perm_b = None
-    fused_body = overflow is None and path == native.LMOE_PATH_GEMV and not mxfp4.is_mx4(w13_slots)
-    if T == 1 and fused_body:
+    fused_body = overflow is None and path == native.LMOE_PATH_GEMV and not mx4
+    mx4_one = T == 1 and overflow is None and path == native.LMOE_PATH_GEMV and mx4
+    if mx4_one and ws.mx4 is None:
+        raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
+    if T == 1 and (fused_body or mx4_one):
         # the one-token body reads the pairs in pair order: no sort at the
         # end of the router's chain (the same bits as the sorted form)
         w, ids, _ = native.router_gate_topk_pairs(hidden, gate_weight, logits_out, k, ws.perm, **sel)
@@ -401,20 +451,23 @@ def decode_layer(
             sel["second"] = (perm_b, overflow.log2phy)
         w, ids, _ = native.router_topk_permute(logits, k, ws.perm, block_m=bm, **sel)
     dst = out if out is not None else ws.out[:T]
+    if mx4_one:
+        native.mx4_decode_one(rows, w, ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add)
+        return dst, w, ids
     if overflow is not None:
         if merged:
-            _two_passes(hidden, kw, w13_slots, w2_slots, overflow, ws, perm_b, path=path)
+            _two_passes(rows, kw, w13_slots, w2_slots, overflow, ws, perm_b, path=path)
         else:
-            native.grouped_mlp(hidden, kw, w13_slots, w2_slots, ws.perm, ws.act[: T * kw], ws.y[: T * kw], path=path)
-            _overflow_pass(hidden, ids, kw, overflow, ws, path=path)
+            native.grouped_mlp(rows, kw, w13_slots, w2_slots, ws.perm, ws.act[: T * kw], ws.y[: T * kw], path=path)
+            _overflow_pass(rows, ids, kw, overflow, ws, path=path)
         native.combine(ws.y[: T * kw], w, dst, row_mask=ws.perm.row_idx[: T * kw], add=add)
         return dst, w, ids
     if fused_body:
         # router-fed ids: distinct experts per token, in distinct slots
-        native.fused_moe_decode(hidden, w, w13_slots, w2_slots, ws.perm, ws.act[: T * kw], dst, add=add,
+        native.fused_moe_decode(rows, w, w13_slots, w2_slots, ws.perm, ws.act[: T * kw], dst, add=add,
                                 y=ws.y[: T * kw], distinct_slots=True)
     else:
-        native.grouped_mlp(hidden, kw, w13_slots, w2_slots, ws.perm, ws.act[: T * kw], ws.y[: T * kw], path=path)
+        native.grouped_mlp(rows, kw, w13_slots, w2_slots, ws.perm, ws.act[: T * kw], ws.y[: T * kw], path=path)
         native.combine(ws.y[: T * kw], w, dst, row_mask=ws.perm.row_idx[: T * kw], add=add)
     return dst, w, ids
 

@@ -70,6 +70,8 @@ EXPORTED_SYMBOLS = (
     "lmoe_mx4_bytes",
     "lmoe_mx4_gateup_silu",
     "lmoe_mx4_down",
+    "lmoe_mx4_fused_moe",
+    "lmoe_mx4_decode_one",
     "lmoe_fused_moe_decode",
     "lmoe_fused_moe_decode_noalloc",
     "lmoe_down_combine",
@@ -157,6 +159,14 @@ _SIGNATURES = {
     "lmoe_mx4_down": (
         _i,
         [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _vp],
+    ),
+    "lmoe_mx4_fused_moe": (
+        _i,
+        [_vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp],
+    ),
+    "lmoe_mx4_decode_one": (
+        _i,
+        [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp],
     ),
     "lmoe_fused_moe_decode": (
         _i,
@@ -272,7 +282,14 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else int(t.data_ptr())
 
 
+# The current stream's handle without a Stream object around it, where torch has
+# the call (a few microseconds less of host time in every wrapper).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(stream: torch.cuda.Stream | None) -> int:
+    if stream is None and _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     s = stream if stream is not None else torch.cuda.current_stream()
     return int(s.cuda_stream)
 
@@ -332,9 +349,18 @@ class Mx8Rows:
         return (self.q.float().unflatten(-1, (-1, mxfp4.GROUP)) * s.unsqueeze(-1)).flatten(-2)
 
 
+def _is(t, dtype: torch.dtype, shape: tuple) -> bool:
+    """What _need checks, without its words: for calls whose host time counts.
+    (_need then says what is wrong.)"""
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.shape == shape and t.is_contiguous()
+
+
 def _need_mx8(rows, name: str, shape: tuple | None = None) -> None:
     if not isinstance(rows, Mx8Rows):
         raise TypeError(f"{name} must be Mx8Rows")
+    if shape is not None and _is(rows.q, torch.float8_e4m3fn, shape) and shape[1] % mxfp4.GROUP == 0 and \
+            _is(rows.scale, torch.uint8, (shape[0], shape[1] // mxfp4.GROUP)):
+        return
     _need(rows.q, f"{name}.q", torch.float8_e4m3fn, shape)
     if rows.q.dim() != 2 or rows.q.shape[1] % mxfp4.GROUP:
         raise ValueError(f"{name} must be [R, K], K a multiple of {mxfp4.GROUP}, got {tuple(rows.q.shape)}")
@@ -345,7 +371,7 @@ def _same_device(*tensors) -> None:
     """Every operand on the current device: a launch goes to its stream."""
     here = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.device.index != here:
+        if t is not None and t.get_device() != here:
             raise ValueError(f"operand on {t.device}, the current device is cuda:{here}")
 
 
@@ -370,35 +396,41 @@ def add_rms_norm(
     multiple of 8 (of 32 with mx8) up to 32768.  Returns (out, mx8,
     residual_out), None for what was not asked for."""
     lib = load_library()
-    _need(x, "x", torch.bfloat16)
-    if x.dim() != 2:
-        raise ValueError(f"x must be [T, H], got {tuple(x.shape)}")
-    T, H = x.shape
-    if weight.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError("weight must be bf16 or f32")
-    _need(weight, "weight", weight.dtype, (H,))
+    bf16, f32 = torch.bfloat16, torch.float32
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a [T, H] tensor")
+    shape = T, H = x.shape
+    if not _is(x, bf16, shape):
+        _need(x, "x", bf16)
+    wdt = f32 if weight.dtype is f32 else bf16
+    if not _is(weight, wdt, (H,)):
+        _need(weight, "weight", wdt, (H,))
+    rdt = bf16
     if residual is not None:
-        if residual.dtype not in (torch.bfloat16, torch.float32):
-            raise ValueError("residual must be bf16 or f32")
-        _need(residual, "residual", residual.dtype, (T, H))
-        residual_out = residual if residual_out is None else residual_out
-        _need(residual_out, "residual_out", residual.dtype, (T, H))
+        rdt = f32 if residual.dtype is f32 else bf16
+        if not _is(residual, rdt, shape):
+            _need(residual, "residual", rdt, shape)
+        if residual_out is None:
+            residual_out = residual
+        elif not _is(residual_out, rdt, shape):
+            _need(residual_out, "residual_out", rdt, shape)
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
     if out is None and mx8 is None:
         out = torch.empty_like(x)
-    if out is not None:
-        _need(out, "out", torch.bfloat16, (T, H))
+    elif out is not None and not _is(out, bf16, shape):
+        _need(out, "out", bf16, shape)
+    q = scale = None
     if mx8 is not None:
-        _need_mx8(mx8, "mx8", (T, H))
-    _same_device(x, weight, residual, residual_out, out, *((mx8.q, mx8.scale) if mx8 is not None else ()))
+        _need_mx8(mx8, "mx8", shape)
+        q, scale = mx8.q, mx8.scale
+    _same_device(x, weight, residual, residual_out, out, q, scale)
     _check(
         lib.lmoe_add_rms_norm(
-            _ptr(x), T, H, _ptr(residual), int(residual is not None and residual.dtype == torch.float32),
-            _ptr(weight), int(weight.dtype == torch.float32), float(eps), _ptr(residual_out), _ptr(out),
-            _ptr(mx8.q) if mx8 is not None else None, _ptr(mx8.scale) if mx8 is not None else None, _stream(stream),
+            x.data_ptr(), T, H, _ptr(residual), rdt is f32, weight.data_ptr(), wdt is f32, eps, _ptr(residual_out),
+            _ptr(out), _ptr(q), _ptr(scale), _stream(stream),
         ),
         "lmoe_add_rms_norm",
     )
@@ -1218,6 +1250,111 @@ def _mx4_down(act, w2_slots: torch.Tensor, perm: Permutation, y: torch.Tensor, *
         "lmoe_mx4_down",
     )
     return y
+
+
+class _Mx4Workspace(ctypes.Structure):
+    """lmoe_mx4_workspace."""
+
+    _fields_ = [(n, _vp) for n in ("counts", "offsets", "sorted_pairs", "row_idx", "active", "tile_off", "meta",
+                                   "permute_workspace")] + \
+               [("permute_workspace_bytes", _sz), ("act", _vp), ("act_scale", _vp), ("y", _vp), ("y_f32", ctypes.c_int32)]
+
+
+class Mx4Buffers:
+    """The buffers of a layer of 4-bit experts (lmoe_mx4_workspace): a permutation,
+    act (bf16 or Mx8Rows, [N, I]) and y (bf16 or f32, [N, H]), checked once."""
+
+    def __init__(self, perm: Permutation, act, y: torch.Tensor) -> None:
+        aq, as_ = _need_rows(act, "act")
+        if y.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("y must be bf16 or f32")
+        _need(y, "y", y.dtype)
+        if aq.shape[0] < perm.n_pairs or y.shape[0] < perm.n_pairs:
+            raise ValueError("act and y need a row for every pair")
+        self.perm, self.act, self.y = perm, act, y
+        self.device_index = y.get_device()
+        self.hidden, self.intermediate = int(y.shape[1]), int(aq.shape[1])
+        self.mx8 = as_ is not None
+        self.act_ptr, self.act_scale_ptr = _ptr(aq), _ptr(as_)
+        p = perm
+        self._struct = _Mx4Workspace(
+            _ptr(p.counts), _ptr(p.offsets), _ptr(p.sorted_pairs), _ptr(p.row_idx), _ptr(p.active), _ptr(p.tile_off),
+            _ptr(p.meta), _ptr(p.workspace), int(p.workspace.numel()), _ptr(aq), _ptr(as_), _ptr(y),
+            int(y.dtype == torch.float32))
+        self.address = ctypes.addressof(self._struct)
+
+
+def _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, bufs: Mx4Buffers, out, add):
+    """Check a layer call over 4-bit banks; (x values, scales, T, k, table length)."""
+    mx8 = isinstance(x, Mx8Rows)
+    xq, xs = (x.q, x.scale) if mx8 else (x, None)
+    H, I, P = bufs.hidden, bufs.intermediate, bufs.perm.n_slots
+    T, k = topk_ids.shape
+    if mx8:
+        _need_mx8(x, "x", (T, H))
+    elif not _is(x, torch.bfloat16, (T, H)):
+        _need(x, "x", torch.bfloat16, (T, H))
+    if mx8 != bufs.mx8:
+        raise ValueError("x and act must both be bf16 or both be Mx8Rows")
+    if T * k != bufs.perm.n_pairs:
+        raise ValueError(f"buffers for {bufs.perm.n_pairs} pairs, got {T * k}")
+    for t, name, dtype, shape in (
+            (topk_weights, "topk_weights", torch.bfloat16, (T, k)), (topk_ids, "topk_ids", torch.int32, (T, k)),
+            (w13_slots, "w13_slots", torch.uint8, (P, 2 * I, mxfp4.row_bytes(H))),
+            (w2_slots, "w2_slots", torch.uint8, (P, H, mxfp4.row_bytes(I))), (out, "out", torch.bfloat16, (T, H))):
+        if not _is(t, dtype, shape):
+            _need(t, name, dtype, shape)
+    if add is not None and not _is(add, torch.bfloat16, (T, H)):
+        _need(add, "add", torch.bfloat16, (T, H))
+    n_table = 0
+    if log2phy is not None:
+        n_table = log2phy.numel()
+        if not _is(log2phy, torch.int32, (n_table,)):
+            _need(log2phy, "log2phy", torch.int32)
+    here = torch.cuda.current_device()
+    if bufs.device_index != here:
+        raise ValueError(f"buffers on cuda:{bufs.device_index}, the current device is cuda:{here}")
+    _same_device(xq, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, out, add)
+    return xq, xs, T, k, n_table
+
+
+def mx4_fused_moe(x, topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_slots: torch.Tensor,
+                  w2_slots: torch.Tensor, log2phy: torch.Tensor | None, bufs: Mx4Buffers, out: torch.Tensor, *,
+                  add: torch.Tensor | None = None, path: int = LMOE_PATH_AUTO, block_m: int, stream=None) -> torch.Tensor:
+    """permute, gateup_silu, down and combine over 4-bit banks, in one call."""
+    lib = load_library()
+    xq, xs, T, k, n_table = _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, bufs, out, add)
+    _check(
+        lib.lmoe_mx4_fused_moe(
+            xq.data_ptr(), _ptr(xs), T, bufs.hidden, bufs.intermediate, k, w13_slots.data_ptr(), w2_slots.data_ptr(),
+            bufs.perm.n_slots, topk_weights.data_ptr(), topk_ids.data_ptr(), _ptr(log2phy), n_table, path, block_m,
+            bufs.address, _ptr(add), out.data_ptr(), _stream(stream),
+        ),
+        "lmoe_mx4_fused_moe",
+    )
+    bufs.perm.block_m = block_m
+    bufs.perm.builds += 1
+    return out
+
+
+def mx4_decode_one(x, topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_slots: torch.Tensor,
+                   w2_slots: torch.Tensor, log2phy: torch.Tensor | None, bufs: Mx4Buffers, out: torch.Tensor, *,
+                   add: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """One token over 4-bit banks, straight from its ids (no permutation is built:
+    bufs.perm is left as it was)."""
+    lib = load_library()
+    xq, xs, T, k, n_table = _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, bufs, out, add)
+    if T != 1:
+        raise ValueError(f"one token, got {T}")
+    _check(
+        lib.lmoe_mx4_decode_one(
+            xq.data_ptr(), _ptr(xs), bufs.hidden, bufs.intermediate, k, w13_slots.data_ptr(), w2_slots.data_ptr(),
+            bufs.perm.n_slots, topk_weights.data_ptr(), topk_ids.data_ptr(), _ptr(log2phy), n_table, _ptr(add),
+            bufs.act_ptr, bufs.act_scale_ptr, out.data_ptr(), _stream(stream),
+        ),
+        "lmoe_mx4_decode_one",
+    )
+    return out
 
 
 def decode_mlp_two_passes(
