@@ -503,12 +503,17 @@ int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int H, int I,
  * the same bits; rows of pairs without a slot untouched), then out = add +
  * sum_j w[j] W2 act[j], summed in f32.  A pair whose id maps to no slot adds
  * nothing and is counted in LMOE_FLAG_UNPLACED.  One slot may serve several
- * pairs.  Shapes and alignment as lmoe_mx4_gateup_silu and lmoe_combine_f32. */
+ * pairs.  w13_b, w2_b, log2phy_b (all null: none) are a second bank of n_slots_b
+ * slots and its table, for experts that the first table leaves out (the decode
+ * overflow buffer); log2phy must then be given.  Shapes and alignment as
+ * lmoe_mx4_gateup_silu and lmoe_combine_f32. */
 int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, int I, int k,
                         const void* w13_slots, const void* w2_slots,
                         int n_slots, const uint16_t* w, const int32_t* ids,
-                        const int32_t* log2phy, int n_log2phy, const void* add,
-                        void* act, void* act_scale, void* out,
+                        const int32_t* log2phy, int n_log2phy,
+                        const void* w13_b, const void* w2_b, int n_slots_b,
+                        const int32_t* log2phy_b, int n_log2phy_b,
+                        const void* add, void* act, void* act_scale, void* out,
                         hipStream_t stream);
 
 /* The second half of lmoe_fused_moe_decode on its own: down GEMV from act

@@ -171,8 +171,10 @@ def test_c_entries_check_their_arguments():
     assert fused(H=48) == 1001 and fused(I=40) == 1001 and fused(P=70000) == 1001 and fused(T=1 << 30, k=4) == 1001
     assert fused(x=P16 + 8) == 1001 and fused(add=P16 + 8) == 1001 and fused(out=P16 + 8) == 1001
     assert fused(path=2, bm=256) == 1001 and fused(path=2, bm=128, H=32 * 4096) == 1001 and fused(path=3) == 1003
-    one = lambda x=P16, xs=P16, H=64, I=32, k=2, w13=P16, w2=P16, P=4, w=P16, ids=P16, n=0, add=N, act=P16, as_=P16, out=P16: \
-        lib.lmoe_mx4_decode_one(x, xs, H, I, k, w13, w2, P, w, ids, N, n, add, act, as_, out, N)
+    one = lambda x=P16, xs=P16, H=64, I=32, k=2, w13=P16, w2=P16, P=4, w=P16, ids=P16, n=0, add=N, act=P16, as_=P16, out=P16, tab=N, b13=N, b2=N, pb=0, tb=N, nb=0: \
+        lib.lmoe_mx4_decode_one(x, xs, H, I, k, w13, w2, P, w, ids, tab, n, b13, b2, pb, tb, nb, add, act, as_, out, N)
+    assert one(b13=P16, tb=P16, tab=P16) == 1000 and one(b13=P16, b2=P16, tb=P16) == 1000
+    assert one(b13=P16, b2=P16, tb=P16, tab=P16, pb=-1) == 1000 and one(b13=P16 + 8, b2=P16, tb=P16, tab=P16) == 1001
     assert one(x=N) == 1000 and one(xs=N) == 1000 and one(as_=N) == 1000 and one(w=N) == 1000 and one(ids=N) == 1000
     assert one(act=N) == 1000 and one(out=N) == 1000 and one(k=0) == 1000 and one(n=-1) == 1000 and one(w2=N) == 1000
     assert one(H=40) == 1001 and one(I=40) == 1001 and one(k=70000) == 1001 and one(add=P16 + 2) == 1001

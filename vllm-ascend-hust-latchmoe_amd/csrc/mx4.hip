@@ -106,8 +106,8 @@ static int launch_tiles(const Mx4Args& g, int block_m, hipStream_t stream) {
   return launch_tiles<GU, A8, 128>(g, stream);
 }
 
-// path AUTO: row tiles past this many pairs per slot, on average
-constexpr int kFewPairsPerSlot = 16;
+// path AUTO: row tiles past this many pairs per slot, on average (native.py has the figures)
+constexpr int kFewPairsPerSlot = 3;
 
 static bool takes_tiles(int path, int block_m, bool a8, int H, int I, int n_pairs, int P) {
   if (path != LMOE_PATH_AUTO) return path == LMOE_PATH_MFMA;
@@ -231,15 +231,23 @@ extern "C" int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int
 
 extern "C" int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, int I, int k, const void* w13_slots,
                                    const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids,
-                                   const int32_t* log2phy, int n_log2phy, const void* add, void* act,
-                                   void* act_scale, void* out, hipStream_t stream) {
+                                   const int32_t* log2phy, int n_log2phy, const void* w13_b,
+                                   const void* w2_b, int n_slots_b, const int32_t* log2phy_b, int n_log2phy_b,
+                                   const void* add, void* act, void* act_scale, void* out, hipStream_t stream) {
   if (H <= 0 || I <= 0 || k <= 0 || n_slots <= 0 || n_log2phy < 0) return LMOE_ERR_ARG;
+  const bool two = w13_b != nullptr;
+  if (two != (w2_b != nullptr) || two != (log2phy_b != nullptr) || n_slots_b < 0 || n_log2phy_b < 0) return LMOE_ERR_ARG;
+  if (two && log2phy == nullptr) return LMOE_ERR_ARG;
   if (H % kMxGroup != 0 || I % kMxGroup != 0 || k > kMaxSlots) return LMOE_ERR_SHAPE;
   if (x == nullptr || w13_slots == nullptr || w2_slots == nullptr || w == nullptr || ids == nullptr ||
       act == nullptr || out == nullptr || (x_scale == nullptr) != (act_scale == nullptr))
     return LMOE_ERR_ARG;
-  if (bad16(x) || bad16(w13_slots) || bad16(w2_slots) || bad16(act) || bad16(add) || bad16(out)) return LMOE_ERR_SHAPE;
-  const OneToken o{ids, log2phy, n_log2phy};
+  if (bad16(x) || bad16(w13_slots) || bad16(w2_slots) || bad16(act) || bad16(add) || bad16(out) ||
+      bad16(w13_b) || bad16(w2_b))
+    return LMOE_ERR_SHAPE;
+  const OneToken gate_up{ids, log2phy, n_log2phy, static_cast<const uint8_t*>(w13_b), log2phy_b, n_log2phy_b, n_slots_b};
+  OneToken down = gate_up;
+  down.w_b = static_cast<const uint8_t*>(w2_b);
   const Mx4Args gu{x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(w13_slots),
                    lmoe_mx4_bytes(2 * I, H), H, I, k, n_slots, k, nullptr, nullptr, nullptr, nullptr, nullptr, act,
                    static_cast<uint8_t*>(act_scale), false};
@@ -249,11 +257,11 @@ extern "C" int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, in
   const dim3 grid(I / 32, k);
   const uint16_t* a = static_cast<const uint16_t*>(add);
   if (x_scale != nullptr) {
-    mx4_one_gateup_kernel<true><<<grid, kOneMxWaves * 64, 0, stream>>>(gu, o);
-    mx4_one_down_kernel<true><<<H / 16, kOneMxWaves * 64, 0, stream>>>(dn, o, w, a);
+    mx4_one_gateup_kernel<true><<<grid, kOneMxWaves * 64, 0, stream>>>(gu, gate_up);
+    mx4_one_down_kernel<true><<<H / 16, kOneMxWaves * 64, 0, stream>>>(dn, down, w, a);
   } else {
-    mx4_one_gateup_kernel<false><<<grid, kOneMxWaves * 64, 0, stream>>>(gu, o);
-    mx4_one_down_kernel<false><<<H / 16, kOneMxWaves * 64, 0, stream>>>(dn, o, w, a);
+    mx4_one_gateup_kernel<false><<<grid, kOneMxWaves * 64, 0, stream>>>(gu, gate_up);
+    mx4_one_down_kernel<false><<<H / 16, kOneMxWaves * 64, 0, stream>>>(dn, down, w, a);
   }
   LMOE_RETURN_LAUNCH();
 }

@@ -316,25 +316,41 @@ __global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g) {
 // One token: no permutation.  Pair j's expert is looked up where it is needed, its
 // act row is row j, and the down product ends in the weighted combine: two launches.
 // ---------------------------------------------------------------------------
+// A pair whose expert the bank's table leaves out may have it in a second bank (the
+// decode overflow buffer).
 struct OneToken {
   const int32_t* ids;
-  const int32_t* log2phy;  // or null
+  const int32_t* log2phy;  // or null: ids are slots
   int n_log2phy;
+  const uint8_t* w_b;      // the second bank, or null
+  const int32_t* log2phy_b;
+  int n_log2phy_b, P_b;
 };
-__device__ __forceinline__ int slot_of_pair(const OneToken& o, int P, int j) {  // -1: none
-  int s = o.ids[j];
-  if (o.log2phy != nullptr) s = s >= 0 && s < o.n_log2phy ? o.log2phy[s] : -1;
-  return s >= 0 && s < P ? s : -1;
+__device__ __forceinline__ const uint8_t* expert_of_pair(const Mx4Args& g, const OneToken& o, int j) {  // or null
+  const int e = o.ids[j];
+  int s = e;
+  if (o.log2phy != nullptr) s = e >= 0 && e < o.n_log2phy ? o.log2phy[e] : -1;
+  if (s >= 0 && s < g.P) return g.w + s * g.w_slot_bytes;
+  if (o.w_b == nullptr) return nullptr;
+  s = e >= 0 && e < o.n_log2phy_b ? o.log2phy_b[e] : -1;
+  return s >= 0 && s < o.P_b ? o.w_b + s * g.w_slot_bytes : nullptr;
+}
+// the same, known to be the same in every lane
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 template <bool A8>
 __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_gateup_kernel(Mx4Args g, OneToken o) {
   __shared__ f32x4_t s_part[kOneMxWaves * kFewMxBlocks * 64];
   const int j = blockIdx.y;
-  const int slot = __builtin_amdgcn_readfirstlane(slot_of_pair(o, g.P, j));
-  if (slot < 0) return;
+  const uint8_t* expert = uniform(expert_of_pair(g, o, j));
+  if (expert == nullptr) return;
   const int cb = blockIdx.x;
-  const uint8_t* wblk = g.w + slot * g.w_slot_bytes + static_cast<size_t>(cb) * 4 * mx4_block_bytes(g.K);
+  const uint8_t* wblk = expert + static_cast<size_t>(cb) * kFewMxBlocks * mx4_block_bytes(g.K);
   few_rows<true, A8, 1, kOneMxWaves, true>(g, wblk, kFewMxBlocks, cb, j, 1, s_part);
 }
 
@@ -356,8 +372,8 @@ __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_down_kernel(Mx4Args 
   f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int u = wave; u < k * parts; u += NW) {
     const int j = u / parts, part = u - j * parts;
-    const int slot = __builtin_amdgcn_readfirstlane(slot_of_pair(o, g.P, j));
-    if (slot < 0) {  // counted once
+    const uint8_t* expert = uniform(expert_of_pair(g, o, j));
+    if (expert == nullptr) {  // counted once
       if (blockIdx.x == 0 && part == 0 && lane == 0) add_device_flag(LMOE_FLAG_UNPLACED, 1);
       continue;
     }
@@ -365,7 +381,7 @@ __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_down_kernel(Mx4Args 
     const char* row[1] = {static_cast<const char*>(g.a) + static_cast<size_t>(j) * g.K * (A8 ? 1 : 2)};
     const uint8_t* row_scale[1] = {A8 ? g.a_scale + static_cast<size_t>(j) * (g.K / kMxGroup) : nullptr};
     f32x4_t acc[1][1] = {{f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}}};
-    const uint8_t* wblk = g.w + slot * g.w_slot_bytes + static_cast<size_t>(blockIdx.x) * bb;
+    const uint8_t* wblk = expert + static_cast<size_t>(blockIdx.x) * bb;
     few_chunks<A8, 1, 1, 4>(wblk, bb, 1, g.K, part * chunks / parts, (part + 1) * chunks / parts, lane, row, row_scale,
                             acc);
     sum += wj * acc[0][0];

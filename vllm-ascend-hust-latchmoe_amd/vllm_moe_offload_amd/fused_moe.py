@@ -206,6 +206,10 @@ def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2
                                 path=path, block_m=native.mx4_block_m(T * k, P))
 
 
+def _second_bank(overflow: PreparedSlotWeights | None) -> tuple | None:
+    return None if overflow is None else (overflow.w1, overflow.w2, overflow.log2phy)
+
+
 def _layer_path(hidden, k: int, n_experts: int, *w13) -> int:
     """native.layer_path of a layer of n_experts experts (the length of its
     slot table) over the gate-up banks w13 (a pass's own and, where there are
@@ -321,13 +325,18 @@ def _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2p
     bm = _block_m(hidden, k, w13_slots, path)
     merged = overflow is not None and log2phy is not None and not events and \
         _merged_passes(hidden, k, w13_slots, overflow, path)
+    if mx4 and T == 1 and path == native.LMOE_PATH_GEMV and (overflow is None or log2phy is not None):
+        # one form of one token, with an overflow pass or without; the permutation is for its counts alone
+        if events:
+            for e in events:
+                e.record()
+        native.permute(topk_ids, ws.perm, log2phy=log2phy, skip_unmapped=overflow is not None, block_m=bm)
+        native.mx4_decode_one(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
+                              second=_second_bank(overflow))
+        return dst, ws
     if mx4 and overflow is None and not events:
-        if T == 1 and path == native.LMOE_PATH_GEMV:  # the permutation for its counts alone
-            native.permute(topk_ids, ws.perm, log2phy=log2phy, block_m=bm)
-            native.mx4_decode_one(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add)
-        else:
-            native.mx4_fused_moe(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
-                                 path=path, block_m=bm)
+        native.mx4_fused_moe(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
+                             path=path, block_m=bm)
         return dst, ws
     if events:
         events[0].record()
@@ -433,7 +442,7 @@ def decode_layer(
     merged = overflow is not None and log2phy is not None and _merged_passes(hidden, kw, w13_slots, overflow, path)
     perm_b = None
     fused_body = overflow is None and path == native.LMOE_PATH_GEMV and not mx4
-    mx4_one = T == 1 and overflow is None and path == native.LMOE_PATH_GEMV and mx4
+    mx4_one = T == 1 and path == native.LMOE_PATH_GEMV and mx4 and (overflow is None or log2phy is not None)
     if mx4_one and ws.mx4 is None:
         raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
     if T == 1 and (fused_body or mx4_one):
@@ -452,7 +461,8 @@ def decode_layer(
         w, ids, _ = native.router_topk_permute(logits, k, ws.perm, block_m=bm, **sel)
     dst = out if out is not None else ws.out[:T]
     if mx4_one:
-        native.mx4_decode_one(rows, w, ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add)
+        native.mx4_decode_one(rows, w, ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
+                              second=_second_bank(overflow))
         return dst, w, ids
     if overflow is not None:
         if merged:

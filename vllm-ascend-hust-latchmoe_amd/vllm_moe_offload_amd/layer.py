@@ -7,6 +7,10 @@ as a pinned suffix row of the slot bank and appended to every token's top-k
 with weight 1 (one combine covers routed + shared); any other shared expert
 runs as a dense 1-slot pass whose output enters the routed combine as `add`.
 
+weight_format "mxfp4" holds the experts (a shared one too) in 4 bits: host store,
+slot bank and staging then move about a quarter of the bytes.  bf16 weights are
+quantized here, uint8 ones are banks that mxfp4.pack_w13 / pack_w2 made.
+
 The three pieces map onto the reference's seam: router() is captured piece
 1 (moe_router_indirect), stage() the eager splitting op
 (moe_offload_stage), forward_experts() captured piece 2 (moe_mlp -> the
@@ -19,7 +23,7 @@ from __future__ import annotations
 
 import torch
 
-from vllm_moe_offload_amd import native
+from vllm_moe_offload_amd import mxfp4, native
 from vllm_moe_offload_amd.fused_moe import (
     MoECommMethod,
     MoEFusedExpertsInput,
@@ -29,6 +33,7 @@ from vllm_moe_offload_amd.fused_moe import (
     fused_experts,
     get_workspace,
     route,
+    rows_kind,
     run_overflow_prefill,
 )
 from vllm_moe_offload_amd.moe_offload.cpu_first_loader import (
@@ -63,8 +68,18 @@ class SlotMoELayer(torch.nn.Module):
         shared_w2: torch.Tensor | None = None,
         layer_name: str | None = None,
         device: torch.device | str = "cuda",
+        weight_format: str = "bf16",
     ) -> None:
         super().__init__()
+        if weight_format not in ("bf16", "mxfp4"):
+            raise ValueError(f"unknown weight_format {weight_format!r}")
+        self.weight_format = weight_format
+        if weight_format == "mxfp4":
+            w13_weight, w2_weight = _mx4_banks(w13_weight, w2_weight)
+            if shared_w13 is not None:
+                shared_w13, shared_w2 = (t[0] for t in _mx4_banks(shared_w13.unsqueeze(0), shared_w2.unsqueeze(0)))
+        elif mxfp4.is_mx4(w13_weight):
+            raise ValueError('4-bit banks need weight_format="mxfp4"')
         self.layer_id = int(layer_id)
         self.layer_name = layer_name or f"model.layers.{layer_id}.mlp.experts"
         self.runtime = runtime
@@ -81,7 +96,7 @@ class SlotMoELayer(torch.nn.Module):
         # the gate's linear bias (f32 [E]), added to the logits before scoring
         self.gate_bias = gate_bias
         self.num_routed_experts = int(w13_weight.shape[0])
-        self.hidden_size = int(w13_weight.shape[2])
+        self.hidden_size = int(w2_weight.shape[1])
         self.intermediate_size = int(w13_weight.shape[1]) // 2
         self.mix_placement = False
         self.n_shared_experts = 0
@@ -116,8 +131,10 @@ class SlotMoELayer(torch.nn.Module):
             holder, num_experts=num_experts, hidden_size=hidden_size, intermediate_size=intermediate_size,
             dtype=dtype, pin_memory=runtime.config.should_pin_host_memory)
         load_expert_checkpoint(holder, files, prefix=prefix, names=names)
-        layer = cls(layer_id=layer_id, runtime=runtime, w13_weight=holder.w13_weight.data,
-                    w2_weight=holder.w2_weight.data, **kwargs)
+        w13, w2 = holder.w13_weight.data, holder.w2_weight.data
+        if kwargs.get("weight_format") == "mxfp4":  # the store then adopts the 4-bit blocks
+            w13, w2 = mxfp4.pack_experts(w13, w2, pin_memory=w13.is_pinned())
+        layer = cls(layer_id=layer_id, runtime=runtime, w13_weight=w13, w2_weight=w2, **kwargs)
         setattr(layer, CPU_FIRST_MARKER, True)
         return layer
 
@@ -167,7 +184,8 @@ class SlotMoELayer(torch.nn.Module):
         T, H = x.shape
         ones = _ones_bf16(T, x.device)
         zeros = _zeros_i32(T, x.device)
-        ws = get_workspace(T, 1, 1, H, int(self.shared_w13.shape[1]) // 2, x.device, tag=f"shared{self.layer_id}")
+        ws = get_workspace(T, 1, 1, H, int(self.shared_w13.shape[1]) // 2, x.device, tag=f"shared{self.layer_id}",
+                           rows=rows_kind(x, self.shared_w13))
         return fused_experts(x, ones, zeros, self.shared_w13, self.shared_w2, None, workspace=ws)
 
     @property
@@ -220,6 +238,18 @@ class SlotMoELayer(torch.nn.Module):
             return self.forward_experts(hidden)
         finally:
             moe_seam_inject.clear_injected_topk(self.layer_id)
+
+
+def _mx4_banks(w13: torch.Tensor, w2: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """4-bit banks of experts given as weights, or as banks already."""
+    if mxfp4.is_mx4(w13) != mxfp4.is_mx4(w2):
+        raise ValueError("w13 and w2 must both be weights or both be 4-bit banks")
+    if not mxfp4.is_mx4(w13):
+        return mxfp4.pack_experts(w13, w2)
+    H, I = int(w2.shape[1]), int(w13.shape[1]) // 2
+    if int(w13.shape[2]) != mxfp4.row_bytes(H) or int(w2.shape[2]) != mxfp4.row_bytes(I):
+        raise ValueError(f"banks {tuple(w13.shape)} and {tuple(w2.shape)} are not one layer's")
+    return w13, w2
 
 
 def _with_shared(counts: dict[int, int], layer: SlotMoELayer) -> dict[int, int]:

@@ -153,14 +153,19 @@ def unpack_w13(bank: torch.Tensor, H: int) -> tuple[torch.Tensor, torch.Tensor]:
     return part(codes), part(scales)
 
 
-def pack_experts(w13: torch.Tensor, w2: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+def pack_experts(w13: torch.Tensor, w2: torch.Tensor, *, pin_memory: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """4-bit banks of bf16 (or f32) experts w13 [E, 2I, H], w2 [E, H, I], an
-    expert at a time: what SlotMoELayer registers for 4-bit experts."""
-    if w13.dim() != 3 or w2.dim() != 3:
+    expert at a time: what SlotMoELayer registers for 4-bit experts.  pin_memory:
+    into page-locked memory (host weights), for the host store to adopt."""
+    if w13.dim() != 3 or w2.dim() != 3 or w13.shape[0] != w2.shape[0]:
         raise ValueError("experts are [E, 2I, H] and [E, H, I]")
-    out13 = torch.empty((*w13.shape[:2], row_bytes(int(w13.shape[2]))), dtype=torch.uint8, device=w13.device)
-    out2 = torch.empty((*w2.shape[:2], row_bytes(int(w2.shape[2]))), dtype=torch.uint8, device=w2.device)
-    for e in range(int(w13.shape[0])):
-        out13[e] = pack_w13(*quantize(w13[e]))
-        out2[e] = pack_w2(*quantize(w2[e]))
-    return out13, out2
+    if int(w2.shape[1]) != int(w13.shape[2]) or 2 * int(w2.shape[2]) != int(w13.shape[1]):
+        raise ValueError(f"w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} are not one layer's")
+    out = []
+    for w, pack in ((w13, pack_w13), (w2, pack_w2)):
+        bank = torch.empty((*w.shape[:2], row_bytes(int(w.shape[2]))), dtype=torch.uint8, device=w.device,
+                           pin_memory=pin_memory)
+        for e in range(int(w.shape[0])):
+            bank[e] = pack(*quantize(w[e]))
+        out.append(bank)
+    return out[0], out[1]

@@ -166,7 +166,7 @@ _SIGNATURES = {
     ),
     "lmoe_mx4_decode_one": (
         _i,
-        [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp],
+        [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp],
     ),
     "lmoe_fused_moe_decode": (
         _i,
@@ -909,7 +909,13 @@ def prefill_block_m(n_experts: int, hidden: int, intermediate: int, device="cuda
 
 
 MX4_BLOCK_M = (32, 64, 128)  # row-tile heights of the 4-bit experts' prefill kernel
-MX4_FEW_PAIRS_PER_EXPERT = 16
+# Up to this many pairs per expert the split-K kernel, row tiles past it.  us, gate-up
+# and down together, split-K / 32-row tiles (H, I, experts, top k; half of the Zipf
+# bias on the routing):
+#   2048, 768, 128, 8    16 tokens 27.2 / 26.2, 32: 49.7 / 47.9, 64: 63.2 / 58.9, 128: 85 / 71
+#   2048, 1408, 60, 4    30: 42.2 / 39.8, 61: 50.0 / 52.4, 120: 66.7 / 56.7
+#   7168, 2048, 32, 8    16: 121 / 128, 32: 139 / 155, 64: 178 / 165 (8-bit rows)
+MX4_FEW_PAIRS_PER_EXPERT = 3
 
 
 def mx4_path(n_pairs: int, n_experts: int) -> int:
@@ -1339,18 +1345,30 @@ def mx4_fused_moe(x, topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_slo
 
 def mx4_decode_one(x, topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_slots: torch.Tensor,
                    w2_slots: torch.Tensor, log2phy: torch.Tensor | None, bufs: Mx4Buffers, out: torch.Tensor, *,
-                   add: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+                   add: torch.Tensor | None = None, second: tuple | None = None, stream=None) -> torch.Tensor:
     """One token over 4-bit banks, straight from its ids (no permutation is built:
-    bufs.perm is left as it was)."""
+    bufs.perm is left as it was).  second = (w13, w2, log2phy) of another bank,
+    for experts that log2phy leaves out (the decode overflow buffer)."""
     lib = load_library()
     xq, xs, T, k, n_table = _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, bufs, out, add)
     if T != 1:
         raise ValueError(f"one token, got {T}")
+    b13 = b2 = tab = None
+    n_slots_b = n_table_b = 0
+    if second is not None:
+        if log2phy is None:
+            raise ValueError("a second bank needs the first one's table")
+        b13, b2, tab = second
+        n_slots_b, n_table_b = b13.shape[0], tab.numel()
+        _need(b13, "second w13", torch.uint8, (n_slots_b, *w13_slots.shape[1:]))
+        _need(b2, "second w2", torch.uint8, (n_slots_b, *w2_slots.shape[1:]))
+        _need(tab, "second log2phy", torch.int32)
+        _same_device(b13, b2, tab)
     _check(
         lib.lmoe_mx4_decode_one(
             xq.data_ptr(), _ptr(xs), bufs.hidden, bufs.intermediate, k, w13_slots.data_ptr(), w2_slots.data_ptr(),
-            bufs.perm.n_slots, topk_weights.data_ptr(), topk_ids.data_ptr(), _ptr(log2phy), n_table, _ptr(add),
-            bufs.act_ptr, bufs.act_scale_ptr, out.data_ptr(), _stream(stream),
+            bufs.perm.n_slots, topk_weights.data_ptr(), topk_ids.data_ptr(), _ptr(log2phy), n_table,
+            _ptr(b13), _ptr(b2), n_slots_b, _ptr(tab), n_table_b, _ptr(add), bufs.act_ptr, bufs.act_scale_ptr, out.data_ptr(), _stream(stream),
         ),
         "lmoe_mx4_decode_one",
     )
@@ -1759,8 +1777,8 @@ def wave_stage(plan: WavePlan, wave: int, *, main_table: torch.Tensor, main_owne
     lib = load_library()
     for name, t in (("main_w13", main_w13), ("main_w2", main_w2), ("stage_w13", stage_w13),
                     ("stage_w2", stage_w2), ("host_w13", host_w13), ("host_w2", host_w2)):
-        if t.dtype != torch.bfloat16 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous bf16 tensor")
+        if t.dtype not in (torch.bfloat16, torch.uint8) or t.dtype != main_w13.dtype or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous bf16 tensor (or all of them 4-bit, uint8)")
     if not (host_w13.is_pinned() and host_w2.is_pinned()):
         raise ValueError("device wave staging reads the host store directly: it must be page-locked")
     if int(host_w13.shape[0]) < plan.n_routed or int(main_table.numel()) < plan.n_routed:
@@ -1772,10 +1790,11 @@ def wave_stage(plan: WavePlan, wave: int, *, main_table: torch.Tensor, main_owne
     if int(main_owner.numel()) < int(main_slots):
         raise ValueError("main_owner must hold one entry per main slot")
     _need(stage_table, "stage_table", torch.int32)
-    b13 = int(host_w13[0].numel()) * 2
-    b2 = int(host_w2[0].numel()) * 2
-    if int(stage_w13[0].numel()) * 2 != b13 or int(stage_w2[0].numel()) * 2 != b2 or \
-            int(main_w13[0].numel()) * 2 != b13 or int(main_w2[0].numel()) * 2 != b2:
+    size = int(host_w13.element_size())
+    b13 = int(host_w13[0].numel()) * size
+    b2 = int(host_w2[0].numel()) * size
+    if int(stage_w13[0].numel()) * size != b13 or int(stage_w2[0].numel()) * size != b2 or \
+            int(main_w13[0].numel()) * size != b13 or int(main_w2[0].numel()) * size != b2:
         raise ValueError("expert row sizes differ between host store, main bank and stage buffer")
     _check(lib.lmoe_wave_stage(
         _ptr(plan.buf), plan.n_routed, plan.n_slots, plan.max_waves, int(wave), _ptr(main_table),
