@@ -507,7 +507,7 @@ def test_empty_batches_and_refusals():
             call()
             pytest.fail(f"call {i} was taken")
     with pytest.raises(RuntimeError, match="unsupported shape"):
-        native.mx4_fused_moe(layer.x, w, ids, layer.w13, layer.w2, None, bufs, out, block_m=256,
+        native.mx4_fused_moe(layer.x, w, ids, layer.w13, layer.w2, None, bufs, out, block_m=96,
                              path=native.LMOE_PATH_MFMA)
     with pytest.raises(RuntimeError, match="unsupported option"):
         native.gateup_silu(layer.x, 1, layer.w13, perm, act, path=native.LMOE_PATH_STREAM)

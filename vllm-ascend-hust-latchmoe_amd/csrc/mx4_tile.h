@@ -54,9 +54,10 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// The slot whose row tiles hold a tile, its first tile and its rows: the last of the
-// slots from first whose tile_off is not past the tile (ascending; P + 1 entries).  A
-// wave looks 64 of them up at once, one per lane.
+// The slot whose row tiles hold a tile, its first tile and its rows: the last slot
+// whose tile_off is not past the tile (ascending; P + 1 entries).  A wave looks 64 of
+// them up at once, one per lane, and has the first 128 on their way before it needs
+// any: the start of a workgroup then waits for one load here.
 struct SlotWindow {
   int t0, o0, o1;
 };
@@ -68,18 +69,17 @@ __device__ __forceinline__ SlotWindow load_window(const int32_t* tile_off, const
 struct TileSlot {
   int slot, tile0, p0, p1;
 };
-// The lookup in a window that was loaded from first on; further windows as needed.
+// v, next: the windows from 0 and from 64 on
 __device__ __forceinline__ TileSlot slot_of_tile(const int32_t* tile_off, const int32_t* offsets, int P, int tile,
-                                                 int first, SlotWindow v, int lane) {
-  for (;;) {
-    const int k = __popcll(__ballot(v.t0 <= tile)) - 1;  // lane 0's always is
-    const int last = min(63, P - 1 - first);             // lanes past it repeat its entry
-    if (k < 63 || last < 63 || first + 64 >= P || tile_off[first + 64] > tile) {
-      const int l = min(k, last);
-      return {first + l, read_lane_i32(v.t0, l), read_lane_i32(v.o0, l), read_lane_i32(v.o1, l)};
-    }
-    first += 64;
-    v = load_window(tile_off, offsets, P, first, lane);
+                                                 SlotWindow v, SlotWindow next, int lane) {
+  for (int first = 0;; first += 64) {
+    // lanes past the last slot repeat it; lane 0's entry is never past the tile
+    const int last = min(63, P - 1 - first);
+    const int k = min(__popcll(__ballot(v.t0 <= tile)) - 1, last);
+    const bool here = k < 63 || first + 64 >= P || read_lane_i32(next.t0, 0) > tile;
+    if (here) return {first + k, read_lane_i32(v.t0, k), read_lane_i32(v.o0, k), read_lane_i32(v.o1, k)};
+    v = next;
+    if (first + 128 < P) next = load_window(tile_off, offsets, P, first + 128, lane);
   }
 }
 
@@ -97,6 +97,8 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   // work item: XCD-contiguous chunks of (row tile, column tile)
   constexpr int OUT_COLS = GU ? kTileCols / 2 : kTileCols;
   const int NT = (g.N + OUT_COLS - 1) / OUT_COLS;
+  const SlotWindow win0 = load_window(g.tile_off, g.offsets, g.P, 0, lane);
+  const SlotWindow win1 = load_window(g.tile_off, g.offsets, g.P, 64, lane);
   const int total = g.meta[LMOE_META_TILES] * NT;
   const int share = (total + 7) >> 3;
   const int jj = blockIdx.x >> 3;
@@ -104,8 +106,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   if (jj >= share || item >= total) return;
   const int tile = item / NT;
   const int n0 = (item - tile * NT) * OUT_COLS;
-  const TileSlot ts = slot_of_tile(g.tile_off, g.offsets, g.P, tile, 0,
-                                   load_window(g.tile_off, g.offsets, g.P, 0, lane), lane);
+  const TileSlot ts = slot_of_tile(g.tile_off, g.offsets, g.P, tile, win0, win1, lane);
   const int slot = ts.slot;
   const int p0 = ts.p0 + (tile - ts.tile0) * BM;
   const int rows = min(BM, ts.p1 - p0);
