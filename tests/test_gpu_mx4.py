@@ -192,6 +192,27 @@ def test_tile_heights_give_the_same_bits(H, I, counts, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("counts", [
+    [0] * 63 + [40, 3],                             # the last of the first 64 slots, then the next
+    [0] * 64 + [33],
+    [5] * 64,
+    [1] * 130 + [0] * 70 + [65],                    # past 128 slots, empty ones between
+    [0] * 300 + [2, 0, 0, 31],
+    [200] + [0] * 400,
+])
+def test_tiles_find_their_slot(counts):
+    native = _native()
+    P = len(counts)
+    layer = Layer(32, 32, P, sum(counts), "bf16", P)
+    ids = _ids(counts, 0, np.random.default_rng(P))
+    for bm in native.MX4_BLOCK_M:
+        print(f"case mx4 slots P={P} block_m={bm}", flush=True)
+        perm, act, y = run_layer(layer, ids, 1, native.LMOE_PATH_MFMA, block_m=bm)
+        torch.cuda.synchronize()
+        check_layer(layer, perm, 1, act, y, ids[:, 0])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", ROWS)
 def test_several_experts_per_token_and_the_same_twice(rows):
     """top_k 3; a token may name one expert twice: both pairs get their row."""

@@ -924,11 +924,23 @@ def mx4_path(n_pairs: int, n_experts: int) -> int:
     return LMOE_PATH_GEMV if n_pairs <= MX4_FEW_PAIRS_PER_EXPERT * n_experts else LMOE_PATH_MFMA
 
 
+# Most pairs per slot, on average, of each row-tile height but the last.  us, gate-up
+# and down together, 32 / 64 / 128 rows (bf16 rows; 8-bit rows):
+#   2048, 768, 128, 8   25 pairs per slot 80 / 82 / 99;    76 / 78 / 81
+#                       40               100 / 97 / 117;   90 / 84 / 87
+#                       64               126 / 116 / 136; 109 / 95 / 96
+#                       100              170 / 148 / 169; 144 / 117 / 115
+#                       256              380 / 321 / 311; 290 / 254 / 209
+#   7168, 2048, 32, 8   50               225 / 183 / 203 (8-bit rows)
+#                       100              325 / 262 / 247
+MX4_BLOCK_MAX_PAIRS = {32: 32, 64: 100}
+
+
 def mx4_block_m(n_pairs: int, n_experts: int) -> int:
     """Row-tile height of 4-bit experts' products (the permutation's block_m)
     for n_pairs pairs over n_experts slots."""
-    for bm in MX4_BLOCK_M:
-        if n_pairs <= bm * n_experts:
+    for bm, most in MX4_BLOCK_MAX_PAIRS.items():
+        if n_pairs <= most * n_experts:
             return bm
     return MX4_BLOCK_M[-1]
 
@@ -996,8 +1008,9 @@ def permute(
     replaces perm.row_idx as the output (the first pass's permutation when
     the passes build separate permutations)."""
     lib = load_library()
-    _need(ids, "topk_ids", torch.int32)
-    n = int(ids.numel())
+    if not _is(ids, torch.int32, getattr(ids, "shape", ())):
+        _need(ids, "topk_ids", torch.int32)
+    n = ids.numel()
     if n != perm.n_pairs:
         raise ValueError(f"permutation buffers sized for {perm.n_pairs} pairs, got {n}")
     rows = perm.row_idx if row_idx is None else row_idx
@@ -1012,11 +1025,11 @@ def permute(
         n_table = int(log2phy.numel()) if table_len is None else min(int(table_len), int(log2phy.numel()))
     _check(
         lib.lmoe_permute(
-            _ptr(ids), n, _ptr(log2phy), n_table,
+            ids.data_ptr(), n, _ptr(log2phy), n_table,
             perm.n_slots, mode, int(block_m),
-            _ptr(perm.counts), _ptr(perm.offsets), _ptr(perm.sorted_pairs),
-            _ptr(rows), _ptr(perm.active), _ptr(perm.tile_off), _ptr(perm.meta),
-            _ptr(perm.workspace), int(perm.workspace.numel()), _stream(stream),
+            perm.counts.data_ptr(), perm.offsets.data_ptr(), perm.sorted_pairs.data_ptr(),
+            rows.data_ptr(), perm.active.data_ptr(), perm.tile_off.data_ptr(), perm.meta.data_ptr(),
+            perm.workspace.data_ptr(), perm.workspace.numel(), _stream(stream),
         ),
         "lmoe_permute",
     )
@@ -1194,43 +1207,60 @@ def down(act: torch.Tensor, w2_slots: torch.Tensor, perm: Permutation, y: torch.
     return y
 
 
-def _need_mx4(bank: torch.Tensor, name: str, perm: Permutation, K: int) -> int:
+def _need_mx4(bank: torch.Tensor, name: str, perm: Permutation, K: int, rows: int | None = None) -> int:
     """Check a 4-bit bank of K columns; returns its rows per expert."""
+    width = mxfp4.row_bytes(K)
+    if rows is not None and _is(bank, torch.uint8, (perm.n_slots, rows, width)):
+        return rows
     _need(bank, name, torch.uint8)
     if bank.dim() != 3 or bank.shape[0] != perm.n_slots:
         raise ValueError(f"{name} has shape {tuple(bank.shape)}, the permutation {perm.n_slots} slots")
-    if int(bank.shape[2]) != mxfp4.row_bytes(K):
+    if int(bank.shape[2]) != width:
         raise ValueError(f"{name} rows of {int(bank.shape[2])} bytes do not hold {K} columns in 4 bits")
+    if rows is not None and int(bank.shape[1]) != rows:
+        raise ValueError(f"{name} has {int(bank.shape[1])} rows per expert, not {rows}")
     return int(bank.shape[1])
 
 
 def _need_rows(rows, name: str, shape: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """bf16 rows or Mx8Rows: (values, scales or None)."""
+    """bf16 rows or Mx8Rows, [R, K]: (values, scales or None)."""
     if isinstance(rows, Mx8Rows):
         _need_mx8(rows, name, shape)
         return rows.q, rows.scale
-    _need(rows, name, torch.bfloat16, shape)
+    if shape is None or not _is(rows, torch.bfloat16, shape):
+        _need(rows, name, torch.bfloat16, shape)
+    if rows.dim() != 2:
+        raise ValueError(f"{name} must be [R, K], got {tuple(rows.shape)}")
     return rows, None
 
 
+def _need_y(y, shape: tuple) -> bool:
+    """bf16 or f32 rows by pair; whether they are f32."""
+    if not isinstance(y, torch.Tensor) or y.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("y must be bf16 or f32")
+    if not _is(y, y.dtype, shape):
+        _need(y, "y", y.dtype, shape)
+    return y.dtype is torch.float32
+
+
 def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, act, *, path: int, stream):
-    lib = load_library()
-    xq, xs = _need_rows(x, "x")
+    xq, xs = _need_rows(x, "x", tuple(x.shape))
     T, H = xq.shape
-    two_i = _need_mx4(w13_slots, "w13_slots", perm, H)
-    if two_i % 2:
-        raise ValueError(f"w13_slots has {two_i} rows per expert")
-    if perm.n_pairs != T * int(top_k):
+    n = perm.n_pairs
+    if n != T * top_k:
         raise ValueError("permutation does not match T * top_k pairs")
-    aq, as_ = _need_rows(act, "act", (perm.n_pairs, two_i // 2))
+    aq, as_ = _need_rows(act, "act", (n, act.shape[-1]))
+    I = aq.shape[1]
     if (xs is None) != (as_ is None):
         raise ValueError("x and act must both be bf16 or both be Mx8Rows")
+    _need_mx4(w13_slots, "w13_slots", perm, H, 2 * I)
     _same_device(xq, w13_slots, perm.offsets, aq)
+    p = perm
     _check(
-        lib.lmoe_mx4_gateup_silu(
-            _ptr(xq), _ptr(xs), T, H, two_i // 2, int(top_k), _ptr(w13_slots), perm.n_slots, _ptr(perm.offsets),
-            _ptr(perm.sorted_pairs), _ptr(perm.active), _ptr(perm.tile_off), _ptr(perm.meta), perm.n_pairs,
-            perm.block_m, int(path), _ptr(aq), _ptr(as_), _stream(stream),
+        load_library().lmoe_mx4_gateup_silu(
+            xq.data_ptr(), _ptr(xs), T, H, I, top_k, w13_slots.data_ptr(), p.n_slots, p.offsets.data_ptr(),
+            p.sorted_pairs.data_ptr(), p.active.data_ptr(), p.tile_off.data_ptr(), p.meta.data_ptr(), n, p.block_m, path,
+            aq.data_ptr(), _ptr(as_), _stream(stream),
         ),
         "lmoe_mx4_gateup_silu",
     )
@@ -1238,20 +1268,18 @@ def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, 
 
 
 def _mx4_down(act, w2_slots: torch.Tensor, perm: Permutation, y: torch.Tensor, *, path: int, stream):
-    lib = load_library()
-    aq, as_ = _need_rows(act, "act")
-    if aq.dim() != 2 or aq.shape[0] != perm.n_pairs:
-        raise ValueError(f"act has shape {tuple(aq.shape)}, the permutation {perm.n_pairs} pairs")
-    H = _need_mx4(w2_slots, "w2_slots", perm, int(aq.shape[1]))
-    if y.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError("y must be bf16 or f32")
-    _need(y, "y", y.dtype, (perm.n_pairs, H))
+    n = perm.n_pairs
+    aq, as_ = _need_rows(act, "act", (n, act.shape[-1]))
+    I = aq.shape[1]
+    H = _need_mx4(w2_slots, "w2_slots", perm, I, w2_slots.shape[1] if w2_slots.dim() == 3 else None)
+    y_f32 = _need_y(y, (n, H))
     _same_device(aq, w2_slots, perm.offsets, y)
+    p = perm
     _check(
-        lib.lmoe_mx4_down(
-            _ptr(aq), _ptr(as_), H, int(aq.shape[1]), _ptr(w2_slots), perm.n_slots, _ptr(perm.offsets),
-            _ptr(perm.sorted_pairs), _ptr(perm.active), _ptr(perm.tile_off), _ptr(perm.meta), perm.n_pairs,
-            perm.block_m, int(path), _ptr(y), int(y.dtype == torch.float32), _stream(stream),
+        load_library().lmoe_mx4_down(
+            aq.data_ptr(), _ptr(as_), H, I, w2_slots.data_ptr(), p.n_slots, p.offsets.data_ptr(),
+            p.sorted_pairs.data_ptr(), p.active.data_ptr(), p.tile_off.data_ptr(), p.meta.data_ptr(), n, p.block_m, path,
+            y.data_ptr(), y_f32, _stream(stream),
         ),
         "lmoe_mx4_down",
     )
