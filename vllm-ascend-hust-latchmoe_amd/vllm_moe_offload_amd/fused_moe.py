@@ -317,6 +317,8 @@ def _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2p
     rows = rows_kind(hidden, w13_slots)
     mx4 = rows != ""
     ws = workspace or get_workspace(T, k, P, H, I, hidden.device, rows=rows)
+    if mx4 and ws.mx4 is None:
+        raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
     dst = out if out is not None else ws.out[:T]
     if path == native.LMOE_PATH_AUTO:
         path = _bank_layer_path(hidden, k, w13_slots, log2phy, overflow)

@@ -392,8 +392,9 @@ def add_rms_norm(
     8-bit rows) or to both; with neither given a bf16 out is made.  r goes to
     residual_out, in place of residual if that is not given.  x [T, H] bf16,
     residual bf16 or f32, weight [H] bf16 or f32; r is kept in f32 between the
-    sum and the outputs.  out or residual_out may be x or residual.  H a
-    multiple of 8 (of 32 with mx8) up to 32768.  Returns (out, mx8,
+    sum and the outputs, the squares are summed in f32.  residual_out may be x,
+    out may be x, or residual if residual_out is another buffer (where an f32
+    residual is not one of them).  H a multiple of 8 (of 32 with mx8) up to 32768.  Returns (out, mx8,
     residual_out), None for what was not asked for."""
     lib = load_library()
     bf16, f32 = torch.bfloat16, torch.float32
@@ -427,6 +428,12 @@ def add_rms_norm(
         _need_mx8(mx8, "mx8", shape)
         q, scale = mx8.q, mx8.scale
     _same_device(x, weight, residual, residual_out, out, q, scale)
+    if residual is not None and T:
+        if out is not None and out.data_ptr() == residual_out.data_ptr():
+            raise ValueError("out and residual_out must be two buffers")
+        if rdt is f32 and ((out is not None and out.data_ptr() == residual.data_ptr()) or
+                           residual_out.data_ptr() == x.data_ptr()):
+            raise ValueError("rows of two types cannot share a buffer")
     _check(
         lib.lmoe_add_rms_norm(
             x.data_ptr(), T, H, _ptr(residual), rdt is f32, weight.data_ptr(), wdt is f32, eps, _ptr(residual_out),
@@ -1254,7 +1261,7 @@ def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, 
     if (xs is None) != (as_ is None):
         raise ValueError("x and act must both be bf16 or both be Mx8Rows")
     _need_mx4(w13_slots, "w13_slots", perm, H, 2 * I)
-    _same_device(xq, w13_slots, perm.offsets, aq)
+    _same_device(xq, xs, w13_slots, perm.offsets, aq, as_)
     p = perm
     _check(
         load_library().lmoe_mx4_gateup_silu(
@@ -1273,7 +1280,7 @@ def _mx4_down(act, w2_slots: torch.Tensor, perm: Permutation, y: torch.Tensor, *
     I = aq.shape[1]
     H = _need_mx4(w2_slots, "w2_slots", perm, I, w2_slots.shape[1] if w2_slots.dim() == 3 else None)
     y_f32 = _need_y(y, (n, H))
-    _same_device(aq, w2_slots, perm.offsets, y)
+    _same_device(aq, as_, w2_slots, perm.offsets, y)
     p = perm
     _check(
         load_library().lmoe_mx4_down(
@@ -1303,10 +1310,16 @@ class Mx4Buffers:
         if y.dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("y must be bf16 or f32")
         _need(y, "y", y.dtype)
+        if y.dim() != 2:
+            raise ValueError(f"y must be [N, H], got {tuple(y.shape)}")
         if aq.shape[0] < perm.n_pairs or y.shape[0] < perm.n_pairs:
             raise ValueError("act and y need a row for every pair")
         self.perm, self.act, self.y = perm, act, y
         self.device_index = y.get_device()
+        for t in (aq, as_, perm.counts, perm.offsets, perm.sorted_pairs, perm.row_idx, perm.active, perm.tile_off,
+                  perm.meta, perm.workspace):
+            if t is not None and t.get_device() != self.device_index:
+                raise ValueError(f"a buffer on {t.device}, y on {y.device}")
         self.hidden, self.intermediate = int(y.shape[1]), int(aq.shape[1])
         self.mx8 = as_ is not None
         self.act_ptr, self.act_scale_ptr = _ptr(aq), _ptr(as_)
@@ -1348,7 +1361,7 @@ def _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, buf
     here = torch.cuda.current_device()
     if bufs.device_index != here:
         raise ValueError(f"buffers on cuda:{bufs.device_index}, the current device is cuda:{here}")
-    _same_device(xq, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, out, add)
+    _same_device(xq, xs, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, out, add)
     return xq, xs, T, k, n_table
 
 
@@ -1375,8 +1388,11 @@ def mx4_decode_one(x, topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_sl
                    w2_slots: torch.Tensor, log2phy: torch.Tensor | None, bufs: Mx4Buffers, out: torch.Tensor, *,
                    add: torch.Tensor | None = None, second: tuple | None = None, stream=None) -> torch.Tensor:
     """One token over 4-bit banks, straight from its ids (no permutation is built:
-    bufs.perm is left as it was).  second = (w13, w2, log2phy) of another bank,
-    for experts that log2phy leaves out (the decode overflow buffer)."""
+    bufs.perm is left as it was).  The sums over K are cut otherwise than
+    mx4_fused_moe's, so out may be off that form's by a rounding; one token taken
+    in waves over fewer slots than it has experts has that form.  second = (w13,
+    w2, log2phy) of another bank, for experts that log2phy leaves out (the decode
+    overflow buffer)."""
     lib = load_library()
     xq, xs, T, k, n_table = _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, bufs, out, add)
     if T != 1:
