@@ -449,7 +449,10 @@ long long lmoe_mx4_bytes(int N, int K);
  * permutation arguments).  Rows are bf16 (x_scale and act_scale null) or MX8
  * rows (both given): then act is rounded to MX8 along I, and both products
  * multiply 8-bit by 4-bit values; f32 accumulation either way, gate, up and
- * their product in f32, act rounded once.  y is bf16 or f32 (y_f32) by pair,
+ * their product in f32, act rounded once.  act_split (bf16 rows, not in row
+ * tiles: LMOE_ERR_UNSUPPORTED): act is [n_pairs, 2, I], two bf16 numbers whose
+ * sum is the value to 16 bits, for batches of few tokens, whose outputs hang on
+ * few act values.  y is bf16 or f32 (y_f32) by pair,
  * rows of unplaced pairs untouched.
  * path = LMOE_PATH_GEMV (few rows per slot: a workgroup's waves split K),
  * LMOE_PATH_MFMA (row tiles of block_m, the height given to lmoe_permute) or
@@ -462,18 +465,18 @@ int lmoe_mx4_gateup_silu(const void* x, const void* x_scale, int T, int H,
                          const int32_t* offsets, const int32_t* sorted_pairs,
                          const int32_t* active, const int32_t* tile_off,
                          const int32_t* meta, int n_pairs, int block_m,
-                         int path, void* act, void* act_scale,
+                         int path, void* act, void* act_scale, int act_split,
                          hipStream_t stream);
-int lmoe_mx4_down(const void* act, const void* act_scale, int H, int I,
-                  const void* w2_slots, int n_slots, const int32_t* offsets,
+int lmoe_mx4_down(const void* act, const void* act_scale, int act_split,
+                  int H, int I, const void* w2_slots, int n_slots, const int32_t* offsets,
                   const int32_t* sorted_pairs, const int32_t* active,
                   const int32_t* tile_off, const int32_t* meta, int n_pairs,
                   int block_m, int path, void* y, int y_f32,
                   hipStream_t stream);
 
 /* Buffers of lmoe_mx4_fused_moe for T*k pairs over n_slots slots: lmoe_permute's
- * outputs and workspace, act (with act_scale: MX8 rows) and y as lmoe_mx4_down
- * writes it. */
+ * outputs and workspace, act (with act_scale: MX8 rows; act_split: room for bf16
+ * rows in two parts, which row tiles do not use) and y as lmoe_mx4_down writes it. */
 typedef struct lmoe_mx4_workspace {
   int32_t* counts;
   int32_t* offsets;
@@ -488,6 +491,7 @@ typedef struct lmoe_mx4_workspace {
   void* act_scale;
   void* y;
   int32_t y_f32;
+  int32_t act_split;
 } lmoe_mx4_workspace;
 
 /* A layer of 4-bit experts in one call: lmoe_permute (skip_unmapped 0),
@@ -502,10 +506,10 @@ int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int H, int I,
                        const void* add, void* out, hipStream_t stream);
 
 /* One token (x [H], ids and w [k]) through 4-bit experts without a permutation,
- * in two launches: act[j] of pair j as lmoe_mx4_gateup_silu makes it (path GEMV,
- * the same bits; rows of pairs without a slot untouched), then out = add +
- * sum_j w[j] W2 act[j], summed in f32 over parts of K of its own: out may be off
- * lmoe_mx4_fused_moe's by a rounding.  A pair whose id maps to no slot adds
+ * in two launches: act[j] of pair j as lmoe_mx4_gateup_silu has it (bf16 rows with
+ * act_split; rows of pairs without a slot untouched), then out = add +
+ * sum_j w[j] W2 act[j].  Both sum in f32 over parts of K of their own: act and out
+ * may be off lmoe_mx4_fused_moe's by a rounding.  A pair whose id maps to no slot adds
  * nothing and is counted in LMOE_FLAG_UNPLACED.  One slot may serve several
  * pairs.  w13_b, w2_b, log2phy_b (all null: none) are a second bank of n_slots_b
  * slots and its table, for experts that the first table leaves out (the decode

@@ -72,14 +72,14 @@ class Layer:
         self.x = x if rows == "bf16" else native.rows_to_mx8(x)
         self.xv = _f64(self.x if rows == "bf16" else self.x.float())
 
-    def act_buffer(self, n):
+    def act_buffer(self, n, split=False):
         native = _native()
         if self.rows == "mx8":
             a = native.Mx8Rows.allocate(n, self.I, "cuda")
             a.q.view(torch.uint8).fill_(0x31)
             a.scale.fill_(99)
             return a
-        return torch.full((n, self.I), 7.0, dtype=torch.bfloat16, device="cuda")
+        return torch.full((n, 2, self.I) if split else (n, self.I), 7.0, dtype=torch.bfloat16, device="cuda")
 
 
 def sum_error(x, w, mx8):
@@ -91,12 +91,19 @@ def sum_error(x, w, mx8):
     return e
 
 
-def check_act(got, gate, up, dg, du, mx8_scale=None):
+def act_values(act):
+    """act rows in 64 bits: bf16, MX8, or bf16 in two parts."""
+    if not isinstance(act, torch.Tensor):
+        return _f64(act.float())
+    return _f64(act) if act.dim() == 2 else _f64(act).sum(1)
+
+
+def check_act(got, gate, up, dg, du, mx8_scale=None, step=2.0**-8):
     sg = gate / (1.0 + np.exp(-gate))
     act = sg * up
     tol = 1.1 * np.abs(up) * dg + np.abs(sg) * du + dg * du + 2.0**-20 * np.abs(act)
     if mx8_scale is None:
-        tol = tol + 2.0**-8 * np.abs(act)
+        tol = tol * (1 + step) + step * np.abs(act)
     else:
         tol = tol * (1 + 2.0**-4) + np.maximum(2.0**-4 * np.abs(act), 2.0**-10 * np.repeat(mx8_scale, 32, axis=1))
     assert np.all(np.abs(got - act) <= tol), float(np.max(np.abs(got - act) / np.maximum(tol, 1e-300)))
@@ -107,7 +114,11 @@ def check_layer(layer, perm, k, act, y, ids_slot):
     offs = perm.offsets.cpu().numpy()
     pairs = perm.sorted_pairs.cpu().numpy()
     mx8 = layer.rows == "mx8"
-    a = _f64(act.float() if mx8 else act)
+    a = act_values(act)
+    # two parts: the high one is off by 2^-8 of the value at most and the low one by
+    # 2^-8 of that; their products are twice as many terms of 1 + 2^-8 the size
+    split = not mx8 and act.dim() == 3
+    step, terms = (2.0**-16, 2.01) if split else (2.0**-8, 1.0)
     sc = np.ldexp(1.0, act.scale.cpu().numpy().astype(np.int64) - 127) if mx8 else None
     yv = _f64(y)
     ystep = 2.0**-8 if y.dtype == torch.bfloat16 else 2.0**-24
@@ -119,9 +130,9 @@ def check_layer(layer, perm, k, act, y, ids_slot):
         x, w = layer.xv[pairs[pos] // k], layer.v13[s]
         g, ab = x @ w.T, sum_error(x, w, mx8)
         I = layer.I
-        check_act(a[pos], g[:, :I], g[:, I:], ab[:, :I], ab[:, I:], sc[pos] if mx8 else None)
+        check_act(a[pos], g[:, :I], g[:, I:], ab[:, :I], ab[:, I:], sc[pos] if mx8 else None, step)
         want = a[pos] @ layer.v2[s].T
-        tol = sum_error(a[pos], layer.v2[s], mx8) * (1 + ystep) + ystep * np.abs(want)
+        tol = terms * sum_error(a[pos], layer.v2[s], mx8) * (1 + ystep) + ystep * np.abs(want)
         got = yv[pairs[pos]]
         assert np.all(np.abs(got - want) <= tol + 1e-30), float(np.max(np.abs(got - want) / (tol + 1e-30)))
 
@@ -131,13 +142,13 @@ def _ids(counts, extra, rng):
     return rng.permutation(ids).reshape(-1, 1)
 
 
-def run_layer(layer, ids, k, path, *, block_m=None, log2phy=None, y_dtype=torch.bfloat16):
+def run_layer(layer, ids, k, path, *, block_m=None, log2phy=None, y_dtype=torch.bfloat16, split=False):
     native = _native()
     n = ids.size
     perm = native.Permutation.allocate(n, layer.P, "cuda")
     bm = native.mx4_block_m(n, layer.P) if block_m is None else block_m
     native.permute(to_dev_i32(ids), perm, log2phy=log2phy, skip_unmapped=True, block_m=bm)
-    act = layer.act_buffer(n)
+    act = layer.act_buffer(n, split)
     y = torch.full((n, layer.H), -7.0, dtype=y_dtype, device="cuda")
     native.grouped_mlp(layer.x, k, layer.w13, layer.w2, perm, act, y, path=path)
     return perm, act, y
@@ -294,7 +305,8 @@ def test_fused_experts_over_a_4_bit_bank(T, k, E, rows):
     assert ws.y.dtype == (torch.float32 if T * k <= native.FUSED_DECODE_MAX_PAIRS else torch.bfloat16)
     assert isinstance(ws.act, native.Mx8Rows) == (rows == "mx8")
     path = native.mx4_path(T * k, E)
-    _, act, y = run_layer(layer, ids, k, path, log2phy=l2p, y_dtype=torch.float32)
+    split = rows == "bf16" and path == native.LMOE_PATH_GEMV  # as the workspace of so few pairs has it
+    _, act, y = run_layer(layer, ids, k, path, log2phy=l2p, y_dtype=torch.float32, split=split)
     yv = _f64(y).reshape(T, k, H)
     want = (_f64(w)[:, :, None] * yv).sum(1) + _f64(add)
     mag = (np.abs(_f64(w))[:, :, None] * np.abs(yv)).sum(1) + np.abs(_f64(add))
@@ -302,8 +314,8 @@ def test_fused_experts_over_a_4_bit_bank(T, k, E, rows):
     # the rows themselves: bf16 past FUSED_DECODE_MAX_PAIRS pairs; a fused form
     # may add the same products of act in another order
     rowtol = 2.0**-8 if ws.y.dtype == torch.bfloat16 else 0.0
-    av = _f64(act.float() if rows == "mx8" else act)
-    worst = max(sum_error(av, v, rows == "mx8").max() for v in layer.v2)
+    av = act_values(act)
+    worst = max(sum_error(av, v, rows == "mx8").max() for v in layer.v2) * (2.01 if split else 1.0)
     tol = tol + rowtol * mag + 2 * k * worst
     assert np.all(np.abs(_f64(out) - want) <= tol)
     again = fused_moe.fused_experts(layer.x, w, to_dev_i32(ids), layer.w13, layer.w2, l2p, add=add)
@@ -315,7 +327,8 @@ def test_fused_experts_over_a_4_bit_bank(T, k, E, rows):
 @pytest.mark.parametrize("H,I,k,E", [(32, 32, 1, 2), (160, 96, 3, 5), (1024, 416, 5, 8), (2048, 768, 8, 16),
                                      (544, 1056, 9, 12), (64, 64, 20, 4)])
 def test_one_token_straight_from_its_ids(H, I, k, E, rows):
-    """act has the split-K kernel's bits, out the pairs' weighted sum; a pair
+    """act is the formula's (its sums over K are cut otherwise than the split-K
+    kernel's, so its last bits may be others), out the pairs' weighted sum; a pair
     without a slot adds nothing and is counted; a slot may serve several pairs."""
     from vllm_moe_offload_amd import fused_moe, native
 
@@ -330,27 +343,31 @@ def test_one_token_straight_from_its_ids(H, I, k, E, rows):
     d_ids, d_l2p = to_dev_i32(ids), to_dev_i32(l2p)
     w = torch.empty((1, k), device="cuda").uniform_(0.05, 1).to(torch.bfloat16)
     add = torch.randn((1, H), device="cuda").to(torch.bfloat16)
-    bufs = native.Mx4Buffers(native.Permutation.allocate(k, E, "cuda"), layer.act_buffer(k),
+    split = rows == "bf16"
+    bufs = native.Mx4Buffers(native.Permutation.allocate(k, E, "cuda"), layer.act_buffer(k, split),
                              torch.empty((k, H), dtype=torch.float32, device="cuda"))
     native.device_flags(clear=True)
     out = native.mx4_decode_one(layer.x, w, d_ids, layer.w13, layer.w2, d_l2p, bufs,
                                 torch.empty((1, H), dtype=torch.bfloat16, device="cuda"), add=add)
     slots = np.array([l2p[e] if e < E else -1 for e in ids[0]])
     assert native.device_flags(clear=True)[native.FLAG_UNPLACED] == int((slots < 0).sum())
-    perm, act, y = run_layer(layer, ids, k, native.LMOE_PATH_GEMV, log2phy=d_l2p, y_dtype=torch.float32)
     bits = lambda a: a.q.view(torch.uint8) if rows == "mx8" else a.view(torch.int16)
-    pos = perm.row_idx.cpu().numpy()
+    mx8 = rows == "mx8"
+    av, wv = act_values(bufs.act), _f64(w)[0]
+    sc = np.ldexp(1.0, bufs.act.scale.cpu().numpy().astype(np.int64) - 127) if mx8 else None
+    want, mag, sums = _f64(add)[0].copy(), np.abs(_f64(add))[0], np.zeros(H)
     for j in range(k):
-        if slots[j] >= 0:
-            assert torch.equal(bits(bufs.act)[j], bits(act)[pos[j]]), j
-        else:
-            assert pos[j] == -1 and torch.equal(bits(bufs.act)[j], bits(layer.act_buffer(1))[0])
-    placed = torch.from_numpy(slots >= 0).cuda()
-    yw = _f64(y[placed]) * _f64(w)[0][slots >= 0][:, None]
-    want, mag = yw.sum(0) + _f64(add)[0], np.abs(yw).sum(0) + np.abs(_f64(add))[0]
-    av = _f64(act.float() if rows == "mx8" else act)[: int((slots >= 0).sum())]
-    worst = max((sum_error(av, v, rows == "mx8").max() for v in layer.v2), default=0.0) if len(av) else 0.0
-    tol = 2.0**-8 * np.abs(want) + (k + 10) * 2.0**-24 * mag + 2 * k * worst
+        if slots[j] < 0:
+            assert torch.equal(bits(bufs.act)[j], bits(layer.act_buffer(1, split))[0])
+            continue
+        gu, e = layer.xv @ layer.v13[slots[j]].T, sum_error(layer.xv, layer.v13[slots[j]], mx8)
+        check_act(av[j:j + 1], gu[:, :I], gu[:, I:], e[:, :I], e[:, I:], sc[j:j + 1] if mx8 else None, 2.0**-16)
+        y = wv[j] * (layer.v2[slots[j]] @ av[j])
+        want, mag = want + y, mag + np.abs(y)
+        # both parts' products: twice as many terms
+        sums += wv[j] * sum_error(av[j:j + 1], layer.v2[slots[j]], mx8)[0] * (2.01 if split else 1.0)
+    # a sum by up to eight waves, the addend and the bf16 rounding on top
+    tol = 2.0**-8 * np.abs(want) + (1 + 2.0**-8) * (sums + (k + 10) * 2.0**-24 * (mag + sums))
     assert np.all(np.abs(_f64(out)[0] - want) <= tol)
     # the layer's calls take this form, with the same bits
     if (slots >= 0).all():
@@ -497,7 +514,8 @@ def test_empty_batches_and_refusals():
     ]
     bf = [torch.zeros(s, dtype=torch.bfloat16, device="cuda") for s in ((2, 64, 64), (2, 64, 32))]
     bufs = native.Mx4Buffers(perm, act, y)
-    one = native.Mx4Buffers(native.Permutation.allocate(1, 2, "cuda"), act[:1], y[:1])
+    one = native.Mx4Buffers(native.Permutation.allocate(1, 2, "cuda"), layer.act_buffer(1, True), y[:1])
+    whole = native.Mx4Buffers(native.Permutation.allocate(1, 2, "cuda"), act[:1], y[:1])
     out = torch.empty((4, 64), dtype=torch.bfloat16, device="cuda")
     layer_call = lambda x=layer.x, w=w, ids=ids, b=bufs, w13=layer.w13, w2=layer.w2, l2p=None, o=out, **kw: \
         native.mx4_fused_moe(x, w, ids, w13, w2, l2p, b, o, block_m=32, **kw)
@@ -515,6 +533,10 @@ def test_empty_batches_and_refusals():
         lambda: layer_call(l2p=torch.zeros(2, device="cuda")),
         lambda: layer_call(add=out.float()),
         lambda: native.mx4_decode_one(layer.x, w, ids, layer.w13, layer.w2, None, bufs, out),
+        lambda: native.mx4_decode_one(layer.x[:1], w[:1], ids[:1], layer.w13, layer.w2, None, whole, out[:1]),
+        lambda: native.gateup_silu(layer.x, 1, layer.w13, perm, layer.act_buffer(3, True)),
+        lambda: native.down(torch.zeros((4, 3, 32), dtype=torch.bfloat16, device="cuda"), layer.w2, perm, y),
+        lambda: native.gateup_silu(x8, 1, layer.w13, perm, layer.act_buffer(4, True)),
         lambda: native.Mx4Buffers(perm, act[:2], y),
         lambda: native.Mx4Buffers(perm, act, y.half()),
         lambda: fused_moe.decode_layer(layer.x, bf[0][0, :16, :].contiguous(), fused_moe.RouterSpec(top_k=1), layer.w13,
@@ -532,6 +554,9 @@ def test_empty_batches_and_refusals():
                              path=native.LMOE_PATH_MFMA)
     with pytest.raises(RuntimeError, match="unsupported option"):
         native.gateup_silu(layer.x, 1, layer.w13, perm, act, path=native.LMOE_PATH_STREAM)
+    native.permute(ids, perm, block_m=32)
+    with pytest.raises(RuntimeError, match="unsupported option"):            # two parts in row tiles
+        native.grouped_mlp(layer.x, 1, layer.w13, layer.w2, perm, layer.act_buffer(4, True), y, path=native.LMOE_PATH_MFMA)
 
 
 @pytest.mark.gpu
@@ -586,7 +611,7 @@ def test_a_slot_past_32_bits():
             assert torch.equal(*res)
         one = []
         for slots, a, b in ((P, b13, b2), (1, w13, w2)):
-            act = torch.empty((1, I), dtype=torch.bfloat16, device="cuda") if rows is x else \
+            act = torch.empty((1, 2, I), dtype=torch.bfloat16, device="cuda") if rows is x else \
                 native.Mx8Rows.allocate(1, I, "cuda")
             bufs = native.Mx4Buffers(native.Permutation.allocate(1, slots, "cuda"), act,
                                      torch.empty((1, H), dtype=torch.float32, device="cuda"))
@@ -666,3 +691,77 @@ def test_buffers_and_workspaces_of_another_kind_are_refused():
                  lambda: fused_moe._fused_experts_ws(layer.x, w, ids, layer.w13, layer.w2, None, workspace=ws)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,I,counts", [
+    (32, 32, [1]),
+    (64, 96, [8, 9, 1, 0, 16]),                    # a fragment for both parts, one for each
+    (160, 160, [17, 7, 33]),                       # several passes, K inside a fragment
+    (1024, 416, [2, 40, 24]),
+    (2048, 768, [3, 12]),
+])
+def test_act_in_two_parts(H, I, counts):
+    """Twice the bits between the products; a row's bits do not depend on the
+    rows beside it, and no path has other values than the formula's."""
+    native = _native()
+    rng = np.random.default_rng(H + I)
+    ids = _ids(counts, 3, rng)
+    layer = Layer(H, I, len(counts), len(ids), "bf16", 21)
+    for y_dtype in (torch.float32, torch.bfloat16):
+        perm, act, y = run_layer(layer, ids, 1, native.LMOE_PATH_GEMV, y_dtype=y_dtype, split=True)
+        torch.cuda.synchronize()
+        check_layer(layer, perm, 1, act, y, ids[:, 0])
+        assert torch.all(y[torch.from_numpy(ids[:, 0] < 0).cuda()] == -7.0)
+        assert torch.all(act[sum(counts):] == 7.0)
+    whole = run_layer(layer, ids, 1, native.LMOE_PATH_GEMV)[1]
+    assert torch.equal(act[:sum(counts), 0], whole[:sum(counts)])                # the high part is the rounded value
+    for t in (int(np.argmax(ids[:, 0] == s)) for s in range(len(counts)) if counts[s]):
+        one = Layer.__new__(Layer)
+        one.__dict__.update(layer.__dict__, x=layer.x[t:t + 1])
+        y1 = run_layer(one, ids[t:t + 1], 1, native.LMOE_PATH_GEMV, split=True)[2]
+        assert torch.equal(y1[0], y[t])
+
+
+@pytest.mark.gpu
+def test_act_in_two_parts_past_the_numbers():
+    """Values that overflow, or are none, keep the high part's."""
+    native = _native()
+    layer = Layer(64, 32, 1, 3, "bf16", 2)
+    layer.x[0] *= 3e36
+    layer.x[1, 5] = float("nan")
+    ids = np.zeros((3, 1), np.int32)
+    whole = run_layer(layer, ids, 1, native.LMOE_PATH_GEMV)[1]
+    _, act, y = run_layer(layer, ids, 1, native.LMOE_PATH_GEMV, split=True)
+    assert torch.equal(act[:, 0].view(torch.int16), whole.view(torch.int16))
+    assert torch.all(act[:, 1][~whole.isfinite()] == 0) and act[:, 1].isfinite().all()
+    assert not whole[0].isfinite().all() and y[1].isnan().all() and y[2].isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,k,E,H,I", [(1, 1, 4, 256, 128), (1, 2, 8, 512, 128), (2, 1, 4, 256, 128), (3, 4, 24, 1024, 416)])
+def test_few_tokens_lose_no_bits_between_the_products(T, k, E, H, I):
+    """out of few tokens: its own rounding and the sums', nothing of act's."""
+    from vllm_moe_offload_amd import fused_moe, native
+
+    for seed in range(4):
+        rng = np.random.default_rng(100 * seed + H)
+        ids = np.stack([rng.choice(E, k, replace=False) for _ in range(T)]).astype(np.int32)
+        layer = Layer(H, I, E, T, "bf16", seed)
+        assert native.mx4_path(T * k, E) == native.LMOE_PATH_GEMV
+        w = torch.empty((T, k), device="cuda").uniform_(0.05, 1).to(torch.bfloat16)
+        out = _f64(fused_moe.fused_experts(layer.x, w, to_dev_i32(ids), layer.w13, layer.w2, None))
+        for t in range(T):
+            want, slack = np.zeros(H), np.zeros(H)
+            for j in range(k):
+                v13, v2 = layer.v13[ids[t, j]], layer.v2[ids[t, j]]
+                gu, e = layer.xv[t] @ v13.T, sum_error(layer.xv[t:t + 1], v13, False)[0]
+                sg = gu[:I] / (1.0 + np.exp(-gu[:I]))
+                act = sg * gu[I:]
+                da = 1.1 * np.abs(gu[I:]) * e[:I] + np.abs(sg) * e[I:] + e[:I] * e[I:] + 2.0**-20 * np.abs(act)
+                da = da * (1 + 2.0**-16) + 2.0**-16 * np.abs(act)
+                wj = _f64(w)[t, j]
+                want += wj * (v2 @ act)
+                slack += wj * (np.abs(v2) @ da + 2.01 * sum_error((np.abs(act) + da)[None], v2, False)[0])
+                slack += 2 * k * 2.0**-24 * wj * (np.abs(v2) @ np.abs(act))
+            assert np.all(np.abs(out[t] - want) <= slack * (1 + 2.0**-8) + 2.0**-8 * np.abs(want))

@@ -140,23 +140,25 @@ def test_c_entries_check_their_arguments():
     rows = lambda x=P16, T=1, H=64, q=P16, s=P16: lib.lmoe_rows_to_mx8(x, T, H, q, s, N)
     assert rows(T=0, x=N, q=N, s=N) == 0 and rows(T=-1) == 1000 and rows(x=N) == 1000 and rows(q=N) == 1000
     assert rows(s=N) == 1000 and rows(H=40) == 1001 and rows(x=P16 + 2) == 1001 and rows(H=65536) == 1001
-    gu = lambda x=P16, xs=P16, T=2, H=64, I=32, k=2, w=P16, P=4, n=4, path=0, act=P16, as_=P16, bm=128: \
-        lib.lmoe_mx4_gateup_silu(x, xs, T, H, I, k, w, P, P16, P16, P16, P16, P16, n, bm, path, act, as_, N)
+    gu = lambda x=P16, xs=P16, T=2, H=64, I=32, k=2, w=P16, P=4, n=4, path=0, act=P16, as_=P16, bm=128, split=0: \
+        lib.lmoe_mx4_gateup_silu(x, xs, T, H, I, k, w, P, P16, P16, P16, P16, P16, n, bm, path, act, as_, split, N)
     assert gu(T=0, n=0, x=N, act=N) == 0
     assert gu(T=-1) == 1000 and gu(k=0) == 1000 and gu(n=5) == 1000 and gu(P=0) == 1000 and gu(x=N) == 1000
     assert gu(xs=N) == 1000 and gu(as_=N) == 1000 and gu(act=N) == 1000 and gu(w=N) == 1000
     assert gu(H=48) == 1001 and gu(I=48) == 1001 and gu(x=P16 + 8) == 1001 and gu(w=P16 + 4) == 1001
     assert gu(path=9) == 1003 and gu(path=3) == 1003
-    dn = lambda act=P16, as_=P16, H=64, I=32, w=P16, P=4, n=4, path=0, y=P16, bm=128: \
-        lib.lmoe_mx4_down(act, as_, H, I, w, P, P16, P16, P16, P16, P16, n, bm, path, y, 0, N)
+    assert gu(split=1) == 1000 and gu(split=1, xs=N, as_=N, path=2) == 1003  # two parts: bf16 rows, no row tiles
+    dn = lambda act=P16, as_=P16, H=64, I=32, w=P16, P=4, n=4, path=0, y=P16, bm=128, split=0: \
+        lib.lmoe_mx4_down(act, as_, split, H, I, w, P, P16, P16, P16, P16, P16, n, bm, path, y, 0, N)
     assert dn(n=0, act=N, y=N) == 0 and dn(n=-1) == 1000 and dn(act=N) == 1000 and dn(y=N) == 1000
     assert dn(H=48) == 1001 and dn(I=16) == 1001 and dn(y=P16 + 8) == 1001 and dn(path=9) == 1003
+    assert dn(split=1) == 1000 and dn(split=1, as_=N, path=2) == 1003
     from vllm_moe_offload_amd.native import _Mx4Workspace
     import ctypes
 
     def ws(**kw):
         v = {n: P16 for n, _ in _Mx4Workspace._fields_}
-        return _Mx4Workspace(**{**v, "y_f32": 1, **kw})
+        return _Mx4Workspace(**{**v, "y_f32": 1, "act_split": 0, **kw})
 
     def fused(x=P16, xs=P16, T=2, H=64, I=32, k=2, w13=P16, w2=P16, P=4, w=P16, ids=P16, path=0, bm=32, wsp=None,
               add=N, out=P16):
@@ -168,6 +170,7 @@ def test_c_entries_check_their_arguments():
     assert fused(T=-1) == 1000 and fused(k=0) == 1000 and fused(P=0) == 1000 and fused(x=N) == 1000 and fused(ids=N) == 1000
     assert fused(w=N) == 1000 and fused(out=N) == 1000 and fused(xs=N) == 1000 and fused(w13=N) == 1000 and fused(w2=N) == 1000
     assert fused(wsp=ws(act=None)) == 1000 and fused(wsp=ws(y=None)) == 1000 and fused(wsp=ws(act_scale=None)) == 1000
+    assert fused(wsp=ws(act_split=1)) == 1000
     assert fused(H=48) == 1001 and fused(I=40) == 1001 and fused(P=70000) == 1001 and fused(T=1 << 30, k=4) == 1001
     assert fused(x=P16 + 8) == 1001 and fused(add=P16 + 8) == 1001 and fused(out=P16 + 8) == 1001
     assert fused(path=2, bm=256) == 1001 and fused(path=2, bm=128, H=32 * 4096) == 1001 and fused(path=3) == 1003

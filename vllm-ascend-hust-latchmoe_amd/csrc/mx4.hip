@@ -63,8 +63,9 @@ template <bool GU>
 static void launch_few(const Mx4Args& g, hipStream_t stream) {
   constexpr int cols = kFewMxBlocks * (GU ? 8 : 16);
   const dim3 grid((g.N + cols - 1) / cols, g.n_pairs < g.P ? g.n_pairs : g.P);
-  if (g.a_scale != nullptr) mx4_few_kernel<GU, true><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
-  else mx4_few_kernel<GU, false><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
+  if (g.a_scale != nullptr) mx4_few_kernel<GU, true, false><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
+  else if (!GU && g.split) mx4_few_kernel<GU, false, !GU><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
+  else mx4_few_kernel<GU, false, false><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
 }
 
 // Row tiles of BM rows, at most n_pairs / BM + one short one per slot.
@@ -110,17 +111,18 @@ static int launch_tiles(const Mx4Args& g, int block_m, hipStream_t stream) {
 // path AUTO: row tiles past this many pairs per slot, on average (native.py has the figures)
 constexpr int kFewPairsPerSlot = 3;
 
-static bool takes_tiles(int path, int block_m, bool a8, int H, int I, int n_pairs, int P) {
+static bool takes_tiles(int path, int block_m, bool a8, int H, int I, int n_pairs, int P, bool split) {
   if (path != LMOE_PATH_AUTO) return path == LMOE_PATH_MFMA;
-  return known_block_m(block_m) && n_pairs > static_cast<long long>(kFewPairsPerSlot) * P &&
+  return !split && known_block_m(block_m) && n_pairs > static_cast<long long>(kFewPairsPerSlot) * P &&
          tiles_fit(block_m, a8, H) && tiles_fit(block_m, a8, I);
 }
 
 template <bool GU>
 static int launch(const Mx4Args& g, int path, int block_m, hipStream_t stream) {
-  if (!takes_tiles(path, block_m, g.a_scale != nullptr, g.K, g.N, g.n_pairs, g.P)) {
+  if (!takes_tiles(path, block_m, g.a_scale != nullptr, g.K, g.N, g.n_pairs, g.P, g.split)) {
     launch_few<GU>(g, stream);
   } else {
+    if (g.split) return LMOE_ERR_UNSUPPORTED;
     if (!known_block_m(block_m) || !tiles_fit(block_m, g.a_scale != nullptr, g.K)) return LMOE_ERR_SHAPE;
     const int st = g.a_scale != nullptr ? launch_tiles<GU, true>(g, block_m, stream)
                                         : launch_tiles<GU, false>(g, block_m, stream);
@@ -142,7 +144,7 @@ extern "C" int lmoe_mx4_gateup_silu(const void* x, const void* x_scale, int T, i
                                     const void* w13_slots, int n_slots, const int32_t* offsets,
                                     const int32_t* sorted_pairs, const int32_t* active,
                                     const int32_t* tile_off, const int32_t* meta, int n_pairs,
-                                    int block_m, int path, void* act, void* act_scale,
+                                    int block_m, int path, void* act, void* act_scale, int act_split,
                                     hipStream_t stream) {
   if (T < 0 || H <= 0 || I <= 0 || k <= 0 || n_slots <= 0 || n_pairs < 0) return LMOE_ERR_ARG;
   if (n_pairs != static_cast<long long>(T) * k) return LMOE_ERR_ARG;
@@ -152,15 +154,15 @@ extern "C" int lmoe_mx4_gateup_silu(const void* x, const void* x_scale, int T, i
   if (x == nullptr || w13_slots == nullptr || offsets == nullptr || sorted_pairs == nullptr ||
       active == nullptr || tile_off == nullptr || meta == nullptr || act == nullptr)
     return LMOE_ERR_ARG;
-  if ((x_scale == nullptr) != (act_scale == nullptr)) return LMOE_ERR_ARG;
+  if ((x_scale == nullptr) != (act_scale == nullptr) || (act_scale != nullptr && act_split)) return LMOE_ERR_ARG;
   if (bad16(x) || bad16(w13_slots) || bad16(act)) return LMOE_ERR_SHAPE;
   const Mx4Args g{x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(w13_slots),
                   lmoe_mx4_bytes(2 * I, H), H, I, k, n_slots, n_pairs, offsets, sorted_pairs, active,
-                  tile_off, meta, act, static_cast<uint8_t*>(act_scale), false};
+                  tile_off, meta, act, static_cast<uint8_t*>(act_scale), false, act_split != 0};
   return launch<true>(g, path, block_m, stream);
 }
 
-extern "C" int lmoe_mx4_down(const void* act, const void* act_scale, int H, int I,
+extern "C" int lmoe_mx4_down(const void* act, const void* act_scale, int act_split, int H, int I,
                              const void* w2_slots, int n_slots, const int32_t* offsets,
                              const int32_t* sorted_pairs, const int32_t* active,
                              const int32_t* tile_off, const int32_t* meta, int n_pairs, int block_m,
@@ -170,12 +172,12 @@ extern "C" int lmoe_mx4_down(const void* act, const void* act_scale, int H, int 
   if (!known_path(path)) return LMOE_ERR_UNSUPPORTED;
   if (n_pairs == 0) return LMOE_OK;
   if (act == nullptr || w2_slots == nullptr || offsets == nullptr || sorted_pairs == nullptr ||
-      active == nullptr || tile_off == nullptr || meta == nullptr || y == nullptr)
+      active == nullptr || tile_off == nullptr || meta == nullptr || y == nullptr || (act_scale != nullptr && act_split))
     return LMOE_ERR_ARG;
   if (bad16(act) || bad16(w2_slots) || bad16(y)) return LMOE_ERR_SHAPE;
   const Mx4Args g{act, static_cast<const uint8_t*>(act_scale), static_cast<const uint8_t*>(w2_slots),
                   lmoe_mx4_bytes(H, I), I, H, 1, n_slots, n_pairs, offsets, sorted_pairs, active,
-                  tile_off, meta, y, nullptr, y_f32 != 0};
+                  tile_off, meta, y, nullptr, y_f32 != 0, act_split != 0};
   return launch<false>(g, path, block_m, stream);
 }
 
@@ -208,7 +210,7 @@ extern "C" int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int
   if (!known_path(path)) return LMOE_ERR_UNSUPPORTED;
   if (T > 0) {
     if (x == nullptr || w13_slots == nullptr || w2_slots == nullptr || ws->act == nullptr || ws->y == nullptr ||
-        (x_scale == nullptr) != (ws->act_scale == nullptr))
+        (x_scale == nullptr) != (ws->act_scale == nullptr) || (x_scale != nullptr && ws->act_split))
       return LMOE_ERR_ARG;
     if (bad16(x) || bad16(w13_slots) || bad16(w2_slots) || bad16(ws->act) || bad16(ws->y) || bad16(add) || bad16(out))
       return LMOE_ERR_SHAPE;
@@ -216,14 +218,16 @@ extern "C" int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int
                                    !tiles_fit(block_m, x_scale != nullptr, I)))
       return LMOE_ERR_SHAPE;
   }
+  const int split = ws->act_split && !takes_tiles(path, block_m, x_scale != nullptr, H, I, static_cast<int>(n), n_slots, false);
   int st = lmoe_permute(ids, static_cast<int>(n), log2phy, n_log2phy, n_slots, 0, block_m, ws->counts, ws->offsets,
                         ws->sorted_pairs, ws->row_idx, ws->active, ws->tile_off, ws->meta, ws->permute_workspace,
                         ws->permute_workspace_bytes, stream);
   if (st != LMOE_OK || T == 0) return st;
   st = lmoe_mx4_gateup_silu(x, x_scale, T, H, I, k, w13_slots, n_slots, ws->offsets, ws->sorted_pairs, ws->active,
-                            ws->tile_off, ws->meta, static_cast<int>(n), block_m, path, ws->act, ws->act_scale, stream);
+                            ws->tile_off, ws->meta, static_cast<int>(n), block_m, path, ws->act, ws->act_scale, split,
+                            stream);
   if (st != LMOE_OK) return st;
-  st = lmoe_mx4_down(ws->act, ws->act_scale, H, I, w2_slots, n_slots, ws->offsets, ws->sorted_pairs, ws->active,
+  st = lmoe_mx4_down(ws->act, ws->act_scale, split, H, I, w2_slots, n_slots, ws->offsets, ws->sorted_pairs, ws->active,
                      ws->tile_off, ws->meta, static_cast<int>(n), block_m, path, ws->y, ws->y_f32, stream);
   if (st != LMOE_OK) return st;
   return ws->y_f32 ? lmoe_combine_f32(ws->y, ws->row_idx, w, T, k, H, add, out, stream)
@@ -251,10 +255,10 @@ extern "C" int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, in
   down.w_b = static_cast<const uint8_t*>(w2_b);
   const Mx4Args gu{x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(w13_slots),
                    lmoe_mx4_bytes(2 * I, H), H, I, k, n_slots, k, nullptr, nullptr, nullptr, nullptr, nullptr, act,
-                   static_cast<uint8_t*>(act_scale), false};
+                   static_cast<uint8_t*>(act_scale), false, x_scale == nullptr};
   const Mx4Args dn{act, static_cast<const uint8_t*>(act_scale), static_cast<const uint8_t*>(w2_slots),
                    lmoe_mx4_bytes(H, I), I, H, 1, n_slots, k, nullptr, nullptr, nullptr, nullptr, nullptr, out, nullptr,
-                   false};
+                   false, x_scale == nullptr};
   const dim3 grid(I / 32, k);
   const uint16_t* a = static_cast<const uint16_t*>(add);
   if (x_scale != nullptr) {

@@ -50,6 +50,7 @@ struct Mx4Args {
   void* out;                // act rows, or y rows by pair
   uint8_t* out_scale;       // act rows in MX8
   bool out_f32;             // y in f32
+  bool split;               // bf16 act rows in two parts, [.., 2, I]
 };
 
 // One row's share of a 16 x 128 fragment: this lane's 32 values.
@@ -155,7 +156,7 @@ __device__ __forceinline__ void store_act(const Mx4Args& g, int pos, int i0, int
   for (int p = 0; p < 2; ++p)
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[p][e] = silu_f32(gate[p][e]) * up[p][e];
-  const size_t row = static_cast<size_t>(pos) * g.N;
+  size_t row = static_cast<size_t>(pos) * g.N;
   if constexpr (A8) {
     uint32_t m = 0;
 #pragma unroll
@@ -178,8 +179,21 @@ __device__ __forceinline__ void store_act(const Mx4Args& g, int pos, int i0, int
         g.out_scale[static_cast<size_t>(pos) * (g.N / kMxGroup) + i0 / kMxGroup] = static_cast<uint8_t>(byte);
     }
   } else {
-    store_bf16x8(static_cast<uint16_t*>(g.out) + row + i0, lane, live, f32x4_t{v[0][0], v[0][1], v[0][2], v[0][3]},
+    if (g.split) row *= 2;
+    uint16_t* out = static_cast<uint16_t*>(g.out) + row + i0;
+    store_bf16x8(out, lane, live, f32x4_t{v[0][0], v[0][1], v[0][2], v[0][3]},
                  f32x4_t{v[1][0], v[1][1], v[1][2], v[1][3]});
+    if (g.split) {  // what the rounding left, none of what is not finite
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float hi = bf16lo(pack_bf16x2(v[p][e], 0.0f));
+          v[p][e] = fabsf(hi) < __builtin_inff() ? v[p][e] - hi : 0.0f;
+        }
+      store_bf16x8(out + g.N, lane, live, f32x4_t{v[0][0], v[0][1], v[0][2], v[0][3]},
+                   f32x4_t{v[1][0], v[1][1], v[1][2], v[1][3]});
+    }
   }
 }
 
@@ -207,6 +221,20 @@ constexpr int kFewMxWaves = 4;
 constexpr int kOneMxWaves = 8;
 constexpr int kFewMxBlocks = 4;  // 16-row weight blocks of a workgroup
 constexpr int kFewMxRows = 32;   // rows of one pass over a slot's weights
+
+// act rows of a few tokens are kept in two bf16 parts, high and low, 16 bits in all:
+// where one token's output hangs on a few act values, their rounding to bf16 does not
+// average out (one token's error against 64 bits was 1.4 to 1.6 times that of the
+// output's own rounding).  Up to eight rows the parts are rows r and r + 8 of one
+// fragment, which multiplies sixteen rows anyway; past that they are two fragments,
+// sixteen rows a pass.  The parts' sums are added last, so a row's bits are the same.
+constexpr int kFewMxSplitRows = 16;
+
+// the other half of sixteen lanes: lane l from lane l ^ 8
+__device__ __forceinline__ f32x4_t other_part(const f32x4_t v) {
+  return f32x4_t{dpp_f32<kDppRowRor8>(v[0]), dpp_f32<kDppRowRor8>(v[1]), dpp_f32<kDppRowRor8>(v[2]),
+                 dpp_f32<kDppRowRor8>(v[3])};
+}
 
 // Chunks [c0, c1) of RB weight blocks by NF row fragments, U chunks' loads at a time.
 // (blocks: how many of the RB there are; the last stands in for the others)
@@ -244,8 +272,8 @@ __device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int bloc
 }
 
 // NF 16-row fragments of rows [p0, p0 + rows) of one slot.  ONE: the one token's
-// row p0, whose pairs keep their order.
-template <bool GU, bool A8, int NF, int NW, bool ONE>
+// row p0, whose pairs keep their order.  SP: rows in two parts, see above.
+template <bool GU, bool A8, int NF, int NW, bool ONE, bool SP>
 __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, int blocks, int cb, int p0, int rows,
                                          f32x4_t* s_part) {
   constexpr int RB = kFewMxBlocks;
@@ -256,9 +284,10 @@ __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, 
   const uint8_t* row_scale[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
-    const int r = 16 * f + (lane & 15);
+    const int r = !SP ? 16 * f + (lane & 15) : NF == 1 ? lane & 7 : lane & 15;
     const int pos = p0 + (r < rows ? r : 0);
-    const size_t src = ONE ? 0 : GU ? g.sorted_pairs[pos] / g.topk : pos;
+    size_t src = ONE ? 0 : GU ? g.sorted_pairs[pos] / g.topk : pos;
+    if constexpr (SP) src = 2 * src + (NF == 1 ? (lane >> 3) & 1 : f);
     row[f] = static_cast<const char*>(g.a) + src * g.K * (A8 ? 1 : 2);
     row_scale[f] = A8 ? g.a_scale + src * (g.K / kMxGroup) : nullptr;
   }
@@ -270,6 +299,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, 
   few_chunks<A8, RB, NF, ONE ? 2 : 1>(wblk, mx4_block_bytes(g.K), blocks, g.K, wave * chunks / NW, (wave + 1) * chunks / NW,
                             lane, row, row_scale, acc);
   // partial sums of a fragment, [wave][block][lane], added in wave order
+  f32x4_t high[2];
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
     if (f > 0) __syncthreads();  // the last fragment's sums have been read
@@ -287,8 +317,22 @@ __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, 
 #pragma unroll
       for (int v = 1; v < NW; ++v) t[b] += s_part[(v * RB + b0 + b) * 64 + lane];
     }
-    const int r = 16 * f + (lane & 15);
-    const bool live = r < rows;
+    if constexpr (SP) {
+      if constexpr (NF == 1) {
+        t[0] += other_part(t[0]);
+        t[1] += other_part(t[1]);
+      } else {
+        if (f == 0) {
+          high[0] = t[0];
+          high[1] = t[1];
+          continue;
+        }
+        t[0] = high[0] + t[0];
+        t[1] = high[1] + t[1];
+      }
+    }
+    const int r = SP ? lane & 15 : 16 * f + (lane & 15);
+    const bool live = r < rows;  // of eight rows at most, those in the lower lanes
     if constexpr (GU) {
       const f32x4_t gate[2] = {t[0], t[2]}, up[2] = {t[1], t[3]};
       store_act<A8>(g, p0 + r, cb * 32, lane, live, gate, up);
@@ -299,7 +343,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, 
 }
 
 // (column block, active slot) of a grid of [ceil(N / 32 or 64), slots]
-template <bool GU, bool A8>
+template <bool GU, bool A8, bool SP>
 __global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g) {
   __shared__ f32x4_t s_part[kFewMxWaves * kFewMxBlocks * 64];
   const int slot = g.active[blockIdx.y];
@@ -308,11 +352,12 @@ __global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g) {
   const int cb = blockIdx.x;
   const int blocks = min(kFewMxBlocks, (GU ? 2 * g.N : g.N) / 16 - cb * kFewMxBlocks);
   const uint8_t* wblk = g.w + slot * g.w_slot_bytes + static_cast<size_t>(cb) * kFewMxBlocks * mx4_block_bytes(g.K);
-  for (int p = p0; p < p1; p += kFewMxRows) {
-    const int rows = min(kFewMxRows, p1 - p);
+  constexpr int PASS = SP ? kFewMxSplitRows : kFewMxRows;
+  for (int p = p0; p < p1; p += PASS) {
+    const int rows = min(PASS, p1 - p);
     if (p > p0) __syncthreads();  // the last pass's sums have been read
-    if (rows > 16) few_rows<GU, A8, 2, kFewMxWaves, false>(g, wblk, blocks, cb, p, rows, s_part);
-    else few_rows<GU, A8, 1, kFewMxWaves, false>(g, wblk, blocks, cb, p, rows, s_part);
+    if (rows > PASS / 2) few_rows<GU, A8, 2, kFewMxWaves, false, SP>(g, wblk, blocks, cb, p, rows, s_part);
+    else few_rows<GU, A8, 1, kFewMxWaves, false, SP>(g, wblk, blocks, cb, p, rows, s_part);
   }
 }
 
@@ -361,12 +406,13 @@ __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_gateup_kernel(Mx4Arg
   if (expert == nullptr) return;
   const int cb = blockIdx.x;
   const uint8_t* wblk = expert + static_cast<size_t>(cb) * kFewMxBlocks * mx4_block_bytes(g.K);
-  few_rows<true, A8, 1, kOneMxWaves, true>(g, wblk, kFewMxBlocks, cb, j, 1, s_part);
+  few_rows<true, A8, 1, kOneMxWaves, true, false>(g, wblk, kFewMxBlocks, cb, j, 1, s_part);
 }
 
 // 16 columns of out = add + sum_j w_j W2_j act_j.  The waves take (pair, part of K)
 // units in turn, each adding its units' weighted sums; the waves' sums are added in
-// order.  A unit is the whole K of a pair where there are eight pairs or more.
+// order.  A unit is the whole K of a pair where there are eight pairs or more.  bf16
+// rows come in two parts, the fragment's lower and upper rows.
 template <bool A8>
 __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_down_kernel(Mx4Args g, OneToken o,
                                                                        const uint16_t* __restrict__ wts,
@@ -388,7 +434,8 @@ __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_down_kernel(Mx4Args 
       continue;
     }
     const float wj = bf16_to_f32(wts[j]);
-    const char* row[1] = {static_cast<const char*>(g.a) + static_cast<size_t>(j) * g.K * (A8 ? 1 : 2)};
+    const size_t src = A8 ? j : 2 * j + ((lane >> 3) & 1);
+    const char* row[1] = {static_cast<const char*>(g.a) + src * g.K * (A8 ? 1 : 2)};
     const uint8_t* row_scale[1] = {A8 ? g.a_scale + static_cast<size_t>(j) * (g.K / kMxGroup) : nullptr};
     f32x4_t acc[1][1] = {{f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}}};
     const uint8_t* wblk = expert + static_cast<size_t>(blockIdx.x) * bb;
@@ -396,6 +443,7 @@ __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_down_kernel(Mx4Args 
                             acc);
     sum += wj * acc[0][0];
   }
+  if constexpr (!A8) sum += other_part(sum);
   // the sixteen rows of the fragment are the same row: lanes 0, 16, 32 and 48 have it
   if ((lane & 15) == 0) s_part[wave * 4 + (lane >> 4)] = sum;
   __syncthreads();

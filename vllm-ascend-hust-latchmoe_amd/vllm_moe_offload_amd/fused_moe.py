@@ -48,11 +48,18 @@ from vllm_moe_offload_amd.moe_offload.slot_mapping import PreparedSlotWeights
 @dataclass
 class MoEWorkspace:
     perm: native.Permutation
-    act: torch.Tensor   # [N, I] bf16 (or Mx8Rows), sorted order
+    act: torch.Tensor   # [N, I] bf16 (or Mx8Rows, or bf16 [N, 2, I] in two parts), sorted order
     y: torch.Tensor     # [N, H] bf16 (or f32), flat pair order
     out: torch.Tensor   # [T, H] bf16
     perm_overflow: native.Permutation | None = None  # the decode overflow pass's permutation
     mx4: native.Mx4Buffers | None = None  # the buffers as the calls over 4-bit banks take them
+
+    def act_rows(self, n: int, path: int):
+        """act of n pairs as a path takes it: two parts on LMOE_PATH_GEMV only."""
+        if isinstance(self.act, native.Mx8Rows) or self.act.dim() == 2 or path == native.LMOE_PATH_GEMV:
+            return self.act[:n]
+        I = self.act.shape[-1]
+        return self.act.view(-1)[: n * I].view(n, I)
 
     def overflow_perm(self, n_pairs: int, n_slots: int, device) -> native.Permutation:
         p = self.perm_overflow
@@ -77,19 +84,20 @@ def rows_kind(hidden, w13_slots) -> str:
 
 def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = "", rows: str = "") -> MoEWorkspace:
     """The workspace of a layer shape.  rows: rows_kind of its experts.  4-bit
-    experts' rows of a few tokens stay f32 until the combine (their bytes are
-    few beside the weights')."""
+    experts' rows of a few tokens stay f32 until the combine, and bf16 act rows
+    are in two parts (their bytes are few beside the weights')."""
     if rows not in ("", "bf16", "mx8"):
         raise ValueError(f"unknown rows {rows!r}")
     key = (int(T), int(k), int(P), int(H), int(I), str(device), tag, rows)
     ws = _WORKSPACES.get(key)
     if ws is None:
         N = T * k
-        y_dtype = torch.float32 if rows and N <= native.FUSED_DECODE_MAX_PAIRS else torch.bfloat16
+        few = rows != "" and N <= native.FUSED_DECODE_MAX_PAIRS
+        y_dtype = torch.float32 if few else torch.bfloat16
         ws = MoEWorkspace(
             perm=native.Permutation.allocate(N, P, device),
             act=native.Mx8Rows.allocate(max(N, 1), I, device) if rows == "mx8" else
-            torch.empty((max(N, 1), I), dtype=torch.bfloat16, device=device),
+            torch.empty((max(N, 1), 2, I) if few else (max(N, 1), I), dtype=torch.bfloat16, device=device),
             y=torch.empty((max(N, 1), H), dtype=y_dtype, device=device),
             out=torch.empty((max(T, 1), H), dtype=torch.bfloat16, device=device),
         )
@@ -272,7 +280,7 @@ def _overflow_pass(hidden, topk_ids, k: int, overflow: PreparedSlotWeights, ws: 
     rows of y."""
     T = hidden.shape[0]
     perm = _overflow_permute(hidden, topk_ids, k, overflow, ws, path=path)
-    native.grouped_mlp(hidden, k, overflow.w1, overflow.w2, perm, ws.act[: T * k], ws.y[: T * k], path=path)
+    native.grouped_mlp(hidden, k, overflow.w1, overflow.w2, perm, ws.act_rows(T * k, path), ws.y[: T * k], path=path)
 
 
 def _merged_passes(hidden, k: int, w13_slots, overflow: PreparedSlotWeights, path: int) -> bool:
@@ -352,10 +360,10 @@ def _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2p
         if merged:
             _two_passes(hidden, k, w13_slots, w2_slots, overflow, ws, perm_b, path=path)
         else:
-            native.gateup_silu(hidden, k, w13_slots, ws.perm, ws.act[: T * k], path=path)
+            native.gateup_silu(hidden, k, w13_slots, ws.perm, ws.act_rows(T * k, path), path=path)
             if events:
                 events[1].record()
-            native.down(ws.act[: T * k], w2_slots, ws.perm, ws.y[: T * k], path=path)
+            native.down(ws.act_rows(T * k, path), w2_slots, ws.perm, ws.y[: T * k], path=path)
             _overflow_pass(hidden, topk_ids, k, overflow, ws, path=path)
             if events:
                 events[2].record()
@@ -368,10 +376,10 @@ def _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2p
         native.fused_moe_decode(hidden, topk_weights, w13_slots, w2_slots, ws.perm, ws.act[: T * k], dst, add=add,
                                 y=ws.y[: T * k], distinct_slots=False)
     else:
-        native.gateup_silu(hidden, k, w13_slots, ws.perm, ws.act[: T * k], path=path)
+        native.gateup_silu(hidden, k, w13_slots, ws.perm, ws.act_rows(T * k, path), path=path)
         if events:
             events[1].record()
-        native.down(ws.act[: T * k], w2_slots, ws.perm, ws.y[: T * k], path=path)
+        native.down(ws.act_rows(T * k, path), w2_slots, ws.perm, ws.y[: T * k], path=path)
         if events:
             events[2].record()
         native.combine(ws.y[: T * k], topk_weights, dst, row_mask=ws.perm.row_idx[: T * k], add=add)
@@ -470,7 +478,7 @@ def decode_layer(
         if merged:
             _two_passes(rows, kw, w13_slots, w2_slots, overflow, ws, perm_b, path=path)
         else:
-            native.grouped_mlp(rows, kw, w13_slots, w2_slots, ws.perm, ws.act[: T * kw], ws.y[: T * kw], path=path)
+            native.grouped_mlp(rows, kw, w13_slots, w2_slots, ws.perm, ws.act_rows(T * kw, path), ws.y[: T * kw], path=path)
             _overflow_pass(rows, ids, kw, overflow, ws, path=path)
         native.combine(ws.y[: T * kw], w, dst, row_mask=ws.perm.row_idx[: T * kw], add=add)
         return dst, w, ids
@@ -479,7 +487,7 @@ def decode_layer(
         native.fused_moe_decode(rows, w, w13_slots, w2_slots, ws.perm, ws.act[: T * kw], dst, add=add,
                                 y=ws.y[: T * kw], distinct_slots=True)
     else:
-        native.grouped_mlp(rows, kw, w13_slots, w2_slots, ws.perm, ws.act[: T * kw], ws.y[: T * kw], path=path)
+        native.grouped_mlp(rows, kw, w13_slots, w2_slots, ws.perm, ws.act_rows(T * kw, path), ws.y[: T * kw], path=path)
         native.combine(ws.y[: T * kw], w, dst, row_mask=ws.perm.row_idx[: T * kw], add=add)
     return dst, w, ids
 
@@ -814,7 +822,7 @@ def run_wave_prefill(
                                block_m=_pass_block_m(len(plan.waves[w]), H, I, hidden.device, T * k, mlp_path, pairs,
                                                      mx4=mxfp4.is_mx4(prepared.w1)))
                 first = False
-                native.grouped_mlp(hidden, k, prepared.w1, prepared.w2, ws.perm, ws.act[: T * k], ws.y[: T * k],
+                native.grouped_mlp(hidden, k, prepared.w1, prepared.w2, ws.perm, ws.act_rows(T * k, mlp_path), ws.y[: T * k],
                                    path=mlp_path, pass_pairs=pairs)
             finally:
                 runtime.end_slot_compute(handle)
@@ -1004,7 +1012,7 @@ def run_device_waves(
         ready.record(tx)
         compute.wait_event(ready)
         native.permute(topk_ids, ws.perm, log2phy=table, skip_unmapped=True, keep_rows=w > 0, block_m=bm)
-        native.grouped_mlp(hidden, k, stage.w13_slots, stage.w2_slots, ws.perm, ws.act[: T * k], ws.y[: T * k],
+        native.grouped_mlp(hidden, k, stage.w13_slots, stage.w2_slots, ws.perm, ws.act_rows(T * k, mlp_path), ws.y[: T * k],
                            path=mlp_path, pass_pairs=pairs)
         done = torch.cuda.Event()
         done.record(compute)

@@ -154,11 +154,11 @@ _SIGNATURES = {
     "lmoe_mx4_bytes": (ctypes.c_longlong, [_i, _i]),
     "lmoe_mx4_gateup_silu": (
         _i,
-        [_vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp],
+        [_vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp],
     ),
     "lmoe_mx4_down": (
         _i,
-        [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _vp],
+        [_vp, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _vp],
     ),
     "lmoe_mx4_fused_moe": (
         _i,
@@ -1139,7 +1139,9 @@ def grouped_mlp(
     pass_pairs: how many of the pairs the pass is expected to place, where it
     is one wave of its layer (chooses the kernel's form, not its bits).
     4-bit banks (mxfp4.pack_experts; uint8): x and act are both bf16 or both
-    Mx8Rows, y is bf16 or f32."""
+    Mx8Rows, y is bf16 or f32.  On path LMOE_PATH_GEMV (which AUTO then is) a
+    bf16 act may be [N, 2, I]: rows in two parts whose sum is the value, so that
+    its rounding does not show in batches of few tokens."""
     if mxfp4.is_mx4(w13_slots) or mxfp4.is_mx4(w2_slots):
         if x.shape[1] != w2_slots.shape[1]:
             raise ValueError(f"rows of {x.shape[1]} columns, w2_slots of {w2_slots.shape[1]} rows")
@@ -1241,6 +1243,16 @@ def _need_rows(rows, name: str, shape: tuple | None = None) -> tuple[torch.Tenso
     return rows, None
 
 
+def _need_act(act, n: int) -> tuple[torch.Tensor, torch.Tensor | None, bool]:
+    """act rows of n pairs: (values, scales or None, bf16 in two parts)."""
+    split = not isinstance(act, Mx8Rows) and act.dim() == 3
+    if not split:
+        return *_need_rows(act, "act", (n, act.shape[-1])), False
+    if not _is(act, torch.bfloat16, (n, 2, act.shape[-1])):
+        _need(act, "act", torch.bfloat16, (n, 2, act.shape[-1]))
+    return act, None, True
+
+
 def _need_y(y, shape: tuple) -> bool:
     """bf16 or f32 rows by pair; whether they are f32."""
     if not isinstance(y, torch.Tensor) or y.dtype not in (torch.bfloat16, torch.float32):
@@ -1256,8 +1268,8 @@ def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, 
     n = perm.n_pairs
     if n != T * top_k:
         raise ValueError("permutation does not match T * top_k pairs")
-    aq, as_ = _need_rows(act, "act", (n, act.shape[-1]))
-    I = aq.shape[1]
+    aq, as_, split = _need_act(act, n)
+    I = aq.shape[-1]
     if (xs is None) != (as_ is None):
         raise ValueError("x and act must both be bf16 or both be Mx8Rows")
     _need_mx4(w13_slots, "w13_slots", perm, H, 2 * I)
@@ -1267,7 +1279,7 @@ def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, 
         load_library().lmoe_mx4_gateup_silu(
             xq.data_ptr(), _ptr(xs), T, H, I, top_k, w13_slots.data_ptr(), p.n_slots, p.offsets.data_ptr(),
             p.sorted_pairs.data_ptr(), p.active.data_ptr(), p.tile_off.data_ptr(), p.meta.data_ptr(), n, p.block_m, path,
-            aq.data_ptr(), _ptr(as_), _stream(stream),
+            aq.data_ptr(), _ptr(as_), split, _stream(stream),
         ),
         "lmoe_mx4_gateup_silu",
     )
@@ -1276,15 +1288,15 @@ def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, 
 
 def _mx4_down(act, w2_slots: torch.Tensor, perm: Permutation, y: torch.Tensor, *, path: int, stream):
     n = perm.n_pairs
-    aq, as_ = _need_rows(act, "act", (n, act.shape[-1]))
-    I = aq.shape[1]
+    aq, as_, split = _need_act(act, n)
+    I = aq.shape[-1]
     H = _need_mx4(w2_slots, "w2_slots", perm, I, w2_slots.shape[1] if w2_slots.dim() == 3 else None)
     y_f32 = _need_y(y, (n, H))
     _same_device(aq, as_, w2_slots, perm.offsets, y)
     p = perm
     _check(
         load_library().lmoe_mx4_down(
-            aq.data_ptr(), _ptr(as_), H, I, w2_slots.data_ptr(), p.n_slots, p.offsets.data_ptr(),
+            aq.data_ptr(), _ptr(as_), split, H, I, w2_slots.data_ptr(), p.n_slots, p.offsets.data_ptr(),
             p.sorted_pairs.data_ptr(), p.active.data_ptr(), p.tile_off.data_ptr(), p.meta.data_ptr(), n, p.block_m, path,
             y.data_ptr(), y_f32, _stream(stream),
         ),
@@ -1298,15 +1310,17 @@ class _Mx4Workspace(ctypes.Structure):
 
     _fields_ = [(n, _vp) for n in ("counts", "offsets", "sorted_pairs", "row_idx", "active", "tile_off", "meta",
                                    "permute_workspace")] + \
-               [("permute_workspace_bytes", _sz), ("act", _vp), ("act_scale", _vp), ("y", _vp), ("y_f32", ctypes.c_int32)]
+               [("permute_workspace_bytes", _sz), ("act", _vp), ("act_scale", _vp), ("y", _vp), ("y_f32", ctypes.c_int32),
+                ("act_split", ctypes.c_int32)]
 
 
 class Mx4Buffers:
     """The buffers of a layer of 4-bit experts (lmoe_mx4_workspace): a permutation,
-    act (bf16 or Mx8Rows, [N, I]) and y (bf16 or f32, [N, H]), checked once."""
+    act (bf16 or Mx8Rows, [N, I]; bf16 [N, 2, I]: rows in two parts, where the
+    split-K kernel runs) and y (bf16 or f32, [N, H]), checked once."""
 
     def __init__(self, perm: Permutation, act, y: torch.Tensor) -> None:
-        aq, as_ = _need_rows(act, "act")
+        aq, as_, self.split = _need_act(act, act.shape[0])
         if y.dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("y must be bf16 or f32")
         _need(y, "y", y.dtype)
@@ -1320,14 +1334,14 @@ class Mx4Buffers:
                   perm.meta, perm.workspace):
             if t is not None and t.get_device() != self.device_index:
                 raise ValueError(f"a buffer on {t.device}, y on {y.device}")
-        self.hidden, self.intermediate = int(y.shape[1]), int(aq.shape[1])
+        self.hidden, self.intermediate = int(y.shape[1]), int(aq.shape[-1])
         self.mx8 = as_ is not None
         self.act_ptr, self.act_scale_ptr = _ptr(aq), _ptr(as_)
         p = perm
         self._struct = _Mx4Workspace(
             _ptr(p.counts), _ptr(p.offsets), _ptr(p.sorted_pairs), _ptr(p.row_idx), _ptr(p.active), _ptr(p.tile_off),
             _ptr(p.meta), _ptr(p.workspace), int(p.workspace.numel()), _ptr(aq), _ptr(as_), _ptr(y),
-            int(y.dtype == torch.float32))
+            int(y.dtype == torch.float32), int(self.split))
         self.address = ctypes.addressof(self._struct)
 
 
@@ -1397,6 +1411,8 @@ def mx4_decode_one(x, topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_sl
     xq, xs, T, k, n_table = _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, bufs, out, add)
     if T != 1:
         raise ValueError(f"one token, got {T}")
+    if xs is None and not bufs.split:
+        raise ValueError("one token's bf16 act rows are in two parts, [k, 2, I]")
     b13 = b2 = tab = None
     n_slots_b = n_table_b = 0
     if second is not None:
