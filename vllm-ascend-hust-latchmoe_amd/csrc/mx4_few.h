@@ -228,6 +228,9 @@ constexpr int kFewMxRows = 32;   // rows of one pass over a slot's weights
 // output's own rounding).  Up to eight rows the parts are rows r and r + 8 of one
 // fragment, which multiplies sixteen rows anyway; past that they are two fragments,
 // sixteen rows a pass.  The parts' sums are added last, so a row's bits are the same.
+// Row tiles keep one bf16 part: many rows average their roundings (the error is then
+// 1.41 times the output's own rounding, 1.35 to 1.46 over 160 layers of 9 to 200
+// tokens), and two would double the down product, which the matrix units bound there.
 constexpr int kFewMxSplitRows = 16;
 
 // the other half of sixteen lanes: lane l from lane l ^ 8
