@@ -398,7 +398,8 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
   const uint64_t v = reinterpret_cast<uint64_t>(p);
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
-  return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
+  typedef const __attribute__((address_space(1))) uint8_t* global_t;  // not flat loads
+  return (const uint8_t*)(global_t)(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 template <bool A8>
