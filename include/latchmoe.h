@@ -505,6 +505,19 @@ int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int H, int I,
                        int block_m, const lmoe_mx4_workspace* ws,
                        const void* add, void* out, hipStream_t stream);
 
+/* Few tokens through 4-bit experts without a permutation (T*k <= 64): the
+ * split-K kernels find each slot's pairs from the ids.  act rows and y rows
+ * ([T*k, H] f32) lie by pair (bf16 rows: act is [T*k, 2, I], as with act_split),
+ * those of pairs without a slot untouched; out has the bits of
+ * lmoe_mx4_fused_moe with path GEMV, act_split and f32 y.  A pair whose id maps
+ * to no slot adds nothing and is counted in LMOE_FLAG_UNPLACED. */
+int lmoe_mx4_decode_few(const void* x, const void* x_scale, int T, int H, int I,
+                        int k, const void* w13_slots, const void* w2_slots,
+                        int n_slots, const uint16_t* w, const int32_t* ids,
+                        const int32_t* log2phy, int n_log2phy, const void* add,
+                        void* act, void* act_scale, void* y, void* out,
+                        hipStream_t stream);
+
 /* One token (x [H], ids and w [k]) through 4-bit experts without a permutation,
  * in two launches: act[j] of pair j as lmoe_mx4_gateup_silu has it (bf16 rows with
  * act_split; rows of pairs without a slot untouched), then out = add +

@@ -765,3 +765,80 @@ def test_few_tokens_lose_no_bits_between_the_products(T, k, E, H, I):
                 slack += wj * (np.abs(v2) @ da + 2.01 * sum_error((np.abs(act) + da)[None], v2, False)[0])
                 slack += 2 * k * 2.0**-24 * wj * (np.abs(v2) @ np.abs(act))
             assert np.all(np.abs(out[t] - want) <= slack * (1 + 2.0**-8) + 2.0**-8 * np.abs(want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("T,k,E,H,I", [
+    (2, 1, 3, 32, 32),
+    (5, 3, 40, 160, 96),
+    (21, 3, 5, 96, 64),             # more pairs than slots
+    (3, 8, 200, 1024, 416),
+    (8, 8, 400, 64, 32),            # the most pairs
+    (64, 1, 2, 32, 32),             # several passes of rows
+])
+def test_few_tokens_straight_from_their_ids(T, k, E, H, I, rows):
+    """The permuted form's bits, of every pair and token; pairs without a slot add
+    nothing, are counted and leave their rows; one slot may serve several pairs."""
+    native = _native()
+    rng = np.random.default_rng(T * k)
+    ids = rng.integers(0, E, (T, k)).astype(np.int32)
+    ids[T // 2] = ids[T // 2, 0]                        # the same expert every time
+    if k > 1:
+        ids[T - 1, 1], ids[0, 1] = -1, E + 7            # outside the table
+    l2p = rng.permutation(E).astype(np.int32)
+    l2p[rng.integers(0, E)] = -1
+    layer = Layer(H, I, E, T, rows, T)
+    d_ids, d_l2p, n = to_dev_i32(ids), to_dev_i32(l2p), T * k
+    w = torch.empty((T, k), device="cuda").uniform_(0.05, 1).to(torch.bfloat16)
+    add = torch.randn((T, H), device="cuda").to(torch.bfloat16)
+    slots = np.where((ids >= 0) & (ids < E), l2p[np.clip(ids, 0, E - 1)], -1).flatten()
+    bits = lambda a: a.q.view(torch.uint8) if rows == "mx8" else a.view(torch.int16)
+    for addend, table in ((add, d_l2p), (None, d_l2p), (add, None)):
+        s = slots if table is not None else np.where((ids >= 0) & (ids < E), ids, -1).flatten()
+        res = []
+        for call in (native.mx4_fused_moe, native.mx4_decode_few):
+            bufs = native.Mx4Buffers(native.Permutation.allocate(n, E, "cuda"), layer.act_buffer(n, rows == "bf16"),
+                                     torch.full((n, H), -7.0, dtype=torch.float32, device="cuda"))
+            opt = dict(path=native.LMOE_PATH_GEMV, block_m=32) if call is native.mx4_fused_moe else {}
+            native.device_flags(clear=True)
+            out = call(layer.x, w, d_ids, layer.w13, layer.w2, table, bufs,
+                       torch.empty((T, H), dtype=torch.bfloat16, device="cuda"), add=addend, **opt)
+            flags = native.device_flags(clear=True)
+            assert flags[native.FLAG_UNPLACED] == int((s < 0).sum())
+            res.append((out, bufs))
+        (want, a), (got, b) = res
+        assert torch.equal(got, want) and torch.equal(b.y, a.y)
+        assert torch.all(b.y[torch.from_numpy(s < 0).cuda()] == -7.0)
+        pos = a.perm.row_idx.cpu().numpy()
+        placed = np.flatnonzero(s >= 0)
+        assert torch.equal(bits(b.act)[placed], bits(a.act)[pos[placed]])
+        left = np.flatnonzero(s < 0)
+        assert torch.equal(bits(b.act)[left], bits(layer.act_buffer(len(left), rows == "bf16")))
+
+
+@pytest.mark.gpu
+def test_few_tokens_refusals():
+    from vllm_moe_offload_amd import fused_moe, native
+
+    layer = Layer(64, 32, 400, 4, "bf16", 0)
+    w, ids = torch.ones((4, 1), dtype=torch.bfloat16, device="cuda"), torch.zeros((4, 1), dtype=torch.int32, device="cuda")
+    out = torch.empty((4, 64), dtype=torch.bfloat16, device="cuda")
+    perm = native.Permutation.allocate(4, 400, "cuda")
+    y = torch.empty((4, 64), dtype=torch.float32, device="cuda")
+    few = lambda b, i=ids: native.mx4_decode_few(layer.x, w, i, layer.w13, layer.w2, None, b, out)
+    for bufs in (native.Mx4Buffers(perm, layer.act_buffer(4), y), native.Mx4Buffers(perm, layer.act_buffer(4, True), y.bfloat16())):
+        with pytest.raises(ValueError):
+            few(bufs)
+    with pytest.raises(ValueError):
+        few(native.Mx4Buffers(perm, layer.act_buffer(4, True), y), ids.long())
+    # past the most pairs the layer's call takes the permuted form
+    big = Layer(64, 32, 400, 9, "bf16", 1)
+    ids8 = torch.randint(0, 400, (9, 8), dtype=torch.int32, device="cuda")
+    w8 = torch.full((9, 8), 0.1, dtype=torch.bfloat16, device="cuda")
+    bufs = native.Mx4Buffers(native.Permutation.allocate(72, 400, "cuda"), big.act_buffer(72, True),
+                             torch.empty((72, 64), dtype=torch.float32, device="cuda"))
+    o8 = torch.empty((9, 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="unsupported shape"):
+        native.mx4_decode_few(big.x, w8, ids8, big.w13, big.w2, None, bufs, o8)
+    assert fused_moe.fused_experts(big.x, w8, ids8, big.w13, big.w2, None).isfinite().all()

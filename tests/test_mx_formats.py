@@ -197,3 +197,19 @@ def test_norm_entries_refuse_shared_buffers():
     for t in (a, b, c, d):
         assert norm(q=t) == 1000, t
     assert lib.lmoe_rows_to_mx8(a, 1, 64, a, P16, N) == 1000
+
+
+def test_few_tokens_entry_checks_its_arguments():
+    from vllm_moe_offload_amd import native
+
+    lib = native.load_library()
+    few = lambda x=P16, xs=P16, T=2, H=64, I=32, k=2, w13=P16, w2=P16, P=4, w=P16, ids=P16, n=0, add=N, act=P16, as_=P16, \
+        y=P16, out=P16: lib.lmoe_mx4_decode_few(x, xs, T, H, I, k, w13, w2, P, w, ids, N, n, add, act, as_, y, out, N)
+    assert few(T=0, x=N, y=N, out=N) == 0
+    assert few(T=-1) == 1000 and few(k=0) == 1000 and few(P=0) == 1000 and few(n=-1) == 1000 and few(H=0) == 1000
+    for t in ("x", "xs", "w13", "w2", "w", "ids", "act", "as_", "y", "out"):
+        assert few(**{t: N}) == 1000, t
+    assert few(H=48) == 1001 and few(I=40) == 1001 and few(P=70000) == 1001 and few(T=33) == 1001
+    assert few(T=1 << 30, k=1 << 30) == 1001
+    for t in ("x", "w13", "w2", "act", "y", "out", "add"):
+        assert few(**{t: P16 + 8}) == 1001, t

@@ -19,8 +19,9 @@ namespace lmoe {
 // ---------------------------------------------------------------------------
 constexpr int kCombineStep = 8;
 
+template <bool SCAN>  // SCAN: which pairs have a slot is looked up from their ids
 __global__ __launch_bounds__(64) void combine_f32_kernel(
-    const float* __restrict__ y, const int32_t* __restrict__ row_idx, const uint16_t* __restrict__ w,
+    const float* __restrict__ y, const int32_t* __restrict__ row_idx, TokenIds o, int P, const uint16_t* __restrict__ w,
     int topk, int H, const uint16_t* __restrict__ add, uint16_t* __restrict__ out) {
   const int t = blockIdx.x;
   const int h = (blockIdx.y * 64 + threadIdx.x) * 4;
@@ -35,7 +36,8 @@ __global__ __launch_bounds__(64) void combine_f32_kernel(
       const int j = j0 + jj;
       const bool in = j < topk;
       const int p = t * topk + (in ? j : 0);
-      use[jj] = in && (row_idx == nullptr || row_idx[p] >= 0);
+      if constexpr (SCAN) use[jj] = in && slot_of_id(o, P, o.ids[p]) >= 0;
+      else use[jj] = in && (row_idx == nullptr || row_idx[p] >= 0);
       if (in && !use[jj] && blockIdx.y == 0 && threadIdx.x == 0) add_device_flag(LMOE_FLAG_UNPLACED, 1);
       wj[jj] = bf16_to_f32(w[p]);
       v[jj] = *reinterpret_cast<const f32x4_t*>(y + static_cast<size_t>(p) * H + h);
@@ -59,13 +61,13 @@ constexpr int kMaxSlots = 65535;  // a grid dimension
 
 static bool bad16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
-template <bool GU>
-static void launch_few(const Mx4Args& g, hipStream_t stream) {
+template <bool GU, bool SCAN>
+static void launch_few(const Mx4Args& g, const TokenIds& o, hipStream_t stream) {
   constexpr int cols = kFewMxBlocks * (GU ? 8 : 16);
-  const dim3 grid((g.N + cols - 1) / cols, g.n_pairs < g.P ? g.n_pairs : g.P);
-  if (g.a_scale != nullptr) mx4_few_kernel<GU, true, false><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
-  else if (!GU && g.split) mx4_few_kernel<GU, false, !GU><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
-  else mx4_few_kernel<GU, false, false><<<grid, kFewMxWaves * 64, 0, stream>>>(g);
+  const dim3 grid((g.N + cols - 1) / cols, SCAN || g.n_pairs < g.P ? g.n_pairs : g.P);
+  if (g.a_scale != nullptr) mx4_few_kernel<GU, true, false, SCAN><<<grid, kFewMxWaves * 64, 0, stream>>>(g, o);
+  else if (!GU && g.split) mx4_few_kernel<GU, false, !GU, SCAN><<<grid, kFewMxWaves * 64, 0, stream>>>(g, o);
+  else if (GU || !SCAN) mx4_few_kernel<GU, false, false, GU && SCAN><<<grid, kFewMxWaves * 64, 0, stream>>>(g, o);
 }
 
 // Row tiles of BM rows, at most n_pairs / BM + one short one per slot.
@@ -120,7 +122,7 @@ static bool takes_tiles(int path, int block_m, bool a8, int H, int I, int n_pair
 template <bool GU>
 static int launch(const Mx4Args& g, int path, int block_m, hipStream_t stream) {
   if (!takes_tiles(path, block_m, g.a_scale != nullptr, g.K, g.N, g.n_pairs, g.P, g.split)) {
-    launch_few<GU>(g, stream);
+    launch_few<GU, false>(g, TokenIds{}, stream);
   } else {
     if (g.split) return LMOE_ERR_UNSUPPORTED;
     if (!known_block_m(block_m) || !tiles_fit(block_m, g.a_scale != nullptr, g.K)) return LMOE_ERR_SHAPE;
@@ -188,8 +190,8 @@ extern "C" int lmoe_combine_f32(const void* y, const int32_t* row_idx, const uin
   if (T == 0) return LMOE_OK;
   if (y == nullptr || w == nullptr || out == nullptr) return LMOE_ERR_ARG;
   if (bad16(y) || bad16(add) || bad16(out)) return LMOE_ERR_SHAPE;
-  combine_f32_kernel<<<dim3(T, (H + 255) / 256), 64, 0, stream>>>(
-      static_cast<const float*>(y), row_idx, w, k, H, static_cast<const uint16_t*>(add),
+  combine_f32_kernel<false><<<dim3(T, (H + 255) / 256), 64, 0, stream>>>(
+      static_cast<const float*>(y), row_idx, TokenIds{}, 0, w, k, H, static_cast<const uint16_t*>(add),
       static_cast<uint16_t*>(out));
   LMOE_RETURN_LAUNCH();
 }
@@ -234,6 +236,35 @@ extern "C" int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int
                    : lmoe_combine(ws->y, ws->row_idx, w, T, k, H, add, out, stream);
 }
 
+extern "C" int lmoe_mx4_decode_few(const void* x, const void* x_scale, int T, int H, int I, int k, const void* w13_slots,
+                                   const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids,
+                                   const int32_t* log2phy, int n_log2phy, const void* add, void* act, void* act_scale,
+                                   void* y, void* out, hipStream_t stream) {
+  if (T < 0 || H <= 0 || I <= 0 || k <= 0 || n_slots <= 0 || n_log2phy < 0) return LMOE_ERR_ARG;
+  if (H % kMxGroup != 0 || I % kMxGroup != 0 || n_slots > kMaxSlots || static_cast<long long>(T) * k > kScanMaxPairs)
+    return LMOE_ERR_SHAPE;
+  if (T == 0) return LMOE_OK;
+  if (x == nullptr || w13_slots == nullptr || w2_slots == nullptr || w == nullptr || ids == nullptr || act == nullptr ||
+      y == nullptr || out == nullptr || (x_scale == nullptr) != (act_scale == nullptr))
+    return LMOE_ERR_ARG;
+  if (bad16(x) || bad16(w13_slots) || bad16(w2_slots) || bad16(act) || bad16(y) || bad16(add) || bad16(out))
+    return LMOE_ERR_SHAPE;
+  const bool split = x_scale == nullptr;
+  const TokenIds o{ids, log2phy, n_log2phy, nullptr, nullptr, 0, 0};
+  const Mx4Args gu{x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(w13_slots),
+                   lmoe_mx4_bytes(2 * I, H), H, I, k, n_slots, T * k, nullptr, nullptr, nullptr, nullptr, nullptr, act,
+                   static_cast<uint8_t*>(act_scale), false, split};
+  const Mx4Args dn{act, static_cast<const uint8_t*>(act_scale), static_cast<const uint8_t*>(w2_slots),
+                   lmoe_mx4_bytes(H, I), I, H, 1, n_slots, T * k, nullptr, nullptr, nullptr, nullptr, nullptr, y, nullptr,
+                   true, split};
+  launch_few<true, true>(gu, o, stream);
+  launch_few<false, true>(dn, o, stream);
+  combine_f32_kernel<true><<<dim3(T, (H + 255) / 256), 64, 0, stream>>>(
+      static_cast<const float*>(y), nullptr, o, n_slots, w, k, H, static_cast<const uint16_t*>(add),
+      static_cast<uint16_t*>(out));
+  LMOE_RETURN_LAUNCH();
+}
+
 extern "C" int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, int I, int k, const void* w13_slots,
                                    const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids,
                                    const int32_t* log2phy, int n_log2phy, const void* w13_b,
@@ -250,8 +281,8 @@ extern "C" int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, in
   if (bad16(x) || bad16(w13_slots) || bad16(w2_slots) || bad16(act) || bad16(add) || bad16(out) ||
       bad16(w13_b) || bad16(w2_b))
     return LMOE_ERR_SHAPE;
-  const OneToken gate_up{ids, log2phy, n_log2phy, static_cast<const uint8_t*>(w13_b), log2phy_b, n_log2phy_b, n_slots_b};
-  OneToken down = gate_up;
+  const TokenIds gate_up{ids, log2phy, n_log2phy, static_cast<const uint8_t*>(w13_b), log2phy_b, n_log2phy_b, n_slots_b};
+  TokenIds down = gate_up;
   down.w_b = static_cast<const uint8_t*>(w2_b);
   const Mx4Args gu{x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(w13_slots),
                    lmoe_mx4_bytes(2 * I, H), H, I, k, n_slots, k, nullptr, nullptr, nullptr, nullptr, nullptr, act,

@@ -275,10 +275,11 @@ __device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int bloc
 }
 
 // NF 16-row fragments of rows [p0, p0 + rows) of one slot.  ONE: the one token's
-// row p0, whose pairs keep their order.  SP: rows in two parts, see above.
-template <bool GU, bool A8, int NF, int NW, bool ONE, bool SP>
+// act row p0.  SP: rows in two parts, see above.  pairs: the rows' pairs; act rows lie
+// from p0 on, or (SCAN) each at its pair.
+template <bool GU, bool A8, int NF, int NW, bool ONE, bool SP, bool SCAN>
 __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, int blocks, int cb, int p0, int rows,
-                                         f32x4_t* s_part) {
+                                         const int32_t* pairs, f32x4_t* s_part) {
   constexpr int RB = kFewMxBlocks;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -288,8 +289,8 @@ __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, 
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
     const int r = !SP ? 16 * f + (lane & 15) : NF == 1 ? lane & 7 : lane & 15;
-    const int pos = p0 + (r < rows ? r : 0);
-    size_t src = ONE ? 0 : GU ? g.sorted_pairs[pos] / g.topk : pos;
+    const int at = r < rows ? r : 0;
+    size_t src = ONE ? 0 : GU ? pairs[at] / g.topk : SCAN ? pairs[at] : p0 + at;
     if constexpr (SP) src = 2 * src + (NF == 1 ? (lane >> 3) & 1 : f);
     row[f] = static_cast<const char*>(g.a) + src * g.K * (A8 ? 1 : 2);
     row_scale[f] = A8 ? g.a_scale + src * (g.K / kMxGroup) : nullptr;
@@ -338,20 +339,68 @@ __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, 
     const bool live = r < rows;  // of eight rows at most, those in the lower lanes
     if constexpr (GU) {
       const f32x4_t gate[2] = {t[0], t[2]}, up[2] = {t[1], t[3]};
-      store_act<A8>(g, p0 + r, cb * 32, lane, live, gate, up);
+      store_act<A8>(g, SCAN ? (live ? pairs[r] : 0) : p0 + r, cb * 32, lane, live, gate, up);
     } else if (b0 < blocks) {
-      store_y(g, live ? g.sorted_pairs[p0 + r] : 0, cb * 64 + 32 * wave, lane, live, t[0], t[1]);
+      store_y(g, live ? pairs[r] : 0, cb * 64 + 32 * wave, lane, live, t[0], t[1]);
     }
   }
 }
 
-// (column block, active slot) of a grid of [ceil(N / 32 or 64), slots]
-template <bool GU, bool A8, bool SP>
-__global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g) {
+// The ids of a call that builds no permutation.  A pair whose expert the bank's table
+// leaves out may have it in a second bank (the decode overflow buffer, one token only).
+struct TokenIds {
+  const int32_t* ids;
+  const int32_t* log2phy;  // or null: ids are slots
+  int n_log2phy;
+  const uint8_t* w_b;      // the second bank, or null
+  const int32_t* log2phy_b;
+  int n_log2phy_b, P_b;
+};
+__device__ __forceinline__ int slot_of_id(const TokenIds& o, int P, int e) {  // or -1
+  int s = e;
+  if (o.log2phy != nullptr) s = e >= 0 && e < o.n_log2phy ? o.log2phy[e] : -1;
+  return s >= 0 && s < P ? s : -1;
+}
+
+// Few tokens straight from their ids: a lane looks a pair's slot up, and a workgroup
+// whose pair is the first of its slot takes all of the slot's pairs, in order.  The
+// permutation's launch and its three dependent loads (slot, offset, pair) become two
+// (id, table): two tokens of the 2048 x 768 layer 26.0 -> 23.0 us.  (A list of up to
+// 1024 ids in LDS, scanned by every workgroup, cost what it saved from 32 pairs on.)
+// Returns the pairs (0: another workgroup has them), the same for the
+// whole workgroup.
+constexpr int kScanMaxPairs = 64;
+__device__ __forceinline__ int scan_pairs(const Mx4Args& g, const TokenIds& o, int32_t* s_pairs, int* slot) {
+  const int lane = threadIdx.x & 63;
+  const int mine = lane < g.n_pairs ? slot_of_id(o, g.P, o.ids[lane]) : -1;
+  const int s = read_lane_i32(mine, blockIdx.y);
+  if (s < 0) return 0;
+  const uint64_t m = __ballot(mine == s);
+  if (__builtin_ctzll(m) != static_cast<int>(blockIdx.y)) return 0;
+  if (mine == s && threadIdx.x < 64) s_pairs[__popcll(m & ((1ull << lane) - 1))] = lane;
+  __syncthreads();
+  *slot = s;
+  return __popcll(m);
+}
+
+// (column block, active slot) of a grid of [ceil(N / 32 or 64), slots]; SCAN: (column
+// block, pair)
+template <bool GU, bool A8, bool SP, bool SCAN>
+__global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g, TokenIds o) {
   __shared__ f32x4_t s_part[kFewMxWaves * kFewMxBlocks * 64];
-  const int slot = g.active[blockIdx.y];
-  if (slot < 0) return;
-  const int p0 = g.offsets[slot], p1 = g.offsets[slot + 1];
+  __shared__ int32_t s_pairs[SCAN ? kScanMaxPairs : 1];
+  int slot, p0, p1;
+  if constexpr (SCAN) {
+    p0 = 0;
+    p1 = scan_pairs(g, o, s_pairs, &slot);
+    if (p1 == 0) return;
+  } else {
+    slot = g.active[blockIdx.y];
+    if (slot < 0) return;
+    p0 = g.offsets[slot];
+    p1 = g.offsets[slot + 1];
+  }
+  const int32_t* pairs = SCAN ? s_pairs : g.sorted_pairs;
   const int cb = blockIdx.x;
   const int blocks = min(kFewMxBlocks, (GU ? 2 * g.N : g.N) / 16 - cb * kFewMxBlocks);
   const uint8_t* wblk = g.w + slot * g.w_slot_bytes + static_cast<size_t>(cb) * kFewMxBlocks * mx4_block_bytes(g.K);
@@ -359,8 +408,10 @@ __global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g) {
   for (int p = p0; p < p1; p += PASS) {
     const int rows = min(PASS, p1 - p);
     if (p > p0) __syncthreads();  // the last pass's sums have been read
-    if (rows > PASS / 2) few_rows<GU, A8, 2, kFewMxWaves, false, SP>(g, wblk, blocks, cb, p, rows, s_part);
-    else few_rows<GU, A8, 1, kFewMxWaves, false, SP>(g, wblk, blocks, cb, p, rows, s_part);
+    if (rows > PASS / 2)
+      few_rows<GU, A8, 2, kFewMxWaves, false, SP, SCAN>(g, wblk, blocks, cb, p, rows, pairs + p, s_part);
+    else
+      few_rows<GU, A8, 1, kFewMxWaves, false, SP, SCAN>(g, wblk, blocks, cb, p, rows, pairs + p, s_part);
   }
 }
 
@@ -374,21 +425,10 @@ __global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g) {
 // their parts of K in another order than the split-K kernel's; the same order, parts
 // through LDS, cost a quarter at 7168 x 2048 (the step 51.7 -> 65.0 us).
 // ---------------------------------------------------------------------------
-// A pair whose expert the bank's table leaves out may have it in a second bank (the
-// decode overflow buffer).
-struct OneToken {
-  const int32_t* ids;
-  const int32_t* log2phy;  // or null: ids are slots
-  int n_log2phy;
-  const uint8_t* w_b;      // the second bank, or null
-  const int32_t* log2phy_b;
-  int n_log2phy_b, P_b;
-};
-__device__ __forceinline__ const uint8_t* expert_of_pair(const Mx4Args& g, const OneToken& o, int j) {  // or null
+__device__ __forceinline__ const uint8_t* expert_of_pair(const Mx4Args& g, const TokenIds& o, int j) {  // or null
   const int e = o.ids[j];
-  int s = e;
-  if (o.log2phy != nullptr) s = e >= 0 && e < o.n_log2phy ? o.log2phy[e] : -1;
-  if (s >= 0 && s < g.P) return g.w + s * g.w_slot_bytes;
+  int s = slot_of_id(o, g.P, e);
+  if (s >= 0) return g.w + s * g.w_slot_bytes;
   if (o.w_b == nullptr) return nullptr;
   s = e >= 0 && e < o.n_log2phy_b ? o.log2phy_b[e] : -1;
   return s >= 0 && s < o.P_b ? o.w_b + s * g.w_slot_bytes : nullptr;
@@ -403,14 +443,14 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
 }
 
 template <bool A8>
-__global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_gateup_kernel(Mx4Args g, OneToken o) {
+__global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_gateup_kernel(Mx4Args g, TokenIds o) {
   __shared__ f32x4_t s_part[kOneMxWaves * kFewMxBlocks * 64];
   const int j = blockIdx.y;
   const uint8_t* expert = uniform(expert_of_pair(g, o, j));
   if (expert == nullptr) return;
   const int cb = blockIdx.x;
   const uint8_t* wblk = expert + static_cast<size_t>(cb) * kFewMxBlocks * mx4_block_bytes(g.K);
-  few_rows<true, A8, 1, kOneMxWaves, true, false>(g, wblk, kFewMxBlocks, cb, j, 1, s_part);
+  few_rows<true, A8, 1, kOneMxWaves, true, false, false>(g, wblk, kFewMxBlocks, cb, j, 1, nullptr, s_part);
 }
 
 // 16 columns of out = add + sum_j w_j W2_j act_j.  The waves take (pair, part of K)
@@ -418,7 +458,7 @@ __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_gateup_kernel(Mx4Arg
 // order.  A unit is the whole K of a pair where there are eight pairs or more.  bf16
 // rows come in two parts, the fragment's lower and upper rows.
 template <bool A8>
-__global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_down_kernel(Mx4Args g, OneToken o,
+__global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_down_kernel(Mx4Args g, TokenIds o,
                                                                        const uint16_t* __restrict__ wts,
                                                                        const uint16_t* __restrict__ add) {
   constexpr int NW = kOneMxWaves;

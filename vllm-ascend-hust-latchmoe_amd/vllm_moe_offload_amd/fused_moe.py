@@ -187,7 +187,7 @@ def fused_experts(
     which holds no one-pair-per-slot assumption.
 
     Over 4-bit banks (uint8, mxfp4.pack_experts) hidden is bf16 or
-    native.Mx8Rows; one token goes straight from its ids, without a permutation
+    native.Mx8Rows; few tokens go straight from their ids, without a permutation
     in the workspace."""
     if w13_slots.dtype is torch.uint8:
         return _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, add, out, path, workspace)
@@ -207,9 +207,9 @@ def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2
     dst = ws.out[:T] if out is None else out
     if path == native.LMOE_PATH_AUTO:
         path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel())
-        if T == 1 and path == native.LMOE_PATH_GEMV:
-            return native.mx4_decode_one(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst,
-                                         add=add)
+        if path == native.LMOE_PATH_GEMV and (T == 1 or T * k <= native.MX4_DIRECT_PAIRS):
+            direct = native.mx4_decode_one if T == 1 else native.mx4_decode_few
+            return direct(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add)
     return native.mx4_fused_moe(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
                                 path=path, block_m=native.mx4_block_m(T * k, P))
 

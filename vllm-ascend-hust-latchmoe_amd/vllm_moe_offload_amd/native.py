@@ -71,6 +71,7 @@ EXPORTED_SYMBOLS = (
     "lmoe_mx4_gateup_silu",
     "lmoe_mx4_down",
     "lmoe_mx4_fused_moe",
+    "lmoe_mx4_decode_few",
     "lmoe_mx4_decode_one",
     "lmoe_fused_moe_decode",
     "lmoe_fused_moe_decode_noalloc",
@@ -163,6 +164,10 @@ _SIGNATURES = {
     "lmoe_mx4_fused_moe": (
         _i,
         [_vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp],
+    ),
+    "lmoe_mx4_decode_few": (
+        _i,
+        [_vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp],
     ),
     "lmoe_mx4_decode_one": (
         _i,
@@ -1395,6 +1400,36 @@ def mx4_fused_moe(x, topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_slo
     )
     bufs.perm.block_m = block_m
     bufs.perm.builds += 1
+    return out
+
+
+# Up to this many pairs fused_experts goes straight from the ids (mx4_decode_few takes
+# 64), past it through the permutation, whose order starts the heavy slots first.  us of
+# the captured layer, permutation / ids (H, I, experts, top k; tokens):
+#   2048, 768, 128, 8    2: 26.0 / 23.0, 3: 27.3 / 25.9, 4: 28.0 / 27.5, 6: 31.0 / 30.8, 8: 32.9 / 32.5
+#   2048, 1408, 60, 4    2: 26.8 / 23.1, 4: 28.0 / 25.4, 8: 32.7 / 31.2
+#   7168, 2048, 64, 8    2: 71.9 / 69.0, 3: 83.7 / 80.9, 4: 97.7 / 96.2, 6: 109.2 / 111.0, 8: 114.4 / 118.5 (8-bit rows)
+MX4_DIRECT_PAIRS = 32
+
+
+def mx4_decode_few(x, topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_slots: torch.Tensor,
+                   w2_slots: torch.Tensor, log2phy: torch.Tensor | None, bufs: Mx4Buffers, out: torch.Tensor, *,
+                   add: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Few tokens over 4-bit banks, straight from their ids (bufs.perm is left as
+    it was; act and y rows lie by pair), with mx4_fused_moe's bits on path
+    LMOE_PATH_GEMV.  At most 64 pairs; y is f32, a bf16 act in two parts."""
+    lib = load_library()
+    xq, xs, T, k, n_table = _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, bufs, out, add)
+    if bufs.y.dtype is not torch.float32 or (xs is None and not bufs.split):
+        raise ValueError("few tokens' y rows are f32, their bf16 act rows in two parts, [N, 2, I]")
+    _check(
+        lib.lmoe_mx4_decode_few(
+            xq.data_ptr(), _ptr(xs), T, bufs.hidden, bufs.intermediate, k, w13_slots.data_ptr(), w2_slots.data_ptr(),
+            bufs.perm.n_slots, topk_weights.data_ptr(), topk_ids.data_ptr(), _ptr(log2phy), n_table, _ptr(add),
+            bufs.act_ptr, bufs.act_scale_ptr, bufs.y.data_ptr(), out.data_ptr(), _stream(stream),
+        ),
+        "lmoe_mx4_decode_few",
+    )
     return out
 
 
