@@ -69,6 +69,7 @@ class MoEWorkspace:
 
 
 _WORKSPACES: dict[tuple, MoEWorkspace] = {}
+_DEVICE_NAMES: dict = {}  # of torch.device or str: making the name takes longer than finding the workspace
 
 
 def rows_kind(hidden, w13_slots) -> str:
@@ -88,7 +89,10 @@ def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = 
     are in two parts (their bytes are few beside the weights')."""
     if rows not in ("", "bf16", "mx8"):
         raise ValueError(f"unknown rows {rows!r}")
-    key = (int(T), int(k), int(P), int(H), int(I), str(device), tag, rows)
+    where = _DEVICE_NAMES.get(device)
+    if where is None:
+        where = _DEVICE_NAMES[device] = str(device)
+    key = (int(T), int(k), int(P), int(H), int(I), where, tag, rows)
     ws = _WORKSPACES.get(key)
     if ws is None:
         N = T * k

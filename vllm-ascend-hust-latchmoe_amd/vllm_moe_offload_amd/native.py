@@ -290,11 +290,12 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 # The current stream's handle without a Stream object around it, where torch has
 # the call (a few microseconds less of host time in every wrapper).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _stream(stream: torch.cuda.Stream | None) -> int:
     if stream is None and _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(_device_index())
     s = stream if stream is not None else torch.cuda.current_stream()
     return int(s.cuda_stream)
 
@@ -380,6 +381,16 @@ def _same_device(*tensors) -> None:
             raise ValueError(f"operand on {t.device}, the current device is cuda:{here}")
 
 
+def _fits(t: torch.Tensor, dtype: torch.dtype, shape, here: int) -> bool:
+    """_is on device here; _refuse says what is wrong."""
+    return t.dtype is dtype and t.get_device() == here and t.shape == shape and t.is_contiguous()
+
+
+def _refuse(t, name: str, dtype: torch.dtype, shape: tuple | None = None) -> None:
+    _need(t, name, dtype, shape)
+    _same_device(t)
+
+
 def add_rms_norm(
     x: torch.Tensor,
     weight: torch.Tensor,
@@ -405,47 +416,49 @@ def add_rms_norm(
     bf16, f32 = torch.bfloat16, torch.float32
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError("x must be a [T, H] tensor")
-    shape = T, H = x.shape
-    if not _is(x, bf16, shape):
-        _need(x, "x", bf16)
+    here = _device_index()
+    shape = x.shape
+    T, H = shape
+    if not _fits(x, bf16, shape, here):
+        _refuse(x, "x", bf16)
     wdt = f32 if weight.dtype is f32 else bf16
-    if not _is(weight, wdt, (H,)):
-        _need(weight, "weight", wdt, (H,))
+    if not _fits(weight, wdt, (H,), here):
+        _refuse(weight, "weight", wdt, (H,))
     rdt = bf16
     if residual is not None:
         rdt = f32 if residual.dtype is f32 else bf16
-        if not _is(residual, rdt, shape):
-            _need(residual, "residual", rdt, shape)
+        if not _fits(residual, rdt, shape, here):
+            _refuse(residual, "residual", rdt, shape)
         if residual_out is None:
             residual_out = residual
-        elif not _is(residual_out, rdt, shape):
-            _need(residual_out, "residual_out", rdt, shape)
+        elif not _fits(residual_out, rdt, shape, here):
+            _refuse(residual_out, "residual_out", rdt, shape)
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
     if out is None and mx8 is None:
         out = torch.empty_like(x)
-    elif out is not None and not _is(out, bf16, shape):
-        _need(out, "out", bf16, shape)
+    elif out is not None and not _fits(out, bf16, shape, here):
+        _refuse(out, "out", bf16, shape)
     q = scale = None
     if mx8 is not None:
         _need_mx8(mx8, "mx8", shape)
         q, scale = mx8.q, mx8.scale
-    _same_device(x, weight, residual, residual_out, out, q, scale)
-    if residual is not None and T:
-        if out is not None and out.data_ptr() == residual_out.data_ptr():
-            raise ValueError("out and residual_out must be two buffers")
-        if rdt is f32 and ((out is not None and out.data_ptr() == residual.data_ptr()) or
-                           residual_out.data_ptr() == x.data_ptr()):
-            raise ValueError("rows of two types cannot share a buffer")
-    _check(
-        lib.lmoe_add_rms_norm(
-            x.data_ptr(), T, H, _ptr(residual), rdt is f32, weight.data_ptr(), wdt is f32, eps, _ptr(residual_out),
-            _ptr(out), _ptr(q), _ptr(scale), _stream(stream),
-        ),
-        "lmoe_add_rms_norm",
-    )
+        _same_device(q, scale)
+    px, po = x.data_ptr(), None if out is None else out.data_ptr()
+    pr = pro = None
+    if residual is not None:
+        pr, pro = residual.data_ptr(), residual_out.data_ptr()
+        if T:
+            if po == pro:
+                raise ValueError("out and residual_out must be two buffers")
+            if rdt is f32 and (po == pr or pro == px):
+                raise ValueError("rows of two types cannot share a buffer")
+    status = lib.lmoe_add_rms_norm(px, T, H, pr, rdt is f32, weight.data_ptr(), wdt is f32, eps, pro, po, _ptr(q),
+                                   _ptr(scale), _stream(stream))
+    if status:
+        _check(status, "lmoe_add_rms_norm")
     return out, mx8, residual_out
 
 
@@ -1341,6 +1354,8 @@ class Mx4Buffers:
                 raise ValueError(f"a buffer on {t.device}, y on {y.device}")
         self.hidden, self.intermediate = int(y.shape[1]), int(aq.shape[-1])
         self.mx8 = as_ is not None
+        H, I, P = self.hidden, self.intermediate, perm.n_slots
+        self.w13_shape, self.w2_shape = (P, 2 * I, mxfp4.row_bytes(H)), (P, H, mxfp4.row_bytes(I))
         self.act_ptr, self.act_scale_ptr = _ptr(aq), _ptr(as_)
         p = perm
         self._struct = _Mx4Workspace(
@@ -1352,35 +1367,43 @@ class Mx4Buffers:
 
 def _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, bufs: Mx4Buffers, out, add):
     """Check a layer call over 4-bit banks; (x values, scales, T, k, table length)."""
+    bf16, i32, u8 = torch.bfloat16, torch.int32, torch.uint8
+    here = _device_index()
+    if bufs.device_index != here:
+        raise ValueError(f"buffers on cuda:{bufs.device_index}, the current device is cuda:{here}")
+    pairs = topk_ids.shape
+    T, k = pairs
+    rows = (T, bufs.hidden)
     mx8 = isinstance(x, Mx8Rows)
-    xq, xs = (x.q, x.scale) if mx8 else (x, None)
-    H, I, P = bufs.hidden, bufs.intermediate, bufs.perm.n_slots
-    T, k = topk_ids.shape
     if mx8:
-        _need_mx8(x, "x", (T, H))
-    elif not _is(x, torch.bfloat16, (T, H)):
-        _need(x, "x", torch.bfloat16, (T, H))
+        _need_mx8(x, "x", rows)
+        xq, xs = x.q, x.scale
+        _same_device(xq, xs)
+    else:
+        xq, xs = x, None
+        if not _fits(x, bf16, rows, here):
+            _refuse(x, "x", bf16, rows)
     if mx8 != bufs.mx8:
         raise ValueError("x and act must both be bf16 or both be Mx8Rows")
     if T * k != bufs.perm.n_pairs:
         raise ValueError(f"buffers for {bufs.perm.n_pairs} pairs, got {T * k}")
-    for t, name, dtype, shape in (
-            (topk_weights, "topk_weights", torch.bfloat16, (T, k)), (topk_ids, "topk_ids", torch.int32, (T, k)),
-            (w13_slots, "w13_slots", torch.uint8, (P, 2 * I, mxfp4.row_bytes(H))),
-            (w2_slots, "w2_slots", torch.uint8, (P, H, mxfp4.row_bytes(I))), (out, "out", torch.bfloat16, (T, H))):
-        if not _is(t, dtype, shape):
-            _need(t, name, dtype, shape)
-    if add is not None and not _is(add, torch.bfloat16, (T, H)):
-        _need(add, "add", torch.bfloat16, (T, H))
+    if not _fits(topk_weights, bf16, pairs, here):
+        _refuse(topk_weights, "topk_weights", bf16, pairs)
+    if not _fits(topk_ids, i32, pairs, here):
+        _refuse(topk_ids, "topk_ids", i32, pairs)
+    if not _fits(w13_slots, u8, bufs.w13_shape, here):
+        _refuse(w13_slots, "w13_slots", u8, bufs.w13_shape)
+    if not _fits(w2_slots, u8, bufs.w2_shape, here):
+        _refuse(w2_slots, "w2_slots", u8, bufs.w2_shape)
+    if not _fits(out, bf16, rows, here):
+        _refuse(out, "out", bf16, rows)
+    if add is not None and not _fits(add, bf16, rows, here):
+        _refuse(add, "add", bf16, rows)
     n_table = 0
     if log2phy is not None:
         n_table = log2phy.numel()
-        if not _is(log2phy, torch.int32, (n_table,)):
-            _need(log2phy, "log2phy", torch.int32)
-    here = torch.cuda.current_device()
-    if bufs.device_index != here:
-        raise ValueError(f"buffers on cuda:{bufs.device_index}, the current device is cuda:{here}")
-    _same_device(xq, xs, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, out, add)
+        if not _fits(log2phy, i32, (n_table,), here):
+            _refuse(log2phy, "log2phy", i32)
     return xq, xs, T, k, n_table
 
 
