@@ -842,3 +842,34 @@ def test_few_tokens_refusals():
     with pytest.raises(RuntimeError, match="unsupported shape"):
         native.mx4_decode_few(big.x, w8, ids8, big.w13, big.w2, None, bufs, o8)
     assert fused_moe.fused_experts(big.x, w8, ids8, big.w13, big.w2, None).isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("T,k,E", [(1, 2, 8), (40, 2, 40), (50, 2, 8), (200, 2, 8), (600, 4, 8)])
+def test_every_form_captured_and_replayed(T, k, E, rows):
+    """One token, the permuted split-K kernel, each height of row tiles: replays on
+    new ids, with eager calls of the same shape between them."""
+    from vllm_moe_offload_amd import fused_moe, native
+
+    H, I = 256, 96
+    rng = np.random.default_rng(T)
+    layer = Layer(H, I, E, T, rows, 4)
+    w = torch.full((T, k), 0.5, dtype=torch.bfloat16, device="cuda")
+    d_ids = to_dev_i32(rng.integers(0, E, (T, k)))
+    ws = fused_moe.get_workspace(T, k, E, H, I, "cuda", tag="forms", rows=rows)
+    out = torch.empty((T, H), dtype=torch.bfloat16, device="cuda")
+    call = lambda o, s: fused_moe.fused_experts(layer.x, w, d_ids, layer.w13, layer.w2, None, out=o, workspace=s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out, ws)
+    for _ in range(3):
+        d_ids.copy_(to_dev_i32(rng.integers(0, E, (T, k))))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = call(torch.empty_like(out), None)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    native.device_flags(clear=True)
