@@ -846,10 +846,11 @@ def test_few_tokens_refusals():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", ROWS)
-@pytest.mark.parametrize("T,k,E", [(1, 2, 8), (40, 2, 40), (50, 2, 8), (200, 2, 8), (600, 4, 8)])
-def test_every_form_captured_and_replayed(T, k, E, rows):
-    """One token, the permuted split-K kernel, each height of row tiles: replays on
-    new ids, with eager calls of the same shape between them."""
+@pytest.mark.parametrize("T,k,E,bm", [(1, 2, 8, 0), (9, 2, 8, 0), (40, 2, 40, 0), (50, 2, 8, 32), (200, 2, 700, 32),
+                                      (200, 2, 8, 64), (600, 4, 8, 128)])
+def test_every_form_captured_and_replayed(T, k, E, bm, rows):
+    """Few tokens, the permuted split-K kernel (bm 0), row tiles of every height and
+    grid: replays on new ids, with eager calls of the same shape between them."""
     from vllm_moe_offload_amd import fused_moe, native
 
     H, I = 256, 96
@@ -857,19 +858,54 @@ def test_every_form_captured_and_replayed(T, k, E, rows):
     layer = Layer(H, I, E, T, rows, 4)
     w = torch.full((T, k), 0.5, dtype=torch.bfloat16, device="cuda")
     d_ids = to_dev_i32(rng.integers(0, E, (T, k)))
-    ws = fused_moe.get_workspace(T, k, E, H, I, "cuda", tag="forms", rows=rows)
+    ws = [fused_moe.get_workspace(T, k, E, H, I, "cuda", tag=t, rows=rows) for t in ("forms", "forms eager")]
     out = torch.empty((T, H), dtype=torch.bfloat16, device="cuda")
-    call = lambda o, s: fused_moe.fused_experts(layer.x, w, d_ids, layer.w13, layer.w2, None, out=o, workspace=s)
+
+    def call(o, s):
+        if bm:
+            return native.mx4_fused_moe(layer.x, w, d_ids, layer.w13, layer.w2, None, s.mx4, o,
+                                        path=native.LMOE_PATH_MFMA, block_m=bm)
+        return fused_moe.fused_experts(layer.x, w, d_ids, layer.w13, layer.w2, None, out=o, workspace=s)
+
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        call(out, ws)
+        call(out, ws[0])
     for _ in range(3):
         d_ids.copy_(to_dev_i32(rng.integers(0, E, (T, k))))
         out.zero_()
         graph.replay()
         torch.cuda.synchronize()
-        want = call(torch.empty_like(out), None)
+        want = call(torch.empty_like(out), ws[1])
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     native.device_flags(clear=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("H,I", [(32, 32), (128, 160), (384, 128), (672, 416), (1120, 96)])
+def test_one_and_two_chunks_a_stage_give_the_same_bits(H, I, rows):
+    """32-row tiles on grids of few and of many workgroups (two chunks a stage, one),
+    odd numbers of chunks, a row that is not a number among the others."""
+    native = _native()
+    layer = Layer(H, I, 3, 40, rows, H)
+    ids = np.random.default_rng(I).integers(0, 3, (40, 1)).astype(np.int32)
+    if rows == "mx8":
+        layer.x.scale[7, -1] = 255
+    else:
+        layer.x[7, H - 1] = float("nan")
+    few = run_layer(layer, ids, 1, native.LMOE_PATH_MFMA, block_m=32)
+    wide = Layer.__new__(Layer)                    # the same experts before many that get no row
+    extra = lambda b: torch.cat([b, torch.zeros((600, *b.shape[1:]), dtype=torch.uint8, device="cuda")])
+    wide.__dict__.update(layer.__dict__, P=603, w13=extra(layer.w13), w2=extra(layer.w2))
+    ids2 = np.concatenate([ids, np.full((600, 1), -1, np.int32)])
+    keep = layer.x
+    wide.x = torch.cat([keep, keep[:1].expand(600, H)]) if rows == "bf16" else native.Mx8Rows(
+        torch.cat([keep.q.view(torch.uint8), keep.q.view(torch.uint8)[:1].expand(600, H)]).view(torch.float8_e4m3fn),
+        torch.cat([keep.scale, keep.scale[:1].expand(600, H // 32)]))
+    many = run_layer(wide, ids2, 1, native.LMOE_PATH_MFMA, block_m=32)
+    bits = lambda a: a.q.view(torch.uint8) if rows == "mx8" else a.view(torch.int16)
+    assert torch.equal(bits(few[1]), bits(many[1])[:40])
+    assert torch.equal(few[2].view(torch.int16), many[2][:40].view(torch.int16))
+    assert few[2][7].isnan().all() and few[2][torch.arange(40, device="cuda") != 7].isfinite().all()

@@ -71,25 +71,36 @@ static void launch_few(const Mx4Args& g, const TokenIds& o, hipStream_t stream) 
 }
 
 // Row tiles of BM rows, at most n_pairs / BM + one short one per slot.
-template <bool GU, bool A8, int BM>
-static int launch_tiles(const Mx4Args& g, hipStream_t stream) {
-  const int lds = Mx4Tile<A8, BM>::lds_bytes(mx4_chunks(g.K));
-  constexpr int cols = GU ? kTileCols / 2 : kTileCols;
-  const long long tiles = g.n_pairs / BM + (g.n_pairs < g.P ? g.n_pairs : g.P);
-  const long long grid = 8 * ((tiles * ((g.N + cols - 1) / cols) + 7) / 8);
-  if (grid > 0x7fffffffLL) return LMOE_ERR_SHAPE;
+constexpr int kFewTileBlocks = 512;  // two workgroups per CU: up to these, two chunks a stage
+
+template <bool GU, bool A8, int BM, int CS>
+static int launch_tiles(const Mx4Args& g, unsigned grid, hipStream_t stream) {
+  const int lds = Mx4Tile<A8, BM, CS>::lds_bytes(mx4_chunks(g.K));
   static bool raised[64] = {};  // per device: dynamic LDS past 64 KiB allowed
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return static_cast<int>(e);
   if (dev < 0 || dev >= 64 || !raised[dev]) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx4_tile_kernel<GU, A8, BM>),
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx4_tile_kernel<GU, A8, BM, CS>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return static_cast<int>(e);
     if (dev >= 0 && dev < 64) raised[dev] = true;
   }
-  mx4_tile_kernel<GU, A8, BM><<<static_cast<unsigned>(grid), kTileWaves * 64, lds, stream>>>(g);
+  mx4_tile_kernel<GU, A8, BM, CS><<<grid, kTileWaves * 64, lds, stream>>>(g);
   return LMOE_OK;
+}
+
+template <bool GU, bool A8, int BM>
+static int launch_tiles(const Mx4Args& g, hipStream_t stream) {
+  constexpr int cols = GU ? kTileCols / 2 : kTileCols;
+  const long long tiles = g.n_pairs / BM + (g.n_pairs < g.P ? g.n_pairs : g.P);
+  const long long blocks = tiles * ((g.N + cols - 1) / cols);
+  const long long grid = 8 * ((blocks + 7) / 8);
+  if (grid > 0x7fffffffLL) return LMOE_ERR_SHAPE;
+  if constexpr (BM == 32) {
+    if (blocks <= kFewTileBlocks) return launch_tiles<GU, A8, BM, 2>(g, static_cast<unsigned>(grid), stream);
+  }
+  return launch_tiles<GU, A8, BM, 1>(g, static_cast<unsigned>(grid), stream);
 }
 
 static bool known_block_m(int bm) { return bm == 32 || bm == 64 || bm == 128; }
@@ -97,9 +108,9 @@ static bool known_block_m(int bm) { return bm == 32 || bm == 64 || bm == 128; }
 // Whether rows of K columns fit the LDS of tiles of block_m rows (MX8 rows: their scales).
 static bool tiles_fit(int block_m, bool a8, int K) {
   const int chunks = mx4_chunks(K);
-  const int lds = block_m == 32   ? (a8 ? Mx4Tile<true, 32>::lds_bytes(chunks) : Mx4Tile<false, 32>::lds_bytes(chunks))
-                  : block_m == 64 ? (a8 ? Mx4Tile<true, 64>::lds_bytes(chunks) : Mx4Tile<false, 64>::lds_bytes(chunks))
-                                  : (a8 ? Mx4Tile<true, 128>::lds_bytes(chunks) : Mx4Tile<false, 128>::lds_bytes(chunks));
+  const int lds = block_m == 32   ? (a8 ? Mx4Tile<true, 32, 2>::lds_bytes(chunks) : Mx4Tile<false, 32, 2>::lds_bytes(chunks))
+                  : block_m == 64 ? (a8 ? Mx4Tile<true, 64, 1>::lds_bytes(chunks) : Mx4Tile<false, 64, 1>::lds_bytes(chunks))
+                                  : (a8 ? Mx4Tile<true, 128, 1>::lds_bytes(chunks) : Mx4Tile<false, 128, 1>::lds_bytes(chunks));
   return lds <= 160 * 1024;
 }
 
@@ -110,12 +121,13 @@ static int launch_tiles(const Mx4Args& g, int block_m, hipStream_t stream) {
   return launch_tiles<GU, A8, 128>(g, stream);
 }
 
-// path AUTO: row tiles past this many pairs per slot, on average (native.py has the figures)
-constexpr int kFewPairsPerSlot = 3;
+// path AUTO: row tiles past this many pairs per slot, on average, of bf16 and of MX8 rows
+// (native.py has the figures)
+constexpr int kFewPairsPerSlot[2] = {4, 6};
 
 static bool takes_tiles(int path, int block_m, bool a8, int H, int I, int n_pairs, int P, bool split) {
   if (path != LMOE_PATH_AUTO) return path == LMOE_PATH_MFMA;
-  return !split && known_block_m(block_m) && n_pairs > static_cast<long long>(kFewPairsPerSlot) * P &&
+  return !split && known_block_m(block_m) && n_pairs > static_cast<long long>(kFewPairsPerSlot[a8]) * P &&
          tiles_fit(block_m, a8, H) && tiles_fit(block_m, a8, I);
 }
 

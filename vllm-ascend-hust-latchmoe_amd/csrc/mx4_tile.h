@@ -41,19 +41,27 @@ constexpr int kTileCols = 256;  // weight rows of a workgroup
 
 __device__ __attribute__((aligned(16))) const uint32_t g_zero16[4] = {0, 0, 0, 0};
 
-template <bool A8, int BM_>
+// CS: chunks of a stage.  Two where a stage's wait is what bounds it, on grids of few
+// workgroups (gate-up us, one / two, 32 rows: 16 experts of 4096 x 1024, 128 tokens x 2,
+// bf16 rows 34.2 / 25.1, MX8 rows 27.6 / 20.2; 16 of 2048 x 512 18.4 / 14.0; 8 of 4096 x
+// 2048, 64 tokens x 2 27.9 / 19.9).  Where there are workgroups to fill a CU their number
+// counts for more, and two chunks' registers cost it (64 tokens x 8 of 128 experts, 2048 x
+// 768, 39.4 / 42.5; 61 x 4 of 60, 2048 x 1408, 34.2 / 36.3; 300 x 8 of 128 49.4 / 46.7).
+template <bool A8, int BM_, int CS_>
 struct Mx4Tile {
   static constexpr int BM = BM_;
+  static constexpr int CS = CS_;
   static constexpr int NF = BM / 16;                 // 16-row fragments
   static constexpr int PIECES = A8 ? 8 : 16;         // 16-byte pieces of a row's chunk
   static constexpr int ROWB = PIECES * 16;
-  static constexpr int STAGE = BM * ROWB;
+  static constexpr int PART = BM * ROWB;             // a chunk's rows
+  static constexpr int STAGE = CS * PART;
   static constexpr int RPL = 64 / PIECES;            // rows one load instruction fills
-  static constexpr int QA = STAGE / 1024 / kTileWaves;  // load instructions per wave and chunk
-  static_assert(QA * kTileWaves * 1024 == STAGE, "whole load instructions");
+  static constexpr int QA = PART / 1024 / kTileWaves;  // load instructions per wave and chunk
+  static_assert(QA * kTileWaves * 1024 == PART, "whole load instructions");
   static constexpr int OFF_PAIR = 2 * STAGE;         // BM pair ids
   static constexpr int OFF_SCALE = OFF_PAIR + BM * 4;
-  // scales go to LDS 64 dwords at a time: two chunks of 32 rows
+  // scales go to LDS 64 dwords at a time: two chunks of 32 rows (two chunks a stage too)
   static int lds_bytes(int chunks) { return OFF_SCALE + (A8 ? BM * 4 * ((chunks + 1) & ~1) : 0); }
   static __device__ __forceinline__ int sw(int r) { return A8 ? (r >> 1) & 7 : (r + 4) & 15; }
 };
@@ -96,9 +104,9 @@ __device__ __forceinline__ TileSlot slot_of_tile(const int32_t* tile_off, const 
   }
 }
 
-template <bool GU, bool A8, int BM>
+template <bool GU, bool A8, int BM, int CS>
 __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g) {
-  using C = Mx4Tile<A8, BM>;
+  using C = Mx4Tile<A8, BM, CS>;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   int* s_pair = reinterpret_cast<int*>(smem + C::OFF_PAIR);
   uint32_t* s_scale = reinterpret_cast<uint32_t*>(smem + C::OFF_SCALE);
@@ -140,18 +148,23 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
     const size_t src = GU ? g.sorted_pairs[pos] / g.topk : pos;
     a_src[q] = static_cast<const char*>(g.a) + src * row_bytes + a_piece(q) * 16;
   }
-  auto issue = [&](int c, int buf) {
-    char* st = smem + buf * C::STAGE + wave * C::QA * 1024;
-    const bool cut = tail != 0 && c == chunks - 1;
-    if (!cut) {
+  const int stages = (chunks + CS - 1) / CS;
+  auto issue = [&](int stage, int buf) {
 #pragma unroll
-      for (int q = 0; q < C::QA; ++q) load_lds16b(a_src[q] + static_cast<size_t>(c) * C::ROWB, st + q * 1024);
-    } else {
+    for (int e = 0; e < CS; ++e) {
+      const int c = stage * CS + e;
+      char* st = smem + buf * C::STAGE + e * C::PART + wave * C::QA * 1024;
+      const int here = K - c * kMxChunk;  // columns of the chunk; past them, and in one past the last, zeros
+      if (here >= kMxChunk) {
 #pragma unroll
-      for (int q = 0; q < C::QA; ++q) {
-        const char* p = a_src[q] + static_cast<size_t>(c) * C::ROWB;
-        if (a_piece(q) * (A8 ? 16 : 8) >= tail) p = reinterpret_cast<const char*>(g_zero16);
-        load_lds16b(p, st + q * 1024);
+        for (int q = 0; q < C::QA; ++q) load_lds16b(a_src[q] + static_cast<size_t>(c) * C::ROWB, st + q * 1024);
+      } else {
+#pragma unroll
+        for (int q = 0; q < C::QA; ++q) {
+          const char* p = a_src[q] + static_cast<size_t>(c) * C::ROWB;
+          if (a_piece(q) * (A8 ? 16 : 8) >= here) p = reinterpret_cast<const char*>(g_zero16);
+          load_lds16b(p, st + q * 1024);
+        }
       }
     }
   };
@@ -165,34 +178,31 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     wsrc[j] = g.w + slot * g.w_slot_bytes + static_cast<size_t>(min(b0 + j, wblocks - 1)) * bb;
-  const uint32_t code_at = 256 + lane * 16, scale_at = lane * 4;
-  auto load_w = [&](int c, i32x4_t (&w)[4], int (&sc)[4]) {  // sc: byte c % 4 is the chunk's
-    const int quad = (c >> 2) * kMxQuadBytes;
-    if constexpr (BM < 128) {
-      // the wave's base in scalar registers, the lane's offset (made here, so that its
-      // 32 bits are seen) beside it: no address arithmetic.  Gate-up us, without /
-      // with: 64 rows 55.1 / 52.5, 32 rows 47.2 / 45.7, but 128 rows 119.0 / 121.5.
-      typedef const __attribute__((address_space(1))) uint8_t* base_t;
-      uint32_t at = lane * 16, sat = lane * 4;
-      asm volatile("" : "+v"(at), "+v"(sat));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const base_t p = (base_t)(wsrc[j] + quad);
-        const base_t codes = p + 256 + (c & 3) * 1024;
-        w[j] = *(const __attribute__((address_space(1))) i32x4_t*)(codes + at);
-        sc[j] = *(const __attribute__((address_space(1))) int*)(p + sat);
-      }
-      return;
-    }
+  const uint32_t code_at = lane * 16, scale_at = lane * 4;
+  // codes of a stage's chunks (one past the last: the last's; its rows are zeros), and
+  // the scales: byte c % 4 is chunk c's, of one dword for the whole stage
+  auto load_w = [&](int stage, i32x4_t (&w)[CS][4], int (&sc)[4]) {
+    typedef const __attribute__((address_space(1))) uint8_t* base_t;
+    const int c0 = stage * CS;
+    const int quad = (c0 >> 2) * kMxQuadBytes;
+    uint32_t at = code_at, sat = scale_at;
+    // up to 64 rows: the wave's base in scalar registers, the lane's offset (made here,
+    // so that its 32 bits are seen) beside it: no address arithmetic.  Gate-up us, without
+    // / with: 64 rows 55.1 / 52.5, 32 rows 47.2 / 45.7, but 128 rows 119.0 / 121.5.
+    if constexpr (BM < 128) asm volatile("" : "+v"(at), "+v"(sat));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint8_t* p = wsrc[j] + quad;
-      w[j] = *reinterpret_cast<const i32x4_t*>(p + (c & 3) * 1024 + code_at);
-      sc[j] = *reinterpret_cast<const int*>(p + scale_at);
+      const base_t p = (base_t)(wsrc[j] + quad);
+#pragma unroll
+      for (int e = 0; e < CS; ++e) {
+        const base_t codes = p + 256 + (min(c0 + e, chunks - 1) & 3) * 1024;
+        w[e][j] = *(const __attribute__((address_space(1))) i32x4_t*)(codes + at);
+      }
+      sc[j] = *(const __attribute__((address_space(1))) int*)(p + sat);
     }
   };
 
-  i32x4_t w_next[4];
+  i32x4_t w_next[CS][4];
   int sc_next[4];
   issue(0, 0);
   load_w(0, w_next, sc_next);
@@ -204,14 +214,14 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
     const uint8_t* sp = g.a_scale + static_cast<size_t>(GU ? g.sorted_pairs[pos] / g.topk : pos) * groups;
     constexpr int STEP = kTileWaves * 64 / BM;
     if (tail == 0 && (reinterpret_cast<uintptr_t>(g.a_scale) & 3) == 0) {  // straight to LDS, 64 of them at a time
-      for (int c = wave * 64 / BM; c < chunks; c += STEP) {
+      for (int c = wave * 64 / BM; c < stages * CS; c += STEP) {
         const int mine = min(c + lane / BM, chunks - 1);  // two chunks where BM is 32
         __builtin_amdgcn_global_load_lds(
             (const __attribute__((address_space(1))) void*)(sp + 4 * mine),
             (__attribute__((address_space(3))) void*)(s_scale + c * BM + (wave * 64 & (BM - 1))), 4, 0, 0);
       }
     } else {
-      for (int c = tid / BM; c < chunks; c += STEP) {
+      for (int c = tid / BM; c < stages * CS; c += STEP) {
         uint32_t v = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -235,63 +245,72 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   // straight-line code; rows past the tile's last are dropped at the store
   auto main_loop = [&](auto nl_tag) {
     constexpr int NL = decltype(nl_tag)::value;
-    for (int c = 0; c < chunks; ++c) {
-      tile_barrier();  // chunk c is in LDS; every wave is done with the other buffer
-      i32x4_t w[4];
-      int sc[4];
+    for (int stage = 0; stage < stages; ++stage) {
+      tile_barrier();  // the stage is in LDS; every wave is done with the other buffer
+      i32x4_t wst[CS][4];
+      int scst[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        w[j] = w_next[j];
-        sc[j] = sc_next[j] >> (8 * (c & 3));
+#pragma unroll
+        for (int e = 0; e < CS; ++e) wst[e][j] = w_next[e][j];
+        scst[j] = sc_next[j] >> (8 * (stage * CS & 3));
       }
-      if (c + 1 < chunks) issue(c + 1, (c + 1) & 1);
-      load_w(c + 1 < chunks ? c + 1 : c, w_next, sc_next);
+      if (stage + 1 < stages) issue(stage + 1, (stage + 1) & 1);
+      load_w(stage + 1 < stages ? stage + 1 : stage, w_next, sc_next);
       __builtin_amdgcn_sched_barrier(0);
-      const char* st = smem + (c & 1) * C::STAGE + fr * C::ROWB;
-      // the next row fragment is on its way from LDS while this one is multiplied
-      if constexpr (A8 && NL > 0) {
-        RowFrag<true> x[2];
-        const uint8_t* xs = reinterpret_cast<const uint8_t*>(s_scale + c * BM + fr) + lg;
-        auto read = [&](int i) {
-          const char* p = st + i * 16 * C::ROWB;
-          const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(p + ((lg ^ fsw) * 16));
-          const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(p + (((4 + lg) ^ fsw) * 16));
-          x[i & 1].v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          x[i & 1].scale = xs[i * 64];
-        };
-        read(0);
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          if (i + 1 < NL) read(i + 1);
-          __builtin_amdgcn_sched_barrier(0);
+      for (int e = 0; e < CS; ++e) {
+        const int c = stage * CS + e;
+        const i32x4_t(&w)[4] = wst[e];
+        int sc[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = mx4_step<true>(w[j], sc[j], x[i & 1], acc[i][j]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      } else if constexpr (NL > 0) {
-        float s[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = mx_scale_f32(sc[j] & 255);
-        bf16x8v_t x[2];
-        auto read = [&](int n) {  // n: quarter of the chunk * NL + fragment
-          const int k = n / NL, i = n % NL;
-          x[n & 1] = *reinterpret_cast<const bf16x8v_t*>(st + i * 16 * C::ROWB + (((4 * lg + k) ^ fsw) * 16));
-        };
-        read(0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {  // quarters as mx4_step takes them
-          bf16x8v_t wb[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) wb[j] = weights_bf16(w[j][k], s[j]);
+        for (int j = 0; j < 4; ++j) sc[j] = scst[j] >> (8 * e);
+        const char* st = smem + (stage & 1) * C::STAGE + e * C::PART + fr * C::ROWB;
+        // the next row fragment is on its way from LDS while this one is multiplied
+        if constexpr (A8 && NL > 0) {
+          RowFrag<true> x[2];
+          const uint8_t* xs = reinterpret_cast<const uint8_t*>(s_scale + c * BM + fr) + lg;
+          auto read = [&](int i) {
+            const char* p = st + i * 16 * C::ROWB;
+            const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(p + ((lg ^ fsw) * 16));
+            const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(p + (((4 + lg) ^ fsw) * 16));
+            x[i & 1].v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            x[i & 1].scale = xs[i * 64];
+          };
+          read(0);
 #pragma unroll
           for (int i = 0; i < NL; ++i) {
-            const int n = k * NL + i;
-            if (n + 1 < 4 * NL) read(n + 1);
+            if (i + 1 < NL) read(i + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j], x[n & 1], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < 4; ++j) acc[i][j] = mx4_step<true>(w[j], sc[j], x[i & 1], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
+          }
+        } else if constexpr (NL > 0) {
+          float s[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[j] = mx_scale_f32(sc[j] & 255);
+          bf16x8v_t x[2];
+          auto read = [&](int n) {  // n: quarter of the chunk * NL + fragment
+            const int k = n / NL, i = n % NL;
+            x[n & 1] = *reinterpret_cast<const bf16x8v_t*>(st + i * 16 * C::ROWB + (((4 * lg + k) ^ fsw) * 16));
+          };
+          read(0);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // quarters as mx4_step takes them
+            bf16x8v_t wb[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wb[j] = weights_bf16(w[j][k], s[j]);
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+              const int n = k * NL + i;
+              if (n + 1 < 4 * NL) read(n + 1);
+              __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j], x[n & 1], acc[i][j], 0, 0, 0);
+              __builtin_amdgcn_sched_barrier(0);
+            }
           }
         }
       }

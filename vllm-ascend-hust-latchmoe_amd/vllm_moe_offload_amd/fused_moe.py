@@ -210,12 +210,12 @@ def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2
         raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
     dst = ws.out[:T] if out is None else out
     if path == native.LMOE_PATH_AUTO:
-        path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel())
+        path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel(), isinstance(hidden, native.Mx8Rows))
         if path == native.LMOE_PATH_GEMV and (T == 1 or T * k <= native.MX4_DIRECT_PAIRS):
             direct = native.mx4_decode_one if T == 1 else native.mx4_decode_few
             return direct(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add)
     return native.mx4_fused_moe(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
-                                path=path, block_m=native.mx4_block_m(T * k, P))
+                                path=path, block_m=native.mx4_block_m(T * k, P, w13_slots.shape[1] // 2))
 
 
 def _second_bank(overflow: PreparedSlotWeights | None) -> tuple | None:
@@ -229,7 +229,7 @@ def _layer_path(hidden, k: int, n_experts: int, *w13) -> int:
     gives the unsplit layer's bits."""
     T, H = hidden.shape
     if mxfp4.is_mx4(w13[0]):
-        return native.mx4_path(T * k, n_experts)
+        return native.mx4_path(T * k, n_experts, isinstance(hidden, native.Mx8Rows))
     return native.layer_path(T, k, H, int(w13[0].shape[1]) // 2, n_experts, aligned=native.aligned16(hidden, *w13))
 
 
@@ -252,7 +252,7 @@ def _pass_block_m(n_experts: int, H: int, I: int, device, n_pairs: int, path: in
     one height), else the MFMA kernel's for pass_pairs of n_pairs pairs.  mx4:
     the experts are in 4 bits."""
     if mx4:
-        return native.mx4_block_m(n_pairs if pass_pairs is None else pass_pairs, n_experts)
+        return native.mx4_block_m(n_pairs if pass_pairs is None else pass_pairs, n_experts, I)
     if path == native.LMOE_PATH_GEMV:
         return native.MFMA_BLOCK_M
     if path == native.LMOE_PATH_STREAM:

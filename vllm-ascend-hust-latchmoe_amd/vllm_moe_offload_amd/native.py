@@ -934,38 +934,54 @@ def prefill_block_m(n_experts: int, hidden: int, intermediate: int, device="cuda
 
 
 MX4_BLOCK_M = (32, 64, 128)  # row-tile heights of the 4-bit experts' prefill kernel
-# Up to this many pairs per expert the split-K kernel, row tiles past it.  us, gate-up
-# and down together, split-K / 32-row tiles (H, I, experts, top k; half of the Zipf
-# bias on the routing):
-#   2048, 768, 128, 8    16 tokens 27.2 / 26.2, 32: 49.7 / 47.9, 64: 63.2 / 58.9, 128: 85 / 71
-#   2048, 1408, 60, 4    30: 42.2 / 39.8, 61: 50.0 / 52.4, 120: 66.7 / 56.7
-#   7168, 2048, 32, 8    16: 121 / 128, 32: 139 / 155, 64: 178 / 165 (8-bit rows)
-MX4_FEW_PAIRS_PER_EXPERT = 3
+# Up to this many pairs per expert the split-K kernel, row tiles past it: bf16 rows, 8-bit
+# rows.  Time of the captured layer, split-K over 32-row tiles (H, I, experts, top k):
+#   pairs per expert     3           4           6           8
+#   2048, 768, 128, 8    .98; .96    1.02; .98   1.13; 1.04
+#   2048, 1408, 60, 4    .96; .93    .95; .93    1.07; .95   1.18; 1.00
+#   4096, 1024, 16, 2                .83; .82    .88; .83    1.07; 1.02
+#   2048, 512, 16, 2                 .86; .89    .90; .89    1.08; 1.09
+#   7168, 2048, 32, 8    1.02; 1.00  1.02; .98   .99; .99    1.07; 1.01
+#   4096, 2048, 64, 4    .94; .90    .97; .90    1.12; 1.00  1.18; .98
+#   1024, 512, 64, 4     1.03; .97   1.08; .99   1.26; 1.13
+MX4_FEW_PAIRS_PER_EXPERT = 4
+MX4_FEW_PAIRS_PER_EXPERT_MX8 = 6
 
 
-def mx4_path(n_pairs: int, n_experts: int) -> int:
+def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False) -> int:
     """The path of a layer of 4-bit experts, for every pass of it: the split-K
-    kernel for few pairs per expert, row tiles past that."""
-    return LMOE_PATH_GEMV if n_pairs <= MX4_FEW_PAIRS_PER_EXPERT * n_experts else LMOE_PATH_MFMA
+    kernel for few pairs per expert (mx8: of 8-bit rows), row tiles past that."""
+    few = MX4_FEW_PAIRS_PER_EXPERT_MX8 if mx8 else MX4_FEW_PAIRS_PER_EXPERT
+    return LMOE_PATH_GEMV if n_pairs <= few * n_experts else LMOE_PATH_MFMA
 
 
-# Most pairs per slot, on average, of each row-tile height but the last.  us, gate-up
-# and down together, 32 / 64 / 128 rows (bf16 rows; 8-bit rows):
-#   2048, 768, 128, 8   25 pairs per slot 80 / 82 / 99;    76 / 78 / 81
-#                       40               100 / 97 / 117;   90 / 84 / 87
-#                       64               126 / 116 / 136; 109 / 95 / 96
-#                       100              170 / 148 / 169; 144 / 117 / 115
-#                       256              380 / 321 / 311; 290 / 254 / 209
-#   7168, 2048, 32, 8   50               225 / 183 / 203 (8-bit rows)
-#                       100              325 / 262 / 247
-MX4_BLOCK_MAX_PAIRS = {32: 32, 64: 100}
+# Row-tile heights but the last, with the most pairs per slot, on average, and the most
+# gate-up workgroups (tiles of that height by 128 columns) that each is used up to: the
+# shorter tiles, while they do not fill the card.  us of the captured layer, 32 / 64 / 128
+# rows (bf16 rows; 8-bit rows; workgroups at 32 rows):
+#   4096, 1024, 8, 2     48 pairs per slot  48 / 65 / 96;  42 / 49 / 64 (160)
+#                        192                75 / 76 / 104; 59 / 64 / 70 (448)
+#   2048, 1024, 16, 2    96                 50 / 57 / 73;  44 / 47 / 52 (512)
+#                        192                72 / 69 / 77;  59 / 54 / 55 (896)
+#   4096, 1408, 16, 4    48                 73 / 78 / 105; 70 / 71 / 76 (440)
+#                        96                 97 / 98 / 117; 87 / 80 / 83 (704)
+#   2048, 768, 32, 4     48                 52 / 56 / 72;  50 / 51 / 55 (480)
+#   1024, 512, 64, 4     48                 43 / 47 / 57;  40 / 40 / 46 (640)
+# and, gate-up and down alone,
+#   2048, 768, 128, 8    25                 80 / 82 / 99;    76 / 78 / 81
+#                        64                 126 / 116 / 136; 109 / 95 / 96
+#                        100                170 / 148 / 169; 144 / 117 / 115
+#                        256                380 / 321 / 311; 290 / 254 / 209
+#   7168, 2048, 32, 8    50                 225 / 183 / 203 (8-bit rows)
+#                        100                325 / 262 / 247
+MX4_HEIGHTS = ((32, 32, 640), (64, 100, 1024))
 
 
-def mx4_block_m(n_pairs: int, n_experts: int) -> int:
-    """Row-tile height of 4-bit experts' products (the permutation's block_m)
-    for n_pairs pairs over n_experts slots."""
-    for bm, most in MX4_BLOCK_MAX_PAIRS.items():
-        if n_pairs <= most * n_experts:
+def mx4_block_m(n_pairs: int, n_experts: int, intermediate: int = 1024) -> int:
+    """Row-tile height of 4-bit experts' products (the permutation's block_m) for
+    n_pairs pairs over n_experts slots of experts intermediate wide."""
+    for bm, pairs, groups in MX4_HEIGHTS:
+        if n_pairs <= pairs * n_experts or (n_pairs // bm + n_experts) * -(-intermediate // 128) <= groups:
             return bm
     return MX4_BLOCK_M[-1]
 
