@@ -19,11 +19,11 @@
 // of 4096 tokens x 8 of 128 experts, 2048 x 768, from 187 to 126 us with MX8 rows.)
 //
 // What bounds it: in large prefills the matrix units and, between their bursts, the
-// wait at each chunk's barrier.  Those 32768 pairs, back to back, gate-up / down: bf16 rows 193 /
-// 119 us, 1.07 / 0.87 PFLOP/s (a large bf16 matrix product here: 1.33), the units 58% /
-// 45% busy; MX8 rows 118 / 87 us, 1.75 / 1.19 PFLOP/s (a large e4m3 product: 2.93),
+// wait at each chunk's barrier.  Those 32768 pairs, back to back, gate-up / down: bf16 rows 195 /
+// 118 us, 1.06 / 0.87 PFLOP/s (a large bf16 matrix product here: 1.33), the units 58% /
+// 45% busy; MX8 rows 120 / 88 us, 1.72 / 1.17 PFLOP/s (a large e4m3 product: 2.93),
 // 46% / 31% busy, the down product held by its 134 MB of y as well.  With few rows per
-// slot it is the weights: 300 tokens 48 / 31 us, 214 / 117 MB at 4.4 / 3.7 TB/s.
+// slot it is the weights: 300 tokens 45 / 30 us, 214 / 117 MB at 4.7 / 3.9 TB/s.
 // Measured and slower: 256-row tiles of eight waves (gate-up 230 us against 193),
 // workgroups that stay for several tiles (220 against 200), two weight chunks ahead
 // (the compiler then waits for every load), K in phases, raised wave priority,
