@@ -3,11 +3,11 @@
 // A workgroup of four waves computes BM rows of one slot by 256 weight rows:
 // gate-up 128 act columns (gate and up), down 256 y columns.  Each wave takes all
 // BM rows and 64 weight rows (four 16-row blocks; gate-up: gate, up, gate, up of
-// 32 act columns).  Per chunk of 128 columns the rows go to LDS without passing
-// through registers (two buffers, the next chunk in flight under this one's
-// products), where all four waves read them; weights go from memory straight to
-// registers, one chunk ahead, since the bank's order is the fragments' order and
-// no two waves share any.
+// 32 act columns).  Per stage, one or two chunks of 128 columns, the rows go to LDS
+// without passing through registers (two buffers, the next stage in flight under this
+// one's products), where all four waves read them; weights go from memory straight to
+// registers, one stage ahead, since the bank's order is the fragments' order and no
+// two waves share any.
 //
 // LDS holds 16-byte piece p of row r at position p ^ sw(r).  A 16-byte read goes
 // by sixteen lanes at a time, 0-3, 12-15, 20-27 first and 4-11, 16-19, 28-31 next
@@ -19,9 +19,9 @@
 // of 4096 tokens x 8 of 128 experts, 2048 x 768, from 187 to 126 us with MX8 rows.)
 //
 // What bounds it: in large prefills the matrix units and, between their bursts, the
-// wait at each chunk's barrier.  Those 32768 pairs, back to back, gate-up / down: bf16 rows 195 /
-// 118 us, 1.06 / 0.87 PFLOP/s (a large bf16 matrix product here: 1.33), the units 58% /
-// 45% busy; MX8 rows 120 / 88 us, 1.72 / 1.17 PFLOP/s (a large e4m3 product: 2.93),
+// wait at each stage's barrier.  Those 32768 pairs, back to back, gate-up / down: bf16
+// rows 195 / 118 us, 1.06 / 0.87 PFLOP/s (a large bf16 matrix product here: 1.33), the
+// units 58% / 45% busy; MX8 rows 120 / 88 us, 1.72 / 1.17 PFLOP/s (a large e4m3 product: 2.93),
 // 46% / 31% busy, the down product held by its 134 MB of y as well.  With few rows per
 // slot it is the weights: 300 tokens 45 / 30 us, 214 / 117 MB at 4.7 / 3.9 TB/s.
 // Measured and slower: 256-row tiles of eight waves (gate-up 230 us against 193),

@@ -386,6 +386,16 @@ def _fits(t: torch.Tensor, dtype: torch.dtype, shape, here: int) -> bool:
     return t.dtype is dtype and t.get_device() == here and t.shape == shape and t.is_contiguous()
 
 
+def _take_mx8(rows, name: str, shape, here: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(values, scales) of 8-bit rows [T, K] on device here."""
+    q, scale = rows.q, rows.scale
+    if not (shape[1] % 32 == 0 and _fits(q, torch.float8_e4m3fn, shape, here) and
+            _fits(scale, torch.uint8, (shape[0], shape[1] // 32), here)):
+        _need_mx8(rows, name, tuple(shape))
+        _same_device(q, scale)
+    return q, scale
+
+
 def _refuse(t, name: str, dtype: torch.dtype, shape: tuple | None = None) -> None:
     _need(t, name, dtype, shape)
     _same_device(t)
@@ -443,9 +453,9 @@ def add_rms_norm(
         _refuse(out, "out", bf16, shape)
     q = scale = None
     if mx8 is not None:
-        _need_mx8(mx8, "mx8", shape)
-        q, scale = mx8.q, mx8.scale
-        _same_device(q, scale)
+        if not isinstance(mx8, Mx8Rows):
+            raise TypeError("mx8 must be Mx8Rows")
+        q, scale = _take_mx8(mx8, "mx8", shape, here)
     px, po = x.data_ptr(), None if out is None else out.data_ptr()
     pr = pro = None
     if residual is not None:
@@ -1392,9 +1402,7 @@ def _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, buf
     rows = (T, bufs.hidden)
     mx8 = isinstance(x, Mx8Rows)
     if mx8:
-        _need_mx8(x, "x", rows)
-        xq, xs = x.q, x.scale
-        _same_device(xq, xs)
+        xq, xs = _take_mx8(x, "x", rows, here)
     else:
         xq, xs = x, None
         if not _fits(x, bf16, rows, here):
