@@ -1,0 +1,48 @@
+"""Calls over 4-bit experts as programs make them: a decode step beside its
+separate calls, the full layer's check, calls on several streams and threads,
+results that are kept, events, very long rows.  (tests/test_gpu_mx4.py checks the
+values, tests/test_gpu_mx4_layer.py the layer.)"""
+
+import numpy as np
+import pytest
+import torch
+
+from tests._util import to_dev_i32
+from tests.test_gpu_mx4 import ROWS, Layer
+
+pytestmark = pytest.mark.gpu
+
+
+def _bits(t):
+    return t.view(torch.int16)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("T", [12, 18, 24, 28])
+def test_a_decode_step_takes_the_path_of_its_separate_calls(T, rows, monkeypatch):
+    """3, 4.5, 6 and 7 pairs per expert, around the borders of both kinds of rows:
+    the router reads bf16 rows, the experts' rows choose the path."""
+    from vllm_moe_offload_amd import fused_moe, native
+
+    E, H, I, k = 16, 2048, 416, 4
+    layer = Layer(H, I, E, T, rows, 6)
+    g = torch.Generator(device="cuda").manual_seed(T)
+    hidden = torch.empty((T, H), device="cuda").normal_(generator=g).to(torch.bfloat16)
+    x = hidden if rows == "bf16" else native.rows_to_mx8(hidden)
+    gate = torch.empty((E, H), device="cuda").normal_(0, 0.2, generator=g).to(torch.bfloat16)
+    l2p = to_dev_i32(np.random.default_rng(1).permutation(E))
+    ws = fused_moe.get_workspace(T, k, E, H, I, "cuda", tag="step", rows=rows)
+    paths, mlp = [], native.grouped_mlp
+
+    def spy(*a, **kw):
+        paths.append(kw["path"])
+        return mlp(*a, **kw)
+
+    monkeypatch.setattr(native, "grouped_mlp", spy)
+    out, w, ids = fused_moe.decode_layer(hidden, gate, fused_moe.RouterSpec(top_k=k), layer.w13, layer.w2, l2p,
+                                         workspace=ws, out=torch.empty_like(hidden),
+                                         expert_rows=x if rows == "mx8" else None)
+    want = fused_moe.fused_experts(x, w, ids, layer.w13, layer.w2, l2p, out=torch.empty_like(hidden))
+    torch.cuda.synchronize()
+    assert paths == [native.mx4_path(T * k, E, rows == "mx8")]
+    assert torch.equal(_bits(out), _bits(want))

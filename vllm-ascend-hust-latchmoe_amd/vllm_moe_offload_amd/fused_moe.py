@@ -451,9 +451,10 @@ def decode_layer(
         renormalize=bool(spec.renormalize), routed_scaling_factor=float(spec.routed_scaling_factor),
         n_shared=int(spec.n_shared), w_bf16=w_out, ids=ids_out, skip_unmapped=overflow is not None,
     )
-    path = _bank_layer_path(hidden, kw, w13_slots, log2phy, overflow)
-    bm = _block_m(hidden, kw, w13_slots, path)
-    merged = overflow is not None and log2phy is not None and _merged_passes(hidden, kw, w13_slots, overflow, path)
+    # as fused_experts chooses: from the rows that the experts read
+    path = _bank_layer_path(rows, kw, w13_slots, log2phy, overflow)
+    bm = _block_m(rows, kw, w13_slots, path)
+    merged = overflow is not None and log2phy is not None and _merged_passes(rows, kw, w13_slots, overflow, path)
     perm_b = None
     fused_body = overflow is None and path == native.LMOE_PATH_GEMV and not mx4
     mx4_one = T == 1 and path == native.LMOE_PATH_GEMV and mx4 and (overflow is None or log2phy is not None)
@@ -466,11 +467,11 @@ def decode_layer(
     elif T <= ONE_LAUNCH_ROUTER_MAX_TOKENS:
         w, ids, _ = native.router_gate_topk_permute(hidden, gate_weight, logits_out, k, ws.perm, block_m=bm, **sel)
         if merged:
-            perm_b = _overflow_permute(hidden, ids, kw, overflow, ws, path=path)
+            perm_b = _overflow_permute(rows, ids, kw, overflow, ws, path=path)
     else:
         logits = native.router_gate(hidden, gate_weight, logits_out)
         if merged:  # the overflow table's build rides with the bank's
-            perm_b = _overflow_perm(hidden, kw, overflow, ws)
+            perm_b = _overflow_perm(rows, kw, overflow, ws)
             sel["second"] = (perm_b, overflow.log2phy)
         w, ids, _ = native.router_topk_permute(logits, k, ws.perm, block_m=bm, **sel)
     dst = out if out is not None else ws.out[:T]
