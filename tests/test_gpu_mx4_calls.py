@@ -46,3 +46,29 @@ def test_a_decode_step_takes_the_path_of_its_separate_calls(T, rows, monkeypatch
     torch.cuda.synchronize()
     assert paths == [native.mx4_path(T * k, E, rows == "mx8")]
     assert torch.equal(_bits(out), _bits(want))
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("T", [1, 2, 8, 9, 60])
+def test_the_full_layer_fails_closed_on_any_number_of_tokens(T, rows):
+    """A pair without a slot is an error, with few pairs (no permutation in the
+    call of fused_experts) as with many; good ids pass, whatever came before."""
+    from tests.test_gpu_mx4_layer import E, H, _layer, _weights, _x
+    from vllm_moe_offload_amd import fused_moe, mxfp4, native
+
+    w13, w2, gate = _weights(11)
+    layer, rt = _layer(210, w13, w2, gate, slots=8, b2_wave_prefill=True)
+    b13, b2 = (t.cuda() for t in mxfp4.pack_experts(w13, w2))
+    x = _x(T, T)
+    w, ids, _ = fused_moe.route(x, gate, layer.router_spec)
+    x = x if rows == "bf16" else native.rows_to_mx8(x)
+    bad = ids.clone()
+    bad[T - 1, 2] = E + 5
+    run = lambda i, **kw: fused_moe.run_full_layer(rt, layer_id=210, hidden=x, topk_weights=w, topk_ids=i,  # noqa: E731
+                                                   num_logical_experts=E, **kw)
+    want = fused_moe.fused_experts(x, w, ids, b13, b2, torch.arange(E, dtype=torch.int32, device="cuda")).clone()
+    for path in (native.LMOE_PATH_AUTO, native.LMOE_PATH_GEMV):
+        with pytest.raises(RuntimeError, match="without ready slots: 1 pairs"):
+            run(bad, path=path)
+        assert torch.equal(_bits(run(ids)), _bits(want))
+    native.device_flags(clear=True)

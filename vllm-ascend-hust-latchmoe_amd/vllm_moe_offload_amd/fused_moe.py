@@ -194,13 +194,18 @@ def fused_experts(
     native.Mx8Rows; few tokens go straight from their ids, without a permutation
     in the workspace."""
     if w13_slots.dtype is torch.uint8:
-        return _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, add, out, path, workspace)
+        return _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, add=add, out=out, path=path,
+                                  workspace=workspace)
     return _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, add=add, out=out,
                              path=path, workspace=workspace)[0]
 
 
-def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, add, out, path, ws):
-    """fused_experts over 4-bit banks."""
+def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, *, add=None, out=None,
+                       path=native.LMOE_PATH_AUTO, workspace=None, counted=False):
+    """fused_experts over 4-bit banks.  counted: with a permutation in the
+    workspace however few the pairs are (its counts and errors are read after the
+    call); out has the same bits."""
+    ws = workspace
     T, H = hidden.shape
     k = topk_ids.shape[1]
     P = w13_slots.shape[0]
@@ -211,7 +216,9 @@ def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2
     dst = ws.out[:T] if out is None else out
     if path == native.LMOE_PATH_AUTO:
         path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel(), isinstance(hidden, native.Mx8Rows))
-        if path == native.LMOE_PATH_GEMV and (T == 1 or T * k <= native.MX4_DIRECT_PAIRS):
+        if path == native.LMOE_PATH_GEMV and (T == 1 or T * k <= native.MX4_DIRECT_PAIRS and not counted):
+            if counted:  # one token's form reads no permutation
+                native.permute(topk_ids, ws.perm, log2phy=log2phy)
             direct = native.mx4_decode_one if T == 1 else native.mx4_decode_few
             return direct(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add)
     return native.mx4_fused_moe(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
@@ -1058,9 +1065,13 @@ def run_full_layer(
     k = int(topk_ids.shape[1])
     ws = get_workspace(T, k, prepared.physical_expert_count, H, int(prepared.w1.shape[1]) // 2, hidden.device, tag="full",
                        rows=rows_kind(hidden, prepared.w1))
-    dst = fused_experts(hidden, topk_weights, topk_ids, prepared.w1, prepared.w2, prepared.log2phy,
-                        add=add, out=out, path=path, workspace=ws)
-    if not _is_current_graph_capturing():
+    checked = not _is_current_graph_capturing()
+    args = (hidden, topk_weights, topk_ids, prepared.w1, prepared.w2, prepared.log2phy)
+    if mxfp4.is_mx4(prepared.w1):
+        dst = _mx4_fused_experts(*args, add=add, out=out, path=path, workspace=ws, counted=checked)
+    else:
+        dst = fused_experts(*args, add=add, out=out, path=path, workspace=ws)
+    if checked:
         check_placed(ws)
     return dst
 
