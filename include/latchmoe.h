@@ -427,8 +427,8 @@ int lmoe_combine_f32(const void* y, const int32_t* row_idx, const uint16_t* w,
  *   out [T, H] bf16 = y (or null), q / scale = y as MX8 rows (or null); each is
  *   rounded once, from f32; the squares are summed in f32.  In place: residual_out
  *   may be residual, or x where residual is bf16; out may be x, or residual where
- *   that is bf16 and residual_out is another buffer.  One buffer for two outputs,
- *   or q over an input, is LMOE_ERR_ARG.
+ *   that is bf16 and residual_out is another buffer.  Any other overlap of an
+ *   output with an input or another output is LMOE_ERR_ARG.
  * H % 8 == 0 (H % 32 == 0 with q), H <= 32768, operands 16-byte aligned (scale
  * any); else LMOE_ERR_SHAPE.  No counterpart in the reference (vLLM's own norm
  * precedes the layer). */
@@ -438,7 +438,7 @@ int lmoe_add_rms_norm(const void* x, int T, int H, const void* residual,
                       void* scale, hipStream_t stream);
 
 /* bf16 rows x [T, H] as MX8 rows.  H % 32 == 0, H <= 32768, x and q 16-byte
- * aligned; else LMOE_ERR_SHAPE. */
+ * aligned; else LMOE_ERR_SHAPE.  x, q and scale may not overlap (LMOE_ERR_ARG). */
 int lmoe_rows_to_mx8(const void* x, int T, int H, void* q, void* scale,
                      hipStream_t stream);
 

@@ -248,3 +248,39 @@ def test_norm_past_32_bits():
         assert torch.equal(native.add_rms_norm(x[a:b].clone(), w, out=torch.empty_like(x[a:b]), mx8=e)[0], out[a:b])
         for got, want in ((m[a:b], e), (q[a:b], f)):
             assert torch.equal(got.q.view(torch.uint8), want.q.view(torch.uint8)) and torch.equal(got.scale, want.scale)
+
+
+@pytest.mark.gpu
+def test_norm_refuses_rows_that_others_still_read():
+    """Outputs that start inside an input, or scales over one: refused, nothing
+    written; next to it, and row for row, the call is taken."""
+    native = _native()
+    buf = torch.empty((9, 64), dtype=torch.bfloat16, device="cuda").normal_()
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    keep, x = buf.clone(), buf[:4]
+    m = native.Mx8Rows.allocate(4, 64, "cuda")
+    over_q = native.Mx8Rows(buf.view(torch.float8_e4m3fn).view(-1)[64:320].view(4, 64), m.scale)
+    over_s = native.Mx8Rows(m.q, buf.view(torch.uint8).view(-1)[3:11].view(4, 2))
+    other = torch.zeros_like(x)
+    bad = [
+        lambda: native.add_rms_norm(x, w, out=buf[1:5]),
+        lambda: native.add_rms_norm(buf[1:5], w, out=x),
+        lambda: native.add_rms_norm(other, w, residual=x, residual_out=buf[3:7]),
+        lambda: native.add_rms_norm(other, w, residual=buf[3:7], out=x),
+        lambda: native.add_rms_norm(x, w, mx8=over_q),
+        lambda: native.add_rms_norm(x, w, mx8=over_s),
+        lambda: native.add_rms_norm(x, buf[4], out=buf[4:8]),
+        lambda: native.rows_to_mx8(x, over_q),
+        lambda: native.rows_to_mx8(x, over_s),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+            pytest.fail(f"call {i} was taken")
+    torch.cuda.synchronize()
+    assert torch.equal(buf, keep) and not other.any()
+    want = native.add_rms_norm(keep[:4], w)[0]
+    native.add_rms_norm(x, w, out=buf[4:8])
+    assert torch.equal(buf[4:8], want) and torch.equal(buf[:4], keep[:4])
+    native.add_rms_norm(x, w, out=x)
+    assert torch.equal(buf[:4], want) and torch.equal(buf[8], keep[8])

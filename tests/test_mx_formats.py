@@ -213,3 +213,41 @@ def test_few_tokens_entry_checks_its_arguments():
     assert few(T=1 << 30, k=1 << 30) == 1001
     for t in ("x", "w13", "w2", "act", "y", "out", "add"):
         assert few(**{t: P16 + 8}) == 1001, t
+
+
+def test_norm_entries_refuse_any_overlap_but_row_for_row():
+    """Every output against every input and the other outputs, from either side,
+    by one byte or one row: refused before any device work."""
+    from vllm_moe_offload_amd import native
+
+    lib = native.load_library()
+    T, H = 3, 64
+    size = {"x": 2 * T * H, "r": 2 * T * H, "w": 2 * H, "ro": 2 * T * H, "out": 2 * T * H, "q": T * H, "s": T * H // 32}
+    at = {n: 65536 * (i + 1) for i, n in enumerate(size)}
+
+    def norm(f32=0, **kw):
+        a = {**at, **kw}
+        return lib.lmoe_add_rms_norm(a["x"], T, H, a["r"], f32, a["w"], 0, 1e-6, a["ro"], a["out"], a["q"], a["s"], N)
+
+    for o in ("ro", "out", "q", "s"):
+        step = 1 if o == "s" else 16
+        for other in size:
+            if other == o:
+                continue
+            ends = [at[other] + size[other] - step, at[other] + 2 * H, at[other] + step]
+            ends += [at[other] + step - size[o]] if size[o] % 16 == 0 or o == "s" else []
+            for p in ends:
+                if p < at[other] + size[other] and p % step == 0:  # else refused for its address
+                    assert norm(**{o: p}) == 1000, (o, other, p - at[other])
+            # row for row: a bf16 output over x, or over a residual that is no output's as well
+            if (o, other) not in (("ro", "x"), ("ro", "r"), ("out", "x"), ("out", "r")):
+                assert norm(**{o: at[other]}) == 1000, (o, other)
+    f32 = 4 * T * H
+    for kw in (dict(ro=at["r"] + 16), dict(ro=at["r"] + f32 - 16), dict(out=at["r"] + f32 - 16), dict(out=at["r"]),
+               dict(ro=at["x"]), dict(x=at["ro"] + f32 - 16), dict(s=at["r"] + f32 - 1), dict(s=at["ro"] + f32 - 1)):
+        assert norm(f32=1, **kw) == 1000, kw
+    rows = lambda x=at["x"], q=at["q"], s=at["s"]: lib.lmoe_rows_to_mx8(x, T, H, q, s, N)
+    x, q = at["x"], at["q"]
+    for kw in (dict(q=x + 16), dict(q=x + size["x"] - 16), dict(q=x + 16 - size["q"]), dict(s=x), dict(s=x + size["x"] - 1),
+               dict(s=x + 1 - size["s"]), dict(s=q), dict(s=q + size["q"] - 1)):
+        assert rows(**kw) == 1000, kw

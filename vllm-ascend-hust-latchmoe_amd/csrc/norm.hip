@@ -147,6 +147,33 @@ static void launch_norm(const NormArgs& g, int T, hipStream_t stream) {
 
 static bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
+struct Span {
+  const void* p;
+  size_t bytes;
+};
+static bool overlap(const Span& a, const Span& b) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a.p), q = reinterpret_cast<uintptr_t>(b.p);
+  return p != 0 && q != 0 && p < q + b.bytes && q < p + a.bytes;
+}
+
+// Whether an output would be written over another one, or over an input that other
+// workgroups (weight: any) still read.  Only a row over itself is safe, where both
+// start at one address and their rows are as long.
+static bool clobbers(const NormArgs& g, int T, bool residual_f32, bool weight_f32) {
+  const size_t n = static_cast<size_t>(T) * g.H;
+  const size_t rb = residual_f32 ? 4 : 2;
+  const Span in[3] = {{g.x, 2 * n}, {g.residual, rb * n}, {g.weight, static_cast<size_t>(g.H) * (weight_f32 ? 4 : 2)}};
+  const Span out[4] = {{g.residual_out, rb * n}, {g.out, 2 * n}, {g.q, n}, {g.scale, n / kMxGroup}};
+  const size_t in_row[3] = {2, rb, 0}, out_row[4] = {rb, 2, 1, 0};  // bytes of a column
+  for (int o = 0; o < 4; ++o) {
+    for (int i = 0; i < 3; ++i)
+      if (overlap(out[o], in[i]) && !(out[o].p == in[i].p && out_row[o] == in_row[i] && in_row[i] != 0)) return true;
+    for (int v = 0; v < o; ++v)
+      if (overlap(out[o], out[v])) return true;
+  }
+  return false;
+}
+
 }  // namespace lmoe
 
 using namespace lmoe;
@@ -165,13 +192,10 @@ extern "C" int lmoe_add_rms_norm(const void* x, int T, int H, const void* residu
   if (misaligned16(x) || misaligned16(residual) || misaligned16(weight) ||
       misaligned16(residual_out) || misaligned16(out) || misaligned16(q))
     return LMOE_ERR_SHAPE;
-  // a row may overwrite itself, but not another one that is still to be read
-  if (out != nullptr && out == residual_out) return LMOE_ERR_ARG;
-  if (residual_f32 && residual != nullptr && (out == residual || residual_out == x)) return LMOE_ERR_ARG;
-  if (q != nullptr && (q == x || q == residual || q == out || q == residual_out)) return LMOE_ERR_ARG;
   const NormArgs g{static_cast<const uint16_t*>(x), residual, weight, residual_out,
                    static_cast<uint16_t*>(out), static_cast<uint8_t*>(q),
                    static_cast<uint8_t*>(scale), eps, H};
+  if (clobbers(g, T, residual_f32 != 0, weight_f32 != 0)) return LMOE_ERR_ARG;
   if (residual == nullptr) {
     if (weight_f32) launch_norm<kNone, kF32>(g, T, stream);
     else launch_norm<kNone, kBf16>(g, T, stream);
@@ -192,9 +216,9 @@ extern "C" int lmoe_rows_to_mx8(const void* x, int T, int H, void* q, void* scal
   if (T == 0) return LMOE_OK;
   if (x == nullptr || q == nullptr || scale == nullptr) return LMOE_ERR_ARG;
   if (misaligned16(x) || misaligned16(q)) return LMOE_ERR_SHAPE;
-  if (q == x) return LMOE_ERR_ARG;  // rows of half the length
   const NormArgs g{static_cast<const uint16_t*>(x), nullptr, nullptr, nullptr, nullptr,
                    static_cast<uint8_t*>(q), static_cast<uint8_t*>(scale), 0.0f, H};
+  if (clobbers(g, T, false, false)) return LMOE_ERR_ARG;
   launch_norm<kNone, kNone>(g, T, stream);
   LMOE_RETURN_LAUNCH();
 }

@@ -420,7 +420,8 @@ def add_rms_norm(
     residual bf16 or f32, weight [H] bf16 or f32; r is kept in f32 between the
     sum and the outputs, the squares are summed in f32.  residual_out may be x,
     out may be x, or residual if residual_out is another buffer (where an f32
-    residual is not one of them).  H a multiple of 8 (of 32 with mx8) up to 32768.  Returns (out, mx8,
+    residual is not one of them); outputs that overlap anything otherwise are
+    refused.  H a multiple of 8 (of 32 with mx8) up to 32768.  Returns (out, mx8,
     residual_out), None for what was not asked for."""
     lib = load_library()
     bf16, f32 = torch.bfloat16, torch.float32
@@ -468,8 +469,15 @@ def add_rms_norm(
     status = lib.lmoe_add_rms_norm(px, T, H, pr, rdt is f32, weight.data_ptr(), wdt is f32, eps, pro, po, _ptr(q),
                                    _ptr(scale), _stream(stream))
     if status:
+        _refuse_overlap(status, H)
         _check(status, "lmoe_add_rms_norm")
     return out, mx8, residual_out
+
+
+def _refuse_overlap(status: int, H: int) -> None:
+    """What LMOE_ERR_ARG means where the operands have been checked."""
+    if status == LMOE_ERR_ARG and H > 0:
+        raise ValueError("operands overlap: an output over another one, or over an input other than row for row")
 
 
 def rows_to_mx8(x: torch.Tensor, mx8: Mx8Rows | None = None, *, stream=None) -> Mx8Rows:
@@ -482,8 +490,9 @@ def rows_to_mx8(x: torch.Tensor, mx8: Mx8Rows | None = None, *, stream=None) -> 
         mx8 = Mx8Rows.allocate(x.shape[0], x.shape[1], x.device)
     _need_mx8(mx8, "mx8", tuple(x.shape))
     _same_device(x, mx8.q, mx8.scale)
-    _check(lib.lmoe_rows_to_mx8(_ptr(x), x.shape[0], x.shape[1], _ptr(mx8.q), _ptr(mx8.scale), _stream(stream)),
-           "lmoe_rows_to_mx8")
+    status = lib.lmoe_rows_to_mx8(_ptr(x), x.shape[0], x.shape[1], _ptr(mx8.q), _ptr(mx8.scale), _stream(stream))
+    _refuse_overlap(status, x.shape[1])
+    _check(status, "lmoe_rows_to_mx8")
     return mx8
 
 
