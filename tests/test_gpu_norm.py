@@ -284,3 +284,35 @@ def test_norm_refuses_rows_that_others_still_read():
     assert torch.equal(buf[4:8], want) and torch.equal(buf[:4], keep[:4])
     native.add_rms_norm(x, w, out=x)
     assert torch.equal(buf[:4], want) and torch.equal(buf[8], keep[8])
+
+
+@pytest.mark.gpu
+def test_outputs_made_for_a_stream_are_its_own():
+    """With stream= an output that the call makes is memory of that stream's pool:
+    what the current stream still has queued on a freed block does not reach it."""
+    native = _native()
+    side = torch.cuda.Stream()
+    x, _, w = _case(64, 2048, torch.bfloat16, torch.bfloat16, 4)
+    gate = torch.empty((64, 2048), device="cuda").normal_(0, 0.05).to(torch.bfloat16)
+    logits = native.router_gate(x, gate, torch.empty((64, 64), dtype=torch.bfloat16, device="cuda"))
+    ids = native.router_topk(logits, 4)[1]
+    perm = native.permute(ids, native.Permutation.allocate(256, 64, "cuda"))
+    flat = lambda r: [t.view(torch.uint8) for t in (  # noqa: E731
+        (r.q, r.scale) if isinstance(r, native.Mx8Rows) else (r,) if isinstance(r, torch.Tensor) else
+        [v for v in r if v is not None])]
+    calls = [lambda **s: native.add_rms_norm(x, w, **s), lambda **s: native.rows_to_mx8(x, **s),
+             lambda **s: native.router_topk(logits, 4, **s)[:2], lambda **s: native.gather_rows(x, 4, perm, **s)]
+    for i, call in enumerate(calls):
+        print(f"case own stream {i}", flush=True)
+        want = [t.clone() for t in flat(call())]
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        old = [torch.empty_like(t) for t in want]
+        torch.cuda._sleep(20_000_000)          # the current stream is behind
+        for t in old:
+            t.fill_(0x55)
+        del old, t                             # their blocks are free for this stream, the fills still queued
+        got = call(stream=side)
+        side.synchronize()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(flat(got), want)), i

@@ -11,6 +11,7 @@ The C declarations live in include/latchmoe.h; `EXPORTED_SYMBOLS` lists them.
 from __future__ import annotations
 
 import atexit
+import contextlib
 import ctypes
 import os
 from dataclasses import dataclass
@@ -300,6 +301,19 @@ def _stream(stream: torch.cuda.Stream | None) -> int:
     return int(s.cuda_stream)
 
 
+def _on(stream: torch.cuda.Stream | None):
+    """Outputs that a call makes come from the pool of the stream that writes them:
+    memory of the current stream's pool may still be in use by its queued work."""
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
+def _new(shape, dtype: torch.dtype, device, stream: torch.cuda.Stream | None) -> torch.Tensor:
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with _on(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple | None = None) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
@@ -449,7 +463,7 @@ def add_rms_norm(
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
     if out is None and mx8 is None:
-        out = torch.empty_like(x)
+        out = _new(shape, bf16, x.device, stream)
     elif out is not None and not _fits(out, bf16, shape, here):
         _refuse(out, "out", bf16, shape)
     q = scale = None
@@ -487,7 +501,8 @@ def rows_to_mx8(x: torch.Tensor, mx8: Mx8Rows | None = None, *, stream=None) -> 
     if x.dim() != 2:
         raise ValueError(f"x must be [T, H], got {tuple(x.shape)}")
     if mx8 is None:
-        mx8 = Mx8Rows.allocate(x.shape[0], x.shape[1], x.device)
+        with _on(stream):
+            mx8 = Mx8Rows.allocate(x.shape[0], x.shape[1], x.device)
     _need_mx8(mx8, "mx8", tuple(x.shape))
     _same_device(x, mx8.q, mx8.scale)
     status = lib.lmoe_rows_to_mx8(_ptr(x), x.shape[0], x.shape[1], _ptr(mx8.q), _ptr(mx8.scale), _stream(stream))
@@ -561,9 +576,9 @@ def router_topk(
     dev = logits.device
     kw = int(top_k) + int(n_shared)
     if w_bf16 is None:
-        w_bf16 = torch.empty((T, kw), dtype=torch.bfloat16, device=dev)
+        w_bf16 = _new((T, kw), torch.bfloat16, dev, stream)
     if ids is None:
-        ids = torch.empty((T, kw), dtype=torch.int32, device=dev)
+        ids = _new((T, kw), torch.int32, dev, stream)
     _need(w_bf16, "topk_weights", torch.bfloat16, (T, kw))
     _need(ids, "topk_ids", torch.int32, (T, kw))
     if w_f32 is not None:
@@ -621,9 +636,9 @@ def router_topk_permute(
     dev = logits.device
     kw = int(top_k) + int(n_shared)
     if w_bf16 is None:
-        w_bf16 = torch.empty((T, kw), dtype=torch.bfloat16, device=dev)
+        w_bf16 = _new((T, kw), torch.bfloat16, dev, stream)
     if ids is None:
-        ids = torch.empty((T, kw), dtype=torch.int32, device=dev)
+        ids = _new((T, kw), torch.int32, dev, stream)
     _need(w_bf16, "topk_weights", torch.bfloat16, (T, kw))
     _need(ids, "topk_ids", torch.int32, (T, kw))
     if w_f32 is not None:
@@ -709,9 +724,9 @@ def router_gate_topk_permute(
     dev = x.device
     kw = int(top_k) + int(n_shared)
     if w_bf16 is None:
-        w_bf16 = torch.empty((T, kw), dtype=torch.bfloat16, device=dev)
+        w_bf16 = _new((T, kw), torch.bfloat16, dev, stream)
     if ids is None:
-        ids = torch.empty((T, kw), dtype=torch.int32, device=dev)
+        ids = _new((T, kw), torch.int32, dev, stream)
     _need(w_bf16, "topk_weights", torch.bfloat16, (T, kw))
     _need(ids, "topk_ids", torch.int32, (T, kw))
     if w_f32 is not None:
@@ -794,9 +809,9 @@ def router_gate_topk_pairs(
     dev = x.device
     kw = int(top_k) + int(n_shared)
     if w_bf16 is None:
-        w_bf16 = torch.empty((T, kw), dtype=torch.bfloat16, device=dev)
+        w_bf16 = _new((T, kw), torch.bfloat16, dev, stream)
     if ids is None:
-        ids = torch.empty((T, kw), dtype=torch.int32, device=dev)
+        ids = _new((T, kw), torch.int32, dev, stream)
     _need(w_bf16, "topk_weights", torch.bfloat16, (T, kw))
     _need(ids, "topk_ids", torch.int32, (T, kw))
     if w_f32 is not None:
@@ -1148,7 +1163,7 @@ def gather_rows(x: torch.Tensor, top_k: int, perm: Permutation, out: torch.Tenso
     _need(x, "x", torch.bfloat16)
     H = x.shape[1]
     if out is None:
-        out = torch.empty((perm.n_pairs, H), dtype=torch.bfloat16, device=x.device)
+        out = _new((perm.n_pairs, H), torch.bfloat16, x.device, stream)
     _need(out, "x_sorted", torch.bfloat16, (perm.n_pairs, H))
     _check(
         lib.lmoe_gather_rows(_ptr(x), H, int(top_k), _ptr(perm.sorted_pairs), _ptr(perm.meta),
