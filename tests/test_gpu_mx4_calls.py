@@ -3,6 +3,8 @@ separate calls, the full layer's check, calls on several streams and threads,
 results that are kept, events, very long rows.  (tests/test_gpu_mx4.py checks the
 values, tests/test_gpu_mx4_layer.py the layer.)"""
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -72,3 +74,90 @@ def test_the_full_layer_fails_closed_on_any_number_of_tokens(T, rows):
             run(bad, path=path)
         assert torch.equal(_bits(run(ids)), _bits(want))
     native.device_flags(clear=True)
+
+
+def _experts(kind, E, H, I, T, seed):
+    """(rows, w13, w2) of bf16 experts, or of 4-bit ones with bf16 or 8-bit rows."""
+    layer = Layer(H, I, E, T, "mx8" if kind == "mx8" else "bf16", seed)
+    if kind != "bf16 experts":
+        return layer.x, layer.w13, layer.w2
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w13, w2 = (torch.empty(s, device="cuda").normal_(0, 0.05, generator=g).to(torch.bfloat16)
+               for s in ((E, 2 * I, H), (E, H, I)))
+    return layer.x, w13, w2
+
+
+KINDS = ("bf16 experts", "bf16", "mx8")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [1, 3, 9, 200])
+def test_default_calls_on_two_streams_and_from_two_threads(T, kind):
+    """Calls of one shape without a workspace of the caller's, at once."""
+    from vllm_moe_offload_amd import fused_moe
+
+    k, E, H, I = 2, 8, 512, 256
+    parts = [_experts(kind, E, H, I, T, s) for s in (5, 6)]
+    rng = np.random.default_rng(T)
+    ids = [to_dev_i32(np.stack([rng.permutation(E)[:k] for _ in range(T)])) for _ in parts]
+    w = torch.full((T, k), 0.5, dtype=torch.bfloat16, device="cuda")
+
+    def call(i):
+        x, w13, w2 = parts[i]
+        return fused_moe.fused_experts(x, w, ids[i], w13, w2, None,
+                                       out=torch.empty((T, H), dtype=torch.bfloat16, device="cuda"))
+
+    want = [call(0), call(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(_bits(o), _bits(want[i])) for i in (0, 1) for o in got[i])
+
+    got = [[], []]
+    ready = threading.Barrier(2)
+
+    def work(i):
+        ready.wait()
+        for _ in range(20):
+            got[i].append(call(i))  # both on the default stream
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert all(len(g) == 20 for g in got)
+    assert all(torch.equal(_bits(o), _bits(want[i])) for i in (0, 1) for o in got[i])
+
+
+def test_workspaces_of_streams_threads_and_captures():
+    from vllm_moe_offload_amd import fused_moe
+
+    get = lambda device="cuda", **kw: fused_moe.get_workspace(7, 2, 4, 64, 32, device, **kw)  # noqa: E731
+    here = get()
+    assert get("cuda:0") is here and get(torch.device("cuda", 0)) is here and get(tag="other") is not here
+    side, other = torch.cuda.Stream(), []
+    with torch.cuda.stream(side):
+        there = get()
+        assert there is not here and get() is there
+    t = threading.Thread(target=lambda: other.append(get()))
+    t.start()
+    t.join()
+    assert other[0] is not here and other[0] is not there
+    assert get() is here
+    # a capture takes the warm-up's, from whichever stream and thread that was
+    warm = get(tag="warm")
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            assert get(tag="warm") is warm
+            warm.out.fill_(1.0)
+    assert get(tag="warm") is warm
+    fused_moe.clear_workspaces()
+    assert get(tag="warm") is not warm

@@ -31,6 +31,7 @@ _run_b2_full_layer_reference :3472-3650; MoEFusedExpertsInput fields
 from __future__ import annotations
 
 import os
+import threading
 from dataclasses import dataclass, field
 from time import perf_counter
 
@@ -68,8 +69,17 @@ class MoEWorkspace:
         return p
 
 
-_WORKSPACES: dict[tuple, MoEWorkspace] = {}
-_DEVICE_NAMES: dict = {}  # of torch.device or str: making the name takes longer than finding the workspace
+_WORKSPACES: dict[tuple, MoEWorkspace] = {}  # by shape, stream and thread
+_WARMED: dict[tuple, MoEWorkspace] = {}      # by shape: the last one made outside a capture
+_DEVICES: dict = {}  # (type, index) of a torch.device or str; asking takes longer than finding the workspace
+
+
+def _device_key(device) -> tuple:
+    key = _DEVICES.get(device)
+    if key is None:
+        d = torch.device(device)
+        key = _DEVICES[device] = (d.type, d.index)
+    return key if key[1] is not None or key[0] != "cuda" else (key[0], torch.cuda.current_device())
 
 
 def rows_kind(hidden, w13_slots) -> str:
@@ -86,15 +96,23 @@ def rows_kind(hidden, w13_slots) -> str:
 def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = "", rows: str = "") -> MoEWorkspace:
     """The workspace of a layer shape.  rows: rows_kind of its experts.  4-bit
     experts' rows of a few tokens stay f32 until the combine, and bf16 act rows
-    are in two parts (their bytes are few beside the weights')."""
+    are in two parts (their bytes are few beside the weights').
+
+    Calls that take the same workspace must run one after the other, so each
+    stream (the device's current one) and each host thread has its own.  A
+    capture takes the one its warm-up made, on whichever stream that was, so a
+    graph shares it with eager calls and other graphs of the shape: where they may
+    run at once, give one of them a tag of its own and pass it as workspace=."""
     if rows not in ("", "bf16", "mx8"):
         raise ValueError(f"unknown rows {rows!r}")
-    where = _DEVICE_NAMES.get(device)
-    if where is None:
-        where = _DEVICE_NAMES[device] = str(device)
-    key = (int(T), int(k), int(P), int(H), int(I), where, tag, rows)
+    where = _device_key(device)
+    shape = (int(T), int(k), int(P), int(H), int(I), where, tag, rows)
+    key = (shape, native.current_stream_handle(where[1]) if where[0] == "cuda" else 0, threading.get_ident())
     ws = _WORKSPACES.get(key)
     if ws is None:
+        capturing = where[0] == "cuda" and _is_current_graph_capturing()
+        if capturing and shape in _WARMED:
+            return _WARMED[shape]
         N = T * k
         few = rows != "" and N <= native.FUSED_DECODE_MAX_PAIRS
         y_dtype = torch.float32 if few else torch.bfloat16
@@ -108,11 +126,14 @@ def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = 
         if rows:
             ws.mx4 = native.Mx4Buffers(ws.perm, ws.act, ws.y)
         _WORKSPACES[key] = ws
+        if not capturing:
+            _WARMED[shape] = ws
     return ws
 
 
 def clear_workspaces() -> None:
     _WORKSPACES.clear()
+    _WARMED.clear()
 
 
 # ---------------------------------------------------------------------------

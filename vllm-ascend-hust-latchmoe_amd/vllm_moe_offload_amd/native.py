@@ -301,6 +301,13 @@ def _stream(stream: torch.cuda.Stream | None) -> int:
     return int(s.cuda_stream)
 
 
+def current_stream_handle(device_index: int) -> int:
+    """The raw handle of a device's current stream (0: the default stream)."""
+    if _raw_stream is not None:
+        return _raw_stream(device_index)
+    return int(torch.cuda.current_stream(device_index).cuda_stream)
+
+
 def _on(stream: torch.cuda.Stream | None):
     """Outputs that a call makes come from the pool of the stream that writes them:
     memory of the current stream's pool may still be in use by its queued work."""
