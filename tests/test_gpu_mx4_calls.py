@@ -161,3 +161,48 @@ def test_workspaces_of_streams_threads_and_captures():
     assert get(tag="warm") is warm
     fused_moe.clear_workspaces()
     assert get(tag="warm") is not warm
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [1, 5, 60])
+def test_results_are_the_callers(T, kind):
+    """A result made by the call outlives the next call of its shape."""
+    from vllm_moe_offload_amd import fused_moe
+
+    E, H, I, k = 16, 256, 128, 4
+    x, w13, w2 = _experts(kind, E, H, I, T, 6)
+    rng = np.random.default_rng(T)
+    w = torch.full((T, k), 0.25, dtype=torch.bfloat16, device="cuda")
+    ids = [to_dev_i32(np.stack([rng.permutation(E)[:k] for _ in range(T)])) for _ in range(2)]
+    ident = torch.arange(E, dtype=torch.int32, device="cuda")
+
+    def contract(i):
+        inp = fused_moe.MoEFusedExpertsInput(
+            hidden_states=x, topk_weights=w, topk_ids=i, weights=fused_moe.MoEWeights(w13, w2),
+            routing=fused_moe.MoERoutingParams(log2phy=ident))
+        return fused_moe.run_fused_experts_contract(inp).routed_out
+
+    for call in (contract, lambda i: fused_moe.fused_experts(x, w, i, w13, w2, ident)):
+        first = call(ids[0])
+        kept = first.clone()
+        second = call(ids[1])
+        assert torch.equal(_bits(first), _bits(kept)) and not torch.equal(first, second)
+
+
+@pytest.mark.parametrize("device_waves", [False, True])
+def test_results_of_waves_and_of_the_full_layer_are_the_callers(device_waves):
+    from tests.test_gpu_mx4_layer import E, _layer, _weights, _x
+    from vllm_moe_offload_amd import fused_moe
+
+    w13, w2, gate = _weights(12)
+    layer, rt = _layer(211, w13, w2, gate, slots=8, b2_wave_prefill=True, device_wave_prefill=device_waves)
+    runs = [lambda **a: fused_moe.run_full_layer(rt, **a),
+            lambda **a: fused_moe.run_device_waves(rt, **a) if device_waves else fused_moe.run_wave_prefill(rt, **a)[0]]
+    for run in runs:
+        res = []
+        for seed in (1, 2):
+            x = _x(150, seed)
+            w, ids, _ = fused_moe.route(x, gate, layer.router_spec)
+            out = run(layer_id=211, hidden=x, topk_weights=w, topk_ids=ids, num_logical_experts=E)
+            res.append((out, out.clone()))
+        assert torch.equal(*res[0]) and not torch.equal(res[0][0], res[1][0])

@@ -186,6 +186,12 @@ def route(hidden: torch.Tensor, gate_weight: torch.Tensor | None, spec: RouterSp
     return w, ids, router_logits
 
 
+def _result(out: torch.Tensor | None, hidden) -> torch.Tensor:
+    """The caller's output, or a new one: the workspaces that calls choose for
+    themselves serve the next call too, so no result is left in one."""
+    return out if out is not None else torch.empty(tuple(hidden.shape), dtype=torch.bfloat16, device=hidden.device)
+
+
 # ---------------------------------------------------------------------------
 # one pass over the slot bank
 # ---------------------------------------------------------------------------
@@ -211,6 +217,9 @@ def fused_experts(
     may name one expert twice: the decode body takes its general form,
     which holds no one-pair-per-slot assumption.
 
+    The result is out; without it a new tensor, or with a workspace of the
+    caller's that workspace's out, which its next call overwrites.
+
     Over 4-bit banks (uint8, mxfp4.pack_experts) hidden is bf16 or
     native.Mx8Rows; few tokens go straight from their ids, without a permutation
     in the workspace."""
@@ -234,7 +243,7 @@ def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2
         ws = get_workspace(T, k, P, H, w13_slots.shape[1] // 2, hidden.device, rows=rows_kind(hidden, w13_slots))
     if ws.mx4 is None:
         raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
-    dst = ws.out[:T] if out is None else out
+    dst = _result(out, hidden) if workspace is None or out is not None else ws.out[:T]
     if path == native.LMOE_PATH_AUTO:
         path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel(), isinstance(hidden, native.Mx8Rows))
         if path == native.LMOE_PATH_GEMV and (T == 1 or T * k <= native.MX4_DIRECT_PAIRS and not counted):
@@ -359,7 +368,7 @@ def _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2p
     ws = workspace or get_workspace(T, k, P, H, I, hidden.device, rows=rows)
     if mx4 and ws.mx4 is None:
         raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
-    dst = out if out is not None else ws.out[:T]
+    dst = _result(out, hidden) if workspace is None or out is not None else ws.out[:T]
     if path == native.LMOE_PATH_AUTO:
         path = _bank_layer_path(hidden, k, w13_slots, log2phy, overflow)
     # the decode body; past its pair count path GEMV runs the two GEMVs apart
@@ -628,7 +637,9 @@ def run_fused_experts_contract(inp, *, result_cls=FusedExpertsResult, record_eve
     """The hook's body: experts over the input's weights (a slot bank with
     its log2phy when prepared), returning the result contract with the
     per-slot token counts (group_list_type 1) and, if asked for, the events
-    before dispatch (permutation), before GMM2 and before the combine."""
+    before dispatch (permutation), before GMM2 and before the combine.
+    expert_tokens is the workspace's count table: the next call of the shape on
+    this stream overwrites it."""
     check_supported_input(inp)
     hidden, w, ids = inp.hidden_states, inp.topk_weights, inp.topk_ids
     routing = getattr(inp, "routing", None)
@@ -870,7 +881,7 @@ def run_wave_prefill(
                 wp["mlp_ms"] = round((perf_counter() - t_mlp) * 1000.0, 3)  # host issue time
                 wp["issue_end_to_compute_ms"] = round((t_wait - wp.pop("_issue_end")) * 1000.0, 3)
     t_scatter = perf_counter()
-    dst = out if out is not None else ws.out[:T]
+    dst = _result(out, hidden)
     native.combine(ws.y[: T * k], topk_weights, dst, row_mask=ws.perm.row_idx[: T * k], add=add)
     t_end = perf_counter()
     report.seconds = t_end - t0
@@ -1059,7 +1070,7 @@ def run_device_waves(
                     stages[b].clear_slot(sid, force=True)
     else:
         compute.wait_stream(tx)  # the forked transfer stream rejoins the capture
-    dst = out if out is not None else ws.out[:T]
+    dst = _result(out, hidden)
     native.combine(ws.y[: T * k], topk_weights, dst, row_mask=ws.perm.row_idx[: T * k], add=add)
     return dst
 
@@ -1087,6 +1098,7 @@ def run_full_layer(
     ws = get_workspace(T, k, prepared.physical_expert_count, H, int(prepared.w1.shape[1]) // 2, hidden.device, tag="full",
                        rows=rows_kind(hidden, prepared.w1))
     checked = not _is_current_graph_capturing()
+    out = _result(out, hidden)
     args = (hidden, topk_weights, topk_ids, prepared.w1, prepared.w2, prepared.log2phy)
     if mxfp4.is_mx4(prepared.w1):
         dst = _mx4_fused_experts(*args, add=add, out=out, path=path, workspace=ws, counted=checked)

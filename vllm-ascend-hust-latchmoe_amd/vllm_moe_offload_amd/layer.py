@@ -186,7 +186,8 @@ class SlotMoELayer(torch.nn.Module):
         zeros = _zeros_i32(T, x.device)
         ws = get_workspace(T, 1, 1, H, int(self.shared_w13.shape[1]) // 2, x.device, tag=f"shared{self.layer_id}",
                            rows=rows_kind(x, self.shared_w13))
-        return fused_experts(x, ones, zeros, self.shared_w13, self.shared_w2, None, workspace=ws)
+        return fused_experts(x, ones, zeros, self.shared_w13, self.shared_w2, None, workspace=ws,
+                             out=torch.empty((T, H), dtype=torch.bfloat16, device=x.device))
 
     @property
     def has_separate_shared_expert(self) -> bool:
