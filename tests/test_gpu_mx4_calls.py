@@ -206,3 +206,44 @@ def test_results_of_waves_and_of_the_full_layer_are_the_callers(device_waves):
             out = run(layer_id=211, hidden=x, topk_weights=w, topk_ids=ids, num_logical_experts=E)
             res.append((out, out.clone()))
         assert torch.equal(*res[0]) and not torch.equal(res[0][0], res[1][0])
+
+
+@pytest.mark.parametrize("T", [1, 3])
+def test_events_come_where_the_contract_has_them(T, monkeypatch):
+    """Before the permutation, before GMM2 and before the combine; one token, whose
+    down product has the combine in it, records the last two after its permutation."""
+    from vllm_moe_offload_amd import fused_moe, native
+
+    E, H, I, k = 8, 256, 96, 2
+    layer = Layer(H, I, E, T, "bf16", 3)
+    w = torch.full((T, k), 0.5, dtype=torch.bfloat16, device="cuda")
+    ids = to_dev_i32(np.stack([np.random.default_rng(t).permutation(E)[:k] for t in range(T)]))
+    order = []
+
+    def spy(name):
+        call = getattr(native, name)
+
+        def run(*a, **kw):
+            order.append(name)
+            return call(*a, **kw)
+
+        monkeypatch.setattr(native, name, run)
+
+    for name in ("permute", "gateup_silu", "down", "combine", "mx4_decode_one", "mx4_fused_moe"):
+        spy(name)
+
+    class Event(torch.cuda.Event):
+        def record(self, stream=None):
+            order.append("event")
+            super().record(*([] if stream is None else [stream]))
+
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    inp = fused_moe.MoEFusedExpertsInput(hidden_states=layer.x, topk_weights=w, topk_ids=ids,
+                                         weights=fused_moe.MoEWeights(layer.w13, layer.w2))
+    res = fused_moe.run_fused_experts_contract(inp, record_events=True)
+    torch.cuda.synchronize()
+    assert all(e.query() for e in (res.before_dispatch_evt, res.before_gmm2_evt, res.before_combine_evt))
+    if T == 1:
+        assert order == ["event", "permute", "event", "event", "mx4_decode_one"]
+    else:
+        assert order == ["event", "permute", "gateup_silu", "event", "down", "event", "combine"]

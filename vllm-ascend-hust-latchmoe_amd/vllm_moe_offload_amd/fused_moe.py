@@ -379,9 +379,11 @@ def _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2p
     if mx4 and T == 1 and path == native.LMOE_PATH_GEMV and (overflow is None or log2phy is not None):
         # one form of one token, with an overflow pass or without; the permutation is for its counts alone
         if events:
-            for e in events:
-                e.record()
+            events[0].record()
         native.permute(topk_ids, ws.perm, log2phy=log2phy, skip_unmapped=overflow is not None, block_m=bm)
+        if events:  # GMM2 has the combine in it
+            events[1].record()
+            events[2].record()
         native.mx4_decode_one(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
                               second=_second_bank(overflow))
         return dst, ws
