@@ -459,7 +459,8 @@ long long lmoe_mx4_bytes(int N, int K);
  * LMOE_PATH_AUTO; the two add the same products in different orders, each the
  * same way whatever the batch, the slots and block_m are.
  * H % 32 == 0, I % 32 == 0, x / act, banks and y 16-byte aligned (scales any); in
- * row tiles MX8 rows of at most 32640 columns; else LMOE_ERR_SHAPE. */
+ * row tiles of 128, 64 and 32 rows MX8 rows of at most 32640, 73600 and 147200
+ * columns (AUTO: the split-K kernel past that); else LMOE_ERR_SHAPE. */
 int lmoe_mx4_gateup_silu(const void* x, const void* x_scale, int T, int H,
                          int I, int k, const void* w13_slots, int n_slots,
                          const int32_t* offsets, const int32_t* sorted_pairs,

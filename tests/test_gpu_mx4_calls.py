@@ -247,3 +247,73 @@ def test_events_come_where_the_contract_has_them(T, monkeypatch):
         assert order == ["event", "permute", "event", "event", "mx4_decode_one"]
     else:
         assert order == ["event", "permute", "gateup_silu", "event", "down", "event", "combine"]
+
+
+def _long_rows(T, K, seed):
+    """8-bit rows of more columns than one call of rows_to_mx8 takes."""
+    from vllm_moe_offload_amd import native
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.empty((T * (K // 320), 320), device="cuda").normal_(generator=g).to(torch.bfloat16)
+    r = native.rows_to_mx8(x)
+    return native.Mx8Rows(r.q.view(T, K), r.scale.view(T, K // 32))
+
+
+@pytest.mark.parametrize("bm", [32, 64, 128])
+@pytest.mark.parametrize("side", ["gateup", "down"])
+def test_the_longest_8_bit_rows_of_each_height(bm, side):
+    """Rows whose scales just fit a tile's LDS, against the split-K kernel, which
+    keeps none there: sums of the same products, cut otherwise."""
+    from vllm_moe_offload_amd import mxfp4, native
+
+    from tests.test_gpu_mx4 import sum_error
+
+    K, T, out = native.MX4_MAX_COLUMNS_MX8[bm], bm + 3, 64
+    print(f"case longest rows K={K} block_m={bm} {side}", flush=True)
+    x = _long_rows(T, K, bm)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    codes, scales = mxfp4.quantize(torch.empty((1, out, K), device="cuda").normal_(0, 0.05, generator=g))
+    ids = torch.zeros((T, 1), dtype=torch.int32, device="cuda")
+    ids[T - 2] = -1
+    perm = native.permute(ids, native.Permutation.allocate(T, 1, "cuda"), skip_unmapped=True, block_m=bm)
+    xv = x.float().double().cpu().numpy()[perm.sorted_pairs.cpu().numpy()[:T - 1]] if side == "gateup" else \
+        x.float().double().cpu().numpy()[:T - 1]
+    wv = mxfp4.dequantize(codes, scales)[0].double().cpu().numpy()
+    want, err = xv @ wv.T, sum_error(xv, wv, True)
+    if side == "down":
+        bank = mxfp4.pack_w2(codes, scales)
+        for path in (native.LMOE_PATH_GEMV, native.LMOE_PATH_MFMA):
+            y = torch.full((T, out), -7.0, dtype=torch.float32, device="cuda")
+            native.down(x, bank, perm, y, path=path)
+            got = y.cpu().double().numpy()[perm.sorted_pairs.cpu().numpy()[:T - 1]]
+            assert np.all(np.abs(got - want) <= err * (1 + 2.0**-24) + 2.0**-24 * np.abs(want))
+            assert torch.all(y[T - 2] == -7.0)
+    else:
+        from tests.test_gpu_mx4 import check_act
+
+        bank = mxfp4.pack_w13(codes, scales)
+        for path in (native.LMOE_PATH_GEMV, native.LMOE_PATH_MFMA):
+            act = native.Mx8Rows.allocate(T, out // 2, "cuda")
+            native.gateup_silu(x, 1, bank, perm, act, path=path)
+            sc = np.ldexp(1.0, act.scale.cpu().numpy().astype(np.int64) - 127)[:T - 1]
+            check_act(act.float().double().cpu().numpy()[:T - 1], want[:, :32], want[:, 32:], err[:, :32], err[:, 32:], sc)
+
+
+def test_many_long_8_bit_rows_choose_a_height_that_holds_them():
+    """The norm gives rows up to 32768 columns, more than the tallest tile holds."""
+    from vllm_moe_offload_amd import fused_moe, mxfp4, native
+
+    T, H, I = 8300, 32704, 1024
+    assert native.mx4_block_m(T, 1, I) == 128 and H > native.MX4_MAX_COLUMNS_MX8[128]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w13, w2 = mxfp4.pack_experts(torch.empty((1, 2 * I, H), device="cuda").normal_(0, 0.05, generator=g),
+                                 torch.empty((1, H, I), device="cuda").normal_(0, 0.05, generator=g))
+    x = native.rows_to_mx8(torch.empty((T, H), dtype=torch.bfloat16, device="cuda").normal_(generator=g))
+    ids, w = torch.zeros((T, 1), dtype=torch.int32, device="cuda"), torch.ones((T, 1), dtype=torch.bfloat16, device="cuda")
+    out = fused_moe.fused_experts(x, w, ids, w13, w2, None)
+    ws = fused_moe.get_workspace(T, 1, 1, H, I, "cuda", tag="long", rows="mx8")
+    want = native.mx4_fused_moe(x, w, ids, w13, w2, None, ws.mx4, torch.empty_like(out), path=native.LMOE_PATH_MFMA,
+                                block_m=32)
+    torch.cuda.synchronize()
+    assert torch.equal(_bits(out), _bits(want)) and out[::100].isfinite().all()
+    fused_moe.clear_workspaces()

@@ -251,3 +251,30 @@ def test_norm_entries_refuse_any_overlap_but_row_for_row():
     for kw in (dict(q=x + 16), dict(q=x + size["x"] - 16), dict(q=x + 16 - size["q"]), dict(s=x), dict(s=x + size["x"] - 1),
                dict(s=x + 1 - size["s"]), dict(s=q), dict(s=q + size["q"] - 1)):
         assert rows(**kw) == 1000, kw
+
+
+def test_row_tiles_take_8_bit_rows_up_to_their_limits():
+    """The heights that the rules choose hold the rows, and the library draws the
+    same lines."""
+    from vllm_moe_offload_amd import native
+
+    lib = native.load_library()
+    limits = native.MX4_MAX_COLUMNS_MX8
+    assert tuple(limits) == native.MX4_BLOCK_M
+    gu = lambda bm, H, I: lib.lmoe_mx4_gateup_silu(P16, P16, 2, H, I, 1, P16, 4, P16, P16, P16, P16, P16, 2, bm, 2, P16, P16, 0, N)
+    dn = lambda bm, H, I: lib.lmoe_mx4_down(P16, P16, 0, H, I, P16, 4, P16, P16, P16, P16, P16, 2, bm, 2, P16, 0, N)
+    for bm, top in limits.items():
+        # LDS: two stages of rows (32-row tiles: of two chunks), a pair id and all scales a row
+        room = 160 * 1024 - bm * 128 * (4 if bm == 32 else 2) - 4 * bm
+        chunks = room // (4 * bm)
+        assert top == 128 * (chunks - chunks % 2 if bm == 32 else chunks)
+        assert gu(bm, top + 32, 32) == 1001 and dn(bm, 32, top + 32) == 1001
+    for columns in (32, 2048, 32640, 32672, 73600, 73632, 147200):
+        for pairs, experts in ((1 << 20, 1), (1 << 20, 128), (5000, 16), (100, 8)):
+            assert native.mx4_path(pairs, experts, True, columns) == native.LMOE_PATH_MFMA
+            bm = native.mx4_block_m(pairs, experts, 4096, columns)
+            assert columns <= limits[bm] and bm <= native.mx4_block_m(pairs, experts, 4096)
+            if columns <= limits[128]:
+                assert bm == native.mx4_block_m(pairs, experts, 4096)
+    assert native.mx4_path(1 << 20, 1, True, 147232) == native.LMOE_PATH_GEMV
+    assert native.mx4_path(1 << 20, 1, False, 147232) == native.LMOE_PATH_MFMA  # bf16 rows need no room for scales

@@ -58,11 +58,13 @@ struct Mx4Tile {
   static constexpr int STAGE = CS * PART;
   static constexpr int RPL = 64 / PIECES;            // rows one load instruction fills
   static constexpr int QA = PART / 1024 / kTileWaves;  // load instructions per wave and chunk
+  static_assert(CS_ == 1 || BM_ < 64, "room for a stage's scales");
   static_assert(QA * kTileWaves * 1024 == PART, "whole load instructions");
   static constexpr int OFF_PAIR = 2 * STAGE;         // BM pair ids
   static constexpr int OFF_SCALE = OFF_PAIR + BM * 4;
   // scales go to LDS 64 dwords at a time: two chunks of 32 rows (two chunks a stage too)
-  static int lds_bytes(int chunks) { return OFF_SCALE + (A8 ? BM * 4 * ((chunks + 1) & ~1) : 0); }
+  static constexpr int CHUNKS = BM < 64 ? 2 : 1;     // room for whole ones
+  static int lds_bytes(int chunks) { return OFF_SCALE + (A8 ? BM * 4 * ((chunks + CHUNKS - 1) / CHUNKS * CHUNKS) : 0); }
   static __device__ __forceinline__ int sw(int r) { return A8 ? (r >> 1) & 7 : (r + 4) & 15; }
 };
 

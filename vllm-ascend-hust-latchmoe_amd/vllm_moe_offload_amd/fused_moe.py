@@ -244,15 +244,17 @@ def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2
     if ws.mx4 is None:
         raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
     dst = _result(out, hidden) if workspace is None or out is not None else ws.out[:T]
+    I = w13_slots.shape[1] // 2
+    mx8 = isinstance(hidden, native.Mx8Rows)
     if path == native.LMOE_PATH_AUTO:
-        path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel(), isinstance(hidden, native.Mx8Rows))
+        path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel(), mx8, max(H, I))
         if path == native.LMOE_PATH_GEMV and (T == 1 or T * k <= native.MX4_DIRECT_PAIRS and not counted):
             if counted:  # one token's form reads no permutation
                 native.permute(topk_ids, ws.perm, log2phy=log2phy)
             direct = native.mx4_decode_one if T == 1 else native.mx4_decode_few
             return direct(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add)
     return native.mx4_fused_moe(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
-                                path=path, block_m=native.mx4_block_m(T * k, P, w13_slots.shape[1] // 2))
+                                path=path, block_m=native.mx4_block_m(T * k, P, I, max(H, I) if mx8 else 0))
 
 
 def _second_bank(overflow: PreparedSlotWeights | None) -> tuple | None:
@@ -266,7 +268,7 @@ def _layer_path(hidden, k: int, n_experts: int, *w13) -> int:
     gives the unsplit layer's bits."""
     T, H = hidden.shape
     if mxfp4.is_mx4(w13[0]):
-        return native.mx4_path(T * k, n_experts, isinstance(hidden, native.Mx8Rows))
+        return native.mx4_path(T * k, n_experts, isinstance(hidden, native.Mx8Rows), max(H, int(w13[0].shape[1]) // 2))
     return native.layer_path(T, k, H, int(w13[0].shape[1]) // 2, n_experts, aligned=native.aligned16(hidden, *w13))
 
 
@@ -283,13 +285,14 @@ def _overflow_perm(hidden, k: int, overflow: PreparedSlotWeights, ws: MoEWorkspa
 
 
 def _pass_block_m(n_experts: int, H: int, I: int, device, n_pairs: int, path: int, pass_pairs: int | None = None,
-                  *, mx4: bool = False) -> int:
+                  *, rows: str = "") -> int:
     """The row-tile height to build the permutation of a pass over n_experts
     slots with: the path's own (the GEMVs read no tile table, path STREAM has
-    one height), else the MFMA kernel's for pass_pairs of n_pairs pairs.  mx4:
-    the experts are in 4 bits."""
-    if mx4:
-        return native.mx4_block_m(n_pairs if pass_pairs is None else pass_pairs, n_experts, I)
+    one height), else the MFMA kernel's for pass_pairs of n_pairs pairs.  rows:
+    rows_kind of the experts."""
+    if rows:
+        return native.mx4_block_m(n_pairs if pass_pairs is None else pass_pairs, n_experts, I,
+                                  max(H, I) if rows == "mx8" else 0)
     if path == native.LMOE_PATH_GEMV:
         return native.MFMA_BLOCK_M
     if path == native.LMOE_PATH_STREAM:
@@ -301,7 +304,7 @@ def _block_m(hidden, k: int, w13_slots, path: int) -> int:
     """_pass_block_m of a pass over a whole bank."""
     T, H = hidden.shape
     P, I = int(w13_slots.shape[0]), int(w13_slots.shape[1]) // 2
-    return _pass_block_m(P, H, I, hidden.device, T * k, path, mx4=mxfp4.is_mx4(w13_slots))
+    return _pass_block_m(P, H, I, hidden.device, T * k, path, rows=rows_kind(hidden, w13_slots))
 
 
 def _overflow_permute(hidden, topk_ids, k: int, overflow: PreparedSlotWeights, ws: MoEWorkspace, *,
@@ -866,7 +869,7 @@ def run_wave_prefill(
                 native.permute(topk_ids, ws.perm, log2phy=prepared.log2phy, skip_unmapped=True, keep_rows=not first,
                                table_len=total_logical if first else routed,
                                block_m=_pass_block_m(len(plan.waves[w]), H, I, hidden.device, T * k, mlp_path, pairs,
-                                                     mx4=mxfp4.is_mx4(prepared.w1)))
+                                                     rows=rows_kind(hidden, prepared.w1)))
                 first = False
                 native.grouped_mlp(hidden, k, prepared.w1, prepared.w2, ws.perm, ws.act_rows(T * k, mlp_path), ws.y[: T * k],
                                    path=mlp_path, pass_pairs=pairs)
@@ -1044,7 +1047,7 @@ def run_device_waves(
     released: list = [None] * len(stages)
     mlp_path = _layer_path(hidden, k, total, bank.w13_slots) if path == native.LMOE_PATH_AUTO else path
     pairs = -(-(T * k) // n_waves)  # of a wave, on average
-    bm = _pass_block_m(P, H, I, dev, T * k, mlp_path, pairs, mx4=mxfp4.is_mx4(bank.w13_slots))
+    bm = _pass_block_m(P, H, I, dev, T * k, mlp_path, pairs, rows=rows_kind(hidden, bank.w13_slots))
     for w in range(n_waves):
         b = w % len(stages)
         stage, table = stages[b], tables[b]

@@ -989,11 +989,19 @@ MX4_FEW_PAIRS_PER_EXPERT = 4
 MX4_FEW_PAIRS_PER_EXPERT_MX8 = 6
 
 
-def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False) -> int:
+# The longest 8-bit rows of a tile of each height: the tile keeps all their scales in LDS
+# (160 KiB, less two stages of rows and the pairs).  The split-K kernel takes any.
+MX4_MAX_COLUMNS_MX8 = {32: 147200, 64: 73600, 128: 32640}
+
+
+def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False, columns: int = 0) -> int:
     """The path of a layer of 4-bit experts, for every pass of it: the split-K
-    kernel for few pairs per expert (mx8: of 8-bit rows), row tiles past that."""
+    kernel for few pairs per expert (mx8: of 8-bit rows) and for 8-bit rows too
+    long for any row tile (columns: the longer of x's and act's), row tiles past that."""
     few = MX4_FEW_PAIRS_PER_EXPERT_MX8 if mx8 else MX4_FEW_PAIRS_PER_EXPERT
-    return LMOE_PATH_GEMV if n_pairs <= few * n_experts else LMOE_PATH_MFMA
+    if n_pairs <= few * n_experts or (mx8 and columns > MX4_MAX_COLUMNS_MX8[MX4_BLOCK_M[0]]):
+        return LMOE_PATH_GEMV
+    return LMOE_PATH_MFMA
 
 
 # Row-tile heights but the last, with the most pairs per slot, on average, and the most
@@ -1018,13 +1026,18 @@ def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False) -> int:
 MX4_HEIGHTS = ((32, 32, 640), (64, 100, 1024))
 
 
-def mx4_block_m(n_pairs: int, n_experts: int, intermediate: int = 1024) -> int:
+def mx4_block_m(n_pairs: int, n_experts: int, intermediate: int = 1024, mx8_columns: int = 0) -> int:
     """Row-tile height of 4-bit experts' products (the permutation's block_m) for
-    n_pairs pairs over n_experts slots of experts intermediate wide."""
+    n_pairs pairs over n_experts slots of experts intermediate wide.  mx8_columns:
+    the longer of x's and act's rows, where they are in 8 bits."""
+    best = MX4_BLOCK_M[-1]
     for bm, pairs, groups in MX4_HEIGHTS:
         if n_pairs <= pairs * n_experts or (n_pairs // bm + n_experts) * -(-intermediate // 128) <= groups:
-            return bm
-    return MX4_BLOCK_M[-1]
+            best = bm
+            break
+    while mx8_columns > MX4_MAX_COLUMNS_MX8[best] and best > MX4_BLOCK_M[0]:
+        best //= 2
+    return best
 
 
 @dataclass
