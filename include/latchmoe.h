@@ -455,8 +455,9 @@ long long lmoe_mx4_bytes(int N, int K);
  * few act values.  y is bf16 or f32 (y_f32) by pair,
  * rows of unplaced pairs untouched.
  * path = LMOE_PATH_GEMV (few rows per slot: a workgroup's waves split K),
- * LMOE_PATH_MFMA (row tiles of block_m, the height given to lmoe_permute) or
- * LMOE_PATH_AUTO; the two add the same products in different orders, each the
+ * LMOE_PATH_MFMA (row tiles of block_m, the height given to lmoe_permute: 32, 64
+ * or 128) or LMOE_PATH_AUTO (row tiles past 4 pairs per slot of bf16 rows, 6 of
+ * MX8 rows; another block_m is then LMOE_ERR_SHAPE); the two add the same products in different orders, each the
  * same way whatever the batch, the slots and block_m are.
  * H % 32 == 0, I % 32 == 0, x / act, banks and y 16-byte aligned (scales any); in
  * row tiles of 128, 64 and 32 rows MX8 rows of at most 32640, 73600 and 147200

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from tests._util import to_dev_i32
-from tests.test_gpu_mx4 import ROWS, Layer
+from tests.test_gpu_mx4 import ROWS, Layer, check_act, check_layer, sum_error
 
 pytestmark = pytest.mark.gpu
 
@@ -266,8 +266,6 @@ def test_the_longest_8_bit_rows_of_each_height(bm, side):
     keeps none there: sums of the same products, cut otherwise."""
     from vllm_moe_offload_amd import mxfp4, native
 
-    from tests.test_gpu_mx4 import sum_error
-
     K, T, out = native.MX4_MAX_COLUMNS_MX8[bm], bm + 3, 64
     print(f"case longest rows K={K} block_m={bm} {side}", flush=True)
     x = _long_rows(T, K, bm)
@@ -289,8 +287,6 @@ def test_the_longest_8_bit_rows_of_each_height(bm, side):
             assert np.all(np.abs(got - want) <= err * (1 + 2.0**-24) + 2.0**-24 * np.abs(want))
             assert torch.all(y[T - 2] == -7.0)
     else:
-        from tests.test_gpu_mx4 import check_act
-
         bank = mxfp4.pack_w13(codes, scales)
         for path in (native.LMOE_PATH_GEMV, native.LMOE_PATH_MFMA):
             act = native.Mx8Rows.allocate(T, out // 2, "cuda")
@@ -317,3 +313,30 @@ def test_many_long_8_bit_rows_choose_a_height_that_holds_them():
     torch.cuda.synchronize()
     assert torch.equal(_bits(out), _bits(want)) and out[::100].isfinite().all()
     fused_moe.clear_workspaces()
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_auto_needs_a_permutation_of_its_own_tiles(rows):
+    """One built at the default height, the bf16 kernels': taken with few pairs per
+    slot, refused by name past them; the split-K kernel by name takes it."""
+    from vllm_moe_offload_amd import native
+
+    E, H, I = 4, 256, 96
+    few = native.MX4_FEW_PAIRS_PER_EXPERT_MX8 if rows == "mx8" else native.MX4_FEW_PAIRS_PER_EXPERT
+    for T in (few * E, few * E + 1):
+        layer = Layer(H, I, E, T, rows, 6)
+        ids = torch.arange(T, dtype=torch.int32, device="cuda").remainder_(E).view(T, 1)
+        perm = native.permute(ids, native.Permutation.allocate(T, E, "cuda"))
+        act, y = layer.act_buffer(T), torch.empty((T, H), dtype=torch.float32, device="cuda")
+        want = native.grouped_mlp(layer.x, 1, layer.w13, layer.w2, perm, act, y, path=native.LMOE_PATH_GEMV).clone()
+        if T == few * E:
+            assert torch.equal(native.grouped_mlp(layer.x, 1, layer.w13, layer.w2, perm, act, y), want)
+            continue
+        for call in (lambda: native.gateup_silu(layer.x, 1, layer.w13, perm, act),
+                     lambda: native.down(act, layer.w2, perm, y),
+                     lambda: native.grouped_mlp(layer.x, 1, layer.w13, layer.w2, perm, act, y)):
+            with pytest.raises(ValueError, match="block_m 256"):
+                call()
+        native.permute(ids, perm, block_m=native.mx4_block_m(T, E, I))
+        native.grouped_mlp(layer.x, 1, layer.w13, layer.w2, perm, act, y)
+        check_layer(layer, perm, 1, act, y, ids.cpu().numpy().flatten())

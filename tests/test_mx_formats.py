@@ -278,3 +278,23 @@ def test_row_tiles_take_8_bit_rows_up_to_their_limits():
                 assert bm == native.mx4_block_m(pairs, experts, 4096)
     assert native.mx4_path(1 << 20, 1, True, 147232) == native.LMOE_PATH_GEMV
     assert native.mx4_path(1 << 20, 1, False, 147232) == native.LMOE_PATH_MFMA  # bf16 rows need no room for scales
+
+
+def test_auto_refuses_tiles_of_another_kernel():
+    """A permutation built for other row tiles, where row tiles are due: refused by
+    AUTO as by an explicit path; with few pairs per slot no height is needed."""
+    import ctypes
+
+    from vllm_moe_offload_amd import native
+
+    lib = native.load_library()
+    P = 4
+    v = {n: P16 for n, _ in native._Mx4Workspace._fields_}
+    for a8, few in ((P16, 6), (N, 4)):
+        n = few * P + 1
+        ws = native._Mx4Workspace(**{**v, "y_f32": 1, "act_split": 0, "act_scale": a8})
+        for bm in (96, 256, 320, 0):
+            assert lib.lmoe_mx4_gateup_silu(P16, a8, n, 64, 32, 1, P16, P, P16, P16, P16, P16, P16, n, bm, 0, P16, a8, 0, N) == 1001
+            assert lib.lmoe_mx4_down(P16, a8, 0, 64, 32, P16, P, P16, P16, P16, P16, P16, n, bm, 0, P16, 1, N) == 1001
+            assert lib.lmoe_mx4_fused_moe(P16, a8, n, 64, 32, 1, P16, P16, P, P16, P16, N, 0, 0, bm, ctypes.addressof(ws), N,
+                                          P16, N) == 1001

@@ -125,14 +125,24 @@ static int launch_tiles(const Mx4Args& g, int block_m, hipStream_t stream) {
 // (native.py has the figures)
 constexpr int kFewPairsPerSlot[2] = {4, 6};
 
+static bool many_pairs(bool a8, int n_pairs, int P) { return n_pairs > static_cast<long long>(kFewPairsPerSlot[a8]) * P; }
+
 static bool takes_tiles(int path, int block_m, bool a8, int H, int I, int n_pairs, int P, bool split) {
   if (path != LMOE_PATH_AUTO) return path == LMOE_PATH_MFMA;
-  return !split && known_block_m(block_m) && n_pairs > static_cast<long long>(kFewPairsPerSlot[a8]) * P &&
-         tiles_fit(block_m, a8, H) && tiles_fit(block_m, a8, I);
+  return !split && known_block_m(block_m) && many_pairs(a8, n_pairs, P) && tiles_fit(block_m, a8, H) &&
+         tiles_fit(block_m, a8, I);
+}
+
+// AUTO with a permutation built for other tiles (the bf16 kernels' 96, 256 or 320 rows):
+// an error where row tiles are due, as with an explicit path.  The split-K kernel is
+// right for any number of rows, but reads the weights once for every 32 of them.
+static bool lacks_height(int path, int block_m, bool a8, int n_pairs, int P, bool split) {
+  return path == LMOE_PATH_AUTO && !split && !known_block_m(block_m) && many_pairs(a8, n_pairs, P);
 }
 
 template <bool GU>
 static int launch(const Mx4Args& g, int path, int block_m, hipStream_t stream) {
+  if (lacks_height(path, block_m, g.a_scale != nullptr, g.n_pairs, g.P, g.split)) return LMOE_ERR_SHAPE;
   if (!takes_tiles(path, block_m, g.a_scale != nullptr, g.K, g.N, g.n_pairs, g.P, g.split)) {
     launch_few<GU, false>(g, TokenIds{}, stream);
   } else {
@@ -231,6 +241,7 @@ extern "C" int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int
     if (path == LMOE_PATH_MFMA && (!known_block_m(block_m) || !tiles_fit(block_m, x_scale != nullptr, H) ||
                                    !tiles_fit(block_m, x_scale != nullptr, I)))
       return LMOE_ERR_SHAPE;
+    if (lacks_height(path, block_m, x_scale != nullptr, static_cast<int>(n), n_slots, false)) return LMOE_ERR_SHAPE;
   }
   const int split = ws->act_split && !takes_tiles(path, block_m, x_scale != nullptr, H, I, static_cast<int>(n), n_slots, false);
   int st = lmoe_permute(ids, static_cast<int>(n), log2phy, n_log2phy, n_slots, 0, block_m, ws->counts, ws->offsets,

@@ -1227,7 +1227,8 @@ def grouped_mlp(
     pass_pairs: how many of the pairs the pass is expected to place, where it
     is one wave of its layer (chooses the kernel's form, not its bits).
     4-bit banks (mxfp4.pack_experts; uint8): x and act are both bf16 or both
-    Mx8Rows, y is bf16 or f32.  On path LMOE_PATH_GEMV (which AUTO then is) a
+    Mx8Rows, y is bf16 or f32, perm is built with block_m=mx4_block_m(..) (where
+    row tiles run, another height is refused).  On path LMOE_PATH_GEMV (which AUTO then is) a
     bf16 act may be [N, 2, I]: rows in two parts whose sum is the value, so that
     its rounding does not show in batches of few tokens."""
     if mxfp4.is_mx4(w13_slots) or mxfp4.is_mx4(w2_slots):
@@ -1350,6 +1351,13 @@ def _need_y(y, shape: tuple) -> bool:
     return y.dtype is torch.float32
 
 
+def _check_products(status: int, fn: str, perm: Permutation) -> None:
+    if status == LMOE_ERR_SHAPE and perm.block_m not in MX4_BLOCK_M:
+        raise ValueError(f"{fn}: unsupported shape; the permutation was built with block_m {perm.block_m}, row tiles "
+                         f"of 4-bit experts have {MX4_BLOCK_M} rows (mx4_block_m)")
+    _check(status, fn)
+
+
 def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, act, *, path: int, stream):
     xq, xs = _need_rows(x, "x", tuple(x.shape))
     T, H = xq.shape
@@ -1363,13 +1371,13 @@ def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, 
     _need_mx4(w13_slots, "w13_slots", perm, H, 2 * I)
     _same_device(xq, xs, w13_slots, perm.offsets, aq, as_)
     p = perm
-    _check(
+    _check_products(
         load_library().lmoe_mx4_gateup_silu(
             xq.data_ptr(), _ptr(xs), T, H, I, top_k, w13_slots.data_ptr(), p.n_slots, p.offsets.data_ptr(),
             p.sorted_pairs.data_ptr(), p.active.data_ptr(), p.tile_off.data_ptr(), p.meta.data_ptr(), n, p.block_m, path,
             aq.data_ptr(), _ptr(as_), split, _stream(stream),
         ),
-        "lmoe_mx4_gateup_silu",
+        "lmoe_mx4_gateup_silu", p,
     )
     return act
 
@@ -1382,13 +1390,13 @@ def _mx4_down(act, w2_slots: torch.Tensor, perm: Permutation, y: torch.Tensor, *
     y_f32 = _need_y(y, (n, H))
     _same_device(aq, as_, w2_slots, perm.offsets, y)
     p = perm
-    _check(
+    _check_products(
         load_library().lmoe_mx4_down(
             aq.data_ptr(), _ptr(as_), split, H, I, w2_slots.data_ptr(), p.n_slots, p.offsets.data_ptr(),
             p.sorted_pairs.data_ptr(), p.active.data_ptr(), p.tile_off.data_ptr(), p.meta.data_ptr(), n, p.block_m, path,
             y.data_ptr(), y_f32, _stream(stream),
         ),
-        "lmoe_mx4_down",
+        "lmoe_mx4_down", p,
     )
     return y
 
