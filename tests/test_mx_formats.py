@@ -298,3 +298,43 @@ def test_auto_refuses_tiles_of_another_kernel():
             assert lib.lmoe_mx4_down(P16, a8, 0, 64, 32, P16, P, P16, P16, P16, P16, P16, n, bm, 0, P16, 1, N) == 1001
             assert lib.lmoe_mx4_fused_moe(P16, a8, n, 64, 32, 1, P16, P16, P, P16, P16, N, 0, 0, bm, ctypes.addressof(ws), N,
                                           P16, N) == 1001
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "bf16"])
+def test_a_checkpoint_in_4_bits_page_locks_no_bf16_copy(fmt, tmp_path, monkeypatch):
+    """What from_checkpoint asks to page-lock: the blocks that the host store keeps."""
+    from safetensors.torch import save_file
+
+    from vllm_moe_offload_amd import layer as layer_mod
+    from vllm_moe_offload_amd.moe_offload.config import MoeOffloadConfig
+    from vllm_moe_offload_amd.moe_offload.runtime import MoeOffloadRuntime
+
+    E, H, I = 2, 64, 32
+    w13, w2 = torch.randn(E, 2 * I, H).to(torch.bfloat16), torch.randn(E, H, I).to(torch.bfloat16)
+    save_file({f"m.experts.{e}.{n}.weight": t.contiguous() for e in range(E)
+               for n, t in (("gate_proj", w13[e, :I]), ("up_proj", w13[e, I:]), ("down_proj", w2[e]))},
+              str(tmp_path / "e.safetensors"))
+    asked = {}
+    make, pack = layer_mod.create_cpu_first_expert_weights, layer_mod.mxfp4.pack_experts
+
+    def make_spy(*a, pin_memory, **kw):
+        asked["bf16"] = pin_memory
+        return make(*a, pin_memory=pin_memory, **kw)
+
+    def pack_spy(*a, pin_memory=False):
+        asked["4 bits"] = pin_memory
+        return pack(*a, pin_memory=pin_memory)
+
+    monkeypatch.setattr(layer_mod, "create_cpu_first_expert_weights", make_spy)
+    monkeypatch.setattr(layer_mod.mxfp4, "pack_experts", pack_spy)
+    rt = MoeOffloadRuntime(MoeOffloadConfig(enabled=True, num_slots=2, async_load=True, pin_host_memory=True, cpu_first_load=True))
+    assert rt.config.should_pin_host_memory
+    layer = layer_mod.SlotMoELayer.from_checkpoint(
+        tmp_path / "e.safetensors", prefix="m", layer_id=3, runtime=rt, num_experts=E, hidden_size=H, intermediate_size=I,
+        gate_weight=torch.zeros(E, H, dtype=torch.bfloat16), top_k=1, weight_format=fmt, device="cpu")
+    if fmt == "mxfp4":
+        assert asked == {"bf16": False, "4 bits": True}
+        b13, b2 = pack(w13, w2)
+        assert torch.equal(layer.w13_weight, b13) and torch.equal(layer.w2_weight, b2)
+    else:
+        assert asked == {"bf16": True} and torch.equal(layer.w13_weight, w13)

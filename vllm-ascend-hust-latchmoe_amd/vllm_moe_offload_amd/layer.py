@@ -127,13 +127,16 @@ class SlotMoELayer(torch.nn.Module):
         device only ever holds the slot bank.  kwargs are the constructor's
         (gate_weight, top_k, routing options, shared expert, device)."""
         holder = torch.nn.Module()
-        create_cpu_first_expert_weights(
+        pin = runtime.config.should_pin_host_memory
+        mx4 = kwargs.get("weight_format") == "mxfp4"
+        create_cpu_first_expert_weights(  # of 4-bit experts page-locked: the 4-bit blocks alone
             holder, num_experts=num_experts, hidden_size=hidden_size, intermediate_size=intermediate_size,
-            dtype=dtype, pin_memory=runtime.config.should_pin_host_memory)
+            dtype=dtype, pin_memory=pin and not mx4)
         load_expert_checkpoint(holder, files, prefix=prefix, names=names)
         w13, w2 = holder.w13_weight.data, holder.w2_weight.data
-        if kwargs.get("weight_format") == "mxfp4":  # the store then adopts the 4-bit blocks
-            w13, w2 = mxfp4.pack_experts(w13, w2, pin_memory=w13.is_pinned())
+        if mx4:  # the store then adopts the 4-bit blocks
+            w13, w2 = mxfp4.pack_experts(w13, w2, pin_memory=pin)
+            del holder
         layer = cls(layer_id=layer_id, runtime=runtime, w13_weight=w13, w2_weight=w2, **kwargs)
         setattr(layer, CPU_FIRST_MARKER, True)
         return layer

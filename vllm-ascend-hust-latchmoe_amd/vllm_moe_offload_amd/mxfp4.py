@@ -153,18 +153,27 @@ def unpack_w13(bank: torch.Tensor, H: int) -> tuple[torch.Tensor, torch.Tensor]:
     return part(codes), part(scales)
 
 
+def _empty(shape: tuple, device, pin: bool) -> torch.Tensor:
+    if pin:
+        try:
+            return torch.empty(shape, dtype=torch.uint8, device=device, pin_memory=True)
+        except RuntimeError:  # no device runtime, or out of page-locked memory
+            pass
+    return torch.empty(shape, dtype=torch.uint8, device=device)
+
+
 def pack_experts(w13: torch.Tensor, w2: torch.Tensor, *, pin_memory: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """4-bit banks of bf16 (or f32) experts w13 [E, 2I, H], w2 [E, H, I], an
     expert at a time: what SlotMoELayer registers for 4-bit experts.  pin_memory:
-    into page-locked memory (host weights), for the host store to adopt."""
+    into page-locked memory (host weights) where there is some, for the host store
+    to adopt."""
     if w13.dim() != 3 or w2.dim() != 3 or w13.shape[0] != w2.shape[0]:
         raise ValueError("experts are [E, 2I, H] and [E, H, I]")
     if int(w2.shape[1]) != int(w13.shape[2]) or 2 * int(w2.shape[2]) != int(w13.shape[1]):
         raise ValueError(f"w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} are not one layer's")
     out = []
     for w, pack in ((w13, pack_w13), (w2, pack_w2)):
-        bank = torch.empty((*w.shape[:2], row_bytes(int(w.shape[2]))), dtype=torch.uint8, device=w.device,
-                           pin_memory=pin_memory)
+        bank = _empty((*w.shape[:2], row_bytes(int(w.shape[2]))), w.device, pin_memory)
         for e in range(int(w.shape[0])):
             bank[e] = pack(*quantize(w[e]))
         out.append(bank)
