@@ -338,3 +338,36 @@ def test_a_checkpoint_in_4_bits_page_locks_no_bf16_copy(fmt, tmp_path, monkeypat
         assert torch.equal(layer.w13_weight, b13) and torch.equal(layer.w2_weight, b2)
     else:
         assert asked == {"bf16": True} and torch.equal(layer.w13_weight, w13)
+
+
+@pytest.mark.gpu
+def test_every_scale_is_exact_on_the_gpu():
+    """Values of every scale byte, and quantizing rows of every size, as on the host:
+    powers of two are built from their bits (a device's pow is off by a bit for some)."""
+    from vllm_moe_offload_amd import native
+
+    m = _m()
+    byte = torch.arange(256, dtype=torch.uint8)
+    codes = torch.arange(16, dtype=torch.uint8).repeat(256, 1)
+    codes = (codes | (codes.flip(1) << 4)).contiguous()                       # [256, 16]: 32 columns
+    want = torch.from_numpy(mx.values_mx4(codes.numpy(), byte.view(256, 1).numpy())).float()
+    want[255] = float("nan")
+    q = torch.arange(32, dtype=torch.uint8).repeat(256, 1) * 4                # e4m3 codes, no NaN
+    rows = native.Mx8Rows(q.view(torch.float8_e4m3fn), byte.view(256, 1))
+    v8 = torch.from_numpy(q.view(torch.float8_e4m3fn).float().numpy().astype(np.float64) *
+                          np.ldexp(1.0, byte.numpy().astype(np.int64) - 127)[:, None]).float()
+    v8[255] = float("nan")
+    for dev in ("cpu", "cuda"):
+        got = m.dequantize(codes.to(dev), byte.view(256, 1).to(dev)).cpu()
+        assert torch.equal(got[:255], want[:255]) and got[255].isnan().all(), dev
+        got = native.Mx8Rows(rows.q.to(dev), rows.scale.to(dev)).float().cpu()
+        assert torch.equal(got[:255], v8[:255]) and got[255].isnan().all(), dev
+    rng = np.random.default_rng(3)
+    ties = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0] * 4, dtype=np.float32) * rng.choice([-1.0, 1.0], 32)
+    w = np.stack([np.ldexp(ties, e) for e in range(-126, 126)]).astype(np.float32)
+    w = np.concatenate([w, np.nextafter(w, np.float32(0)), rng.standard_normal(w.shape).astype(np.float32) *
+                        np.ldexp(np.float32(1), rng.integers(-120, 120, (w.shape[0], 1)))])
+    c, s = mx.quantize_mx4(w)
+    for dev in ("cpu", "cuda"):
+        got_c, got_s = m.quantize(torch.from_numpy(w).to(dev))
+        assert np.array_equal(got_s.cpu().numpy(), s) and np.array_equal(got_c.cpu().numpy(), c), dev

@@ -40,6 +40,20 @@ def is_mx4(bank) -> bool:
     return isinstance(bank, torch.Tensor) and bank.dtype == torch.uint8
 
 
+def exp2i(e: torch.Tensor) -> torch.Tensor:
+    """2^e in f32 of integers e in [-149, 127], from its bits: torch.ldexp and pow are
+    off by a bit for some of them on a GPU."""
+    e = e.to(torch.int32)
+    small = torch.ones_like(e) << (e + 149).clamp(0, 22)  # below the normal numbers
+    return torch.where(e >= -126, (e + 127) << 23, small).view(torch.float32)
+
+
+def scale_values(scales: torch.Tensor) -> torch.Tensor:
+    """The f32 scales that scale bytes stand for (255: NaN)."""
+    v = exp2i((scales.to(torch.int32) - 127).clamp(max=127))
+    return torch.where(scales == 255, torch.full_like(v, float("nan")), v)
+
+
 def quantize(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of weights w [..., N, K].  Round to nearest even; the
     scale is the smallest power of two that keeps the group within +-6 (nothing
@@ -56,7 +70,7 @@ def quantize(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     e = (ex - 3 + (m > 0.75)).clamp_(min=-127)          # 6 = 0.75 * 2^3
     e = torch.where(amax > 0, e, torch.full_like(e, -127))
     # two exact steps: 2^127 alone would not reach the smallest scales' inverses
-    v = torch.ldexp(torch.ldexp(g, (-e // 2).unsqueeze(-1)), (-e - (-e // 2)).unsqueeze(-1))
+    v = g * exp2i(-e // 2).unsqueeze(-1) * exp2i(-e - (-e // 2)).unsqueeze(-1)
     a = v.abs()
     code = torch.zeros(a.shape, dtype=torch.uint8, device=a.device)
     for border, up in ((0.25, False), (0.75, True), (1.25, False), (1.75, True), (2.5, False), (3.5, True), (5.0, False)):
@@ -71,8 +85,7 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """The f32 weights that (codes, scales) stand for."""
     lut = torch.tensor(_VALUES + tuple(-v for v in _VALUES), device=codes.device)
     v = torch.stack([lut[(codes & 15).long()], lut[(codes >> 4).long()]], dim=-1).flatten(-2)
-    s = torch.ldexp(torch.ones_like(scales, dtype=torch.float32), scales.int() - 127)
-    s = torch.where(scales == 255, torch.full_like(s, float("nan")), s)
+    s = scale_values(scales)
     return (v.unflatten(-1, (-1, GROUP)) * s.unsqueeze(-1)).flatten(-2)
 
 

@@ -371,8 +371,7 @@ class Mx8Rows:
 
     def float(self) -> torch.Tensor:
         """The f32 values that the rows stand for (checks and exports)."""
-        s = torch.ldexp(torch.ones_like(self.scale, dtype=torch.float32), self.scale.int() - 127)
-        s = torch.where(self.scale == 255, torch.full_like(s, float("nan")), s)
+        s = mxfp4.scale_values(self.scale)
         return (self.q.float().unflatten(-1, (-1, mxfp4.GROUP)) * s.unsqueeze(-1)).flatten(-2)
 
 
