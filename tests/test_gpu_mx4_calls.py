@@ -9,8 +9,9 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import mx
 from tests._util import to_dev_i32
-from tests.test_gpu_mx4 import ROWS, Layer, check_act, check_layer, sum_error
+from tests.test_gpu_mx4 import ROWS, Layer, check_act, check_layer, run_layer, sum_error
 
 pytestmark = pytest.mark.gpu
 
@@ -340,3 +341,119 @@ def test_auto_needs_a_permutation_of_its_own_tiles(rows):
         native.permute(ids, perm, block_m=native.mx4_block_m(T, E, I))
         native.grouped_mlp(layer.x, 1, layer.w13, layer.w2, perm, act, y)
         check_layer(layer, perm, 1, act, y, ids.cpu().numpy().flatten())
+
+
+def _at(v, e):
+    """v [R, K] rounded to e4m3 at the given group exponents."""
+    s = np.ldexp(1.0, np.repeat(e, 32, axis=1))
+    g = mx.e4m3_grid()
+    return np.sign(v) * g[mx._nearest(v / s, g)] * s
+
+
+def check_rounded_act(got, act, da):
+    """MX8 act rows (values, exponents) against act in 64 bits, off by da at most: the
+    exponent is the smallest that holds the group (the formula's, or where its largest
+    value lies within da of a border the one beyond it), and the values are act's own
+    rounding at that exponent, or where act lies within da of a tie its neighbour."""
+    values, e = got
+    amax = np.abs(act).reshape(act.shape[0], -1, 32)
+    slack = da.reshape(amax.shape)
+    low, high = (np.maximum(amax - slack, 0.0)).max(axis=2), (amax + slack).max(axis=2)
+    top = lambda v: mx.group_exponents(np.repeat(v, 32, axis=1), 448.0)  # noqa: E731
+    assert np.all((top(low) <= e) & (e <= top(high)))
+    sign = np.where(act < 0, -1.0, 1.0)
+    a, b = _at(sign * np.maximum(np.abs(act) - da, 0.0), e), _at(sign * (np.abs(act) + da), e)
+    crossing = np.abs(act) <= da  # either sign
+    lo, hi = np.minimum(a, b), np.maximum(a, b)
+    lo, hi = np.where(crossing, np.minimum(lo, -hi), lo), np.where(crossing, np.maximum(hi, -lo), hi)
+    assert np.all((lo <= values) & (values <= hi)), float(np.max(np.maximum(lo - values, values - hi)))
+
+
+@pytest.mark.parametrize("H,I,counts", [(32, 32, [1, 0, 2]), (64, 96, [3, 17, 1]), (544, 288, [1, 32, 33, 2]),
+                                        (1024, 416, [5, 65, 100, 1]), (2048, 768, [1, 9, 40])])
+def test_act_in_8_bits_is_its_own_rounding(H, I, counts):
+    """The scale that the gate-up product gives a group of act, from the formula and
+    not from what it stored; groups of one row are far from those beside them."""
+    from vllm_moe_offload_amd import native
+
+    rng = np.random.default_rng(H + I)
+    P, T = len(counts), sum(counts)
+    layer = Layer(H, I, P, T, "mx8", 31)
+    # rows of very different sizes: a scale taken from another row would show at once
+    step = torch.from_numpy(rng.integers(-12, 13, (T, 1)).astype(np.int16)).cuda()
+    layer.x = native.Mx8Rows(layer.x.q, (layer.x.scale.to(torch.int16) + step).to(torch.uint8))
+    layer.xv = layer.x.float().double().cpu().numpy()
+    ids = rng.permutation(np.repeat(np.arange(P), counts)).astype(np.int32).reshape(-1, 1)
+
+    def check(values, exps, t, slot):
+        x, w = layer.xv[t], layer.v13[slot]
+        gu, err = x @ w.T, sum_error(x, w, True)
+        gate, up, dg, du = gu[:, :I], gu[:, I:], err[:, :I], err[:, I:]
+        sg = gate / (1.0 + np.exp(-gate))
+        act = sg * up
+        da = 1.1 * np.abs(up) * dg + np.abs(sg) * du + dg * du + 2.0**-20 * np.abs(act)
+        check_rounded_act((values, exps), act, da)
+
+    take = lambda rows: (rows.float().double().cpu().numpy(), rows.scale.cpu().numpy().astype(np.int64) - 127)  # noqa: E731
+    for path, bm in [(native.LMOE_PATH_GEMV, 32)] + [(native.LMOE_PATH_MFMA, b) for b in native.MX4_BLOCK_M]:
+        print(f"case act scales H={H} I={I} path={path} block_m={bm}", flush=True)
+        perm, act, _ = run_layer(layer, ids, 1, path, block_m=bm)
+        values, exps = take(act)
+        pairs, offs = perm.sorted_pairs.cpu().numpy(), perm.offsets.cpu().numpy()
+        for s in range(P):
+            pos = np.arange(offs[s], offs[s + 1])
+            if len(pos):
+                check(values[pos], exps[pos], pairs[pos], s)
+    # one token and few, straight from their ids: act rows lie by pair
+    for t, call in ((1, native.mx4_decode_one), (min(T, 30), native.mx4_decode_few)):
+        part = native.Mx8Rows(layer.x.q[:t].clone(), layer.x.scale[:t].clone())
+        bufs = native.Mx4Buffers(native.Permutation.allocate(t, P, "cuda"), layer.act_buffer(t),
+                                 torch.empty((t, H), dtype=torch.float32, device="cuda"))
+        call(part, torch.ones((t, 1), dtype=torch.bfloat16, device="cuda"), to_dev_i32(ids[:t]), layer.w13, layer.w2, None,
+             bufs, torch.empty((t, H), dtype=torch.bfloat16, device="cuda"))
+        values, exps = take(bufs.act)
+        for s in range(P):
+            pos = np.flatnonzero(ids[:t, 0] == s)
+            if len(pos):
+                check(values[pos], exps[pos], pos, s)
+
+
+@pytest.mark.parametrize("T,k,E,H,I", [(1, 2, 8, 512, 128), (3, 4, 24, 1024, 416), (12, 4, 8, 256, 160), (90, 3, 8, 512, 256)])
+def test_8_bit_rows_end_to_end(T, k, E, H, I):
+    """out of every form against the experts in 64 bits, act rounded to MX8 in between:
+    where act lies near a tie its other neighbour is allowed, nothing more."""
+    from vllm_moe_offload_amd import fused_moe, native
+
+    rng = np.random.default_rng(T)
+    layer = Layer(H, I, E, T, "mx8", 17)
+    ids = np.stack([rng.permutation(E)[:k] for _ in range(T)]).astype(np.int32)
+    w = torch.empty((T, k), device="cuda").uniform_(0.05, 1, generator=torch.Generator(device="cuda").manual_seed(T)).to(torch.bfloat16)
+    out = fused_moe.fused_experts(layer.x, w, to_dev_i32(ids), layer.w13, layer.w2, None).double().cpu().numpy()
+    wv = w.double().cpu().numpy()
+    want, slack = np.zeros((T, H)), np.zeros((T, H))
+    for s in range(E):
+        t, j = np.nonzero(ids == s)
+        if not len(t):
+            continue
+        x, v13, v2 = layer.xv[t], layer.v13[s], layer.v2[s]
+        gu, err = x @ v13.T, sum_error(x, v13, True)
+        gate, up, dg, du = gu[:, :I], gu[:, I:], err[:, :I], err[:, I:]
+        sg = gate / (1.0 + np.exp(-gate))
+        exact = sg * up
+        da = 1.1 * np.abs(up) * dg + np.abs(sg) * du + dg * du + 2.0**-20 * np.abs(exact)
+        act, y = mx.expert(x, v13, v2, True)
+        # how far the stored act may be from the rounded one: at the group's exponent and,
+        # where its largest value is within da of a border, at the next one
+        grp = np.abs(exact).reshape(len(t), -1, 32)
+        top = lambda v: mx.group_exponents(np.repeat(v, 32, axis=1), 448.0)  # noqa: E731
+        e0 = top(np.maximum(grp - da.reshape(grp.shape), 0.0).max(axis=2))
+        e1 = top((grp + da.reshape(grp.shape)).max(axis=2))
+        off = np.zeros_like(act)
+        for e in (e0, e1):
+            for v in (exact - da, exact, exact + da):
+                off = np.maximum(off, np.abs(_at(v, e) - act))
+        wj = wv[t, j][:, None]
+        dy = off @ np.abs(v2).T + sum_error(np.abs(act) + off, v2, True)
+        np.add.at(want, t, wj * y)
+        np.add.at(slack, t, wj * (dy + 2 * k * 2.0**-24 * (np.abs(y) + dy)))
+    assert np.all(np.abs(out - want) <= slack * (1 + 2.0**-8) + 2.0**-8 * np.abs(want))
