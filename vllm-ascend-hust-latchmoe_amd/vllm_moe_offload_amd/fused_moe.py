@@ -132,6 +132,7 @@ def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = 
 
 
 def clear_workspaces() -> None:
+    """Drop every workspace; not while a captured graph that used one may replay."""
     _WORKSPACES.clear()
     _WARMED.clear()
 
@@ -189,7 +190,11 @@ def route(hidden: torch.Tensor, gate_weight: torch.Tensor | None, spec: RouterSp
 def _result(out: torch.Tensor | None, hidden) -> torch.Tensor:
     """The caller's output, or a new one: the workspaces that calls choose for
     themselves serve the next call too, so no result is left in one."""
-    return out if out is not None else torch.empty(tuple(hidden.shape), dtype=torch.bfloat16, device=hidden.device)
+    if out is not None:
+        return out
+    if isinstance(hidden, torch.Tensor):
+        return torch.empty_like(hidden)  # half the host time of torch.empty
+    return torch.empty(hidden.shape, dtype=torch.bfloat16, device=hidden.device)
 
 
 # ---------------------------------------------------------------------------
@@ -619,9 +624,10 @@ class FusedExpertsResult:
 
 def check_supported_input(inp) -> None:
     """Fail closed on the parts of the contract the gfx950 kernels do not
-    implement (bf16 SwiGLU experts on one GPU)."""
+    implement (SwiGLU experts, bf16 or 4-bit banks, on one GPU)."""
     if getattr(inp, "quant", None) not in (None, False):
-        raise RuntimeError("slot-bank fused experts run bf16 weights only; quantized experts are not supported")
+        raise RuntimeError("slot-bank fused experts take no quantized weights by a quant argument: 4-bit experts are slot "
+                           "banks (mxfp4.pack_experts), known by their dtype")
     act = getattr(inp, "activation", None)
     if act not in (None, "silu", "swiglu", "SiluAndMul"):
         raise RuntimeError(f"slot-bank fused experts implement SwiGLU only, got activation={act!r}")
