@@ -2,7 +2,8 @@
 //
 // gate-up: act[pos] = silu(W_g x) * (W_u x);  down: y[pair] = W_2 act[pos].
 // Weights are MX4 blocks (mx.h), rows bf16 or MX8.  What bounds it is the
-// weights' bytes: each slot's are read once for up to 32 rows.  Measured, gate-up /
+// weights' bytes: each slot's are read once for up to 32 rows (16 where act comes in two
+// parts, below).  Measured, gate-up /
 // down: 7 tokens x 8 of 64 experts, 7168 x 2048, MX8 rows 94 / 49 us (561 / 281 MB at
 // 6.0 / 5.7 TB/s); 16 x 8 of 128, 2048 x 768, bf16 rows 16.6 / 10.6 us (66 / 33 MB at
 // 4.0 / 3.1 TB/s: the start and the longest slot's passes of so short a kernel).
@@ -228,9 +229,11 @@ constexpr int kFewMxRows = 32;   // rows of one pass over a slot's weights
 // output's own rounding).  Up to eight rows the parts are rows r and r + 8 of one
 // fragment, which multiplies sixteen rows anyway; past that they are two fragments,
 // sixteen rows a pass.  The parts' sums are added last, so a row's bits are the same.
-// Row tiles keep one bf16 part: many rows average their roundings (the error is then
-// 1.41 times the output's own rounding, 1.35 to 1.46 over 160 layers of 9 to 200
-// tokens), and two would double the down product, which the matrix units bound there.
+// Row tiles keep one bf16 part: two would double the down product, which the matrix
+// units bound in tall tiles, and short ones, which weights bound, take the same form so
+// that a row's bits do not depend on its tile's height.  The price is act's rounding in
+// every output: its error is 1.41 times the output's own rounding (1.35 to 1.46 over 160
+// layers of 9 to 200 tokens), whatever rows are beside it.
 constexpr int kFewMxSplitRows = 16;
 
 // the other half of sixteen lanes: lane l from lane l ^ 8
@@ -421,7 +424,8 @@ __global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g, To
 // where the permutation, the split-K kernel twice and the combine are four.  Measured,
 // gate-up / down, 8 experts: 2048 x 768 6.4 / 6.6 us (13.4 / 6.7 MB: latency of the
 // id, table, weight chain), 7168 x 2048 24.0 / 20.8 us from bf16 rows, 22.4 / 15.9 us
-// from MX8 rows (125 / 62 MB at 5.6 / 3.9 TB/s).  The down product's waves then add
+// from MX8 rows (125 / 62 MB at 5.6 / 3.9 TB/s); both of 2048 x 768 in a graph 12.2 us
+// from bf16 rows, 10.4 from MX8 rows.  The down product's waves then add
 // their parts of K in another order than the split-K kernel's; the same order, parts
 // through LDS, cost a quarter at 7168 x 2048 (the step 51.7 -> 65.0 us).
 // ---------------------------------------------------------------------------
