@@ -457,3 +457,28 @@ def test_8_bit_rows_end_to_end(T, k, E, H, I):
         np.add.at(want, t, wj * y)
         np.add.at(slack, t, wj * (dy + 2 * k * 2.0**-24 * (np.abs(y) + dy)))
     assert np.all(np.abs(out - want) <= slack * (1 + 2.0**-8) + 2.0**-8 * np.abs(want))
+
+
+def test_constants_are_there_for_every_stream():
+    """The shared expert's ones and zeros, made on a stream that is behind and read on
+    another; one made in a capture is not kept for eager calls."""
+    from vllm_moe_offload_amd import layer as layer_mod
+
+    dev, side = torch.device("cuda", 0), torch.cuda.Stream()
+    layer_mod.clear_constants()
+    torch.cuda._sleep(20_000_000)
+    a, b = layer_mod._ones_bf16(4099, dev), layer_mod._zeros_i32(4099, dev)
+    with torch.cuda.stream(side):
+        got = layer_mod._ones_bf16(4099, dev).clone(), layer_mod._zeros_i32(4099, dev).clone()
+    side.synchronize()
+    assert (got[0] == 1).all() and not got[1].any()
+    assert layer_mod._ones_bf16(4099, dev) is a and layer_mod._zeros_i32(4099, dev) is b
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = layer_mod._ones_bf16(4101, dev)
+        out = inside + 1
+    assert layer_mod._ones_bf16(4101, dev) is not inside and (layer_mod._ones_bf16(4101, dev) == 1).all()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (out == 2).all()

@@ -270,15 +270,22 @@ def clear_constants() -> None:
     _CONST.clear()
 
 
+def _constant(value: int, T: int, dtype: torch.dtype, device) -> torch.Tensor:
+    key = (value, T, dtype, str(device))
+    t = _CONST.get(key)
+    if t is None:
+        t = torch.full((T, 1), value, dtype=dtype, device=device)
+        if t.is_cuda:
+            if torch.cuda.is_current_stream_capturing():
+                return t  # filled by the graph's replays alone: of no use outside it
+            torch.cuda.current_stream(t.device).synchronize()  # once: other streams read it too
+        _CONST[key] = t
+    return t
+
+
 def _ones_bf16(T: int, device) -> torch.Tensor:
-    key = ("ones", T, str(device))
-    if key not in _CONST:
-        _CONST[key] = torch.ones((T, 1), dtype=torch.bfloat16, device=device)
-    return _CONST[key]
+    return _constant(1, T, torch.bfloat16, device)
 
 
 def _zeros_i32(T: int, device) -> torch.Tensor:
-    key = ("zeros", T, str(device))
-    if key not in _CONST:
-        _CONST[key] = torch.zeros((T, 1), dtype=torch.int32, device=device)
-    return _CONST[key]
+    return _constant(0, T, torch.int32, device)
