@@ -137,6 +137,51 @@ def test_default_calls_on_two_streams_and_from_two_threads(T, kind):
     assert all(torch.equal(_bits(o), _bits(want[i])) for i in (0, 1) for o in got[i])
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [1, 3, 9, 200])
+def test_graphs_of_default_calls_replayed_at_once(T, kind):
+    """Two graphs of one shape on two streams, eager calls of the shape on a third; each
+    graph holds the layer twice, the second over the first's result."""
+    from vllm_moe_offload_amd import fused_moe, native
+
+    k, E, H, I = 2, 8, 512, 256
+    parts = [_experts(kind, E, H, I, T, s) for s in (5, 6, 7)]
+    rng = np.random.default_rng(T)
+    ids = [to_dev_i32(np.stack([rng.permutation(E)[:k] for _ in range(T)])) for _ in parts]
+    w = torch.full((T, k), 0.5, dtype=torch.bfloat16, device="cuda")
+
+    def layers(i):
+        x, w13, w2 = parts[i]
+        first = fused_moe.fused_experts(x, w, ids[i], w13, w2, None)
+        again = native.rows_to_mx8(first) if kind == "mx8" else first
+        return first, fused_moe.fused_experts(again, w, ids[i], w13, w2, None)
+
+    want = [tuple(t.clone() for t in layers(i)) for i in range(3)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in (0, 1):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs.append(layers(i))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        for o in outs:
+            for t in o:
+                t.zero_()
+        torch.cuda.synchronize()
+        eager = []
+        for _ in range(4):
+            for i in (0, 1):
+                with torch.cuda.stream(streams[i]):
+                    graphs[i].replay()
+            with torch.cuda.stream(streams[2]):
+                eager.append(layers(2))
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(outs[i], want[i]))
+        assert all(torch.equal(_bits(a), _bits(b)) for e in eager for a, b in zip(e, want[2]))
+
+
 def test_workspaces_of_streams_threads_and_captures():
     from vllm_moe_offload_amd import fused_moe
 
@@ -152,14 +197,19 @@ def test_workspaces_of_streams_threads_and_captures():
     t.join()
     assert other[0] is not here and other[0] is not there
     assert get() is here
-    # a capture takes the warm-up's, from whichever stream and thread that was
+    # a capture's is its own, one that a caller asks for there starts as zeros
     warm = get(tag="warm")
-    with torch.cuda.stream(side):
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
-            assert get(tag="warm") is warm
-            warm.out.fill_(1.0)
-    assert get(tag="warm") is warm
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = get(tag="warm")
+        meta = inside.perm.meta.clone()
+        inside.perm.meta.fill_(5)
+        inside.out.fill_(1.0)
+    assert inside is not warm and get(tag="warm") is warm
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not meta.any() and (inside.perm.meta == 5).all() and not warm.perm.meta.any()
     fused_moe.clear_workspaces()
     assert get(tag="warm") is not warm
 

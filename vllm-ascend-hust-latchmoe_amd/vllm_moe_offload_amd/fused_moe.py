@@ -54,6 +54,7 @@ class MoEWorkspace:
     out: torch.Tensor   # [T, H] bf16
     perm_overflow: native.Permutation | None = None  # the decode overflow pass's permutation
     mx4: native.Mx4Buffers | None = None  # the buffers as the calls over 4-bit banks take them
+    cleared: bool = True  # whether its permutations start as zeros (the one-launch router needs that)
 
     def act_rows(self, n: int, path: int):
         """act of n pairs as a path takes it: two parts on LMOE_PATH_GEMV only."""
@@ -65,12 +66,12 @@ class MoEWorkspace:
     def overflow_perm(self, n_pairs: int, n_slots: int, device) -> native.Permutation:
         p = self.perm_overflow
         if p is None or p.n_pairs != int(n_pairs) or p.n_slots != int(n_slots):
-            p = self.perm_overflow = native.Permutation.allocate(int(n_pairs), int(n_slots), device)
+            p = self.perm_overflow = native.Permutation.allocate(int(n_pairs), int(n_slots), device,
+                                                                       cleared=self.cleared)
         return p
 
 
 _WORKSPACES: dict[tuple, MoEWorkspace] = {}  # by shape, stream and thread
-_WARMED: dict[tuple, MoEWorkspace] = {}      # by shape: the last one made outside a capture
 _DEVICES: dict = {}  # (type, index) of a torch.device or str; asking takes longer than finding the workspace
 
 
@@ -104,42 +105,57 @@ def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = 
     512 experts of 1024 x 512, 960 pairs against 1280 and 4800).
 
     Calls that take the same workspace must run one after the other, so each
-    stream (the device's current one) and each host thread has its own.  A
-    capture takes the one its warm-up made, on whichever stream that was, so a
-    graph shares it with eager calls and other graphs of the shape: where they may
-    run at once, give one of them a tag of its own and pass it as workspace=."""
+    stream (the device's current one) and each host thread has its own.  Inside a
+    capture it is a new one each time, of the graph's memory, which the caller keeps
+    while it captures."""
+    return _workspace(T, k, P, H, I, device, tag, rows, True)
+
+
+def _workspace(T, k, P, H, I, device, tag: str, rows: str, cleared: bool) -> MoEWorkspace:
     if rows not in ("", "bf16", "mx8"):
         raise ValueError(f"unknown rows {rows!r}")
     where = _device_key(device)
-    shape = (int(T), int(k), int(P), int(H), int(I), where, tag, rows)
-    key = (shape, native.current_stream_handle(where[1]) if where[0] == "cuda" else 0, threading.get_ident())
+    stream = 0
+    if where[0] == "cuda":
+        if torch.cuda.is_current_stream_capturing():
+            return _make_workspace(int(T), int(k), int(P), int(H), int(I), device, rows, cleared=cleared)
+        stream = native.current_stream_handle(where[1])
+    key = (int(T), int(k), int(P), int(H), int(I), where, tag, rows, stream, threading.get_ident())
     ws = _WORKSPACES.get(key)
     if ws is None:
-        capturing = where[0] == "cuda" and _is_current_graph_capturing()
-        if capturing and shape in _WARMED:
-            return _WARMED[shape]
-        N = T * k
-        few = rows != "" and N <= native.FUSED_DECODE_MAX_PAIRS
-        y_dtype = torch.float32 if few else torch.bfloat16
-        ws = MoEWorkspace(
-            perm=native.Permutation.allocate(N, P, device),
-            act=native.Mx8Rows.allocate(max(N, 1), I, device) if rows == "mx8" else
-            torch.empty((max(N, 1), 2, I) if few else (max(N, 1), I), dtype=torch.bfloat16, device=device),
-            y=torch.empty((max(N, 1), H), dtype=y_dtype, device=device),
-            out=torch.empty((max(T, 1), H), dtype=torch.bfloat16, device=device),
-        )
-        if rows:
-            ws.mx4 = native.Mx4Buffers(ws.perm, ws.act, ws.y)
-        _WORKSPACES[key] = ws
-        if not capturing:
-            _WARMED[shape] = ws
+        ws = _WORKSPACES[key] = _make_workspace(*key[:5], device, rows)
     return ws
 
 
+def _make_workspace(T: int, k: int, P: int, H: int, I: int, device, rows: str, *, cleared: bool = True) -> MoEWorkspace:
+    N = T * k
+    few = rows != "" and N <= native.FUSED_DECODE_MAX_PAIRS
+    y_dtype = torch.float32 if few else torch.bfloat16
+    ws = MoEWorkspace(
+        perm=native.Permutation.allocate(N, P, device, cleared=cleared),
+        act=native.Mx8Rows.allocate(max(N, 1), I, device) if rows == "mx8" else
+        torch.empty((max(N, 1), 2, I) if few else (max(N, 1), I), dtype=torch.bfloat16, device=device),
+        y=torch.empty((max(N, 1), H), dtype=y_dtype, device=device),
+        out=torch.empty((max(T, 1), H), dtype=torch.bfloat16, device=device),
+        cleared=cleared,
+    )
+    if rows:
+        ws.mx4 = native.Mx4Buffers(ws.perm, ws.act, ws.y)
+    return ws
+
+
+def call_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = "", rows: str = "") -> MoEWorkspace:
+    """get_workspace for the length of one call that builds its permutation itself.
+    In a capture its memory returns to the graph's pool with the call, in stream
+    order: no graph shares it with eager calls or another graph, and no clearing is
+    captured (lmoe_permute writes all that is read)."""
+    return _workspace(T, k, P, H, I, device, tag, rows, False)
+
+
 def clear_workspaces() -> None:
-    """Drop every workspace; not while a captured graph that used one may replay."""
+    """Drop every workspace; not while a graph that was captured with one (workspace=) may
+    replay."""
     _WORKSPACES.clear()
-    _WARMED.clear()
 
 
 # ---------------------------------------------------------------------------
@@ -250,7 +266,7 @@ def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2
     k = topk_ids.shape[1]
     P = w13_slots.shape[0]
     if ws is None:
-        ws = get_workspace(T, k, P, H, w13_slots.shape[1] // 2, hidden.device, rows=rows_kind(hidden, w13_slots))
+        ws = call_workspace(T, k, P, H, w13_slots.shape[1] // 2, hidden.device, rows=rows_kind(hidden, w13_slots))
     if ws.mx4 is None:
         raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
     dst = _result(out, hidden) if workspace is None or out is not None else ws.out[:T]
@@ -378,7 +394,7 @@ def _fused_experts_ws(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2p
     I = int(w13_slots.shape[1]) // 2
     rows = rows_kind(hidden, w13_slots)
     mx4 = rows != ""
-    ws = workspace or get_workspace(T, k, P, H, I, hidden.device, rows=rows)
+    ws = workspace or call_workspace(T, k, P, H, I, hidden.device, rows=rows)
     if mx4 and ws.mx4 is None:
         raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
     dst = _result(out, hidden) if workspace is None or out is not None else ws.out[:T]
@@ -826,7 +842,7 @@ def run_wave_prefill(
     t_sched = perf_counter()
     profiling = bool(runtime.profile_path)
     wave_profiles: dict[int, dict] = {}
-    ws = get_workspace(T, k, P, H, I, hidden.device, tag="waves", rows=rows_kind(hidden, bank.w13_slots))
+    ws = call_workspace(T, k, P, H, I, hidden.device, tag="waves", rows=rows_kind(hidden, bank.w13_slots))
     report = WaveRunReport(plan.waves, sched.compute_order)
     staged: dict[int, tuple] = {}
     total_logical = runtime.total_logical_expert_count_for_layer(layer_id=layer_id, fallback=num_logical_experts)
@@ -1029,8 +1045,8 @@ def run_device_waves(
               for b in range(min(n_buf, n_waves))]
     tables = [runtime._get_prefill_stage_log2phy_buffer(template_bank=bank, buffer_index=b, num_logical_experts=total,
                                                         device=dev) for b in range(len(stages))]
-    ws = get_workspace(T, k, int(stages[0].physical_expert_count), H, I, dev, tag="device_waves",
-                       rows=rows_kind(hidden, bank.w13_slots))
+    ws = call_workspace(T, k, int(stages[0].physical_expert_count), H, I, dev, tag="device_waves",
+                        rows=rows_kind(hidden, bank.w13_slots))
     capturing = _is_current_graph_capturing()
     compute = torch.cuda.current_stream(dev)
     tx = runtime.transfer_engine._transfer_stream(dev)
@@ -1111,8 +1127,8 @@ def run_full_layer(
     )
     T, H = hidden.shape
     k = int(topk_ids.shape[1])
-    ws = get_workspace(T, k, prepared.physical_expert_count, H, int(prepared.w1.shape[1]) // 2, hidden.device, tag="full",
-                       rows=rows_kind(hidden, prepared.w1))
+    ws = call_workspace(T, k, prepared.physical_expert_count, H, int(prepared.w1.shape[1]) // 2, hidden.device, tag="full",
+                        rows=rows_kind(hidden, prepared.w1))
     checked = not _is_current_graph_capturing()
     out = _result(out, hidden)
     args = (hidden, topk_weights, topk_ids, prepared.w1, prepared.w2, prepared.log2phy)

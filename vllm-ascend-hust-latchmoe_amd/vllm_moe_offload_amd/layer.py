@@ -30,8 +30,8 @@ from vllm_moe_offload_amd.fused_moe import (
     MoEOffloadParams,
     MoEWeights,
     RouterSpec,
+    call_workspace,
     fused_experts,
-    get_workspace,
     route,
     rows_kind,
     run_overflow_prefill,
@@ -187,8 +187,8 @@ class SlotMoELayer(torch.nn.Module):
         T, H = x.shape
         ones = _ones_bf16(T, x.device)
         zeros = _zeros_i32(T, x.device)
-        ws = get_workspace(T, 1, 1, H, int(self.shared_w13.shape[1]) // 2, x.device, tag=f"shared{self.layer_id}",
-                           rows=rows_kind(x, self.shared_w13))
+        ws = call_workspace(T, 1, 1, H, int(self.shared_w13.shape[1]) // 2, x.device, tag=f"shared{self.layer_id}",
+                            rows=rows_kind(x, self.shared_w13))
         return fused_experts(x, ones, zeros, self.shared_w13, self.shared_w2, None, workspace=ws,
                              out=torch.empty((T, H), dtype=torch.bfloat16, device=x.device))
 

@@ -1063,22 +1063,25 @@ class Permutation:
     builds: int = 0  # lmoe_permute builds issued on these buffers
 
     @classmethod
-    def allocate(cls, n_pairs: int, n_slots: int, device) -> "Permutation":
+    def allocate(cls, n_pairs: int, n_slots: int, device, *, cleared: bool = True) -> "Permutation":
+        """cleared: the buffers start as zeros, as the router calls that build the
+        permutation need; lmoe_permute does not."""
         lib = load_library()
+        new = torch.zeros if cleared else torch.empty
         ws = int(lib.lmoe_permute_workspace_bytes(int(n_pairs), int(n_slots)))
         i32 = dict(dtype=torch.int32, device=device)
         return cls(
             n_pairs=int(n_pairs),
             n_slots=int(n_slots),
-            counts=torch.zeros(n_slots, **i32),
-            offsets=torch.zeros(n_slots + 1, **i32),
-            sorted_pairs=torch.zeros(max(1, n_pairs), **i32),
-            row_idx=torch.zeros(max(1, n_pairs), **i32),
-            active=torch.zeros(n_slots, **i32),
-            tile_off=torch.zeros(n_slots + 1, **i32),
-            meta=torch.zeros(META_COUNT, **i32),
+            counts=new(n_slots, **i32),
+            offsets=new(n_slots + 1, **i32),
+            sorted_pairs=new(max(1, n_pairs), **i32),
+            row_idx=new(max(1, n_pairs), **i32),
+            active=new(n_slots, **i32),
+            tile_off=new(n_slots + 1, **i32),
+            meta=new(META_COUNT, **i32),
             workspace=torch.empty(max(ws, 1), dtype=torch.int8, device=device),
-            sync=torch.zeros(ROUTER_SYNC_WORDS, **i32),
+            sync=new(ROUTER_SYNC_WORDS, **i32),
         )
 
 
