@@ -410,6 +410,8 @@ int lmoe_combine_f32(const void* y, const int32_t* row_idx, const uint16_t* w,
  * integer >= -127 that keeps the group's largest magnitude within the element
  * format, so nothing saturates; a group with a NaN or an infinity is NaN.
  *   MX8 rows: q [R, K] e4m3 (largest 448), scale [R, K/32] u8.
+ *   MX4 rows: q [R, K/2] bytes of two e2m1 values each (largest 6; the even column
+ *   in the low half), scale [R, K/32] u8.  Codes of a NaN group made here are zeros.
  *   MX4 weights of [N, K]: e2m1 (largest 6) codes and scales in one run of
  *   lmoe_mx4_bytes(N, K) bytes: N/16 blocks of 16 rows; a block is its columns
  *   by 512: 256 bytes of scales (byte 4 l + c: row l % 16, columns
@@ -441,6 +443,49 @@ int lmoe_add_rms_norm(const void* x, int T, int H, const void* residual,
  * aligned; else LMOE_ERR_SHAPE.  x, q and scale may not overlap (LMOE_ERR_ARG). */
 int lmoe_rows_to_mx8(const void* x, int T, int H, void* q, void* scale,
                      hipStream_t stream);
+
+/* lmoe_add_rms_norm (same arguments and results) with y as MX4 rows in q / scale. */
+int lmoe_add_rms_norm_mx4(const void* x, int T, int H, const void* residual,
+                          int residual_f32, const void* weight, int weight_f32,
+                          float eps, void* residual_out, void* out, void* q,
+                          void* scale, hipStream_t stream);
+
+/* Rows x [T, H], bf16 or f32 (x_f32), as MX4 rows.  H % 32 == 0, x and q 16-byte
+ * aligned; else LMOE_ERR_SHAPE.  x, q and scale may not overlap (LMOE_ERR_ARG). */
+int lmoe_rows_to_mx4(const void* x, int x_f32, int T, int H, void* q, void* scale,
+                     hipStream_t stream);
+
+/* The values that MX4 rows stand for, [T, H] bf16 or f32 (out_f32): exact, infinite past
+ * the type's largest number (scale bytes from 253 on).  Shapes, alignment and overlap
+ * as lmoe_rows_to_mx4. */
+int lmoe_mx4_rows_values(const void* q, const void* scale, int T, int H, void* out,
+                         int out_f32, hipStream_t stream);
+
+/* Weights w [E, N, K], bf16 or f32 (w_f32), as MX4 weights: bank is
+ * [E, lmoe_mx4_bytes(N, K)].  gate_up: w's N rows are a gate and an up half, which
+ * the bank holds in blocks of 16 rows in turn (w13).  N % 16 == 0 (N % 64 == 0 with
+ * gate_up), K % 32 == 0, w and bank 16-byte aligned; else LMOE_ERR_SHAPE.  The two
+ * may not overlap (LMOE_ERR_ARG). */
+int lmoe_mx4_quantize(const void* w, int w_f32, int E, int N, int K, int gate_up,
+                      void* bank, hipStream_t stream);
+
+/* The values that MX4 weights stand for, [E, N, K] bf16 or f32 (out_f32) with the
+ * rows in w's order: the way back from lmoe_mx4_quantize, with its arguments. */
+int lmoe_mx4_bank_values(const void* bank, int E, int N, int K, int gate_up,
+                         void* out, int out_f32, hipStream_t stream);
+
+/* out = x W^T (+ bias) (+ add) over MX4 weights w of [N, K] (in order, as w2).
+ * rows says what x [T, K] is: LMOE_ROWS_BF16 (x_scale null), LMOE_ROWS_MX8 or
+ * LMOE_ROWS_MX4.  Products are summed in f32, bias [N] (bf16 or f32, may be null) and
+ * add [T, N] (bf16, may be null) are added in f32, out [T, N] is rounded once, to
+ * bf16 or f32 (out_f32).  Which partial sums are added depends on the sizes, never on
+ * the values.  K % 32 == 0, N % 16 == 0, operands 16-byte aligned (x_scale any); else
+ * LMOE_ERR_SHAPE.  out may be add (bf16); any other overlap of out with an operand is
+ * LMOE_ERR_ARG. */
+enum { LMOE_ROWS_BF16 = 0, LMOE_ROWS_MX8 = 1, LMOE_ROWS_MX4 = 2 };
+int lmoe_mx4_linear(const void* x, const void* x_scale, int rows, int T, int K,
+                    int N, const void* w, const void* bias, int bias_f32,
+                    const void* add, void* out, int out_f32, hipStream_t stream);
 
 /* Bytes of MX4 weights of [N, K]; -1 unless N % 16 == 0 and K % 32 == 0. */
 long long lmoe_mx4_bytes(int N, int K);
@@ -538,6 +583,43 @@ int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, int I, int k,
                         const int32_t* log2phy_b, int n_log2phy_b,
                         const void* add, void* act, void* act_scale, void* out,
                         hipStream_t stream);
+
+/* The entries above for MX4 rows: x / x_scale and act / act_scale are MX4 rows (act is
+ * rounded to MX4 along I between the products, which multiply 4-bit by 4-bit values,
+ * exactly up to their f32 sums), act_split is 0; everything else is as there. */
+int lmoe_mx44_gateup_silu(const void* x, const void* x_scale, int T, int H,
+                          int I, int k, const void* w13_slots, int n_slots,
+                          const int32_t* offsets, const int32_t* sorted_pairs,
+                          const int32_t* active, const int32_t* tile_off,
+                          const int32_t* meta, int n_pairs, int block_m,
+                          int path, void* act, void* act_scale, int act_split,
+                          hipStream_t stream);
+int lmoe_mx44_down(const void* act, const void* act_scale, int act_split,
+                   int H, int I, const void* w2_slots, int n_slots, const int32_t* offsets,
+                   const int32_t* sorted_pairs, const int32_t* active,
+                   const int32_t* tile_off, const int32_t* meta, int n_pairs,
+                   int block_m, int path, void* y, int y_f32,
+                   hipStream_t stream);
+int lmoe_mx44_fused_moe(const void* x, const void* x_scale, int T, int H, int I,
+                        int k, const void* w13_slots, const void* w2_slots,
+                        int n_slots, const uint16_t* w, const int32_t* ids,
+                        const int32_t* log2phy, int n_log2phy, int path,
+                        int block_m, const lmoe_mx4_workspace* ws,
+                        const void* add, void* out, hipStream_t stream);
+int lmoe_mx44_decode_few(const void* x, const void* x_scale, int T, int H, int I,
+                         int k, const void* w13_slots, const void* w2_slots,
+                         int n_slots, const uint16_t* w, const int32_t* ids,
+                         const int32_t* log2phy, int n_log2phy, const void* add,
+                         void* act, void* act_scale, void* y, void* out,
+                         hipStream_t stream);
+int lmoe_mx44_decode_one(const void* x, const void* x_scale, int H, int I, int k,
+                         const void* w13_slots, const void* w2_slots,
+                         int n_slots, const uint16_t* w, const int32_t* ids,
+                         const int32_t* log2phy, int n_log2phy,
+                         const void* w13_b, const void* w2_b, int n_slots_b,
+                         const int32_t* log2phy_b, int n_log2phy_b,
+                         const void* add, void* act, void* act_scale, void* out,
+                         hipStream_t stream);
 
 /* The second half of lmoe_fused_moe_decode on its own: down GEMV from act
  * (sorted order) fused with the weighted combine into out (same argument

@@ -9,6 +9,10 @@
 //
 // MX8 rows: q [R, K] e4m3 bytes, scale [R, K / 32] bytes, both row-major.
 //
+// MX4 rows: q [R, K / 2] bytes, two e2m1 values each (the even column in the low half),
+// scale [R, K / 32] bytes, both row-major.  A row's 16 bytes of a group are the matrix
+// instruction's operand as they lie.
+//
 // MX4 weights of an [N, K] matrix, in the order the matrix instructions read
 // them: N / 16 blocks of 16 rows; a block is a run of quads (512 columns), each
 // 256 bytes of scales and then up to four chunks (128 columns) of 1 KiB.  Lane l
@@ -60,6 +64,18 @@ __device__ __forceinline__ float mx_scale_f32(int byte) {
 // that must not lose them (fmaxf drops NaN): compared as unsigned bits.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+__device__ __forceinline__ int mx4_scale_byte(float amax) {
+  return mx_scale_byte<2, 0x400000u>(amax);  // 6 = 1.5 * 2^2
+}
+
+// What a product's rows are held in.
+enum RowKind : int { kRowsBf16 = 0, kRowsMx8 = 1, kRowsMx4 = 2 };
+// Bytes before row r of K columns.
+template <int R>
+__host__ __device__ __forceinline__ size_t row_bytes(size_t r, int K) {
+  return R == kRowsMx4 ? r * (static_cast<size_t>(K) >> 1) : r * K * (R == kRowsMx8 ? 1 : 2);
+}
+
 typedef short i16x2_t __attribute__((ext_vector_type(2)));
 
 // Four values / 2^e as e4m3 bytes, lowest first, round to nearest even.
@@ -68,6 +84,23 @@ __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float
   r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, scale, false);
   r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
   return __builtin_bit_cast(uint32_t, r);
+}
+
+// Values / 2^e as e2m1 codes, the first in the lowest bits, round to nearest even.  byte:
+// the scale's; the codes of a group that is NaN are zeros.
+__device__ __forceinline__ uint32_t pack_e2m1x4(float a, float b, float c, float d, float scale, int byte) {
+  uint32_t r = 0;
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, a, b, scale, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, c, d, scale, 1);
+  return byte == 255 ? 0 : r;
+}
+__device__ __forceinline__ uint32_t pack_e2m1x8(const float (&v)[8], float scale, int byte) {
+  uint32_t r = 0;
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], scale, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], scale, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], scale, 2);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], scale, 3);
+  return byte == 255 ? 0 : r;
 }
 
 }  // namespace lmoe

@@ -1,7 +1,7 @@
 // Expert products over 4-bit weights for few rows per slot (decode).
 //
 // gate-up: act[pos] = silu(W_g x) * (W_u x);  down: y[pair] = W_2 act[pos].
-// Weights are MX4 blocks (mx.h), rows bf16 or MX8.  What bounds it is the
+// Weights are MX4 blocks (mx.h), rows bf16, MX8 or MX4.  What bounds it is the
 // weights' bytes: each slot's are read once for up to 32 rows (16 where act comes in two
 // parts, below).  Measured, gate-up /
 // down: 7 tokens x 8 of 64 experts, 7168 x 2048, MX8 rows 94 / 49 us (561 / 281 MB at
@@ -38,7 +38,7 @@ typedef __bf16 bf16x8v_t __attribute__((ext_vector_type(8)));
 
 struct Mx4Args {
   const void* a;            // gate-up: rows [T, K]; down: rows [n_pairs, K] in sorted order
-  const uint8_t* a_scale;   // MX8 rows: [.., K / 32], else null
+  const uint8_t* a_scale;   // MX8 and MX4 rows: [.., K / 32], else null
   const uint8_t* w;
   long long w_slot_bytes;
   int K, N;                 // row length; output columns (I or H)
@@ -49,33 +49,45 @@ struct Mx4Args {
   const int32_t* tile_off;
   const int32_t* meta;
   void* out;                // act rows, or y rows by pair
-  uint8_t* out_scale;       // act rows in MX8
+  uint8_t* out_scale;       // act rows in MX8 or MX4
   bool out_f32;             // y in f32
   bool split;               // bf16 act rows in two parts, [.., 2, I]
+  int rows;                 // RowKind of a, and of act
 };
 
 // One row's share of a 16 x 128 fragment: this lane's 32 values.
-template <bool A8>
+template <int R>
 struct RowFrag;
 template <>
-struct RowFrag<true> {
+struct RowFrag<kRowsMx8> {
   i32x8_t v;
   int scale;
 };
 template <>
-struct RowFrag<false> {
+struct RowFrag<kRowsMx4> {
+  i32x4_t v;
+  int scale;
+};
+template <>
+struct RowFrag<kRowsBf16> {
   i32x4_t v[4];
 };
 
 // The fragment of chunk c of the row at p (sp: its scales).  Values past K read
 // as zero: the weights' padding is zero, but zero times a stray NaN is not.
-template <bool A8>
-__device__ __forceinline__ RowFrag<A8> load_row_frag(const char* p, const uint8_t* sp, int c, int K,
-                                                     int g) {
-  RowFrag<A8> f;
+template <int R>
+__device__ __forceinline__ RowFrag<R> load_row_frag(const char* p, const uint8_t* sp, int c, int K,
+                                                    int g) {
+  RowFrag<R> f;
   const int k0 = c * kMxChunk;
   const i32x4_t zero = {0, 0, 0, 0};
-  if constexpr (A8) {
+  if constexpr (R == kRowsMx4) {
+    const bool in = k0 + 32 * g < K;
+    f.v = *reinterpret_cast<const i32x4_t*>(p + (in ? (k0 >> 1) + 16 * g : 0));
+    const int s = sp[in ? 4 * c + g : 0];
+    if (!in) f.v = zero;
+    f.scale = in ? s : kScaleOne;
+  } else if constexpr (R == kRowsMx8) {
     const bool lo = k0 + 16 * g < K, hi = k0 + 64 + 16 * g < K, sc = k0 + 32 * g < K;
     i32x4_t a = *reinterpret_cast<const i32x4_t*>(p + (lo ? k0 + 16 * g : 0));
     i32x4_t b = *reinterpret_cast<const i32x4_t*>(p + (hi ? k0 + 64 + 16 * g : 0));
@@ -107,9 +119,13 @@ __device__ __forceinline__ bf16x8v_t weights_bf16(int word, float s) {
 
 // acc += W x^T of one chunk: 16 weight rows, 16 rows.  Byte B of scale: the
 // weights' scale.
-template <bool A8, int B = 0>
-__device__ __forceinline__ f32x4_t mx4_step(i32x4_t w, int scale, const RowFrag<A8>& x, f32x4_t acc) {
-  if constexpr (A8) {
+template <int R, int B = 0>
+__device__ __forceinline__ f32x4_t mx4_step(i32x4_t w, int scale, const RowFrag<R>& x, f32x4_t acc) {
+  if constexpr (R == kRowsMx4) {
+    const i32x8_t wide = __builtin_shufflevector(w, w, 0, 1, 2, 3, 0, 1, 2, 3);
+    const i32x8_t row = __builtin_shufflevector(x.v, x.v, 0, 1, 2, 3, 0, 1, 2, 3);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide, row, acc, 4 /* e2m1 */, 4, B, scale, 0, x.scale);
+  } else if constexpr (R == kRowsMx8) {
     const i32x8_t wide = __builtin_shufflevector(w, w, 0, 1, 2, 3, 0, 1, 2, 3);
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide, x.v, acc, 4 /* e2m1 */, 0 /* e4m3 */, B,
                                                             scale, 0, x.scale);
@@ -147,8 +163,8 @@ __device__ __forceinline__ void store_bf16x8(uint16_t* p, int lane, bool live, c
 
 // act = silu(gate) * up of eight columns of one row, held by the four lanes
 // l, l ^ 16, l ^ 32, l ^ 48 (lane group g: columns i0 + 4 g.. and i0 + 16 + 4 g..
-// of a group of 32): stored in bf16, or in MX8 with the group's scale.
-template <bool A8>
+// of a group of 32): stored in bf16, or in MX8 or MX4 with the group's scale.
+template <int R>
 __device__ __forceinline__ void store_act(const Mx4Args& g, int pos, int i0, int lane, bool live,
                                           const f32x4_t (&gate)[2], const f32x4_t (&up)[2]) {
   const int col = 4 * (lane >> 4);
@@ -158,7 +174,7 @@ __device__ __forceinline__ void store_act(const Mx4Args& g, int pos, int i0, int
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[p][e] = silu_f32(gate[p][e]) * up[p][e];
   size_t row = static_cast<size_t>(pos) * g.N;
-  if constexpr (A8) {
+  if constexpr (R != kRowsBf16) {
     uint32_t m = 0;
 #pragma unroll
     for (int p = 0; p < 2; ++p)
@@ -169,13 +185,23 @@ __device__ __forceinline__ void store_act(const Mx4Args& g, int pos, int i0, int
     m = umax32(__float_as_uint(a), __float_as_uint(b));
     a = b = __uint_as_float(m);
     permlane_swap<32>(a, b);
-    const int byte = mx8_scale_byte(__uint_as_float(umax32(__float_as_uint(a), __float_as_uint(b))));
+    const float amax = __uint_as_float(umax32(__float_as_uint(a), __float_as_uint(b)));
+    const int byte = R == kRowsMx8 ? mx8_scale_byte(amax) : mx4_scale_byte(amax);
     const float s = mx_scale_f32(byte);
-    uint32_t lo = pack_e4m3x4(v[0][0], v[0][1], v[0][2], v[0][3], s);
-    uint32_t hi = pack_e4m3x4(v[1][0], v[1][1], v[1][2], v[1][3], s);
+    uint32_t lo, hi;
+    if constexpr (R == kRowsMx8) {
+      lo = pack_e4m3x4(v[0][0], v[0][1], v[0][2], v[0][3], s);
+      hi = pack_e4m3x4(v[1][0], v[1][1], v[1][2], v[1][3], s);
+    } else {
+      lo = pack_e2m1x4(v[0][0], v[0][1], v[0][2], v[0][3], s, byte);
+      hi = pack_e2m1x4(v[1][0], v[1][1], v[1][2], v[1][3], s, byte);
+    }
     join_columns(lo, hi);
     if (live) {
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(g.out) + row + i0 + joined_column(lane)) = make_uint2(lo, hi);
+      uint8_t* out = static_cast<uint8_t*>(g.out);
+      const size_t at = row + i0 + joined_column(lane);
+      if constexpr (R == kRowsMx8) *reinterpret_cast<uint2*>(out + at) = make_uint2(lo, hi);
+      else *reinterpret_cast<uint32_t*>(out + at / 2) = lo | hi << 16;
       if (col == 0)
         g.out_scale[static_cast<size_t>(pos) * (g.N / kMxGroup) + i0 / kMxGroup] = static_cast<uint8_t>(byte);
     }
@@ -244,14 +270,14 @@ __device__ __forceinline__ f32x4_t other_part(const f32x4_t v) {
 
 // Chunks [c0, c1) of RB weight blocks by NF row fragments, U chunks' loads at a time.
 // (blocks: how many of the RB there are; the last stands in for the others)
-template <bool A8, int RB, int NF, int U>
+template <int R, int RB, int NF, int U>
 __device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int blocks, int K, int c0, int c1, int lane,
                                            const char* const (&row)[NF], const uint8_t* const (&row_scale)[NF],
                                            f32x4_t (&acc)[RB][NF]) {
   for (int c = c0; c < c1; c += U) {
     i32x4_t w[U][RB];
     int sc[U][RB];
-    RowFrag<A8> x[U][NF];
+    RowFrag<R> x[U][NF];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (u > 0 && c + u >= c1) break;
@@ -264,7 +290,7 @@ __device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int bloc
         sc[u][b] = p[lane * 4 + ((c + u) & 3)];
       }
 #pragma unroll
-      for (int f = 0; f < NF; ++f) x[u][f] = load_row_frag<A8>(row[f], row_scale[f], c + u, K, lane >> 4);
+      for (int f = 0; f < NF; ++f) x[u][f] = load_row_frag<R>(row[f], row_scale[f], c + u, K, lane >> 4);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -272,7 +298,7 @@ __device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int bloc
 #pragma unroll
       for (int b = 0; b < RB; ++b)
 #pragma unroll
-        for (int f = 0; f < NF; ++f) acc[b][f] = mx4_step<A8>(w[u][b], sc[u][b], x[u][f], acc[b][f]);
+        for (int f = 0; f < NF; ++f) acc[b][f] = mx4_step<R>(w[u][b], sc[u][b], x[u][f], acc[b][f]);
     }
   }
 }
@@ -280,7 +306,7 @@ __device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int bloc
 // NF 16-row fragments of rows [p0, p0 + rows) of one slot.  ONE: the one token's
 // act row p0.  SP: rows in two parts, see above.  pairs: the rows' pairs; act rows lie
 // from p0 on, or (SCAN) each at its pair.
-template <bool GU, bool A8, int NF, int NW, bool ONE, bool SP, bool SCAN>
+template <bool GU, int R, int NF, int NW, bool ONE, bool SP, bool SCAN>
 __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, int blocks, int cb, int p0, int rows,
                                          const int32_t* pairs, f32x4_t* s_part) {
   constexpr int RB = kFewMxBlocks;
@@ -295,15 +321,15 @@ __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, 
     const int at = r < rows ? r : 0;
     size_t src = ONE ? 0 : GU ? pairs[at] / g.topk : SCAN ? pairs[at] : p0 + at;
     if constexpr (SP) src = 2 * src + (NF == 1 ? (lane >> 3) & 1 : f);
-    row[f] = static_cast<const char*>(g.a) + src * g.K * (A8 ? 1 : 2);
-    row_scale[f] = A8 ? g.a_scale + src * (g.K / kMxGroup) : nullptr;
+    row[f] = static_cast<const char*>(g.a) + row_bytes<R>(src, g.K);
+    row_scale[f] = R != kRowsBf16 ? g.a_scale + src * (g.K / kMxGroup) : nullptr;
   }
   f32x4_t acc[RB][NF];
 #pragma unroll
   for (int b = 0; b < RB; ++b)
 #pragma unroll
     for (int f = 0; f < NF; ++f) acc[b][f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  few_chunks<A8, RB, NF, ONE ? 2 : 1>(wblk, mx4_block_bytes(g.K), blocks, g.K, wave * chunks / NW, (wave + 1) * chunks / NW,
+  few_chunks<R, RB, NF, ONE ? 2 : 1>(wblk, mx4_block_bytes(g.K), blocks, g.K, wave * chunks / NW, (wave + 1) * chunks / NW,
                             lane, row, row_scale, acc);
   // partial sums of a fragment, [wave][block][lane], added in wave order
   f32x4_t high[2];
@@ -342,7 +368,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, 
     const bool live = r < rows;  // of eight rows at most, those in the lower lanes
     if constexpr (GU) {
       const f32x4_t gate[2] = {t[0], t[2]}, up[2] = {t[1], t[3]};
-      store_act<A8>(g, SCAN ? (live ? pairs[r] : 0) : p0 + r, cb * 32, lane, live, gate, up);
+      store_act<R>(g, SCAN ? (live ? pairs[r] : 0) : p0 + r, cb * 32, lane, live, gate, up);
     } else if (b0 < blocks) {
       store_y(g, live ? pairs[r] : 0, cb * 64 + 32 * wave, lane, live, t[0], t[1]);
     }
@@ -388,7 +414,7 @@ __device__ __forceinline__ int scan_pairs(const Mx4Args& g, const TokenIds& o, i
 
 // (column block, active slot) of a grid of [ceil(N / 32 or 64), slots]; SCAN: (column
 // block, pair)
-template <bool GU, bool A8, bool SP, bool SCAN>
+template <bool GU, int R, bool SP, bool SCAN>
 __global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g, TokenIds o) {
   __shared__ f32x4_t s_part[kFewMxWaves * kFewMxBlocks * 64];
   __shared__ int32_t s_pairs[SCAN ? kScanMaxPairs : 1];
@@ -412,9 +438,9 @@ __global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g, To
     const int rows = min(PASS, p1 - p);
     if (p > p0) __syncthreads();  // the last pass's sums have been read
     if (rows > PASS / 2)
-      few_rows<GU, A8, 2, kFewMxWaves, false, SP, SCAN>(g, wblk, blocks, cb, p, rows, pairs + p, s_part);
+      few_rows<GU, R, 2, kFewMxWaves, false, SP, SCAN>(g, wblk, blocks, cb, p, rows, pairs + p, s_part);
     else
-      few_rows<GU, A8, 1, kFewMxWaves, false, SP, SCAN>(g, wblk, blocks, cb, p, rows, pairs + p, s_part);
+      few_rows<GU, R, 1, kFewMxWaves, false, SP, SCAN>(g, wblk, blocks, cb, p, rows, pairs + p, s_part);
   }
 }
 
@@ -446,7 +472,7 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
   return (const uint8_t*)(global_t)(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-template <bool A8>
+template <int R>
 __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_gateup_kernel(Mx4Args g, TokenIds o) {
   __shared__ f32x4_t s_part[kOneMxWaves * kFewMxBlocks * 64];
   const int j = blockIdx.y;
@@ -454,14 +480,14 @@ __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_gateup_kernel(Mx4Arg
   if (expert == nullptr) return;
   const int cb = blockIdx.x;
   const uint8_t* wblk = expert + static_cast<size_t>(cb) * kFewMxBlocks * mx4_block_bytes(g.K);
-  few_rows<true, A8, 1, kOneMxWaves, true, false, false>(g, wblk, kFewMxBlocks, cb, j, 1, nullptr, s_part);
+  few_rows<true, R, 1, kOneMxWaves, true, false, false>(g, wblk, kFewMxBlocks, cb, j, 1, nullptr, s_part);
 }
 
 // 16 columns of out = add + sum_j w_j W2_j act_j.  The waves take (pair, part of K)
 // units in turn, each adding its units' weighted sums; the waves' sums are added in
 // order.  A unit is the whole K of a pair where there are eight pairs or more.  bf16
 // rows come in two parts, the fragment's lower and upper rows.
-template <bool A8>
+template <int R>
 __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_down_kernel(Mx4Args g, TokenIds o,
                                                                        const uint16_t* __restrict__ wts,
                                                                        const uint16_t* __restrict__ add) {
@@ -482,16 +508,16 @@ __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_down_kernel(Mx4Args 
       continue;
     }
     const float wj = bf16_to_f32(wts[j]);
-    const size_t src = A8 ? j : 2 * j + ((lane >> 3) & 1);
-    const char* row[1] = {static_cast<const char*>(g.a) + src * g.K * (A8 ? 1 : 2)};
-    const uint8_t* row_scale[1] = {A8 ? g.a_scale + static_cast<size_t>(j) * (g.K / kMxGroup) : nullptr};
+    const size_t src = R != kRowsBf16 ? j : 2 * j + ((lane >> 3) & 1);
+    const char* row[1] = {static_cast<const char*>(g.a) + row_bytes<R>(src, g.K)};
+    const uint8_t* row_scale[1] = {R != kRowsBf16 ? g.a_scale + static_cast<size_t>(j) * (g.K / kMxGroup) : nullptr};
     f32x4_t acc[1][1] = {{f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}}};
     const uint8_t* wblk = expert + static_cast<size_t>(blockIdx.x) * bb;
-    few_chunks<A8, 1, 1, 4>(wblk, bb, 1, g.K, part * chunks / parts, (part + 1) * chunks / parts, lane, row, row_scale,
+    few_chunks<R, 1, 1, 4>(wblk, bb, 1, g.K, part * chunks / parts, (part + 1) * chunks / parts, lane, row, row_scale,
                             acc);
     sum += wj * acc[0][0];
   }
-  if constexpr (!A8) sum += other_part(sum);
+  if constexpr (R == kRowsBf16) sum += other_part(sum);
   // the sixteen rows of the fragment are the same row: lanes 0, 16, 32 and 48 have it
   if ((lane & 15) == 0) s_part[wave * 4 + (lane >> 4)] = sum;
   __syncthreads();

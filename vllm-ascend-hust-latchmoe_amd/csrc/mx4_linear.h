@@ -1,0 +1,85 @@
+// One matrix of 4-bit weights: y = x W^T (+ bias) (+ add).
+//
+// Rows are bf16, MX8 or MX4; weights one slot of a bank in order (mx.h), sums in f32.
+#pragma once
+
+#include "mx4_few.h"
+
+namespace lmoe {
+
+struct LinearArgs {
+  const void* x;            // rows [T, K]
+  const uint8_t* x_scale;   // MX8 and MX4 rows, else null
+  const uint8_t* w;
+  int T, K, N;
+  const void* bias;         // [N] bf16 or f32, or null
+  const uint16_t* add;      // [T, N] bf16, or null
+  void* out;                // [T, N] bf16 or f32
+  bool bias_f32, out_f32;
+};
+
+// Four neighbouring columns of a row: bias and add, rounded once.
+__device__ __forceinline__ void store_linear4(const LinearArgs& g, int row, int n, f32x4_t v) {
+  if (g.bias != nullptr) {
+    if (g.bias_f32) {
+      v += *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(g.bias) + n);
+    } else {
+      const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(g.bias) + n);
+      v += f32x4_t{bf16lo(b.x), bf16hi(b.x), bf16lo(b.y), bf16hi(b.y)};
+    }
+  }
+  const size_t at = static_cast<size_t>(row) * g.N + n;
+  if (g.add != nullptr) {
+    const uint2 a = *reinterpret_cast<const uint2*>(g.add + at);
+    v += f32x4_t{bf16lo(a.x), bf16hi(a.x), bf16lo(a.y), bf16hi(a.y)};
+  }
+  if (g.out_f32) *reinterpret_cast<f32x4_t*>(static_cast<float*>(g.out) + at) = v;
+  else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(g.out) + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+
+// Few rows: a workgroup takes RB blocks of 16 columns by NF fragments of 16 rows; its NW
+// waves split K, their partial sums are added in LDS in wave order.
+template <int R, int RB, int NF, int NW>
+__global__ __launch_bounds__(NW * 64) void mx4_linear_few_kernel(LinearArgs g) {
+  __shared__ f32x4_t s_part[NW * RB * NF * 64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunks = mx4_chunks(g.K);
+  const int bb = mx4_block_bytes(g.K);
+  const int cols = ((g.N >> 4) + RB - 1) / RB;
+  const int group = blockIdx.x / cols, cb = blockIdx.x - group * cols;
+  const int t0 = group * (16 * NF);
+  const int blocks = min(RB, (g.N >> 4) - cb * RB);
+  const uint8_t* wblk = g.w + static_cast<size_t>(cb) * RB * bb;
+  const char* row[NF];
+  const uint8_t* row_scale[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    const int r = t0 + 16 * f + (lane & 15);
+    const size_t src = r < g.T ? r : t0;
+    row[f] = static_cast<const char*>(g.x) + row_bytes<R>(src, g.K);
+    row_scale[f] = R != kRowsBf16 ? g.x_scale + src * (g.K / kMxGroup) : nullptr;
+  }
+  f32x4_t acc[RB][NF];
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int f = 0; f < NF; ++f) acc[b][f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  few_chunks<R, RB, NF, RB == 1 ? 2 : 1>(wblk, bb, blocks, g.K, wave * chunks / NW, (wave + 1) * chunks / NW, lane, row,
+                                         row_scale, acc);
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int f = 0; f < NF; ++f) s_part[((wave * RB + b) * NF + f) * 64 + lane] = acc[b][f];
+  __syncthreads();
+  for (int u = wave; u < RB * NF; u += NW) {
+    const int b = u / NF, f = u - b * NF;
+    f32x4_t v = s_part[u * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) v += s_part[(w * RB * NF + u) * 64 + lane];
+    const int r = t0 + 16 * f + (lane & 15);
+    if (b < blocks && r < g.T) store_linear4(g, r, (cb * RB + b) * 16 + 4 * (lane >> 4), v);
+  }
+}
+
+}  // namespace lmoe

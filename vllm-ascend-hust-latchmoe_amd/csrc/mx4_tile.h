@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   const int K = g.K;
   const int chunks = mx4_chunks(K);
   const int tail = K & (kMxChunk - 1);  // columns of a short last chunk, 0: none
-  const size_t row_bytes = static_cast<size_t>(K) * (A8 ? 1 : 2);
+  constexpr int R = A8 ? kRowsMx8 : kRowsBf16;
 
   // this lane's source of each load instruction: row, and piece within a chunk
   auto a_row = [&](int q) { return (wave * C::QA + q) * C::RPL + lane / C::PIECES; };
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
     const int r = a_row(q);
     const int pos = p0 + (r < rows ? r : 0);
     const size_t src = GU ? g.sorted_pairs[pos] / g.topk : pos;
-    a_src[q] = static_cast<const char*>(g.a) + src * row_bytes + a_piece(q) * 16;
+    a_src[q] = static_cast<const char*>(g.a) + row_bytes<R>(src, K) + a_piece(q) * 16;
   }
   const int stages = (chunks + CS - 1) / CS;
   auto issue = [&](int stage, int buf) {
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
         const char* st = smem + (stage & 1) * C::STAGE + e * C::PART + fr * C::ROWB;
         // the next row fragment is on its way from LDS while this one is multiplied
         if constexpr (A8 && NL > 0) {
-          RowFrag<true> x[2];
+          RowFrag<kRowsMx8> x[2];
           const uint8_t* xs = reinterpret_cast<const uint8_t*>(s_scale + c * BM + fr) + lg;
           auto read = [&](int i) {
             const char* p = st + i * 16 * C::ROWB;
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
             if (i + 1 < NL) read(i + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = mx4_step<true>(w[j], sc[j], x[i & 1], acc[i][j]);
+            for (int j = 0; j < 4; ++j) acc[i][j] = mx4_step<kRowsMx8>(w[j], sc[j], x[i & 1], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
           }
         } else if constexpr (NL > 0) {
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
     if (i >= live) break;
     if constexpr (GU) {
       const f32x4_t gate[2] = {acc[i][0], acc[i][2]}, up[2] = {acc[i][1], acc[i][3]};
-      store_act<A8>(g, p0 + r, n0 + 32 * wave, lane, r < rows, gate, up);
+      store_act<R>(g, p0 + r, n0 + 32 * wave, lane, r < rows, gate, up);
     } else {
       const int pair = s_pair[r];
       store_y(g, pair, n0 + 64 * wave, lane, r < rows, acc[i][0], acc[i][1]);

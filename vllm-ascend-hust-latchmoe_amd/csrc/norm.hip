@@ -14,6 +14,7 @@
 #include <hip/hip_runtime.h>
 
 #include "mx.h"
+#include "spans.h"
 
 namespace lmoe {
 
@@ -27,6 +28,7 @@ struct NormArgs {
   uint8_t* scale;
   float eps;
   int H;
+  bool q4;                 // q holds MX4 rows, not MX8 ones
 };
 
 enum { kNone = 0, kBf16 = 1, kF32 = 2 };
@@ -51,20 +53,25 @@ __device__ __forceinline__ void load8(const void* p, size_t at, float (&f)[8]) {
   }
 }
 
-// Eight columns to 8 bits.  Four neighbouring lanes hold a group of 32, which
+// Eight columns to 8 or 4 bits.  Four neighbouring lanes hold a group of 32, which
 // never straddles the end of the row (H % 32 == 0); the maximum over the four
 // goes by two quad permutes.
-__device__ __forceinline__ void store_mx8(const NormArgs& g, int row, int h, const float (&y)[8]) {
+__device__ __forceinline__ void store_mx(const NormArgs& g, int row, int h, const float (&y)[8]) {
   uint32_t m = abs_bits(y[0]);
 #pragma unroll
   for (int e = 1; e < 8; ++e) m = umax32(m, abs_bits(y[e]));
   m = umax32(m, dpp_u32<kDppQuadXor1>(m));
   m = umax32(m, dpp_u32<kDppQuadXor2>(m));
-  const int b = mx8_scale_byte(__uint_as_float(m));
+  const int b = g.q4 ? mx4_scale_byte(__uint_as_float(m)) : mx8_scale_byte(__uint_as_float(m));
   const float s = mx_scale_f32(b);
-  const uint2 v = make_uint2(pack_e4m3x4(y[0], y[1], y[2], y[3], s),
-                             pack_e4m3x4(y[4], y[5], y[6], y[7], s));
-  *reinterpret_cast<uint2*>(g.q + static_cast<size_t>(row) * g.H + h) = v;
+  const size_t at = static_cast<size_t>(row) * g.H + h;
+  if (g.q4) {
+    *reinterpret_cast<uint32_t*>(g.q + at / 2) = pack_e2m1x8(y, s, b);
+  } else {
+    const uint2 v = make_uint2(pack_e4m3x4(y[0], y[1], y[2], y[3], s),
+                               pack_e4m3x4(y[4], y[5], y[6], y[7], s));
+    *reinterpret_cast<uint2*>(g.q + at) = v;
+  }
   if ((h & (kMxGroup - 1)) == 0)
     g.scale[static_cast<size_t>(row) * (g.H / kMxGroup) + h / kMxGroup] = static_cast<uint8_t>(b);
 }
@@ -130,7 +137,7 @@ __global__ __launch_bounds__(1024) void add_rms_norm_kernel(NormArgs g) {
     const int h = v * step + threadIdx.x * 8;
     if (h >= H) continue;
     if (g.out != nullptr) *reinterpret_cast<uint4*>(g.out + base + h) = pack8(r[v]);
-    if (g.q != nullptr) store_mx8(g, row, h, r[v]);
+    if (g.q != nullptr) store_mx(g, row, h, r[v]);
   }
 }
 
@@ -147,17 +154,6 @@ static void launch_norm(const NormArgs& g, int T, hipStream_t stream) {
   else add_rms_norm_kernel<4, RES, WEIGHT><<<T, threads, 0, stream>>>(g);
 }
 
-static bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
-
-struct Span {
-  const void* p;
-  size_t bytes;
-};
-static bool overlap(const Span& a, const Span& b) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(a.p), q = reinterpret_cast<uintptr_t>(b.p);
-  return p != 0 && q != 0 && p < q + b.bytes && q < p + a.bytes;
-}
-
 // Whether an output would be written over another one, or over an input that other
 // workgroups (weight: any) still read.  Only a row over itself is safe, where both
 // start at one address and their rows are as long.
@@ -165,7 +161,7 @@ static bool clobbers(const NormArgs& g, int T, bool residual_f32, bool weight_f3
   const size_t n = static_cast<size_t>(T) * g.H;
   const size_t rb = residual_f32 ? 4 : 2;
   const Span in[3] = {{g.x, 2 * n}, {g.residual, rb * n}, {g.weight, static_cast<size_t>(g.H) * (weight_f32 ? 4 : 2)}};
-  const Span out[4] = {{g.residual_out, rb * n}, {g.out, 2 * n}, {g.q, n}, {g.scale, n / kMxGroup}};
+  const Span out[4] = {{g.residual_out, rb * n}, {g.out, 2 * n}, {g.q, g.q4 ? n / 2 : n}, {g.scale, n / kMxGroup}};
   const size_t in_row[3] = {2, rb, 0}, out_row[4] = {rb, 2, 1, 0};  // bytes of a column
   for (int o = 0; o < 4; ++o) {
     for (int i = 0; i < 3; ++i)
@@ -180,10 +176,9 @@ static bool clobbers(const NormArgs& g, int T, bool residual_f32, bool weight_f3
 
 using namespace lmoe;
 
-extern "C" int lmoe_add_rms_norm(const void* x, int T, int H, const void* residual,
-                                 int residual_f32, const void* weight, int weight_f32, float eps,
-                                 void* residual_out, void* out, void* q, void* scale,
-                                 hipStream_t stream) {
+static int add_rms_norm(const void* x, int T, int H, const void* residual, int residual_f32, const void* weight,
+                        int weight_f32, float eps, void* residual_out, void* out, void* q, void* scale, bool q4,
+                        hipStream_t stream) {
   if (T < 0 || H <= 0 || !(eps >= 0.0f)) return LMOE_ERR_ARG;
   if (H % 8 != 0 || H > kNormMaxCols) return LMOE_ERR_SHAPE;
   if (q != nullptr && H % kMxGroup != 0) return LMOE_ERR_SHAPE;
@@ -196,7 +191,7 @@ extern "C" int lmoe_add_rms_norm(const void* x, int T, int H, const void* residu
     return LMOE_ERR_SHAPE;
   const NormArgs g{static_cast<const uint16_t*>(x), residual, weight, residual_out,
                    static_cast<uint16_t*>(out), static_cast<uint8_t*>(q),
-                   static_cast<uint8_t*>(scale), eps, H};
+                   static_cast<uint8_t*>(scale), eps, H, q4};
   if (clobbers(g, T, residual_f32 != 0, weight_f32 != 0)) return LMOE_ERR_ARG;
   if (residual == nullptr) {
     if (weight_f32) launch_norm<kNone, kF32>(g, T, stream);
@@ -211,6 +206,21 @@ extern "C" int lmoe_add_rms_norm(const void* x, int T, int H, const void* residu
   LMOE_RETURN_LAUNCH();
 }
 
+extern "C" int lmoe_add_rms_norm(const void* x, int T, int H, const void* residual,
+                                 int residual_f32, const void* weight, int weight_f32, float eps,
+                                 void* residual_out, void* out, void* q, void* scale,
+                                 hipStream_t stream) {
+  return add_rms_norm(x, T, H, residual, residual_f32, weight, weight_f32, eps, residual_out, out, q, scale, false,
+                      stream);
+}
+
+extern "C" int lmoe_add_rms_norm_mx4(const void* x, int T, int H, const void* residual, int residual_f32,
+                                     const void* weight, int weight_f32, float eps, void* residual_out, void* out,
+                                     void* q, void* scale, hipStream_t stream) {
+  return add_rms_norm(x, T, H, residual, residual_f32, weight, weight_f32, eps, residual_out, out, q, scale, true,
+                      stream);
+}
+
 extern "C" int lmoe_rows_to_mx8(const void* x, int T, int H, void* q, void* scale,
                                 hipStream_t stream) {
   if (T < 0 || H <= 0) return LMOE_ERR_ARG;
@@ -219,7 +229,7 @@ extern "C" int lmoe_rows_to_mx8(const void* x, int T, int H, void* q, void* scal
   if (x == nullptr || q == nullptr || scale == nullptr) return LMOE_ERR_ARG;
   if (misaligned16(x) || misaligned16(q)) return LMOE_ERR_SHAPE;
   const NormArgs g{static_cast<const uint16_t*>(x), nullptr, nullptr, nullptr, nullptr,
-                   static_cast<uint8_t*>(q), static_cast<uint8_t*>(scale), 0.0f, H};
+                   static_cast<uint8_t*>(q), static_cast<uint8_t*>(scale), 0.0f, H, false};
   if (clobbers(g, T, false, false)) return LMOE_ERR_ARG;
   launch_norm<kNone, kNone>(g, T, stream);
   LMOE_RETURN_LAUNCH();

@@ -49,7 +49,7 @@ from vllm_moe_offload_amd.moe_offload.slot_mapping import PreparedSlotWeights
 @dataclass
 class MoEWorkspace:
     perm: native.Permutation
-    act: torch.Tensor   # [N, I] bf16 (or Mx8Rows, or bf16 [N, 2, I] in two parts), sorted order
+    act: torch.Tensor   # [N, I] bf16 (or Mx8Rows, Mx4Rows, or bf16 [N, 2, I] in two parts), sorted order
     y: torch.Tensor     # [N, H] bf16 (or f32), flat pair order
     out: torch.Tensor   # [T, H] bf16
     perm_overflow: native.Permutation | None = None  # the decode overflow pass's permutation
@@ -58,7 +58,7 @@ class MoEWorkspace:
 
     def act_rows(self, n: int, path: int):
         """act of n pairs as a path takes it: two parts on LMOE_PATH_GEMV only."""
-        if isinstance(self.act, native.Mx8Rows) or self.act.dim() == 2 or path == native.LMOE_PATH_GEMV:
+        if not isinstance(self.act, torch.Tensor) or self.act.dim() == 2 or path == native.LMOE_PATH_GEMV:
             return self.act[:n]
         I = self.act.shape[-1]
         return self.act.view(-1)[: n * I].view(n, I)
@@ -85,13 +85,14 @@ def _device_key(device) -> tuple:
 
 def rows_kind(hidden, w13_slots) -> str:
     """What a layer's workspace holds: "" for bf16 experts; for 4-bit experts
-    the kind of the rows, "bf16" or "mx8" (hidden is native.Mx8Rows)."""
-    mx8 = isinstance(hidden, native.Mx8Rows)
+    the kind of the rows, "bf16", "mx8" (hidden is native.Mx8Rows) or "mx4"
+    (native.Mx4Rows)."""
+    kind = "mx8" if isinstance(hidden, native.Mx8Rows) else "mx4" if isinstance(hidden, native.Mx4Rows) else "bf16"
     if not mxfp4.is_mx4(w13_slots):
-        if mx8:
-            raise ValueError("8-bit rows go through 4-bit experts only (bf16 slot bank)")
+        if kind != "bf16":
+            raise ValueError(f"{kind[2]}-bit rows go through 4-bit experts only (bf16 slot bank)")
         return ""
-    return "mx8" if mx8 else "bf16"
+    return kind
 
 
 def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = "", rows: str = "") -> MoEWorkspace:
@@ -112,7 +113,7 @@ def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = 
 
 
 def _workspace(T, k, P, H, I, device, tag: str, rows: str, cleared: bool) -> MoEWorkspace:
-    if rows not in ("", "bf16", "mx8"):
+    if rows not in ("", "bf16", "mx8", "mx4"):
         raise ValueError(f"unknown rows {rows!r}")
     where = _device_key(device)
     stream = 0
@@ -134,6 +135,7 @@ def _make_workspace(T: int, k: int, P: int, H: int, I: int, device, rows: str, *
     ws = MoEWorkspace(
         perm=native.Permutation.allocate(N, P, device, cleared=cleared),
         act=native.Mx8Rows.allocate(max(N, 1), I, device) if rows == "mx8" else
+        native.Mx4Rows.allocate(max(N, 1), I, device) if rows == "mx4" else
         torch.empty((max(N, 1), 2, I) if few else (max(N, 1), I), dtype=torch.bfloat16, device=device),
         y=torch.empty((max(N, 1), H), dtype=y_dtype, device=device),
         out=torch.empty((max(T, 1), H), dtype=torch.bfloat16, device=device),
@@ -246,8 +248,8 @@ def fused_experts(
     The result is out; without it a new tensor, or with a workspace of the
     caller's that workspace's out, which its next call overwrites.
 
-    Over 4-bit banks (uint8, mxfp4.pack_experts) hidden is bf16 or
-    native.Mx8Rows; few tokens go straight from their ids, without a permutation
+    Over 4-bit banks (uint8, mxfp4.pack_experts) hidden is bf16, native.Mx8Rows or
+    native.Mx4Rows (act is then rounded to 4 bits between the products); few tokens go straight from their ids, without a permutation
     in the workspace."""
     if w13_slots.dtype is torch.uint8:
         return _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, add=add, out=out, path=path,
@@ -271,9 +273,9 @@ def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2
         raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
     dst = _result(out, hidden) if workspace is None or out is not None else ws.out[:T]
     I = w13_slots.shape[1] // 2
-    mx8 = isinstance(hidden, native.Mx8Rows)
+    mx8, mx4 = isinstance(hidden, native.Mx8Rows), isinstance(hidden, native.Mx4Rows)
     if path == native.LMOE_PATH_AUTO:
-        path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel(), mx8, max(H, I))
+        path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel(), mx8, max(H, I), mx4=mx4)
         if path == native.LMOE_PATH_GEMV and (T == 1 or T * k <= native.MX4_DIRECT_PAIRS and not counted):
             if counted:  # one token's form reads no permutation
                 native.permute(topk_ids, ws.perm, log2phy=log2phy)
@@ -294,7 +296,8 @@ def _layer_path(hidden, k: int, n_experts: int, *w13) -> int:
     gives the unsplit layer's bits."""
     T, H = hidden.shape
     if mxfp4.is_mx4(w13[0]):
-        return native.mx4_path(T * k, n_experts, isinstance(hidden, native.Mx8Rows), max(H, int(w13[0].shape[1]) // 2))
+        return native.mx4_path(T * k, n_experts, isinstance(hidden, native.Mx8Rows), max(H, int(w13[0].shape[1]) // 2),
+                               mx4=isinstance(hidden, native.Mx4Rows))
     return native.layer_path(T, k, H, int(w13[0].shape[1]) // 2, n_experts, aligned=native.aligned16(hidden, *w13))
 
 
@@ -482,7 +485,7 @@ def decode_layer(
     w_out: torch.Tensor | None = None,
     ids_out: torch.Tensor | None = None,
     overflow: PreparedSlotWeights | None = None,
-    expert_rows: native.Mx8Rows | None = None,
+    expert_rows: native.Mx8Rows | native.Mx4Rows | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """route() followed by fused_experts(), for a slot table that is final
     before the router runs (the decode replay after staging): gate, expert
@@ -495,7 +498,7 @@ def decode_layer(
     overflow: the layer's second pass (stage buffer + overflow table) for a
     working set past the bank; both passes and the combine are fixed-shape
     launches, so a graph captured with them replays any split.
-    expert_rows: the same hidden states in 8 bits (native.add_rms_norm gives
+    expert_rows: the same hidden states in 8 or 4 bits (native.add_rms_norm gives
     both), for the experts of a 4-bit bank; the gate reads hidden."""
     T = hidden.shape[0]
     rows = hidden if expert_rows is None else expert_rows

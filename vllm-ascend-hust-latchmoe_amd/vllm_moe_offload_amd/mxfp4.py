@@ -13,7 +13,8 @@ holds a gate and its up column together.  An expert is one contiguous run of
 bytes either way: host store, slot bank and staging move it like any other
 weight.
 
-Everything here runs on the tensors' own device, once per weight.
+Everything here runs on the tensors' own device, once per weight; pack_experts takes
+weights on the GPU through its kernel (native.quantize_mx4), which gives the same bytes.
 """
 
 from __future__ import annotations
@@ -175,6 +176,12 @@ def _empty(shape: tuple, device, pin: bool) -> torch.Tensor:
     return torch.empty(shape, dtype=torch.uint8, device=device)
 
 
+def _has_kernel(w: torch.Tensor, gate_up: bool) -> bool:
+    """Whether native.quantize_mx4 takes these weights."""
+    return w.is_cuda and w.dtype in (torch.bfloat16, torch.float32) and w.is_contiguous() and \
+        w.data_ptr() % 16 == 0 and int(w.shape[1]) % (64 if gate_up else ROWS) == 0
+
+
 def pack_experts(w13: torch.Tensor, w2: torch.Tensor, *, pin_memory: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """4-bit banks of bf16 (or f32) experts w13 [E, 2I, H], w2 [E, H, I], an
     expert at a time: what SlotMoELayer registers for 4-bit experts.  pin_memory:
@@ -187,6 +194,13 @@ def pack_experts(w13: torch.Tensor, w2: torch.Tensor, *, pin_memory: bool = Fals
     out = []
     for w, pack in ((w13, pack_w13), (w2, pack_w2)):
         bank = _empty((*w.shape[:2], row_bytes(int(w.shape[2]))), w.device, pin_memory)
+        if _has_kernel(w, pack is pack_w13):
+            from vllm_moe_offload_amd import native  # which needs this module
+
+            with torch.cuda.device(w.device):
+                native.quantize_mx4(w.detach(), bank, gate_up=pack is pack_w13)
+            out.append(bank)
+            continue
         for e in range(int(w.shape[0])):
             bank[e] = pack(*quantize(w[e]))
         out.append(bank)

@@ -67,13 +67,24 @@ EXPORTED_SYMBOLS = (
     "lmoe_combine",
     "lmoe_combine_f32",
     "lmoe_add_rms_norm",
+    "lmoe_add_rms_norm_mx4",
     "lmoe_rows_to_mx8",
+    "lmoe_rows_to_mx4",
+    "lmoe_mx4_rows_values",
+    "lmoe_mx4_quantize",
+    "lmoe_mx4_bank_values",
+    "lmoe_mx4_linear",
     "lmoe_mx4_bytes",
     "lmoe_mx4_gateup_silu",
     "lmoe_mx4_down",
     "lmoe_mx4_fused_moe",
     "lmoe_mx4_decode_few",
     "lmoe_mx4_decode_one",
+    "lmoe_mx44_gateup_silu",
+    "lmoe_mx44_down",
+    "lmoe_mx44_fused_moe",
+    "lmoe_mx44_decode_few",
+    "lmoe_mx44_decode_one",
     "lmoe_fused_moe_decode",
     "lmoe_fused_moe_decode_noalloc",
     "lmoe_down_combine",
@@ -153,6 +164,11 @@ _SIGNATURES = {
     "lmoe_combine_f32": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
     "lmoe_add_rms_norm": (_i, [_vp, _i, _i, _vp, _i, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp]),
     "lmoe_rows_to_mx8": (_i, [_vp, _i, _i, _vp, _vp, _vp]),
+    "lmoe_rows_to_mx4": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
+    "lmoe_mx4_rows_values": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp]),
+    "lmoe_mx4_quantize": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp]),
+    "lmoe_mx4_bank_values": (_i, [_vp, _i, _i, _i, _i, _vp, _i, _vp]),
+    "lmoe_mx4_linear": (_i, [_vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _i, _vp]),
     "lmoe_mx4_bytes": (ctypes.c_longlong, [_i, _i]),
     "lmoe_mx4_gateup_silu": (
         _i,
@@ -196,6 +212,10 @@ _SIGNATURES = {
          _vp, _i, _i, _i, _vp],
     ),
 }
+
+_SIGNATURES["lmoe_add_rms_norm_mx4"] = _SIGNATURES["lmoe_add_rms_norm"]
+for _name in ("gateup_silu", "down", "fused_moe", "decode_few", "decode_one"):  # the same over MX4 rows
+    _SIGNATURES[f"lmoe_mx44_{_name}"] = _SIGNATURES[f"lmoe_mx4_{_name}"]
 
 _LIB: ctypes.CDLL | None = None
 
@@ -375,6 +395,46 @@ class Mx8Rows:
         return (self.q.float().unflatten(-1, (-1, mxfp4.GROUP)) * s.unsqueeze(-1)).flatten(-2)
 
 
+@dataclass(frozen=True)
+class Mx4Rows:
+    """Rows in 4 bits: e2m1 codes, two per byte (the even column in the low half), one
+    power-of-two scale per 32 columns (value[r, c] = code * 2^(scale[r, c // 32] - 127);
+    255: NaN)."""
+
+    q: torch.Tensor      # [R, K / 2] uint8
+    scale: torch.Tensor  # [R, K / 32] uint8
+
+    @classmethod
+    def allocate(cls, rows: int, columns: int, device) -> "Mx4Rows":
+        if int(columns) <= 0 or int(columns) % mxfp4.GROUP:
+            raise ValueError(f"4-bit rows are multiples of {mxfp4.GROUP} columns, got {columns}")
+        return cls(torch.empty((int(rows), int(columns) // 2), dtype=torch.uint8, device=device),
+                   torch.empty((int(rows), int(columns) // mxfp4.GROUP), dtype=torch.uint8, device=device))
+
+    @property
+    def shape(self) -> torch.Size:
+        """[R, K]: of the values, not of the bytes."""
+        q = self.q.shape
+        return torch.Size((*q[:-1], 2 * q[-1]))
+
+    @property
+    def device(self) -> torch.device:
+        return self.q.device
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.q.dtype
+
+    def __getitem__(self, rows: slice) -> "Mx4Rows":
+        if not isinstance(rows, slice):
+            raise TypeError("4-bit rows are sliced by rows")
+        return Mx4Rows(self.q[rows], self.scale[rows])
+
+    def float(self) -> torch.Tensor:
+        """The f32 values that the rows stand for (checks and exports)."""
+        return mxfp4.dequantize(self.q, self.scale)
+
+
 def _is(t, dtype: torch.dtype, shape: tuple) -> bool:
     """What _need checks, without its words: for calls whose host time counts.
     (_need then says what is wrong.)"""
@@ -391,6 +451,21 @@ def _need_mx8(rows, name: str, shape: tuple | None = None) -> None:
     if rows.q.dim() != 2 or rows.q.shape[1] % mxfp4.GROUP:
         raise ValueError(f"{name} must be [R, K], K a multiple of {mxfp4.GROUP}, got {tuple(rows.q.shape)}")
     _need(rows.scale, f"{name}.scale", torch.uint8, (rows.q.shape[0], rows.q.shape[1] // mxfp4.GROUP))
+
+
+def _need_mx4_rows(rows, name: str, shape: tuple | None = None) -> None:
+    if not isinstance(rows, Mx4Rows):
+        raise TypeError(f"{name} must be Mx4Rows")
+    if shape is not None and len(shape) == 2 and shape[1] % mxfp4.GROUP == 0 and \
+            _is(rows.q, torch.uint8, (shape[0], shape[1] // 2)) and \
+            _is(rows.scale, torch.uint8, (shape[0], shape[1] // mxfp4.GROUP)):
+        return
+    _need(rows.q, f"{name}.q", torch.uint8)
+    if rows.q.dim() != 2 or rows.q.shape[1] % (mxfp4.GROUP // 2):
+        raise ValueError(f"{name}.q must be [R, K / 2], K a multiple of {mxfp4.GROUP}, got {tuple(rows.q.shape)}")
+    if shape is not None and tuple(rows.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(rows.shape)}, expected {tuple(shape)}")
+    _need(rows.scale, f"{name}.scale", torch.uint8, (rows.q.shape[0], rows.q.shape[1] * 2 // mxfp4.GROUP))
 
 
 def _same_device(*tensors) -> None:
@@ -416,6 +491,16 @@ def _take_mx8(rows, name: str, shape, here: int) -> tuple[torch.Tensor, torch.Te
     return q, scale
 
 
+def _take_mx4(rows, name: str, shape, here: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of 4-bit rows [T, K] on device here."""
+    q, scale = rows.q, rows.scale
+    if not (shape[1] % 32 == 0 and _fits(q, torch.uint8, (shape[0], shape[1] // 2), here) and
+            _fits(scale, torch.uint8, (shape[0], shape[1] // 32), here)):
+        _need_mx4_rows(rows, name, tuple(shape))
+        _same_device(q, scale)
+    return q, scale
+
+
 def _refuse(t, name: str, dtype: torch.dtype, shape: tuple | None = None) -> None:
     _need(t, name, dtype, shape)
     _same_device(t)
@@ -429,20 +514,22 @@ def add_rms_norm(
     residual_out: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
     mx8: Mx8Rows | None = None,
+    mx4: Mx4Rows | None = None,
     eps: float = 1e-6,
     stream=None,
 ):
     """r = x + residual; y = r / sqrt(mean(r^2) + eps) * weight.
 
-    y goes to out (bf16: the router gate, bf16 experts), to mx8 (4-bit experts'
-    8-bit rows) or to both; with neither given a bf16 out is made.  r goes to
+    y goes to out (bf16: the router gate, bf16 experts), to mx8 or mx4 (4-bit experts'
+    rows in 8 or in 4 bits), or to out and one of these; with none given a bf16 out is
+    made.  r goes to
     residual_out, in place of residual if that is not given.  x [T, H] bf16,
     residual bf16 or f32, weight [H] bf16 or f32; r is kept in f32 between the
     sum and the outputs, the squares are summed in f32.  residual_out may be x,
     out may be x, or residual if residual_out is another buffer (where an f32
     residual is not one of them); outputs that overlap anything otherwise are
-    refused.  H a multiple of 8 (of 32 with mx8) up to 32768.  Returns (out, mx8,
-    residual_out), None for what was not asked for."""
+    refused.  H a multiple of 8 (of 32 with mx8 or mx4) up to 32768.  Returns (out,
+    mx8 or mx4, residual_out), None for what was not asked for."""
     lib = load_library()
     bf16, f32 = torch.bfloat16, torch.float32
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
@@ -468,7 +555,7 @@ def add_rms_norm(
         raise ValueError("residual_out needs a residual")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    if out is None and mx8 is None:
+    if out is None and mx8 is None and mx4 is None:
         out = _new(shape, bf16, x.device, stream)
     elif out is not None and not _fits(out, bf16, shape, here):
         _refuse(out, "out", bf16, shape)
@@ -477,6 +564,14 @@ def add_rms_norm(
         if not isinstance(mx8, Mx8Rows):
             raise TypeError("mx8 must be Mx8Rows")
         q, scale = _take_mx8(mx8, "mx8", shape, here)
+    norm = lib.lmoe_add_rms_norm
+    if mx4 is not None:
+        if mx8 is not None:
+            raise ValueError("mx8 or mx4, not both")
+        if not isinstance(mx4, Mx4Rows):
+            raise TypeError("mx4 must be Mx4Rows")
+        q, scale = _take_mx4(mx4, "mx4", shape, here)
+        norm = lib.lmoe_add_rms_norm_mx4
     px, po = x.data_ptr(), None if out is None else out.data_ptr()
     pr = pro = None
     if residual is not None:
@@ -486,12 +581,12 @@ def add_rms_norm(
                 raise ValueError("out and residual_out must be two buffers")
             if rdt is f32 and (po == pr or pro == px):
                 raise ValueError("rows of two types cannot share a buffer")
-    status = lib.lmoe_add_rms_norm(px, T, H, pr, rdt is f32, weight.data_ptr(), wdt is f32, eps, pro, po, _ptr(q),
-                                   _ptr(scale), _stream(stream))
+    status = norm(px, T, H, pr, rdt is f32, weight.data_ptr(), wdt is f32, eps, pro, po, _ptr(q), _ptr(scale),
+                  _stream(stream))
     if status:
         _refuse_overlap(status, H)
         _check(status, "lmoe_add_rms_norm")
-    return out, mx8, residual_out
+    return out, mx8 if mx4 is None else mx4, residual_out
 
 
 def _refuse_overlap(status: int, H: int) -> None:
@@ -515,6 +610,169 @@ def rows_to_mx8(x: torch.Tensor, mx8: Mx8Rows | None = None, *, stream=None) -> 
     _refuse_overlap(status, x.shape[1])
     _check(status, "lmoe_rows_to_mx8")
     return mx8
+
+
+_BF16_OR_F32 = (torch.bfloat16, torch.float32)
+
+
+def rows_to_mx4(x: torch.Tensor, mx4: Mx4Rows | None = None, *, stream=None) -> Mx4Rows:
+    """bf16 or f32 rows x [T, H] in 4 bits, H a multiple of 32: mxfp4.quantize's codes
+    and scales."""
+    lib = load_library()
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a [T, H] tensor")
+    here = _device_index()
+    shape, dtype = x.shape, x.dtype
+    if dtype not in _BF16_OR_F32:
+        raise ValueError(f"x must be bf16 or f32, got {dtype}")
+    if not _fits(x, dtype, shape, here):
+        _refuse(x, "x", dtype)
+    if mx4 is None:
+        with _on(stream):
+            mx4 = Mx4Rows.allocate(shape[0], shape[1], x.device)
+    elif not isinstance(mx4, Mx4Rows):
+        raise TypeError("mx4 must be Mx4Rows")
+    q, scale = _take_mx4(mx4, "mx4", shape, here)
+    status = lib.lmoe_rows_to_mx4(x.data_ptr(), dtype is torch.float32, shape[0], shape[1], q.data_ptr(), scale.data_ptr(),
+                                  _stream(stream))
+    if status:
+        _refuse_overlap(status, shape[1])
+        _check(status, "lmoe_rows_to_mx4")
+    return mx4
+
+
+def _bank_rows(bank: torch.Tensor, name: str, columns: int, here: int) -> tuple[int, int]:
+    """(matrices, rows of each) of a 4-bit bank [..., N, row_bytes(columns)]."""
+    if not isinstance(bank, torch.Tensor) or bank.dim() < 2:
+        raise ValueError(f"{name} must be a bank [..., N, bytes of a row]")
+    shape = bank.shape
+    if not _fits(bank, torch.uint8, shape, here):
+        _refuse(bank, name, torch.uint8)
+    if shape[-1] != mxfp4.row_bytes(columns):
+        raise ValueError(f"{name} rows of {shape[-1]} bytes do not hold {columns} columns in 4 bits")
+    n = 1
+    for d in shape[:-2]:
+        n *= d
+    return n, shape[-2]
+
+
+def quantize_mx4(w: torch.Tensor, bank: torch.Tensor | None = None, *, gate_up: bool = False, stream=None) -> torch.Tensor:
+    """Weights w [..., N, K], bf16 or f32, as the 4-bit bank that holds them, uint8
+    [..., N, mxfp4.row_bytes(K)]: mxfp4.quantize and pack_w2 (gate_up: pack_w13) in one
+    pass.  N a multiple of 16 (64 with gate_up), K of 32."""
+    lib = load_library()
+    if not isinstance(w, torch.Tensor) or w.dim() < 2 or w.dtype not in _BF16_OR_F32:
+        raise ValueError("w must be bf16 or f32 weights [..., N, K]")
+    here = _device_index()
+    shape, dtype = w.shape, w.dtype
+    if not _fits(w, dtype, shape, here):
+        _refuse(w, "w", dtype)
+    N, K = shape[-2:]
+    wide = mxfp4.row_bytes(K)
+    if bank is None:
+        bank = _new((*shape[:-1], wide), torch.uint8, w.device, stream)
+    E, _ = _bank_rows(bank, "bank", K, here)
+    if bank.shape[:-1] != shape[:-1]:
+        raise ValueError(f"bank {tuple(bank.shape)} is not of weights {tuple(shape)}")
+    status = lib.lmoe_mx4_quantize(w.data_ptr(), dtype is torch.float32, E, N, K, bool(gate_up), bank.data_ptr(),
+                                   _stream(stream))
+    if status:
+        _refuse_overlap(status, min(N, K))
+        _check(status, "lmoe_mx4_quantize")
+    return bank
+
+
+def mx4_values(mx4, out: torch.Tensor | None = None, *, columns: int | None = None, gate_up: bool = False,
+               stream=None) -> torch.Tensor:
+    """The values that 4-bit rows (Mx4Rows) or a 4-bit bank (uint8 [..., N, bytes of a
+    row]; gate_up: of quantize_mx4's or pack_w13's) stand for, into out (bf16 or f32, bf16
+    where none is given).  A bank without out needs its columns: rows that end within 128
+    of them have the same bytes."""
+    lib = load_library()
+    here = _device_index()
+    rows = isinstance(mx4, Mx4Rows)
+    if out is not None and (not isinstance(out, torch.Tensor) or out.dtype not in _BF16_OR_F32 or out.dim() < 2):
+        raise ValueError("out must be a bf16 or f32 tensor")
+    if rows:
+        shape = mx4.shape
+        if columns not in (None, shape[-1]) or gate_up:
+            raise ValueError("columns and gate_up are for banks")
+    else:
+        if columns is None:
+            if out is None:
+                raise ValueError("the values of a bank need out or columns")
+            columns = out.shape[-1]
+        E, N = _bank_rows(mx4, "bank", columns, here)
+        shape = (*mx4.shape[:-1], columns)
+    if out is None:
+        out = _new(shape, torch.bfloat16, mx4.device, stream)
+    dtype = out.dtype
+    if not _fits(out, dtype, shape, here):
+        _refuse(out, "out", dtype, tuple(shape))
+    f32 = dtype is torch.float32
+    if rows:
+        q, scale = _take_mx4(mx4, "mx4", shape, here)
+        status = lib.lmoe_mx4_rows_values(q.data_ptr(), scale.data_ptr(), shape[0], shape[1], out.data_ptr(), f32,
+                                          _stream(stream))
+    else:
+        status = lib.lmoe_mx4_bank_values(mx4.data_ptr(), E, N, columns, bool(gate_up), out.data_ptr(), f32,
+                                          _stream(stream))
+    if status:
+        _refuse_overlap(status, shape[-1])
+        _check(status, "lmoe_mx4_rows_values" if rows else "lmoe_mx4_bank_values")
+    return out
+
+
+def mx4_linear(x, w: torch.Tensor, out: torch.Tensor | None = None, *, bias: torch.Tensor | None = None,
+               add: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """out = x W^T (+ bias) (+ add) over one matrix of 4-bit weights w [N, row_bytes(K)]
+    (quantize_mx4, mxfp4.pack_w2): an attention's projections, a dense block, the head.
+
+    x [T, K] is bf16, Mx8Rows or Mx4Rows; out [T, N] bf16 (made where none is given) or
+    f32; bias [N] bf16 or f32; add [T, N] bf16, which out may be.  Sums in f32, one
+    rounding."""
+    lib = load_library()
+    bf16, f32 = torch.bfloat16, torch.float32
+    here = _device_index()
+    if isinstance(x, Mx4Rows):
+        T, K = shape = x.shape
+        (xq, xs), rows = _take_mx4(x, "x", shape, here), 2
+    elif isinstance(x, Mx8Rows):
+        T, K = shape = x.shape
+        (xq, xs), rows = _take_mx8(x, "x", shape, here), 1
+    else:
+        if not isinstance(x, torch.Tensor) or x.dim() != 2:
+            raise ValueError("x must be rows [T, K]: bf16, Mx8Rows or Mx4Rows")
+        T, K = shape = x.shape
+        xq, xs, rows = x, None, 0
+        if not _fits(x, bf16, shape, here):
+            _refuse(x, "x", bf16)
+    if not isinstance(w, torch.Tensor) or w.dim() != 2:
+        raise ValueError("w must be one matrix in 4 bits, [N, bytes of a row]")
+    _, N = _bank_rows(w, "w", K, here)
+    if out is None:
+        out = _new((T, N), bf16, xq.device, stream)
+    odt = f32 if out.dtype is f32 else bf16
+    if not _fits(out, odt, (T, N), here):
+        _refuse(out, "out", odt, (T, N))
+    pb = pa = None
+    bdt = bf16
+    if bias is not None:
+        bdt = f32 if bias.dtype is f32 else bf16
+        if not _fits(bias, bdt, (N,), here):
+            _refuse(bias, "bias", bdt, (N,))
+        pb = bias.data_ptr()
+    if add is not None:
+        if not _fits(add, bf16, (T, N), here):
+            _refuse(add, "add", bf16, (T, N))
+        pa = add.data_ptr()
+    status = lib.lmoe_mx4_linear(xq.data_ptr(), None if xs is None else xs.data_ptr(), rows, T, K, N, w.data_ptr(), pb,
+                                 bdt is f32, pa, out.data_ptr(), odt is f32, _stream(stream))
+    if status:
+        if status == LMOE_ERR_ARG and T > 0:
+            raise ValueError("operands overlap: out over an operand other than a bf16 add")
+        _check(status, "lmoe_mx4_linear")
+    return out
 
 
 # ---------------------------------------------------------------------------
@@ -974,6 +1232,7 @@ def prefill_block_m(n_experts: int, hidden: int, intermediate: int, device="cuda
 
 
 MX4_BLOCK_M = (32, 64, 128)  # row-tile heights of the 4-bit experts' prefill kernel
+MX4_ROWS_BLOCK_M = ()  # and of its form for 4-bit rows
 # Up to this many pairs per expert the split-K kernel, row tiles past it: bf16 rows, 8-bit
 # rows.  Time of the captured layer, split-K over 32-row tiles (H, I, experts, top k):
 #   pairs per expert     3           4           6           8
@@ -995,10 +1254,12 @@ MX4_FEW_PAIRS_PER_EXPERT_MX8 = 6
 MX4_MAX_COLUMNS_MX8 = {32: 147200, 64: 73600, 128: 32640}
 
 
-def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False, columns: int = 0) -> int:
+def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False, columns: int = 0, *, mx4: bool = False) -> int:
     """The path of a layer of 4-bit experts, for every pass of it: the split-K
-    kernel for few pairs per expert (mx8: of 8-bit rows) and for 8-bit rows too
-    long for any row tile (columns: the longer of x's and act's), row tiles past that."""
+    kernel for few pairs per expert (mx8, mx4: of 8-bit, 4-bit rows) and for 8-bit rows
+    too long for any row tile (columns: the longer of x's and act's), row tiles past that."""
+    if mx4:
+        return LMOE_PATH_GEMV
     few = MX4_FEW_PAIRS_PER_EXPERT_MX8 if mx8 else MX4_FEW_PAIRS_PER_EXPERT
     if n_pairs <= few * n_experts or (mx8 and columns > MX4_MAX_COLUMNS_MX8[MX4_BLOCK_M[0]]):
         return LMOE_PATH_GEMV
@@ -1230,8 +1491,8 @@ def grouped_mlp(
     """y[pair] = W2_s . (silu(W13_s[:I] x) * W13_s[I:] x) for the placed pairs.
     pass_pairs: how many of the pairs the pass is expected to place, where it
     is one wave of its layer (chooses the kernel's form, not its bits).
-    4-bit banks (mxfp4.pack_experts; uint8): x and act are both bf16 or both
-    Mx8Rows, y is bf16 or f32, perm is built with block_m=mx4_block_m(..) (where
+    4-bit banks (mxfp4.pack_experts; uint8): x and act are both bf16, both
+    Mx8Rows or both Mx4Rows, y is bf16 or f32, perm is built with block_m=mx4_block_m(..) (where
     row tiles run, another height is refused).  On path LMOE_PATH_GEMV (which AUTO then is) a
     bf16 act may be [N, 2, I]: rows in two parts whose sum is the value, so that
     its rounding does not show in batches of few tokens."""
@@ -1325,9 +1586,12 @@ def _need_mx4(bank: torch.Tensor, name: str, perm: Permutation, K: int, rows: in
 
 
 def _need_rows(rows, name: str, shape: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """bf16 rows or Mx8Rows, [R, K]: (values, scales or None)."""
+    """bf16 rows, Mx8Rows or Mx4Rows, [R, K]: (values, scales or None)."""
     if isinstance(rows, Mx8Rows):
         _need_mx8(rows, name, shape)
+        return rows.q, rows.scale
+    if isinstance(rows, Mx4Rows):
+        _need_mx4_rows(rows, name, shape)
         return rows.q, rows.scale
     if shape is None or not _is(rows, torch.bfloat16, shape):
         _need(rows, name, torch.bfloat16, shape)
@@ -1338,7 +1602,7 @@ def _need_rows(rows, name: str, shape: tuple | None = None) -> tuple[torch.Tenso
 
 def _need_act(act, n: int) -> tuple[torch.Tensor, torch.Tensor | None, bool]:
     """act rows of n pairs: (values, scales or None, bf16 in two parts)."""
-    split = not isinstance(act, Mx8Rows) and act.dim() == 3
+    split = isinstance(act, torch.Tensor) and act.dim() == 3
     if not split:
         return *_need_rows(act, "act", (n, act.shape[-1])), False
     if not _is(act, torch.bfloat16, (n, 2, act.shape[-1])):
@@ -1355,6 +1619,16 @@ def _need_y(y, shape: tuple) -> bool:
     return y.dtype is torch.float32
 
 
+def _need_alike(x, act) -> None:
+    if not _alike(x, act):
+        raise ValueError("x and act must both be bf16, both be Mx8Rows or both be Mx4Rows")
+
+
+def _alike(x, act) -> bool:
+    """Whether rows are held the same way."""
+    return type(x) is type(act) or not isinstance(x, (Mx8Rows, Mx4Rows)) and not isinstance(act, (Mx8Rows, Mx4Rows))
+
+
 def _check_products(status: int, fn: str, perm: Permutation) -> None:
     if status == LMOE_ERR_SHAPE and perm.block_m not in MX4_BLOCK_M:
         raise ValueError(f"{fn}: unsupported shape; the permutation was built with block_m {perm.block_m}, row tiles "
@@ -1364,19 +1638,19 @@ def _check_products(status: int, fn: str, perm: Permutation) -> None:
 
 def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, act, *, path: int, stream):
     xq, xs = _need_rows(x, "x", tuple(x.shape))
-    T, H = xq.shape
+    T, H = x.shape
     n = perm.n_pairs
     if n != T * top_k:
         raise ValueError("permutation does not match T * top_k pairs")
     aq, as_, split = _need_act(act, n)
-    I = aq.shape[-1]
-    if (xs is None) != (as_ is None):
-        raise ValueError("x and act must both be bf16 or both be Mx8Rows")
+    I = act.shape[-1]
+    _need_alike(x, act)
     _need_mx4(w13_slots, "w13_slots", perm, H, 2 * I)
     _same_device(xq, xs, w13_slots, perm.offsets, aq, as_)
     p = perm
+    lib = load_library()
     _check_products(
-        load_library().lmoe_mx4_gateup_silu(
+        (lib.lmoe_mx44_gateup_silu if isinstance(x, Mx4Rows) else lib.lmoe_mx4_gateup_silu)(
             xq.data_ptr(), _ptr(xs), T, H, I, top_k, w13_slots.data_ptr(), p.n_slots, p.offsets.data_ptr(),
             p.sorted_pairs.data_ptr(), p.active.data_ptr(), p.tile_off.data_ptr(), p.meta.data_ptr(), n, p.block_m, path,
             aq.data_ptr(), _ptr(as_), split, _stream(stream),
@@ -1389,13 +1663,14 @@ def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, 
 def _mx4_down(act, w2_slots: torch.Tensor, perm: Permutation, y: torch.Tensor, *, path: int, stream):
     n = perm.n_pairs
     aq, as_, split = _need_act(act, n)
-    I = aq.shape[-1]
+    I = act.shape[-1]
     H = _need_mx4(w2_slots, "w2_slots", perm, I, w2_slots.shape[1] if w2_slots.dim() == 3 else None)
     y_f32 = _need_y(y, (n, H))
     _same_device(aq, as_, w2_slots, perm.offsets, y)
     p = perm
+    lib = load_library()
     _check_products(
-        load_library().lmoe_mx4_down(
+        (lib.lmoe_mx44_down if isinstance(act, Mx4Rows) else lib.lmoe_mx4_down)(
             aq.data_ptr(), _ptr(as_), split, H, I, w2_slots.data_ptr(), p.n_slots, p.offsets.data_ptr(),
             p.sorted_pairs.data_ptr(), p.active.data_ptr(), p.tile_off.data_ptr(), p.meta.data_ptr(), n, p.block_m, path,
             y.data_ptr(), y_f32, _stream(stream),
@@ -1416,7 +1691,7 @@ class _Mx4Workspace(ctypes.Structure):
 
 class Mx4Buffers:
     """The buffers of a layer of 4-bit experts (lmoe_mx4_workspace): a permutation,
-    act (bf16 or Mx8Rows, [N, I]; bf16 [N, 2, I]: rows in two parts, where the
+    act (bf16, Mx8Rows or Mx4Rows, [N, I]; bf16 [N, 2, I]: rows in two parts, where the
     split-K kernel runs) and y (bf16 or f32, [N, H]), checked once."""
 
     def __init__(self, perm: Permutation, act, y: torch.Tensor) -> None:
@@ -1434,8 +1709,8 @@ class Mx4Buffers:
                   perm.meta, perm.workspace):
             if t is not None and t.get_device() != self.device_index:
                 raise ValueError(f"a buffer on {t.device}, y on {y.device}")
-        self.hidden, self.intermediate = int(y.shape[1]), int(aq.shape[-1])
-        self.mx8 = as_ is not None
+        self.hidden, self.intermediate = int(y.shape[1]), int(act.shape[-1])
+        self.mx8, self.mx4 = isinstance(act, Mx8Rows), isinstance(act, Mx4Rows)
         H, I, P = self.hidden, self.intermediate, perm.n_slots
         self.w13_shape, self.w2_shape = (P, 2 * I, mxfp4.row_bytes(H)), (P, H, mxfp4.row_bytes(I))
         self.act_ptr, self.act_scale_ptr = _ptr(aq), _ptr(as_)
@@ -1456,15 +1731,17 @@ def _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, buf
     pairs = topk_ids.shape
     T, k = pairs
     rows = (T, bufs.hidden)
-    mx8 = isinstance(x, Mx8Rows)
+    mx8, mx4 = isinstance(x, Mx8Rows), isinstance(x, Mx4Rows)
     if mx8:
         xq, xs = _take_mx8(x, "x", rows, here)
+    elif mx4:
+        xq, xs = _take_mx4(x, "x", rows, here)
     else:
         xq, xs = x, None
         if not _fits(x, bf16, rows, here):
             _refuse(x, "x", bf16, rows)
-    if mx8 != bufs.mx8:
-        raise ValueError("x and act must both be bf16 or both be Mx8Rows")
+    if mx8 is not bufs.mx8 or mx4 is not bufs.mx4:
+        _need_alike(x, bufs.act)
     if T * k != bufs.perm.n_pairs:
         raise ValueError(f"buffers for {bufs.perm.n_pairs} pairs, got {T * k}")
     if not _fits(topk_weights, bf16, pairs, here):
@@ -1494,7 +1771,7 @@ def mx4_fused_moe(x, topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_slo
     lib = load_library()
     xq, xs, T, k, n_table = _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, bufs, out, add)
     _check(
-        lib.lmoe_mx4_fused_moe(
+        (lib.lmoe_mx44_fused_moe if bufs.mx4 else lib.lmoe_mx4_fused_moe)(
             xq.data_ptr(), _ptr(xs), T, bufs.hidden, bufs.intermediate, k, w13_slots.data_ptr(), w2_slots.data_ptr(),
             bufs.perm.n_slots, topk_weights.data_ptr(), topk_ids.data_ptr(), _ptr(log2phy), n_table, path, block_m,
             bufs.address, _ptr(add), out.data_ptr(), _stream(stream),
@@ -1526,7 +1803,7 @@ def mx4_decode_few(x, topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_sl
     if bufs.y.dtype is not torch.float32 or (xs is None and not bufs.split):
         raise ValueError("few tokens' y rows are f32, their bf16 act rows in two parts, [N, 2, I]")
     _check(
-        lib.lmoe_mx4_decode_few(
+        (lib.lmoe_mx44_decode_few if bufs.mx4 else lib.lmoe_mx4_decode_few)(
             xq.data_ptr(), _ptr(xs), T, bufs.hidden, bufs.intermediate, k, w13_slots.data_ptr(), w2_slots.data_ptr(),
             bufs.perm.n_slots, topk_weights.data_ptr(), topk_ids.data_ptr(), _ptr(log2phy), n_table, _ptr(add),
             bufs.act_ptr, bufs.act_scale_ptr, bufs.y.data_ptr(), out.data_ptr(), _stream(stream),
@@ -1563,7 +1840,7 @@ def mx4_decode_one(x, topk_weights: torch.Tensor, topk_ids: torch.Tensor, w13_sl
         _need(tab, "second log2phy", torch.int32)
         _same_device(b13, b2, tab)
     _check(
-        lib.lmoe_mx4_decode_one(
+        (lib.lmoe_mx44_decode_one if bufs.mx4 else lib.lmoe_mx4_decode_one)(
             xq.data_ptr(), _ptr(xs), bufs.hidden, bufs.intermediate, k, w13_slots.data_ptr(), w2_slots.data_ptr(),
             bufs.perm.n_slots, topk_weights.data_ptr(), topk_ids.data_ptr(), _ptr(log2phy), n_table,
             _ptr(b13), _ptr(b2), n_slots_b, _ptr(tab), n_table_b, _ptr(add), bufs.act_ptr, bufs.act_scale_ptr, out.data_ptr(), _stream(stream),
