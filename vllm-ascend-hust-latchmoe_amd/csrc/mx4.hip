@@ -5,6 +5,7 @@
 
 #include "gemm_lds.h"
 #include "mx4_few.h"
+#include "mx44_tile.h"
 #include "mx4_tile.h"
 #include "spans.h"
 
@@ -104,7 +105,9 @@ static int launch_tiles(const Mx4Args& g, hipStream_t stream) {
   return launch_tiles<GU, A8, BM, 1>(g, static_cast<unsigned>(grid), stream);
 }
 
-static bool known_block_m(int bm) { return bm == 32 || bm == 64 || bm == 128; }
+static bool known_block_m(int bm, int rows) {
+  return bm == 32 || bm == 64 || bm == 128 || (bm == 256 && rows == kRowsMx4);
+}
 
 // Whether rows of K columns fit the LDS of tiles of block_m rows (MX8 rows: their scales).
 static bool tiles_fit(int block_m, int rows, int K) {
@@ -124,6 +127,16 @@ static int launch_tiles(const Mx4Args& g, int block_m, hipStream_t stream) {
   return launch_tiles<GU, A8, 128>(g, stream);
 }
 
+template <bool GU>
+static int launch_tiles4(const Mx4Args& g, int block_m, hipStream_t stream) {
+  constexpr Op op = GU ? Op::kGateUp : Op::kDown;
+  const long long tiles = g.n_pairs / block_m + (g.n_pairs < g.P ? g.n_pairs : g.P);
+  if (block_m == 32) return launch_mx44<op, Mx44Tile32>(g, LinearArgs{}, tiles, stream);
+  if (block_m == 64) return launch_mx44<op, Mx44Tile64>(g, LinearArgs{}, tiles, stream);
+  if (block_m == 128) return launch_mx44<op, Mx44Tile128>(g, LinearArgs{}, tiles, stream);
+  return launch_mx44<op, Mx44Tile256>(g, LinearArgs{}, tiles, stream);
+}
+
 // path AUTO: row tiles past this many pairs per slot, on average, of bf16, MX8 and MX4 rows
 // (native.py has the figures)
 constexpr int kFewPairsPerSlot[3] = {4, 6, 6};
@@ -132,7 +145,7 @@ static bool many_pairs(int rows, int n_pairs, int P) { return n_pairs > static_c
 
 static bool takes_tiles(int path, int block_m, int rows, int H, int I, int n_pairs, int P, bool split) {
   if (path != LMOE_PATH_AUTO) return path == LMOE_PATH_MFMA;
-  return !split && known_block_m(block_m) && many_pairs(rows, n_pairs, P) && tiles_fit(block_m, rows, H) &&
+  return !split && known_block_m(block_m, rows) && many_pairs(rows, n_pairs, P) && tiles_fit(block_m, rows, H) &&
          tiles_fit(block_m, rows, I);
 }
 
@@ -140,7 +153,7 @@ static bool takes_tiles(int path, int block_m, int rows, int H, int I, int n_pai
 // an error where row tiles are due, as with an explicit path.  The split-K kernel is
 // right for any number of rows, but reads the weights once for every 32 of them.
 static bool lacks_height(int path, int block_m, int rows, int n_pairs, int P, bool split) {
-  return path == LMOE_PATH_AUTO && !split && !known_block_m(block_m) && many_pairs(rows, n_pairs, P);
+  return path == LMOE_PATH_AUTO && !split && !known_block_m(block_m, rows) && many_pairs(rows, n_pairs, P);
 }
 
 template <bool GU>
@@ -150,10 +163,10 @@ static int launch(const Mx4Args& g, int path, int block_m, hipStream_t stream) {
     launch_few<GU, false>(g, TokenIds{}, stream);
   } else {
     if (g.split) return LMOE_ERR_UNSUPPORTED;
-    if (!known_block_m(block_m) || !tiles_fit(block_m, g.rows, g.K)) return LMOE_ERR_SHAPE;
-    if (g.rows == kRowsMx4) return LMOE_ERR_UNSUPPORTED;
-    const int st = g.rows == kRowsMx8 ? launch_tiles<GU, true>(g, block_m, stream)
-                                      : launch_tiles<GU, false>(g, block_m, stream);
+    if (!known_block_m(block_m, g.rows) || !tiles_fit(block_m, g.rows, g.K)) return LMOE_ERR_SHAPE;
+    const int st = g.rows == kRowsMx4   ? launch_tiles4<GU>(g, block_m, stream)
+                   : g.rows == kRowsMx8 ? launch_tiles<GU, true>(g, block_m, stream)
+                                        : launch_tiles<GU, false>(g, block_m, stream);
     if (st != LMOE_OK) return st;
   }
   LMOE_RETURN_LAUNCH();
@@ -253,7 +266,7 @@ static int fused_moe(int rows, const void* x, const void* x_scale, int T, int H,
     if (misaligned16(x) || misaligned16(w13_slots) || misaligned16(w2_slots) || misaligned16(ws->act) ||
         misaligned16(ws->y) || misaligned16(add) || misaligned16(out))
       return LMOE_ERR_SHAPE;
-    if (path == LMOE_PATH_MFMA && (!known_block_m(block_m) || !tiles_fit(block_m, rows, H) ||
+    if (path == LMOE_PATH_MFMA && (!known_block_m(block_m, rows) || !tiles_fit(block_m, rows, H) ||
                                    !tiles_fit(block_m, rows, I)))
       return LMOE_ERR_SHAPE;
     if (lacks_height(path, block_m, rows, static_cast<int>(n), n_slots, false)) return LMOE_ERR_SHAPE;

@@ -1,0 +1,388 @@
+// Products of 4-bit rows with 4-bit weights in row tiles.
+//
+// A workgroup of four waves computes BM rows by 256 weight rows: gate-up 128 act columns
+// (gate and up), down 256 y columns, the plain product 256 columns.  Each wave takes all BM
+// rows and 64 weight rows (four 16-row blocks; gate-up: gate, up, gate, up of 32 act
+// columns).  A stage is 256 columns: 128 bytes of a row, which go to LDS without passing
+// through registers (two buffers, the next stage in flight under this one's products) and
+// are read there by all four waves; weights go from memory straight to registers, one stage
+// ahead, since the bank's order is the fragments' order and no two waves share any.
+//
+// LDS holds 16-byte piece p of row r at position p ^ (r / 2) % 8, which puts the sixteen
+// lanes of a read on sixteen different positions (mx4_tile.h).  A quad is two stages: its
+// scales are one dword for a lane's row and group on either side (byte c: chunk c), so the
+// matrix instruction picks its bytes without any arithmetic.  The weights' scales lie that
+// way in the bank; the rows' are transposed on their way to LDS, a quad ahead.
+//
+// Every output adds its chunks in order, whatever BM is: the same bits.
+#pragma once
+
+#include "mx4_linear.h"
+#include "mx4_tile.h"
+
+namespace lmoe {
+
+enum class Op { kGateUp, kDown, kLinear };
+
+// n scales of a row from `at` on, from any address; past the row's groups, ones.
+template <class T>
+__device__ __forceinline__ T load_scales(const uint8_t* sp, int at, int groups) {
+  T v;
+  if (at + static_cast<int>(sizeof(T)) <= groups) {
+    __builtin_memcpy(&v, sp + at, sizeof(T));
+  } else {
+    v = 0;
+    for (int e = 0; e < static_cast<int>(sizeof(T)); ++e)
+      v |= static_cast<T>(at + e < groups ? sp[at + e] : kScaleOne) << (8 * e);
+  }
+  return v;
+}
+
+// W x^T of one chunk; B: the byte of both scales.
+template <int B>
+__device__ __forceinline__ f32x4_t mx44_step(const i32x4_t w, int ws, const i32x4_t x, int xs, f32x4_t acc) {
+  const i32x8_t a = __builtin_shufflevector(w, w, 0, 1, 2, 3, 0, 1, 2, 3);
+  const i32x8_t b = __builtin_shufflevector(x, x, 0, 1, 2, 3, 0, 1, 2, 3);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4 /* e2m1 */, 4, B, ws, B, xs);
+}
+
+// 32 columns of a row from n on, this lane's: n + 4 g.. (lo) and n + 16 + 4 g.. (hi); hi's
+// may be past the matrix.
+__device__ __forceinline__ f32x4_t linear_terms(const LinearArgs& l, int row, int n, bool live, f32x4_t v) {
+  if (!live) return v;
+  if (l.bias != nullptr) {
+    if (l.bias_f32) {
+      v += *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(l.bias) + n);
+    } else {
+      const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(l.bias) + n);
+      v += f32x4_t{bf16lo(b.x), bf16hi(b.x), bf16lo(b.y), bf16hi(b.y)};
+    }
+  }
+  if (l.add != nullptr) {
+    const uint2 a = *reinterpret_cast<const uint2*>(l.add + static_cast<size_t>(row) * l.N + n);
+    v += f32x4_t{bf16lo(a.x), bf16hi(a.x), bf16lo(a.y), bf16hi(a.y)};
+  }
+  return v;
+}
+__device__ __forceinline__ void store_linear(const LinearArgs& l, int row, int n, int lane, bool live, f32x4_t lo, f32x4_t hi) {
+  const int col = n + 4 * (lane >> 4);
+  if (n + 32 > l.N) {  // the last block alone
+    if (live) store_linear4(l, row, col, lo);
+    return;
+  }
+  lo = linear_terms(l, row, col, live, lo);
+  hi = linear_terms(l, row, col + 16, live, hi);
+  const size_t at = static_cast<size_t>(row) * l.N + n;
+  if (l.out_f32) {
+    if (live) {
+      float* p = static_cast<float*>(l.out) + at + 4 * (lane >> 4);
+      *reinterpret_cast<f32x4_t*>(p) = lo;
+      *reinterpret_cast<f32x4_t*>(p + 16) = hi;
+    }
+  } else {
+    store_bf16x8(static_cast<uint16_t*>(l.out) + at, lane, live, lo, hi);
+  }
+}
+
+// A workgroup's shape: WR x WC waves of MI x NJ fragments of 16 rows by 16 weight rows, NB
+// chunks of both operands in LDS.
+template <int MI_, int NJ_, int WR_, int WC_, int NB_>
+struct Mx44Shape {
+  static constexpr int MI = MI_, NJ = NJ_, WR = WR_, WC = WC_, NB = NB_;
+  static constexpr int BM = 16 * MI * WR, BN = 16 * NJ * WC;
+  static constexpr int WAVES = WR * WC, THREADS = 64 * WAVES;
+  static constexpr int QA = BM / 16 / WAVES > 0 ? BM / 16 / WAVES : 1;  // load instructions of a wave and chunk: rows
+  static constexpr int QB = BN / 16 / WAVES;                            // and weights
+  static constexpr int A_WAVES = BM / 16 / QA;                          // waves that load rows
+  static constexpr int PART_A = BM * 64, PART_B = BN * 64, STAGE = PART_A + PART_B;
+  static constexpr int OFF_SCALE = NB * STAGE;           // a quad's scales: BM x 16 bytes of rows,
+  static constexpr int OFF_WSCALE = OFF_SCALE + BM * 16;  // BN / 16 blocks of 256 of weights
+  static constexpr int OFF_PAIR = OFF_WSCALE + BN * 16;
+  static constexpr int LDS = OFF_PAIR + BM * 4;
+  static constexpr int PER_ROW = THREADS / BM;  // threads that bring a row's scales of a quad
+  using scales_t = std::conditional_t<PER_ROW == 2, uint64_t, std::conditional_t<PER_ROW == 4, uint32_t, uint16_t>>;
+  static_assert(PER_ROW * sizeof(scales_t) == 16);
+  static_assert(LDS <= 160 * 1024 && BM <= THREADS && QB * 16 * WAVES == BN && A_WAVES * QA * 16 == BM);
+  // 16-byte piece p (of four) of row r lies at position p ^ sw(r)
+  static __device__ __forceinline__ int sw(int r) { return (0x78 >> (2 * ((r >> 2) & 3))) & 3; }
+};
+
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+// 16 (4) bytes a lane from base + lane_at + at to LDS, 1 KiB (256 bytes) from dst on,
+// without passing through registers.  Off: the load is out of range and fetches nothing (its
+// address is that of the first chunk or quad, inside the operand either way).
+__device__ __forceinline__ void buffer_to_lds16(const uint8_t* base, bool on, char* dst, uint32_t lane_at, int at) {
+  const int range = __builtin_amdgcn_readfirstlane(on ? -1 : 0);
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, range, 0x00027000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 16, lane_at, __builtin_amdgcn_readfirstlane(on ? at : 0), 0, 0);
+}
+__device__ __forceinline__ void buffer_to_lds4(const uint8_t* base, bool on, char* dst, uint32_t lane_at, int at) {
+  const int range = __builtin_amdgcn_readfirstlane(on ? -1 : 0);
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, range, 0x00027000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 4, lane_at, __builtin_amdgcn_readfirstlane(on ? at : 0), 0, 0);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vm_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// g: the experts' arguments, l: the plain product's (the other is not read)
+template <Op OP, class C>
+__global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(Mx4Args g, LinearArgs l) {
+  constexpr bool GU = OP == Op::kGateUp, LIN = OP == Op::kLinear;
+  constexpr int BM = C::BM, MI = C::MI, NJ = C::NJ, NB = C::NB;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  int* s_pair = reinterpret_cast<int*>(smem + C::OFF_PAIR);
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave / C::WC, wc = wave - wr * C::WC;
+  const int K = LIN ? l.K : g.K, N = LIN ? l.N : g.N;
+
+  constexpr int OUT_COLS = GU ? C::BN / 2 : C::BN;
+  const int NT = (N + OUT_COLS - 1) / OUT_COLS;
+  SlotWindow win0, win1;
+  int total;
+  if constexpr (LIN) {
+    total = (l.T + BM - 1) / BM * NT;
+  } else {
+    win0 = load_window(g.tile_off, g.offsets, g.P, 0, lane);
+    win1 = load_window(g.tile_off, g.offsets, g.P, 64, lane);
+    total = g.meta[LMOE_META_TILES] * NT;
+  }
+  // work item: XCD-contiguous chunks of (row tile, column tile)
+  const int share = (total + 7) >> 3;
+  const int jj = blockIdx.x >> 3;
+  const int item = (blockIdx.x & 7) * share + jj;
+  if (jj >= share || item >= total) return;
+  const int tile = __builtin_amdgcn_readfirstlane(item / NT);
+  const int n0 = (item - tile * NT) * OUT_COLS;
+  int slot = 0, p0 = tile * BM, rows = BM;
+  if constexpr (LIN) {
+    rows = min(BM, l.T - p0);
+  } else {
+    const TileSlot ts = slot_of_tile(g.tile_off, g.offsets, g.P, tile, win0, win1, lane);
+    slot = ts.slot;
+    p0 = ts.p0 + (tile - ts.tile0) * BM;
+    rows = min(BM, ts.p1 - p0);
+  }
+  const int chunks = mx4_chunks(K);
+  const int groups = K / kMxGroup;
+  const uint8_t* scale_base = LIN ? l.x_scale : g.a_scale;
+  auto source_row = [&](int r) -> int {  // of the tile's row r; rows past the last repeat the first
+    const int pos = r < rows ? r : 0;
+    return GU ? g.sorted_pairs[p0 + pos] / g.topk : pos;
+  };
+  // rows: gate-up's lie anywhere, the others' from the tile's first on
+  const size_t row0 = GU ? 0 : p0;
+  const uint8_t* rows_base = uniform(static_cast<const uint8_t*>(LIN ? l.x : g.a) + row_bytes<kRowsMx4>(row0, K));
+  uint32_t a_off[C::QA], a_piece[C::QA];
+#pragma unroll
+  for (int q = 0; q < C::QA; ++q) {
+    const int r = (wave * C::QA + q) * 16 + lane / 4;
+    a_piece[q] = (lane & 3) ^ C::sw(r);
+    a_off[q] = static_cast<uint32_t>(source_row(r < BM ? r : 0)) * (K >> 1) + a_piece[q] * 16;
+  }
+  const uint32_t tail = K - (chunks - 1) * kMxChunk;  // columns of the last chunk
+  // weight blocks; those past the matrix repeat the last one
+  const int wblocks = (GU ? 2 * N : N) / 16;
+  const int b0 = (GU ? 2 * n0 : n0) / 16;
+  const int bb = mx4_block_bytes(K);
+  const uint8_t* wbase = uniform((LIN ? l.w : g.w + slot * g.w_slot_bytes) + static_cast<size_t>(b0) * bb);
+  const int last_block = wblocks - 1 - b0;
+  // chunk c to buffer buf; past the last chunk the same loads, out of range: they fetch
+  // nothing, and what they leave there is not read
+  auto issue = [&](int c, int buf) {
+    char* st = smem + buf * C::STAGE;
+    const bool on = c < chunks;
+    if (C::A_WAVES == C::WAVES || wave < C::A_WAVES) {
+#pragma unroll
+      for (int q = 0; q < C::QA; ++q) {
+        // past the row's end any codes do: the weights' are zeros there
+        const uint32_t back = c + 1 >= chunks && a_piece[q] * 32 >= tail ? a_piece[q] * 16 : 0;
+        buffer_to_lds16(rows_base, on, st + (wave * C::QA + q) * 1024, a_off[q] - back, c * 64);
+      }
+    }
+    const int at = (c >> 2) * kMxQuadBytes + 256 + (c & 3) * 1024;
+#pragma unroll
+    for (int q = 0; q < C::QB; ++q) {
+      const int b = wave * C::QB + q;
+      buffer_to_lds16(wbase, on, st + C::PART_A + b * 1024, lane * 16, min(b, last_block) * bb + at);
+    }
+  };
+  constexpr int LOADS = C::QB + (C::A_WAVES == C::WAVES ? C::QA : 0);  // of a wave and chunk, at least
+
+  const int first = wc * NJ;  // this wave's weight blocks, from b0
+  const bool wave_live = first <= last_block;
+  const int quads = (chunks + 3) >> 2;
+  auto issue_ws = [&](int quad) {  // the weights' scales of a quad
+#pragma unroll
+    for (int q = 0; q < C::QB; ++q) {
+      const int b = wave * C::QB + q;
+      buffer_to_lds4(wbase, quad < quads, smem + C::OFF_WSCALE + b * 256, lane * 4,
+                     min(b, last_block) * bb + quad * kMxQuadBytes);
+    }
+  };
+  // the rows' scales of a quad, as they lie: PER_ROW threads to a row
+  constexpr int SB = sizeof(typename C::scales_t);
+  const uint8_t* my_scales = scale_base + (row0 + source_row(tid / C::PER_ROW)) * groups;
+  typename C::scales_t qs;
+  auto get_scales = [&](int quad) { qs = load_scales<typename C::scales_t>(my_scales, 16 * quad + tid % C::PER_ROW * SB, groups); };
+  auto put_scales = [&]() { *reinterpret_cast<typename C::scales_t*>(smem + C::OFF_SCALE + tid * SB) = qs; };
+
+  get_scales(0);
+  issue_ws(0);
+  if constexpr (!LIN)
+    if (tid < BM) s_pair[tid] = g.sorted_pairs[p0 + (tid < rows ? tid : 0)];
+#pragma unroll
+  for (int c = 0; c < NB - 1; ++c) issue(c, c);
+  put_scales();
+
+  f32x4_t acc[MI][NJ];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const int fr = lane & 15;
+  const int wrow = wr * 16 * MI;  // this wave's first row
+  const int live = min(MI, max(0, (rows - wrow + 15) >> 4));
+  // this lane's bytes of a fragment: rows from wrow on, weights from block `first` on
+  const char* x_at = smem + (wrow + fr) * 64 + ((lg ^ C::sw(fr)) * 16);
+  const char* w_at = smem + C::PART_A + first * 1024 + lane * 16;
+  const char* s_at = smem + C::OFF_SCALE + (wrow + fr) * 16;
+  const char* ws_at = smem + C::OFF_WSCALE + first * 256 + lane * 4;
+  const uint32_t pick = 0x0400u + 0x0101u * lg;  // byte lg of two dwords
+
+  // NL: 16-row fragments computed, a compile-time count so that the products are
+  // straight-line code; rows past the tile's last are dropped at the store
+  auto main_loop = [&](auto nl_tag) {
+    constexpr int NL = decltype(nl_tag)::value;
+    int xs[NL > 0 ? NL : 1], ws[NJ];
+    int buf = 0;
+    // byte B of the scales: chunk c of its quad.  No branch: the products before the
+    // barrier would sink behind it
+    auto chunk = [&](int c, auto b_tag) {
+      constexpr int B = decltype(b_tag)::value;
+      const char* xp = x_at + buf * C::STAGE;
+      const char* wp = w_at + buf * C::STAGE;
+      const int before = buf == 0 ? NB - 1 : buf - 1;  // the buffer that chunk c - 1 had
+      // when every wave has got here chunk c + 1 is in LDS and chunk c - 1 read
+      auto turn = [&]() {
+        if constexpr (B == 2) {  // every wave has read this quad's scales
+          put_scales();
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        wait_vm_barrier<(NB - 3) * (LOADS + (B == 2 ? C::QB : 0))>();
+        issue(c + NB - 1, before);
+        if constexpr (B == 1) issue_ws((c >> 2) + 1);
+      };
+      if constexpr (NL > 0) {
+        i32x4_t w[NJ], x[3];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) w[j] = *reinterpret_cast<const i32x4_t*>(wp + j * 1024);
+        x[0] = *reinterpret_cast<const i32x4_t*>(xp);
+        if (NL > 1) x[1] = *reinterpret_cast<const i32x4_t*>(xp + 1024);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          if (i == NL / 2) turn();
+          if (i + 2 < NL) x[(i + 2) % 3] = *reinterpret_cast<const i32x4_t*>(xp + (i + 2) * 1024);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[i][j] = mx44_step<B>(w[j], ws[j], x[i % 3], xs[i], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        turn();
+      }
+      buf = buf + 1 == NB ? 0 : buf + 1;
+    };
+    auto begin_quad = [&](int quad) {
+      if constexpr (NL > 0) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) ws[j] = *reinterpret_cast<const int*>(ws_at + j * 256);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const i32x4_t v = *reinterpret_cast<const i32x4_t*>(s_at + i * 256);
+          const uint32_t lo = __builtin_amdgcn_perm(v[1], v[0], pick), hi = __builtin_amdgcn_perm(v[3], v[2], pick);
+          xs[i] = static_cast<int>(__builtin_amdgcn_perm(hi, lo, 0x05040100u));
+        }
+      }
+      if (quad + 1 < quads) get_scales(quad + 1);
+    };
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    wait_vm_barrier<0>();  // chunks 0 to NB - 2, and the scales
+    int quad = 0;
+    for (; quad < chunks >> 2; ++quad) {
+      begin_quad(quad);
+      chunk(4 * quad, std::integral_constant<int, 0>{});
+      chunk(4 * quad + 1, std::integral_constant<int, 1>{});
+      chunk(4 * quad + 2, std::integral_constant<int, 2>{});
+      chunk(4 * quad + 3, std::integral_constant<int, 3>{});
+    }
+    const int rest = chunks & 3;
+    if (rest > 0) {
+      begin_quad(quad);
+      chunk(4 * quad, std::integral_constant<int, 0>{});
+      if (rest > 1) chunk(4 * quad + 1, std::integral_constant<int, 1>{});
+      if (rest > 2) chunk(4 * quad + 2, std::integral_constant<int, 2>{});
+    }
+  };
+  if (!wave_live || live == 0) main_loop(std::integral_constant<int, 0>{});
+  else if (MI > 6 && live > 6) main_loop(std::integral_constant<int, MI>{});
+  else if (MI > 4 && live > 4) main_loop(std::integral_constant<int, MI < 6 ? MI : 6>{});
+  else if (MI > 2 && live > 2) main_loop(std::integral_constant<int, MI < 4 ? MI : 4>{});
+  else if (MI > 1 && live > 1) main_loop(std::integral_constant<int, MI < 2 ? MI : 2>{});
+  else main_loop(std::integral_constant<int, 1>{});
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load writes to LDS past the workgroup's end
+  if (!wave_live) return;
+
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int r = wrow + 16 * i + fr;
+    if (i >= live) break;
+#pragma unroll
+    for (int j = 0; j < NJ; j += GU ? 4 : 2) {
+      if (first + j > last_block) break;
+      if constexpr (GU) {
+        const f32x4_t gate[2] = {acc[i][j], acc[i][j + 2]}, up[2] = {acc[i][j + 1], acc[i][j + 3]};
+        store_act<kRowsMx4>(g, p0 + r, n0 + 8 * (first + j), lane, r < rows, gate, up);
+      } else if constexpr (LIN) {
+        store_linear(l, p0 + r, n0 + 16 * (first + j), lane, r < rows, acc[i][j], acc[i][j + 1]);
+      } else {
+        store_y(g, s_pair[r], n0 + 16 * (first + j), lane, r < rows, acc[i][j], acc[i][j + 1]);
+      }
+    }
+  }
+}
+
+using Mx44Tile32 = Mx44Shape<2, 4, 1, 4, 4>;
+using Mx44Tile64 = Mx44Shape<4, 4, 1, 4, 3>;
+using Mx44Tile128 = Mx44Shape<8, 4, 1, 4, 3>;
+using Mx44Tile256 = Mx44Shape<8, 4, 2, 4, 4>;
+
+// Row tiles over `tiles` of them at most.
+template <Op OP, class C>
+int launch_mx44(const Mx4Args& g, const LinearArgs& l, long long tiles, hipStream_t stream) {
+  constexpr int cols = OP == Op::kGateUp ? C::BN / 2 : C::BN;
+  const long long blocks = tiles * (((OP == Op::kLinear ? l.N : g.N) + cols - 1) / cols);
+  const long long grid = 8 * ((blocks + 7) / 8);
+  if (grid > 0x7fffffffLL) return LMOE_ERR_SHAPE;
+  static bool raised[64] = {};  // per device: dynamic LDS past 64 KiB allowed
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return static_cast<int>(e);
+  if (dev < 0 || dev >= 64 || !raised[dev]) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx44_tile_kernel<OP, C>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e != hipSuccess) return static_cast<int>(e);
+    if (dev >= 0 && dev < 64) raised[dev] = true;
+  }
+  mx44_tile_kernel<OP, C><<<static_cast<unsigned>(grid), C::THREADS, C::LDS, stream>>>(g, l);
+  LMOE_RETURN_LAUNCH();
+}
+
+}  // namespace lmoe

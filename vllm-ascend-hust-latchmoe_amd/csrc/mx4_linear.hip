@@ -1,6 +1,9 @@
 // Entry point of the product with one matrix of 4-bit weights.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
+#include "mx44_tile.h"
 #include "mx4_linear.h"
 #include "spans.h"
 
@@ -16,6 +19,11 @@ static int launch_linear_few(const LinearArgs& g, hipStream_t stream) {
 
 template <int R>
 static int launch_linear(const LinearArgs& g, hipStream_t stream) {
+  if constexpr (R == kRowsMx4) {
+    if (g.T > 512) return launch_mx44<Op::kLinear, Mx44Tile256>(Mx4Args{}, g, (g.T + 255ll) / 256, stream);
+    if (g.T > 128) return launch_mx44<Op::kLinear, Mx44Tile128>(Mx4Args{}, g, (g.T + 127ll) / 128, stream);
+    if (g.T > 32) return launch_mx44<Op::kLinear, Mx44Tile64>(Mx4Args{}, g, (g.T + 63ll) / 64, stream);
+  }
   if (g.T <= 16) {
     if (g.N <= 16384) return launch_linear_few<R, 1, 1, 8>(g, stream);
     return launch_linear_few<R, 4, 1, 4>(g, stream);

@@ -1232,7 +1232,7 @@ def prefill_block_m(n_experts: int, hidden: int, intermediate: int, device="cuda
 
 
 MX4_BLOCK_M = (32, 64, 128)  # row-tile heights of the 4-bit experts' prefill kernel
-MX4_ROWS_BLOCK_M = ()  # and of its form for 4-bit rows
+MX4_ROWS_BLOCK_M = (32, 64, 128, 256)  # and of its form for 4-bit rows
 # Up to this many pairs per expert the split-K kernel, row tiles past it: bf16 rows, 8-bit
 # rows.  Time of the captured layer, split-K over 32-row tiles (H, I, experts, top k):
 #   pairs per expert     3           4           6           8
@@ -1258,8 +1258,6 @@ def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False, columns: int = 0, 
     """The path of a layer of 4-bit experts, for every pass of it: the split-K
     kernel for few pairs per expert (mx8, mx4: of 8-bit, 4-bit rows) and for 8-bit rows
     too long for any row tile (columns: the longer of x's and act's), row tiles past that."""
-    if mx4:
-        return LMOE_PATH_GEMV
     few = MX4_FEW_PAIRS_PER_EXPERT_MX8 if mx8 else MX4_FEW_PAIRS_PER_EXPERT
     if n_pairs <= few * n_experts or (mx8 and columns > MX4_MAX_COLUMNS_MX8[MX4_BLOCK_M[0]]):
         return LMOE_PATH_GEMV
