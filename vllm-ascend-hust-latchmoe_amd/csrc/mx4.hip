@@ -75,49 +75,20 @@ static void launch_few(const Mx4Args& g, const TokenIds& o, hipStream_t stream) 
 // Row tiles of BM rows, at most n_pairs / BM + one short one per slot.
 constexpr int kFewTileBlocks = 512;  // two workgroups per CU: up to these, two chunks a stage
 
-template <bool GU, bool A8, int BM, int CS>
-static int launch_tiles(const Mx4Args& g, unsigned grid, hipStream_t stream) {
-  const int lds = Mx4Tile<A8, BM, CS>::lds_bytes(mx4_chunks(g.K));
-  static bool raised[64] = {};  // per device: dynamic LDS past 64 KiB allowed
-  int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
-  if (e != hipSuccess) return static_cast<int>(e);
-  if (dev < 0 || dev >= 64 || !raised[dev]) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx4_tile_kernel<GU, A8, BM, CS>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (e != hipSuccess) return static_cast<int>(e);
-    if (dev >= 0 && dev < 64) raised[dev] = true;
-  }
-  mx4_tile_kernel<GU, A8, BM, CS><<<grid, kTileWaves * 64, lds, stream>>>(g);
-  return LMOE_OK;
-}
-
 template <bool GU, bool A8, int BM>
 static int launch_tiles(const Mx4Args& g, hipStream_t stream) {
   constexpr int cols = GU ? kTileCols / 2 : kTileCols;
   const long long tiles = g.n_pairs / BM + (g.n_pairs < g.P ? g.n_pairs : g.P);
   const long long blocks = tiles * ((g.N + cols - 1) / cols);
   const long long grid = 8 * ((blocks + 7) / 8);
-  if (grid > 0x7fffffffLL) return LMOE_ERR_SHAPE;
   if constexpr (BM == 32) {
-    if (blocks <= kFewTileBlocks) return launch_tiles<GU, A8, BM, 2>(g, static_cast<unsigned>(grid), stream);
+    if (blocks <= kFewTileBlocks) return launch_tile<GU ? Op::kGateUp : Op::kDown, A8, BM, 2>(g, grid, stream);
   }
-  return launch_tiles<GU, A8, BM, 1>(g, static_cast<unsigned>(grid), stream);
+  return launch_tile<GU ? Op::kGateUp : Op::kDown, A8, BM, 1>(g, grid, stream);
 }
 
 static bool known_block_m(int bm, int rows) {
-  return bm == 32 || bm == 64 || bm == 128 || (bm == 256 && rows == kRowsMx4);
-}
-
-// Whether rows of K columns fit the LDS of tiles of block_m rows (MX8 rows: their scales).
-static bool tiles_fit(int block_m, int rows, int K) {
-  if (rows == kRowsMx4) return true;
-  const bool a8 = rows == kRowsMx8;
-  const int chunks = mx4_chunks(K);
-  const int lds = block_m == 32   ? (a8 ? Mx4Tile<true, 32, 2>::lds_bytes(chunks) : Mx4Tile<false, 32, 2>::lds_bytes(chunks))
-                  : block_m == 64 ? (a8 ? Mx4Tile<true, 64, 1>::lds_bytes(chunks) : Mx4Tile<false, 64, 1>::lds_bytes(chunks))
-                                  : (a8 ? Mx4Tile<true, 128, 1>::lds_bytes(chunks) : Mx4Tile<false, 128, 1>::lds_bytes(chunks));
-  return lds <= 160 * 1024;
+  return bm == 64 || bm == 128 || bm == (rows == kRowsMx4 ? 256 : 32);
 }
 
 template <bool GU, bool A8>
@@ -129,23 +100,23 @@ static int launch_tiles(const Mx4Args& g, int block_m, hipStream_t stream) {
 
 template <bool GU>
 static int launch_tiles4(const Mx4Args& g, int block_m, hipStream_t stream) {
-  constexpr Op op = GU ? Op::kGateUp : Op::kDown;
-  const long long tiles = g.n_pairs / block_m + (g.n_pairs < g.P ? g.n_pairs : g.P);
-  if (block_m == 32) return launch_mx44<op, Mx44Tile32>(g, LinearArgs{}, tiles, stream);
-  if (block_m == 64) return launch_mx44<op, Mx44Tile64>(g, LinearArgs{}, tiles, stream);
-  if (block_m == 128) return launch_mx44<op, Mx44Tile128>(g, LinearArgs{}, tiles, stream);
-  return launch_mx44<op, Mx44Tile256>(g, LinearArgs{}, tiles, stream);
+  if (block_m == 64) return launch_mx44_experts<GU, Mx44Tile64x128>(g, stream);
+  if (block_m == 128) return launch_mx44_experts<GU, Mx44Tile128x256>(g, stream);
+  return launch_mx44_experts<GU, Mx44Tile256x256>(g, stream);
 }
 
 // path AUTO: row tiles past this many pairs per slot, on average, of bf16, MX8 and MX4 rows
 // (native.py has the figures)
-constexpr int kFewPairsPerSlot[3] = {4, 6, 6};
+constexpr int kFewPairsPerSlot[3] = {4, 6, 14};
 
 static bool many_pairs(int rows, int n_pairs, int P) { return n_pairs > static_cast<long long>(kFewPairsPerSlot[rows]) * P; }
 
-static bool takes_tiles(int path, int block_m, int rows, int H, int I, int n_pairs, int P, bool split) {
+// Whether row tiles reach x: the tiles of MX4 rows form its offsets in 32 bits.
+static bool tiles_reach(int rows, long long T, int H) { return rows != kRowsMx4 || T * (H / 2) <= 0xffffffffLL; }
+
+static bool takes_tiles(int path, int block_m, int rows, int T, int H, int I, int n_pairs, int P, bool split) {
   if (path != LMOE_PATH_AUTO) return path == LMOE_PATH_MFMA;
-  return !split && known_block_m(block_m, rows) && many_pairs(rows, n_pairs, P) && tiles_fit(block_m, rows, H) &&
+  return !split && tiles_reach(rows, T, H) && known_block_m(block_m, rows) && many_pairs(rows, n_pairs, P) && tiles_fit(block_m, rows, H) &&
          tiles_fit(block_m, rows, I);
 }
 
@@ -159,11 +130,13 @@ static bool lacks_height(int path, int block_m, int rows, int n_pairs, int P, bo
 template <bool GU>
 static int launch(const Mx4Args& g, int path, int block_m, hipStream_t stream) {
   if (lacks_height(path, block_m, g.rows, g.n_pairs, g.P, g.split)) return LMOE_ERR_SHAPE;
-  if (!takes_tiles(path, block_m, g.rows, g.K, g.N, g.n_pairs, g.P, g.split)) {
+  const int T = GU ? g.n_pairs / g.topk : 0;  // the down product's rows start at a tile's first
+  if (!takes_tiles(path, block_m, g.rows, T, g.K, g.N, g.n_pairs, g.P, g.split)) {
     launch_few<GU, false>(g, TokenIds{}, stream);
   } else {
     if (g.split) return LMOE_ERR_UNSUPPORTED;
-    if (!known_block_m(block_m, g.rows) || !tiles_fit(block_m, g.rows, g.K)) return LMOE_ERR_SHAPE;
+    if (!known_block_m(block_m, g.rows) || !tiles_fit(block_m, g.rows, g.K) || !tiles_reach(g.rows, T, g.K))
+      return LMOE_ERR_SHAPE;
     const int st = g.rows == kRowsMx4   ? launch_tiles4<GU>(g, block_m, stream)
                    : g.rows == kRowsMx8 ? launch_tiles<GU, true>(g, block_m, stream)
                                         : launch_tiles<GU, false>(g, block_m, stream);
@@ -267,11 +240,11 @@ static int fused_moe(int rows, const void* x, const void* x_scale, int T, int H,
         misaligned16(ws->y) || misaligned16(add) || misaligned16(out))
       return LMOE_ERR_SHAPE;
     if (path == LMOE_PATH_MFMA && (!known_block_m(block_m, rows) || !tiles_fit(block_m, rows, H) ||
-                                   !tiles_fit(block_m, rows, I)))
+                                   !tiles_fit(block_m, rows, I) || !tiles_reach(rows, T, H)))
       return LMOE_ERR_SHAPE;
     if (lacks_height(path, block_m, rows, static_cast<int>(n), n_slots, false)) return LMOE_ERR_SHAPE;
   }
-  const int split = ws->act_split && !takes_tiles(path, block_m, rows, H, I, static_cast<int>(n), n_slots, false);
+  const int split = ws->act_split && !takes_tiles(path, block_m, rows, T, H, I, static_cast<int>(n), n_slots, false);
   int st = lmoe_permute(ids, static_cast<int>(n), log2phy, n_log2phy, n_slots, 0, block_m, ws->counts, ws->offsets,
                         ws->sorted_pairs, ws->row_idx, ws->active, ws->tile_off, ws->meta, ws->permute_workspace,
                         ws->permute_workspace_bytes, stream);

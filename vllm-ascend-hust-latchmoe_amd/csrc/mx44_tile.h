@@ -17,12 +17,9 @@
 // Every output adds its chunks in order, whatever BM is: the same bits.
 #pragma once
 
-#include "mx4_linear.h"
 #include "mx4_tile.h"
 
 namespace lmoe {
-
-enum class Op { kGateUp, kDown, kLinear };
 
 // n scales of a row from `at` on, from any address; past the row's groups, ones.
 template <class T>
@@ -46,44 +43,6 @@ __device__ __forceinline__ f32x4_t mx44_step(const i32x4_t w, int ws, const i32x
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4 /* e2m1 */, 4, B, ws, B, xs);
 }
 
-// 32 columns of a row from n on, this lane's: n + 4 g.. (lo) and n + 16 + 4 g.. (hi); hi's
-// may be past the matrix.
-__device__ __forceinline__ f32x4_t linear_terms(const LinearArgs& l, int row, int n, bool live, f32x4_t v) {
-  if (!live) return v;
-  if (l.bias != nullptr) {
-    if (l.bias_f32) {
-      v += *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(l.bias) + n);
-    } else {
-      const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(l.bias) + n);
-      v += f32x4_t{bf16lo(b.x), bf16hi(b.x), bf16lo(b.y), bf16hi(b.y)};
-    }
-  }
-  if (l.add != nullptr) {
-    const uint2 a = *reinterpret_cast<const uint2*>(l.add + static_cast<size_t>(row) * l.N + n);
-    v += f32x4_t{bf16lo(a.x), bf16hi(a.x), bf16lo(a.y), bf16hi(a.y)};
-  }
-  return v;
-}
-__device__ __forceinline__ void store_linear(const LinearArgs& l, int row, int n, int lane, bool live, f32x4_t lo, f32x4_t hi) {
-  const int col = n + 4 * (lane >> 4);
-  if (n + 32 > l.N) {  // the last block alone
-    if (live) store_linear4(l, row, col, lo);
-    return;
-  }
-  lo = linear_terms(l, row, col, live, lo);
-  hi = linear_terms(l, row, col + 16, live, hi);
-  const size_t at = static_cast<size_t>(row) * l.N + n;
-  if (l.out_f32) {
-    if (live) {
-      float* p = static_cast<float*>(l.out) + at + 4 * (lane >> 4);
-      *reinterpret_cast<f32x4_t*>(p) = lo;
-      *reinterpret_cast<f32x4_t*>(p + 16) = hi;
-    }
-  } else {
-    store_bf16x8(static_cast<uint16_t*>(l.out) + at, lane, live, lo, hi);
-  }
-}
-
 // A workgroup's shape: WR x WC waves of MI x NJ fragments of 16 rows by 16 weight rows, NB
 // chunks of both operands in LDS.
 template <int MI_, int NJ_, int WR_, int WC_, int NB_>
@@ -100,7 +59,8 @@ struct Mx44Shape {
   static constexpr int OFF_PAIR = OFF_WSCALE + BN * 16;
   static constexpr int LDS = OFF_PAIR + BM * 4;
   static constexpr int PER_ROW = THREADS / BM;  // threads that bring a row's scales of a quad
-  using scales_t = std::conditional_t<PER_ROW == 2, uint64_t, std::conditional_t<PER_ROW == 4, uint32_t, uint16_t>>;
+  using scales_t = std::conditional_t<PER_ROW == 1, unsigned __int128, std::conditional_t<PER_ROW == 2, uint64_t,
+                                      std::conditional_t<PER_ROW == 4, uint32_t, uint16_t>>>;
   static_assert(PER_ROW * sizeof(scales_t) == 16);
   static_assert(LDS <= 160 * 1024 && BM <= THREADS && QB * 16 * WAVES == BN && A_WAVES * QA * 16 == BM);
   // 16-byte piece p (of four) of row r lies at position p ^ sw(r)
@@ -128,9 +88,8 @@ __device__ __forceinline__ void wait_vm_barrier() {
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// g: the experts' arguments, l: the plain product's (the other is not read)
 template <Op OP, class C>
-__global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(Mx4Args g, LinearArgs l) {
+__global__ __launch_bounds__(C::THREADS, C::NJ > 4 ? 1 : 2) void mx44_tile_kernel(TileArgs<OP> g) {
   constexpr bool GU = OP == Op::kGateUp, LIN = OP == Op::kLinear;
   constexpr int BM = C::BM, MI = C::MI, NJ = C::NJ, NB = C::NB;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -140,30 +99,25 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(Mx4Args g, Lin
   const int lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave / C::WC, wc = wave - wr * C::WC;
-  const int K = LIN ? l.K : g.K, N = LIN ? l.N : g.N;
+  const int K = g.K, N = g.N;
 
   constexpr int OUT_COLS = GU ? C::BN / 2 : C::BN;
-  const int NT = (N + OUT_COLS - 1) / OUT_COLS;
-  SlotWindow win0, win1;
-  int total;
+  int slot = 0, p0, rows, n0;
   if constexpr (LIN) {
-    total = (l.T + BM - 1) / BM * NT;
+    if (!linear_tile(g, BM, OUT_COLS, &p0, &n0)) return;
+    rows = min(BM, g.T - p0);
   } else {
-    win0 = load_window(g.tile_off, g.offsets, g.P, 0, lane);
-    win1 = load_window(g.tile_off, g.offsets, g.P, 64, lane);
-    total = g.meta[LMOE_META_TILES] * NT;
-  }
-  // work item: XCD-contiguous chunks of (row tile, column tile)
-  const int share = (total + 7) >> 3;
-  const int jj = blockIdx.x >> 3;
-  const int item = (blockIdx.x & 7) * share + jj;
-  if (jj >= share || item >= total) return;
-  const int tile = __builtin_amdgcn_readfirstlane(item / NT);
-  const int n0 = (item - tile * NT) * OUT_COLS;
-  int slot = 0, p0 = tile * BM, rows = BM;
-  if constexpr (LIN) {
-    rows = min(BM, l.T - p0);
-  } else {
+    const SlotWindow win0 = load_window(g.tile_off, g.offsets, g.P, 0, lane);
+    const SlotWindow win1 = load_window(g.tile_off, g.offsets, g.P, 64, lane);
+    // work item: XCD-contiguous chunks of (row tile, column tile)
+    const int NT = (N + OUT_COLS - 1) / OUT_COLS;
+    const int total = g.meta[LMOE_META_TILES] * NT;
+    const int share = (total + 7) >> 3;
+    const int jj = blockIdx.x >> 3;
+    const int item = (blockIdx.x & 7) * share + jj;
+    if (jj >= share || item >= total) return;
+    const int tile = __builtin_amdgcn_readfirstlane(item / NT);
+    n0 = (item - tile * NT) * OUT_COLS;
     const TileSlot ts = slot_of_tile(g.tile_off, g.offsets, g.P, tile, win0, win1, lane);
     slot = ts.slot;
     p0 = ts.p0 + (tile - ts.tile0) * BM;
@@ -171,14 +125,15 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(Mx4Args g, Lin
   }
   const int chunks = mx4_chunks(K);
   const int groups = K / kMxGroup;
-  const uint8_t* scale_base = LIN ? l.x_scale : g.a_scale;
+  const uint8_t* scale_base = g.a_scale;
   auto source_row = [&](int r) -> int {  // of the tile's row r; rows past the last repeat the first
     const int pos = r < rows ? r : 0;
-    return GU ? g.sorted_pairs[p0 + pos] / g.topk : pos;
+    if constexpr (GU) return g.sorted_pairs[p0 + pos] / g.topk;
+    else return pos;
   };
   // rows: gate-up's lie anywhere, the others' from the tile's first on
   const size_t row0 = GU ? 0 : p0;
-  const uint8_t* rows_base = uniform(static_cast<const uint8_t*>(LIN ? l.x : g.a) + row_bytes<kRowsMx4>(row0, K));
+  const uint8_t* rows_base = uniform(static_cast<const uint8_t*>(g.a) + row_bytes<kRowsMx4>(row0, K));
   uint32_t a_off[C::QA], a_piece[C::QA];
 #pragma unroll
   for (int q = 0; q < C::QA; ++q) {
@@ -191,7 +146,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(Mx4Args g, Lin
   const int wblocks = (GU ? 2 * N : N) / 16;
   const int b0 = (GU ? 2 * n0 : n0) / 16;
   const int bb = mx4_block_bytes(K);
-  const uint8_t* wbase = uniform((LIN ? l.w : g.w + slot * g.w_slot_bytes) + static_cast<size_t>(b0) * bb);
+  const uint8_t* wbase = uniform(slot_weights(g, slot) + static_cast<size_t>(b0) * bb);
   const int last_block = wblocks - 1 - b0;
   // chunk c to buffer buf; past the last chunk the same loads, out of range: they fetch
   // nothing, and what they leave there is not read
@@ -261,15 +216,26 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(Mx4Args g, Lin
   // straight-line code; rows past the tile's last are dropped at the store
   auto main_loop = [&](auto nl_tag) {
     constexpr int NL = decltype(nl_tag)::value;
+    constexpr int PAIRS = (NL + 1) / 2;
     int xs[NL > 0 ? NL : 1], ws[NJ];
+    i32x4_t w[NJ], x[2][2];  // a chunk's weights, and two fragments of rows; the next two are on their way
     int buf = 0;
+    const char* xp = x_at;  // in the chunk's buffer
+    auto read_w = [&](int j, const char* p) { w[j] = *reinterpret_cast<const i32x4_t*>(p + j * 1024); };
+    auto read_x = [&](int to, int pair, const char* p) {
+#pragma unroll
+      for (int i = 2 * pair; i < 2 * pair + 2 && i < NL; ++i)
+        x[to][i & 1] = *reinterpret_cast<const i32x4_t*>(p + i * 1024);
+    };
     // byte B of the scales: chunk c of its quad.  No branch: the products before the
     // barrier would sink behind it
     auto chunk = [&](int c, auto b_tag) {
       constexpr int B = decltype(b_tag)::value;
-      const char* xp = x_at + buf * C::STAGE;
-      const char* wp = w_at + buf * C::STAGE;
-      const int before = buf == 0 ? NB - 1 : buf - 1;  // the buffer that chunk c - 1 had
+      const int before = buf == 0 ? NB - 1 : buf - 1, next = buf + 1 == NB ? 0 : buf + 1;
+      // not a constant: past what an instruction's offset reaches each would get a register
+      int next_at = next * C::STAGE;
+      asm volatile("" : "+s"(next_at));
+      const char *xn = x_at + next_at, *wn = w_at + next_at;
       // when every wave has got here chunk c + 1 is in LDS and chunk c - 1 read
       auto turn = [&]() {
         if constexpr (B == 2) {  // every wave has read this quad's scales
@@ -281,24 +247,31 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(Mx4Args g, Lin
         if constexpr (B == 1) issue_ws((c >> 2) + 1);
       };
       if constexpr (NL > 0) {
-        i32x4_t w[NJ], x[3];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) w[j] = *reinterpret_cast<const i32x4_t*>(wp + j * 1024);
-        x[0] = *reinterpret_cast<const i32x4_t*>(xp);
-        if (NL > 1) x[1] = *reinterpret_cast<const i32x4_t*>(xp + 1024);
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          if (i == NL / 2) turn();
-          if (i + 2 < NL) x[(i + 2) % 3] = *reinterpret_cast<const i32x4_t*>(xp + (i + 2) * 1024);
+        for (int p = 0; p < PAIRS; ++p) {
+          constexpr int first_x = B * PAIRS & 1;
+          if (p == PAIRS / 2) turn();
+          if (p + 1 < PAIRS) read_x((first_x + p + 1) & 1, p + 1, xp);
+          else read_x((first_x + p + 1) & 1, 0, xn);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) acc[i][j] = mx44_step<B>(w[j], ws[j], x[i % 3], xs[i], acc[i][j]);
+          for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+            for (int i = 2 * p; i < 2 * p + 2 && i < NL; ++i)
+              acc[i][j] = mx44_step<B>(w[j], ws[j], x[(first_x + p) & 1][i & 1], xs[i], acc[i][j]);
+            if (p + 1 == PAIRS) {  // the next chunk's, as this one's are done with
+              __builtin_amdgcn_sched_barrier(0);
+              read_w(j, wn);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
       } else {
         turn();
       }
-      buf = buf + 1 == NB ? 0 : buf + 1;
+      buf = next;
+      xp = xn;
     };
     auto begin_quad = [&](int quad) {
       if constexpr (NL > 0) {
@@ -315,6 +288,11 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(Mx4Args g, Lin
     };
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     wait_vm_barrier<0>();  // chunks 0 to NB - 2, and the scales
+    if constexpr (NL > 0) {
+      read_x(0, 0, x_at);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) read_w(j, w_at);
+    }
     int quad = 0;
     for (; quad < chunks >> 2; ++quad) {
       begin_quad(quad);
@@ -351,7 +329,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(Mx4Args g, Lin
         const f32x4_t gate[2] = {acc[i][j], acc[i][j + 2]}, up[2] = {acc[i][j + 1], acc[i][j + 3]};
         store_act<kRowsMx4>(g, p0 + r, n0 + 8 * (first + j), lane, r < rows, gate, up);
       } else if constexpr (LIN) {
-        store_linear(l, p0 + r, n0 + 16 * (first + j), lane, r < rows, acc[i][j], acc[i][j + 1]);
+        store_linear(g, p0 + r, n0 + 16 * (first + j), lane, r < rows, acc[i][j], acc[i][j + 1]);
       } else {
         store_y(g, s_pair[r], n0 + 16 * (first + j), lane, r < rows, acc[i][j], acc[i][j + 1]);
       }
@@ -359,17 +337,15 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(Mx4Args g, Lin
   }
 }
 
-using Mx44Tile32 = Mx44Shape<2, 4, 1, 4, 4>;
-using Mx44Tile64 = Mx44Shape<4, 4, 1, 4, 3>;
-using Mx44Tile128 = Mx44Shape<8, 4, 1, 4, 3>;
-using Mx44Tile256 = Mx44Shape<8, 4, 2, 4, 4>;
+// By rows and weight rows.
+using Mx44Tile256x256 = Mx44Shape<8, 4, 2, 4, 4>;
+using Mx44Tile128x256 = Mx44Shape<8, 4, 1, 4, 3>;
+using Mx44Tile128x128 = Mx44Shape<4, 4, 2, 2, 4>;
+using Mx44Tile64x128 = Mx44Shape<2, 4, 2, 2, 4>;
+using Mx44Tile64x64 = Mx44Shape<2, 2, 2, 2, 4>;
 
-// Row tiles over `tiles` of them at most.
 template <Op OP, class C>
-int launch_mx44(const Mx4Args& g, const LinearArgs& l, long long tiles, hipStream_t stream) {
-  constexpr int cols = OP == Op::kGateUp ? C::BN / 2 : C::BN;
-  const long long blocks = tiles * (((OP == Op::kLinear ? l.N : g.N) + cols - 1) / cols);
-  const long long grid = 8 * ((blocks + 7) / 8);
+int launch_mx44(const TileArgs<OP>& g, long long grid, hipStream_t stream) {
   if (grid > 0x7fffffffLL) return LMOE_ERR_SHAPE;
   static bool raised[64] = {};  // per device: dynamic LDS past 64 KiB allowed
   int dev = 0;
@@ -381,8 +357,23 @@ int launch_mx44(const Mx4Args& g, const LinearArgs& l, long long tiles, hipStrea
     if (e != hipSuccess) return static_cast<int>(e);
     if (dev >= 0 && dev < 64) raised[dev] = true;
   }
-  mx44_tile_kernel<OP, C><<<static_cast<unsigned>(grid), C::THREADS, C::LDS, stream>>>(g, l);
+  mx44_tile_kernel<OP, C><<<static_cast<unsigned>(grid), C::THREADS, C::LDS, stream>>>(g);
   LMOE_RETURN_LAUNCH();
+}
+
+// Experts: at most n_pairs / BM row tiles and a short one per slot.
+template <bool GU, class C>
+int launch_mx44_experts(const Mx4Args& g, hipStream_t stream) {
+  constexpr int cols = GU ? C::BN / 2 : C::BN;
+  const long long tiles = g.n_pairs / C::BM + (g.n_pairs < g.P ? g.n_pairs : g.P);
+  const long long blocks = tiles * ((g.N + cols - 1) / cols);
+  return launch_mx44<GU ? Op::kGateUp : Op::kDown, C>(g, 8 * ((blocks + 7) / 8), stream);
+}
+
+template <class C>
+int launch_mx44_linear(LinearArgs g, hipStream_t stream) {
+  const long long grid = linear_grid(&g, C::BM, C::BN);
+  return launch_mx44<Op::kLinear, C>(g, grid, stream);
 }
 
 }  // namespace lmoe

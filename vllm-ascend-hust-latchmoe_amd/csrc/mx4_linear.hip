@@ -3,32 +3,99 @@
 
 #include <type_traits>
 
+#include "gemm_lds.h"
 #include "mx44_tile.h"
-#include "mx4_linear.h"
+#include "mx4_tile.h"
 #include "spans.h"
 
 namespace lmoe {
 
-template <int R, int RB, int NF, int NW>
-static int launch_linear_few(const LinearArgs& g, hipStream_t stream) {
+template <int R, int RB, int NF, int NW, int U>
+static int launch_few(const LinearArgs& g, hipStream_t stream) {
   const long long grid = (g.N / 16 + RB - 1) / RB * ((g.T + 16ll * NF - 1) / (16 * NF));
   if (grid > 0x7fffffffll) return LMOE_ERR_SHAPE;
-  mx4_linear_few_kernel<R, RB, NF, NW><<<static_cast<unsigned>(grid), NW * 64, 0, stream>>>(g);
+  mx4_linear_few_kernel<R, RB, NF, NW, U><<<static_cast<unsigned>(grid), NW * 64, 0, stream>>>(g);
   LMOE_RETURN_LAUNCH();
 }
 
+// Workgroups of tiles of BM rows by BN columns.
+static long long tiles_of(const LinearArgs& g, long long BM, long long BN) {
+  return (g.T + BM - 1) / BM * ((g.N + BN - 1) / BN);
+}
+
+// bf16 and MX8 rows in row tiles: the shorter ones while they do not fill the card.  us of
+// 128 / 64 / 32 rows (workgroups of 32 rows; MX8 rows, bf16 rows):
+//   300 x 2048 x 5120   (200)   20.8 / 15.8 / 10.8   30.6 / 21.2 / 14.2
+//   512 x 7168 x 7168   (448)   70.4 / 61.2 / 44.4   106 / 73.5 / 56.8
+//   1024 x 7168 x 7168  (896)   72.0 / 65.8 / 75.7   108 / 94.0 / 108
+//   4096 x 2048 x 5120  (2560)  53.1 / 46.2 / 57.3   79.3 / 71.1 / 86.8
+//   4096 x 7168 x 7168  (3584)  182 / 210 / 262      316 / 321 / 381
+template <bool A8>
+static int launch_rows(LinearArgs g, int cus, hipStream_t stream) {
+  constexpr int R = A8 ? kRowsMx8 : kRowsBf16;
+  int bm = tiles_of(g, 32, kTileCols) <= 2 * cus ? 32 : tiles_of(g, 64, kTileCols) <= 5 * cus ? 64 : 128;
+  while (!tiles_fit(bm, R, g.K) && bm > 32) bm /= 2;  // MX8 rows whose scales do not fit LDS
+  if (!tiles_fit(bm, R, g.K)) return launch_few<R, 4, 2, 8, 2>(g, stream);
+  const long long grid = linear_grid(&g, bm, kTileCols);
+  int st;
+  if (bm == 128) st = launch_tile<Op::kLinear, A8, 128, 1>(g, grid, stream);
+  else if (bm == 64) st = launch_tile<Op::kLinear, A8, 64, 1>(g, grid, stream);
+  else if (grid <= 2 * cus) st = launch_tile<Op::kLinear, A8, 32, 2>(g, grid, stream);
+  else st = launch_tile<Op::kLinear, A8, 32, 1>(g, grid, stream);
+  if (st != LMOE_OK) return st;
+  LMOE_RETURN_LAUNCH();
+}
+
+// MX4 rows: the shape with the least time by this measure, tenths of a us a chunk of K for
+// the workgroups that a CU has at once, 1, 2, .. of them (its last round may have fewer).
+struct ShapeCost {
+  int BM, BN, at_once;
+  int tenths[4];
+};
+// us of 256 x 256 / 128 x 128 / 64 x 128 / 64 x 64 tiles: 4096 x 7168 x 7168 118 / 146 / 184
+// / 252, 4096 x 2048 x 5120 39.9 / 35.2 / 39.6 / 46.5, 1024 x 7168 x 7168 51.0 / 45.4 / 55.9
+// / 63.5, 300 x 2048 x 5120 19.8 / 10.3 / 8.5 / 8.2, 300 x 1408 x 2048 15.5 / 8.8 / 6.8 / 5.8
+constexpr ShapeCost kShapes[4] = {{256, 256, 1, {105}}, {128, 128, 2, {47, 65}}, {64, 128, 3, {34, 48, 66}},
+                                  {64, 64, 4, {28, 36, 50, 64}}};
+static int launch_rows4(const LinearArgs& g, int cus, hipStream_t stream) {
+  int best = 0;
+  long long least = 0;
+  for (int s = 0; s < 4; ++s) {
+    const ShapeCost& c = kShapes[s];
+    const long long each = (tiles_of(g, c.BM, c.BN) + cus - 1) / cus;  // a CU's tiles
+    const long long last = each % c.at_once;
+    const long long time = each / c.at_once * c.tenths[c.at_once - 1] + (last > 0 ? c.tenths[last - 1] : 0);
+    if (s == 0 || time < least) {
+      best = s;
+      least = time;
+    }
+  }
+  if (best == 0) return launch_mx44_linear<Mx44Tile256x256>(g, stream);
+  if (best == 1) return launch_mx44_linear<Mx44Tile128x128>(g, stream);
+  if (best == 2) return launch_mx44_linear<Mx44Tile64x128>(g, stream);
+  return launch_mx44_linear<Mx44Tile64x64>(g, stream);
+}
+
+// Split K while that makes workgroups enough: for the fewest rows 32 columns by 16 rows a
+// workgroup, then 64 by 16, then 64 by 32.  us of these three and of row tiles (T x K x N):
+//              16 x 2048 x 5120    32 x 7168 x 7168       64 x 7168 x 7168       128 x 2048 x 5120
+//   MX4 rows   4.4 / 4.7 / 5.0 /   15.3 / 12.2 / 15.8 / 19  27 / 20.6 / 15.2 / 19.5    - / - / 9.3 / 6.8
+//   bf16 rows  5.4 / 6.4 / 7.3 /   20.8 / 15.2 / 23.5 / -   37 / 25.8 / 23.2 / 44.3    15.3 / 12.5 / 15.6 / 13.8
+// Past 16384 columns, up to 16 rows: bf16 rows, which are read again by every workgroup,
+// 128 columns a workgroup (16 x 2048 x 50000 20.1 -> 15.7; 4-bit rows 13.8, 13.6).
 template <int R>
 static int launch_linear(const LinearArgs& g, hipStream_t stream) {
+  const int cus = device_cus();
+  if (R == kRowsBf16 && g.T <= 16 && g.N > 16384) return launch_few<R, 8, 1, 4, 1>(g, stream);
+  if (g.T <= 16 || tiles_of(g, 16, 32) <= cus) return launch_few<R, 2, 1, 8, 2>(g, stream);
+  if (tiles_of(g, 16, 64) <= cus + cus / 4) return launch_few<R, 4, 1, 8, 2>(g, stream);
+  if (tiles_of(g, 32, 64) <= cus) return launch_few<R, 4, 2, 8, 2>(g, stream);
   if constexpr (R == kRowsMx4) {
-    if (g.T > 512) return launch_mx44<Op::kLinear, Mx44Tile256>(Mx4Args{}, g, (g.T + 255ll) / 256, stream);
-    if (g.T > 128) return launch_mx44<Op::kLinear, Mx44Tile128>(Mx4Args{}, g, (g.T + 127ll) / 128, stream);
-    if (g.T > 32) return launch_mx44<Op::kLinear, Mx44Tile64>(Mx4Args{}, g, (g.T + 63ll) / 64, stream);
+    return launch_rows4(g, cus, stream);
+  } else {
+    if (tiles_of(g, 16, 64) <= 5 * cus / 2) return launch_few<R, 4, 1, 8, 2>(g, stream);
+    return launch_rows<R == kRowsMx8>(g, cus, stream);
   }
-  if (g.T <= 16) {
-    if (g.N <= 16384) return launch_linear_few<R, 1, 1, 8>(g, stream);
-    return launch_linear_few<R, 4, 1, 4>(g, stream);
-  }
-  return launch_linear_few<R, 4, 2, 4>(g, stream);
 }
 
 }  // namespace lmoe
@@ -55,7 +122,7 @@ extern "C" int lmoe_mx4_linear(const void* x, const void* x_scale, int rows, int
   for (int i = 0; i < 5; ++i)  // in place over add: each value is read where its sum is written
     if (overlap(o, in[i]) && !(i == 4 && add == out && !out_f32)) return LMOE_ERR_ARG;
   const LinearArgs g{x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(w), T, K, N, bias,
-                     static_cast<const uint16_t*>(add), out, bias_f32 != 0, out_f32 != 0};
+                     static_cast<const uint16_t*>(add), out, bias_f32 != 0, out_f32 != 0, 1};
   if (rows == kRowsMx4) return launch_linear<kRowsMx4>(g, stream);
   if (rows == kRowsMx8) return launch_linear<kRowsMx8>(g, stream);
   return launch_linear<kRowsBf16>(g, stream);

@@ -32,7 +32,9 @@
 // Every output adds its chunks in order, whatever BM is: the same bits.
 #pragma once
 
-#include "mx4_few.h"
+#include <type_traits>
+
+#include "mx4_linear.h"
 
 namespace lmoe {
 
@@ -106,8 +108,50 @@ __device__ __forceinline__ TileSlot slot_of_tile(const int32_t* tile_off, const 
   }
 }
 
-template <bool GU, bool A8, int BM, int CS>
-__global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g) {
+__device__ __forceinline__ const uint8_t* slot_weights(const Mx4Args& g, int slot) { return g.w + slot * g.w_slot_bytes; }
+__device__ __forceinline__ const uint8_t* slot_weights(const LinearArgs& g, int) { return g.w; }
+
+// What a tile kernel computes: the experts' two products, or the product with one matrix.
+enum class Op { kGateUp, kDown, kLinear };
+template <Op OP>
+using TileArgs = std::conditional_t<OP == Op::kLinear, LinearArgs, Mx4Args>;
+
+// The tile of one workgroup of the plain product, its first row and column: false where
+// there is none.  An XCD has a block of row tiles by column tiles, which shares its L2, and
+// takes the row tiles of a column one after the other.
+__device__ __forceinline__ bool linear_tile(const LinearArgs& g, int BM, int BN, int* p0, int* n0) {
+  const int xcd = blockIdx.x & 7, jj = blockIdx.x >> 3;
+  const int RT = (g.T + BM - 1) / BM, NT = (g.N + BN - 1) / BN, xcs = 8 / g.xcd_rows;
+  const int xr = xcd / xcs, xc = xcd - xr * xcs;
+  const int r0 = RT * xr / g.xcd_rows, rn = RT * (xr + 1) / g.xcd_rows - r0;
+  const int c0 = NT * xc / xcs, cn = NT * (xc + 1) / xcs - c0;
+  if (jj >= rn * cn) return false;
+  const int col = __builtin_amdgcn_readfirstlane(jj / rn);
+  *p0 = (r0 + jj - col * rn) * BM;
+  *n0 = (c0 + col) * BN;
+  return true;
+}
+// Its grid: the eight XCDs divide the row tiles by xcd_rows and the column tiles by the
+// rest, as evenly as they can, then with the fewest bytes for each L2.
+inline long long linear_grid(LinearArgs* g, long long BM, long long BN) {
+  const long long RT = (g->T + BM - 1) / BM, NT = (g->N + BN - 1) / BN;
+  if (RT > 0x7fffffffLL / 8 || NT > 0x7fffffffLL / 8) return 0x80000000LL;
+  long long best = 0, best_lines = 0;
+  for (int xr = 1; xr <= 8; xr *= 2) {
+    const long long r = (RT + xr - 1) / xr, c = (NT * xr + 7) / 8;
+    const long long items = r * c, lines = r * BM + c * BN;
+    if (best == 0 || items < best || (items == best && lines < best_lines)) {
+      best = items;
+      best_lines = lines;
+      g->xcd_rows = xr;
+    }
+  }
+  return 8 * best;
+}
+
+template <Op OP, bool A8, int BM, int CS>
+__global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(TileArgs<OP> g) {
+  constexpr bool GU = OP == Op::kGateUp, LIN = OP == Op::kLinear;
   using C = Mx4Tile<A8, BM, CS>;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   int* s_pair = reinterpret_cast<int*>(smem + C::OFF_PAIR);
@@ -117,28 +161,38 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   const int lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  // work item: XCD-contiguous chunks of (row tile, column tile)
   constexpr int OUT_COLS = GU ? kTileCols / 2 : kTileCols;
-  const int NT = (g.N + OUT_COLS - 1) / OUT_COLS;
-  const SlotWindow win0 = load_window(g.tile_off, g.offsets, g.P, 0, lane);
-  const SlotWindow win1 = load_window(g.tile_off, g.offsets, g.P, 64, lane);
-  const int total = g.meta[LMOE_META_TILES] * NT;
-  const int share = (total + 7) >> 3;
-  const int jj = blockIdx.x >> 3;
-  const int item = (blockIdx.x & 7) * share + jj;
-  if (jj >= share || item >= total) return;
-  const int tile = item / NT;
-  const int n0 = (item - tile * NT) * OUT_COLS;
-  const TileSlot ts = slot_of_tile(g.tile_off, g.offsets, g.P, tile, win0, win1, lane);
-  const int slot = ts.slot;
-  const int p0 = ts.p0 + (tile - ts.tile0) * BM;
-  const int rows = min(BM, ts.p1 - p0);
+  int slot = 0, p0, rows, n0;
+  if constexpr (LIN) {
+    if (!linear_tile(g, BM, OUT_COLS, &p0, &n0)) return;
+    rows = min(BM, g.T - p0);
+  } else {
+    // work item: XCD-contiguous chunks of (row tile, column tile)
+    const int NT = (g.N + OUT_COLS - 1) / OUT_COLS;
+    const SlotWindow win0 = load_window(g.tile_off, g.offsets, g.P, 0, lane);
+    const SlotWindow win1 = load_window(g.tile_off, g.offsets, g.P, 64, lane);
+    const int total = g.meta[LMOE_META_TILES] * NT;
+    const int share = (total + 7) >> 3;
+    const int jj = blockIdx.x >> 3;
+    const int item = (blockIdx.x & 7) * share + jj;
+    if (jj >= share || item >= total) return;
+    const int tile = item / NT;
+    n0 = (item - tile * NT) * OUT_COLS;
+    const TileSlot ts = slot_of_tile(g.tile_off, g.offsets, g.P, tile, win0, win1, lane);
+    slot = ts.slot;
+    p0 = ts.p0 + (tile - ts.tile0) * BM;
+    rows = min(BM, ts.p1 - p0);
+  }
 
   const int K = g.K;
   const int chunks = mx4_chunks(K);
   const int tail = K & (kMxChunk - 1);  // columns of a short last chunk, 0: none
   constexpr int R = A8 ? kRowsMx8 : kRowsBf16;
 
+  auto source_row = [&](int pos) -> size_t {
+    if constexpr (GU) return g.sorted_pairs[pos] / g.topk;
+    else return pos;
+  };
   // this lane's source of each load instruction: row, and piece within a chunk
   auto a_row = [&](int q) { return (wave * C::QA + q) * C::RPL + lane / C::PIECES; };
   auto a_piece = [&](int q) { return (lane % C::PIECES) ^ C::sw(a_row(q)); };
@@ -147,7 +201,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   for (int q = 0; q < C::QA; ++q) {
     const int r = a_row(q);
     const int pos = p0 + (r < rows ? r : 0);
-    const size_t src = GU ? g.sorted_pairs[pos] / g.topk : pos;
+    const size_t src = source_row(pos);
     a_src[q] = static_cast<const char*>(g.a) + row_bytes<R>(src, K) + a_piece(q) * 16;
   }
   const int stages = (chunks + CS - 1) / CS;
@@ -179,7 +233,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   const uint8_t* wsrc[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    wsrc[j] = g.w + slot * g.w_slot_bytes + static_cast<size_t>(min(b0 + j, wblocks - 1)) * bb;
+    wsrc[j] = slot_weights(g, slot) + static_cast<size_t>(min(b0 + j, wblocks - 1)) * bb;
   const uint32_t code_at = lane * 16, scale_at = lane * 4;
   // codes of a stage's chunks (one past the last: the last's; its rows are zeros), and
   // the scales: byte c % 4 is chunk c's, of one dword for the whole stage
@@ -208,12 +262,13 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
   int sc_next[4];
   issue(0, 0);
   load_w(0, w_next, sc_next);
-  for (int r = tid; r < BM; r += kTileWaves * 64) s_pair[r] = g.sorted_pairs[p0 + (r < rows ? r : 0)];
+  if constexpr (!LIN)
+    for (int r = tid; r < BM; r += kTileWaves * 64) s_pair[r] = g.sorted_pairs[p0 + (r < rows ? r : 0)];
   if constexpr (A8) {
     const int groups = K / kMxGroup;
     const int r = tid & (BM - 1);  // a row's scales, some chunks of it
     const int pos = p0 + (r < rows ? r : 0);
-    const uint8_t* sp = g.a_scale + static_cast<size_t>(GU ? g.sorted_pairs[pos] / g.topk : pos) * groups;
+    const uint8_t* sp = g.a_scale + source_row(pos) * groups;
     constexpr int STEP = kTileWaves * 64 / BM;
     if (tail == 0 && (reinterpret_cast<uintptr_t>(g.a_scale) & 3) == 0) {  // straight to LDS, 64 of them at a time
       for (int c = wave * 64 / BM; c < stages * CS; c += STEP) {
@@ -333,12 +388,44 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(Mx4Args g)
     if constexpr (GU) {
       const f32x4_t gate[2] = {acc[i][0], acc[i][2]}, up[2] = {acc[i][1], acc[i][3]};
       store_act<R>(g, p0 + r, n0 + 32 * wave, lane, r < rows, gate, up);
+    } else if constexpr (LIN) {
+      store_linear(g, p0 + r, n0 + 64 * wave, lane, r < rows, acc[i][0], acc[i][1]);
+      if (b0 + 2 < wblocks) store_linear(g, p0 + r, n0 + 64 * wave + 32, lane, r < rows, acc[i][2], acc[i][3]);
     } else {
       const int pair = s_pair[r];
       store_y(g, pair, n0 + 64 * wave, lane, r < rows, acc[i][0], acc[i][1]);
       if (b0 + 2 < wblocks) store_y(g, pair, n0 + 64 * wave + 32, lane, r < rows, acc[i][2], acc[i][3]);
     }
   }
+}
+
+template <Op OP, bool A8, int BM, int CS>
+int launch_tile(const TileArgs<OP>& g, long long grid, hipStream_t stream) {
+  if (grid > 0x7fffffffLL) return LMOE_ERR_SHAPE;
+  const int lds = Mx4Tile<A8, BM, CS>::lds_bytes(mx4_chunks(g.K));
+  static bool raised[64] = {};  // per device: dynamic LDS past 64 KiB allowed
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return static_cast<int>(e);
+  if (dev < 0 || dev >= 64 || !raised[dev]) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx4_tile_kernel<OP, A8, BM, CS>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e != hipSuccess) return static_cast<int>(e);
+    if (dev >= 0 && dev < 64) raised[dev] = true;
+  }
+  mx4_tile_kernel<OP, A8, BM, CS><<<static_cast<unsigned>(grid), kTileWaves * 64, lds, stream>>>(g);
+  return LMOE_OK;
+}
+
+// Whether rows of K columns fit the LDS of tiles of block_m rows (MX8 rows: their scales).
+inline bool tiles_fit(int block_m, int rows, int K) {
+  if (rows == kRowsMx4) return true;
+  const bool a8 = rows == kRowsMx8;
+  const int chunks = mx4_chunks(K);
+  const int lds = block_m == 32   ? (a8 ? Mx4Tile<true, 32, 2>::lds_bytes(chunks) : Mx4Tile<false, 32, 2>::lds_bytes(chunks))
+                  : block_m == 64 ? (a8 ? Mx4Tile<true, 64, 1>::lds_bytes(chunks) : Mx4Tile<false, 64, 1>::lds_bytes(chunks))
+                                  : (a8 ? Mx4Tile<true, 128, 1>::lds_bytes(chunks) : Mx4Tile<false, 128, 1>::lds_bytes(chunks));
+  return lds <= 160 * 1024;
 }
 
 }  // namespace lmoe

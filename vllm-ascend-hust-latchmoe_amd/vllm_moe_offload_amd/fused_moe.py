@@ -275,14 +275,16 @@ def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2
     I = w13_slots.shape[1] // 2
     mx8, mx4 = isinstance(hidden, native.Mx8Rows), isinstance(hidden, native.Mx4Rows)
     if path == native.LMOE_PATH_AUTO:
-        path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel(), mx8, max(H, I), mx4=mx4)
+        path = native.mx4_path(T * k, P if log2phy is None else log2phy.numel(), mx8, max(H, I), mx4=mx4,
+                               row_values=T * H)
         if path == native.LMOE_PATH_GEMV and (T == 1 or T * k <= native.MX4_DIRECT_PAIRS and not counted):
             if counted:  # one token's form reads no permutation
                 native.permute(topk_ids, ws.perm, log2phy=log2phy)
             direct = native.mx4_decode_one if T == 1 else native.mx4_decode_few
             return direct(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add)
     return native.mx4_fused_moe(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, ws.mx4, dst, add=add,
-                                path=path, block_m=native.mx4_block_m(T * k, P, I, max(H, I) if mx8 else 0))
+                                path=path, block_m=native.mx4_block_m(T * k, P, I, max(H, I) if mx8 else 0,
+                                                           mx4_columns=max(H, I) if mx4 else 0))
 
 
 def _second_bank(overflow: PreparedSlotWeights | None) -> tuple | None:
@@ -297,7 +299,7 @@ def _layer_path(hidden, k: int, n_experts: int, *w13) -> int:
     T, H = hidden.shape
     if mxfp4.is_mx4(w13[0]):
         return native.mx4_path(T * k, n_experts, isinstance(hidden, native.Mx8Rows), max(H, int(w13[0].shape[1]) // 2),
-                               mx4=isinstance(hidden, native.Mx4Rows))
+                               mx4=isinstance(hidden, native.Mx4Rows), row_values=T * H)
     return native.layer_path(T, k, H, int(w13[0].shape[1]) // 2, n_experts, aligned=native.aligned16(hidden, *w13))
 
 
@@ -321,7 +323,8 @@ def _pass_block_m(n_experts: int, H: int, I: int, device, n_pairs: int, path: in
     rows_kind of the experts."""
     if rows:
         return native.mx4_block_m(n_pairs if pass_pairs is None else pass_pairs, n_experts, I,
-                                  max(H, I) if rows == "mx8" else 0)
+                                  max(H, I) if rows == "mx8" else 0,
+                                  mx4_columns=max(H, I) if rows == "mx4" else 0)
     if path == native.LMOE_PATH_GEMV:
         return native.MFMA_BLOCK_M
     if path == native.LMOE_PATH_STREAM:

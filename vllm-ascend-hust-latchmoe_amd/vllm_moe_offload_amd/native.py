@@ -1232,7 +1232,7 @@ def prefill_block_m(n_experts: int, hidden: int, intermediate: int, device="cuda
 
 
 MX4_BLOCK_M = (32, 64, 128)  # row-tile heights of the 4-bit experts' prefill kernel
-MX4_ROWS_BLOCK_M = (32, 64, 128, 256)  # and of its form for 4-bit rows
+MX4_ROWS_BLOCK_M = (64, 128, 256)  # and of its form for 4-bit rows
 # Up to this many pairs per expert the split-K kernel, row tiles past it: bf16 rows, 8-bit
 # rows.  Time of the captured layer, split-K over 32-row tiles (H, I, experts, top k):
 #   pairs per expert     3           4           6           8
@@ -1247,6 +1247,15 @@ MX4_ROWS_BLOCK_M = (32, 64, 128, 256)  # and of its form for 4-bit rows
 # (1024 x 512 x 64) and 12% at 6 (4096 x 1024 x 16), of 8-bit rows 13% at 6 (1024 x 512).
 MX4_FEW_PAIRS_PER_EXPERT = 4
 MX4_FEW_PAIRS_PER_EXPERT_MX8 = 6
+# 4-bit rows (us of the captured layer, split-K / tiles of 64 rows by 128 weight rows):
+#   pairs per expert     8            12           16           24
+#   2048, 768, 128, 8    69.5 / 74.7  76.7 / 80.1  83.8 / 82.1  99.1 / 84.7
+#   2048, 1408, 60, 4    60.7 / 72.1  63.9 / 72.0  69.5 / 72.9  80.3 / 77.9
+#   4096, 1024, 16, 2    30.2 / 34.8  33.6 / 36.4  35.6 / 37.5  39.5 / 37.8
+#   7168, 2048, 32, 8    157 / 158    154 / 156    169 / 160    190 / 165
+#   1024, 512, 64, 4     23.8 / 25.6  25.0 / 26.3  26.8 / 27.3  33.9 / 29.8
+#   4096, 2048, 64, 4    163 / 170    176 / 175    189 / 179    220 / 181
+MX4_FEW_PAIRS_PER_EXPERT_MX4 = 14
 
 
 # The longest 8-bit rows of a tile of each height: the tile keeps all their scales in LDS
@@ -1254,10 +1263,14 @@ MX4_FEW_PAIRS_PER_EXPERT_MX8 = 6
 MX4_MAX_COLUMNS_MX8 = {32: 147200, 64: 73600, 128: 32640}
 
 
-def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False, columns: int = 0, *, mx4: bool = False) -> int:
+def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False, columns: int = 0, *, mx4: bool = False, row_values: int = 0) -> int:
     """The path of a layer of 4-bit experts, for every pass of it: the split-K
     kernel for few pairs per expert (mx8, mx4: of 8-bit, 4-bit rows) and for 8-bit rows
-    too long for any row tile (columns: the longer of x's and act's), row tiles past that."""
+    too long for any row tile (columns: the longer of x's and act's) or more 4-bit rows
+    than its 32-bit offsets reach (row_values: of all tokens), row tiles past that."""
+    if mx4:
+        few = n_pairs <= MX4_FEW_PAIRS_PER_EXPERT_MX4 * n_experts or row_values // 2 > 0xFFFFFFFF
+        return LMOE_PATH_GEMV if few else LMOE_PATH_MFMA
     few = MX4_FEW_PAIRS_PER_EXPERT_MX8 if mx8 else MX4_FEW_PAIRS_PER_EXPERT
     if n_pairs <= few * n_experts or (mx8 and columns > MX4_MAX_COLUMNS_MX8[MX4_BLOCK_M[0]]):
         return LMOE_PATH_GEMV
@@ -1284,12 +1297,36 @@ def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False, columns: int = 0, 
 #   7168, 2048, 32, 8    50                 225 / 183 / 203 (8-bit rows)
 #                        100                325 / 262 / 247
 MX4_HEIGHTS = ((32, 32, 640), (64, 100, 1024))
+# Heights of 4-bit rows' tiles.  64 rows (by 128 weight rows) up to this many pairs per
+# slot, on average, or this many gate-up workgroups; 128 rows (by 256); 256 rows (by 256),
+# whose rows are read from LDS for twice the weights, from 110 pairs on where rows are
+# long, and where they are short up to 200 (past them the second of two tiles is nearly
+# empty as often as not).  us of the captured layer, 64 / 128 / 256 rows:
+#   pairs per slot       48               80               128              192              256
+#   2048, 768, 128, 8    95 / 100 / 103   126 / 109 / 115  156 / 140 / 134  202 / 164 / 162  252 / 206 / 222
+#   2048, 1408, 60, 4    83 / 86 / 88     107 / 94 / 98    125 / 116 / 109  161 / 132 / 130  187 / 160 / 167
+#   1024, 512, 64, 4     32 / 34 / 34     42 / 37 / 37     47 / 46 / 41     57 / 47 / 48     68 / 66 / 71
+#   7168, 2048, 32, 8    176 / 172 / 179  255 / 186 / 195  302 / 264 / 220  407 / 271 / 254  515 / 368 / 343
+#   4096, 2048, 64, 4    202 / 196 / 206  278 / 210 / 223  346 / 279 / 251  453 / 312 / 290  565 / 391 / 383
+#   4096, 1024, 16, 2    41 / 56 / 49     51 / 59 / 54     68 / 67 / 62     79 / 68 / 73     90 / 81 / 90
+MX4_ROWS_LOW_PAIRS = 50
+MX4_ROWS_LOW_GROUPS = 700
+MX4_ROWS_TALL_PAIRS = (110, 200)
+MX4_ROWS_TALL_COLUMNS = 4096
 
 
-def mx4_block_m(n_pairs: int, n_experts: int, intermediate: int = 1024, mx8_columns: int = 0) -> int:
+def mx4_block_m(n_pairs: int, n_experts: int, intermediate: int = 1024, mx8_columns: int = 0, *,
+                mx4_columns: int = 0) -> int:
     """Row-tile height of 4-bit experts' products (the permutation's block_m) for
     n_pairs pairs over n_experts slots of experts intermediate wide.  mx8_columns:
-    the longer of x's and act's rows, where they are in 8 bits."""
+    the longer of x's and act's rows, where they are in 8 bits; mx4_columns: in 4 bits."""
+    if mx4_columns:
+        groups = (n_pairs // 64 + n_experts) * -(-intermediate // 64)
+        if n_pairs <= MX4_ROWS_LOW_PAIRS * n_experts or groups <= MX4_ROWS_LOW_GROUPS:
+            return 64
+        tall = n_pairs > MX4_ROWS_TALL_PAIRS[0] * n_experts and \
+            (mx4_columns >= MX4_ROWS_TALL_COLUMNS or n_pairs <= MX4_ROWS_TALL_PAIRS[1] * n_experts)
+        return 256 if tall else 128
     best = MX4_BLOCK_M[-1]
     for bm, pairs, groups in MX4_HEIGHTS:
         if n_pairs <= pairs * n_experts or (n_pairs // bm + n_experts) * -(-intermediate // 128) <= groups:
@@ -1627,10 +1664,11 @@ def _alike(x, act) -> bool:
     return type(x) is type(act) or not isinstance(x, (Mx8Rows, Mx4Rows)) and not isinstance(act, (Mx8Rows, Mx4Rows))
 
 
-def _check_products(status: int, fn: str, perm: Permutation) -> None:
-    if status == LMOE_ERR_SHAPE and perm.block_m not in MX4_BLOCK_M:
+def _check_products(status: int, fn: str, perm: Permutation, rows) -> None:
+    heights = MX4_ROWS_BLOCK_M if isinstance(rows, Mx4Rows) else MX4_BLOCK_M
+    if status == LMOE_ERR_SHAPE and perm.block_m not in heights:
         raise ValueError(f"{fn}: unsupported shape; the permutation was built with block_m {perm.block_m}, row tiles "
-                         f"of 4-bit experts have {MX4_BLOCK_M} rows (mx4_block_m)")
+                         f"of 4-bit experts have {heights} rows (mx4_block_m)")
     _check(status, fn)
 
 
@@ -1653,7 +1691,7 @@ def _mx4_gateup_silu(x, top_k: int, w13_slots: torch.Tensor, perm: Permutation, 
             p.sorted_pairs.data_ptr(), p.active.data_ptr(), p.tile_off.data_ptr(), p.meta.data_ptr(), n, p.block_m, path,
             aq.data_ptr(), _ptr(as_), split, _stream(stream),
         ),
-        "lmoe_mx4_gateup_silu", p,
+        "lmoe_mx4_gateup_silu", p, x,
     )
     return act
 
@@ -1673,7 +1711,7 @@ def _mx4_down(act, w2_slots: torch.Tensor, perm: Permutation, y: torch.Tensor, *
             p.sorted_pairs.data_ptr(), p.active.data_ptr(), p.tile_off.data_ptr(), p.meta.data_ptr(), n, p.block_m, path,
             y.data_ptr(), y_f32, _stream(stream),
         ),
-        "lmoe_mx4_down", p,
+        "lmoe_mx4_down", p, act,
     )
     return y
 
