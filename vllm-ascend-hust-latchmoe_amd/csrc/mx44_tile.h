@@ -50,19 +50,16 @@ struct Mx44Shape {
   static constexpr int MI = MI_, NJ = NJ_, WR = WR_, WC = WC_, NB = NB_;
   static constexpr int BM = 16 * MI * WR, BN = 16 * NJ * WC;
   static constexpr int WAVES = WR * WC, THREADS = 64 * WAVES;
-  static constexpr int QA = BM / 16 / WAVES > 0 ? BM / 16 / WAVES : 1;  // load instructions of a wave and chunk: rows
-  static constexpr int QB = BN / 16 / WAVES;                            // and weights
-  static constexpr int A_WAVES = BM / 16 / QA;                          // waves that load rows
+  static constexpr int QA = BM / 16 / WAVES, QB = BN / 16 / WAVES;  // load instructions of a wave and chunk: rows, weights
   static constexpr int PART_A = BM * 64, PART_B = BN * 64, STAGE = PART_A + PART_B;
   static constexpr int OFF_SCALE = NB * STAGE;           // a quad's scales: BM x 16 bytes of rows,
   static constexpr int OFF_WSCALE = OFF_SCALE + BM * 16;  // BN / 16 blocks of 256 of weights
   static constexpr int OFF_PAIR = OFF_WSCALE + BN * 16;
   static constexpr int LDS = OFF_PAIR + BM * 4;
   static constexpr int PER_ROW = THREADS / BM;  // threads that bring a row's scales of a quad
-  using scales_t = std::conditional_t<PER_ROW == 1, unsigned __int128, std::conditional_t<PER_ROW == 2, uint64_t,
-                                      std::conditional_t<PER_ROW == 4, uint32_t, uint16_t>>>;
+  using scales_t = std::conditional_t<PER_ROW == 2, uint64_t, uint32_t>;
   static_assert(PER_ROW * sizeof(scales_t) == 16);
-  static_assert(LDS <= 160 * 1024 && BM <= THREADS && QB * 16 * WAVES == BN && A_WAVES * QA * 16 == BM);
+  static_assert(LDS <= 160 * 1024 && BM <= THREADS && QA * 16 * WAVES == BM && QB * 16 * WAVES == BN);
   // 16-byte piece p (of four) of row r lies at position p ^ sw(r)
   static __device__ __forceinline__ int sw(int r) { return (0x78 >> (2 * ((r >> 2) & 3))) & 3; }
 };
@@ -89,7 +86,7 @@ __device__ __forceinline__ void wait_vm_barrier() {
 }
 
 template <Op OP, class C>
-__global__ __launch_bounds__(C::THREADS, C::NJ > 4 ? 1 : 2) void mx44_tile_kernel(TileArgs<OP> g) {
+__global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(TileArgs<OP> g) {
   constexpr bool GU = OP == Op::kGateUp, LIN = OP == Op::kLinear;
   constexpr int BM = C::BM, MI = C::MI, NJ = C::NJ, NB = C::NB;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -126,22 +123,27 @@ __global__ __launch_bounds__(C::THREADS, C::NJ > 4 ? 1 : 2) void mx44_tile_kerne
   const int chunks = mx4_chunks(K);
   const int groups = K / kMxGroup;
   const uint8_t* scale_base = g.a_scale;
-  auto source_row = [&](int r) -> int {  // of the tile's row r; rows past the last repeat the first
-    const int pos = r < rows ? r : 0;
-    if constexpr (GU) return g.sorted_pairs[p0 + pos] / g.topk;
-    else return pos;
+  // the pair of the tile's row r; rows past the last repeat the first
+  auto pair_of = [&](int r) -> int {
+    if constexpr (LIN) return 0;
+    else return g.sorted_pairs[p0 + (r < rows ? r : 0)];
+  };
+  // its row of the operand, from row0 on
+  auto source_row = [&](int r, int pair) -> int {
+    if constexpr (GU) return pair / g.topk;
+    else return r < rows ? r : 0;
   };
   // rows: gate-up's lie anywhere, the others' from the tile's first on
   const size_t row0 = GU ? 0 : p0;
   const uint8_t* rows_base = uniform(static_cast<const uint8_t*>(g.a) + row_bytes<kRowsMx4>(row0, K));
-  uint32_t a_off[C::QA], a_piece[C::QA];
+  auto a_row = [&](int q) { return (wave * C::QA + q) * 16 + lane / 4; };
+  int a_pair[C::QA];
 #pragma unroll
-  for (int q = 0; q < C::QA; ++q) {
-    const int r = (wave * C::QA + q) * 16 + lane / 4;
-    a_piece[q] = (lane & 3) ^ C::sw(r);
-    a_off[q] = static_cast<uint32_t>(source_row(r < BM ? r : 0)) * (K >> 1) + a_piece[q] * 16;
-  }
-  const uint32_t tail = K - (chunks - 1) * kMxChunk;  // columns of the last chunk
+  for (int q = 0; q < C::QA; ++q) a_pair[q] = GU ? pair_of(a_row(q)) : 0;
+  const int s_row = tid / C::PER_ROW;  // the row whose scales this thread brings
+  const int scale_pair = GU ? pair_of(s_row) : 0;
+  const int my_pair = tid < BM ? pair_of(tid) : 0;
+  asm volatile("" ::: "memory");  // on their way before the loads below, which do not need them
   // weight blocks; those past the matrix repeat the last one
   const int wblocks = (GU ? 2 * N : N) / 16;
   const int b0 = (GU ? 2 * n0 : n0) / 16;
@@ -150,25 +152,31 @@ __global__ __launch_bounds__(C::THREADS, C::NJ > 4 ? 1 : 2) void mx44_tile_kerne
   const int last_block = wblocks - 1 - b0;
   // chunk c to buffer buf; past the last chunk the same loads, out of range: they fetch
   // nothing, and what they leave there is not read
-  auto issue = [&](int c, int buf) {
-    char* st = smem + buf * C::STAGE;
-    const bool on = c < chunks;
-    if (C::A_WAVES == C::WAVES || wave < C::A_WAVES) {
-#pragma unroll
-      for (int q = 0; q < C::QA; ++q) {
-        // past the row's end any codes do: the weights' are zeros there
-        const uint32_t back = c + 1 >= chunks && a_piece[q] * 32 >= tail ? a_piece[q] * 16 : 0;
-        buffer_to_lds16(rows_base, on, st + (wave * C::QA + q) * 1024, a_off[q] - back, c * 64);
-      }
-    }
+  auto issue_w = [&](int c, int buf) {
     const int at = (c >> 2) * kMxQuadBytes + 256 + (c & 3) * 1024;
 #pragma unroll
     for (int q = 0; q < C::QB; ++q) {
       const int b = wave * C::QB + q;
-      buffer_to_lds16(wbase, on, st + C::PART_A + b * 1024, lane * 16, min(b, last_block) * bb + at);
+      buffer_to_lds16(wbase, c < chunks, smem + buf * C::STAGE + C::PART_A + b * 1024, lane * 16,
+                      min(b, last_block) * bb + at);
     }
   };
-  constexpr int LOADS = C::QB + (C::A_WAVES == C::WAVES ? C::QA : 0);  // of a wave and chunk, at least
+  uint32_t a_off[C::QA];
+  const uint32_t tail = K - (chunks - 1) * kMxChunk;  // columns of the last chunk
+  auto issue_a = [&](int c, int buf) {
+#pragma unroll
+    for (int q = 0; q < C::QA; ++q) {
+      // past the row's end any codes do: the weights' are zeros there
+      const uint32_t piece = (lane & 3) ^ C::sw(a_row(q));
+      const uint32_t back = c + 1 >= chunks && piece * 32 >= tail ? piece * 16 : 0;
+      buffer_to_lds16(rows_base, c < chunks, smem + buf * C::STAGE + (wave * C::QA + q) * 1024, a_off[q] - back, c * 64);
+    }
+  };
+  auto issue = [&](int c, int buf) {
+    issue_a(c, buf);
+    issue_w(c, buf);
+  };
+  constexpr int LOADS = C::QA + C::QB;  // of a wave and chunk
 
   const int first = wc * NJ;  // this wave's weight blocks, from b0
   const bool wave_live = first <= last_block;
@@ -181,19 +189,23 @@ __global__ __launch_bounds__(C::THREADS, C::NJ > 4 ? 1 : 2) void mx44_tile_kerne
                      min(b, last_block) * bb + quad * kMxQuadBytes);
     }
   };
+  issue_w(0, 0);
+  issue_ws(0);
+#pragma unroll
+  for (int q = 0; q < C::QA; ++q)
+    a_off[q] = static_cast<uint32_t>(source_row(a_row(q), a_pair[q])) * (K >> 1) + ((lane & 3) ^ C::sw(a_row(q))) * 16;
   // the rows' scales of a quad, as they lie: PER_ROW threads to a row
   constexpr int SB = sizeof(typename C::scales_t);
-  const uint8_t* my_scales = scale_base + (row0 + source_row(tid / C::PER_ROW)) * groups;
+  const uint8_t* my_scales = g.a_scale + (row0 + source_row(s_row, scale_pair)) * groups;
   typename C::scales_t qs;
   auto get_scales = [&](int quad) { qs = load_scales<typename C::scales_t>(my_scales, 16 * quad + tid % C::PER_ROW * SB, groups); };
   auto put_scales = [&]() { *reinterpret_cast<typename C::scales_t*>(smem + C::OFF_SCALE + tid * SB) = qs; };
-
   get_scales(0);
-  issue_ws(0);
-  if constexpr (!LIN)
-    if (tid < BM) s_pair[tid] = g.sorted_pairs[p0 + (tid < rows ? tid : 0)];
+  issue_a(0, 0);
 #pragma unroll
-  for (int c = 0; c < NB - 1; ++c) issue(c, c);
+  for (int c = 1; c < NB - 1; ++c) issue(c, c);
+  if constexpr (!LIN)
+    if (tid < BM) s_pair[tid] = my_pair;
   put_scales();
 
   f32x4_t acc[MI][NJ];
@@ -287,7 +299,7 @@ __global__ __launch_bounds__(C::THREADS, C::NJ > 4 ? 1 : 2) void mx44_tile_kerne
       if (quad + 1 < quads) get_scales(quad + 1);
     };
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    wait_vm_barrier<0>();  // chunks 0 to NB - 2, and the scales
+    wait_vm_barrier<(NB - 2) * LOADS>();  // chunk 0 and the scales
     if constexpr (NL > 0) {
       read_x(0, 0, x_at);
 #pragma unroll

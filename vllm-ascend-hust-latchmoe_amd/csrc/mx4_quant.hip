@@ -77,32 +77,54 @@ __device__ __forceinline__ void store_values(void* out, size_t at, uint32_t word
 // ---------------------------------------------------------------------------
 constexpr int kQuantThreads = 256;
 
+constexpr int kOctets = 2;  // of a lane, kQuantThreads apart, both on their way at once
+
 template <bool F32>
 __global__ __launch_bounds__(kQuantThreads) void rows_to_mx4_kernel(const void* __restrict__ x, size_t octets,
                                                                     uint32_t* __restrict__ q, uint8_t* __restrict__ scale) {
-  const size_t o = static_cast<size_t>(blockIdx.x) * kQuantThreads + threadIdx.x;  // groups are whole: quads are
-  if (o >= octets) return;
-  float v[8];
-  load_columns<F32>(x, o * 8, v);
-  const int b = group_scale_byte(v);
-  q[o] = pack_e2m1x8(v, mx_scale_f32(b), b);
-  if ((o & 3) == 0) scale[o >> 2] = static_cast<uint8_t>(b);
+  const size_t first = static_cast<size_t>(blockIdx.x) * (kOctets * kQuantThreads) + threadIdx.x;
+  float v[kOctets][8];
+#pragma unroll
+  for (int u = 0; u < kOctets; ++u) {
+    const size_t o = first + u * kQuantThreads;
+    load_columns<F32>(x, o < octets ? o * 8 : 0, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kOctets; ++u) {
+    const size_t o = first + u * kQuantThreads;
+    const int b = group_scale_byte(v[u]);
+    if (o >= octets) break;  // groups are whole: so are quads of lanes
+    q[o] = pack_e2m1x8(v[u], mx_scale_f32(b), b);
+    if ((o & 3) == 0) scale[o >> 2] = static_cast<uint8_t>(b);
+  }
 }
 
 template <bool F32>
 __global__ __launch_bounds__(kQuantThreads) void mx4_rows_values_kernel(const uint32_t* __restrict__ q,
                                                                         const uint8_t* __restrict__ scale, size_t octets,
                                                                         void* __restrict__ out) {
-  const size_t o = static_cast<size_t>(blockIdx.x) * kQuantThreads + threadIdx.x;
-  if (o >= octets) return;
-  store_values<F32>(out, o * 8, q[o], scale_value(scale[o >> 2]));
+  const size_t first = static_cast<size_t>(blockIdx.x) * (kOctets * kQuantThreads) + threadIdx.x;
+  uint32_t word[kOctets];
+  int b[kOctets];
+#pragma unroll
+  for (int u = 0; u < kOctets; ++u) {
+    const size_t o = first + u * kQuantThreads, at = o < octets ? o : 0;
+    word[u] = q[at];
+    b[u] = scale[at >> 2];
+  }
+#pragma unroll
+  for (int u = 0; u < kOctets; ++u) {
+    const size_t o = first + u * kQuantThreads;
+    if (o < octets) store_values<F32>(out, o * 8, word[u], scale_value(b[u]));
+  }
 }
 
 // ---------------------------------------------------------------------------
-// weights: a wave takes one quad (512 columns) of one block of 16 rows, four rows at a
-// time: its 16 lanes of a row have 128 columns, a chunk.  Codes go to the chunk's KiB (16
-// bytes of a group together, those of four rows side by side), the four chunks' scales of
-// a row and group are one dword.
+// weights: a workgroup takes one quad (512 columns) of one block of 16 rows, each of its
+// four waves four rows: the 16 lanes of a row have 128 columns, a chunk.  Codes go to the
+// chunk's KiB (16 bytes of a group together, those of four rows side by side), the four
+// chunks' scales of a row and group are one dword; the quad is put together in LDS and
+// leaves in whole lines.
 // ---------------------------------------------------------------------------
 struct BankArgs {
   const void* w;     // [E, N, K], or the values to write
@@ -133,61 +155,56 @@ __device__ __forceinline__ BankUnit bank_unit(const BankArgs& g, size_t unit) {
 
 template <bool F32>
 __global__ __launch_bounds__(kQuantThreads) void mx4_quantize_kernel(BankArgs g) {
-  const int lane = threadIdx.x & 63;
-  const size_t unit = static_cast<size_t>(blockIdx.x) * (kQuantThreads / 64) + (threadIdx.x >> 6);
-  if (unit >= g.units) return;
-  const BankUnit u = bank_unit(g, unit);
+  __shared__ __attribute__((aligned(16))) uint8_t s_quad[kMxQuadBytes];  // as the bank has it
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const BankUnit u = bank_unit(g, blockIdx.x);
   const int piece = lane & 15;  // eight columns of a chunk
+  const int r = 4 * wave + (lane >> 4);
+  const size_t base = (u.row0 + r) * static_cast<size_t>(g.K) + u.k0 + 8 * piece;
+  const int at = r + 16 * (piece >> 2);  // the lane that a product gives this row and group to
+  float v[4][8];
 #pragma unroll
-  for (int step = 0; step < 4; ++step) {
-    const int r = 4 * step + (lane >> 4);
-    const size_t base = (u.row0 + r) * static_cast<size_t>(g.K) + u.k0 + 8 * piece;
-    const int at = r + 16 * (piece >> 2);  // the lane that a product gives this row and group to
-    float v[4][8];
+  for (int c = 0; c < 4; ++c) {
+    const bool in = u.k0 + c * kMxChunk + 8 * piece < g.K;
+    load_columns<F32>(g.w, in ? base + c * kMxChunk : 0, v[c]);
+    if (!in) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const bool in = u.k0 + c * kMxChunk + 8 * piece < g.K;
-      load_columns<F32>(g.w, in ? base + c * kMxChunk : 0, v[c]);
-      if (!in) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[c][e] = 0.0f;
-      }
+      for (int e = 0; e < 8; ++e) v[c][e] = 0.0f;
     }
-    uint32_t scales = 0;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const bool in = u.k0 + c * kMxChunk + 8 * piece < g.K;  // the same for a group
-      const int b = in ? group_scale_byte(v[c]) : kScaleOne;
-      scales |= static_cast<uint32_t>(b) << (8 * c);
-      const uint32_t word = pack_e2m1x8(v[c], mx_scale_f32(b), b);
-      if (c < u.chunks) *reinterpret_cast<uint32_t*>(u.quad + 256 + c * 1024 + at * 16 + 4 * (piece & 3)) = word;
-    }
-    if ((piece & 3) == 0) *reinterpret_cast<uint32_t*>(u.quad + 4 * at) = scales;
   }
+  uint32_t scales = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const bool in = u.k0 + c * kMxChunk + 8 * piece < g.K;  // the same for a group
+    const int b = in ? group_scale_byte(v[c]) : kScaleOne;
+    scales |= static_cast<uint32_t>(b) << (8 * c);
+    *reinterpret_cast<uint32_t*>(s_quad + 256 + c * 1024 + at * 16 + 4 * (piece & 3)) = pack_e2m1x8(v[c], mx_scale_f32(b), b);
+  }
+  if ((piece & 3) == 0) *reinterpret_cast<uint32_t*>(s_quad + 4 * at) = scales;
+  __syncthreads();
+  if (wave == 0) *reinterpret_cast<uint32_t*>(u.quad + 4 * lane) = *reinterpret_cast<const uint32_t*>(s_quad + 4 * lane);
+  if (wave < u.chunks)
+    *reinterpret_cast<uint4*>(u.quad + 256 + wave * 1024 + 16 * lane) =
+        *reinterpret_cast<const uint4*>(s_quad + 256 + wave * 1024 + 16 * lane);
 }
 
 template <bool F32>
 __global__ __launch_bounds__(kQuantThreads) void mx4_bank_values_kernel(BankArgs g) {
-  const int lane = threadIdx.x & 63;
-  const size_t unit = static_cast<size_t>(blockIdx.x) * (kQuantThreads / 64) + (threadIdx.x >> 6);
-  if (unit >= g.units) return;
-  const BankUnit u = bank_unit(g, unit);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const BankUnit u = bank_unit(g, blockIdx.x);
   const int piece = lane & 15;
+  const int r = 4 * wave + (lane >> 4);
+  const size_t base = (u.row0 + r) * static_cast<size_t>(g.K) + u.k0 + 8 * piece;
+  const int at = r + 16 * (piece >> 2);
+  const uint32_t scales = *reinterpret_cast<const uint32_t*>(u.quad + 4 * at);
+  uint32_t word[4];
 #pragma unroll
-  for (int step = 0; step < 4; ++step) {
-    const int r = 4 * step + (lane >> 4);
-    const size_t base = (u.row0 + r) * static_cast<size_t>(g.K) + u.k0 + 8 * piece;
-    const int at = r + 16 * (piece >> 2);
-    const uint32_t scales = *reinterpret_cast<const uint32_t*>(u.quad + 4 * at);
-    uint32_t word[4];
+  for (int c = 0; c < 4; ++c)
+    word[c] = *reinterpret_cast<const uint32_t*>(u.quad + 256 + (c < u.chunks ? c : 0) * 1024 + at * 16 + 4 * (piece & 3));
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      word[c] = *reinterpret_cast<const uint32_t*>(u.quad + 256 + (c < u.chunks ? c : 0) * 1024 + at * 16 + 4 * (piece & 3));
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (u.k0 + c * kMxChunk + 8 * piece < g.K)
-        store_values<F32>(const_cast<void*>(g.w), base + c * kMxChunk, word[c], scale_value((scales >> (8 * c)) & 255));
-  }
+  for (int c = 0; c < 4; ++c)
+    if (u.k0 + c * kMxChunk + 8 * piece < g.K)
+      store_values<F32>(const_cast<void*>(g.w), base + c * kMxChunk, word[c], scale_value((scales >> (8 * c)) & 255));
 }
 
 static unsigned grid_of(size_t n, size_t per) { return static_cast<unsigned>((n + per - 1) / per); }
@@ -197,7 +214,7 @@ static int check_bank(const void* values, int E, int N, int K, int gate_up, cons
   if (E < 0 || N <= 0 || K <= 0) return LMOE_ERR_ARG;
   if (N % 16 != 0 || K % kMxGroup != 0 || (gate_up && N % 64 != 0)) return LMOE_ERR_SHAPE;
   const size_t units = static_cast<size_t>(E) * (N / 16) * ((K + 511) / 512);
-  if (units / (kQuantThreads / 64) >= 0x7fffffffull) return LMOE_ERR_SHAPE;
+  if (units >= 0x7fffffffull) return LMOE_ERR_SHAPE;
   if (E == 0) return LMOE_OK;
   if (values == nullptr || bank == nullptr) return LMOE_ERR_ARG;
   if (misaligned16(values) || misaligned16(bank)) return LMOE_ERR_SHAPE;
@@ -211,7 +228,7 @@ static int check_bank(const void* values, int E, int N, int K, int gate_up, cons
 static int check_rows(const void* values, int T, int H, const void* q, const void* scale, int f32) {
   if (T < 0 || H <= 0) return LMOE_ERR_ARG;
   const size_t n = static_cast<size_t>(T) * H;
-  if (H % kMxGroup != 0 || n / 8 / kQuantThreads >= 0x7fffffffull) return LMOE_ERR_SHAPE;
+  if (H % kMxGroup != 0 || n / 8 / (kOctets * kQuantThreads) >= 0x7fffffffull) return LMOE_ERR_SHAPE;
   if (T == 0) return LMOE_OK;
   if (values == nullptr || q == nullptr || scale == nullptr) return LMOE_ERR_ARG;
   if (misaligned16(values) || misaligned16(q)) return LMOE_ERR_SHAPE;
@@ -227,7 +244,7 @@ extern "C" int lmoe_rows_to_mx4(const void* x, int x_f32, int T, int H, void* q,
   const int st = check_rows(x, T, H, q, scale, x_f32);
   if (st != LMOE_OK || T == 0) return st;
   const size_t octets = static_cast<size_t>(T) * H / 8;
-  const unsigned grid = grid_of(octets, kQuantThreads);
+  const unsigned grid = grid_of(octets, kOctets * kQuantThreads);
   uint32_t* codes = static_cast<uint32_t*>(q);
   uint8_t* s = static_cast<uint8_t*>(scale);
   if (x_f32) rows_to_mx4_kernel<true><<<grid, kQuantThreads, 0, stream>>>(x, octets, codes, s);
@@ -240,7 +257,7 @@ extern "C" int lmoe_mx4_rows_values(const void* q, const void* scale, int T, int
   const int st = check_rows(out, T, H, q, scale, out_f32);
   if (st != LMOE_OK || T == 0) return st;
   const size_t octets = static_cast<size_t>(T) * H / 8;
-  const unsigned grid = grid_of(octets, kQuantThreads);
+  const unsigned grid = grid_of(octets, kOctets * kQuantThreads);
   const uint32_t* codes = static_cast<const uint32_t*>(q);
   const uint8_t* s = static_cast<const uint8_t*>(scale);
   if (out_f32) mx4_rows_values_kernel<true><<<grid, kQuantThreads, 0, stream>>>(codes, s, octets, out);
@@ -253,7 +270,7 @@ extern "C" int lmoe_mx4_quantize(const void* w, int w_f32, int E, int N, int K, 
   BankArgs g;
   const int st = check_bank(w, E, N, K, gate_up, bank, w_f32, &g);
   if (st != LMOE_OK || E == 0) return st;
-  const unsigned grid = grid_of(g.units, kQuantThreads / 64);
+  const unsigned grid = static_cast<unsigned>(g.units);
   if (w_f32) mx4_quantize_kernel<true><<<grid, kQuantThreads, 0, stream>>>(g);
   else mx4_quantize_kernel<false><<<grid, kQuantThreads, 0, stream>>>(g);
   LMOE_RETURN_LAUNCH();
@@ -264,7 +281,7 @@ extern "C" int lmoe_mx4_bank_values(const void* bank, int E, int N, int K, int g
   BankArgs g;
   const int st = check_bank(out, E, N, K, gate_up, bank, out_f32, &g);
   if (st != LMOE_OK || E == 0) return st;
-  const unsigned grid = grid_of(g.units, kQuantThreads / 64);
+  const unsigned grid = static_cast<unsigned>(g.units);
   if (out_f32) mx4_bank_values_kernel<true><<<grid, kQuantThreads, 0, stream>>>(g);
   else mx4_bank_values_kernel<false><<<grid, kQuantThreads, 0, stream>>>(g);
   LMOE_RETURN_LAUNCH();
