@@ -217,7 +217,7 @@ def _result(out: torch.Tensor | None, hidden) -> torch.Tensor:
         return out
     if isinstance(hidden, torch.Tensor):
         return torch.empty_like(hidden)  # half the host time of torch.empty
-    return torch.empty(hidden.shape, dtype=torch.bfloat16, device=hidden.device)
+    return hidden.q.new_empty(hidden.shape, dtype=torch.bfloat16)
 
 
 # ---------------------------------------------------------------------------

@@ -395,7 +395,7 @@ class Mx8Rows:
         return (self.q.float().unflatten(-1, (-1, mxfp4.GROUP)) * s.unsqueeze(-1)).flatten(-2)
 
 
-@dataclass(frozen=True)
+@dataclass(slots=True, eq=False)
 class Mx4Rows:
     """Rows in 4 bits: e2m1 codes, two per byte (the even column in the low half), one
     power-of-two scale per 32 columns (value[r, c] = code * 2^(scale[r, c // 32] - 127);
@@ -414,8 +414,8 @@ class Mx4Rows:
     @property
     def shape(self) -> torch.Size:
         """[R, K]: of the values, not of the bytes."""
-        q = self.q.shape
-        return torch.Size((*q[:-1], 2 * q[-1]))
+        *rows, half = self.q.shape
+        return torch.Size((*rows, 2 * half))
 
     @property
     def device(self) -> torch.device:
@@ -618,14 +618,14 @@ _BF16_OR_F32 = (torch.bfloat16, torch.float32)
 def rows_to_mx4(x: torch.Tensor, mx4: Mx4Rows | None = None, *, stream=None) -> Mx4Rows:
     """bf16 or f32 rows x [T, H] in 4 bits, H a multiple of 32: mxfp4.quantize's codes
     and scales."""
-    lib = load_library()
+    lib = _LIB or load_library()
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError("x must be a [T, H] tensor")
     here = _device_index()
     shape, dtype = x.shape, x.dtype
     if dtype not in _BF16_OR_F32:
         raise ValueError(f"x must be bf16 or f32, got {dtype}")
-    if not _fits(x, dtype, shape, here):
+    if x.get_device() != here or not x.is_contiguous():
         _refuse(x, "x", dtype)
     if mx4 is None:
         with _on(stream):
@@ -633,10 +633,11 @@ def rows_to_mx4(x: torch.Tensor, mx4: Mx4Rows | None = None, *, stream=None) -> 
     elif not isinstance(mx4, Mx4Rows):
         raise TypeError("mx4 must be Mx4Rows")
     q, scale = _take_mx4(mx4, "mx4", shape, here)
-    status = lib.lmoe_rows_to_mx4(x.data_ptr(), dtype is torch.float32, shape[0], shape[1], q.data_ptr(), scale.data_ptr(),
+    T, H = shape
+    status = lib.lmoe_rows_to_mx4(x.data_ptr(), dtype is torch.float32, T, H, q.data_ptr(), scale.data_ptr(),
                                   _stream(stream))
     if status:
-        _refuse_overlap(status, shape[1])
+        _refuse_overlap(status, H)
         _check(status, "lmoe_rows_to_mx4")
     return mx4
 
@@ -688,15 +689,16 @@ def mx4_values(mx4, out: torch.Tensor | None = None, *, columns: int | None = No
     row]; gate_up: of quantize_mx4's or pack_w13's) stand for, into out (bf16 or f32, bf16
     where none is given).  A bank without out needs its columns: rows that end within 128
     of them have the same bytes."""
-    lib = load_library()
+    lib = _LIB or load_library()
     here = _device_index()
-    rows = isinstance(mx4, Mx4Rows)
     if out is not None and (not isinstance(out, torch.Tensor) or out.dtype not in _BF16_OR_F32 or out.dim() < 2):
         raise ValueError("out must be a bf16 or f32 tensor")
+    rows = isinstance(mx4, Mx4Rows)
     if rows:
         shape = mx4.shape
-        if columns not in (None, shape[-1]) or gate_up:
+        if gate_up or columns not in (None, shape[-1]):
             raise ValueError("columns and gate_up are for banks")
+        q, scale = _take_mx4(mx4, "mx4", shape, here)
     else:
         if columns is None:
             if out is None:
@@ -706,12 +708,10 @@ def mx4_values(mx4, out: torch.Tensor | None = None, *, columns: int | None = No
         shape = (*mx4.shape[:-1], columns)
     if out is None:
         out = _new(shape, torch.bfloat16, mx4.device, stream)
-    dtype = out.dtype
-    if not _fits(out, dtype, shape, here):
-        _refuse(out, "out", dtype, tuple(shape))
-    f32 = dtype is torch.float32
+    elif out.shape != shape or out.get_device() != here or not out.is_contiguous():
+        _refuse(out, "out", out.dtype, tuple(shape))
+    f32 = out.dtype is torch.float32
     if rows:
-        q, scale = _take_mx4(mx4, "mx4", shape, here)
         status = lib.lmoe_mx4_rows_values(q.data_ptr(), scale.data_ptr(), shape[0], shape[1], out.data_ptr(), f32,
                                           _stream(stream))
     else:
@@ -731,7 +731,7 @@ def mx4_linear(x, w: torch.Tensor, out: torch.Tensor | None = None, *, bias: tor
     x [T, K] is bf16, Mx8Rows or Mx4Rows; out [T, N] bf16 (made where none is given) or
     f32; bias [N] bf16 or f32; add [T, N] bf16, which out may be.  Sums in f32, one
     rounding."""
-    lib = load_library()
+    lib = _LIB or load_library()
     bf16, f32 = torch.bfloat16, torch.float32
     here = _device_index()
     if isinstance(x, Mx4Rows):
@@ -749,12 +749,18 @@ def mx4_linear(x, w: torch.Tensor, out: torch.Tensor | None = None, *, bias: tor
             _refuse(x, "x", bf16)
     if not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise ValueError("w must be one matrix in 4 bits, [N, bytes of a row]")
-    _, N = _bank_rows(w, "w", K, here)
+    N, wide = w.shape
+    # bytes of a row of K columns: mxfp4.row_bytes
+    if wide != (K + 127) // 128 * 64 + (K + 511) // 512 * 16 or K % 32 or w.dtype is not torch.uint8 or \
+            w.get_device() != here or not w.is_contiguous():
+        _bank_rows(w, "w", K, here)
     if out is None:
         out = _new((T, N), bf16, xq.device, stream)
-    odt = f32 if out.dtype is f32 else bf16
-    if not _fits(out, odt, (T, N), here):
-        _refuse(out, "out", odt, (T, N))
+        odt = bf16
+    else:
+        odt = f32 if out.dtype is f32 else bf16
+        if not _fits(out, odt, (T, N), here):
+            _refuse(out, "out", odt, (T, N))
     pb = pa = None
     bdt = bf16
     if bias is not None:
