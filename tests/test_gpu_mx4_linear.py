@@ -245,3 +245,13 @@ def test_rows_do_not_depend_on_their_neighbours(kind):
         b[T // 2] = a[T // 2]
         ya, yb = (native.mx4_linear(make_rows(t, kind)[0], w) for t in (a, b))
         assert torch.equal(ya[T // 2], yb[T // 2])
+
+
+@pytest.mark.parametrize("kind", ["mx8", "mx4"])
+@pytest.mark.parametrize("T,K,N", [(4090, 672, 4112), (1000, 2080, 7184), (500, 2080, 7184), (2050, 544, 2064)])
+def test_tall_products(T, K, N, kind):
+    """Enough of both for the tiles of 128 and 256, with ends inside a tile and a chunk."""
+    _, native = _mods()
+    x, xv = make_rows(torch.randn((T, K), generator=torch.Generator().manual_seed(T)), kind)
+    w, wv = make_weights(N, K, N)
+    check(native.mx4_linear(x, w), xv, wv, kind)

@@ -5,7 +5,7 @@
 
 #include "gemm_lds.h"
 #include "mx4_few.h"
-#include "mx44_tile.h"
+#include "mx_tile.h"
 #include "mx4_tile.h"
 #include "spans.h"
 
@@ -100,9 +100,9 @@ static int launch_tiles(const Mx4Args& g, int block_m, hipStream_t stream) {
 
 template <bool GU>
 static int launch_tiles4(const Mx4Args& g, int block_m, hipStream_t stream) {
-  if (block_m == 64) return launch_mx44_experts<GU, Mx44Tile64x128>(g, stream);
-  if (block_m == 128) return launch_mx44_experts<GU, Mx44Tile128x256>(g, stream);
-  return launch_mx44_experts<GU, Mx44Tile256x256>(g, stream);
+  if (block_m == 64) return launch_mx_experts<GU, Tile4_64x128>(g, stream);
+  if (block_m == 128) return launch_mx_experts<GU, Tile4_128x256>(g, stream);
+  return launch_mx_experts<GU, Tile4_256x256>(g, stream);
 }
 
 // path AUTO: row tiles past this many pairs per slot, on average, of bf16, MX8 and MX4 rows

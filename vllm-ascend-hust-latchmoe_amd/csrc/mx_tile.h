@@ -1,20 +1,35 @@
-// Products of 4-bit rows with 4-bit weights in row tiles.
+// Products of MX rows (4 or 8 bits) with 4-bit weights in row tiles: the experts' products of
+// MX4 rows, and the plain product of MX4 and MX8 rows.
 //
-// A workgroup of four waves computes BM rows by 256 weight rows: gate-up 128 act columns
-// (gate and up), down 256 y columns, the plain product 256 columns.  Each wave takes all BM
-// rows and 64 weight rows (four 16-row blocks; gate-up: gate, up, gate, up of 32 act
-// columns).  A stage is 256 columns: 128 bytes of a row, which go to LDS without passing
-// through registers (two buffers, the next stage in flight under this one's products) and
-// are read there by all four waves; weights go from memory straight to registers, one stage
-// ahead, since the bank's order is the fragments' order and no two waves share any.
+// A workgroup of WR x WC waves computes BM rows by BN weight rows (gate-up: BN / 2 act
+// columns, whose gate and up blocks alternate).  K goes by in chunks of 128, the depth of
+// v_mfma_scale_f32_16x16x128; NB buffers of LDS hold a chunk of both operands each (a row's
+// chunk is 64 bytes in 4 bits, 128 in 8; a 16-row block's 1 KiB, as it lies in the bank).
+// Both go there from memory without passing through registers, NB - 1 chunks ahead, and are
+// read by all waves that share them: with the weights in registers straight from memory, as
+// few rows have them, 128 and 256 rows a wave spilled.
 //
-// LDS holds 16-byte piece p of row r at position p ^ (r / 2) % 8, which puts the sixteen
-// lanes of a read on sixteen different positions (mx4_tile.h).  A quad is two stages: its
-// scales are one dword for a lane's row and group on either side (byte c: chunk c), so the
-// matrix instruction picks its bytes without any arithmetic.  The weights' scales lie that
-// way in the bank; the rows' are transposed on their way to LDS, a quad ahead.
+// In the middle of a chunk's products each wave waits for its loads of the next chunk and
+// for the others; after that barrier the next chunk is in LDS and the buffer before this
+// one's is free: the loads for it are sent, and the last products run while the next chunk's
+// first fragments come out of LDS.  So the matrix instructions never wait for a barrier with
+// nothing to do.  No branch stands between them: past the last chunk the loads go on, out of
+// range, which fetches nothing.
 //
-// Every output adds its chunks in order, whatever BM is: the same bits.
+// LDS holds 16-byte piece p of row r at position p ^ sw(r), which puts the sixteen lanes of
+// a read on different banks.  The scales of a quad (four chunks) are one dword for a lane's
+// row and group on either side (byte c: chunk c), so the matrix instruction picks its bytes
+// without any arithmetic.  The weights' scales lie that way in the bank; the rows' are put
+// together from their 16 bytes a row.
+//
+// Bound: 256 x 256 of 4-bit rows takes 1.05 us a chunk where its products alone take 0.84
+// (7.3 PFLOP/s from registers, with values that are not zeros) and loads and reads of LDS
+// 0.75; the plain product of 4096 x 7168 x 7168 takes 110 us (3.84 PFLOP/s; without its
+// products 94, without its loads 94).  MX8 rows: 161 us (2.62 PFLOP/s; a large library
+// product of 8-bit floats with one scale reaches 2.8).  Four waves of 128 x 128 took 141 us
+// to the 123 of this shape in the same run, six buffers with one workgroup a CU were slower.
+//
+// Every output adds its chunks in order, whatever the shape is: the same bits.
 #pragma once
 
 #include "mx4_tile.h"
@@ -35,23 +50,46 @@ __device__ __forceinline__ T load_scales(const uint8_t* sp, int at, int groups) 
   return v;
 }
 
+// A lane's part of a 16 x 128 fragment of rows, from LDS; p: its row, sw: the row's.
+template <int R>
+struct TileFrag;
+template <>
+struct TileFrag<kRowsMx4> {
+  i32x4_t v;
+  __device__ __forceinline__ void read(const char* p, int lg, int sw) {
+    v = *reinterpret_cast<const i32x4_t*>(p + ((lg ^ sw) * 16));
+  }
+  __device__ __forceinline__ i32x8_t operand() const { return __builtin_shufflevector(v, v, 0, 1, 2, 3, 0, 1, 2, 3); }
+};
+template <>
+struct TileFrag<kRowsMx8> {
+  i32x4_t lo, hi;
+  __device__ __forceinline__ void read(const char* p, int lg, int sw) {
+    lo = *reinterpret_cast<const i32x4_t*>(p + ((lg ^ sw) * 16));
+    hi = *reinterpret_cast<const i32x4_t*>(p + (((4 + lg) ^ sw) * 16));
+  }
+  __device__ __forceinline__ i32x8_t operand() const { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
+};
+
 // W x^T of one chunk; B: the byte of both scales.
-template <int B>
-__device__ __forceinline__ f32x4_t mx44_step(const i32x4_t w, int ws, const i32x4_t x, int xs, f32x4_t acc) {
+template <int R, int B>
+__device__ __forceinline__ f32x4_t mx_step(const i32x4_t w, int ws, const TileFrag<R>& x, int xs, f32x4_t acc) {
   const i32x8_t a = __builtin_shufflevector(w, w, 0, 1, 2, 3, 0, 1, 2, 3);
-  const i32x8_t b = __builtin_shufflevector(x, x, 0, 1, 2, 3, 0, 1, 2, 3);
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4 /* e2m1 */, 4, B, ws, B, xs);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x.operand(), acc, 4 /* e2m1 */, R == kRowsMx8 ? 0 : 4, B, ws,
+                                                          B, xs);
 }
 
 // A workgroup's shape: WR x WC waves of MI x NJ fragments of 16 rows by 16 weight rows, NB
 // chunks of both operands in LDS.
-template <int MI_, int NJ_, int WR_, int WC_, int NB_>
-struct Mx44Shape {
-  static constexpr int MI = MI_, NJ = NJ_, WR = WR_, WC = WC_, NB = NB_;
+template <int R_, int MI_, int NJ_, int WR_, int WC_, int NB_>
+struct MxShape {
+  static constexpr int R = R_, MI = MI_, NJ = NJ_, WR = WR_, WC = WC_, NB = NB_;
   static constexpr int BM = 16 * MI * WR, BN = 16 * NJ * WC;
   static constexpr int WAVES = WR * WC, THREADS = 64 * WAVES;
-  static constexpr int QA = BM / 16 / WAVES, QB = BN / 16 / WAVES;  // load instructions of a wave and chunk: rows, weights
-  static constexpr int PART_A = BM * 64, PART_B = BN * 64, STAGE = PART_A + PART_B;
+  static constexpr int PIECES = R == kRowsMx8 ? 8 : 4;  // 16-byte pieces of a row's chunk
+  static constexpr int ROWB = 16 * PIECES, RPL = 64 / PIECES;  // its bytes; rows of a load instruction
+  static constexpr int PART_A = BM * ROWB, PART_B = BN * 64, STAGE = PART_A + PART_B;
+  static constexpr int QA = PART_A / 1024 / WAVES, QB = BN / 16 / WAVES;  // load instructions of a wave and chunk
   static constexpr int OFF_SCALE = NB * STAGE;           // a quad's scales: BM x 16 bytes of rows,
   static constexpr int OFF_WSCALE = OFF_SCALE + BM * 16;  // BN / 16 blocks of 256 of weights
   static constexpr int OFF_PAIR = OFF_WSCALE + BN * 16;
@@ -59,9 +97,11 @@ struct Mx44Shape {
   static constexpr int PER_ROW = THREADS / BM;  // threads that bring a row's scales of a quad
   using scales_t = std::conditional_t<PER_ROW == 2, uint64_t, uint32_t>;
   static_assert(PER_ROW * sizeof(scales_t) == 16);
-  static_assert(LDS <= 160 * 1024 && BM <= THREADS && QA * 16 * WAVES == BM && QB * 16 * WAVES == BN);
-  // 16-byte piece p (of four) of row r lies at position p ^ sw(r)
-  static __device__ __forceinline__ int sw(int r) { return (0x78 >> (2 * ((r >> 2) & 3))) & 3; }
+  static_assert(LDS <= 160 * 1024 && BM <= THREADS && QA * 1024 * WAVES == PART_A && QB * 16 * WAVES == BN);
+  // piece p of row r lies at position p ^ sw(r)
+  static __device__ __forceinline__ int sw(int r) {
+    return R == kRowsMx8 ? (r >> 1) & 7 : (0x78 >> (2 * ((r >> 2) & 3))) & 3;
+  }
 };
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
@@ -86,9 +126,9 @@ __device__ __forceinline__ void wait_vm_barrier() {
 }
 
 template <Op OP, class C>
-__global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(TileArgs<OP> g) {
+__global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) {
   constexpr bool GU = OP == Op::kGateUp, LIN = OP == Op::kLinear;
-  constexpr int BM = C::BM, MI = C::MI, NJ = C::NJ, NB = C::NB;
+  constexpr int R = C::R, BM = C::BM, MI = C::MI, NJ = C::NJ, NB = C::NB;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   int* s_pair = reinterpret_cast<int*>(smem + C::OFF_PAIR);
   const int tid = threadIdx.x;
@@ -135,8 +175,9 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(TileArgs<OP> g
   };
   // rows: gate-up's lie anywhere, the others' from the tile's first on
   const size_t row0 = GU ? 0 : p0;
-  const uint8_t* rows_base = uniform(static_cast<const uint8_t*>(g.a) + row_bytes<kRowsMx4>(row0, K));
-  auto a_row = [&](int q) { return (wave * C::QA + q) * 16 + lane / 4; };
+  const uint8_t* rows_base = uniform(static_cast<const uint8_t*>(g.a) + row_bytes<R>(row0, K));
+  auto a_row = [&](int q) { return (wave * C::QA + q) * C::RPL + lane / C::PIECES; };
+  auto a_piece = [&](int q) { return (lane % C::PIECES) ^ C::sw(a_row(q)); };
   int a_pair[C::QA];
 #pragma unroll
   for (int q = 0; q < C::QA; ++q) a_pair[q] = GU ? pair_of(a_row(q)) : 0;
@@ -166,10 +207,12 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(TileArgs<OP> g
   auto issue_a = [&](int c, int buf) {
 #pragma unroll
     for (int q = 0; q < C::QA; ++q) {
-      // past the row's end any codes do: the weights' are zeros there
-      const uint32_t piece = (lane & 3) ^ C::sw(a_row(q));
-      const uint32_t back = c + 1 >= chunks && piece * 32 >= tail ? piece * 16 : 0;
-      buffer_to_lds16(rows_base, c < chunks, smem + buf * C::STAGE + (wave * C::QA + q) * 1024, a_off[q] - back, c * 64);
+      // past the row's end, where the weights are zeros, columns of the chunk's first group
+      // again: what is not a number there has made the row's sums so already
+      const uint32_t piece = a_piece(q);
+      const uint32_t back = c + 1 >= chunks && piece * (128 / C::PIECES) >= tail ? piece * 16 : 0;
+      buffer_to_lds16(rows_base, c < chunks, smem + buf * C::STAGE + (wave * C::QA + q) * 1024, a_off[q] - back,
+                      c * C::ROWB);
     }
   };
   auto issue = [&](int c, int buf) {
@@ -193,7 +236,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(TileArgs<OP> g
   issue_ws(0);
 #pragma unroll
   for (int q = 0; q < C::QA; ++q)
-    a_off[q] = static_cast<uint32_t>(source_row(a_row(q), a_pair[q])) * (K >> 1) + ((lane & 3) ^ C::sw(a_row(q))) * 16;
+    a_off[q] = static_cast<uint32_t>(source_row(a_row(q), a_pair[q])) * (R == kRowsMx8 ? K : K >> 1) + a_piece(q) * 16;
   // the rows' scales of a quad, as they lie: PER_ROW threads to a row
   constexpr int SB = sizeof(typename C::scales_t);
   const uint8_t* my_scales = g.a_scale + (row0 + source_row(s_row, scale_pair)) * groups;
@@ -218,7 +261,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(TileArgs<OP> g
   const int wrow = wr * 16 * MI;  // this wave's first row
   const int live = min(MI, max(0, (rows - wrow + 15) >> 4));
   // this lane's bytes of a fragment: rows from wrow on, weights from block `first` on
-  const char* x_at = smem + (wrow + fr) * 64 + ((lg ^ C::sw(fr)) * 16);
+  const char* x_at = smem + (wrow + fr) * C::ROWB;
+  const int fsw = C::sw(fr);  // fragments start at multiples of 16 rows
   const char* w_at = smem + C::PART_A + first * 1024 + lane * 16;
   const char* s_at = smem + C::OFF_SCALE + (wrow + fr) * 16;
   const char* ws_at = smem + C::OFF_WSCALE + first * 256 + lane * 4;
@@ -230,14 +274,15 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(TileArgs<OP> g
     constexpr int NL = decltype(nl_tag)::value;
     constexpr int PAIRS = (NL + 1) / 2;
     int xs[NL > 0 ? NL : 1], ws[NJ];
-    i32x4_t w[NJ], x[2][2];  // a chunk's weights, and two fragments of rows; the next two are on their way
+    i32x4_t w[NJ];
+    TileFrag<R> x[2][2];  // with a chunk's weights two fragments of rows; the next two are on their way
     int buf = 0;
     const char* xp = x_at;  // in the chunk's buffer
     auto read_w = [&](int j, const char* p) { w[j] = *reinterpret_cast<const i32x4_t*>(p + j * 1024); };
     auto read_x = [&](int to, int pair, const char* p) {
 #pragma unroll
       for (int i = 2 * pair; i < 2 * pair + 2 && i < NL; ++i)
-        x[to][i & 1] = *reinterpret_cast<const i32x4_t*>(p + i * 1024);
+        x[to][i & 1].read(p + i * 16 * C::ROWB, lg, fsw);
     };
     // byte B of the scales: chunk c of its quad.  No branch: the products before the
     // barrier would sink behind it
@@ -270,7 +315,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(TileArgs<OP> g
           for (int j = 0; j < NJ; ++j) {
 #pragma unroll
             for (int i = 2 * p; i < 2 * p + 2 && i < NL; ++i)
-              acc[i][j] = mx44_step<B>(w[j], ws[j], x[(first_x + p) & 1][i & 1], xs[i], acc[i][j]);
+              acc[i][j] = mx_step<R, B>(w[j], ws[j], x[(first_x + p) & 1][i & 1], xs[i], acc[i][j]);
             if (p + 1 == PAIRS) {  // the next chunk's, as this one's are done with
               __builtin_amdgcn_sched_barrier(0);
               read_w(j, wn);
@@ -339,7 +384,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(TileArgs<OP> g
       if (first + j > last_block) break;
       if constexpr (GU) {
         const f32x4_t gate[2] = {acc[i][j], acc[i][j + 2]}, up[2] = {acc[i][j + 1], acc[i][j + 3]};
-        store_act<kRowsMx4>(g, p0 + r, n0 + 8 * (first + j), lane, r < rows, gate, up);
+        store_act<R>(g, p0 + r, n0 + 8 * (first + j), lane, r < rows, gate, up);
       } else if constexpr (LIN) {
         store_linear(g, p0 + r, n0 + 16 * (first + j), lane, r < rows, acc[i][j], acc[i][j + 1]);
       } else {
@@ -350,42 +395,47 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx44_tile_kernel(TileArgs<OP> g
 }
 
 // By rows and weight rows.
-using Mx44Tile256x256 = Mx44Shape<8, 4, 2, 4, 4>;
-using Mx44Tile128x256 = Mx44Shape<8, 4, 1, 4, 3>;
-using Mx44Tile128x128 = Mx44Shape<4, 4, 2, 2, 4>;
-using Mx44Tile64x128 = Mx44Shape<2, 4, 2, 2, 4>;
-using Mx44Tile64x64 = Mx44Shape<2, 2, 2, 2, 4>;
+using Tile4_256x256 = MxShape<kRowsMx4, 8, 4, 2, 4, 4>;
+using Tile4_128x256 = MxShape<kRowsMx4, 8, 4, 1, 4, 3>;
+using Tile4_128x128 = MxShape<kRowsMx4, 4, 4, 2, 2, 4>;
+using Tile4_64x128 = MxShape<kRowsMx4, 2, 4, 2, 2, 4>;
+using Tile4_64x64 = MxShape<kRowsMx4, 2, 2, 2, 2, 4>;
+using Tile8_256x256 = MxShape<kRowsMx8, 8, 4, 2, 4, 3>;
+using Tile8_128x256 = MxShape<kRowsMx8, 4, 4, 2, 4, 4>;
+using Tile8_128x128 = MxShape<kRowsMx8, 4, 4, 2, 2, 3>;
+using Tile8_64x128 = MxShape<kRowsMx8, 2, 4, 2, 2, 4>;
+using Tile8_64x64 = MxShape<kRowsMx8, 2, 2, 2, 2, 4>;
 
 template <Op OP, class C>
-int launch_mx44(const TileArgs<OP>& g, long long grid, hipStream_t stream) {
+int launch_mx(const TileArgs<OP>& g, long long grid, hipStream_t stream) {
   if (grid > 0x7fffffffLL) return LMOE_ERR_SHAPE;
   static bool raised[64] = {};  // per device: dynamic LDS past 64 KiB allowed
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return static_cast<int>(e);
   if (dev < 0 || dev >= 64 || !raised[dev]) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx44_tile_kernel<OP, C>),
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx_tile_kernel<OP, C>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return static_cast<int>(e);
     if (dev >= 0 && dev < 64) raised[dev] = true;
   }
-  mx44_tile_kernel<OP, C><<<static_cast<unsigned>(grid), C::THREADS, C::LDS, stream>>>(g);
+  mx_tile_kernel<OP, C><<<static_cast<unsigned>(grid), C::THREADS, C::LDS, stream>>>(g);
   LMOE_RETURN_LAUNCH();
 }
 
 // Experts: at most n_pairs / BM row tiles and a short one per slot.
 template <bool GU, class C>
-int launch_mx44_experts(const Mx4Args& g, hipStream_t stream) {
+int launch_mx_experts(const Mx4Args& g, hipStream_t stream) {
   constexpr int cols = GU ? C::BN / 2 : C::BN;
   const long long tiles = g.n_pairs / C::BM + (g.n_pairs < g.P ? g.n_pairs : g.P);
   const long long blocks = tiles * ((g.N + cols - 1) / cols);
-  return launch_mx44<GU ? Op::kGateUp : Op::kDown, C>(g, 8 * ((blocks + 7) / 8), stream);
+  return launch_mx<GU ? Op::kGateUp : Op::kDown, C>(g, 8 * ((blocks + 7) / 8), stream);
 }
 
 template <class C>
-int launch_mx44_linear(LinearArgs g, hipStream_t stream) {
+int launch_mx_linear(LinearArgs g, hipStream_t stream) {
   const long long grid = linear_grid(&g, C::BM, C::BN);
-  return launch_mx44<Op::kLinear, C>(g, grid, stream);
+  return launch_mx<Op::kLinear, C>(g, grid, stream);
 }
 
 }  // namespace lmoe
