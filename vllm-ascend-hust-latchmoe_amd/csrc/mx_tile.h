@@ -108,11 +108,14 @@ typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 // 16 (4) bytes a lane from base + lane_at + at to LDS, 1 KiB (256 bytes) from dst on,
 // without passing through registers.  Off: the load is out of range and fetches nothing (its
-// address is that of the first chunk or quad, inside the operand either way).
+// address is that of the first chunk or quad, inside the operand either way).  ONCE: nobody
+// reads them again.
+template <bool ONCE>
 __device__ __forceinline__ void buffer_to_lds16(const uint8_t* base, bool on, char* dst, uint32_t lane_at, int at) {
   const int range = __builtin_amdgcn_readfirstlane(on ? -1 : 0);
   const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, range, 0x00027000);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 16, lane_at, __builtin_amdgcn_readfirstlane(on ? at : 0), 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 16, lane_at, __builtin_amdgcn_readfirstlane(on ? at : 0), 0,
+                                           ONCE ? 2 /* nt */ : 0);
 }
 __device__ __forceinline__ void buffer_to_lds4(const uint8_t* base, bool on, char* dst, uint32_t lane_at, int at) {
   const int range = __builtin_amdgcn_readfirstlane(on ? -1 : 0);
@@ -140,6 +143,13 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
 
   constexpr int OUT_COLS = GU ? C::BN / 2 : C::BN;
   int slot = 0, p0, rows, n0;
+  // Experts, low tiles: weights that one row tile reads are read once.  Fetched so, from the
+  // loop on, they leave the caches to the rows (60 experts of 2048 x 1408, 22 rows each, none
+  // in a cache before: gate-up 39.4 -> 36.0 us, down 23.1 -> 21.1; 32 of 7168 x 2048 91 -> 81
+  // and 52 -> 47.4); those that two tiles read, so fetched, cost 15% more than they do now.
+  // (The first chunks too: down 22.1.  The plain product gains nothing.)
+  constexpr bool kOnce = !LIN && BM <= 64;
+  bool alone = false;
   if constexpr (LIN) {
     if (!linear_tile(g, BM, OUT_COLS, &p0, &n0)) return;
     rows = min(BM, g.T - p0);
@@ -159,10 +169,10 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
     slot = ts.slot;
     p0 = ts.p0 + (tile - ts.tile0) * BM;
     rows = min(BM, ts.p1 - p0);
+    alone = kOnce && __builtin_amdgcn_readfirstlane(ts.p1 - ts.p0) <= BM;
   }
   const int chunks = mx4_chunks(K);
   const int groups = K / kMxGroup;
-  const uint8_t* scale_base = g.a_scale;
   // the pair of the tile's row r; rows past the last repeat the first
   auto pair_of = [&](int r) -> int {
     if constexpr (LIN) return 0;
@@ -193,12 +203,12 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
   const int last_block = wblocks - 1 - b0;
   // chunk c to buffer buf; past the last chunk the same loads, out of range: they fetch
   // nothing, and what they leave there is not read
-  auto issue_w = [&](int c, int buf) {
+  auto issue_w = [&](int c, int buf, auto once) {
     const int at = (c >> 2) * kMxQuadBytes + 256 + (c & 3) * 1024;
 #pragma unroll
     for (int q = 0; q < C::QB; ++q) {
       const int b = wave * C::QB + q;
-      buffer_to_lds16(wbase, c < chunks, smem + buf * C::STAGE + C::PART_A + b * 1024, lane * 16,
+      buffer_to_lds16<decltype(once)::value>(wbase, c < chunks, smem + buf * C::STAGE + C::PART_A + b * 1024, lane * 16,
                       min(b, last_block) * bb + at);
     }
   };
@@ -211,13 +221,9 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
       // again: what is not a number there has made the row's sums so already
       const uint32_t piece = a_piece(q);
       const uint32_t back = c + 1 >= chunks && piece * (128 / C::PIECES) >= tail ? piece * 16 : 0;
-      buffer_to_lds16(rows_base, c < chunks, smem + buf * C::STAGE + (wave * C::QA + q) * 1024, a_off[q] - back,
+      buffer_to_lds16<false>(rows_base, c < chunks, smem + buf * C::STAGE + (wave * C::QA + q) * 1024, a_off[q] - back,
                       c * C::ROWB);
     }
-  };
-  auto issue = [&](int c, int buf) {
-    issue_a(c, buf);
-    issue_w(c, buf);
   };
   constexpr int LOADS = C::QA + C::QB;  // of a wave and chunk
 
@@ -232,7 +238,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
                      min(b, last_block) * bb + quad * kMxQuadBytes);
     }
   };
-  issue_w(0, 0);
+  issue_w(0, 0, std::false_type{});
   issue_ws(0);
 #pragma unroll
   for (int q = 0; q < C::QA; ++q)
@@ -246,7 +252,10 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
   get_scales(0);
   issue_a(0, 0);
 #pragma unroll
-  for (int c = 1; c < NB - 1; ++c) issue(c, c);
+  for (int c = 1; c < NB - 1; ++c) {
+    issue_a(c, c);
+    issue_w(c, c, std::false_type{});
+  }
   if constexpr (!LIN)
     if (tid < BM) s_pair[tid] = my_pair;
   put_scales();
@@ -270,7 +279,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
 
   // NL: 16-row fragments computed, a compile-time count so that the products are
   // straight-line code; rows past the tile's last are dropped at the store
-  auto main_loop = [&](auto nl_tag) {
+  auto main_loop = [&](auto nl_tag, auto once) __attribute__((always_inline)) {
     constexpr int NL = decltype(nl_tag)::value;
     constexpr int PAIRS = (NL + 1) / 2;
     int xs[NL > 0 ? NL : 1], ws[NJ];
@@ -286,7 +295,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
     };
     // byte B of the scales: chunk c of its quad.  No branch: the products before the
     // barrier would sink behind it
-    auto chunk = [&](int c, auto b_tag) {
+    auto chunk = [&](int c, auto b_tag) __attribute__((always_inline)) {
       constexpr int B = decltype(b_tag)::value;
       const int before = buf == 0 ? NB - 1 : buf - 1, next = buf + 1 == NB ? 0 : buf + 1;
       // not a constant: past what an instruction's offset reaches each would get a register
@@ -300,7 +309,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
         wait_vm_barrier<(NB - 3) * (LOADS + (B == 2 ? C::QB : 0))>();
-        issue(c + NB - 1, before);
+        issue_a(c + NB - 1, before);
+        issue_w(c + NB - 1, before, once);
         if constexpr (B == 1) issue_ws((c >> 2) + 1);
       };
       if constexpr (NL > 0) {
@@ -330,7 +340,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
       buf = next;
       xp = xn;
     };
-    auto begin_quad = [&](int quad) {
+    auto begin_quad = [&](int quad) __attribute__((always_inline)) {
       if constexpr (NL > 0) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) ws[j] = *reinterpret_cast<const int*>(ws_at + j * 256);
@@ -366,12 +376,16 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
       if (rest > 2) chunk(4 * quad + 2, std::integral_constant<int, 2>{});
     }
   };
-  if (!wave_live || live == 0) main_loop(std::integral_constant<int, 0>{});
-  else if (MI > 6 && live > 6) main_loop(std::integral_constant<int, MI>{});
-  else if (MI > 4 && live > 4) main_loop(std::integral_constant<int, MI < 6 ? MI : 6>{});
-  else if (MI > 2 && live > 2) main_loop(std::integral_constant<int, MI < 4 ? MI : 4>{});
-  else if (MI > 1 && live > 1) main_loop(std::integral_constant<int, MI < 2 ? MI : 2>{});
-  else main_loop(std::integral_constant<int, 1>{});
+  auto run = [&](auto once) __attribute__((always_inline)) {
+    if (!wave_live || live == 0) main_loop(std::integral_constant<int, 0>{}, once);
+    else if (MI > 6 && live > 6) main_loop(std::integral_constant<int, MI>{}, once);
+    else if (MI > 4 && live > 4) main_loop(std::integral_constant<int, MI < 6 ? MI : 6>{}, once);
+    else if (MI > 2 && live > 2) main_loop(std::integral_constant<int, MI < 4 ? MI : 4>{}, once);
+    else if (MI > 1 && live > 1) main_loop(std::integral_constant<int, MI < 2 ? MI : 2>{}, once);
+    else main_loop(std::integral_constant<int, 1>{}, once);
+  };
+  if (alone) run(std::integral_constant<bool, kOnce>{});
+  else run(std::false_type{});
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load writes to LDS past the workgroup's end
   if (!wave_live) return;
 
