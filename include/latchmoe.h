@@ -587,7 +587,7 @@ int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, int I, int k,
 /* The entries above for MX4 rows: x / x_scale and act / act_scale are MX4 rows (act is
  * rounded to MX4 along I between the products, which multiply 4-bit by 4-bit values,
  * exactly up to their f32 sums), act_split is 0.  Row tiles have 64, 128 or 256 rows,
- * AUTO takes them past 14 pairs per slot; they reach up to 2^33 values of x (AUTO: the
+ * AUTO takes them past 6 pairs per slot; they reach up to 2^33 values of x (AUTO: the
  * split-K kernel past that, LMOE_PATH_MFMA: LMOE_ERR_SHAPE).  Everything else is as there. */
 int lmoe_mx44_gateup_silu(const void* x, const void* x_scale, int T, int H,
                           int I, int k, const void* w13_slots, int n_slots,

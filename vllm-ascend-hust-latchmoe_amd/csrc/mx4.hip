@@ -107,7 +107,7 @@ static int launch_tiles4(const Mx4Args& g, int block_m, hipStream_t stream) {
 
 // path AUTO: row tiles past this many pairs per slot, on average, of bf16, MX8 and MX4 rows
 // (native.py has the figures)
-constexpr int kFewPairsPerSlot[3] = {4, 6, 14};
+constexpr int kFewPairsPerSlot[3] = {4, 6, 6};
 
 static bool many_pairs(int rows, int n_pairs, int P) { return n_pairs > static_cast<long long>(kFewPairsPerSlot[rows]) * P; }
 

@@ -1253,15 +1253,17 @@ MX4_ROWS_BLOCK_M = (64, 128, 256)  # and of its form for 4-bit rows
 # (1024 x 512 x 64) and 12% at 6 (4096 x 1024 x 16), of 8-bit rows 13% at 6 (1024 x 512).
 MX4_FEW_PAIRS_PER_EXPERT = 4
 MX4_FEW_PAIRS_PER_EXPERT_MX8 = 6
-# 4-bit rows (us of the captured layer, split-K / tiles of 64 rows by 128 weight rows):
-#   pairs per expert     8            12           16           24
-#   2048, 768, 128, 8    69.5 / 74.7  76.7 / 80.1  83.8 / 82.1  99.1 / 84.7
-#   2048, 1408, 60, 4    60.7 / 72.1  63.9 / 72.0  69.5 / 72.9  80.3 / 77.9
-#   4096, 1024, 16, 2    30.2 / 34.8  33.6 / 36.4  35.6 / 37.5  39.5 / 37.8
-#   7168, 2048, 32, 8    157 / 158    154 / 156    169 / 160    190 / 165
-#   1024, 512, 64, 4     23.8 / 25.6  25.0 / 26.3  26.8 / 27.3  33.9 / 29.8
-#   4096, 2048, 64, 4    163 / 170    176 / 175    189 / 179    220 / 181
-MX4_FEW_PAIRS_PER_EXPERT_MX4 = 14
+# 4-bit rows (us of the captured layer with weights that no cache holds, split-K / tiles of
+# 64 rows by 128 weight rows; one number costs 4% at most at 6 and 8 pairs but for 9% of
+# 4096 x 2048 x 64 at 6):
+#   pairs per expert     4            6            8            12           16
+#   2048, 768, 128, 8    63.9 / 65.2  71.2 / 66.3  69.4 / 66.7  77.1 / 71.1  82.8 / 72.4
+#   2048, 1408, 60, 4    55.4 / 59.1  59.4 / 61.8  59.3 / 61.1  63.7 / 62.4  70.0 / 64.1
+#   4096, 1024, 16, 2    28.3 / 30.2  29.3 / 30.7  30.3 / 30.9  34.6 / 34.6  37.4 / 35.2
+#   7168, 2048, 32, 8    129 / 130    138 / 133    144 / 133    154 / 133    168 / 141
+#   1024, 512, 64, 4     23.8 / 24.0  22.8 / 23.8  24.1 / 24.2  24.6 / 24.0  26.1 / 25.0
+#   4096, 2048, 64, 4    144 / 140    163 / 149    174 / 143    180 / 146    192 / 150
+MX4_FEW_PAIRS_PER_EXPERT_MX4 = 6
 
 
 # The longest 8-bit rows of a tile of each height: the tile keeps all their scales in LDS
@@ -1308,13 +1310,13 @@ MX4_HEIGHTS = ((32, 32, 640), (64, 100, 1024))
 # whose rows are read from LDS for twice the weights, from 110 pairs on where rows are
 # long, and where they are short up to 200 (past them the second of two tiles is nearly
 # empty as often as not).  us of the captured layer, 64 / 128 / 256 rows:
-#   pairs per slot       48               80               128              192              256
-#   2048, 768, 128, 8    95 / 100 / 103   126 / 109 / 115  156 / 140 / 134  202 / 164 / 162  252 / 206 / 222
-#   2048, 1408, 60, 4    83 / 86 / 88     107 / 94 / 98    125 / 116 / 109  161 / 132 / 130  187 / 160 / 167
-#   1024, 512, 64, 4     32 / 34 / 34     42 / 37 / 37     47 / 46 / 41     57 / 47 / 48     68 / 66 / 71
-#   7168, 2048, 32, 8    176 / 172 / 179  255 / 186 / 195  302 / 264 / 220  407 / 271 / 254  515 / 368 / 343
-#   4096, 2048, 64, 4    202 / 196 / 206  278 / 210 / 223  346 / 279 / 251  453 / 312 / 290  565 / 391 / 383
-#   4096, 1024, 16, 2    41 / 56 / 49     51 / 59 / 54     68 / 67 / 62     79 / 68 / 73     90 / 81 / 90
+#   pairs per slot       48                  80               128              192              256
+#   2048, 768, 128, 8    85.8 / 98.7 / 98.5  125 / 107 / 110  153 / 138 / 130  198 / 162 / 160  248 / 202 / 219
+#   2048, 1408, 60, 4    74.7 / 85.7 / 84.6  105 / 93 / 94    123 / 115 / 107  156 / 130 / 129  186 / 159 / 165
+#   1024, 512, 64, 4     29.9 / 34.0 / 31.7  41 / 36 / 36     47 / 46 / 41     57 / 47 / 47     67 / 66 / 72
+#   7168, 2048, 32, 8    155 / 172 / 176     255 / 185 / 191  302 / 262 / 217  406 / 266 / 251  515 / 367 / 340
+#   4096, 2048, 64, 4    176 / 193 / 199     274 / 208 / 218  346 / 277 / 247  455 / 303 / 286  566 / 390 / 381
+#   4096, 1024, 16, 2    38.3 / 55.1 / 46.8  52 / 59 / 55     66 / 66 / 64     78 / 68 / 73     89 / 82 / 88
 MX4_ROWS_LOW_PAIRS = 50
 MX4_ROWS_LOW_GROUPS = 700
 MX4_ROWS_TALL_PAIRS = (110, 200)
