@@ -464,8 +464,8 @@ int lmoe_mx4_rows_values(const void* q, const void* scale, int T, int H, void* o
 /* Weights w [E, N, K], bf16 or f32 (w_f32), as MX4 weights: bank is
  * [E, lmoe_mx4_bytes(N, K)].  gate_up: w's N rows are a gate and an up half, which
  * the bank holds in blocks of 16 rows in turn (w13).  N % 16 == 0 (N % 64 == 0 with
- * gate_up), K % 32 == 0, w and bank 16-byte aligned; else LMOE_ERR_SHAPE.  The two
- * may not overlap (LMOE_ERR_ARG). */
+ * gate_up), K % 32 == 0 up to 2^23, w and bank 16-byte aligned; else LMOE_ERR_SHAPE.
+ * The two may not overlap (LMOE_ERR_ARG). */
 int lmoe_mx4_quantize(const void* w, int w_f32, int E, int N, int K, int gate_up,
                       void* bank, hipStream_t stream);
 
@@ -479,8 +479,8 @@ int lmoe_mx4_bank_values(const void* bank, int E, int N, int K, int gate_up,
  * LMOE_ROWS_MX4.  Products are summed in f32, bias [N] (bf16 or f32, may be null) and
  * add [T, N] (bf16, may be null) are added in f32, out [T, N] is rounded once, to
  * bf16 or f32 (out_f32).  Which partial sums are added depends on the sizes, never on
- * the values.  K % 32 == 0, N % 16 == 0, operands 16-byte aligned (x_scale any); else
- * LMOE_ERR_SHAPE.  out may be add (bf16); any other overlap of out with an operand is
+ * the values.  K % 32 == 0 up to 2^23, N % 16 == 0, operands 16-byte aligned (x_scale
+ * any); else LMOE_ERR_SHAPE.  out may be add (bf16); any other overlap of out with an operand is
  * LMOE_ERR_ARG. */
 enum { LMOE_ROWS_BF16 = 0, LMOE_ROWS_MX8 = 1, LMOE_ROWS_MX4 = 2 };
 int lmoe_mx4_linear(const void* x, const void* x_scale, int rows, int T, int K,
@@ -587,8 +587,8 @@ int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, int I, int k,
 /* The entries above for MX4 rows: x / x_scale and act / act_scale are MX4 rows (act is
  * rounded to MX4 along I between the products, which multiply 4-bit by 4-bit values,
  * exactly up to their f32 sums), act_split is 0.  Row tiles have 64, 128 or 256 rows,
- * AUTO takes them past 6 pairs per slot; they reach up to 2^33 values of x (AUTO: the
- * split-K kernel past that, LMOE_PATH_MFMA: LMOE_ERR_SHAPE).  Everything else is as there. */
+ * AUTO takes them past 6 pairs per slot; they reach fewer than 2^33 values of x and rows
+ * of up to 2^23 (AUTO: the split-K kernel past that, LMOE_PATH_MFMA: LMOE_ERR_SHAPE).  Everything else is as there. */
 int lmoe_mx44_gateup_silu(const void* x, const void* x_scale, int T, int H,
                           int I, int k, const void* w13_slots, int n_slots,
                           const int32_t* offsets, const int32_t* sorted_pairs,

@@ -490,3 +490,69 @@ def test_decode_overflow_equals_one_bank(T, top_k):
         want = fused_moe.fused_experts(rows, w, ids, b13, b2, torch.arange(E, dtype=torch.int32, device="cuda"))
         torch.cuda.synchronize()
         assert torch.equal(out, want), (step, plan.overflow is not None)
+
+
+def test_rows_past_2_gib():
+    """x of more than 2^31 bytes: the last tokens' act is that of a small call, bit for bit
+    (row tiles add a row's chunks in order, whatever lies beside it)."""
+    native = _native()
+    T, H, I, P = 300_100, 16384, 32, 2
+    layer = Layer4(H, I, P, 40, 11)
+    ids = to_dev_i32(np.zeros((40, 1), np.int32))
+    perm = native.Permutation.allocate(40, P, "cuda")
+    want = layer.act_buffer(40)
+    native.permute(ids, perm, block_m=64)
+    native.gateup_silu(layer.x, 1, layer.w13, perm, want, path=native.LMOE_PATH_MFMA)
+    q = torch.zeros((T, H // 2), dtype=torch.uint8, device="cuda")
+    sc = torch.full((T, H // 32), 127, dtype=torch.uint8, device="cuda")
+    q[-40:], sc[-40:] = layer.x.q, layer.x.scale
+    act = layer.act_buffer(T)
+    perm = native.Permutation.allocate(T, P, "cuda")
+    for bm in native.MX4_ROWS_BLOCK_M:
+        native.permute(to_dev_i32(np.zeros((T, 1), np.int32)), perm, block_m=bm)
+        native.gateup_silu(native.Mx4Rows(q, sc), 1, layer.w13, perm, act, path=native.LMOE_PATH_MFMA)
+        torch.cuda.synchronize()
+        assert torch.equal(act.q[-40:], want.q) and torch.equal(act.scale[-40:], want.scale), bm
+        assert not bool(act.q[:-40].bitwise_and(0x77).any()), bm
+
+
+def test_two_threads_at_once():
+    """A thread each with a stream of its own: rows, projection and experts, over and over."""
+    import threading
+
+    from vllm_moe_offload_amd import fused_moe, mxfp4
+
+    native = _native()
+    H, I, E, k, T = 512, 96, 8, 2, 33
+    layers = [Layer4(H, I, E, T, s) for s in (21, 22)]
+    proj = [native.quantize_mx4(torch.randn((H, H), generator=torch.Generator().manual_seed(s)).cuda() * 0.05)
+            for s in (1, 2)]
+    assert proj[0].shape == (H, mxfp4.row_bytes(H))
+    ids = [to_dev_i32(np.random.default_rng(s).integers(0, E, (T, k))) for s in (1, 2)]
+    w = torch.full((T, k), 0.5, dtype=torch.bfloat16, device="cuda")
+
+    def once(i):
+        mid = native.rows_to_mx4(native.mx4_linear(layers[i].x, proj[i]))
+        return fused_moe.fused_experts(mid, w, ids[i], layers[i].w13, layers[i].w2, None)
+
+    want = [once(i) for i in (0, 1)]
+    torch.cuda.synchronize()
+    got, failed = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    got[i].append(once(i))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # reported by the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for i in (0, 1):
+        assert all(torch.equal(y, want[i]) for y in got[i])

@@ -119,3 +119,71 @@ def test_kinds_of_rows():
     assert fused_moe.rows_kind(native.Mx4Rows.allocate(3, 32, "cpu"), bank) == "mx4"
     with pytest.raises(ValueError, match="4-bit rows"):
         fused_moe.rows_kind(native.Mx4Rows.allocate(3, 32, "cpu"), x)
+
+
+def test_sizes_past_the_tiles_offsets_are_refused():
+    lib = _lib()
+    mb = 1 << 20
+    long = (1 << 23) + 32
+    x, xs, w, out = mb, 1 << 40, 1 << 41, 1 << 42
+    for rows in (0, 1, 2):
+        scale = xs if rows else None
+        assert lib.lmoe_mx4_linear(x, scale, rows, 1, long, 16, w, None, 0, None, out, 0, None) == 1001
+    assert lib.lmoe_mx4_quantize(x, 0, 1, 16, long, 0, w, None) == 1001
+    assert lib.lmoe_mx4_bank_values(w, 1, 16, long, 0, x, 0, None) == 1001
+    assert lib.lmoe_mx4_quantize(x, 0, 1 << 30, 1 << 30, 1 << 22, 0, w, None) == 1001  # 2^68 quads
+    p, N = ctypes.c_void_p(P16), None
+    i = [p] * 5
+    tiles = 2  # LMOE_PATH_MFMA
+
+    def gateup(T, H, I, block_m, path=tiles):
+        return lib.lmoe_mx44_gateup_silu(p, p, T, H, I, 1, p, 4, *i, T, block_m, path, p, p, 0, N)
+
+    assert gateup(1 << 19, 1 << 14, 64, 64) == 1001          # 2^33 values of x
+    assert gateup(64, long, 64, 64) == 1001
+    assert lib.lmoe_mx44_down(p, p, 0, 64, long, p, 4, *i, 64, 64, tiles, p, 0, N) == 1001
+    for block_m in (0, 16, 32, 96, 320, 512):                # no tile of 4-bit rows is so high
+        assert gateup(64, 64, 64, block_m) == 1001, block_m
+        assert gateup(64, 64, 64, block_m, 0) == 1001, block_m  # AUTO, where tiles are due
+        assert lib.lmoe_mx44_down(p, p, 0, 64, 64, p, 4, *i, 64, block_m, tiles, p, 0, N) == 1001, block_m
+    assert lib.lmoe_mx4_gateup_silu(p, p, 64, 64, 64, 1, p, 4, *i, 64, 256, tiles, p, p, 0, N) == 1001  # nor of 8-bit ones
+
+
+def test_path_and_height_of_4_bit_rows():
+    from vllm_moe_offload_amd import native
+
+    few, tiles = native.LMOE_PATH_GEMV, native.LMOE_PATH_MFMA
+    per = native.MX4_FEW_PAIRS_PER_EXPERT_MX4
+    assert native.mx4_path(per * 8, 8, mx4=True) == few and native.mx4_path(per * 8 + 1, 8, mx4=True) == tiles
+    assert native.mx4_path(1 << 20, 8, columns=native.MX4_MAX_COLUMNS_MX4, mx4=True) == tiles
+    assert native.mx4_path(1 << 20, 8, columns=native.MX4_MAX_COLUMNS_MX4 + 32, mx4=True) == few
+    assert native.mx4_path(1 << 20, 8, mx4=True, row_values=(1 << 33) - 2) == tiles
+    assert native.mx4_path(1 << 20, 8, mx4=True, row_values=1 << 33) == few
+    for pairs in (1, 63, 64, 500, 5_000, 33_000, 100_000, 1_000_000):
+        for experts in (1, 8, 60, 128):
+            for wide in (32, 768, 2048):
+                for columns in (64, 2048, 7168):
+                    assert native.mx4_block_m(pairs, experts, wide, mx4_columns=columns) in native.MX4_ROWS_BLOCK_M
+    # low while the card is not full, then 128; 256 where rows are long, or up to 200 pairs
+    heights = [native.mx4_block_m(n * 128, 128, 768, mx4_columns=2048) for n in (1, 50, 51, 110, 111, 200, 201)]
+    assert heights == [64, 64, 128, 128, 256, 256, 128]
+    assert native.mx4_block_m(201 * 128, 128, 768, mx4_columns=4096) == 256
+    assert native.mx4_block_m(201, 1, 768, mx4_columns=4096) == 64
+
+
+def test_python_refusals_before_any_launch():
+    """What the wrappers refuse by looking: nothing here needs a device."""
+    from vllm_moe_offload_amd import native
+
+    rows = native.Mx4Rows.allocate(2, 64, "cpu")
+    x = torch.zeros((2, 64), dtype=torch.bfloat16)
+    with pytest.raises(TypeError):
+        native._need_mx4_rows(x, "x")
+    with pytest.raises(ValueError):
+        native._need_mx4_rows(native.Mx4Rows(rows.q[:, :24], rows.scale), "x", (2, 48))
+    with pytest.raises(ValueError):
+        native._need_alike(rows, x)
+    with pytest.raises(ValueError):
+        native._need_alike(rows, native.Mx8Rows.allocate(2, 64, "cpu"))
+    native._need_alike(rows, rows)
+    native._need_alike(x, x)

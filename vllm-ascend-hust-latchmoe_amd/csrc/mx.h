@@ -32,6 +32,9 @@ constexpr int kMxGroup = 32;
 constexpr int kMxChunk = 128;                 // columns of one fragment
 constexpr int kMxQuadBytes = 256 + 4 * 1024;  // scales and four chunks
 constexpr int kScaleOne = 127;
+// Of the plain product, weights' quantisation and MX4 rows' tiles: a tile's blocks and rows
+// (256 x 2^23 values) are then within 32 bits of its first.
+constexpr int kMxMaxColumns = 1 << 23;
 
 __host__ __device__ inline int mx4_chunks(int K) { return (K + kMxChunk - 1) / kMxChunk; }
 __host__ __device__ inline int mx4_block_bytes(int K) {

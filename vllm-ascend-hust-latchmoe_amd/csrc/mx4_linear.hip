@@ -130,7 +130,7 @@ extern "C" int lmoe_mx4_linear(const void* x, const void* x_scale, int rows, int
                                hipStream_t stream) {
   if (T < 0 || K <= 0 || N <= 0) return LMOE_ERR_ARG;
   if (rows != kRowsBf16 && rows != kRowsMx8 && rows != kRowsMx4) return LMOE_ERR_UNSUPPORTED;
-  if (K % kMxGroup != 0 || N % 16 != 0) return LMOE_ERR_SHAPE;
+  if (K % kMxGroup != 0 || N % 16 != 0 || K > kMxMaxColumns) return LMOE_ERR_SHAPE;
   if (T == 0) return LMOE_OK;
   if (x == nullptr || w == nullptr || out == nullptr || (x_scale == nullptr) != (rows == kRowsBf16)) return LMOE_ERR_ARG;
   if (misaligned16(x) || misaligned16(w) || misaligned16(bias) || misaligned16(add) || misaligned16(out))

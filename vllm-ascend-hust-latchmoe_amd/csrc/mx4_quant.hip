@@ -213,8 +213,9 @@ static unsigned grid_of(size_t n, size_t per) { return static_cast<unsigned>((n 
 static int check_bank(const void* values, int E, int N, int K, int gate_up, const void* bank, int f32, BankArgs* g) {
   if (E < 0 || N <= 0 || K <= 0) return LMOE_ERR_ARG;
   if (N % 16 != 0 || K % kMxGroup != 0 || (gate_up && N % 64 != 0)) return LMOE_ERR_SHAPE;
-  const size_t units = static_cast<size_t>(E) * (N / 16) * ((K + 511) / 512);
-  if (units >= 0x7fffffffull) return LMOE_ERR_SHAPE;
+  if (K > kMxMaxColumns) return LMOE_ERR_SHAPE;
+  const size_t each = static_cast<size_t>(N / 16) * ((K + 511) / 512), units = E * each;
+  if (each >= 0x7fffffffull || units >= 0x7fffffffull) return LMOE_ERR_SHAPE;
   if (E == 0) return LMOE_OK;
   if (values == nullptr || bank == nullptr) return LMOE_ERR_ARG;
   if (misaligned16(values) || misaligned16(bank)) return LMOE_ERR_SHAPE;

@@ -419,9 +419,10 @@ int launch_tile(const TileArgs<OP>& g, long long grid, hipStream_t stream) {
   return LMOE_OK;
 }
 
-// Whether rows of K columns fit the LDS of tiles of block_m rows (MX8 rows: their scales).
+// Whether rows of K columns fit the LDS of tiles of block_m rows (MX8 rows: their scales;
+// MX4 rows: whether the tiles' offsets reach them).
 inline bool tiles_fit(int block_m, int rows, int K) {
-  if (rows == kRowsMx4) return true;
+  if (rows == kRowsMx4) return K <= kMxMaxColumns;
   const bool a8 = rows == kRowsMx8;
   const int chunks = mx4_chunks(K);
   const int lds = block_m == 32   ? (a8 ? Mx4Tile<true, 32, 2>::lds_bytes(chunks) : Mx4Tile<false, 32, 2>::lds_bytes(chunks))

@@ -775,7 +775,7 @@ def mx4_linear(x, w: torch.Tensor, out: torch.Tensor | None = None, *, bias: tor
     status = lib.lmoe_mx4_linear(xq.data_ptr(), None if xs is None else xs.data_ptr(), rows, T, K, N, w.data_ptr(), pb,
                                  bdt is f32, pa, out.data_ptr(), odt is f32, _stream(stream))
     if status:
-        if status == LMOE_ERR_ARG and T > 0:
+        if status == LMOE_ERR_ARG and T > 0 and K > 0 and N > 0:
             raise ValueError("operands overlap: out over an operand other than a bf16 add")
         _check(status, "lmoe_mx4_linear")
     return out
@@ -1269,15 +1269,18 @@ MX4_FEW_PAIRS_PER_EXPERT_MX4 = 6
 # The longest 8-bit rows of a tile of each height: the tile keeps all their scales in LDS
 # (160 KiB, less two stages of rows and the pairs).  The split-K kernel takes any.
 MX4_MAX_COLUMNS_MX8 = {32: 147200, 64: 73600, 128: 32640}
+# 4-bit rows of a tile of any height: its offsets are 32 bits wide.
+MX4_MAX_COLUMNS_MX4 = 1 << 23
 
 
 def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False, columns: int = 0, *, mx4: bool = False, row_values: int = 0) -> int:
     """The path of a layer of 4-bit experts, for every pass of it: the split-K
-    kernel for few pairs per expert (mx8, mx4: of 8-bit, 4-bit rows) and for 8-bit rows
-    too long for any row tile (columns: the longer of x's and act's) or more 4-bit rows
-    than its 32-bit offsets reach (row_values: of all tokens), row tiles past that."""
+    kernel for few pairs per expert (mx8, mx4: of 8-bit, 4-bit rows) and for rows too
+    long for any row tile (columns: the longer of x's and act's) or more 4-bit rows than
+    its 32-bit offsets reach (row_values: of all tokens), row tiles past that."""
     if mx4:
-        few = n_pairs <= MX4_FEW_PAIRS_PER_EXPERT_MX4 * n_experts or row_values // 2 > 0xFFFFFFFF
+        few = n_pairs <= MX4_FEW_PAIRS_PER_EXPERT_MX4 * n_experts or columns > MX4_MAX_COLUMNS_MX4 or \
+            row_values // 2 > 0xFFFFFFFF
         return LMOE_PATH_GEMV if few else LMOE_PATH_MFMA
     few = MX4_FEW_PAIRS_PER_EXPERT_MX8 if mx8 else MX4_FEW_PAIRS_PER_EXPERT
     if n_pairs <= few * n_experts or (mx8 and columns > MX4_MAX_COLUMNS_MX8[MX4_BLOCK_M[0]]):
