@@ -6,7 +6,12 @@
 // parts, below).  Measured, gate-up /
 // down: 7 tokens x 8 of 64 experts, 7168 x 2048, MX8 rows 94 / 49 us (561 / 281 MB at
 // 6.0 / 5.7 TB/s); 16 x 8 of 128, 2048 x 768, bf16 rows 16.6 / 10.6 us (66 / 33 MB at
-// 4.0 / 3.1 TB/s: the start and the longest slot's passes of so short a kernel).
+// 4.0 / 3.1 TB/s: the start and the longest slot's passes of so short a kernel); MX4 rows
+// 97 / 49 us and, the experts drawn unevenly, 13.0 / 8.4 (55 / 28 MB; reading 54 and 33 MB
+// and nothing else takes 9.7 and 6.6 us).  MX4 rows, measured and not kept: the first
+// chunk's weights sent before the rows' addresses are known (down 8.4 -> 7.5, gate-up of 16
+// experts of 4096 x 1024 17.3 -> 18.0, elsewhere within 2%), weights a chunk ahead of the
+// products (13.7 / 10.0), 2 or 4 chunks at a time.
 //
 // A workgroup computes 64 weight rows, four 16-row blocks, for one slot: 32 act
 // columns (gate and up) or 64 y columns.  Its waves split the row's K between them,
@@ -16,7 +21,8 @@
 //
 // The matrix instruction's first operand is the weights, so a lane's four
 // results are four neighbouring output columns of one row (lane l: row l % 16,
-// columns 4 (l / 16)..).  MX8 rows: v_mfma_scale_f32_16x16x128_f8f6f4 multiplies
+// columns 4 (l / 16)..).  MX4 rows: e2m1 by e2m1, a lane group's 32 columns on either side
+// as they lie, one instruction for 128 columns.  MX8 rows: v_mfma_scale_f32_16x16x128_f8f6f4 multiplies
 // e2m1 by e4m3 with both groups' scales; its e4m3 operand holds columns 16 g..
 // and 64 + 16 g.. of a chunk in lane group g = l / 16, while scales and the e2m1
 // operand go by columns 32 g...  It adds the products of 8 neighbouring columns in

@@ -1,6 +1,7 @@
 // One matrix of 4-bit weights: y = x W^T (+ bias) (+ add).
 //
-// Rows are bf16, MX8 or MX4; weights one slot of a bank in order (mx.h), sums in f32.
+// Rows are bf16, MX8 or MX4; weights one slot of a bank in order (mx.h).  Sums, bias and add
+// are in f32 and are rounded once, to out's type.
 #pragma once
 
 #include "mx4_few.h"
@@ -70,7 +71,9 @@ __device__ __forceinline__ void store_linear(const LinearArgs& g, int row, int n
 
 // Few rows: a workgroup takes RB blocks of 16 columns by NF fragments of 16 rows; its NW
 // waves split K, U chunks' loads at a time, and their partial sums are added in LDS in wave
-// order.
+// order.  Bound by the weights' bytes and, below some 20 MB of them, by the launch: 1 x 2048 x
+// 5120 of MX4 rows 4.0 us (an empty launch 2.1), 1 x 2048 x 50000 11.1 (54 MB; reading them
+// and nothing else 9.7), 16 bf16 rows there 13.6 with 3.2 MB of f32 sums to write.
 template <int R, int RB, int NF, int NW, int U>
 __global__ __launch_bounds__(NW * 64) void mx4_linear_few_kernel(LinearArgs g) {
   __shared__ f32x4_t s_part[NW * RB * NF * 64];

@@ -9,7 +9,10 @@
 // Everything here reads its input once and writes its output once; what bounds it is HBM.
 // A lane takes eight neighbouring columns (one 16-byte load of bf16 values, one dword of
 // codes), so that both sides of a wave's access are whole lines; four neighbouring lanes
-// hold a group, and its maximum goes by two quad permutes.
+// hold a group, and its maximum goes by two quad permutes.  Measured, there / back (a copy
+// of 1 GiB here: 5.05 TB/s): rows 4096 x 7168 11.9 / 14.4 us, 4096 x 2048 3.8 / 6.4, one row
+// 2.1 / 2.1 (an empty launch); banks of 128 x 1536 x 2048 186 / 185 us (5.5 TB/s), 32 x 4096
+// x 7168 431 / 427.
 #include <hip/hip_runtime.h>
 
 #include "mx.h"
@@ -76,7 +79,6 @@ __device__ __forceinline__ void store_values(void* out, size_t at, uint32_t word
 // rows: groups and their scales lie one after the other, whatever the row length is
 // ---------------------------------------------------------------------------
 constexpr int kQuantThreads = 256;
-
 constexpr int kOctets = 2;  // of a lane, kQuantThreads apart, both on their way at once
 
 template <bool F32>
@@ -124,7 +126,8 @@ __global__ __launch_bounds__(kQuantThreads) void mx4_rows_values_kernel(const ui
 // four waves four rows: the 16 lanes of a row have 128 columns, a chunk.  Codes go to the
 // chunk's KiB (16 bytes of a group together, those of four rows side by side), the four
 // chunks' scales of a row and group are one dword; the quad is put together in LDS and
-// leaves in whole lines.
+// leaves in whole lines (straight from the lanes, a dword each, 128 x 1536 x 2048 took 222
+// us to 186).
 // ---------------------------------------------------------------------------
 struct BankArgs {
   const void* w;     // [E, N, K], or the values to write
