@@ -221,7 +221,10 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
       // again: what is not a number there has made the row's sums so already
       const uint32_t piece = a_piece(q);
       const uint32_t back = c + 1 >= chunks && piece * (128 / C::PIECES) >= tail ? piece * 16 : 0;
-      buffer_to_lds16<false>(rows_base, c < chunks, smem + buf * C::STAGE + (wave * C::QA + q) * 1024, a_off[q] - back,
+      // Experts: rows past the tile's last, whose sums are dropped, are not fetched (tiles of
+      // 256, 4096 tokens x 8 of 128 experts, 2048 x 768: 95 -> 93 us, down 85 -> 81).  Products
+      // of MX8 rows have no registers left for it, and one such tile a column.
+      buffer_to_lds16<false>(rows_base, c < chunks && (LIN || (wave * C::QA + q) * C::RPL < rows), smem + buf * C::STAGE + (wave * C::QA + q) * 1024, a_off[q] - back,
                       c * C::ROWB);
     }
   };

@@ -1313,13 +1313,13 @@ MX4_HEIGHTS = ((32, 32, 640), (64, 100, 1024))
 # whose rows are read from LDS for twice the weights, from 110 pairs on where rows are
 # long, and where they are short up to 200 (past them the second of two tiles is nearly
 # empty as often as not).  us of the captured layer, 64 / 128 / 256 rows:
-#   pairs per slot       48                  80               128              192              256
-#   2048, 768, 128, 8    85.8 / 98.7 / 98.5  125 / 107 / 110  153 / 138 / 130  198 / 162 / 160  248 / 202 / 219
-#   2048, 1408, 60, 4    74.7 / 85.7 / 84.6  105 / 93 / 94    123 / 115 / 107  156 / 130 / 129  186 / 159 / 165
-#   1024, 512, 64, 4     29.9 / 34.0 / 31.7  41 / 36 / 36     47 / 46 / 41     57 / 47 / 47     67 / 66 / 72
-#   7168, 2048, 32, 8    155 / 172 / 176     255 / 185 / 191  302 / 262 / 217  406 / 266 / 251  515 / 367 / 340
-#   4096, 2048, 64, 4    176 / 193 / 199     274 / 208 / 218  346 / 277 / 247  455 / 303 / 286  566 / 390 / 381
-#   4096, 1024, 16, 2    38.3 / 55.1 / 46.8  52 / 59 / 55     66 / 66 / 64     78 / 68 / 73     89 / 82 / 88
+#   pairs per slot       48               80               128              192              256
+#   2048, 768, 128, 8    86 / 97 / 98     125 / 107 / 110  154 / 138 / 128  198 / 160 / 156  248 / 201 / 212
+#   2048, 1408, 60, 4    75 / 85 / 84     104 / 92 / 94    124 / 114 / 105  156 / 129 / 126  186 / 158 / 160
+#   1024, 512, 64, 4     30.0 / 33.7 / 32.441 / 35.7 / 35.3 47 / 46 / 40     58 / 46 / 48     67 / 64 / 69
+#   7168, 2048, 32, 8    154 / 169 / 174  255 / 183 / 190  304 / 259 / 214  407 / 266 / 249  515 / 367 / 324
+#   4096, 2048, 64, 4    177 / 191 / 198  275 / 206 / 219  345 / 274 / 243  454 / 301 / 281  565 / 392 / 374
+#   4096, 1024, 16, 2    37.7 / 54 / 46   52 / 59 / 55     67 / 65 / 62     78 / 67 / 72     89 / 81 / 86
 MX4_ROWS_LOW_PAIRS = 50
 MX4_ROWS_LOW_GROUPS = 700
 MX4_ROWS_TALL_PAIRS = (110, 200)
