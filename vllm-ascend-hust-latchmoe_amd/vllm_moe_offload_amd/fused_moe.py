@@ -271,7 +271,12 @@ def _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2
         ws = call_workspace(T, k, P, H, w13_slots.shape[1] // 2, hidden.device, rows=rows_kind(hidden, w13_slots))
     if ws.mx4 is None:
         raise ValueError("a workspace for 4-bit experts is made with get_workspace(rows=rows_kind(hidden, w13_slots))")
-    dst = _result(out, hidden) if workspace is None or out is not None else ws.out[:T]
+    if out is not None:
+        dst = out
+    elif workspace is None:
+        dst = torch.empty_like(ws.out) if T > 0 else _result(None, hidden)  # half the host time of torch.empty
+    else:
+        dst = ws.out[:T]
     I = w13_slots.shape[1] // 2
     mx8, mx4 = isinstance(hidden, native.Mx8Rows), isinstance(hidden, native.Mx4Rows)
     if path == native.LMOE_PATH_AUTO:

@@ -321,6 +321,11 @@ def _stream(stream: torch.cuda.Stream | None) -> int:
     return int(s.cuda_stream)
 
 
+def _stream_on(stream: torch.cuda.Stream | None, here: int) -> int:
+    """_stream where the current device is known."""
+    return _raw_stream(here) if stream is None and _raw_stream is not None else _stream(stream)
+
+
 def current_stream_handle(device_index: int) -> int:
     """The raw handle of a device's current stream (0: the default stream)."""
     if _raw_stream is not None:
@@ -491,11 +496,15 @@ def _take_mx8(rows, name: str, shape, here: int) -> tuple[torch.Tensor, torch.Te
     return q, scale
 
 
+_U8, _BF16, _F32 = torch.uint8, torch.bfloat16, torch.float32
+
+
 def _take_mx4(rows, name: str, shape, here: int) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of 4-bit rows [T, K] on device here."""
     q, scale = rows.q, rows.scale
-    if not (shape[1] % 32 == 0 and _fits(q, torch.uint8, (shape[0], shape[1] // 2), here) and
-            _fits(scale, torch.uint8, (shape[0], shape[1] // 32), here)):
+    T, K = shape
+    if q.shape != (T, K >> 1) or scale.shape != (T, K >> 5) or K & 31 or q.dtype is not _U8 or scale.dtype is not _U8 or \
+            q.get_device() != here or scale.get_device() != here or not (q.is_contiguous() and scale.is_contiguous()):
         _need_mx4_rows(rows, name, tuple(shape))
         _same_device(q, scale)
     return q, scale
@@ -612,7 +621,7 @@ def rows_to_mx8(x: torch.Tensor, mx8: Mx8Rows | None = None, *, stream=None) -> 
     return mx8
 
 
-_BF16_OR_F32 = (torch.bfloat16, torch.float32)
+_BF16_OR_F32 = (_BF16, _F32)
 
 
 def rows_to_mx4(x: torch.Tensor, mx4: Mx4Rows | None = None, *, stream=None) -> Mx4Rows:
@@ -634,8 +643,8 @@ def rows_to_mx4(x: torch.Tensor, mx4: Mx4Rows | None = None, *, stream=None) -> 
         raise TypeError("mx4 must be Mx4Rows")
     q, scale = _take_mx4(mx4, "mx4", shape, here)
     T, H = shape
-    status = lib.lmoe_rows_to_mx4(x.data_ptr(), dtype is torch.float32, T, H, q.data_ptr(), scale.data_ptr(),
-                                  _stream(stream))
+    status = lib.lmoe_rows_to_mx4(x.data_ptr(), dtype is _F32, T, H, q.data_ptr(), scale.data_ptr(),
+                                  _stream_on(stream, here))
     if status:
         _refuse_overlap(status, H)
         _check(status, "lmoe_rows_to_mx4")
@@ -695,8 +704,9 @@ def mx4_values(mx4, out: torch.Tensor | None = None, *, columns: int | None = No
         raise ValueError("out must be a bf16 or f32 tensor")
     rows = isinstance(mx4, Mx4Rows)
     if rows:
-        shape = mx4.shape
-        if gate_up or columns not in (None, shape[-1]):
+        T, half = mx4.q.shape
+        shape = (T, 2 * half)
+        if gate_up or columns is not None and columns != shape[1]:
             raise ValueError("columns and gate_up are for banks")
         q, scale = _take_mx4(mx4, "mx4", shape, here)
     else:
@@ -710,13 +720,12 @@ def mx4_values(mx4, out: torch.Tensor | None = None, *, columns: int | None = No
         out = _new(shape, torch.bfloat16, mx4.device, stream)
     elif out.shape != shape or out.get_device() != here or not out.is_contiguous():
         _refuse(out, "out", out.dtype, tuple(shape))
-    f32 = out.dtype is torch.float32
+    f32 = out.dtype is _F32
+    st = _stream_on(stream, here)
     if rows:
-        status = lib.lmoe_mx4_rows_values(q.data_ptr(), scale.data_ptr(), shape[0], shape[1], out.data_ptr(), f32,
-                                          _stream(stream))
+        status = lib.lmoe_mx4_rows_values(q.data_ptr(), scale.data_ptr(), *shape, out.data_ptr(), f32, st)
     else:
-        status = lib.lmoe_mx4_bank_values(mx4.data_ptr(), E, N, columns, bool(gate_up), out.data_ptr(), f32,
-                                          _stream(stream))
+        status = lib.lmoe_mx4_bank_values(mx4.data_ptr(), E, N, columns, bool(gate_up), out.data_ptr(), f32, st)
     if status:
         _refuse_overlap(status, shape[-1])
         _check(status, "lmoe_mx4_rows_values" if rows else "lmoe_mx4_bank_values")
@@ -732,48 +741,50 @@ def mx4_linear(x, w: torch.Tensor, out: torch.Tensor | None = None, *, bias: tor
     f32; bias [N] bf16 or f32; add [T, N] bf16, which out may be.  Sums in f32, one
     rounding."""
     lib = _LIB or load_library()
-    bf16, f32 = torch.bfloat16, torch.float32
     here = _device_index()
     if isinstance(x, Mx4Rows):
-        T, K = shape = x.shape
-        (xq, xs), rows = _take_mx4(x, "x", shape, here), 2
+        T, half = x.q.shape
+        K = 2 * half
+        (xq, xs), rows = _take_mx4(x, "x", (T, K), here), 2
+        px = xs.data_ptr()
     elif isinstance(x, Mx8Rows):
         T, K = shape = x.shape
         (xq, xs), rows = _take_mx8(x, "x", shape, here), 1
+        px = xs.data_ptr()
     else:
         if not isinstance(x, torch.Tensor) or x.dim() != 2:
             raise ValueError("x must be rows [T, K]: bf16, Mx8Rows or Mx4Rows")
-        T, K = shape = x.shape
-        xq, xs, rows = x, None, 0
-        if not _fits(x, bf16, shape, here):
-            _refuse(x, "x", bf16)
+        T, K = x.shape
+        xq, px, rows = x, None, 0
+        if x.dtype is not _BF16 or x.get_device() != here or not x.is_contiguous():
+            _refuse(x, "x", _BF16)
     if not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise ValueError("w must be one matrix in 4 bits, [N, bytes of a row]")
     N, wide = w.shape
     # bytes of a row of K columns: mxfp4.row_bytes
-    if wide != (K + 127) // 128 * 64 + (K + 511) // 512 * 16 or K % 32 or w.dtype is not torch.uint8 or \
+    if wide != (K + 127) // 128 * 64 + (K + 511) // 512 * 16 or K & 31 or w.dtype is not _U8 or \
             w.get_device() != here or not w.is_contiguous():
         _bank_rows(w, "w", K, here)
+    wide_out = False
     if out is None:
-        out = _new((T, N), bf16, xq.device, stream)
-        odt = bf16
+        out = _new((T, N), _BF16, xq.device, stream)
     else:
-        odt = f32 if out.dtype is f32 else bf16
-        if not _fits(out, odt, (T, N), here):
-            _refuse(out, "out", odt, (T, N))
+        wide_out = out.dtype is _F32
+        if not _fits(out, _F32 if wide_out else _BF16, (T, N), here):
+            _refuse(out, "out", _F32 if wide_out else _BF16, (T, N))
     pb = pa = None
-    bdt = bf16
+    wide_bias = False
     if bias is not None:
-        bdt = f32 if bias.dtype is f32 else bf16
-        if not _fits(bias, bdt, (N,), here):
-            _refuse(bias, "bias", bdt, (N,))
+        wide_bias = bias.dtype is _F32
+        if not _fits(bias, _F32 if wide_bias else _BF16, (N,), here):
+            _refuse(bias, "bias", _F32 if wide_bias else _BF16, (N,))
         pb = bias.data_ptr()
     if add is not None:
-        if not _fits(add, bf16, (T, N), here):
-            _refuse(add, "add", bf16, (T, N))
+        if not _fits(add, _BF16, (T, N), here):
+            _refuse(add, "add", _BF16, (T, N))
         pa = add.data_ptr()
-    status = lib.lmoe_mx4_linear(xq.data_ptr(), None if xs is None else xs.data_ptr(), rows, T, K, N, w.data_ptr(), pb,
-                                 bdt is f32, pa, out.data_ptr(), odt is f32, _stream(stream))
+    status = lib.lmoe_mx4_linear(xq.data_ptr(), px, rows, T, K, N, w.data_ptr(), pb, wide_bias, pa, out.data_ptr(), wide_out,
+                                 _stream_on(stream, here))
     if status:
         if status == LMOE_ERR_ARG and T > 0 and K > 0 and N > 0:
             raise ValueError("operands overlap: out over an operand other than a bf16 add")
@@ -1316,7 +1327,7 @@ MX4_HEIGHTS = ((32, 32, 640), (64, 100, 1024))
 #   pairs per slot       48               80               128              192              256
 #   2048, 768, 128, 8    86 / 97 / 98     125 / 107 / 110  154 / 138 / 128  198 / 160 / 156  248 / 201 / 212
 #   2048, 1408, 60, 4    75 / 85 / 84     104 / 92 / 94    124 / 114 / 105  156 / 129 / 126  186 / 158 / 160
-#   1024, 512, 64, 4     30.0 / 33.7 / 32.441 / 35.7 / 35.3 47 / 46 / 40     58 / 46 / 48     67 / 64 / 69
+#   1024, 512, 64, 4     30 / 34 / 32     41 / 36 / 35     47 / 46 / 40      58 / 46 / 48     67 / 64 / 69
 #   7168, 2048, 32, 8    154 / 169 / 174  255 / 183 / 190  304 / 259 / 214  407 / 266 / 249  515 / 367 / 324
 #   4096, 2048, 64, 4    177 / 191 / 198  275 / 206 / 219  345 / 274 / 243  454 / 301 / 281  565 / 392 / 374
 #   4096, 1024, 16, 2    37.7 / 54 / 46   52 / 59 / 55     67 / 65 / 62     78 / 67 / 72     89 / 81 / 86
@@ -1771,7 +1782,7 @@ class Mx4Buffers:
 
 def _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, bufs: Mx4Buffers, out, add):
     """Check a layer call over 4-bit banks; (x values, scales, T, k, table length)."""
-    bf16, i32, u8 = torch.bfloat16, torch.int32, torch.uint8
+    bf16, i32, u8 = _BF16, torch.int32, _U8
     here = _device_index()
     if bufs.device_index != here:
         raise ValueError(f"buffers on cuda:{bufs.device_index}, the current device is cuda:{here}")
@@ -1791,16 +1802,17 @@ def _mx4_layer_args(x, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, buf
         _need_alike(x, bufs.act)
     if T * k != bufs.perm.n_pairs:
         raise ValueError(f"buffers for {bufs.perm.n_pairs} pairs, got {T * k}")
-    if not _fits(topk_weights, bf16, pairs, here):
-        _refuse(topk_weights, "topk_weights", bf16, pairs)
-    if not _fits(topk_ids, i32, pairs, here):
-        _refuse(topk_ids, "topk_ids", i32, pairs)
-    if not _fits(w13_slots, u8, bufs.w13_shape, here):
-        _refuse(w13_slots, "w13_slots", u8, bufs.w13_shape)
-    if not _fits(w2_slots, u8, bufs.w2_shape, here):
-        _refuse(w2_slots, "w2_slots", u8, bufs.w2_shape)
-    if not _fits(out, bf16, rows, here):
-        _refuse(out, "out", bf16, rows)
+    if topk_weights.dtype is not bf16 or topk_ids.dtype is not i32 or w13_slots.dtype is not u8 or \
+            w2_slots.dtype is not u8 or out.dtype is not bf16 or topk_weights.shape != pairs or out.shape != rows or \
+            w13_slots.shape != bufs.w13_shape or w2_slots.shape != bufs.w2_shape or \
+            not here == topk_weights.get_device() == topk_ids.get_device() == w13_slots.get_device() == \
+            w2_slots.get_device() == out.get_device() or \
+            not (topk_weights.is_contiguous() and topk_ids.is_contiguous() and w13_slots.is_contiguous() and
+                 w2_slots.is_contiguous() and out.is_contiguous()):
+        for t, name, dtype, shape in ((topk_weights, "topk_weights", bf16, pairs), (topk_ids, "topk_ids", i32, pairs),
+                                      (w13_slots, "w13_slots", u8, bufs.w13_shape),
+                                      (w2_slots, "w2_slots", u8, bufs.w2_shape), (out, "out", bf16, rows)):
+            _refuse(t, name, dtype, shape)
     if add is not None and not _fits(add, bf16, rows, here):
         _refuse(add, "add", bf16, rows)
     n_table = 0
