@@ -164,9 +164,9 @@ def test_path_and_height_of_4_bit_rows():
             for wide in (32, 768, 2048):
                 for columns in (64, 2048, 7168):
                     assert native.mx4_block_m(pairs, experts, wide, mx4_columns=columns) in native.MX4_ROWS_BLOCK_M
-    # low while the card is not full, then 128; 256 where rows are long, or up to 200 pairs
-    heights = [native.mx4_block_m(n * 128, 128, 768, mx4_columns=2048) for n in (1, 50, 51, 110, 111, 200, 201)]
-    assert heights == [64, 64, 128, 128, 256, 256, 128]
+    # low while the card is not full, then 128, 256 where rows are long
+    assert [native.mx4_block_m(n * 128, 128, 768, mx4_columns=2048) for n in (1, 50, 51, 300)] == [64, 64, 128, 128]
+    assert [native.mx4_block_m(n * 32, 32, 2048, mx4_columns=7168) for n in (1, 50, 51, 300)] == [64, 64, 256, 256]
     assert native.mx4_block_m(201 * 128, 128, 768, mx4_columns=4096) == 256
     assert native.mx4_block_m(201, 1, 768, mx4_columns=4096) == 64
 

@@ -1320,10 +1320,10 @@ def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False, columns: int = 0, 
 #                        100                325 / 262 / 247
 MX4_HEIGHTS = ((32, 32, 640), (64, 100, 1024))
 # Heights of 4-bit rows' tiles.  64 rows (by 128 weight rows) up to this many pairs per
-# slot, on average, or this many gate-up workgroups; 128 rows (by 256); 256 rows (by 256),
-# whose rows are read from LDS for twice the weights, from 110 pairs on where rows are
-# long, and where they are short up to 200 (past them the second of two tiles is nearly
-# empty as often as not).  us of the captured layer, 64 / 128 / 256 rows:
+# slot, on average, or this many gate-up workgroups (shorter rows; longer ones).  Past them
+# long rows go in tiles of 256 rows (by 256), whose weights are read half as often, short
+# ones in tiles of 128 (by 256), of which fewer are nearly empty.  us of the captured layer,
+# 64 / 128 / 256 rows, experts drawn evenly:
 #   pairs per slot       48               80               128              192              256
 #   2048, 768, 128, 8    86 / 97 / 98     125 / 107 / 110  154 / 138 / 128  198 / 160 / 156  248 / 201 / 212
 #   2048, 1408, 60, 4    75 / 85 / 84     104 / 92 / 94    124 / 114 / 105  156 / 129 / 126  186 / 158 / 160
@@ -1331,10 +1331,15 @@ MX4_HEIGHTS = ((32, 32, 640), (64, 100, 1024))
 #   7168, 2048, 32, 8    154 / 169 / 174  255 / 183 / 190  304 / 259 / 214  407 / 266 / 249  515 / 367 / 324
 #   4096, 2048, 64, 4    177 / 191 / 198  275 / 206 / 219  345 / 274 / 243  454 / 301 / 281  565 / 392 / 374
 #   4096, 1024, 16, 2    37.7 / 54 / 46   52 / 59 / 55     67 / 65 / 62     78 / 67 / 72     89 / 81 / 86
+# drawn unevenly:  7168, 2048, 32, 8 (55 pairs, 63, 84)       193 / 221 / 186  195 / 222 / 186  234 / 232 / 216
+#                  2048, 768, 128, 8 (69, 173)                98 / 111 / 116   190 / 157 / 165
+#                  2048, 1408, 60, 4 (136, 259)               127 / 114 / 119  201 / 164 / 160
+#   (workgroups)   512, 736, 21, 6 (828)                      26 / 31 / 35
+#                  2112, 1312, 16, 4 (840)                    46 / 50 / 53
+#                  1120, 992, 32, 7 (1700)                    55 / 51 / 57
 MX4_ROWS_LOW_PAIRS = 50
-MX4_ROWS_LOW_GROUPS = 700
-MX4_ROWS_TALL_PAIRS = (110, 200)
-MX4_ROWS_TALL_COLUMNS = 4096
+MX4_ROWS_LOW_GROUPS = (900, 700)
+MX4_ROWS_LONG_COLUMNS = 4096
 
 
 def mx4_block_m(n_pairs: int, n_experts: int, intermediate: int = 1024, mx8_columns: int = 0, *,
@@ -1344,11 +1349,10 @@ def mx4_block_m(n_pairs: int, n_experts: int, intermediate: int = 1024, mx8_colu
     the longer of x's and act's rows, where they are in 8 bits; mx4_columns: in 4 bits."""
     if mx4_columns:
         groups = (n_pairs // 64 + n_experts) * -(-intermediate // 64)
-        if n_pairs <= MX4_ROWS_LOW_PAIRS * n_experts or groups <= MX4_ROWS_LOW_GROUPS:
+        long = mx4_columns >= MX4_ROWS_LONG_COLUMNS
+        if n_pairs <= MX4_ROWS_LOW_PAIRS * n_experts or groups <= MX4_ROWS_LOW_GROUPS[long]:
             return 64
-        tall = n_pairs > MX4_ROWS_TALL_PAIRS[0] * n_experts and \
-            (mx4_columns >= MX4_ROWS_TALL_COLUMNS or n_pairs <= MX4_ROWS_TALL_PAIRS[1] * n_experts)
-        return 256 if tall else 128
+        return 256 if long else 128
     best = MX4_BLOCK_M[-1]
     for bm, pairs, groups in MX4_HEIGHTS:
         if n_pairs <= pairs * n_experts or (n_pairs // bm + n_experts) * -(-intermediate // 128) <= groups:
