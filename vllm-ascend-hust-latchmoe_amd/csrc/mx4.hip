@@ -163,10 +163,10 @@ static bool unlike(int rows, const void* x_scale, const void* act_scale) {
 // The kind of rows of the entries that take bf16 rows or, with scales, MX8 ones.
 static int kind_of(const void* scale) { return scale != nullptr ? kRowsMx8 : kRowsBf16; }
 
-static int gateup_silu(int rows, const void* x, const void* x_scale, int T, int H, int I, int k, const void*
-                       w13_slots, int n_slots, const int32_t* offsets, const int32_t* sorted_pairs, const int32_t*
-                       active, const int32_t* tile_off, const int32_t* meta, int n_pairs, int block_m, int path,
-                       void* act, void* act_scale, int act_split, hipStream_t stream) {
+static int gateup_silu(int rows, const void* x, const void* x_scale, int T, int H, int I, int k,
+                       const void* w13_slots, int n_slots, const int32_t* offsets, const int32_t* sorted_pairs,
+                       const int32_t* active, const int32_t* tile_off, const int32_t* meta, int n_pairs, int block_m,
+                       int path, void* act, void* act_scale, int act_split, hipStream_t stream) {
   if (T < 0 || H <= 0 || I <= 0 || k <= 0 || n_slots <= 0 || n_pairs < 0) return LMOE_ERR_ARG;
   if (n_pairs != static_cast<long long>(T) * k) return LMOE_ERR_ARG;
   if (H % kMxGroup != 0 || I % kMxGroup != 0 || n_slots > kMaxSlots) return LMOE_ERR_SHAPE;
@@ -183,10 +183,10 @@ static int gateup_silu(int rows, const void* x, const void* x_scale, int T, int 
   return launch<true>(g, path, block_m, stream);
 }
 
-static int down(int rows, const void* act, const void* act_scale, int act_split, int H, int I, const void*
-                w2_slots, int n_slots, const int32_t* offsets, const int32_t* sorted_pairs, const int32_t* active,
-                const int32_t* tile_off, const int32_t* meta, int n_pairs, int block_m, int path, void* y, int
-                y_f32, hipStream_t stream) {
+static int down(int rows, const void* act, const void* act_scale, int act_split, int H, int I, const void* w2_slots,
+                int n_slots, const int32_t* offsets, const int32_t* sorted_pairs, const int32_t* active,
+                const int32_t* tile_off, const int32_t* meta, int n_pairs, int block_m, int path, void* y, int y_f32,
+                hipStream_t stream) {
   if (H <= 0 || I <= 0 || n_slots <= 0 || n_pairs < 0) return LMOE_ERR_ARG;
   if (H % kMxGroup != 0 || I % kMxGroup != 0 || n_slots > kMaxSlots) return LMOE_ERR_SHAPE;
   if (!known_path(path)) return LMOE_ERR_UNSUPPORTED;
@@ -220,10 +220,10 @@ extern "C" int lmoe_combine_f32(const void* y, const int32_t* row_idx, const uin
 namespace lmoe {
 
 // The layer of few or many tokens: what the four calls do, in one.
-static int fused_moe(int rows, const void* x, const void* x_scale, int T, int H, int I, int k, const void*
-                     w13_slots, const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids, const
-                     int32_t* log2phy, int n_log2phy, int path, int block_m, const lmoe_mx4_workspace* ws, const
-                     void* add, void* out, hipStream_t stream) {
+static int fused_moe(int rows, const void* x, const void* x_scale, int T, int H, int I, int k, const void* w13_slots,
+                     const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids, const int32_t* log2phy,
+                     int n_log2phy, int path, int block_m, const lmoe_mx4_workspace* ws, const void* add, void* out,
+                     hipStream_t stream) {
   if (ws == nullptr || T < 0 || k <= 0) return LMOE_ERR_ARG;
   const long long n = static_cast<long long>(T) * k;
   if (n > 0x7fffffffLL) return LMOE_ERR_SHAPE;
@@ -260,10 +260,10 @@ static int fused_moe(int rows, const void* x, const void* x_scale, int T, int H,
                    : lmoe_combine(ws->y, ws->row_idx, w, T, k, H, add, out, stream);
 }
 
-static int decode_few(int rows, const void* x, const void* x_scale, int T, int H, int I, int k, const void*
-                      w13_slots, const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids, const
-                      int32_t* log2phy, int n_log2phy, const void* add, void* act, void* act_scale, void* y, void*
-                      out, hipStream_t stream) {
+static int decode_few(int rows, const void* x, const void* x_scale, int T, int H, int I, int k, const void* w13_slots,
+                      const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids,
+                      const int32_t* log2phy, int n_log2phy, const void* add, void* act, void* act_scale, void* y,
+                      void* out, hipStream_t stream) {
   if (T < 0 || H <= 0 || I <= 0 || k <= 0 || n_slots <= 0 || n_log2phy < 0) return LMOE_ERR_ARG;
   if (H % kMxGroup != 0 || I % kMxGroup != 0 || n_slots > kMaxSlots || static_cast<long long>(T) * k > kScanMaxPairs)
     return LMOE_ERR_SHAPE;
@@ -291,10 +291,10 @@ static int decode_few(int rows, const void* x, const void* x_scale, int T, int H
 }
 
 static int decode_one(int rows, const void* x, const void* x_scale, int H, int I, int k, const void* w13_slots,
-                      const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids, const int32_t*
-                      log2phy, int n_log2phy, const void* w13_b, const void* w2_b, int n_slots_b, const int32_t*
-                      log2phy_b, int n_log2phy_b, const void* add, void* act, void* act_scale, void* out,
-                      hipStream_t stream) {
+                      const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids,
+                      const int32_t* log2phy, int n_log2phy, const void* w13_b, const void* w2_b, int n_slots_b,
+                      const int32_t* log2phy_b, int n_log2phy_b, const void* add, void* act, void* act_scale,
+                      void* out, hipStream_t stream) {
   if (H <= 0 || I <= 0 || k <= 0 || n_slots <= 0 || n_log2phy < 0) return LMOE_ERR_ARG;
   const bool two = w13_b != nullptr;
   if (two != (w2_b != nullptr) || two != (log2phy_b != nullptr) || n_slots_b < 0 || n_log2phy_b < 0) return LMOE_ERR_ARG;
@@ -333,86 +333,86 @@ static int decode_one(int rows, const void* x, const void* x_scale, int H, int I
 
 }  // namespace lmoe
 
-extern "C" int lmoe_mx4_gateup_silu(const void* x, const void* x_scale, int T, int H, int I, int k, const void*
-                                    w13_slots, int n_slots, const int32_t* offsets, const int32_t* sorted_pairs,
-                                    const int32_t* active, const int32_t* tile_off, const int32_t* meta, int
-                                    n_pairs, int block_m, int path, void* act, void* act_scale, int act_split,
-                                    hipStream_t stream) {
+extern "C" int lmoe_mx4_gateup_silu(const void* x, const void* x_scale, int T, int H, int I, int k,
+                                    const void* w13_slots, int n_slots, const int32_t* offsets,
+                                    const int32_t* sorted_pairs, const int32_t* active, const int32_t* tile_off,
+                                    const int32_t* meta, int n_pairs, int block_m, int path, void* act,
+                                    void* act_scale, int act_split, hipStream_t stream) {
   return gateup_silu(kind_of(x_scale), x, x_scale, T, H, I, k, w13_slots, n_slots, offsets, sorted_pairs, active,
                      tile_off, meta, n_pairs, block_m, path, act, act_scale, act_split, stream);
 }
 
-extern "C" int lmoe_mx44_gateup_silu(const void* x, const void* x_scale, int T, int H, int I, int k, const void*
-                                     w13_slots, int n_slots, const int32_t* offsets, const int32_t* sorted_pairs,
-                                     const int32_t* active, const int32_t* tile_off, const int32_t* meta, int
-                                     n_pairs, int block_m, int path, void* act, void* act_scale, int act_split,
-                                     hipStream_t stream) {
+extern "C" int lmoe_mx44_gateup_silu(const void* x, const void* x_scale, int T, int H, int I, int k,
+                                     const void* w13_slots, int n_slots, const int32_t* offsets,
+                                     const int32_t* sorted_pairs, const int32_t* active, const int32_t* tile_off,
+                                     const int32_t* meta, int n_pairs, int block_m, int path, void* act,
+                                     void* act_scale, int act_split, hipStream_t stream) {
   return gateup_silu(kRowsMx4, x, x_scale, T, H, I, k, w13_slots, n_slots, offsets, sorted_pairs, active, tile_off,
                      meta, n_pairs, block_m, path, act, act_scale, act_split, stream);
 }
 
-extern "C" int lmoe_mx4_down(const void* act, const void* act_scale, int act_split, int H, int I, const void*
-                             w2_slots, int n_slots, const int32_t* offsets, const int32_t* sorted_pairs, const
-                             int32_t* active, const int32_t* tile_off, const int32_t* meta, int n_pairs, int
-                             block_m, int path, void* y, int y_f32, hipStream_t stream) {
+extern "C" int lmoe_mx4_down(const void* act, const void* act_scale, int act_split, int H, int I,
+                             const void* w2_slots, int n_slots, const int32_t* offsets, const int32_t* sorted_pairs,
+                             const int32_t* active, const int32_t* tile_off, const int32_t* meta, int n_pairs,
+                             int block_m, int path, void* y, int y_f32, hipStream_t stream) {
   return down(kind_of(act_scale), act, act_scale, act_split, H, I, w2_slots, n_slots, offsets, sorted_pairs, active,
               tile_off, meta, n_pairs, block_m, path, y, y_f32, stream);
 }
 
-extern "C" int lmoe_mx44_down(const void* act, const void* act_scale, int act_split, int H, int I, const void*
-                              w2_slots, int n_slots, const int32_t* offsets, const int32_t* sorted_pairs, const
-                              int32_t* active, const int32_t* tile_off, const int32_t* meta, int n_pairs, int
-                              block_m, int path, void* y, int y_f32, hipStream_t stream) {
+extern "C" int lmoe_mx44_down(const void* act, const void* act_scale, int act_split, int H, int I,
+                              const void* w2_slots, int n_slots, const int32_t* offsets, const int32_t* sorted_pairs,
+                              const int32_t* active, const int32_t* tile_off, const int32_t* meta, int n_pairs,
+                              int block_m, int path, void* y, int y_f32, hipStream_t stream) {
   return down(kRowsMx4, act, act_scale, act_split, H, I, w2_slots, n_slots, offsets, sorted_pairs, active, tile_off,
               meta, n_pairs, block_m, path, y, y_f32, stream);
 }
 
-extern "C" int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int H, int I, int k, const void*
-                                  w13_slots, const void* w2_slots, int n_slots, const uint16_t* w, const int32_t*
-                                  ids, const int32_t* log2phy, int n_log2phy, int path, int block_m, const
-                                  lmoe_mx4_workspace* ws, const void* add, void* out, hipStream_t stream) {
+extern "C" int lmoe_mx4_fused_moe(const void* x, const void* x_scale, int T, int H, int I, int k,
+                                  const void* w13_slots, const void* w2_slots, int n_slots, const uint16_t* w,
+                                  const int32_t* ids, const int32_t* log2phy, int n_log2phy, int path, int block_m,
+                                  const lmoe_mx4_workspace* ws, const void* add, void* out, hipStream_t stream) {
   return fused_moe(kind_of(x_scale), x, x_scale, T, H, I, k, w13_slots, w2_slots, n_slots, w, ids, log2phy,
                    n_log2phy, path, block_m, ws, add, out, stream);
 }
 
-extern "C" int lmoe_mx44_fused_moe(const void* x, const void* x_scale, int T, int H, int I, int k, const void*
-                                   w13_slots, const void* w2_slots, int n_slots, const uint16_t* w, const int32_t*
-                                   ids, const int32_t* log2phy, int n_log2phy, int path, int block_m, const
-                                   lmoe_mx4_workspace* ws, const void* add, void* out, hipStream_t stream) {
+extern "C" int lmoe_mx44_fused_moe(const void* x, const void* x_scale, int T, int H, int I, int k,
+                                   const void* w13_slots, const void* w2_slots, int n_slots, const uint16_t* w,
+                                   const int32_t* ids, const int32_t* log2phy, int n_log2phy, int path, int block_m,
+                                   const lmoe_mx4_workspace* ws, const void* add, void* out, hipStream_t stream) {
   return fused_moe(kRowsMx4, x, x_scale, T, H, I, k, w13_slots, w2_slots, n_slots, w, ids, log2phy, n_log2phy, path,
                    block_m, ws, add, out, stream);
 }
 
-extern "C" int lmoe_mx4_decode_few(const void* x, const void* x_scale, int T, int H, int I, int k, const void*
-                                   w13_slots, const void* w2_slots, int n_slots, const uint16_t* w, const int32_t*
-                                   ids, const int32_t* log2phy, int n_log2phy, const void* add, void* act, void*
-                                   act_scale, void* y, void* out, hipStream_t stream) {
+extern "C" int lmoe_mx4_decode_few(const void* x, const void* x_scale, int T, int H, int I, int k,
+                                   const void* w13_slots, const void* w2_slots, int n_slots, const uint16_t* w,
+                                   const int32_t* ids, const int32_t* log2phy, int n_log2phy, const void* add,
+                                   void* act, void* act_scale, void* y, void* out, hipStream_t stream) {
   return decode_few(kind_of(x_scale), x, x_scale, T, H, I, k, w13_slots, w2_slots, n_slots, w, ids, log2phy,
                     n_log2phy, add, act, act_scale, y, out, stream);
 }
 
-extern "C" int lmoe_mx44_decode_few(const void* x, const void* x_scale, int T, int H, int I, int k, const void*
-                                    w13_slots, const void* w2_slots, int n_slots, const uint16_t* w, const int32_t*
-                                    ids, const int32_t* log2phy, int n_log2phy, const void* add, void* act, void*
-                                    act_scale, void* y, void* out, hipStream_t stream) {
+extern "C" int lmoe_mx44_decode_few(const void* x, const void* x_scale, int T, int H, int I, int k,
+                                    const void* w13_slots, const void* w2_slots, int n_slots, const uint16_t* w,
+                                    const int32_t* ids, const int32_t* log2phy, int n_log2phy, const void* add,
+                                    void* act, void* act_scale, void* y, void* out, hipStream_t stream) {
   return decode_few(kRowsMx4, x, x_scale, T, H, I, k, w13_slots, w2_slots, n_slots, w, ids, log2phy, n_log2phy, add,
                     act, act_scale, y, out, stream);
 }
 
 extern "C" int lmoe_mx4_decode_one(const void* x, const void* x_scale, int H, int I, int k, const void* w13_slots,
-                                   const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids, const
-                                   int32_t* log2phy, int n_log2phy, const void* w13_b, const void* w2_b, int
-                                   n_slots_b, const int32_t* log2phy_b, int n_log2phy_b, const void* add, void*
-                                   act, void* act_scale, void* out, hipStream_t stream) {
+                                   const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids,
+                                   const int32_t* log2phy, int n_log2phy, const void* w13_b, const void* w2_b,
+                                   int n_slots_b, const int32_t* log2phy_b, int n_log2phy_b, const void* add,
+                                   void* act, void* act_scale, void* out, hipStream_t stream) {
   return decode_one(kind_of(x_scale), x, x_scale, H, I, k, w13_slots, w2_slots, n_slots, w, ids, log2phy, n_log2phy,
                     w13_b, w2_b, n_slots_b, log2phy_b, n_log2phy_b, add, act, act_scale, out, stream);
 }
 
 extern "C" int lmoe_mx44_decode_one(const void* x, const void* x_scale, int H, int I, int k, const void* w13_slots,
-                                    const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids, const
-                                    int32_t* log2phy, int n_log2phy, const void* w13_b, const void* w2_b, int
-                                    n_slots_b, const int32_t* log2phy_b, int n_log2phy_b, const void* add, void*
-                                    act, void* act_scale, void* out, hipStream_t stream) {
+                                    const void* w2_slots, int n_slots, const uint16_t* w, const int32_t* ids,
+                                    const int32_t* log2phy, int n_log2phy, const void* w13_b, const void* w2_b,
+                                    int n_slots_b, const int32_t* log2phy_b, int n_log2phy_b, const void* add,
+                                    void* act, void* act_scale, void* out, hipStream_t stream) {
   return decode_one(kRowsMx4, x, x_scale, H, I, k, w13_slots, w2_slots, n_slots, w, ids, log2phy, n_log2phy, w13_b,
                     w2_b, n_slots_b, log2phy_b, n_log2phy_b, add, act, act_scale, out, stream);
 }

@@ -224,8 +224,9 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
       // Experts: rows past the tile's last, whose sums are dropped, are not fetched (tiles of
       // 256, 4096 tokens x 8 of 128 experts, 2048 x 768: 95 -> 93 us, down 85 -> 81).  Products
       // of MX8 rows have no registers left for it, and one such tile a column.
-      buffer_to_lds16<false>(rows_base, c < chunks && (LIN || (wave * C::QA + q) * C::RPL < rows), smem + buf * C::STAGE + (wave * C::QA + q) * 1024, a_off[q] - back,
-                      c * C::ROWB);
+      const int load = wave * C::QA + q;
+      buffer_to_lds16<false>(rows_base, c < chunks && (LIN || load * C::RPL < rows), smem + buf * C::STAGE + load * 1024,
+                             a_off[q] - back, c * C::ROWB);
     }
   };
   constexpr int LOADS = C::QA + C::QB;  // of a wave and chunk
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
           put_scales();
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        wait_vm_barrier<(NB - 3) * (LOADS + (B == 2 ? C::QB : 0))>();
+        wait_vm_barrier<(NB - 3) * LOADS + (B == 2 && NB > 3 ? C::QB : 0)>();  // scales behind chunk c + NB - 2
         issue_a(c + NB - 1, before);
         issue_w(c + NB - 1, before, once);
         if constexpr (B == 1) issue_ws((c >> 2) + 1);

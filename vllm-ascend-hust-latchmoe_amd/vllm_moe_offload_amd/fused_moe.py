@@ -249,8 +249,8 @@ def fused_experts(
     caller's that workspace's out, which its next call overwrites.
 
     Over 4-bit banks (uint8, mxfp4.pack_experts) hidden is bf16, native.Mx8Rows or
-    native.Mx4Rows (act is then rounded to 4 bits between the products); few tokens go straight from their ids, without a permutation
-    in the workspace."""
+    native.Mx4Rows (act is then rounded to 4 bits between the products); few tokens
+    go straight from their ids, without a permutation in the workspace."""
     if w13_slots.dtype is torch.uint8:
         return _mx4_fused_experts(hidden, topk_weights, topk_ids, w13_slots, w2_slots, log2phy, add=add, out=out, path=path,
                                   workspace=workspace)

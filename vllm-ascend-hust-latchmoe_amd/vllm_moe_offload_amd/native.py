@@ -503,8 +503,9 @@ def _take_mx4(rows, name: str, shape, here: int) -> tuple[torch.Tensor, torch.Te
     """(codes, scales) of 4-bit rows [T, K] on device here."""
     q, scale = rows.q, rows.scale
     T, K = shape
-    if q.shape != (T, K >> 1) or scale.shape != (T, K >> 5) or K & 31 or q.dtype is not _U8 or scale.dtype is not _U8 or \
-            q.get_device() != here or scale.get_device() != here or not (q.is_contiguous() and scale.is_contiguous()):
+    if q.shape != (T, K >> 1) or scale.shape != (T, K >> 5) or K & 31 or q.dtype is not _U8 or \
+            scale.dtype is not _U8 or q.get_device() != here or scale.get_device() != here or \
+            not (q.is_contiguous() and scale.is_contiguous()):
         _need_mx4_rows(rows, name, tuple(shape))
         _same_device(q, scale)
     return q, scale
@@ -666,7 +667,8 @@ def _bank_rows(bank: torch.Tensor, name: str, columns: int, here: int) -> tuple[
     return n, shape[-2]
 
 
-def quantize_mx4(w: torch.Tensor, bank: torch.Tensor | None = None, *, gate_up: bool = False, stream=None) -> torch.Tensor:
+def quantize_mx4(w: torch.Tensor, bank: torch.Tensor | None = None, *, gate_up: bool = False,
+                 stream=None) -> torch.Tensor:
     """Weights w [..., N, K], bf16 or f32, as the 4-bit bank that holds them, uint8
     [..., N, mxfp4.row_bytes(K)]: mxfp4.quantize and pack_w2 (gate_up: pack_w13) in one
     pass.  N a multiple of 16 (64 with gate_up), K of 32."""
@@ -783,8 +785,8 @@ def mx4_linear(x, w: torch.Tensor, out: torch.Tensor | None = None, *, bias: tor
         if not _fits(add, _BF16, (T, N), here):
             _refuse(add, "add", _BF16, (T, N))
         pa = add.data_ptr()
-    status = lib.lmoe_mx4_linear(xq.data_ptr(), px, rows, T, K, N, w.data_ptr(), pb, wide_bias, pa, out.data_ptr(), wide_out,
-                                 _stream_on(stream, here))
+    status = lib.lmoe_mx4_linear(xq.data_ptr(), px, rows, T, K, N, w.data_ptr(), pb, wide_bias, pa, out.data_ptr(),
+                                 wide_out, _stream_on(stream, here))
     if status:
         if status == LMOE_ERR_ARG and T > 0 and K > 0 and N > 0:
             raise ValueError("operands overlap: out over an operand other than a bf16 add")
@@ -1284,7 +1286,8 @@ MX4_MAX_COLUMNS_MX8 = {32: 147200, 64: 73600, 128: 32640}
 MX4_MAX_COLUMNS_MX4 = 1 << 23
 
 
-def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False, columns: int = 0, *, mx4: bool = False, row_values: int = 0) -> int:
+def mx4_path(n_pairs: int, n_experts: int, mx8: bool = False, columns: int = 0, *, mx4: bool = False,
+             row_values: int = 0) -> int:
     """The path of a layer of 4-bit experts, for every pass of it: the split-K
     kernel for few pairs per expert (mx8, mx4: of 8-bit, 4-bit rows) and for rows too
     long for any row tile (columns: the longer of x's and act's) or more 4-bit rows than
