@@ -486,17 +486,19 @@ def _fits(t: torch.Tensor, dtype: torch.dtype, shape, here: int) -> bool:
     return t.dtype is dtype and t.get_device() == here and t.shape == shape and t.is_contiguous()
 
 
+_U8, _BF16, _F32, _E4M3 = torch.uint8, torch.bfloat16, torch.float32, torch.float8_e4m3fn
+
+
 def _take_mx8(rows, name: str, shape, here: int) -> tuple[torch.Tensor, torch.Tensor]:
     """(values, scales) of 8-bit rows [T, K] on device here."""
     q, scale = rows.q, rows.scale
-    if not (shape[1] % 32 == 0 and _fits(q, torch.float8_e4m3fn, shape, here) and
-            _fits(scale, torch.uint8, (shape[0], shape[1] // 32), here)):
+    T, K = shape
+    if q.shape != shape or scale.shape != (T, K >> 5) or K & 31 or q.dtype is not _E4M3 or \
+            scale.dtype is not _U8 or q.get_device() != here or scale.get_device() != here or \
+            not (q.is_contiguous() and scale.is_contiguous()):
         _need_mx8(rows, name, tuple(shape))
         _same_device(q, scale)
     return q, scale
-
-
-_U8, _BF16, _F32 = torch.uint8, torch.bfloat16, torch.float32
 
 
 def _take_mx4(rows, name: str, shape, here: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -750,7 +752,7 @@ def mx4_linear(x, w: torch.Tensor, out: torch.Tensor | None = None, *, bias: tor
         (xq, xs), rows = _take_mx4(x, "x", (T, K), here), 2
         px = xs.data_ptr()
     elif isinstance(x, Mx8Rows):
-        T, K = shape = x.shape
+        T, K = shape = x.q.shape
         (xq, xs), rows = _take_mx8(x, "x", shape, here), 1
         px = xs.data_ptr()
     else:
