@@ -11,7 +11,7 @@
 //
 // In the middle of a chunk's products each wave waits for its loads of the next chunk and
 // for the others; after that barrier the next chunk is in LDS and the buffer before this
-// one's is free: the loads for it are sent, and the last products run while the next chunk's
+// one's is free: loads for it are sent, and the last products run while the next chunk's
 // first fragments come out of LDS.  So the matrix instructions never wait for a barrier with
 // nothing to do.  No branch stands between them: past the last chunk the loads go on, out of
 // range, which fetches nothing.
@@ -22,11 +22,12 @@
 // without any arithmetic.  The weights' scales lie that way in the bank; the rows' are put
 // together from their 16 bytes a row.
 //
-// Bound: 256 x 256 of 4-bit rows takes 1.05 us a chunk where its products alone take 0.84
-// (7.3 PFLOP/s from registers, with values that are not zeros) and loads and reads of LDS
-// 0.75; the plain product of 4096 x 7168 x 7168 takes 110 us (3.84 PFLOP/s; without its
-// products 94, without its loads 94).  MX8 rows: 161 us (2.62 PFLOP/s; a large library
-// product of 8-bit floats with one scale reaches 2.8).  Four waves of 128 x 128 took 141 us
+// Bound: of 4-bit rows the plain product of 4096 x 7168 x 7168 takes 108 us (3.9 PFLOP/s;
+// 7.3 from registers with random values, 9.7 with zeros).  With zeros, which cost no power,
+// and 8192 columns, two full rounds of workgroups, 96: 8 us a round are its start and its
+// stores (33 MB), a chunk takes 0.71 us where its products take 0.44, a chunk without loads
+// and reads of LDS 0.65, without the barrier as well 0.58.  MX8 rows: 162 us (2.6 PFLOP/s; a
+// large library product of 8-bit floats with one scale reaches 2.8).  Four waves of 128 x 128 took 141 us
 // to the 123 of this shape in the same run, six buffers with one workgroup a CU were slower.
 //
 // Every output adds its chunks in order, whatever the shape is: the same bits.
@@ -107,21 +108,23 @@ struct MxShape {
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 // 16 (4) bytes a lane from base + lane_at + at to LDS, 1 KiB (256 bytes) from dst on,
-// without passing through registers.  Off: the load is out of range and fetches nothing (its
-// address is that of the first chunk or quad, inside the operand either way).  ONCE: nobody
-// reads them again.
+// without passing through registers.  on: -1, or 0: the load is out of range and fetches
+// nothing (its address is that of the first chunk or quad, inside the operand either way).
+// ONCE: nobody reads them again.
 template <bool ONCE>
-__device__ __forceinline__ void buffer_to_lds16(const uint8_t* base, bool on, char* dst, uint32_t lane_at, int at) {
-  const int range = __builtin_amdgcn_readfirstlane(on ? -1 : 0);
-  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, range, 0x00027000);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 16, lane_at, __builtin_amdgcn_readfirstlane(on ? at : 0), 0,
+__device__ __forceinline__ void buffer_to_lds16(const uint8_t* base, int on, char* dst, uint32_t lane_at, int at) {
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, __builtin_amdgcn_readfirstlane(on),
+                                                   0x00027000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 16, lane_at, __builtin_amdgcn_readfirstlane(at & on), 0,
                                            ONCE ? 2 /* nt */ : 0);
 }
-__device__ __forceinline__ void buffer_to_lds4(const uint8_t* base, bool on, char* dst, uint32_t lane_at, int at) {
-  const int range = __builtin_amdgcn_readfirstlane(on ? -1 : 0);
-  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, range, 0x00027000);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 4, lane_at, __builtin_amdgcn_readfirstlane(on ? at : 0), 0, 0);
+__device__ __forceinline__ void buffer_to_lds4(const uint8_t* base, int on, char* dst, uint32_t lane_at, int at) {
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, __builtin_amdgcn_readfirstlane(on),
+                                                   0x00027000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 4, lane_at, __builtin_amdgcn_readfirstlane(at & on), 0, 0);
 }
+// -1 where a < b, else 0; scalar arithmetic all the way
+__device__ __forceinline__ int below(int a, int b) { return (a - b) >> 31; }
 
 template <int N>
 __device__ __forceinline__ void wait_vm_barrier() {
@@ -201,49 +204,56 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
   const int bb = mx4_block_bytes(K);
   const uint8_t* wbase = uniform(slot_weights(g, slot) + static_cast<size_t>(b0) * bb);
   const int last_block = wblocks - 1 - b0;
-  // chunk c to buffer buf; past the last chunk the same loads, out of range: they fetch
-  // nothing, and what they leave there is not read
-  auto issue_w = [&](int c, int buf, auto once) {
+  // load q of chunk c's weights to buffer buf; past the last chunk the same loads, out of
+  // range: they fetch nothing, and what they leave there is not read
+  auto issue_w = [&](int q, int c, int buf, auto once) {
     const int at = (c >> 2) * kMxQuadBytes + 256 + (c & 3) * 1024;
-#pragma unroll
-    for (int q = 0; q < C::QB; ++q) {
-      const int b = wave * C::QB + q;
-      buffer_to_lds16<decltype(once)::value>(wbase, c < chunks, smem + buf * C::STAGE + C::PART_A + b * 1024, lane * 16,
-                      min(b, last_block) * bb + at);
-    }
+    const int b = wave * C::QB + q;
+    buffer_to_lds16<decltype(once)::value>(wbase, below(c, chunks), smem + buf * C::STAGE + C::PART_A + b * 1024,
+                                           lane * 16, min(b, last_block) * bb + at);
   };
   uint32_t a_off[C::QA];
   const uint32_t tail = K - (chunks - 1) * kMxChunk;  // columns of the last chunk
-  auto issue_a = [&](int c, int buf) {
-#pragma unroll
-    for (int q = 0; q < C::QA; ++q) {
-      // past the row's end, where the weights are zeros, columns of the chunk's first group
-      // again: what is not a number there has made the row's sums so already
-      const uint32_t piece = a_piece(q);
-      const uint32_t back = c + 1 >= chunks && piece * (128 / C::PIECES) >= tail ? piece * 16 : 0;
-      // Experts: rows past the tile's last, whose sums are dropped, are not fetched (tiles of
-      // 256, 4096 tokens x 8 of 128 experts, 2048 x 768: 95 -> 93 us, down 85 -> 81).  Products
-      // of MX8 rows have no registers left for it, and one such tile a column.
-      const int load = wave * C::QA + q;
-      buffer_to_lds16<false>(rows_base, c < chunks && (LIN || load * C::RPL < rows), smem + buf * C::STAGE + load * 1024,
-                             a_off[q] - back, c * C::ROWB);
-    }
+  auto issue_a = [&](int q, int c, int buf) {
+    // past the row's end, where the weights are zeros, columns of the chunk's first group
+    // again: what is not a number there has made the row's sums so already
+    const uint32_t piece = a_piece(q);
+    const uint32_t back = piece * (128 / C::PIECES) >= tail ? piece * 16 & ~below(c + 1, chunks) : 0;
+    // Experts: rows past the tile's last, whose sums are dropped, are not fetched (tiles of
+    // 256, 4096 tokens x 8 of 128 experts, 2048 x 768: 95 -> 93 us, down 85 -> 81).  Products
+    // of MX8 rows have no registers left for it, and one such tile a column.
+    const int load = wave * C::QA + q;
+    const int on = below(c, chunks) & (LIN ? -1 : below(load * C::RPL, rows));
+    buffer_to_lds16<false>(rows_base, on, smem + buf * C::STAGE + load * 1024, a_off[q] - back, c * C::ROWB);
   };
   constexpr int LOADS = C::QA + C::QB;  // of a wave and chunk
 
   const int first = wc * NJ;  // this wave's weight blocks, from b0
   const bool wave_live = first <= last_block;
   const int quads = (chunks + 3) >> 2;
-  auto issue_ws = [&](int quad) {  // the weights' scales of a quad
-#pragma unroll
-    for (int q = 0; q < C::QB; ++q) {
-      const int b = wave * C::QB + q;
-      buffer_to_lds4(wbase, quad < quads, smem + C::OFF_WSCALE + b * 256, lane * 4,
-                     min(b, last_block) * bb + quad * kMxQuadBytes);
-    }
+  auto issue_ws = [&](int q, int quad) {  // load q of a quad's weights' scales
+    const int b = wave * C::QB + q;
+    buffer_to_lds4(wbase, below(quad, quads), smem + C::OFF_WSCALE + b * 256, lane * 4,
+                   min(b, last_block) * bb + quad * kMxQuadBytes);
   };
-  issue_w(0, 0, std::false_type{});
-  issue_ws(0);
+  // load n of a chunk
+  auto issue = [&](int n, int c, int buf, auto once) {
+    if (n < C::QA) issue_a(n, c, buf);
+    else issue_w(n - C::QA, c, buf, once);
+  };
+  // Eight waves that send a chunk's loads all at once wait for each other's addresses (32
+  // loads of 16 clocks each), so they send them between the products, FIRST of them behind
+  // the barrier and the others before the next one: 4096 x 7168 x 7168 of MX4 rows 112 -> 108
+  // us (of zeros, which cost no power, 100 -> 96), gate-up of 2049 tokens x 4 of 32 experts,
+  // 7168 x 2048 185 -> 179, 1024 x 7168 x 7168 of MX8 rows 50.5 -> 48.  Two workgroups of four
+  // waves a CU gain nothing, lower tiles lose (7168 x 2048 87 -> 94: the loads that go out
+  // later arrive later), and with three buffers the later ones would not arrive in time.
+  constexpr bool SPREAD = NB > 3 && C::WAVES == 8;
+  constexpr int FIRST = SPREAD ? LOADS / 2 : LOADS;
+#pragma unroll
+  for (int q = 0; q < C::QB; ++q) issue_w(q, 0, 0, std::false_type{});
+#pragma unroll
+  for (int q = 0; q < C::QB; ++q) issue_ws(q, 0);
 #pragma unroll
   for (int q = 0; q < C::QA; ++q)
     a_off[q] = static_cast<uint32_t>(source_row(a_row(q), a_pair[q])) * (R == kRowsMx8 ? K : K >> 1) + a_piece(q) * 16;
@@ -254,12 +264,12 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
   auto get_scales = [&](int quad) { qs = load_scales<typename C::scales_t>(my_scales, 16 * quad + tid % C::PER_ROW * SB, groups); };
   auto put_scales = [&]() { *reinterpret_cast<typename C::scales_t*>(smem + C::OFF_SCALE + tid * SB) = qs; };
   get_scales(0);
-  issue_a(0, 0);
 #pragma unroll
-  for (int c = 1; c < NB - 1; ++c) {
-    issue_a(c, c);
-    issue_w(c, c, std::false_type{});
-  }
+  for (int q = 0; q < C::QA; ++q) issue_a(q, 0, 0);
+#pragma unroll
+  for (int c = 1; c < NB - 1; ++c)
+#pragma unroll
+    for (int n = 0; n < (c == NB - 2 ? FIRST : LOADS); ++n) issue(n, c, c, std::false_type{});
   if constexpr (!LIN)
     if (tid < BM) s_pair[tid] = my_pair;
   put_scales();
@@ -313,15 +323,31 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
         wait_vm_barrier<(NB - 3) * LOADS + (B == 2 && NB > 3 ? C::QB : 0)>();  // scales behind chunk c + NB - 2
-        issue_a(c + NB - 1, before);
-        issue_w(c + NB - 1, before, once);
-        if constexpr (B == 1) issue_ws((c >> 2) + 1);
       };
+      const int last = before == 0 ? NB - 1 : before - 1;
+      constexpr int SENT = FIRST + (B == 1 ? C::QB : 0);
+      auto send = [&](int n) {  // behind the barrier
+        if (n < FIRST) issue(n, c + NB - 1, before, once);
+        else issue_ws(n - FIRST, (c >> 2) + 1);
+      };
+      // before it: the rest of the chunk begun in the one before this
+      auto send_rest = [&](int n) { issue(FIRST + n, c + NB - 2, last, once); };
       if constexpr (NL > 0) {
+        // loads between the products, so that no wave waits for the others' addresses
+        constexpr int BEFORE = PAIRS / 2 * NJ, AFTER = (PAIRS - PAIRS / 2) * NJ;  // groups of products
+        constexpr int REST = LOADS - FIRST;
+        if constexpr (BEFORE == 0)
+#pragma unroll
+          for (int n = 0; n < REST; ++n) send_rest(n);
 #pragma unroll
         for (int p = 0; p < PAIRS; ++p) {
           constexpr int first_x = B * PAIRS & 1;
-          if (p == PAIRS / 2) turn();
+          if (p == PAIRS / 2) {
+            turn();
+            if constexpr (!SPREAD)
+#pragma unroll
+              for (int n = 0; n < SENT; ++n) send(n);
+          }
           if (p + 1 < PAIRS) read_x((first_x + p + 1) & 1, p + 1, xp);
           else read_x((first_x + p + 1) & 1, 0, xn);
           __builtin_amdgcn_sched_barrier(0);
@@ -330,16 +356,29 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
 #pragma unroll
             for (int i = 2 * p; i < 2 * p + 2 && i < NL; ++i)
               acc[i][j] = mx_step<R, B>(w[j], ws[j], x[(first_x + p) & 1][i & 1], xs[i], acc[i][j]);
-            if (p + 1 == PAIRS) {  // the next chunk's, as this one's are done with
-              __builtin_amdgcn_sched_barrier(0);
-              read_w(j, wn);
-              __builtin_amdgcn_sched_barrier(0);
+            if (p + 1 == PAIRS || SPREAD) __builtin_amdgcn_sched_barrier(0);
+            if (p + 1 == PAIRS) read_w(j, wn);  // the next chunk's, as this one's are done with
+            if constexpr (SPREAD) {
+              const int k = p * NJ + j;
+              if (k < BEFORE) {
+#pragma unroll
+                for (int n = k * REST / (BEFORE > 0 ? BEFORE : 1); n < (k + 1) * REST / (BEFORE > 0 ? BEFORE : 1); ++n)
+                  send_rest(n);
+              } else {
+#pragma unroll
+                for (int n = (k - BEFORE) * SENT / AFTER; n < (k - BEFORE + 1) * SENT / AFTER; ++n) send(n);
+              }
             }
+            if (p + 1 == PAIRS || SPREAD) __builtin_amdgcn_sched_barrier(0);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
       } else {
+#pragma unroll
+        for (int n = 0; n < LOADS - FIRST; ++n) send_rest(n);
         turn();
+#pragma unroll
+        for (int n = 0; n < SENT; ++n) send(n);
       }
       buf = next;
       xp = xn;
@@ -358,7 +397,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
       if (quad + 1 < quads) get_scales(quad + 1);
     };
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    wait_vm_barrier<(NB - 2) * LOADS>();  // chunk 0 and the scales
+    wait_vm_barrier<(NB - 3) * LOADS + FIRST>();  // chunk 0 and the scales
     if constexpr (NL > 0) {
       read_x(0, 0, x_at);
 #pragma unroll
