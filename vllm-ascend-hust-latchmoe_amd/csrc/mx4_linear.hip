@@ -111,14 +111,19 @@ static int launch_rows8(const LinearArgs& g, int cus, hipStream_t stream) {
 template <int R>
 static int launch_linear(const LinearArgs& g, hipStream_t stream) {
   const int cus = device_cus();
-  if (R == kRowsBf16 && g.T <= 16 && g.N > 16384) return launch_few<R, 8, 1, 8, 1>(g, stream);
+  if constexpr (R == kRowsBf16)
+    if (g.T <= 16 && g.N > 16384) return launch_few<R, 8, 1, 8, 1>(g, stream);
   if (g.T <= 16 || tiles_of(g, 16, 32) <= cus) return launch_few<R, 2, 1, 8, 2>(g, stream);
   if (tiles_of(g, 16, 64) <= cus + cus / 4) return launch_few<R, 4, 1, 8, 2>(g, stream);
   if (tiles_of(g, 32, 64) <= cus) return launch_few<R, 4, 2, 8, 2>(g, stream);
-  if (R == kRowsMx4) return launch_rows4(g, cus, stream);
-  if (R == kRowsMx8) return launch_rows8(g, cus, stream);
-  if (tiles_of(g, 16, 64) <= 5 * cus / 2) return launch_few<kRowsBf16, 4, 1, 8, 2>(g, stream);
-  return launch_rows(g, cus, stream);
+  if constexpr (R == kRowsMx4) {
+    return launch_rows4(g, cus, stream);
+  } else if constexpr (R == kRowsMx8) {
+    return launch_rows8(g, cus, stream);
+  } else {
+    if (tiles_of(g, 16, 64) <= 5 * cus / 2) return launch_few<R, 4, 1, 8, 2>(g, stream);
+    return launch_rows(g, cus, stream);
+  }
 }
 
 }  // namespace lmoe

@@ -179,7 +179,7 @@ def _empty(shape: tuple, device, pin: bool) -> torch.Tensor:
 def _has_kernel(w: torch.Tensor, gate_up: bool) -> bool:
     """Whether native.quantize_mx4 takes these weights."""
     return w.is_cuda and w.dtype in (torch.bfloat16, torch.float32) and w.is_contiguous() and \
-        w.data_ptr() % 16 == 0 and int(w.shape[1]) % (64 if gate_up else ROWS) == 0
+        w.data_ptr() % 16 == 0 and int(w.shape[1]) % (64 if gate_up else ROWS) == 0 and int(w.shape[2]) <= 1 << 23
 
 
 def pack_experts(w13: torch.Tensor, w2: torch.Tensor, *, pin_memory: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
