@@ -3,15 +3,14 @@
 // gate-up: act[pos] = silu(W_g x) * (W_u x);  down: y[pair] = W_2 act[pos].
 // Weights are MX4 blocks (mx.h), rows bf16, MX8 or MX4.  What bounds it is the
 // weights' bytes: each slot's are read once for up to 32 rows (16 where act comes in two
-// parts, below).  Measured, gate-up /
-// down: 7 tokens x 8 of 64 experts, 7168 x 2048, MX8 rows 94 / 49 us (561 / 281 MB at
-// 6.0 / 5.7 TB/s); 16 x 8 of 128, 2048 x 768, bf16 rows 16.6 / 10.6 us (66 / 33 MB at
-// 4.0 / 3.1 TB/s: the start and the longest slot's passes of so short a kernel); MX4 rows
-// 97 / 49 us and, the experts drawn unevenly, 13.0 / 8.4 (55 / 28 MB; reading 54 and 33 MB
-// and nothing else takes 9.7 and 6.6 us).  MX4 rows, measured and not kept: the first
-// chunk's weights sent before the rows' addresses are known (down 8.4 -> 7.5, gate-up of 16
-// experts of 4096 x 1024 17.3 -> 18.0, elsewhere within 2%), weights a chunk ahead of the
-// products (13.7 / 10.0), 2 or 4 chunks at a time.
+// parts, below).  Measured, weights in no cache, gate-up / down: 7 tokens x 8 of 64 experts,
+// 7168 x 2048, MX8 rows 100 / 51 us (at 6.6 / 6.4 TB/s), MX4 rows 99 / 50; 16 x 8 of 128,
+// 2048 x 768, drawn unevenly, bf16 rows 14.2 / 10.3 us (62 / 31 MB at 4.3 / 3.0 TB/s: the
+// start and the longest slot's passes of so short a kernel), MX4 rows 13.2 / 7.7 (reading 54
+// and 33 MB and nothing else takes 9.7 and 6.6 us).  MX4 rows, measured and not kept: the
+// first chunk's weights sent before the rows' addresses are known (down 8.4 -> 7.5, gate-up
+// of 16 experts of 4096 x 1024 17.3 -> 18.0, elsewhere within 2%), weights a chunk ahead of
+// the products (13.7 / 10.0), 2 or 4 chunks at a time.
 //
 // A workgroup computes 64 weight rows, four 16-row blocks, for one slot: 32 act
 // columns (gate and up) or 64 y columns.  Its waves split the row's K between them,
@@ -276,10 +275,17 @@ __device__ __forceinline__ f32x4_t other_part(const f32x4_t v) {
 
 // Chunks [c0, c1) of RB weight blocks by NF row fragments, U chunks' loads at a time.
 // (blocks: how many of the RB there are; the last stands in for the others)
-template <int R, int RB, int NF, int U>
+// QUADS: a quad's scales come as one dword at its first chunk, not as a byte at each chunk,
+// which saves a third of the loads: 16 tokens x 8 of 128 experts, 2048 x 768, gate-up / down
+// of bf16 rows 15.8 / 10.7 -> 14.2 / 10.3 us, MX8 rows 15.4 / 10.6 -> 13.8 / 9.4, MX4 rows
+// 13.7 / 8.9 -> 13.1 / 7.8.  Not where few waves each take two chunks or more in one round
+// trip, which the test of a quad's start cuts in two: one token of 2048 x 768 from MX8 rows
+// 10.4 -> 11.1, its plain product 7168 x 7168 of MX4 rows 7.9 -> 9.0.
+template <int R, int RB, int NF, int U, bool QUADS>
 __device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int blocks, int K, int c0, int c1, int lane,
                                            const char* const (&row)[NF], const uint8_t* const (&row_scale)[NF],
                                            f32x4_t (&acc)[RB][NF]) {
+  int quad_sc[RB];
   for (int c = c0; c < c1; c += U) {
     i32x4_t w[U][RB];
     int sc[U][RB];
@@ -288,12 +294,21 @@ __device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int bloc
     for (int u = 0; u < U; ++u) {
       if (u > 0 && c + u >= c1) break;
       const uint8_t* quad = wblk + ((c + u) >> 2) * kMxQuadBytes;
+      const int byte = (c + u) & 3;
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
         const uint8_t* p = quad + min(b, blocks - 1) * bb;
-        w[u][b] = __builtin_nontemporal_load(
-            reinterpret_cast<const i32x4_t*>(p + 256 + ((c + u) & 3) * 1024 + lane * 16));
-        sc[u][b] = p[lane * 4 + ((c + u) & 3)];
+        w[u][b] = __builtin_nontemporal_load(reinterpret_cast<const i32x4_t*>(p + 256 + byte * 1024 + lane * 16));
+        if constexpr (!QUADS) sc[u][b] = p[lane * 4 + byte];
+      }
+      if constexpr (QUADS) {
+        if (c + u == c0 || byte == 0) {
+#pragma unroll
+          for (int b = 0; b < RB; ++b)
+            quad_sc[b] = *reinterpret_cast<const int*>(quad + min(b, blocks - 1) * bb + lane * 4);
+        }
+#pragma unroll
+        for (int b = 0; b < RB; ++b) sc[u][b] = quad_sc[b];
       }
 #pragma unroll
       for (int f = 0; f < NF; ++f) x[u][f] = load_row_frag<R>(row[f], row_scale[f], c + u, K, lane >> 4);
@@ -302,9 +317,11 @@ __device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int bloc
     for (int u = 0; u < U; ++u) {
       if (u > 0 && c + u >= c1) break;
 #pragma unroll
-      for (int b = 0; b < RB; ++b)
+      for (int b = 0; b < RB; ++b) {
+        const int scale = QUADS ? sc[u][b] >> (8 * ((c + u) & 3)) : sc[u][b];
 #pragma unroll
-        for (int f = 0; f < NF; ++f) acc[b][f] = mx4_step<R>(w[u][b], sc[u][b], x[u][f], acc[b][f]);
+        for (int f = 0; f < NF; ++f) acc[b][f] = mx4_step<R>(w[u][b], scale, x[u][f], acc[b][f]);
+      }
     }
   }
 }
@@ -335,8 +352,8 @@ __device__ __forceinline__ void few_rows(const Mx4Args& g, const uint8_t* wblk, 
   for (int b = 0; b < RB; ++b)
 #pragma unroll
     for (int f = 0; f < NF; ++f) acc[b][f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  few_chunks<R, RB, NF, ONE ? 2 : 1>(wblk, mx4_block_bytes(g.K), blocks, g.K, wave * chunks / NW, (wave + 1) * chunks / NW,
-                            lane, row, row_scale, acc);
+  few_chunks<R, RB, NF, ONE ? 2 : 1, !ONE>(wblk, mx4_block_bytes(g.K), blocks, g.K, wave * chunks / NW,
+                                           (wave + 1) * chunks / NW, lane, row, row_scale, acc);
   // partial sums of a fragment, [wave][block][lane], added in wave order
   f32x4_t high[2];
 #pragma unroll
@@ -519,8 +536,8 @@ __global__ __launch_bounds__(kOneMxWaves * 64) void mx4_one_down_kernel(Mx4Args 
     const uint8_t* row_scale[1] = {R != kRowsBf16 ? g.a_scale + static_cast<size_t>(j) * (g.K / kMxGroup) : nullptr};
     f32x4_t acc[1][1] = {{f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}}};
     const uint8_t* wblk = expert + static_cast<size_t>(blockIdx.x) * bb;
-    few_chunks<R, 1, 1, 4>(wblk, bb, 1, g.K, part * chunks / parts, (part + 1) * chunks / parts, lane, row, row_scale,
-                            acc);
+    few_chunks<R, 1, 1, 4, false>(wblk, bb, 1, g.K, part * chunks / parts, (part + 1) * chunks / parts, lane, row,
+                                  row_scale, acc);
     sum += wj * acc[0][0];
   }
   if constexpr (R == kRowsBf16) sum += other_part(sum);

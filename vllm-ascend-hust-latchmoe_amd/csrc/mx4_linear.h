@@ -72,8 +72,8 @@ __device__ __forceinline__ void store_linear(const LinearArgs& g, int row, int n
 // Few rows: a workgroup takes RB blocks of 16 columns by NF fragments of 16 rows; its NW
 // waves split K, U chunks' loads at a time, and their partial sums are added in LDS in wave
 // order.  Bound by the weights' bytes and, below some 20 MB of them, by the launch: 1 x 2048 x
-// 5120 of MX4 rows 4.0 us (an empty launch 2.1), 1 x 2048 x 50000 11.1 (54 MB; reading them
-// and nothing else 9.7), 16 bf16 rows there 13.6 with 3.2 MB of f32 sums to write.
+// 5120 of MX4 rows 3.9 us (an empty launch 2.1), 1 x 2048 x 50000 11.0 (54 MB; reading them
+// and nothing else 9.7), 16 rows there 12.0 (MX4) and 14.3 (bf16).
 template <int R, int RB, int NF, int NW, int U>
 __global__ __launch_bounds__(NW * 64) void mx4_linear_few_kernel(LinearArgs g) {
   __shared__ f32x4_t s_part[NW * RB * NF * 64];
@@ -100,8 +100,8 @@ __global__ __launch_bounds__(NW * 64) void mx4_linear_few_kernel(LinearArgs g) {
   for (int b = 0; b < RB; ++b)
 #pragma unroll
     for (int f = 0; f < NF; ++f) acc[b][f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  few_chunks<R, RB, NF, U>(wblk, bb, blocks, g.K, wave * chunks / NW, (wave + 1) * chunks / NW, lane, row, row_scale,
-                           acc);
+  few_chunks<R, RB, NF, U, R != kRowsMx4 || U == 1>(wblk, bb, blocks, g.K, wave * chunks / NW, (wave + 1) * chunks / NW,
+                                                    lane, row, row_scale, acc);
 #pragma unroll
   for (int b = 0; b < RB; ++b)
 #pragma unroll

@@ -104,15 +104,17 @@ static int launch_rows8(const LinearArgs& g, int cus, hipStream_t stream) {
 //   MX8 rows    -   -   -   -       -    -    -    -    31.8 22.9 18.1 20.2   13.3 11.1 13.0  7.2
 //   bf16 rows  5.4 6.4 7.3  -     20.8 15.2 23.5   -    37.0 25.8 23.2 44.3   15.3 12.5 15.6 13.8
 // (bf16 rows' tiles need more workgroups than the others' to be worth it.)
-// Past 16384 columns, up to 16 rows: bf16 rows, which are read again by every workgroup,
-// 128 columns a workgroup (us of 32 / 64 / 128: 16 x 2048 x 50000 20.1 / 17.0 / 14.6, 1 x 2048 x
-// 50000 15.4 / 13.4 / 12.5, 16 x 4096 x 32000 23.5 / 18.3 / 15.7, 16 x 2048 x 20000 10.6 / 10.0 /
-// 8.5; below, 8 x 7168 x 16384 16.6 / 14.6 / 19.1; 4-bit rows 13.8, 13.6, 13.1).
+// Past 16384 columns, up to 16 rows, whose rows every workgroup reads again: 128 columns a
+// workgroup, a chunk at a time.  us of 32 / 64 / 128 columns:
+//                1 x 2048 x 50000    16 x 2048 x 50000   16 x 2048 x 20000  16 x 7168 x 32000
+//   MX4 rows     10.9 / 12.4 / 11.0  13.8 / 13.7 / 12.0  7.7 / 8.3 / 7.9    28.5 / 24.1 / 21.5
+//   MX8 rows     12.4 / 12.3 / 11.2  15.6 / 14.5 / 12.3  8.5 / 8.6 / 7.7    31.0 / 24.6 / 21.7
+//   bf16 rows    15.2 / 13.7 / 12.1  20.5 / 16.8 / 14.3  10.4 / 10.0 / 8.4  36.5 / 27.8 / 23.8
+// and below, 8 x 7168 x 16384: 13.2 / 12.9 / 16.4, 14.0 / 13.0 / 16.5, 16.0 / 14.3 / 17.5.
 template <int R>
 static int launch_linear(const LinearArgs& g, hipStream_t stream) {
   const int cus = device_cus();
-  if constexpr (R == kRowsBf16)
-    if (g.T <= 16 && g.N > 16384) return launch_few<R, 8, 1, 8, 1>(g, stream);
+  if (g.T <= 16 && g.N > 16384) return launch_few<R, 8, 1, 8, 1>(g, stream);
   if (g.T <= 16 || tiles_of(g, 16, 32) <= cus) return launch_few<R, 2, 1, 8, 2>(g, stream);
   if (tiles_of(g, 16, 64) <= cus + cus / 4) return launch_few<R, 4, 1, 8, 2>(g, stream);
   if (tiles_of(g, 32, 64) <= cus) return launch_few<R, 4, 2, 8, 2>(g, stream);
