@@ -275,21 +275,27 @@ __device__ __forceinline__ f32x4_t other_part(const f32x4_t v) {
 
 // Chunks [c0, c1) of RB weight blocks by NF row fragments, U chunks' loads at a time.
 // (blocks: how many of the RB there are; the last stands in for the others)
-// QUADS: a quad's scales come as one dword at its first chunk, not as a byte at each chunk,
-// which saves a third of the loads: 16 tokens x 8 of 128 experts, 2048 x 768, gate-up / down
-// of bf16 rows 15.8 / 10.7 -> 14.2 / 10.3 us, MX8 rows 15.4 / 10.6 -> 13.8 / 9.4, MX4 rows
-// 13.7 / 8.9 -> 13.1 / 7.8.  Not where few waves each take two chunks or more in one round
-// trip, which the test of a quad's start cuts in two: one token of 2048 x 768 from MX8 rows
-// 10.4 -> 11.1, its plain product 7168 x 7168 of MX4 rows 7.9 -> 9.0.
-template <int R, int RB, int NF, int U, bool QUADS>
+// A quad's scales come as one dword, not as a byte at each chunk, which saves a third of the
+// loads.  CARRY: at the quad's first chunk, and kept: 16 tokens x 8 of 128 experts, 2048 x
+// 768, gate-up / down of bf16 rows 15.8 / 10.7 -> 14.2 / 10.3 us, MX8 rows 15.4 / 10.6 -> 13.8
+// / 9.4, MX4 rows 13.7 / 8.9 -> 13.1 / 7.8.  Else once a round, twice where a round's chunks
+// lie in two quads: where a few waves each have little more than one round, the test of a
+// quad's start would cut it in two (one token of 2048 x 768 and of 7168 x 2048, bf16 rows
+// 12.4 -> 11.6 and 50.5 -> 47.0 us, MX8 rows 10.5 -> 10.2, 41.0 -> 37.9, MX4 rows 10.2 -> 9.8,
+// 37.4 -> 35.0; kept, MX8 rows 11.1 and 38.8).
+template <int R, int RB, int NF, int U, bool CARRY>
 __device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int blocks, int K, int c0, int c1, int lane,
                                            const char* const (&row)[NF], const uint8_t* const (&row_scale)[NF],
                                            f32x4_t (&acc)[RB][NF]) {
-  int quad_sc[RB];
+  auto scales_of = [&](const uint8_t* quad, int b) {
+    return *reinterpret_cast<const int*>(quad + min(b, blocks - 1) * bb + lane * 4);
+  };
+  int quad_sc[RB], next_sc[RB];
   for (int c = c0; c < c1; c += U) {
     i32x4_t w[U][RB];
     int sc[U][RB];
     RowFrag<R> x[U][NF];
+    const int first = c >> 2;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (u > 0 && c + u >= c1) break;
@@ -299,26 +305,32 @@ __device__ __forceinline__ void few_chunks(const uint8_t* wblk, int bb, int bloc
       for (int b = 0; b < RB; ++b) {
         const uint8_t* p = quad + min(b, blocks - 1) * bb;
         w[u][b] = __builtin_nontemporal_load(reinterpret_cast<const i32x4_t*>(p + 256 + byte * 1024 + lane * 16));
-        if constexpr (!QUADS) sc[u][b] = p[lane * 4 + byte];
       }
-      if constexpr (QUADS) {
-        if (c + u == c0 || byte == 0) {
+      if (CARRY ? c + u == c0 || byte == 0 : u == 0) {
 #pragma unroll
-          for (int b = 0; b < RB; ++b)
-            quad_sc[b] = *reinterpret_cast<const int*>(quad + min(b, blocks - 1) * bb + lane * 4);
-        }
+        for (int b = 0; b < RB; ++b) quad_sc[b] = scales_of(quad, b);
+      }
+      if constexpr (CARRY) {
 #pragma unroll
         for (int b = 0; b < RB; ++b) sc[u][b] = quad_sc[b];
       }
 #pragma unroll
       for (int f = 0; f < NF; ++f) x[u][f] = load_row_frag<R>(row[f], row_scale[f], c + u, K, lane >> 4);
     }
+    if constexpr (!CARRY) {
+      const int last = (min(c + U, c1) - 1) >> 2;
+      if (last != first) {
+#pragma unroll
+        for (int b = 0; b < RB; ++b) next_sc[b] = scales_of(wblk + last * kMxQuadBytes, b);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (u > 0 && c + u >= c1) break;
+      const bool next = (c + u) >> 2 != first;
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        const int scale = QUADS ? sc[u][b] >> (8 * ((c + u) & 3)) : sc[u][b];
+        const int scale = (CARRY ? sc[u][b] : next ? next_sc[b] : quad_sc[b]) >> (8 * ((c + u) & 3));
 #pragma unroll
         for (int f = 0; f < NF; ++f) acc[b][f] = mx4_step<R>(w[u][b], scale, x[u][f], acc[b][f]);
       }
@@ -471,10 +483,9 @@ __global__ __launch_bounds__(kFewMxWaves * 64) void mx4_few_kernel(Mx4Args g, To
 // One token: no permutation.  Pair j's expert is looked up where it is needed, its
 // act row is row j, and the down product ends in the weighted combine: two launches
 // where the permutation, the split-K kernel twice and the combine are four.  Measured,
-// gate-up / down, 8 experts: 2048 x 768 6.4 / 6.6 us (13.4 / 6.7 MB: latency of the
-// id, table, weight chain), 7168 x 2048 24.0 / 20.8 us from bf16 rows, 22.4 / 15.9 us
-// from MX8 rows (125 / 62 MB at 5.6 / 3.9 TB/s); both of 2048 x 768 in a graph 12.2 us
-// from bf16 rows, 10.4 from MX8 rows.  The down product's waves then add
+// both in a graph, 8 experts: 2048 x 768 (13.4 + 6.7 MB: latency of the id, table, weight
+// chain) 11.6 us from bf16 rows, 10.3 from MX8 rows, 9.8 from MX4 rows; 7168 x 2048 (125 +
+// 62 MB) 47.2 / 37.9 / 35.0.  The down product's waves then add
 // their parts of K in another order than the split-K kernel's; the same order, parts
 // through LDS, cost a quarter at 7168 x 2048 (the step 51.7 -> 65.0 us).
 // ---------------------------------------------------------------------------
