@@ -476,7 +476,9 @@ int lmoe_mx4_bank_values(const void* bank, int E, int N, int K, int gate_up,
 
 /* out = x W^T (+ bias) (+ add) over MX4 weights w of [N, K] (in order, as w2).
  * rows says what x [T, K] is: LMOE_ROWS_BF16 (x_scale null), LMOE_ROWS_MX8 or
- * LMOE_ROWS_MX4.  Products are summed in f32, bias [N] (bf16 or f32, may be null) and
+ * LMOE_ROWS_MX4.  Products are summed in f32 (MX8 rows with a bf16 out: the products of
+ * each eight columns in fixed point, cut 13 bits below the largest, each off by less than
+ * 2^-13 of that one, and those sums in f32), bias [N] (bf16 or f32, may be null) and
  * add [T, N] (bf16, may be null) are added in f32, out [T, N] is rounded once, to
  * bf16 or f32 (out_f32).  Which partial sums are added depends on the sizes, never on
  * the values.  K % 32 == 0 up to 2^23, N % 16 == 0, operands 16-byte aligned (x_scale
@@ -493,7 +495,8 @@ long long lmoe_mx4_bytes(int N, int K);
 /* lmoe_gateup_silu and lmoe_down over slot banks of MX4 weights (the same
  * permutation arguments).  Rows are bf16 (x_scale and act_scale null) or MX8
  * rows (both given): then act is rounded to MX8 along I, and both products
- * multiply 8-bit by 4-bit values; f32 accumulation either way, gate, up and
+ * multiply 8-bit by 4-bit values, adding the products of each eight columns in fixed
+ * point, cut 13 bits below the largest; f32 accumulation otherwise, gate, up and
  * their product in f32, act rounded once.  act_split (bf16 rows, not in row
  * tiles: LMOE_ERR_UNSUPPORTED): act is [n_pairs, 2, I], two bf16 numbers whose
  * sum is the value to 16 bits, for batches of few tokens, whose outputs hang on

@@ -1,7 +1,8 @@
 // One matrix of 4-bit weights: y = x W^T (+ bias) (+ add).
 //
 // Rows are bf16, MX8 or MX4; weights one slot of a bank in order (mx.h).  Sums, bias and add
-// are in f32 and are rounded once, to out's type.
+// are in f32 and are rounded once, to out's type; of MX8 rows with a bf16 out the products of
+// eight neighbouring columns are added in fixed point first (rows8_part in mx.h).
 #pragma once
 
 #include "mx4_few.h"

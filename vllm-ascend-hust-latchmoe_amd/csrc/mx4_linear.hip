@@ -63,6 +63,14 @@ constexpr ShapeCost kShapes4[4] = {{256, 256, 1, 43, {8.3}}, {128, 128, 2, 0, {4
 constexpr ShapeCost kShapes8[5] = {{256, 256, 1, 67, {12.0}}, {128, 256, 1, 41, {7.5}}, {128, 128, 2, 10, {7.5, 9.6}},
                                    {64, 128, 2, 25, {3.6, 5.5}}, {64, 64, 3, 15, {3.3, 4.2, 4.9}}};
 
+// MX8 rows with f32 outputs, in two parts (twice the products; 256 x 256 tiles spill 112
+// registers), us of 128 x 256 / 128 x 128 / 64 x 128 / 64 x 64 tiles: 4096 x 7168 x 7168 352 /
+// 335 / 361 / 474, 4096 x 2048 x 5120 88.7 / 80.2 / 87.3 / 109, 1024 x 7168 x 7168 89.2 / 89.8 /
+// 95.2 / 115, 512 x 7168 x 7168 85.0 / 63.3 / 52.5 / 64.8, 300 x 2048 x 5120 29.3 / 21.4 / 13.8 /
+// 13.9, 300 x 1408 x 2048 21.8 / 16.3 / 10.4 / 8.4
+constexpr ShapeCost kShapes8Parts[4] = {{128, 256, 1, 64, {14.0}}, {128, 128, 2, 48, {10.4, 15.2}},
+                                        {64, 128, 2, 35, {6.2, 8.4}}, {64, 64, 3, 32, {4.3, 6.7, 8.0}}};
+
 static int cheapest(const ShapeCost* shapes, int n, const LinearArgs& g, int cus) {
   const int chunks = mx4_chunks(g.K);
   int best = 0;
@@ -97,12 +105,22 @@ static int launch_rows8(const LinearArgs& g, int cus, hipStream_t stream) {
   return launch_mx_linear<Tile8_64x64>(g, stream);
 }
 
+static int launch_rows8_parts(const LinearArgs& g, int cus, hipStream_t stream) {
+  const int shape = cheapest(kShapes8Parts, 4, g, cus);
+  if (shape == 0) return launch_mx_linear<Tile8P_128x256>(g, stream);
+  if (shape == 1) return launch_mx_linear<Tile8P_128x128>(g, stream);
+  if (shape == 2) return launch_mx_linear<Tile8P_64x128>(g, stream);
+  return launch_mx_linear<Tile8P_64x64>(g, stream);
+}
+
 // Split K while that makes workgroups enough: for the fewest rows 32 columns by 16 rows a
 // workgroup, then 64 by 16, then 64 by 32.  us of these three and of row tiles (T x K x N):
 //              16 x 2048 x 5120   32 x 7168 x 7168      64 x 7168 x 7168      128 x 2048 x 5120
 //   MX4 rows   4.4 4.7 5.0  -     15.3 12.2 15.8 19.0   27.0 20.6 15.2 19.5     -    -   9.3  6.8
 //   MX8 rows    -   -   -   -       -    -    -    -    31.8 22.9 18.1 20.2   13.3 11.1 13.0  7.2
 //   bf16 rows  5.4 6.4 7.3  -     20.8 15.2 23.5   -    37.0 25.8 23.2 44.3   15.3 12.5 15.6 13.8
+// MX8 rows in two parts (f32 outputs) cost up to 0.4 us more there, 128 x 2048 x 5120 11.9 10.5
+// 13.2 10.8, 64 x 7168 x 7168 31.3 22.1 17.8 27.1.
 // (bf16 rows' tiles need more workgroups than the others' to be worth it.)
 // Past 16384 columns, up to 16 rows, whose rows every workgroup reads again: 128 columns a
 // workgroup, a chunk at a time.  us of 32 / 64 / 128 columns:
@@ -122,6 +140,8 @@ static int launch_linear(const LinearArgs& g, hipStream_t stream) {
     return launch_rows4(g, cus, stream);
   } else if constexpr (R == kRowsMx8) {
     return launch_rows8(g, cus, stream);
+  } else if constexpr (R == kRowsMx8Parts) {
+    return launch_rows8_parts(g, cus, stream);
   } else {
     if (tiles_of(g, 16, 64) <= 5 * cus / 2) return launch_few<R, 4, 1, 8, 2>(g, stream);
     return launch_rows(g, cus, stream);
@@ -154,6 +174,8 @@ extern "C" int lmoe_mx4_linear(const void* x, const void* x_scale, int rows, int
   const LinearArgs g{x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(w), T, K, N, bias,
                      static_cast<const uint16_t*>(add), out, bias_f32 != 0, out_f32 != 0, 1};
   if (rows == kRowsMx4) return launch_linear<kRowsMx4>(g, stream);
-  if (rows == kRowsMx8) return launch_linear<kRowsMx8>(g, stream);
+  // 8-bit rows: what one instruction's fixed-point sums lose, some 1e-4 of a result, would be
+  // most of an f32 output's error and does not show beside a bf16 store's 1.7e-3
+  if (rows == kRowsMx8) return out_f32 ? launch_linear<kRowsMx8Parts>(g, stream) : launch_linear<kRowsMx8>(g, stream);
   return launch_linear<kRowsBf16>(g, stream);
 }

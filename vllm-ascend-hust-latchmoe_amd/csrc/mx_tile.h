@@ -72,10 +72,17 @@ struct TileFrag<kRowsMx8> {
   __device__ __forceinline__ i32x8_t operand() const { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
 };
 
+template <>
+struct TileFrag<kRowsMx8Parts> : TileFrag<kRowsMx8> {};
+
 // W x^T of one chunk; B: the byte of both scales.
 template <int R, int B>
 __device__ __forceinline__ f32x4_t mx_step(const i32x4_t w, int ws, const TileFrag<R>& x, int xs, f32x4_t acc) {
   const i32x8_t a = __builtin_shufflevector(w, w, 0, 1, 2, 3, 0, 1, 2, 3);
+  if constexpr (R == kRowsMx8Parts) {
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, rows8_part<false>(x.operand()), acc, 4, 0, B, ws, B, xs);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, rows8_part<true>(x.operand()), acc, 4, 0, B, ws, B, xs);
+  }
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x.operand(), acc, 4 /* e2m1 */, R == kRowsMx8 ? 0 : 4, B, ws,
                                                           B, xs);
 }
@@ -87,7 +94,7 @@ struct MxShape {
   static constexpr int R = R_, MI = MI_, NJ = NJ_, WR = WR_, WC = WC_, NB = NB_;
   static constexpr int BM = 16 * MI * WR, BN = 16 * NJ * WC;
   static constexpr int WAVES = WR * WC, THREADS = 64 * WAVES;
-  static constexpr int PIECES = R == kRowsMx8 ? 8 : 4;  // 16-byte pieces of a row's chunk
+  static constexpr int PIECES = holds_mx8(R) ? 8 : 4;  // 16-byte pieces of a row's chunk
   static constexpr int ROWB = 16 * PIECES, RPL = 64 / PIECES;  // its bytes; rows of a load instruction
   static constexpr int PART_A = BM * ROWB, PART_B = BN * 64, STAGE = PART_A + PART_B;
   static constexpr int QA = PART_A / 1024 / WAVES, QB = BN / 16 / WAVES;  // load instructions of a wave and chunk
@@ -101,7 +108,7 @@ struct MxShape {
   static_assert(LDS <= 160 * 1024 && BM <= THREADS && QA * 1024 * WAVES == PART_A && QB * 16 * WAVES == BN);
   // piece p of row r lies at position p ^ sw(r)
   static __device__ __forceinline__ int sw(int r) {
-    return R == kRowsMx8 ? (r >> 1) & 7 : (0x78 >> (2 * ((r >> 2) & 3))) & 3;
+    return holds_mx8(R) ? (r >> 1) & 7 : (0x78 >> (2 * ((r >> 2) & 3))) & 3;
   }
 };
 
@@ -256,7 +263,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx_tile_kernel(TileArgs<OP> g) 
   for (int q = 0; q < C::QB; ++q) issue_ws(q, 0);
 #pragma unroll
   for (int q = 0; q < C::QA; ++q)
-    a_off[q] = static_cast<uint32_t>(source_row(a_row(q), a_pair[q])) * (R == kRowsMx8 ? K : K >> 1) + a_piece(q) * 16;
+    a_off[q] = static_cast<uint32_t>(source_row(a_row(q), a_pair[q])) * (holds_mx8(R) ? K : K >> 1) + a_piece(q) * 16;
   // the rows' scales of a quad, as they lie: PER_ROW threads to a row
   constexpr int SB = sizeof(typename C::scales_t);
   const uint8_t* my_scales = g.a_scale + (row0 + source_row(s_row, scale_pair)) * groups;
@@ -462,6 +469,10 @@ using Tile8_128x256 = MxShape<kRowsMx8, 4, 4, 2, 4, 4>;
 using Tile8_128x128 = MxShape<kRowsMx8, 4, 4, 2, 2, 3>;
 using Tile8_64x128 = MxShape<kRowsMx8, 2, 4, 2, 2, 4>;
 using Tile8_64x64 = MxShape<kRowsMx8, 2, 2, 2, 2, 4>;
+using Tile8P_128x256 = MxShape<kRowsMx8Parts, 4, 4, 2, 4, 4>;
+using Tile8P_128x128 = MxShape<kRowsMx8Parts, 4, 4, 2, 2, 3>;
+using Tile8P_64x128 = MxShape<kRowsMx8Parts, 2, 4, 2, 2, 4>;
+using Tile8P_64x64 = MxShape<kRowsMx8Parts, 2, 2, 2, 2, 4>;
 
 template <Op OP, class C>
 int launch_mx(const TileArgs<OP>& g, long long grid, hipStream_t stream) {
