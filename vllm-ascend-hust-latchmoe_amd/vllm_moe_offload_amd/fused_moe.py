@@ -95,43 +95,58 @@ def rows_kind(hidden, w13_slots) -> str:
     return kind
 
 
-def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = "", rows: str = "") -> MoEWorkspace:
+# Up to this many pairs the rows of 4-bit experts' second product stay f32 up to the combine.
+# Of 4-bit rows past 1024 pairs, us of the captured layer with y in bf16 / f32 (tokens, H, I,
+# experts, top k): 130, 2048, 768, 128, 8 71 / 71; 333, 2048, 1408, 60, 4 72.2 / 73.1; 600,
+# 4096, 1024, 16, 2 51.0 / 53.9; 600, 2048, 1408, 60, 4 75.5 / 78.0; 512, 2048, 768, 128, 8
+# 79.8 / 85.0, and past 4096 pairs 1024 of these 105 / 116, 2048 145 / 167, 4096 215 / 267;
+# 2049, 7168, 2048, 32, 4 338 / 387.
+Y_F32_MAX_PAIRS = {"bf16": native.FUSED_DECODE_MAX_PAIRS, "mx8": native.FUSED_DECODE_MAX_PAIRS, "mx4": 4096}
+
+
+def get_workspace(T: int, k: int, P: int, H: int, I: int, device, *, tag: str = "", rows: str = "",
+                  y_f32: bool = False) -> MoEWorkspace:
     """The workspace of a layer shape.  rows: rows_kind of its experts.  4-bit
     experts' rows of a few tokens stay f32 until the combine, and bf16 act rows
     are in two parts (their bytes are few beside the weights').  Past
-    FUSED_DECODE_MAX_PAIRS pairs both are bf16, as bf16 experts' rows are: their
+    Y_F32_MAX_PAIRS pairs (act: FUSED_DECODE_MAX_PAIRS) both are bf16, as bf16 experts' rows are: their
     bytes are then a good part of all (134 MB of y beside 321 MB of weights at 4096
     tokens x 8 of 128 experts, 2048 x 768, and twice that in f32).  The layer's
     error is 2.9e-3 of the output's size there, 1.65e-3 below (its own rounding;
-    512 experts of 1024 x 512, 960 pairs against 1280 and 4800).
+    512 experts of 1024 x 512, 960 pairs against 1280 and 4800), of 4-bit rows 2.4e-3
+    and 1.7e-3.  y_f32: they stay f32 however many there are (4-bit experts).
 
     Calls that take the same workspace must run one after the other, so each
     stream (the device's current one) and each host thread has its own.  Inside a
     capture it is a new one each time, of the graph's memory, which the caller keeps
     while it captures."""
-    return _workspace(T, k, P, H, I, device, tag, rows, True)
+    return _workspace(T, k, P, H, I, device, tag, rows, True, y_f32)
 
 
-def _workspace(T, k, P, H, I, device, tag: str, rows: str, cleared: bool) -> MoEWorkspace:
+def _workspace(T, k, P, H, I, device, tag: str, rows: str, cleared: bool, y_f32: bool = False) -> MoEWorkspace:
     if rows not in ("", "bf16", "mx8", "mx4"):
         raise ValueError(f"unknown rows {rows!r}")
+    if y_f32 and rows == "":
+        raise ValueError("y_f32 is for 4-bit experts (rows=)")
+    y_f32 = y_f32 or rows != "" and T * k <= Y_F32_MAX_PAIRS[rows]
     where = _device_key(device)
     stream = 0
     if where[0] == "cuda":
         if torch.cuda.is_current_stream_capturing():
-            return _make_workspace(int(T), int(k), int(P), int(H), int(I), device, rows, cleared=cleared)
+            return _make_workspace(int(T), int(k), int(P), int(H), int(I), device, rows, y_f32, cleared=cleared)
         stream = native.current_stream_handle(where[1])
-    key = (int(T), int(k), int(P), int(H), int(I), where, tag, rows, stream, threading.get_ident())
+    key = (int(T), int(k), int(P), int(H), int(I), where, tag, rows, y_f32, stream, threading.get_ident())
     ws = _WORKSPACES.get(key)
     if ws is None:
-        ws = _WORKSPACES[key] = _make_workspace(*key[:5], device, rows)
+        ws = _WORKSPACES[key] = _make_workspace(*key[:5], device, rows, y_f32)
     return ws
 
 
-def _make_workspace(T: int, k: int, P: int, H: int, I: int, device, rows: str, *, cleared: bool = True) -> MoEWorkspace:
+def _make_workspace(T: int, k: int, P: int, H: int, I: int, device, rows: str, y_f32: bool, *,
+                    cleared: bool = True) -> MoEWorkspace:
     N = T * k
     few = rows != "" and N <= native.FUSED_DECODE_MAX_PAIRS
-    y_dtype = torch.float32 if few else torch.bfloat16
+    y_dtype = torch.float32 if y_f32 else torch.bfloat16
     ws = MoEWorkspace(
         perm=native.Permutation.allocate(N, P, device, cleared=cleared),
         act=native.Mx8Rows.allocate(max(N, 1), I, device) if rows == "mx8" else
@@ -247,6 +262,9 @@ def fused_experts(
 
     The result is out; without it a new tensor, or with a workspace of the
     caller's that workspace's out, which its next call overwrites.
+
+    The pairs' rows are bf16 before the weighted sum, of 4-bit banks f32 up to
+    Y_F32_MAX_PAIRS pairs, or as the workspace has them (get_workspace(y_f32=True)).
 
     Over 4-bit banks (uint8, mxfp4.pack_experts) hidden is bf16, native.Mx8Rows or
     native.Mx4Rows (act is then rounded to 4 bits between the products); few tokens
