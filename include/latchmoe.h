@@ -489,6 +489,11 @@ int lmoe_mx4_linear(const void* x, const void* x_scale, int rows, int T, int K,
                     int N, const void* w, const void* bias, int bias_f32,
                     const void* add, void* out, int out_f32, hipStream_t stream);
 
+/* The form that lmoe_mx4_linear takes for these sizes (its checks of them, T > 0) on a card
+ * of cus compute units (0: the current device's): form[0] rows by form[1] columns of out a
+ * workgroup, form[2] 1 where its waves split K and 0 for a row tile.  Queues nothing. */
+int lmoe_mx4_linear_form(int rows, int out_f32, int T, int K, int N, int cus, int* form);
+
 /* Bytes of MX4 weights of [N, K]; -1 unless N % 16 == 0 and K % 32 == 0. */
 long long lmoe_mx4_bytes(int N, int K);
 

@@ -23,6 +23,13 @@ static long long tiles_of(const LinearArgs& g, long long BM, long long BN) {
   return (g.T + BM - 1) / BM * ((g.N + BN - 1) / BN);
 }
 
+// A workgroup's rows and columns.  split_k: its waves split K (mx4_linear_few_kernel), else
+// a row tile.
+struct LinearForm {
+  int rows, cols;
+  bool split_k;
+};
+
 // bf16 rows in row tiles: the shorter ones while they do not fill the card.  us of 128 / 64 /
 // 32 rows (workgroups of 32 rows):
 //   300 x 2048 x 5120   (200)   30.6 / 21.2 / 14.2
@@ -30,16 +37,8 @@ static long long tiles_of(const LinearArgs& g, long long BM, long long BN) {
 //   1024 x 7168 x 7168  (896)   108 / 94.0 / 108
 //   4096 x 2048 x 5120  (2560)  79.3 / 71.1 / 86.8
 //   4096 x 7168 x 7168  (3584)  316 / 321 / 381
-static int launch_rows(LinearArgs g, int cus, hipStream_t stream) {
-  const int bm = tiles_of(g, 32, kTileCols) <= 2 * cus ? 32 : tiles_of(g, 64, kTileCols) <= 5 * cus ? 64 : 128;
-  const long long grid = linear_grid(&g, bm, kTileCols);
-  int st;
-  if (bm == 128) st = launch_tile<Op::kLinear, false, 128, 1>(g, grid, stream);
-  else if (bm == 64) st = launch_tile<Op::kLinear, false, 64, 1>(g, grid, stream);
-  else if (grid <= 2 * cus) st = launch_tile<Op::kLinear, false, 32, 2>(g, grid, stream);
-  else st = launch_tile<Op::kLinear, false, 32, 1>(g, grid, stream);
-  if (st != LMOE_OK) return st;
-  LMOE_RETURN_LAUNCH();
+static int rows16_height(const LinearArgs& g, int cus) {
+  return tiles_of(g, 32, kTileCols) <= 2 * cus ? 32 : tiles_of(g, 64, kTileCols) <= 5 * cus ? 64 : 128;
 }
 
 // MX4 and MX8 rows: the shape with the least time by this measure, in tenths of a us: for
@@ -71,11 +70,12 @@ constexpr ShapeCost kShapes8[5] = {{256, 256, 1, 67, {12.0}}, {128, 256, 1, 41, 
 constexpr ShapeCost kShapes8Parts[4] = {{128, 256, 1, 64, {14.0}}, {128, 128, 2, 48, {10.4, 15.2}},
                                         {64, 128, 2, 35, {6.2, 8.4}}, {64, 64, 3, 32, {4.3, 6.7, 8.0}}};
 
-static int cheapest(const ShapeCost* shapes, int n, const LinearArgs& g, int cus) {
+template <int S>
+static LinearForm cheapest(const ShapeCost (&shapes)[S], const LinearArgs& g, int cus) {
   const int chunks = mx4_chunks(g.K);
   int best = 0;
   double least = 0;
-  for (int s = 0; s < n; ++s) {
+  for (int s = 0; s < S; ++s) {
     const ShapeCost& c = shapes[s];
     const long long each = (tiles_of(g, c.BM, c.BN) + cus - 1) / cus;  // a CU's tiles
     const long long full = each / c.at_once, last = each % c.at_once;
@@ -86,31 +86,7 @@ static int cheapest(const ShapeCost* shapes, int n, const LinearArgs& g, int cus
       least = time;
     }
   }
-  return best;
-}
-
-static int launch_rows4(const LinearArgs& g, int cus, hipStream_t stream) {
-  const int shape = cheapest(kShapes4, 4, g, cus);
-  if (shape == 0) return launch_mx_linear<Tile4_256x256>(g, stream);
-  if (shape == 1) return launch_mx_linear<Tile4_128x128>(g, stream);
-  if (shape == 2) return launch_mx_linear<Tile4_64x128>(g, stream);
-  return launch_mx_linear<Tile4_64x64>(g, stream);
-}
-static int launch_rows8(const LinearArgs& g, int cus, hipStream_t stream) {
-  const int shape = cheapest(kShapes8, 5, g, cus);
-  if (shape == 0) return launch_mx_linear<Tile8_256x256>(g, stream);
-  if (shape == 1) return launch_mx_linear<Tile8_128x256>(g, stream);
-  if (shape == 2) return launch_mx_linear<Tile8_128x128>(g, stream);
-  if (shape == 3) return launch_mx_linear<Tile8_64x128>(g, stream);
-  return launch_mx_linear<Tile8_64x64>(g, stream);
-}
-
-static int launch_rows8_parts(const LinearArgs& g, int cus, hipStream_t stream) {
-  const int shape = cheapest(kShapes8Parts, 4, g, cus);
-  if (shape == 0) return launch_mx_linear<Tile8P_128x256>(g, stream);
-  if (shape == 1) return launch_mx_linear<Tile8P_128x128>(g, stream);
-  if (shape == 2) return launch_mx_linear<Tile8P_64x128>(g, stream);
-  return launch_mx_linear<Tile8P_64x64>(g, stream);
+  return {shapes[best].BM, shapes[best].BN, false};
 }
 
 // Split K while that makes workgroups enough: for the fewest rows 32 columns by 16 rows a
@@ -129,24 +105,70 @@ static int launch_rows8_parts(const LinearArgs& g, int cus, hipStream_t stream) 
 //   MX8 rows     12.4 / 12.3 / 11.2  15.6 / 14.5 / 12.3  8.5 / 8.6 / 7.7    31.0 / 24.6 / 21.7
 //   bf16 rows    15.2 / 13.7 / 12.1  20.5 / 16.8 / 14.3  10.4 / 10.0 / 8.4  36.5 / 27.8 / 23.8
 // and below, 8 x 7168 x 16384: 13.2 / 12.9 / 16.4, 14.0 / 13.0 / 16.5, 16.0 / 14.3 / 17.5.
+static LinearForm linear_form(int rows, const LinearArgs& g, int cus) {
+  if (g.T <= 16 && g.N > 16384) return {16, 128, true};
+  if (g.T <= 16 || tiles_of(g, 16, 32) <= cus) return {16, 32, true};
+  if (tiles_of(g, 16, 64) <= cus + cus / 4) return {16, 64, true};
+  if (tiles_of(g, 32, 64) <= cus) return {32, 64, true};
+  if (rows == kRowsMx4) return cheapest(kShapes4, g, cus);
+  if (rows == kRowsMx8) return cheapest(kShapes8, g, cus);
+  if (rows == kRowsMx8Parts) return cheapest(kShapes8Parts, g, cus);
+  if (tiles_of(g, 16, 64) <= 5 * cus / 2) return {16, 64, true};
+  return {rows16_height(g, cus), kTileCols, false};
+}
+
+template <int BM, int CS>
+static int launch_rows16(LinearArgs g, long long grid, hipStream_t stream) {
+  const int st = launch_tile<Op::kLinear, false, BM, CS>(g, grid, stream);
+  if (st != LMOE_OK) return st;
+  LMOE_RETURN_LAUNCH();
+}
+
 template <int R>
-static int launch_linear(const LinearArgs& g, hipStream_t stream) {
+static int launch_linear(LinearArgs g, hipStream_t stream) {
   const int cus = device_cus();
-  if (g.T <= 16 && g.N > 16384) return launch_few<R, 8, 1, 8, 1>(g, stream);
-  if (g.T <= 16 || tiles_of(g, 16, 32) <= cus) return launch_few<R, 2, 1, 8, 2>(g, stream);
-  if (tiles_of(g, 16, 64) <= cus + cus / 4) return launch_few<R, 4, 1, 8, 2>(g, stream);
-  if (tiles_of(g, 32, 64) <= cus) return launch_few<R, 4, 2, 8, 2>(g, stream);
+  const LinearForm f = linear_form(R, g, cus);
+  auto is = [&](int rows, int cols) { return f.rows == rows && f.cols == cols; };
+  if (f.split_k) {
+    if (is(16, 128)) return launch_few<R, 8, 1, 8, 1>(g, stream);
+    if (is(16, 32)) return launch_few<R, 2, 1, 8, 2>(g, stream);
+    if (is(16, 64)) return launch_few<R, 4, 1, 8, 2>(g, stream);
+    return launch_few<R, 4, 2, 8, 2>(g, stream);
+  }
   if constexpr (R == kRowsMx4) {
-    return launch_rows4(g, cus, stream);
+    if (is(256, 256)) return launch_mx_linear<Tile4_256x256>(g, stream);
+    if (is(128, 128)) return launch_mx_linear<Tile4_128x128>(g, stream);
+    if (is(64, 128)) return launch_mx_linear<Tile4_64x128>(g, stream);
+    return launch_mx_linear<Tile4_64x64>(g, stream);
   } else if constexpr (R == kRowsMx8) {
-    return launch_rows8(g, cus, stream);
+    if (is(256, 256)) return launch_mx_linear<Tile8_256x256>(g, stream);
+    if (is(128, 256)) return launch_mx_linear<Tile8_128x256>(g, stream);
+    if (is(128, 128)) return launch_mx_linear<Tile8_128x128>(g, stream);
+    if (is(64, 128)) return launch_mx_linear<Tile8_64x128>(g, stream);
+    return launch_mx_linear<Tile8_64x64>(g, stream);
   } else if constexpr (R == kRowsMx8Parts) {
-    return launch_rows8_parts(g, cus, stream);
+    if (is(128, 256)) return launch_mx_linear<Tile8P_128x256>(g, stream);
+    if (is(128, 128)) return launch_mx_linear<Tile8P_128x128>(g, stream);
+    if (is(64, 128)) return launch_mx_linear<Tile8P_64x128>(g, stream);
+    return launch_mx_linear<Tile8P_64x64>(g, stream);
   } else {
-    if (tiles_of(g, 16, 64) <= 5 * cus / 2) return launch_few<R, 4, 1, 8, 2>(g, stream);
-    return launch_rows(g, cus, stream);
+    const long long grid = linear_grid(&g, f.rows, f.cols);
+    if (f.rows == 128) return launch_rows16<128, 1>(g, grid, stream);
+    if (f.rows == 64) return launch_rows16<64, 1>(g, grid, stream);
+    if (grid <= 2 * cus) return launch_rows16<32, 2>(g, grid, stream);
+    return launch_rows16<32, 1>(g, grid, stream);
   }
 }
+
+// The checks of sizes.
+static int check_sizes(int rows, int T, int K, int N) {
+  if (T < 0 || K <= 0 || N <= 0) return LMOE_ERR_ARG;
+  if (rows != kRowsBf16 && rows != kRowsMx8 && rows != kRowsMx4) return LMOE_ERR_UNSUPPORTED;
+  return K % kMxGroup != 0 || N % 16 != 0 || K > kMxMaxColumns ? LMOE_ERR_SHAPE : LMOE_OK;
+}
+// 8-bit rows: what one instruction's fixed-point sums lose, some 1e-4 of a result, would be
+// most of an f32 output's error and does not show beside a bf16 store's 1.7e-3.
+static int rows_taken(int rows, int out_f32) { return rows == kRowsMx8 && out_f32 ? kRowsMx8Parts : rows; }
 
 }  // namespace lmoe
 
@@ -155,10 +177,8 @@ using namespace lmoe;
 extern "C" int lmoe_mx4_linear(const void* x, const void* x_scale, int rows, int T, int K, int N, const void* w,
                                const void* bias, int bias_f32, const void* add, void* out, int out_f32,
                                hipStream_t stream) {
-  if (T < 0 || K <= 0 || N <= 0) return LMOE_ERR_ARG;
-  if (rows != kRowsBf16 && rows != kRowsMx8 && rows != kRowsMx4) return LMOE_ERR_UNSUPPORTED;
-  if (K % kMxGroup != 0 || N % 16 != 0 || K > kMxMaxColumns) return LMOE_ERR_SHAPE;
-  if (T == 0) return LMOE_OK;
+  const int st = check_sizes(rows, T, K, N);
+  if (st != LMOE_OK || T == 0) return st;
   if (x == nullptr || w == nullptr || out == nullptr || (x_scale == nullptr) != (rows == kRowsBf16)) return LMOE_ERR_ARG;
   if (misaligned16(x) || misaligned16(w) || misaligned16(bias) || misaligned16(add) || misaligned16(out))
     return LMOE_ERR_SHAPE;
@@ -173,9 +193,25 @@ extern "C" int lmoe_mx4_linear(const void* x, const void* x_scale, int rows, int
     if (overlap(o, in[i]) && !(i == 4 && add == out && !out_f32)) return LMOE_ERR_ARG;
   const LinearArgs g{x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(w), T, K, N, bias,
                      static_cast<const uint16_t*>(add), out, bias_f32 != 0, out_f32 != 0, 1};
-  if (rows == kRowsMx4) return launch_linear<kRowsMx4>(g, stream);
-  // 8-bit rows: what one instruction's fixed-point sums lose, some 1e-4 of a result, would be
-  // most of an f32 output's error and does not show beside a bf16 store's 1.7e-3
-  if (rows == kRowsMx8) return out_f32 ? launch_linear<kRowsMx8Parts>(g, stream) : launch_linear<kRowsMx8>(g, stream);
-  return launch_linear<kRowsBf16>(g, stream);
+  switch (rows_taken(rows, out_f32)) {
+    case kRowsMx4: return launch_linear<kRowsMx4>(g, stream);
+    case kRowsMx8: return launch_linear<kRowsMx8>(g, stream);
+    case kRowsMx8Parts: return launch_linear<kRowsMx8Parts>(g, stream);
+    default: return launch_linear<kRowsBf16>(g, stream);
+  }
+}
+
+extern "C" int lmoe_mx4_linear_form(int rows, int out_f32, int T, int K, int N, int cus, int* form) {
+  const int st = check_sizes(rows, T, K, N);
+  if (st != LMOE_OK) return st;
+  if (T == 0 || cus < 0 || form == nullptr) return LMOE_ERR_ARG;
+  LinearArgs g{};
+  g.T = T;
+  g.K = K;
+  g.N = N;
+  const LinearForm f = linear_form(rows_taken(rows, out_f32), g, cus > 0 ? cus : device_cus());
+  form[0] = f.rows;
+  form[1] = f.cols;
+  form[2] = f.split_k;
+  return LMOE_OK;
 }

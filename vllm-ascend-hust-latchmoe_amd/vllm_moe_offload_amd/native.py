@@ -74,6 +74,7 @@ EXPORTED_SYMBOLS = (
     "lmoe_mx4_quantize",
     "lmoe_mx4_bank_values",
     "lmoe_mx4_linear",
+    "lmoe_mx4_linear_form",
     "lmoe_mx4_bytes",
     "lmoe_mx4_gateup_silu",
     "lmoe_mx4_down",
@@ -169,6 +170,7 @@ _SIGNATURES = {
     "lmoe_mx4_quantize": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp]),
     "lmoe_mx4_bank_values": (_i, [_vp, _i, _i, _i, _i, _vp, _i, _vp]),
     "lmoe_mx4_linear": (_i, [_vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _i, _vp]),
+    "lmoe_mx4_linear_form": (_i, [_i, _i, _i, _i, _i, _i, _vp]),
     "lmoe_mx4_bytes": (ctypes.c_longlong, [_i, _i]),
     "lmoe_mx4_gateup_silu": (
         _i,
@@ -796,6 +798,15 @@ def mx4_linear(x, w: torch.Tensor, out: torch.Tensor | None = None, *, bias: tor
             raise ValueError("operands overlap: out over an operand other than a bf16 add")
         _check(status, "lmoe_mx4_linear")
     return out
+
+
+def mx4_linear_form(kind: str, T: int, K: int, N: int, *, out_f32: bool = False, cu_count: int = 0) -> tuple[int, int, bool]:
+    """(rows, columns of a workgroup, whether its waves split K) of mx4_linear for T rows of
+    kind "bf16", "mx8" or "mx4" on a card of cu_count compute units (0: the current one)."""
+    form = (ctypes.c_int * 3)()
+    _check(load_library().lmoe_mx4_linear_form(("bf16", "mx8", "mx4").index(kind), out_f32, T, K, N, cu_count, form),
+           "lmoe_mx4_linear_form")
+    return form[0], form[1], bool(form[2])
 
 
 # ---------------------------------------------------------------------------
