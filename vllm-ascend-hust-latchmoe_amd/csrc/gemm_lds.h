@@ -39,6 +39,7 @@
 // up rows I+i0..; kDown writes y[pair][h] in flat pair order.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "gemm_mfma.h"
@@ -358,15 +359,15 @@ __global__ __launch_bounds__(C::THREADS) void grouped_gemm_lds_kernel(GemmArgs g
 
 // CUs of the current device, queried once per device.
 static int device_cus() {
-  static int cached[64] = {0};
+  static std::atomic<int> cached[64] = {};  // host threads may call at once
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 256;
-  if (dev < 64 && cached[dev] > 0) return cached[dev];
+  if (const int known = dev < 64 ? cached[dev].load(std::memory_order_relaxed) : 0; known > 0) return known;
   int cus = 0;
   if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
       cus <= 0)
     cus = 256;
-  if (dev < 64) cached[dev] = cus;
+  if (dev < 64) cached[dev].store(cus, std::memory_order_relaxed);
   return cus;
 }
 

@@ -33,6 +33,7 @@
 // Every output adds its chunks in order, whatever BM is: the same bits.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "mx4_linear.h"
@@ -401,20 +402,30 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void mx4_tile_kernel(TileArgs<O
   }
 }
 
+// Devices on which a kernel may take all of LDS, which past 64 KiB it has to be allowed to.
+// Host threads may call at once: each then asks for the same.
+struct LdsRaised {
+  std::atomic<bool> on[64] = {};
+};
+inline int raise_lds(const void* kernel, LdsRaised& raised) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return static_cast<int>(e);
+  const bool known = dev >= 0 && dev < 64;
+  if (known && raised.on[dev].load(std::memory_order_relaxed)) return LMOE_OK;
+  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  if (e != hipSuccess) return static_cast<int>(e);
+  if (known) raised.on[dev].store(true, std::memory_order_relaxed);
+  return LMOE_OK;
+}
+
 template <Op OP, bool A8, int BM, int CS>
 int launch_tile(const TileArgs<OP>& g, long long grid, hipStream_t stream) {
   if (grid > 0x7fffffffLL) return LMOE_ERR_SHAPE;
   const int lds = Mx4Tile<A8, BM, CS>::lds_bytes(mx4_chunks(g.K));
-  static bool raised[64] = {};  // per device: dynamic LDS past 64 KiB allowed
-  int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
-  if (e != hipSuccess) return static_cast<int>(e);
-  if (dev < 0 || dev >= 64 || !raised[dev]) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx4_tile_kernel<OP, A8, BM, CS>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (e != hipSuccess) return static_cast<int>(e);
-    if (dev >= 0 && dev < 64) raised[dev] = true;
-  }
+  static LdsRaised raised;
+  const int st = raise_lds(reinterpret_cast<const void*>(mx4_tile_kernel<OP, A8, BM, CS>), raised);
+  if (st != LMOE_OK) return st;
   mx4_tile_kernel<OP, A8, BM, CS><<<static_cast<unsigned>(grid), kTileWaves * 64, lds, stream>>>(g);
   return LMOE_OK;
 }

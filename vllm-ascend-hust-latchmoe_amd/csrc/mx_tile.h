@@ -477,16 +477,9 @@ using Tile8P_64x64 = MxShape<kRowsMx8Parts, 2, 2, 2, 2, 4>;
 template <Op OP, class C>
 int launch_mx(const TileArgs<OP>& g, long long grid, hipStream_t stream) {
   if (grid > 0x7fffffffLL) return LMOE_ERR_SHAPE;
-  static bool raised[64] = {};  // per device: dynamic LDS past 64 KiB allowed
-  int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
-  if (e != hipSuccess) return static_cast<int>(e);
-  if (dev < 0 || dev >= 64 || !raised[dev]) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx_tile_kernel<OP, C>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (e != hipSuccess) return static_cast<int>(e);
-    if (dev >= 0 && dev < 64) raised[dev] = true;
-  }
+  static LdsRaised raised;
+  const int st = raise_lds(reinterpret_cast<const void*>(mx_tile_kernel<OP, C>), raised);
+  if (st != LMOE_OK) return st;
   mx_tile_kernel<OP, C><<<static_cast<unsigned>(grid), C::THREADS, C::LDS, stream>>>(g);
   LMOE_RETURN_LAUNCH();
 }
