@@ -15,22 +15,22 @@ pytestmark = pytest.mark.gpu
 
 #: kind of rows ("-f32": into f32), a workgroup's rows and columns, T, K, N
 CASES = [
-    ("bf16", 32, 256, 333, 672, 2064), ("bf16", 32, 256, 600, 1184, 6640),
+    ("bf16", 32, 256, 333, 672, 2064), ("bf16", 32, 256, 1030, 2080, 3088),
     ("bf16", 64, 256, 1000, 672, 4112), ("bf16", 64, 256, 1030, 1376, 6640),
-    ("bf16", 128, 256, 4090, 672, 5136), ("bf16", 128, 256, 3001, 1440, 7184),
+    ("bf16", 128, 256, 2050, 2080, 5136), ("bf16", 128, 256, 4090, 2080, 3088),
     ("mx8", 64, 64, 301, 672, 2064), ("mx8", 64, 64, 600, 1184, 2064),
-    ("mx8", 64, 128, 333, 2080, 3088), ("mx8", 64, 128, 700, 1184, 5136),
-    ("mx8", 128, 128, 600, 672, 5136), ("mx8", 128, 128, 1000, 1376, 5136),
+    ("mx8", 64, 128, 333, 2080, 3088), ("mx8", 64, 128, 600, 672, 5136),
+    ("mx8", 128, 128, 1030, 672, 6640), ("mx8", 128, 128, 1030, 1376, 6640),
     ("mx8", 128, 256, 1000, 2080, 4112), ("mx8", 128, 256, 2050, 2080, 2064),
     ("mx8", 256, 256, 2050, 1376, 4112), ("mx8", 256, 256, 4090, 2080, 2064),
     ("mx8-f32", 64, 64, 301, 672, 2064), ("mx8-f32", 64, 64, 333, 1184, 2064),
-    ("mx8-f32", 64, 128, 333, 672, 3088), ("mx8-f32", 64, 128, 1030, 2080, 1040),
-    ("mx8-f32", 128, 128, 600, 672, 6640), ("mx8-f32", 128, 128, 1500, 1440, 4112),
-    ("mx8-f32", 128, 256, 1000, 2080, 4112), ("mx8-f32", 128, 256, 2050, 2080, 3088),
+    ("mx8-f32", 64, 128, 700, 672, 4112), ("mx8-f32", 64, 128, 1000, 2080, 5136),
+    ("mx8-f32", 128, 128, 1030, 672, 5136), ("mx8-f32", 128, 128, 1500, 1440, 4112),
     ("mx4", 64, 64, 301, 672, 2064), ("mx4", 64, 64, 700, 1184, 1040),
-    ("mx4", 64, 128, 333, 672, 3088), ("mx4", 64, 128, 600, 1440, 2064),
-    ("mx4", 128, 128, 1030, 672, 2064), ("mx4", 128, 128, 1000, 1376, 5136),
+    ("mx4", 64, 128, 700, 672, 4112), ("mx4", 64, 128, 1000, 1376, 4112),
+    ("mx4", 128, 128, 1030, 672, 5136), ("mx4", 128, 128, 1500, 1376, 4112),
     ("mx4", 256, 256, 3001, 1376, 4112), ("mx4", 256, 256, 4090, 2080, 7184),
+    ("bf16", 32, 256, 2050, 1440, 7184),  # more than two workgroups a unit
 ]
 ONE_EACH = CASES[::2]
 SCALED = [c for c in ONE_EACH if c[0] != "bf16"]

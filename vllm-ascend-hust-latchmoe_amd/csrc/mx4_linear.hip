@@ -30,54 +30,59 @@ struct LinearForm {
   bool split_k;
 };
 
-// bf16 rows in row tiles: the shorter ones while they do not fill the card.  us of 128 / 64 /
-// 32 rows (workgroups of 32 rows):
-//   300 x 2048 x 5120   (200)   30.6 / 21.2 / 14.2
-//   512 x 7168 x 7168   (448)   106 / 73.5 / 56.8
-//   1024 x 7168 x 7168  (896)   108 / 94.0 / 108
-//   4096 x 2048 x 5120  (2560)  79.3 / 71.1 / 86.8
-//   4096 x 7168 x 7168  (3584)  316 / 321 / 381
-static int rows16_height(const LinearArgs& g, int cus) {
-  return tiles_of(g, 32, kTileCols) <= 2 * cus ? 32 : tiles_of(g, 64, kTileCols) <= 5 * cus ? 64 : 128;
-}
-
-// MX4 and MX8 rows: the shape with the least time by this measure, in tenths of a us: for
-// each round of the workgroups that a CU has at once `round`, and for each of its chunks of K
-// the time of 1, 2, .. of them (the last round may have fewer).
+// Row tiles: the shape with the least time by this measure, in tenths of a us: for each
+// round of the workgroups that a CU has at once `round`, and for each of its chunks of K the
+// time of 1, 2, .. of them (the last round may have fewer).  A CU's workgroups are those of
+// the XCD that has most: 2839 x 6752 x 5136 in tiles of 256 x 256 are 252, but 33 of one XCD's
+// 32 CUs, and take 1.7 times what tiles of 128 x 256 do.  The constants are fitted to 900
+// random products of 100 to 5000 rows, 512 to 7360 columns and 640 to 9600 outputs, whose
+// chosen form takes 1.003 to 1.007 of the best one's time on average (before the XCDs were
+// counted: 1.015 to 1.04).  The figures below are
+// us of 20 calls in a row, of random values, the shapes in turn (a card that comes from
+// lighter work runs the largest up to 10% faster).
 struct ShapeCost {
   int BM, BN, at_once, round;
   double chunk[4];
 };
-// MX4 rows, us of 256 x 256 / 128 x 128 / 64 x 128 / 64 x 64 tiles: 4096 x 7168 x 7168 118 /
-// 146 / 184 / 252, 4096 x 2048 x 5120 39.9 / 35.2 / 39.6 / 46.5, 1024 x 7168 x 7168 51.0 /
-// 45.4 / 55.9 / 63.5, 300 x 2048 x 5120 19.8 / 10.3 / 8.5 / 8.2, 300 x 1408 x 2048 15.5 / 8.8
-// / 6.8 / 5.8
-constexpr ShapeCost kShapes4[4] = {{256, 256, 1, 43, {8.3}}, {128, 128, 2, 0, {4.7, 6.5}},
-                                   {64, 128, 3, 0, {3.4, 4.8, 6.6}}, {64, 64, 4, 0, {2.8, 3.6, 5.0, 6.4}}};
-// MX8 rows, us of 256 x 256 / 128 x 256 / 128 x 128 / 64 x 128 / 64 x 64 tiles: 4096 x 7168 x
-// 7168 161 / 182 / 198 / 243 / 436, 4096 x 2048 x 5120 54.3 / 51.5 / 46.8 / 54.7 / 67.4, 1024 x
-// 7168 x 7168 73.2 / 46.0 / 55.1 / 64.8 / 78.9, 512 x 7168 x 7168 72.1 / 43.0 / 43.3 / 34.1 /
-// 46.4, 300 x 2048 x 5120 25.7 / 16.1 / 13.1 / 9.0 / 9.2, 300 x 1408 x 2048 20.5 / 12.7 / 10.7 /
-// 7.3 / 6.1
-constexpr ShapeCost kShapes8[5] = {{256, 256, 1, 67, {12.0}}, {128, 256, 1, 41, {7.5}}, {128, 128, 2, 10, {7.5, 9.6}},
-                                   {64, 128, 2, 25, {3.6, 5.5}}, {64, 64, 3, 15, {3.3, 4.2, 4.9}}};
-
-// MX8 rows with f32 outputs, in two parts (twice the products; 256 x 256 tiles spill 112
-// registers), us of 128 x 256 / 128 x 128 / 64 x 128 / 64 x 64 tiles: 4096 x 7168 x 7168 352 /
-// 335 / 361 / 474, 4096 x 2048 x 5120 88.7 / 80.2 / 87.3 / 109, 1024 x 7168 x 7168 89.2 / 89.8 /
-// 95.2 / 115, 512 x 7168 x 7168 85.0 / 63.3 / 52.5 / 64.8, 300 x 2048 x 5120 29.3 / 21.4 / 13.8 /
-// 13.9, 300 x 1408 x 2048 21.8 / 16.3 / 10.4 / 8.4
-constexpr ShapeCost kShapes8Parts[4] = {{128, 256, 1, 64, {14.0}}, {128, 128, 2, 48, {10.4, 15.2}},
-                                        {64, 128, 2, 35, {6.2, 8.4}}, {64, 64, 3, 32, {4.3, 6.7, 8.0}}};
+// MX4 rows, 256 x 256 / 128 x 128 / 64 x 128 / 64 x 64 tiles:
+//   4096 x 7168 x 7168  112 / 143 / 181 / 256      512 x 7168 x 7168   44.3 / 23.8 / 25.1 / 32.0
+//   4096 x 2048 x 5120  40.0 / 35.4 / 40.6 / 48.7  300 x 2048 x 5120   18.4 / 10.1 / 8.2 / 8.1
+//   2048 x 7168 x 7168  56.7 / 73.8 / 83.5 / 114   300 x 1408 x 2048   15.1 / 8.7 / 6.8 / 5.6
+//   1024 x 7168 x 7168  48.5 / 37.5 / 47.0 / 55.2  1000 x 2048 x 2048  18.2 / 10.5 / 8.5 / 8.5
+constexpr ShapeCost kShapes4[4] = {{256, 256, 1, 74, {7.8}}, {128, 128, 2, 49, {3.5, 6.1}},
+                                   {64, 128, 3, 37, {3.0, 3.9, 5.7}}, {64, 64, 4, 29, {2.5, 3.4, 4.2, 5.5}}};
+// MX8 rows, 256 x 256 / 128 x 256 / 128 x 128 / 64 x 128 / 64 x 64 tiles:
+//   4096 x 7168 x 7168  167 / 186 / 199 / 246 / 437       512 x 7168 x 7168   73.1 / 40.8 / 36.7 / 31.0 / 41.4
+//   4096 x 2048 x 5120  59.4 / 53.4 / 48.1 / 58.3 / 70.1  300 x 2048 x 5120   26.0 / 15.6 / 12.9 / 9.1 / 9.5
+//   2048 x 7168 x 7168  90.7 / 94.4 / 104 / 109 / 149     300 x 1408 x 2048   21.0 / 12.2 / 10.4 / 7.3 / 6.1
+//   1024 x 7168 x 7168  81.1 / 47.0 / 52.8 / 62.2 / 73.4  1000 x 2048 x 2048  25.8 / 15.7 / 13.3 / 9.4 / 9.8
+constexpr ShapeCost kShapes8[5] = {{256, 256, 1, 87, {13.4}}, {128, 256, 1, 53, {6.8}}, {128, 128, 2, 40, {6.4, 9.7}},
+                                   {64, 128, 2, 42, {3.2, 4.4}}, {64, 64, 3, 35, {2.5, 3.8, 5.1}}};
+// MX8 rows with f32 outputs, in two parts (twice the products; tiles of 256 x 256 spill 112
+// registers, those of 128 x 256 are no faster anywhere), 128 x 128 / 64 x 128 / 64 x 64 tiles:
+//   4096 x 7168 x 7168  341 / 375 / 487     512 x 7168 x 7168   63.4 / 51.2 / 67.0
+//   4096 x 2048 x 5120  81.1 / 87.5 / 106   300 x 2048 x 5120   21.9 / 14.1 / 14.2
+//   2048 x 7168 x 7168  188 / 182 / 236     300 x 1408 x 2048   16.8 / 10.6 / 8.5
+//   1024 x 7168 x 7168  91.7 / 96.1 / 111   1000 x 2048 x 2048  22.1 / 14.6 / 15.0
+constexpr ShapeCost kShapes8Parts[3] = {{128, 128, 2, 66, {9.7, 15.5}}, {64, 128, 2, 40, {5.5, 7.7}},
+                                        {64, 64, 3, 38, {4.4, 5.5, 7.3}}};
+// bf16 rows, 128 x 256 / 64 x 256 / 32 x 256 tiles:
+//   8192 x 7168 x 7168  607 / 642             1024 x 7168 x 7168  111 / 90.1 / 111
+//   4096 x 7168 x 7168  350 / 332 / 396       512 x 7168 x 7168   107 / 73.9 / 57.2
+//   4096 x 2048 x 5120  88.8 / 73.6 / 89.4    300 x 2048 x 5120   31.0 / 21.2 / 14.5
+//   2048 x 7168 x 7168  169 / 185             4096 x 4096 x 4096  105 / 119
+constexpr ShapeCost kShapes16[3] = {{128, kTileCols, 2, 32, {19.2, 30.7}}, {64, kTileCols, 2, 0, {12.7, 16.5}},
+                                    {32, kTileCols, 2, 16, {8.3, 10.0}}};
 
 template <int S>
 static LinearForm cheapest(const ShapeCost (&shapes)[S], const LinearArgs& g, int cus) {
-  const int chunks = mx4_chunks(g.K);
+  const int chunks = mx4_chunks(g.K), per_xcd = cus < 8 ? 1 : cus / 8;
   int best = 0;
   double least = 0;
   for (int s = 0; s < S; ++s) {
     const ShapeCost& c = shapes[s];
-    const long long each = (tiles_of(g, c.BM, c.BN) + cus - 1) / cus;  // a CU's tiles
+    LinearArgs shared = g;
+    const long long each = (linear_grid(&shared, c.BM, c.BN) / 8 + per_xcd - 1) / per_xcd;  // a CU's tiles
     const long long full = each / c.at_once, last = each % c.at_once;
     double time = full * (c.round + chunks * c.chunk[c.at_once - 1]);
     if (last > 0) time += c.round + chunks * c.chunk[last - 1];
@@ -91,12 +96,11 @@ static LinearForm cheapest(const ShapeCost (&shapes)[S], const LinearArgs& g, in
 
 // Split K while that makes workgroups enough: for the fewest rows 32 columns by 16 rows a
 // workgroup, then 64 by 16, then 64 by 32.  us of these three and of row tiles (T x K x N):
-//              16 x 2048 x 5120   32 x 7168 x 7168      64 x 7168 x 7168      128 x 2048 x 5120
-//   MX4 rows   4.4 4.7 5.0  -     15.3 12.2 15.8 19.0   27.0 20.6 15.2 19.5     -    -   9.3  6.8
-//   MX8 rows    -   -   -   -       -    -    -    -    31.8 22.9 18.1 20.2   13.3 11.1 13.0  7.2
-//   bf16 rows  5.4 6.4 7.3  -     20.8 15.2 23.5   -    37.0 25.8 23.2 44.3   15.3 12.5 15.6 13.8
-// MX8 rows in two parts (f32 outputs) cost up to 0.4 us more there, 128 x 2048 x 5120 11.9 10.5
-// 13.2 10.8, 64 x 7168 x 7168 31.3 22.1 17.8 27.1.
+//                 16 x 2048 x 5120   32 x 7168 x 7168     64 x 7168 x 7168     128 x 2048 x 5120
+//   MX4 rows      4.4 5.3 5.6  7.0   14.9 11.5 15.2 16.7  25.9 20.3 14.7 17.3   9.4  9.2  9.0  7.5
+//   MX8 rows      5.0 5.6 6.1  7.3   17.5 12.5 17.5 17.8  30.4 22.0 17.0 18.2  12.4 10.2 12.0  7.9
+//   .. into f32   5.2 5.9 6.8  8.1   17.3 12.5 18.3 26.2  30.2 22.3 18.0 26.7  12.0 10.7 13.3 10.7
+//   bf16 rows     5.5 6.5 7.3 13.4   20.1 14.2 20.9 43.6  35.2 24.9 20.8 43.5  16.2 12.2 14.8 13.9
 // (bf16 rows' tiles need more workgroups than the others' to be worth it.)
 // Past 16384 columns, up to 16 rows, whose rows every workgroup reads again: 128 columns a
 // workgroup, a chunk at a time.  us of 32 / 64 / 128 columns:
@@ -114,7 +118,7 @@ static LinearForm linear_form(int rows, const LinearArgs& g, int cus) {
   if (rows == kRowsMx8) return cheapest(kShapes8, g, cus);
   if (rows == kRowsMx8Parts) return cheapest(kShapes8Parts, g, cus);
   if (tiles_of(g, 16, 64) <= 5 * cus / 2) return {16, 64, true};
-  return {rows16_height(g, cus), kTileCols, false};
+  return cheapest(kShapes16, g, cus);
 }
 
 template <int BM, int CS>
@@ -147,7 +151,6 @@ static int launch_linear(LinearArgs g, hipStream_t stream) {
     if (is(64, 128)) return launch_mx_linear<Tile8_64x128>(g, stream);
     return launch_mx_linear<Tile8_64x64>(g, stream);
   } else if constexpr (R == kRowsMx8Parts) {
-    if (is(128, 256)) return launch_mx_linear<Tile8P_128x256>(g, stream);
     if (is(128, 128)) return launch_mx_linear<Tile8P_128x128>(g, stream);
     if (is(64, 128)) return launch_mx_linear<Tile8P_64x128>(g, stream);
     return launch_mx_linear<Tile8P_64x64>(g, stream);

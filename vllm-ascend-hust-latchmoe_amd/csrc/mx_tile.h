@@ -469,7 +469,6 @@ using Tile8_128x256 = MxShape<kRowsMx8, 4, 4, 2, 4, 4>;
 using Tile8_128x128 = MxShape<kRowsMx8, 4, 4, 2, 2, 3>;
 using Tile8_64x128 = MxShape<kRowsMx8, 2, 4, 2, 2, 4>;
 using Tile8_64x64 = MxShape<kRowsMx8, 2, 2, 2, 2, 4>;
-using Tile8P_128x256 = MxShape<kRowsMx8Parts, 4, 4, 2, 4, 4>;
 using Tile8P_128x128 = MxShape<kRowsMx8Parts, 4, 4, 2, 2, 3>;
 using Tile8P_64x128 = MxShape<kRowsMx8Parts, 2, 4, 2, 2, 4>;
 using Tile8P_64x64 = MxShape<kRowsMx8Parts, 2, 2, 2, 2, 4>;
