@@ -766,6 +766,8 @@ def mx4_linear(x, w: torch.Tensor, out: torch.Tensor | None = None, *, bias: tor
         xq, px, rows = x, None, 0
         if x.dtype is not _BF16 or x.get_device() != here or not x.is_contiguous():
             _refuse(x, "x", _BF16)
+    if T > 0x7FFFFFFF:
+        raise ValueError(f"x has {T} rows, more than an int holds")
     if not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise ValueError("w must be one matrix in 4 bits, [N, bytes of a row]")
     N, wide = w.shape
