@@ -64,7 +64,7 @@ constexpr ShapeCost kShapes8[5] = {{256, 256, 1, 87, {13.4}}, {128, 256, 1, 53, 
 //   4096 x 2048 x 5120  81.1 / 87.5 / 106   300 x 2048 x 5120   21.9 / 14.1 / 14.2
 //   2048 x 7168 x 7168  188 / 182 / 236     300 x 1408 x 2048   16.8 / 10.6 / 8.5
 //   1024 x 7168 x 7168  91.7 / 96.1 / 111   1000 x 2048 x 2048  22.1 / 14.6 / 15.0
-constexpr ShapeCost kShapes8Parts[3] = {{128, 128, 2, 66, {9.7, 15.5}}, {64, 128, 2, 40, {5.5, 7.7}},
+constexpr ShapeCost kShapes8Parts[3] = {{128, 128, 2, 66, {9.7, 15.5}}, {64, 128, 2, 40, {5.5, 8.0}},
                                         {64, 64, 3, 38, {4.4, 5.5, 7.3}}};
 // bf16 rows, 128 x 256 / 64 x 256 / 32 x 256 tiles:
 //   8192 x 7168 x 7168  607 / 642             1024 x 7168 x 7168  111 / 90.1 / 111
