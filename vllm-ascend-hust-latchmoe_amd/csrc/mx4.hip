@@ -250,11 +250,10 @@ static int fused_moe(int rows, const void* x, const void* x_scale, int T, int H,
                         ws->permute_workspace_bytes, stream);
   if (st != LMOE_OK || T == 0) return st;
   st = gateup_silu(rows, x, x_scale, T, H, I, k, w13_slots, n_slots, ws->offsets, ws->sorted_pairs, ws->active,
-                            ws->tile_off, ws->meta, static_cast<int>(n), block_m, path, ws->act, ws->act_scale, split,
-                            stream);
+                   ws->tile_off, ws->meta, static_cast<int>(n), block_m, path, ws->act, ws->act_scale, split, stream);
   if (st != LMOE_OK) return st;
   st = down(rows, ws->act, ws->act_scale, split, H, I, w2_slots, n_slots, ws->offsets, ws->sorted_pairs, ws->active,
-                     ws->tile_off, ws->meta, static_cast<int>(n), block_m, path, ws->y, ws->y_f32, stream);
+            ws->tile_off, ws->meta, static_cast<int>(n), block_m, path, ws->y, ws->y_f32, stream);
   if (st != LMOE_OK) return st;
   return ws->y_f32 ? lmoe_combine_f32(ws->y, ws->row_idx, w, T, k, H, add, out, stream)
                    : lmoe_combine(ws->y, ws->row_idx, w, T, k, H, add, out, stream);

@@ -251,10 +251,13 @@ __device__ __forceinline__ void store_y(const Mx4Args& g, int pair, int n, int l
 }
 
 // Waves of a workgroup.  Past one token there are workgroups enough, and four waves
-// with twice the work each are ahead of eight (us, gate-up / down, four against
-// eight): 16 tokens over 128 experts of 2048 x 768 16.6 / 10.6 against 16.1 / 11.0,
-// 7 of 7168 x 2048 94.0 / 49.3 against 94.5 / 53.8, 61 over 60 of 2048 x 1408
-// 31.6 / 18.4 against 33.2 / 21.1.  One token has few, and short ones.
+// with twice the work each are ahead of eight (us, gate-up / down of bf16 rows, four against
+// eight): 16 tokens x 8 over 128 experts of 2048 x 768 15.2 / 10.8 against 16.4 / 12.4,
+// 7 x 8 over 64 of 7168 x 2048 96.0 / 47.7 against 95.0 / 50.9, 61 x 4 over 60 of 2048 x 1408
+// 34.6 / 20.7 against 36.6 / 23.4, 40 x 4 over 64 of 1024 x 512 8.9 / 6.1 against 10.5 / 7.5;
+// eight are ahead where workgroups are few and rows long, 16 x 2 over 16 of 4096 x 1024 17.4 /
+// 8.9 against 15.3 / 9.4 (MX8 and MX4 rows 14.3 / 8.1 against 14.0 / 8.9).  One token has few,
+// and short ones.
 constexpr int kFewMxWaves = 4;
 constexpr int kOneMxWaves = 8;
 constexpr int kFewMxBlocks = 4;  // 16-row weight blocks of a workgroup

@@ -11,8 +11,8 @@
 // codes), so that both sides of a wave's access are whole lines; four neighbouring lanes
 // hold a group, and its maximum goes by two quad permutes.  Measured, there / back (a copy
 // of 1 GiB here: 5.05 TB/s): rows 4096 x 7168 11.9 / 14.4 us, 4096 x 2048 3.8 / 6.4, one row
-// 2.1 / 2.1 (an empty launch); banks of 128 x 1536 x 2048 186 / 185 us (5.5 TB/s), 32 x 4096
-// x 7168 431 / 427.
+// 2.1 / 2.1 (an empty launch); banks of 128 x 1536 x 2048, each over and over, 184 / 176 us
+// (5.5 / 5.8 TB/s), in turn 371 together, 32 x 4096 x 7168 431 / 427.
 #include <hip/hip_runtime.h>
 
 #include "mx.h"

@@ -22,13 +22,14 @@
 // without any arithmetic.  The weights' scales lie that way in the bank; the rows' are put
 // together from their 16 bytes a row.
 //
-// Bound: of 4-bit rows the plain product of 4096 x 7168 x 7168 takes 108 us (3.9 PFLOP/s;
-// 7.3 from registers with random values, 9.7 with zeros).  With zeros, which cost no power,
-// and 8192 columns, two full rounds of workgroups, 96: 8 us a round are its start and its
-// stores (33 MB), a chunk takes 0.71 us where its products take 0.44, a chunk without loads
-// and reads of LDS 0.65, without the barrier as well 0.58.  MX8 rows: 162 us (2.6 PFLOP/s; a
-// large library product of 8-bit floats with one scale reaches 2.8).  Four waves of 128 x 128 took 141 us
-// to the 123 of this shape in the same run, six buffers with one workgroup a CU were slower.
+// Bound: of 4-bit rows the plain product of 4096 x 7168 x 7168 takes 105 us (4.0 PFLOP/s; 20
+// in a row 108 to 116 by the card's power; from registers 7.3 with random values, 9.7 with
+// zeros).  With zeros, which cost no power, and 8192 columns, two full rounds of workgroups,
+// 96: 8 us a round are its start and its stores (33 MB), a chunk takes 0.71 us where its
+// products take 0.44, a chunk without loads and reads of LDS 0.65, without the barrier as well
+// 0.58.  MX8 rows: 160 to 171 us (2.6 PFLOP/s; a large library product of 8-bit floats with
+// one scale reaches 2.8), in two parts 341.  Four waves of 128 x 128 took 141 us to the 123 of
+// this shape in the same run, six buffers with one workgroup a CU were slower.
 //
 // Every output adds its chunks in order, whatever the shape is: the same bits.
 #pragma once
