@@ -225,3 +225,21 @@ def test_captured_and_on_two_streams(kind, rows, columns, T, K, N):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(sout, swant) and bool(want.any())
+
+
+@pytest.mark.parametrize("kind,rows,columns,T,K,N", [c for c in ONE_EACH if not c[0].endswith("-f32")])
+def test_added_in_place(kind, rows, columns, T, K, N):
+    """out over add has the bits of out beside it: each value is read before its sum is
+    written, by whichever lanes."""
+    _, native = _mods()
+    _reaches(kind, rows, columns, T, K, N)
+    g = torch.Generator().manual_seed(T + N)
+    x, _ = _rows(kind, torch.randn((T, K), generator=g))
+    w, _ = make_weights(N, K, N)
+    add = torch.randn((T, N), generator=g).to(torch.bfloat16).cuda()
+    bias = torch.randn(N, generator=g).to(torch.bfloat16).cuda()
+    want = native.mx4_linear(x, w, bias=bias, add=add)
+    for _ in range(3):
+        out = add.clone()
+        native.mx4_linear(x, w, out, bias=bias, add=out)
+        assert torch.equal(out, want)
