@@ -1,4 +1,4 @@
-"""The row tiles of the product with one 4-bit matrix, each shape by name.
+"""The kernel forms of the product with one 4-bit matrix, row tiles and split K, each by name.
 
 Sizes end inside a tile, a chunk of 128 columns and a block of 32 outputs, K takes each
 number of chunks past the last four (what is loaded ahead goes round several times).
@@ -32,7 +32,11 @@ CASES = [
     ("mx4", 256, 256, 3001, 1376, 4112), ("mx4", 256, 256, 4090, 2080, 7184),
     ("bf16", 32, 256, 2050, 1440, 7184),  # more than two workgroups a unit
 ]
-ONE_EACH = CASES[::2]
+#: few rows: a workgroup's waves split K
+SPLIT = [(kind, *size) for kind in ("bf16", "mx8", "mx8-f32", "mx4") for size in (
+    (16, 32, 13, 1184, 2064), (16, 32, 40, 672, 1040), (16, 64, 40, 672, 4112), (32, 64, 61, 1440, 7184),
+    (16, 128, 13, 672, 20016))]
+ONE_EACH = CASES[::2] + SPLIT
 SCALED = [c for c in ONE_EACH if c[0] != "bf16"]
 
 
@@ -45,7 +49,7 @@ def _mods():
 def _reaches(kind, rows, columns, T, K, N):
     _, native = _mods()
     form = native.mx4_linear_form(kind.removesuffix("-f32"), T, K, N, out_f32=kind.endswith("-f32"))
-    assert form == (rows, columns, False)
+    assert form == (rows, columns, (kind, rows, columns, T, K, N) in SPLIT)
 
 
 def _rows(kind, x):
@@ -74,7 +78,7 @@ def check(got, x, w, kind, bias=None, add=None):
     assert bool((off <= tol).all()), float((off / tol).max())
 
 
-@pytest.mark.parametrize("kind,rows,columns,T,K,N", CASES)
+@pytest.mark.parametrize("kind,rows,columns,T,K,N", CASES + SPLIT)
 def test_product(kind, rows, columns, T, K, N):
     _, native = _mods()
     _reaches(kind, rows, columns, T, K, N)

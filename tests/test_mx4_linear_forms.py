@@ -5,18 +5,19 @@ import ctypes
 
 import pytest
 
-from tests.test_gpu_mx4_linear_tiles import CASES
+from tests.test_gpu_mx4_linear_tiles import CASES, SPLIT
 
 
-@pytest.mark.parametrize("kind,rows,columns,T,K,N", CASES)
+@pytest.mark.parametrize("kind,rows,columns,T,K,N", CASES + SPLIT)
 def test_the_cases_reach_their_form(kind, rows, columns, T, K, N):
     from vllm_moe_offload_amd import native
 
     form = native.mx4_linear_form(kind.removesuffix("-f32"), T, K, N, out_f32=kind.endswith("-f32"), cu_count=256)
-    assert form == (rows, columns, False)
+    assert form == (rows, columns, (kind, rows, columns, T, K, N) in SPLIT)
 
 
-def test_every_row_tile_has_cases():
+def test_every_form_has_cases():
+    assert {(r, c) for _, r, c, *_ in SPLIT} == {(16, 32), (16, 64), (32, 64), (16, 128)}
     forms = {(kind, rows, columns) for kind, rows, columns, *_ in CASES}
     assert forms == {("bf16", 32, 256), ("bf16", 64, 256), ("bf16", 128, 256),
                      *(("mx8", r, c) for r, c in ((64, 64), (64, 128), (128, 128), (128, 256), (256, 256))),
